@@ -153,7 +153,7 @@ def prepare(case, seed):
     scores = randn(tokens, E) + popular
     top = scores.topk(k, -1)
     state = {"case": case, "X": randn(tokens, C).to(dtype), "experts": top.indices.to(torch.int32),
-             "weights": torch.softmax(top.values, -1)}
+             "weights": torch.softmax(top.values, -1).to(dtype)}     # in the layer's type, as its products take them
     W = randn(E, C, N) / math.sqrt(C)
     if case["op"] == "experts":
         state["W"] = W.to(dtype)
@@ -242,7 +242,7 @@ def _segments(experts, E):
 
 def _experts_plain(state):
     case = state["case"]
-    X, w, W = state["X"].float(), state["weights"], state["W"]
+    X, w, W = state["X"].float(), state["weights"].float(), state["W"]
     k, E, dtype = case["k"], case["E"], state["X"].dtype
     order, counts = _segments(state["experts"], E)
     token = order // k
@@ -273,7 +273,7 @@ def _experts_plain(state):
     dXslot = torch.empty_like(dXs)
     dXslot[order] = dXs
     dX = dXslot.view(-1, k, case["C"]).sum(1)
-    return out.to(dtype), dX.to(dtype), dW.to(dtype), dw
+    return out.to(dtype), dX.to(dtype), dW.to(dtype), dw.to(dtype)
 
 
 def _int8_plain(state):
@@ -295,7 +295,7 @@ def _int8_plain(state):
             at += n
     Yslot = torch.empty_like(Y)
     Yslot[order] = Y
-    out = (Yslot.view(-1, k, case["N"]) * state["weights"].unsqueeze(-1)).sum(1)
+    out = (Yslot.view(-1, k, case["N"]) * state["weights"].float().unsqueeze(-1)).sum(1)
     return (out.to(state["X"].dtype),)
 
 
@@ -311,7 +311,7 @@ def work(case):
     tokens, E, k = case["tokens"], case["E"], case["k"]
     es = torch.empty((), dtype=_DTYPES[case["dtype"]]).element_size()
     slots = tokens * k
-    if case["op"] == "route":
+    if case["op"] == "route":     # the ids and, in float32, the weights and their gradient
         nbytes, flops = tokens * E * es + 8 * slots, 8 * tokens * E
         if case["train"]:
             nbytes, flops = nbytes + tokens * E * es + 4 * slots, flops + 8 * tokens * E
@@ -319,11 +319,11 @@ def work(case):
     C, N = case["C"], case["N"]
     used = min(E - case["idle"], slots)
     if case["op"] == "int8":
-        routed = 0 if E == 1 else 8 * slots
+        routed = 0 if E == 1 else (4 + es) * slots
         return {"bytes": tokens * (C + N) * es + used * (C + 4) * N + routed, "flops": 2 * slots * C * N}
-    nbytes, flops = tokens * (C + N) * es + used * C * N * es + 8 * slots, 2 * slots * C * N
+    nbytes, flops = tokens * (C + N) * es + used * C * N * es + (4 + es) * slots, 2 * slots * C * N
     if case["train"]:
-        nbytes += tokens * (C + N) * es + E * C * N * es + 4 * slots
+        nbytes += tokens * (C + N) * es + E * C * N * es + es * slots
         flops *= 3
     return {"bytes": nbytes, "flops": flops}
 
