@@ -13,10 +13,11 @@ import sys
 
 from .torch_interface import ExpertGather, ExpertGatherScatter, ExpertScatter
 from .kernels import ExpertGatherFunction, ExpertScatterFunction, create_kernels
-from . import ops
+from .token_choice import RoutedExperts, RoutedExpertsInt8, TokenRouter
+from . import ops, token_choice
 
 __all__ = ["ExpertGather", "ExpertScatter", "ExpertGatherScatter", "ExpertGatherFunction", "ExpertScatterFunction", "create_kernels",
-           "ops", "install_as_egs"]
+           "TokenRouter", "RoutedExperts", "RoutedExpertsInt8", "token_choice", "ops", "install_as_egs"]
 __version__ = "0.1.0"
 
 

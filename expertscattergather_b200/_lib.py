@@ -31,11 +31,23 @@ EXPORTS = (
     "egs_describe_plan", "egs_describe_kept_rows", "egs_describe_half_tiles", "egs_gather_gemm_bias", "egs_gemm_scatter_bias", "egs_route_topk", "egs_index_csr",
     "egs_index_csr_scratch_bytes", "egs_index_compact", "egs_gemm_scatter_prepared", "egs_gemm_scatter_csr",
     "egs_set_status_mirror", "egs_expert_row_sum",
+    "egs_route_tokens", "egs_route_tokens_backward", "egs_plan_experts", "egs_plan_workspace_bytes", "egs_expert_matmul",
+    "egs_expert_matmul_workspace_bytes", "egs_expert_dweight", "egs_expert_dweight_workspace_bytes", "egs_combine",
+    "egs_combine_backward", "egs_quantize_rows", "egs_expert_matmul_int8",
 )
 
 
 class Dims(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("B", "T", "E", "K", "C", "N")]
+
+
+class Route(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64)] + [(n, ctypes.c_int) for n in ("E", "top_k", "groups", "top_groups", "group_top", "score", "renormalize")] + \
+               [("scale", ctypes.c_float)]
+
+
+class Ragged(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("tokens", "k", "E", "C", "N")]
 
 
 class PlanInfo(ctypes.Structure):
@@ -108,6 +120,22 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.egs_launch_count.argtypes = []
     lib.egs_gather_scatter_pair.restype = i
     lib.egs_gather_scatter_pair.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i, i, i, i, i, vp, sz, vp, vp]
+    route, ragged = ctypes.POINTER(Route), ctypes.POINTER(Ragged)
+    for name, result, args in (
+            ("egs_route_tokens", i, [vp, vp, vp, vp, route, i64, i, vp]),
+            ("egs_route_tokens_backward", i, [vp, vp, vp, vp, route, i64, i, vp]),
+            ("egs_plan_experts", i, [vp, i64, i, vp, vp, vp, vp, sz, vp, vp]),
+            ("egs_plan_workspace_bytes", sz, [i64, i]),
+            ("egs_expert_matmul", i, [vp, vp, vp, vp, vp, ragged, i, i, i, i, vp, sz, vp, vp]),
+            ("egs_expert_matmul_workspace_bytes", sz, [ragged, i, i, i]),
+            ("egs_expert_dweight", i, [vp, vp, vp, vp, vp, ragged, i, i, i, vp, sz, vp, vp]),
+            ("egs_expert_dweight_workspace_bytes", sz, [ragged, i, i]),
+            ("egs_combine", i, [vp, vp, vp, vp, i64, i64, i64, i, i, vp]),
+            ("egs_combine_backward", i, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i, i, vp]),
+            ("egs_quantize_rows", i, [vp, vp, vp, i64, i64, i64, i64, i, vp]),
+            ("egs_expert_matmul_int8", i, [vp, vp, i64, vp, vp, i64, vp, vp, vp, ragged, i, i, i, vp, vp])):
+        getattr(lib, name).restype = result
+        getattr(lib, name).argtypes = args
     lib.egs_fused_pair_eligible.restype = i
     lib.egs_fused_pair_eligible.argtypes = [i64, i64, i64, i, i, i]
 

@@ -83,12 +83,26 @@ StatusRef status_ref(int32_t* status_word) {
   return {status_word, nullptr};
 }
 
-namespace {
-
 int fail_cuda(cudaError_t err, const char* where) {
   std::snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", where, cudaGetErrorString(err));
   return EGS_ERR_CUDA;
 }
+
+bool device_is_sm100() {
+  static thread_local int cached_dev = -1;
+  static thread_local int cached_ok = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev != cached_dev) {
+    int major = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cached_dev = dev;
+    cached_ok = (major == 10);
+  }
+  return cached_ok != 0;
+}
+
+namespace {
 
 bool valid_dtype(int d) { return d == EGS_F32 || d == EGS_F16 || d == EGS_BF16; }
 bool valid_index(int d) { return d == EGS_I16 || d == EGS_I32 || d == EGS_I64; }
@@ -107,20 +121,6 @@ constexpr size_t kRoundInKernel = 64 << 10;
 // egs_strict.cu), and longest that one accumulator of the fused pair kernel sees.
 constexpr long long kStrictMaxContraction = 2048;
 constexpr long long kStrictMaxFusedContraction = 512;
-
-bool device_is_sm100() {
-  static thread_local int cached_dev = -1;
-  static thread_local int cached_ok = 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  if (dev != cached_dev) {
-    int major = 0;
-    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-    cached_dev = dev;
-    cached_ok = (major == 10);
-  }
-  return cached_ok != 0;
-}
 
 // The tensor-core kernels move rows with 16-byte copies: every row pitch must be a multiple of 16 bytes
 // and every base pointer 16-byte aligned.

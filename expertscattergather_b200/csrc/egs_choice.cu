@@ -1,0 +1,889 @@
+// Tokens that choose experts: routing and its gradient, the counting sort of the routed slots by expert, the weighted sum of a
+// token's rows and its gradient, rows rounded to 8 bits, copies with another row pitch, and the CUDA-core products over ragged rows.
+//
+// Vocabulary beside egs_internal.cuh's:
+//   slot         one (token, choice) pair; its number is token * k + choice
+//   sorted row   place of a slot among all slots sorted by expert (slots of one expert in ascending order); the rows of expert e are
+//                offsets[e] .. offsets[e + 1] - 1, those behind offsets[E] belong to slots that chose no expert
+#include "egs_internal.cuh"
+
+namespace egs {
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// Floats as unsigned numbers of the same order; NaN lies below everything and above 0, which stands for "no candidate".
+__device__ __forceinline__ uint32_t ordered(float x) {
+  x += 0.f;                                    // -0 and 0 are equal
+  const uint32_t b = __float_as_uint(x);
+  return x != x ? 1u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+
+// ------------------------------------------------------------------------------------------------
+// Routing.  A warp has a token, lane l its experts l, l + 32, ...; every choice is a maximum over the lane's own keys, one over the
+// warp (redux on the ordered keys) and the lowest expert that has it.  Softmax and no bias: the logits' order is the scores', so the
+// logits are the keys, and a row's sum is only formed where something needs it.  Renormalised softmax weights are formed from the
+// chosen logits alone.
+// ------------------------------------------------------------------------------------------------
+constexpr int kRouteWarps = 8;
+
+struct RouteParams {
+  const void* logits;
+  const float* bias;
+  float* weights;
+  int* experts;
+  long long stride;      // elements from one token's logits to the next's
+  int tokens, E, k, groups, top_groups, group_top, per;
+  int sigmoid, renormalize;
+  float scale;
+  Div by_per;            // experts of a group
+  int lanes_log2;        // lanes that look at a group together
+};
+
+template <typename T, int NPER>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __grid_constant__ RouteParams p) {
+  extern __shared__ float group_values[];
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
+  if (t >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + t * p.stride;
+  float x[NPER];
+#pragma unroll
+  for (int i = 0; i < NPER; ++i) {
+    const int e = i * 32 + lane;
+    x[i] = e < p.E ? to_f32<T>(row[e]) : 0.f;
+  }
+  const bool pairs = p.groups > 1 && p.group_top == 2;
+  const bool need_scores = p.bias || pairs || (!p.sigmoid && !p.renormalize);
+  float m = 0.f, total = 1.f;
+  if (!p.sigmoid && need_scores) {
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NPER; ++i)
+      if (i * 32 + lane < p.E) m = fmaxf(m, x[i]);
+    m = warp_max(m);
+    total = 0.f;
+#pragma unroll
+    for (int i = 0; i < NPER; ++i)
+      if (i * 32 + lane < p.E) total += m == -INFINITY ? 0.f : expf(x[i] - m);
+    total = warp_sum(total);
+  }
+  auto score = [&](float v) { return p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total; };
+  uint32_t key[NPER];
+  uint32_t kept = kFull;                       // groups
+  if (!need_scores) {
+#pragma unroll
+    for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(x[i]) : 0u;
+  }
+  if (need_scores || p.groups > 1) {
+    float* values = group_values + warp * p.E;
+#pragma unroll
+    for (int i = 0; i < NPER; ++i) {
+      const int e = i * 32 + lane;
+      if (e < p.E) {
+        float v = x[i];
+        if (p.bias) v = score(x[i]) + p.bias[e];
+        key[i] = ordered(v);
+        if (p.groups > 1) values[e] = pairs && !p.bias ? score(x[i]) : v;
+      } else {
+        key[i] = 0u;
+      }
+    }
+  }
+  if (p.groups > 1) {
+    // the lanes of a group look at every 2^lanes_log2-th of its values and join what they found; group g's value ends up in lane g
+    float* values = group_values + warp * p.E;
+    __syncwarp();
+    const int lanes = 1 << p.lanes_log2, g = lane >> p.lanes_log2;
+    uint32_t k1 = 0u, k2 = 0u;
+    float v1 = 0.f, v2 = 0.f;
+    auto take = [&](uint32_t kk, float v) {
+      if (kk > k1) {
+        k2 = k1; v2 = v1;
+        k1 = kk; v1 = v;
+      } else if (kk > k2) {
+        k2 = kk; v2 = v;
+      }
+    };
+    if (g < p.groups)
+      for (int i = lane & (lanes - 1); i < p.per; i += lanes) {
+        const float v = values[g * p.per + i];
+        take(ordered(v), v);
+      }
+    for (int o = 1; o < lanes; o <<= 1) {
+      const uint32_t o1 = __shfl_xor_sync(kFull, k1, o), o2 = __shfl_xor_sync(kFull, k2, o);
+      const float w1 = __shfl_xor_sync(kFull, v1, o), w2 = __shfl_xor_sync(kFull, v2, o);
+      take(o1, w1);
+      take(o2, w2);
+    }
+    const float value = p.group_top == 2 && k2 ? v1 + v2 : v1;
+    uint32_t gk = g < p.groups ? ordered(value) : 0u;
+    gk = __shfl_sync(kFull, gk, (lane << p.lanes_log2) & 31);
+    if (lane >= p.groups) gk = 0u;
+    kept = 0u;
+    for (int i = 0; i < p.top_groups; ++i) {
+      const uint32_t best = __reduce_max_sync(kFull, gk);
+      const int at = __ffs(__ballot_sync(kFull, gk == best)) - 1;
+      kept |= 1u << at;
+      if (lane == at) gk = 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < NPER; ++i)
+      if (!((kept >> (p.by_per.quotient(i * 32 + lane) & 31)) & 1u)) key[i] = 0u;
+  }
+  int mine = 0;
+  for (int j = 0; j < p.k; ++j) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < NPER; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(kFull, best);
+    uint32_t at = kFull;
+#pragma unroll
+    for (int i = NPER - 1; i >= 0; --i)
+      if (key[i] == best) at = i * 32 + lane;
+    at = __reduce_min_sync(kFull, at);
+#pragma unroll
+    for (int i = 0; i < NPER; ++i)
+      if (at == i * 32 + lane) key[i] = 0u;
+    if (lane == j) mine = static_cast<int>(at);
+  }
+  const bool chosen = lane < p.k;
+  const float xc = chosen ? to_f32<T>(row[mine]) : -INFINITY;
+  float w;
+  if (p.renormalize) {
+    const float top = p.sigmoid ? 0.f : warp_max(xc);
+    const float s = !chosen ? 0.f : p.sigmoid ? sigmoid(xc) : top == -INFINITY ? 0.f : expf(xc - top);
+    const float sum = warp_sum(s);
+    w = sum == 0.f ? 0.f : s / sum;
+  } else {
+    w = score(xc);
+  }
+  if (chosen) {
+    p.weights[t * p.k + lane] = w * p.scale;
+    p.experts[t * p.k + lane] = mine;
+  }
+}
+
+// The gradient: rows of zeros with a value for every chosen expert, except where softmax weights are not renormalised.  Ids outside
+// [0, E) (a choice that was taken away) have no part in it.
+struct RouteBackwardParams {
+  const float* dweights;
+  const void* logits;
+  const int* experts;
+  void* dlogits;
+  long long stride;
+  int tokens, E, k;
+  int sigmoid, renormalize, vectors;     // vectors: rows of whole, aligned 16 bytes
+  float scale;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_backward_kernel(const __grid_constant__ RouteBackwardParams p) {
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
+  if (t >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + t * p.stride;
+  T* out = static_cast<T*>(p.dlogits) + t * p.E;
+  int e = lane < p.k ? p.experts[t * p.k + lane] : -1;
+  const bool on = e >= 0 && e < p.E;
+  const float g = on ? p.dweights[t * p.k + lane] * p.scale : 0.f;
+  const float x = on ? to_f32<T>(row[e]) : -INFINITY;
+  const bool whole_row = !p.sigmoid && !p.renormalize;
+  float d;
+  if (whole_row) {
+    float m = -INFINITY;
+    for (int i = lane; i < p.E; i += 32) m = fmaxf(m, to_f32<T>(row[i]));
+    m = warp_max(m);
+    float total = 0.f;
+    for (int i = lane; i < p.E; i += 32) total += m == -INFINITY ? 0.f : expf(to_f32<T>(row[i]) - m);
+    total = warp_sum(total);
+    const float s = on && m != -INFINITY ? expf(x - m) / total : 0.f;
+    const float back = warp_sum(g * s);
+    for (int i = lane; i < p.E; i += 32)
+      out[i] = from_f32<T>(m == -INFINITY ? 0.f : -(expf(to_f32<T>(row[i]) - m) / total) * back);
+    d = s * (g - back);
+  } else {
+    if (p.vectors) {
+      constexpr int V = 16 / sizeof(T);
+      for (int i = lane; i < p.E / V; i += 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int i = lane; i < p.E; i += 32) out[i] = from_f32<T>(0.f);
+    }
+    if (p.sigmoid) {
+      const float s = on ? sigmoid(x) : 0.f, slope = s / (1.f + expf(x));          // s (1 - s)
+      if (p.renormalize) {
+        const float sum = warp_sum(s), back = sum == 0.f ? 0.f : warp_sum(g * s) / sum;
+        d = sum == 0.f ? 0.f : (g - back) / sum * slope;
+      } else {
+        d = g * slope;
+      }
+    } else {
+      const float top = warp_max(x);
+      const float s = on && top != -INFINITY ? expf(x - top) : 0.f;
+      const float sum = warp_sum(s), w = sum == 0.f ? 0.f : s / sum;
+      d = w * (g - warp_sum(w * g));
+    }
+  }
+  __syncwarp();                                // the row before its chosen experts
+  if (on) out[e] = from_f32<T>(d);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Counting sort of the slots by expert.  Every CTA has a stretch of slots; the first kernel counts each stretch (not needed where there
+// is only one), the second finds the start of its stretch within every expert and places its slots.  Inside a stretch every warp has a
+// part, counted and placed 32 slots at a time, so that slots of one expert stay in order.  Ids outside [0, E) are an expert of their
+// own behind the others.
+// ------------------------------------------------------------------------------------------------
+constexpr int kPlanWarps = 16, kPlanThreads = kPlanWarps * 32;
+
+struct PlanParams {
+  const int* experts;
+  int* offsets;      // [E + 1]
+  int* slots;        // [n]
+  int* position;     // [n]
+  int* counts;       // [stretches][E + 1], unused with one stretch
+  int n, E, part, stretches;      // part: slots of a warp, a multiple of 32; a stretch is kPlanWarps of them
+  StatusRef status;
+};
+
+// smem: [kPlanWarps][E + 1] counts of the warps' parts
+__device__ __forceinline__ void count_parts(const PlanParams& p, int* table, bool report) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E1 = p.E + 1;
+  for (int i = threadIdx.x; i < kPlanWarps * E1; i += kPlanThreads) table[i] = 0;
+  __syncthreads();
+  int* mine = table + warp * E1;
+  const long long first = (static_cast<long long>(blockIdx.x) * kPlanWarps + warp) * p.part;
+  const int n = static_cast<int>(min(static_cast<long long>(p.part), p.n - first));
+  for (int i = lane; i < n; i += 32) {
+    int e = p.experts[first + i];
+    if (e < 0 || e >= p.E) {
+      if (e != -1 && report) p.status.report(EGS_STATUS_INDEX_OUT_OF_RANGE);
+      e = p.E;
+    }
+    atomicAdd(mine + e, 1);
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int table[];
+  pdl_wait();
+  pdl_trigger();
+  count_parts(p, table, true);
+  const int E1 = p.E + 1;
+  for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
+    int sum = 0;
+    for (int w = 0; w < kPlanWarps; ++w) sum += table[w * E1 + e];
+    p.counts[blockIdx.x * E1 + e] = sum;
+  }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int table[];
+  __shared__ int sums[kPlanWarps];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E1 = p.E + 1;
+  const bool one = p.stretches == 1;
+  count_parts(p, table, one);
+  // offsets of the experts (exclusive sums over all slots), a part of them at a time, and from them where each warp's slots begin
+  int carry = 0;
+  for (int e0 = 0; e0 < E1; e0 += kPlanThreads) {
+    const int e = e0 + threadIdx.x;
+    int before = 0, all = 0;                   // slots of e in the stretches before this one, in all of them
+    if (e < E1) {
+      if (one) {
+        for (int w = 0; w < kPlanWarps; ++w) all += table[w * E1 + e];
+      } else {
+        for (int s = 0; s < p.stretches; ++s) {
+          const int c = p.counts[s * E1 + e];
+          if (s < static_cast<int>(blockIdx.x)) before += c;
+          all += c;
+        }
+      }
+    }
+    int incl = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFull, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    int base = carry;
+    for (int w = 0; w < warp; ++w) base += sums[w];
+    for (int w = 0; w < kPlanWarps; ++w) carry += sums[w];
+    const int offset = base + incl - all;
+    if (e < E1) {
+      if (blockIdx.x == 0) p.offsets[e] = offset;
+      int at = offset + before;
+      for (int w = 0; w < kPlanWarps; ++w) {
+        const int c = table[w * E1 + e];
+        table[w * E1 + e] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+  }
+  int* mine = table + warp * E1;
+  const long long first = (static_cast<long long>(blockIdx.x) * kPlanWarps + warp) * p.part;
+  const int n = static_cast<int>(min(static_cast<long long>(p.part), p.n - first));
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    const bool on = i < n;
+    int e = on ? p.experts[first + i] : p.E;
+    const bool real = e >= 0 && e < p.E;
+    if (!real) e = p.E;
+    const unsigned same = __match_any_sync(kFull, on ? e : -1);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    const int at = on ? mine[e] + rank : 0;
+    __syncwarp();
+    if (on && rank == 0) mine[e] += __popc(same);
+    __syncwarp();
+    if (on) {
+      p.slots[at] = static_cast<int>(first + i);
+      p.position[first + i] = real ? at : ~at;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Weighted sum of a token's rows, float32 in the order of its choices, rounded once.  A thread has V columns of a token.
+// ------------------------------------------------------------------------------------------------
+template <typename T, int V> struct Vec;
+template <typename T> struct Vec<T, 1> {
+  static __device__ __forceinline__ void load(const T* p, float (&v)[1]) { v[0] = to_f32<T>(*p); }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { *p = from_f32<T>(v[0]); }
+};
+template <> struct Vec<float, 4> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+};
+template <typename T> struct Vec<T, 8> {
+  static __device__ __forceinline__ void load(const T* p, float (&v)[8]) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const T* h = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(h[i]);
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[8]) {
+    uint4 x;
+    T* h = reinterpret_cast<T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = x;
+  }
+};
+
+struct CombineParams {
+  const void* Y;           // sorted rows
+  const void* weights;     // [tokens, k] or NULL (ones)
+  const int* position;
+  void* out;               // token rows;  backward: dY, sorted rows
+  const void* dOut;        // backward: token rows
+  void* dweights;          // backward: [tokens, k]
+  int tokens, k, N, vecs;  // vecs: threads of a token (forward), lanes' worth of a row (backward)
+  int w_f32;               // weights (and their gradient) in float32, else in the rows' type
+  Div by_vecs;
+  long long work;          // forward: tokens * vecs
+};
+template <typename T>
+__device__ __forceinline__ float weight_of(const CombineParams& p, long long slot) {
+  return !p.weights ? 1.f : p.w_f32 ? static_cast<const float*>(p.weights)[slot] : to_f32<T>(static_cast<const T*>(p.weights)[slot]);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
+  pdl_wait();
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.work) return;
+  const long long t = i / p.vecs;
+  const int c = static_cast<int>(i - t * p.vecs) * V;
+  const T* Y = static_cast<const T*>(p.Y) + c;
+  const int* pos = p.position + t * p.k;
+  float sum[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = 0.f;
+  for (int j0 = 0; j0 < p.k; j0 += 4) {
+    int at[4];
+    float w[4], y[4][V];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      at[j] = j0 + j < p.k ? pos[j0 + j] : -1;
+      if (at[j] >= 0) Vec<T, V>::load(Y + static_cast<long long>(at[j]) * p.N, y[j]);
+      w[j] = at[j] >= 0 ? weight_of<T>(p, t * p.k + j0 + j) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (at[j] >= 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] = fmaf(w[j], y[j][v], sum[v]);
+      }
+  }
+  Vec<T, V>::store(static_cast<T*>(p.out) + t * p.N + c, sum);
+}
+
+// A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
+// zeros and a gradient of zero.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_constant__ CombineParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long slot = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (slot >= static_cast<long long>(p.tokens) * p.k) return;
+  const long long t = slot / p.k;
+  const int at = p.position[slot];
+  float dot = 0.f;
+  if (at >= 0) {
+    const float w = weight_of<T>(p, slot);
+    const T* g = static_cast<const T*>(p.dOut) + t * p.N;
+    const T* y = static_cast<const T*>(p.Y) + static_cast<long long>(at) * p.N;
+    T* d = static_cast<T*>(p.out) + static_cast<long long>(at) * p.N;
+    for (int c = lane; c < p.vecs; c += 32) {
+      float gv[V], yv[V];
+      Vec<T, V>::load(g + c * V, gv);
+      if (p.dweights) Vec<T, V>::load(y + c * V, yv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (p.dweights) dot = fmaf(gv[v], yv[v], dot);
+        gv[v] *= w;
+      }
+      Vec<T, V>::store(d + c * V, gv);
+    }
+  }
+  if (at < 0) {
+    T* d = static_cast<T*>(p.out) + static_cast<long long>(~at) * p.N;
+    const float zeros[V] = {};
+    for (int c = lane; c < p.vecs; c += 32) Vec<T, V>::store(d + c * V, zeros);
+  }
+  if (!p.dweights) return;
+  dot = warp_sum(dot);
+  if (lane == 0) {
+    if (p.w_f32) static_cast<float*>(p.dweights)[slot] = dot;
+    else static_cast<T*>(p.dweights)[slot] = from_f32<T>(dot);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Rows in 8 bits: scale = largest magnitude / 127, q = x / scale to the nearest integer, ties to even.  A row with an infinity or a
+// NaN in it has the scale NaN and zeros, so that its products are NaN.  The elements a thread has seen for the maximum stay in
+// registers as far as they fit.
+// ------------------------------------------------------------------------------------------------
+struct QuantizeParams {
+  const void* X;
+  int8_t* q;
+  float* scale;
+  long long x_stride, q_stride;
+  int rows, C;
+};
+
+template <typename T, int V, int WARPS>
+__global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
+  constexpr int kKeep = 4;
+  __shared__ float found[4];
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kRowThreads = WARPS * 32;
+  const int r = threadIdx.x / kRowThreads, i0 = threadIdx.x % kRowThreads;
+  const long long row = static_cast<long long>(blockIdx.x) * (128 / kRowThreads) + r;
+  const bool on = row < p.rows;
+  const T* x = static_cast<const T*>(p.X) + row * p.x_stride;
+  const int n = on ? p.C / V : 0;
+  float kept[kKeep][V];
+  // the magnitudes' bit patterns have their order, and a NaN lies above infinity
+  uint32_t top = 0u;
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) {
+    const int i = i0 + j * kRowThreads;
+    if (i < n) {
+      Vec<T, V>::load(x + static_cast<long long>(i) * V, kept[j]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(kept[j][v]) & 0x7fffffffu);
+    }
+  }
+  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) {
+    float y[V];
+    Vec<T, V>::load(x + static_cast<long long>(i) * V, y);
+#pragma unroll
+    for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(y[v]) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(kFull, top);
+  if (WARPS > 1) {
+    if ((threadIdx.x & 31) == 0) found[threadIdx.x >> 5] = __uint_as_float(top);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = max(top, __float_as_uint(found[w]));
+  }
+  const bool finite = top < 0x7f800000u;
+  const float scale = finite ? __uint_as_float(top) / 127.f : __uint_as_float(0x7fc00000u);
+  const bool zeros = !finite || scale == 0.f;
+  if (on && i0 == 0) p.scale[row] = scale;
+  int8_t* q = p.q + row * p.q_stride;
+  auto put = [&](int i, const float (&y)[V]) {
+    int8_t b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[v] = zeros ? 0 : static_cast<int8_t>(max(-127, min(127, __float2int_rn(y[v] / scale))));
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(q + static_cast<long long>(i) * V) = *reinterpret_cast<const uint2*>(b);
+    else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(q + static_cast<long long>(i) * V) = *reinterpret_cast<const uint32_t*>(b);
+    else q[i] = b[0];
+  };
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) {
+    const int i = i0 + j * kRowThreads;
+    if (i < n) put(i, kept[j]);
+  }
+  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) {
+    float y[V];
+    Vec<T, V>::load(x + static_cast<long long>(i) * V, y);
+    put(i, y);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Products over ragged rows on the CUDA cores: any type, width and alignment.  Tiles of 64 x 64, a step of 16 contraction elements,
+// 4 x 4 products a thread; float32 (8-bit operands: int32) sums.
+// ------------------------------------------------------------------------------------------------
+constexpr int kGTile = 64, kGStep = 16;
+
+// The tile-th block of `rows` rows of an expert: its expert and first sorted row, by the first warp; -1 behind the last one.
+__device__ __forceinline__ void locate_block(const int* offsets, int E, int rows, int tile, int* expert, int* first, int* end) {
+  const int lane = threadIdx.x & 31;
+  int seen = 0, e_found = -1, first_found = 0, end_found = 0;
+  for (int e0 = 0; e0 < E && e_found < 0; e0 += 32) {
+    const int e = e0 + lane;
+    const int a = e < E ? offsets[e] : 0, b = e < E ? offsets[e + 1] : 0;
+    const int blocks = (b - a + rows - 1) / rows;
+    int incl = blocks;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFull, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned hit = __ballot_sync(kFull, seen + incl > tile);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int f = a + (tile - seen - (incl - blocks)) * rows;
+      e_found = e0 + src;
+      first_found = __shfl_sync(kFull, f, src);
+      end_found = __shfl_sync(kFull, b, src);
+    }
+    seen += __shfl_sync(kFull, incl, 31);
+  }
+  if (lane == 0) {
+    *expert = e_found;
+    *first = first_found;
+    *end = end_found;
+  }
+}
+
+template <typename T> struct Acc { using type = float; };
+template <> struct Acc<int8_t> { using type = int; };
+template <typename T> __device__ __forceinline__ typename Acc<T>::type widen(T v) { return to_f32<T>(v); }
+template <> __device__ __forceinline__ int widen<int8_t>(int8_t v) { return v; }
+__device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ int mac(int a, int b, int c) { return a * b + c; }
+
+// Rows behind the last expert's: zeros.
+template <typename T>
+__device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int part, int parts) {
+  if (!p.offsets) return;
+  T* out = static_cast<T*>(p.Out);
+  const long long begin = static_cast<long long>(p.offsets[p.E]) * p.N, end = static_cast<long long>(p.rows) * p.N;
+  for (long long i = begin + part; i < end; i += parts) out[i] = from_f32<T>(0.f);
+}
+
+template <typename T, typename OutT>
+__global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant__ RaggedParams p) {
+  using A = typename Acc<T>::type;
+  __shared__ A As[kGStep][kGTile + 4], Bs[kGStep][kGTile + 4];
+  __shared__ int s_expert, s_first, s_end;
+  __shared__ int src[kGTile];
+  pdl_wait();
+  const int tid = threadIdx.x;
+  zero_unrouted<OutT>(p, (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid, gridDim.x * gridDim.y * 256);
+  if (p.offsets) {
+    if (tid < 32) locate_block(p.offsets, p.E, kGTile, blockIdx.x, &s_expert, &s_first, &s_end);
+  } else if (tid == 0) {
+    s_expert = 0;
+    s_first = blockIdx.x * kGTile;
+    s_end = p.rows;
+  }
+  __syncthreads();
+  const int e = s_expert, first = s_first, end = s_end;
+  if (e < 0) return;
+  if (tid < kGTile) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
+  const T* X = static_cast<const T*>(p.A);
+  const T* W = static_cast<const T*>(p.W) + e * p.w_expert;
+  const int n0 = blockIdx.y * kGTile, tx = tid & 15, ty = tid >> 4;
+  A acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0;
+  for (int c0 = 0; c0 < p.C; c0 += kGStep) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = (tid >> 4) + 16 * i, c = c0 + (tid & 15);
+      As[tid & 15][m] = src[m] >= 0 && c < p.C ? widen<T>(X[src[m] * p.a_row + c]) : A(0);
+      if (p.nc) {
+        const int n = n0 + m;
+        Bs[tid & 15][m] = n < p.N && c < p.C ? widen<T>(W[n * p.w_row + c]) : A(0);
+      } else {
+        const int cc = c0 + (tid >> 6) + 4 * i, n = n0 + (tid & 63);
+        Bs[(tid >> 6) + 4 * i][tid & 63] = n < p.N && cc < p.C ? widen<T>(W[cc * p.w_row + n]) : A(0);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kGStep; ++c) {
+      A a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = As[c][ty * 4 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = Bs[c][tx * 4 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mac(a[i], b[j], acc[i][j]);
+    }
+  }
+  OutT* out = static_cast<OutT*>(p.Out);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = ty * 4 + i;
+    if (src[m] < 0) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + tx * 4 + j;
+      if (n >= p.N) continue;
+      float v = static_cast<float>(acc[i][j]);
+      if (p.a_scale) v *= p.a_scale[src[m]] * p.w_scale[static_cast<long long>(e) * p.N + n];
+      out[static_cast<long long>(first + m) * p.N + n] = from_f32<OutT>(v);
+    }
+  }
+}
+
+// dW[e, c, n] = sum over the rows of e of X[row, c] dY[row, n]
+template <typename T>
+__global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p) {
+  __shared__ float As[kGStep][kGTile + 4], Bs[kGStep][kGTile + 4];
+  pdl_wait();
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int e = blockIdx.z, c0 = blockIdx.x * kGTile, n0 = blockIdx.y * kGTile;
+  const int first = p.offsets[e], end = p.offsets[e + 1];
+  const T* X = static_cast<const T*>(p.A);
+  const T* Y = static_cast<const T*>(p.W);
+  float acc[4][4] = {};
+  for (int r0 = first; r0 < end; r0 += kGStep) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + (tid >> 6) + 4 * i, f = tid & 63;
+      const long long row = r >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[r]) : r;
+      As[(tid >> 6) + 4 * i][f] = row >= 0 && c0 + f < p.C ? to_f32<T>(X[row * p.a_row + c0 + f]) : 0.f;
+      Bs[(tid >> 6) + 4 * i][f] = r < end && n0 + f < p.N ? to_f32<T>(Y[static_cast<long long>(r) * p.w_row + n0 + f]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kGStep; ++r) {
+      float a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = As[r][ty * 4 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = Bs[r][tx * 4 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+    }
+  }
+  T* out = static_cast<T*>(p.Out) + static_cast<long long>(e) * p.C * p.N;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c0 + ty * 4 + i, n = n0 + tx * 4 + j;
+      if (c < p.C && n < p.N) out[static_cast<long long>(c) * p.N + n] = from_f32<T>(acc[i][j]);
+    }
+}
+
+template <typename T, int NPER>
+cudaError_t route_n(const RouteParams& p, cudaStream_t st) {
+  const size_t smem = p.groups > 1 ? sizeof(float) * kRouteWarps * p.E : 0;
+  return launch_kernel(route_tokens_kernel<T, NPER>, (p.tokens + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, smem, st, true, p);
+}
+template <typename T>
+cudaError_t route_t(const RouteParams& p, cudaStream_t st) {
+  if (p.E <= 32) return route_n<T, 1>(p, st);
+  if (p.E <= 64) return route_n<T, 2>(p, st);
+  if (p.E <= 128) return route_n<T, 4>(p, st);
+  if (p.E <= 256) return route_n<T, 8>(p, st);
+  if (p.E <= 512) return route_n<T, 16>(p, st);
+  return route_n<T, 32>(p, st);
+}
+
+template <class F16, class BF16, class F32>
+cudaError_t by_type(int dtype, F16&& f16, BF16&& bf16, F32&& f32) {
+  return dtype == EGS_F16 ? f16() : dtype == EGS_BF16 ? bf16() : f32();
+}
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, int V>
+cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
+  p.vecs = p.N / V;
+  if (backward) {
+    const long long slots = static_cast<long long>(p.tokens) * p.k;
+    return launch_kernel(combine_backward_kernel<T, V>, static_cast<unsigned>((slots + 7) / 8), 256, 0, st, true, p);
+  }
+  p.work = static_cast<long long>(p.tokens) * p.vecs;
+  return launch_kernel(combine_kernel<T, V>, static_cast<unsigned>((p.work + 255) / 256), 256, 0, st, true, p);
+}
+template <typename T>
+cudaError_t combine_t(CombineParams& p, bool backward, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (p.N % V == 0 && aligned(p.Y) && aligned(p.out) && aligned(p.dOut)) return combine_v<T, V>(p, backward, st);
+  return combine_v<T, 1>(p, backward, st);
+}
+
+template <typename T, int V>
+cudaError_t quantize_v(const QuantizeParams& p, cudaStream_t st) {
+  if (p.C <= 32 * V * 4) return launch_kernel(quantize_rows_kernel<T, V, 1>, (p.rows + 3) / 4, 128, 0, st, true, p);
+  return launch_kernel(quantize_rows_kernel<T, V, 4>, p.rows, 128, 0, st, true, p);
+}
+template <typename T>
+cudaError_t quantize_t(const QuantizeParams& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (p.C % V == 0 && p.x_stride % V == 0 && aligned(p.X) && p.q_stride % V == 0 && (reinterpret_cast<uintptr_t>(p.q) % V) == 0)
+    return quantize_v<T, V>(p, st);
+  return quantize_v<T, 1>(p, st);
+}
+
+}  // namespace
+
+cudaError_t launch_route_tokens(const void* logits, const float* bias, float* weights, int* experts, const egs_route& r, long long stride,
+                                int dtype, cudaStream_t st) {
+  RouteParams p{};
+  p.logits = logits; p.bias = bias; p.weights = weights; p.experts = experts; p.stride = stride;
+  p.tokens = static_cast<int>(r.tokens); p.E = r.E; p.k = r.top_k; p.groups = r.groups; p.top_groups = r.top_groups;
+  p.group_top = r.group_top; p.per = r.E / r.groups; p.by_per = Div(p.per);
+  p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
+  while ((32 >> p.lanes_log2) > 1 && (32 >> (p.lanes_log2 + 1)) >= r.groups) ++p.lanes_log2;
+  count_launch();
+  return by_type(dtype, [&] { return route_t<__half>(p, st); }, [&] { return route_t<__nv_bfloat16>(p, st); }, [&] { return route_t<float>(p, st); });
+}
+
+cudaError_t launch_route_backward(const float* dweights, const void* logits, const int* experts, void* dlogits, const egs_route& r,
+                                  long long stride, int dtype, cudaStream_t st) {
+  RouteBackwardParams p{};
+  p.dweights = dweights; p.logits = logits; p.experts = experts; p.dlogits = dlogits; p.stride = stride;
+  p.tokens = static_cast<int>(r.tokens); p.E = r.E; p.k = r.top_k;
+  p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
+  p.vectors = (r.E * (dtype == EGS_F32 ? 4 : 2)) % 16 == 0 && aligned(dlogits);
+  const int grid = (p.tokens + kRouteWarps - 1) / kRouteWarps;
+  count_launch();
+  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, kRouteWarps * 32, 0, st, true, p); };
+  return by_type(dtype, [&] { return go(route_backward_kernel<__half>); }, [&] { return go(route_backward_kernel<__nv_bfloat16>); },
+                 [&] { return go(route_backward_kernel<float>); });
+}
+
+// Slots of a warp: 128 up to 256 stretches of them, then more.
+static int plan_part(long long n) {
+  long long part = (n + 256ll * kPlanWarps - 1) / (256ll * kPlanWarps);
+  part = (part + 31) / 32 * 32;
+  return static_cast<int>(part < 128 ? 128 : part);
+}
+static long long plan_stretches(long long n) {
+  const long long stretch = static_cast<long long>(plan_part(n)) * kPlanWarps;
+  return n ? (n + stretch - 1) / stretch : 1;
+}
+size_t plan_workspace_ints(long long n, int E) { return plan_stretches(n) == 1 ? 0 : static_cast<size_t>(plan_stretches(n)) * (E + 1); }
+
+cudaError_t launch_plan_experts(const int* experts, long long n, int E, int* offsets, int* slots, int* position, int* workspace,
+                                StatusRef status, cudaStream_t st) {
+  PlanParams p{experts, offsets, slots, position, workspace, static_cast<int>(n), E, plan_part(n), static_cast<int>(plan_stretches(n)), status};
+  const size_t smem = sizeof(int) * kPlanWarps * (E + 1);
+  cudaError_t err = ensure_smem_optin<plan_place_kernel>(sizeof(int) * kPlanWarps * (EGS_MAX_EXPERTS + 1));
+  if (err != cudaSuccess) return err;
+  if (p.stretches > 1) {
+    err = ensure_smem_optin<plan_count_kernel>(sizeof(int) * kPlanWarps * (EGS_MAX_EXPERTS + 1));
+    if (err != cudaSuccess) return err;
+    err = launch_kernel(plan_count_kernel, p.stretches, kPlanThreads, smem, st, true, p);
+    count_launch();
+    if (err != cudaSuccess) return err;
+  }
+  count_launch();
+  return launch_kernel(plan_place_kernel, p.stretches, kPlanThreads, smem, st, true, p);
+}
+
+cudaError_t launch_combine(const void* Y, const void* weights, const int* position, void* out, long long tokens, int k, int N, int dtype,
+                           int w_f32, cudaStream_t st) {
+  CombineParams p{};
+  p.Y = Y; p.weights = weights; p.position = position; p.out = out; p.tokens = static_cast<int>(tokens); p.k = k; p.N = N; p.w_f32 = w_f32;
+  count_launch();
+  return by_type(dtype, [&] { return combine_t<__half>(p, false, st); }, [&] { return combine_t<__nv_bfloat16>(p, false, st); },
+                 [&] { return combine_t<float>(p, false, st); });
+}
+
+cudaError_t launch_combine_backward(const void* dOut, const void* Y, const void* weights, const int* position, void* dY, void* dweights,
+                                    long long tokens, int k, int N, int dtype, int w_f32, cudaStream_t st) {
+  CombineParams p{};
+  p.Y = Y; p.weights = weights; p.position = position; p.out = dY; p.dOut = dOut; p.dweights = dweights;
+  p.tokens = static_cast<int>(tokens); p.k = k; p.N = N; p.w_f32 = w_f32;
+  count_launch();
+  return by_type(dtype, [&] { return combine_t<__half>(p, true, st); }, [&] { return combine_t<__nv_bfloat16>(p, true, st); },
+                 [&] { return combine_t<float>(p, true, st); });
+}
+
+cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long long rows, int C, long long x_stride, long long q_stride, int dtype,
+                                 cudaStream_t st) {
+  const QuantizeParams p{X, q, scale, x_stride, q_stride, static_cast<int>(rows), C};
+  count_launch();
+  return by_type(dtype, [&] { return quantize_t<__half>(p, st); }, [&] { return quantize_t<__nv_bfloat16>(p, st); },
+                 [&] { return quantize_t<float>(p, st); });
+}
+
+// Row blocks there can be: every expert with rows may have one that is not full.
+static long long blocks_bound(const RaggedParams& p, int rows) {
+  return p.offsets ? p.rows / rows + (p.rows < p.E ? p.rows : p.E) : (p.rows + rows - 1) / rows;
+}
+
+cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st) {
+  long long blocks = blocks_bound(p, kGTile);
+  if (blocks < 1) blocks = 1;
+  const dim3 grid(static_cast<unsigned>(blocks), (p.N + kGTile - 1) / kGTile);
+  count_launch();
+  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, 256, 0, st, true, p); };
+  if (dtype == EGS_I8)
+    return by_type(out_dtype, [&] { return go(ragged_rows_kernel<int8_t, __half>); }, [&] { return go(ragged_rows_kernel<int8_t, __nv_bfloat16>); },
+                   [&] { return go(ragged_rows_kernel<int8_t, float>); });
+  return by_type(dtype, [&] { return go(ragged_rows_kernel<__half, __half>); }, [&] { return go(ragged_rows_kernel<__nv_bfloat16, __nv_bfloat16>); },
+                 [&] { return go(ragged_rows_kernel<float, float>); });
+}
+
+cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, cudaStream_t st) {
+  const dim3 grid((p.C + kGTile - 1) / kGTile, (p.N + kGTile - 1) / kGTile, p.E);
+  count_launch();
+  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, 256, 0, st, true, p); };
+  return by_type(dtype, [&] { return go(ragged_dweight_kernel<__half>); }, [&] { return go(ragged_dweight_kernel<__nv_bfloat16>); },
+                 [&] { return go(ragged_dweight_kernel<float>); });
+}
+
+}  // namespace egs

@@ -44,7 +44,10 @@ struct Api {
   X(egs_status_string) X(egs_last_cuda_error) X(egs_gather_gemm_bias) X(egs_gemm_scatter_bias) X(egs_gemm_scatter_prepared) \
   X(egs_scatter_workspace_bytes) X(egs_dweight) X(egs_dweight_prezeroed) X(egs_dw_workspace_bytes)                          \
   X(egs_gather_scatter_pair) X(egs_fused_pair_eligible) X(egs_route_topk) X(egs_index_csr) X(egs_index_csr_scratch_bytes)   \
-  X(egs_fill_zero) X(egs_set_status_mirror) X(egs_expert_row_sum)
+  X(egs_fill_zero) X(egs_set_status_mirror) X(egs_expert_row_sum)                                                          \
+  X(egs_route_tokens) X(egs_route_tokens_backward) X(egs_plan_experts) X(egs_plan_workspace_bytes) X(egs_expert_matmul)     \
+  X(egs_expert_matmul_workspace_bytes) X(egs_expert_dweight) X(egs_expert_dweight_workspace_bytes) X(egs_combine)           \
+  X(egs_combine_backward) X(egs_quantize_rows) X(egs_expert_matmul_int8)
 #define EGS_FIELD(name) decltype(&::name) name = nullptr;
   EGS_API(EGS_FIELD)
 #undef EGS_FIELD
@@ -702,6 +705,8 @@ struct GatherScatterFunction : torch::autograd::Function<GatherScatterFunction> 
   }
 };
 
+#include "egs_host_choice.h"
+
 // Tensors this path takes as they are: plain tensors outside any tracing, transform or dispatch mode.  (Fake tensors, tensor
 // subclasses and functorch wrappers go through the Python functions and their dispatcher ops.)
 bool plain(const Tensor& t) {
@@ -808,4 +813,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gather_scatter_forward", &gather_scatter_forward, nogil());
   m.def("gather_scatter_backward", &gather_scatter_backward_op, nogil());
   m.def("train_step", &train_step, nogil());
+  m.def("route_tokens", &route_tokens, nogil());
+  m.def("route_tokens_backward", &route_tokens_backward, nogil());
+  m.def("plan_experts", &plan_experts, nogil());
+  m.def("expert_matmul", &expert_matmul, nogil());
+  m.def("expert_dweight", &expert_dweight, nogil());
+  m.def("combine", &combine, nogil());
+  m.def("combine_backward", &combine_backward, nogil());
+  m.def("quantize_rows", &quantize_rows, nogil());
+  m.def("matmul_int8", &matmul_int8, nogil());
 }

@@ -156,6 +156,23 @@ struct FusedParams {
   uint32_t slot_bytes; // 16-bit kernel: bytes of one ring slot
 };
 
+// Products over ragged rows: the rows of expert e are the sorted rows offsets[e] .. offsets[e + 1] - 1 (see egs_choice.cu).
+struct RaggedParams {
+  const void* A;       // rows: token rows through `slots`, or sorted rows
+  const void* W;       // weights; for weight gradients the sorted rows of dY
+  void* Out;           // sorted rows [rows, N]; weight gradients [E, C, N]
+  const int* offsets;  // [E + 1]; NULL: one expert that has all rows
+  const int* slots;    // slot of a sorted row; NULL: A's rows are the sorted rows
+  const float* a_scale;      // 8-bit operands: scales of A's rows and of the weights' channels [E, N]
+  const float* w_scale;
+  StatusRef status;
+  long long a_row, w_row, w_expert;      // pitches in elements: rows of A, rows of W (of dY), experts of W
+  int rows, a_rows;    // sorted rows, rows of A
+  int E, C, N;
+  int nc;              // 1 = weights [E, N, C]
+  Div by_k;            // slot -> token row
+};
+
 // ------------------------------------------------------------------------------------------------
 // launchers implemented in the kernel files; each returns a cudaError_t from the launch
 // ------------------------------------------------------------------------------------------------
@@ -230,6 +247,28 @@ cudaError_t launch_compact_index(const void* ind, int index_dtype, long long n, 
 cudaError_t launch_csr_scatter(const void* Y, const void* W, const void* bias, const int* offsets, const int* entries, void* Out,
                                long long rows, int E, int K, int C, int N, int w_layout, int accumulate, int dtype,
                                cudaStream_t st);
+
+// Tokens that choose experts (egs_choice.cu)
+cudaError_t launch_route_tokens(const void* logits, const float* bias, float* weights, int* experts, const egs_route& r, long long stride,
+                                int dtype, cudaStream_t st);
+cudaError_t launch_route_backward(const float* dweights, const void* logits, const int* experts, void* dlogits, const egs_route& r,
+                                  long long stride, int dtype, cudaStream_t st);
+size_t plan_workspace_ints(long long n, int E);
+cudaError_t launch_plan_experts(const int* experts, long long n, int E, int* offsets, int* slots, int* position, int* workspace,
+                                StatusRef status, cudaStream_t st);
+cudaError_t launch_combine(const void* Y, const void* weights, const int* position, void* out, long long tokens, int k, int N, int dtype,
+                           int w_f32, cudaStream_t st);
+cudaError_t launch_combine_backward(const void* dOut, const void* Y, const void* weights, const int* position, void* dY, void* dweights,
+                                    long long tokens, int k, int N, int dtype, int w_f32, cudaStream_t st);
+cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long long rows, int C, long long x_stride, long long q_stride, int dtype,
+                                 cudaStream_t st);
+// dtype EGS_I8: 8-bit operands with scales, products in out_dtype
+cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
+cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, cudaStream_t st);
+
+// Errors of the C entries (egs_api.cu): remembers the text, returns EGS_ERR_CUDA.
+int fail_cuda(cudaError_t err, const char* where);
+bool device_is_sm100();
 
 // Bounded-wait self-test (see the kernel): out = two ints on the device.
 cudaError_t launch_wait_timeout_selftest(int32_t* status, int* out, long long limit_cycles, cudaStream_t st);

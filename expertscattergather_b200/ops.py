@@ -15,7 +15,9 @@ import torch
 from . import _lib
 
 __all__ = ["gather_gemm", "gemm_scatter", "gather_scatter_pair", "fused_pair_eligible", "fused_pair_preferred", "dweight", "fill_zero", "side_stream", "fill_stream", "set_precision", "get_precision", "set_path", "get_path",
-           "check_status", "reset_status", "publish_status", "launch_count", "dtype_to_type_id", "tensor_path_eligible", "describe_plan", "describe_kept_rows", "describe_half_tiles", "route_topk", "build_index_csr", "compact_index", "gemm_scatter_csr", "IndexCSR"]
+           "check_status", "reset_status", "publish_status", "launch_count", "dtype_to_type_id", "tensor_path_eligible", "describe_plan", "describe_kept_rows", "describe_half_tiles", "route_topk", "build_index_csr", "compact_index", "gemm_scatter_csr", "IndexCSR",
+           "route_tokens", "route_tokens_backward", "plan_experts", "ExpertPlan", "expert_matmul", "expert_dweight", "combine", "combine_backward",
+           "quantize_rows", "matmul_int8", "expert_matmul_int8"]
 
 _PRECISIONS = {"strict": _lib.PREC_STRICT, "fp32": _lib.PREC_STRICT, "tf32": _lib.PREC_TF32}
 _PATHS = {"auto": _lib.PATH_AUTO, "generic": _lib.PATH_GENERIC, "tensor": _lib.PATH_TENSOR,
@@ -414,3 +416,91 @@ def tensor_path_eligible(op: str, B, T, E, K, C, N, dtype, tensors=()) -> bool:
     ptrs = (ctypes.c_void_p * max(1, len(tensors)))(*[t.data_ptr() for t in tensors])
     return bool(lib.egs_tensor_path_eligible({"G": 0, "S": 1, "D": 2}[op], ctypes.byref(dims), dtype_to_type_id(dtype),
                                              ptrs, len(tensors)))
+
+
+# ---- tokens that choose experts ------------------------------------------------------------------------
+
+def route_tokens(logits, top_k, bias=None, *, score="softmax", groups=1, top_groups=1, group_top=2, renormalize=True, scale=1.0):
+    """Token-choice routing: ``logits`` [..., E] -> ``weights`` [..., top_k] (float32) and ``experts`` [..., top_k] (int32).
+
+    ``s = softmax(logits)`` or ``sigmoid(logits)`` (``score``); an expert's key is ``s + bias`` (``bias`` [E] balances the load: it takes
+    part in the choice, not in the weights).  The experts are ``groups`` groups of consecutive ones; a group's value is the sum of its
+    ``group_top`` (1 or 2) highest keys, and a token takes its ``top_k`` experts of highest key from its ``top_groups`` groups of highest
+    value: best first, equal keys lower expert first, NaN last.  The weights are the chosen scores, divided by their sum with
+    ``renormalize`` (zeros where that is zero), times ``scale``.  At most 1024 experts, 32 choices, 32 groups."""
+    return _host().route_tokens(logits, int(top_k), bias, score, int(groups), int(top_groups), int(group_top), bool(renormalize), float(scale))
+
+
+def route_tokens_backward(dweights, logits, experts, *, score="softmax", renormalize=True, scale=1.0):
+    """Gradient of :func:`route_tokens`' weights: ``dweights`` [..., k] -> dlogits [..., E].  The choice and the bias have none; a token's
+    ids are distinct, and ids outside [0, E) take no part."""
+    return _host().route_tokens_backward(dweights, logits, experts, score, bool(renormalize), float(scale))
+
+
+class ExpertPlan:
+    """The routed slots (token * k + choice) of an ``experts`` [..., k] sorted by expert, built on the device by :func:`plan_experts`:
+    ``offsets`` [E+1] (the sorted rows of expert e are ``offsets[e] .. offsets[e+1]-1``), ``slots`` [tokens*k] (slot of a sorted row,
+    ascending inside an expert), ``position`` [tokens*k] (sorted row of a slot; ``~row`` for slots that were not routed, which lie behind
+    ``offsets[E]``).  All int32 CUDA tensors."""
+
+    __slots__ = ("offsets", "slots", "position", "tokens", "k", "E")
+
+    def __init__(self, offsets, slots, position, tokens, k, E):
+        self.offsets, self.slots, self.position = offsets, slots, position
+        self.tokens, self.k, self.E = tokens, k, E
+
+    def counts(self):
+        """Rows of every expert [E] (no synchronisation): what a load-balancing bias is adjusted by."""
+        return self.offsets[1:] - self.offsets[:-1]
+
+
+def plan_experts(experts, E: int) -> ExpertPlan:
+    """Counting sort of the slots of ``experts`` [..., k] by expert (see :class:`ExpertPlan`); the same result in every run.  -1 marks a
+    slot that is not routed; other ids outside [0, E) are left out too and reported through the status word."""
+    if experts.dim() < 1 or experts.shape[-1] < 1:
+        raise ValueError("expected experts[..., k] with k >= 1")
+    E, k = int(E), experts.shape[-1]
+    offsets, slots, position = _host().plan_experts(experts, E)
+    return ExpertPlan(offsets, slots, position, experts.numel() // k, k, E)
+
+
+def expert_matmul(X, W, plan: ExpertPlan, *, rows="tokens", w_layout="cn", path=None):
+    """``Y[r] = X[row(r)] @ Wv[expert(r)]`` for every sorted row r of ``plan`` (zeros for slots that were not routed): [tokens*k, N].
+    ``rows``: 'tokens' - X holds token rows [..., C], gathered through the plan; 'sorted' - X holds sorted rows [tokens*k, C].
+    ``w_layout`` as in :func:`gather_gemm`.  Sums in float32, rounded once to X's dtype."""
+    return _host().expert_matmul(X, W, plan.offsets, plan.slots, plan.tokens, plan.k, rows, _layout(w_layout), _path(path))
+
+
+def expert_dweight(X, dY, plan: ExpertPlan, *, rows="tokens", path=None):
+    """``dW[e] = sum over the sorted rows r of e of X[row(r)]^T dY[r]``: [E, C, N], zeros for experts without rows.  ``rows`` says what X
+    holds, as in :func:`expert_matmul`; ``dY`` holds sorted rows [tokens*k, N]."""
+    return _host().expert_dweight(X, dY, plan.offsets, plan.slots, plan.tokens, plan.k, rows, _path(path))
+
+
+def combine(Y, weights, plan: ExpertPlan):
+    """``out[t] = sum_j weights[t, j] * Y[position[t, j]]``: sorted rows [tokens*k, N] -> token rows [tokens, N]; float32 in the order of
+    j, rounded once.  ``weights`` [..., k] in float32 or Y's dtype, None for ones.  Slots that were not routed add nothing."""
+    return _host().combine(Y, weights, plan.position, plan.tokens, plan.k)
+
+
+def combine_backward(dOut, Y, weights, plan: ExpertPlan):
+    """Gradients of :func:`combine`: dY [tokens*k, N] and dweights (None where ``weights`` is None)."""
+    return _host().combine_backward(dOut, Y, weights, plan.position, plan.tokens, plan.k)
+
+
+def quantize_rows(X):
+    """Rows in 8 bits: ``scale = max|x| / 127`` [...] (float32) and ``q = x / scale`` [..., C] (int8, to the nearest integer, ties to
+    even).  A row of zeros has the scale 0; a row with an infinity or a NaN the scale NaN.  q's rows lie a multiple of 16 bytes apart.
+    Weights [E, N, C] quantised this way have a scale for each output channel."""
+    return _host().quantize_rows(X)
+
+
+def matmul_int8(q, q_scale, Wq, w_scale, *, out_dtype=torch.bfloat16, path=None):
+    """``Y[r, n] = q_scale[r] * w_scale[n] * sum_c q[r, c] Wq[n, c]``: q [..., C], Wq [N, C] (see :func:`quantize_rows`) -> [..., N].
+    int32 sums (C < 131072).  Operands whose rows do not lie a multiple of 16 bytes apart are copied first."""
+    return _host().matmul_int8(q, q_scale, Wq, w_scale, None, None, 0, 1, "tokens", out_dtype, _path(path))
+
+
+def expert_matmul_int8(q, q_scale, Wq, w_scale, plan: ExpertPlan, *, rows="tokens", out_dtype=torch.bfloat16, path=None):
+    """:func:`expert_matmul` in 8-bit integers: q [rows, C] with a scale for each row, Wq [E, N, C] with one for each channel [E, N]."""
+    return _host().matmul_int8(q, q_scale, Wq, w_scale, plan.offsets, plan.slots, plan.tokens, plan.k, rows, out_dtype, _path(path))

@@ -1,0 +1,160 @@
+"""Layers whose tokens choose their experts: the router, the experts' products with their gradients, and the layer made of them, for
+training and, with 8-bit weights, for serving.
+
+    layer = RoutedExperts(E, I, J, top_k).cuda()        # x [..., I] -> [..., I]
+    served = layer.quantized()                          # the same layer on int8 weights, no gradients
+
+No counterpart in the reference, whose experts choose their tokens (``ExpertGather`` / ``ExpertScatter``).  The operators are those of
+``ops``; here they have gradients.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from . import ops
+
+__all__ = ["RouteTokensFunction", "ExpertMatmulFunction", "CombineFunction", "route_tokens", "expert_matmul", "combine", "TokenRouter",
+           "RoutedExperts", "RoutedExpertsInt8"]
+
+
+class RouteTokensFunction(torch.autograd.Function):
+    """``apply(logits, bias, top_k, options) -> (weights, experts)``; options as ``ops.route_tokens`` takes them, as a dict."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, options):
+        weights, experts = ops.route_tokens(logits, top_k, bias, **options)
+        ctx.save_for_backward(logits, experts)
+        ctx.options = {n: options[n] for n in ("score", "renormalize", "scale") if n in options}
+        ctx.mark_non_differentiable(experts)
+        return weights, experts
+
+    @staticmethod
+    def backward(ctx, dweights, _):
+        logits, experts = ctx.saved_tensors
+        return ops.route_tokens_backward(dweights, logits, experts, **ctx.options), None, None, None
+
+
+class ExpertMatmulFunction(torch.autograd.Function):
+    """``apply(X, W, plan, rows) -> Y`` (``ops.expert_matmul``, W [E, C, N])."""
+
+    @staticmethod
+    def forward(ctx, X, W, plan, rows):
+        ctx.save_for_backward(X, W)
+        ctx.plan, ctx.rows = plan, rows
+        return ops.expert_matmul(X, W, plan, rows=rows)
+
+    @staticmethod
+    def backward(ctx, dY):
+        X, W = ctx.saved_tensors
+        dX = dW = None
+        if ctx.needs_input_grad[0]:
+            dX = ops.expert_matmul(dY, W, ctx.plan, rows="sorted", w_layout="nc")
+            if ctx.rows == "tokens":
+                dX = ops.combine(dX, None, ctx.plan)       # a token's row went to each of its experts
+            dX = dX.view(X.shape)
+        if ctx.needs_input_grad[1]:
+            dW = ops.expert_dweight(X, dY, ctx.plan, rows=ctx.rows)
+        return dX, dW, None, None
+
+
+class CombineFunction(torch.autograd.Function):
+    """``apply(Y, weights, plan) -> out`` (``ops.combine``)."""
+
+    @staticmethod
+    def forward(ctx, Y, weights, plan):
+        ctx.save_for_backward(Y, weights)
+        ctx.plan = plan
+        return ops.combine(Y, weights, plan)
+
+    @staticmethod
+    def backward(ctx, dOut):
+        Y, weights = ctx.saved_tensors
+        return (*ops.combine_backward(dOut, Y, weights, ctx.plan), None)
+
+
+def route_tokens(logits, top_k, bias=None, **options):
+    """``ops.route_tokens`` with a gradient for the logits."""
+    return RouteTokensFunction.apply(logits, bias, top_k, options)
+
+
+def expert_matmul(X, W, plan, *, rows="tokens"):
+    """``ops.expert_matmul`` (W [E, C, N]) with gradients for X and W."""
+    return ExpertMatmulFunction.apply(X, W, plan, rows)
+
+
+def combine(Y, weights, plan):
+    """``ops.combine`` with gradients for Y and the weights."""
+    return CombineFunction.apply(Y, weights, plan)
+
+
+class TokenRouter(nn.Module):
+    """``forward(x [..., I]) -> (weights [..., top_k], experts [..., top_k])``.  ``balance`` [E] is added to the keys of the choice;
+    :meth:`adjust` moves it against the load (it is a buffer: no gradient reaches it).  Options as for ``ops.route_tokens``."""
+
+    def __init__(self, E: int, I: int, top_k: int, **options):
+        super().__init__()
+        self.E, self.I, self.top_k, self.options = E, I, top_k, options
+        self.W = nn.Parameter(torch.empty(E, I))
+        self.register_buffer("balance", None)
+        nn.init.uniform_(self.W, -1 / math.sqrt(I), 1 / math.sqrt(I))
+
+    def forward(self, x):
+        return route_tokens(F.linear(x, self.W), self.top_k, self.balance, **self.options)
+
+    @torch.no_grad()
+    def adjust(self, plan: ops.ExpertPlan, rate: float) -> None:
+        """Lowers the keys of experts with more rows than the mean by ``rate``, raises those of the others (no synchronisation)."""
+        counts = plan.counts().float()
+        if self.balance is None:
+            self.balance = torch.zeros_like(counts)
+        self.balance += rate * torch.sign(counts.mean() - counts)
+
+
+class RoutedExperts(nn.Module):
+    """``out[t] = sum_j weights[t, j] * act(x[t] @ up[e]) @ down[e]`` over the experts ``e`` that the router chose for token t;
+    x [..., I] -> [..., I], up [E, I, J], down [E, J, I], act = SiLU.  No token is dropped, whatever the load of an expert."""
+
+    def __init__(self, E: int, I: int, J: int, top_k: int, **options):
+        super().__init__()
+        self.E, self.I, self.J = E, I, J
+        self.router = TokenRouter(E, I, top_k, **options)
+        self.up = nn.Parameter(torch.empty(E, I, J))
+        self.down = nn.Parameter(torch.empty(E, J, I))
+        nn.init.uniform_(self.up, -1 / math.sqrt(I), 1 / math.sqrt(I))
+        nn.init.uniform_(self.down, -1 / math.sqrt(J), 1 / math.sqrt(J))
+        self.plan = None                                   # of the last call: what router.adjust takes
+
+    def forward(self, x):
+        weights, experts = self.router(x)
+        self.plan = plan = ops.plan_experts(experts, self.E)
+        h = F.silu(expert_matmul(x, self.up, plan))
+        return combine(expert_matmul(h, self.down, plan, rows="sorted"), weights, plan).view(x.shape)
+
+    @torch.no_grad()
+    def quantized(self) -> "RoutedExpertsInt8":
+        return RoutedExpertsInt8(self)
+
+
+class RoutedExpertsInt8(nn.Module):
+    """A :class:`RoutedExperts` for serving: weights in 8 bits with a scale for each output channel, rows quantised on the way into each
+    product with a scale for each row."""
+
+    def __init__(self, layer: RoutedExperts):
+        super().__init__()
+        self.E, self.router = layer.E, layer.router
+        for name in ("up", "down"):
+            q, scale = ops.quantize_rows(getattr(layer, name).detach().transpose(1, 2))
+            self.register_buffer(name, q)
+            self.register_buffer(name + "_scale", scale)
+
+    @torch.no_grad()
+    def forward(self, x):
+        weights, experts = self.router(x)
+        plan = ops.plan_experts(experts, self.E)
+        h = F.silu(ops.expert_matmul_int8(*ops.quantize_rows(x), self.up, self.up_scale, plan, out_dtype=x.dtype))
+        y = ops.expert_matmul_int8(*ops.quantize_rows(h), self.down, self.down_scale, plan, rows="sorted", out_dtype=x.dtype)
+        return ops.combine(y, weights, plan).view(x.shape)

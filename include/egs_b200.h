@@ -304,6 +304,86 @@ int egs_expert_row_sum(const void* Src, const void* Ind, void* out, int64_t B, i
  * Replaces the torch.zeros_like calls of the reference's wrappers (egs/triton_kernels.py:408-409). */
 int egs_fill_zero(void* p, size_t n_bytes, void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Tokens that choose experts.  (No counterpart in the reference, whose experts choose their tokens.)
+ *
+ * A slot is one (token, choice) pair, its number token * k + choice.  A plan sorts the slots by expert, those of one expert in
+ * ascending order; "sorted rows" are rows in that order.  The rows of expert e are offsets[e] .. offsets[e + 1] - 1.
+ * ------------------------------------------------------------------------------------------------ */
+enum { EGS_I8 = 3 };                                     /* element type of the products in 8-bit integers alone */
+enum { EGS_SCORE_SOFTMAX = 0, EGS_SCORE_SIGMOID = 1 };
+enum { EGS_ROWS_TOKENS = 0 /* row token of a slot */, EGS_ROWS_SORTED = 1 };
+enum { EGS_MAX_EXPERTS = 1024, EGS_MAX_CHOICES = 32, EGS_MAX_GROUPS = 32 };
+
+typedef struct egs_route {
+  int64_t tokens;
+  int E;            /* experts, at most EGS_MAX_EXPERTS */
+  int top_k;        /* experts a token takes, at most EGS_MAX_CHOICES */
+  int groups;       /* the experts are that many groups of E / groups consecutive ones, at most EGS_MAX_GROUPS */
+  int top_groups;   /* groups a token may take experts from */
+  int group_top;    /* 1 or 2: a group's value is the sum of that many of its highest keys */
+  int score;        /* EGS_SCORE_* of the logits */
+  int renormalize;  /* weights are divided by their sum (0 where that is 0) */
+  float scale;      /* ... and multiplied by this */
+} egs_route;
+
+/*
+ * Routing: s = softmax or sigmoid of a token's logits; key = s + bias (bias NULL: s, compared by the logits); of the top_groups groups
+ * of highest value the top_k experts of highest key, best first, equal keys and values in ascending order (NaN last).
+ * weights [tokens, top_k] float32: s of those experts, renormalised and scaled.  experts [tokens, top_k].
+ * logits [tokens, E], a token's `row_stride` elements behind the one before.  A token whose logits are all -infinity has weights of 0.
+ */
+int egs_route_tokens(const void* logits, const float* bias, float* weights, int32_t* experts, const egs_route* route, int64_t row_stride,
+                     int dtype, void* cuda_stream);
+/* Its gradient: dlogits [tokens, E] from dweights [tokens, top_k], the logits and the experts chosen (ids outside [0, E) take no part;
+ * those of a token are distinct).  The choice itself and the bias have none.  groups, top_groups, group_top are ignored. */
+int egs_route_tokens_backward(const float* dweights, const void* logits, const int32_t* experts, void* dlogits, const egs_route* route,
+                              int64_t row_stride, int dtype, void* cuda_stream);
+
+/*
+ * The plan of `n` slots: offsets [E + 1], slots [n] (slot of a sorted row), position [n] (sorted row of a slot).  A slot whose expert is
+ * -1 was not routed: it sorts behind offsets[E], and its position is ~row.  Other ids outside [0, E) are treated so too and set
+ * EGS_STATUS_INDEX_OUT_OF_RANGE.  workspace: egs_plan_workspace_bytes() bytes.
+ */
+int egs_plan_experts(const int32_t* experts, int64_t n, int E, int32_t* offsets, int32_t* slots, int32_t* position, void* workspace,
+                     size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
+size_t egs_plan_workspace_bytes(int64_t n, int E);
+
+typedef struct egs_ragged {
+  int64_t tokens, k;  /* slots = tokens * k */
+  int64_t E, C, N;    /* contracted and produced width */
+} egs_ragged;
+
+/* Y[r] = X[row(r)] W[expert(r)] for every sorted row, rows behind offsets[E] zero.  X: token rows [tokens, C] or sorted rows
+ * [tokens * k, C] (rows: EGS_ROWS_*); W [E, C, N] or [E, N, C] (w_layout).  Sums in float32, rounded once.
+ * workspace: egs_expert_matmul_workspace_bytes() bytes (16-bit operands whose rows do not begin on 16 bytes are copied there). */
+int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
+                      int w_layout, int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
+size_t egs_expert_matmul_workspace_bytes(const egs_ragged* dims, int rows, int w_layout, int dtype);
+/* dW[e] = sum over the rows r of e of X[row(r)]^T dY[r]: [E, C, N], zero for experts without rows.  dY: sorted rows [tokens * k, N]. */
+int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, const int32_t* slots, void* dW, const egs_ragged* dims, int rows,
+                       int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
+size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype);
+
+/* out[t] = sum over j of weights[t, j] Y[position[t * k + j]]: token rows [tokens, N] from sorted rows.  weights NULL: ones.  Float32 in
+ * the order of j, rounded once.  weights_dtype: EGS_F32 or the rows' type. */
+int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
+                int weights_dtype, void* cuda_stream);
+/* Its gradients: dY (sorted rows; zeros for slots that were not routed) and, where dweights is given, dweights[t, j] = <dOut[t], Y[..]>. */
+int egs_combine_backward(const void* dOut, const void* Y, const void* weights, const int32_t* position, void* dY, void* dweights,
+                         int64_t tokens, int64_t k, int64_t N, int dtype, int weights_dtype, void* cuda_stream);
+
+/* Rows in 8 bits: scale[r] = max |X[r]| / 127, q = X / scale to the nearest integer (ties to even), in [-127, 127].  A row of zeros has
+ * the scale 0; one with an infinity or a NaN the scale NaN.  Strides in elements. */
+int egs_quantize_rows(const void* X, int8_t* q, float* scale, int64_t rows, int64_t C, int64_t x_stride, int64_t q_stride, int dtype,
+                      void* cuda_stream);
+/* Y[r, n] = q_scale[row] * w_scale[e, n] * sum over c of q[row, c] Wq[e, n, c], int32 sums (C < 131072), in out_dtype.
+ * Wq [E, N, C] with w_stride elements from one channel to the next; offsets NULL: one expert that has all tokens (k = 1).
+ * Runs on the tensor cores where both strides are multiples of 16 and both bases 16-byte aligned. */
+int egs_expert_matmul_int8(const int8_t* q, const float* q_scale, int64_t q_stride, const int8_t* Wq, const float* w_scale, int64_t w_stride,
+                           const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows, int out_dtype, int path,
+                           int32_t* status_word, void* cuda_stream);
+
 /* Number of kernels the library has launched in this process since load (for launch accounting). */
 int64_t egs_launch_count(void);
 
