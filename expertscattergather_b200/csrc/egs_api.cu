@@ -44,7 +44,7 @@ static bool encode_tensor_map(TensorMap3* out, const void* base, int elem_bytes,
     if (i + 1 < rank) gstride[i] = strides ? strides[i] : pitch;
   }
   // integer types: the loads only move bits
-  const CUresult rc = encode(reinterpret_cast<CUtensorMap*>(out), elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim,
+  const CUresult rc = encode(reinterpret_cast<CUtensorMap*>(out), elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim,
                              gstride, bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS;
@@ -55,6 +55,10 @@ bool encode_tensor_map_16bit(TensorMap3* out, const void* base, int rank, const 
 bool encode_tensor_map_16bit_strided(TensorMap3* out, const void* base, int rank, const unsigned long long* dims, const unsigned long long* strides,
                                      const unsigned* box) {
   return encode_tensor_map(out, base, 2, rank, dims, box, CU_TENSOR_MAP_SWIZZLE_128B, strides);
+}
+bool encode_tensor_map_strided(TensorMap3* out, const void* base, int elem_bytes, int rank, const unsigned long long* dims, const unsigned long long* strides,
+                               const unsigned* box) {
+  return encode_tensor_map(out, base, elem_bytes, rank, dims, box, CU_TENSOR_MAP_SWIZZLE_128B, strides);
 }
 bool encode_tensor_map_32bit(TensorMap3* out, const void* base, int rank, const unsigned long long* dims, const unsigned* box, int swizzle) {
   return encode_tensor_map(out, base, 4, rank, dims, box,

@@ -725,6 +725,20 @@ __global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_consta
     }
 }
 
+// Rows of 16-bit elements with another pitch; a thread writes eight elements.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short* src, uint4* dst, long long vectors, int width, int per_row) {
+  pdl_wait();
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= vectors) return;
+  const long long row = i / per_row;
+  const int c = static_cast<int>(i - row * per_row) * 8;
+  const unsigned short* s = src + row * width + c;
+  unsigned short v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c + j < width ? s[j] : 0;
+  dst[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+}
+
 template <typename T, int NPER>
 cudaError_t route_n(const RouteParams& p, cudaStream_t st) {
   const size_t smem = p.groups > 1 ? sizeof(float) * kRouteWarps * p.E : 0;
@@ -858,6 +872,13 @@ cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long lo
   count_launch();
   return by_type(dtype, [&] { return quantize_t<__half>(p, st); }, [&] { return quantize_t<__nv_bfloat16>(p, st); },
                  [&] { return quantize_t<float>(p, st); });
+}
+
+cudaError_t launch_pad_rows(const void* src, void* dst, long long rows, int width, int pitch, cudaStream_t st) {
+  const long long vectors = rows * (pitch / 8);
+  count_launch();
+  return launch_kernel(pad_rows_kernel, static_cast<unsigned>((vectors + 255) / 256), 256, 0, st, true, static_cast<const unsigned short*>(src),
+                       static_cast<uint4*>(dst), vectors, width, pitch / 8);
 }
 
 // Row blocks there can be: every expert with rows may have one that is not full.

@@ -43,6 +43,31 @@ RaggedParams ragged(const egs_ragged& d, int rows) {
   return p;
 }
 
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Tiles have 32-bit numbers.
+bool tiles_fit(const RaggedParams& p) {
+  const double blocks = p.rows / 128.0 + p.E + 1, wide = p.N / 64.0 + 1, deep = p.C / 128.0 + 1;
+  return blocks * wide < 2e9 && p.E * deep * wide < 2e9;
+}
+
+// The tensor cores read 16-bit rows that begin on 16 bytes.  Others are copied: bytes of such a copy, 0 where none is needed.
+long long pitch8(long long width) { return (width + 7) / 8 * 8; }
+size_t copy_bytes(long long rows, long long width) {
+  return width % 8 ? (static_cast<size_t>(rows) * pitch8(width) * 2 + 255) & ~static_cast<size_t>(255) : 0;
+}
+// ... of `rows` rows of `width` elements at *src, which *pitch becomes the pitch of; moves `workspace` on
+cudaError_t copy_padded(const void** src, long long* pitch, long long rows, long long width, char** workspace, cudaStream_t st) {
+  if (width % 8 == 0) return cudaSuccess;
+  char* to = *workspace;
+  *workspace += copy_bytes(rows, width);
+  *pitch = pitch8(width);
+  const cudaError_t err = launch_pad_rows(*src, to, rows, static_cast<int>(width), static_cast<int>(*pitch), st);
+  *src = to;
+  return err;
+}
+long long a_rows_of(const egs_ragged& d, int rows) { return rows == EGS_ROWS_TOKENS ? d.tokens : d.tokens * d.k; }
+
 }  // namespace
 }  // namespace egs
 
@@ -80,7 +105,11 @@ int egs_plan_experts(const int32_t* experts, int64_t n, int E, int32_t* offsets,
               "plan_experts launch");
 }
 
-size_t egs_expert_matmul_workspace_bytes(const egs_ragged* dims, int rows, int w_layout, int dtype) { return 0; }
+size_t egs_expert_matmul_workspace_bytes(const egs_ragged* dims, int rows, int w_layout, int dtype) {
+  if (dtype == EGS_F32 || check_ragged(dims) != EGS_OK || !valid_rows(rows) || !valid_layout(w_layout)) return 0;
+  return copy_bytes(a_rows_of(*dims, rows), dims->C) +
+         (w_layout == EGS_W_NC ? copy_bytes(dims->E * dims->N, dims->C) : copy_bytes(dims->E * dims->C, dims->N));
+}
 
 int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
                       int w_layout, int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream) {
@@ -93,10 +122,24 @@ int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, cons
   p.status = status_ref(status_word);
   p.nc = w_layout == EGS_W_NC;
   p.a_row = p.C; p.w_row = p.nc ? p.C : p.N; p.w_expert = static_cast<long long>(p.C) * p.N;
-  return done(launch_ragged_rows(p, dtype, dtype, stream_of(cuda_stream)), "expert_matmul launch");
+  const cudaStream_t st = stream_of(cuda_stream);
+  const bool able = device_is_sm100() && dtype != EGS_F32 && p.C > 0 && aligned16(X) && aligned16(W) && tiles_fit(p);
+  if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
+  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_rows(p, dtype, dtype, st), "expert_matmul launch");
+  const size_t need = egs_expert_matmul_workspace_bytes(dims, rows, w_layout, dtype);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  cudaError_t err = copy_padded(&p.A, &p.a_row, p.a_rows, p.C, &ws, st);
+  if (err == cudaSuccess) err = copy_padded(&p.W, &p.w_row, dims->E * (p.nc ? p.N : p.C), p.w_row, &ws, st);
+  if (err != cudaSuccess) return fail_cuda(err, "expert_matmul copies");
+  p.w_expert = p.w_row * (p.nc ? p.N : p.C);
+  return done(launch_ragged_rows_tensor(p, dtype, dtype, st), "expert_matmul launch");
 }
 
-size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype) { return 0; }
+size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype) {
+  if (dtype == EGS_F32 || check_ragged(dims) != EGS_OK || !valid_rows(rows)) return 0;
+  return copy_bytes(a_rows_of(*dims, rows), dims->C) + copy_bytes(dims->tokens * dims->k, dims->N);
+}
 
 int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, const int32_t* slots, void* dW, const egs_ragged* dims, int rows,
                        int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream) {
@@ -111,7 +154,17 @@ int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, co
   p.A = X; p.W = dY; p.Out = dW; p.offsets = offsets; p.slots = rows == EGS_ROWS_TOKENS ? slots : nullptr;
   p.status = status_ref(status_word);
   p.a_row = p.C; p.w_row = p.N;
-  return done(launch_ragged_dweight(p, dtype, stream_of(cuda_stream)), "expert_dweight launch");
+  const cudaStream_t st = stream_of(cuda_stream);
+  const bool able = device_is_sm100() && dtype != EGS_F32 && aligned16(X) && aligned16(dY) && tiles_fit(p);
+  if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
+  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_dweight(p, dtype, st), "expert_dweight launch");
+  const size_t need = egs_expert_dweight_workspace_bytes(dims, rows, dtype);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  cudaError_t err = copy_padded(&p.A, &p.a_row, p.a_rows, p.C, &ws, st);
+  if (err == cudaSuccess) err = copy_padded(&p.W, &p.w_row, p.rows, p.N, &ws, st);
+  if (err != cudaSuccess) return fail_cuda(err, "expert_dweight copies");
+  return done(launch_ragged_dweight_tensor(p, dtype, st), "expert_dweight launch");
 }
 
 int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
@@ -162,7 +215,10 @@ int egs_expert_matmul_int8(const int8_t* q, const float* q_scale, int64_t q_stri
   p.status = status_ref(status_word);
   p.nc = 1;
   p.a_row = q_stride; p.w_row = w_stride; p.w_expert = w_stride * p.N;
-  return done(launch_ragged_rows(p, EGS_I8, out_dtype, stream_of(cuda_stream)), "expert_matmul_int8 launch");
+  const bool able = device_is_sm100() && p.C > 0 && p.a_row % 16 == 0 && p.w_row % 16 == 0 && aligned16(q) && aligned16(Wq) && tiles_fit(p);
+  if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
+  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_rows(p, EGS_I8, out_dtype, stream_of(cuda_stream)), "expert_matmul_int8 launch");
+  return done(launch_ragged_rows_tensor(p, EGS_I8, out_dtype, stream_of(cuda_stream)), "expert_matmul_int8 launch");
 }
 
 }  // extern "C"

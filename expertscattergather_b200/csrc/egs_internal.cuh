@@ -233,6 +233,9 @@ bool encode_tensor_map_16bit(TensorMap3* out, const void* base, int rank, const 
 // ... of up to five dimensions whose strides (bytes, of all but the first) are given
 bool encode_tensor_map_16bit_strided(TensorMap3* out, const void* base, int rank, const unsigned long long* dims, const unsigned long long* strides,
                                      const unsigned* box);
+// ... of elements of 1 or 2 bytes
+bool encode_tensor_map_strided(TensorMap3* out, const void* base, int elem_bytes, int rank, const unsigned long long* dims, const unsigned long long* strides,
+                               const unsigned* box);
 // The same for 32-bit elements.  kMapSwizzle128Base32: the XOR of the 128-byte swizzle acts on 32-byte pairs of chunks with the row modulo 4.
 enum { kMapSwizzleNone = 0, kMapSwizzle128 = 1, kMapSwizzle128Base32 = 2 };
 bool encode_tensor_map_32bit(TensorMap3* out, const void* base, int rank, const unsigned long long* dims, const unsigned* box, int swizzle);
@@ -265,6 +268,11 @@ cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long lo
 // dtype EGS_I8: 8-bit operands with scales, products in out_dtype
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, cudaStream_t st);
+// ... on the tensor cores (egs_ragged.cu): 16-bit or 8-bit operands whose rows begin on 16 bytes, C and N at least 1
+cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
+cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, cudaStream_t st);
+// Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; what lies behind a row's end is not defined).
+cudaError_t launch_pad_rows(const void* src, void* dst, long long rows, int width, int pitch, cudaStream_t st);
 
 // Errors of the C entries (egs_api.cu): remembers the text, returns EGS_ERR_CUDA.
 int fail_cuda(cudaError_t err, const char* where);

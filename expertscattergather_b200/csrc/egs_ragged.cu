@@ -1,0 +1,641 @@
+// Products over ragged rows on the tensor cores (sm_100a): the rows of expert e are the sorted rows offsets[e] .. offsets[e + 1] - 1,
+// a different number for every expert, known on the device alone.  16-bit operands with float32 sums, 8-bit integers with int32 sums.
+//
+//   rows      Y[r] = X[row(r)] W[e]            tiles of 128 sorted rows of one expert (256 on a pair of CTAs) x BN columns
+//   weights   dW[e] = sum of X[row(r)]^T dY[r]   tiles of 128 (256) features of X x BN features of dY, the contraction over the rows of e
+//
+// Persistent CTAs (or pairs, cta_group::2), one per SM, walk the tiles; how many there are every CTA finds from the offsets when it
+// begins.  All operands come by TMA: rows that lie anywhere four at a time (tile::gather4), rows that follow one another and weights in
+// boxes.  A step is 128 bytes of the contraction for `rows` and 64 rows for `weights`.
+//
+//   warps 0..3    gathered rows of X, where they are gathered
+//   warp  4       boxes; announces the bytes of a stage
+//   warp  5       tensor-memory allocation; four tcgen05.mma a stage, issued by the leader of a pair for both CTAs
+//   warps 8..15   read-out: tensor memory -> (scales) -> rows of the output; zeros for rows that belong to no expert
+//
+// Rows of a tile that belong to the next expert are computed and not stored.  In a contraction over rows they would do harm, even where
+// the other operand is 0 (0 * infinity), so the last step of an expert takes the rows behind its end from outside the tensor: zeros.
+#include <type_traits>
+
+#include "egs_tcgen05.cuh"
+
+namespace egs {
+
+namespace {
+
+constexpr int kGatherWarps = 4, kBoxWarp = 4, kIssueWarp = 5, kReadWarp0 = 8, kReadWarps = 8;
+constexpr int kRaggedThreads = (kReadWarp0 + kReadWarps) * 32;
+constexpr uint32_t kRaggedHeader = 512;
+constexpr uint32_t kATile = 16384;                 // 128 rows x 128 bytes, or 64 rows x 128 features of 2 bytes
+constexpr uint32_t kSegBytes = 8192;               // 64 rows x 128 bytes: a column segment of a tile whose rows are the contraction's
+constexpr uint32_t kReadArea = 4096;               // transpose of a read-out warp
+constexpr size_t kRaggedSmem = 227 * 1024;
+constexpr int kSmCount = 148;
+
+struct __align__(16) RaggedHeader {
+  unsigned long long full[kMaxStages];
+  unsigned long long empty[kMaxStages];
+  unsigned long long acc_full[2];
+  unsigned long long acc_empty[2];
+  unsigned long long drain;
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+  int warp_sums[kRaggedThreads / 32];
+};
+static_assert(sizeof(RaggedHeader) <= kRaggedHeader, "header does not fit");
+
+struct RaggedTiles {
+  int BN, stages, steps;       // steps: of `rows`
+  int tiles_n, tiles_c;        // column tiles; `weights`: tiles over X's features
+  int units;                   // `weights`: all of them
+  int gathers;                 // X's rows are gathered
+  int vectors;                 // rows of the output begin on 16 bytes and are whole 16 bytes
+  uint32_t table_bytes;        // of each of the two tables
+  Div by_n, by_c;
+};
+
+__host__ __device__ constexpr uint32_t b_tile_bytes(int columns) { return static_cast<uint32_t>(columns) * 128u; }
+
+template <bool PAIR>
+__device__ __forceinline__ void load_box(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
+  if (PAIR) tma_load_3d_pair(dst, map, x, y, z, bar);
+  else tma_load_3d(dst, map, x, y, z, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_rows4(uint32_t dst, const void* map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
+  if (PAIR)
+    tma_gather4_pair(dst, map, x, r0, r1, r2, r3, bar);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+        : "memory");
+}
+
+// Four contraction steps of 32 bytes of 8-bit integers (16-bit operands: umma_f16_x4).
+#define EGS_I8_X4(GROUP)                                                    \
+  asm volatile(                                                             \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"                        \
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"                   \
+      "tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], %1, %2, %3, p;\n\t"  \
+      "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 2;\n\t"                          \
+      "tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %3, q;\n\t"    \
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t"                            \
+      "tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %3, q;\n\t"    \
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t"                            \
+      "tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %3, q;\n\t}"   \
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)    \
+      : "memory")
+template <bool PAIR>
+__device__ __forceinline__ void umma_i8_x4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR) EGS_I8_X4("2");
+  else EGS_I8_X4("1");
+}
+
+struct RingCursor {
+  int slot = 0, round = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++slot == stages) {
+      slot = 0;
+      ++round;
+    }
+  }
+};
+
+// The expert of row block `block`, from the numbers of the blocks before each expert's; `e` is where the last search ended.
+__device__ __forceinline__ int expert_of(const int* starts, int E, int block, int e) {
+  if (starts[e + 1] > block) return e;
+  int lo = e + 1, hi = E - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid + 1] > block) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+template <typename OutT>
+__device__ __forceinline__ uint32_t pack_out(uint32_t a, uint32_t b) { return pack2(static_cast<OutT*>(nullptr), a, b); }
+
+// T: operands' type (int8_t: with scales), OutT: the output's.
+template <typename T, typename OutT, bool WEIGHTS, bool PAIR>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kRaggedThreads, 1)
+ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ RaggedTiles q, const __grid_constant__ TensorMap3 map_a,
+              const __grid_constant__ TensorMap3 map_a4, const __grid_constant__ TensorMap3 map_b, const __grid_constant__ TensorMap3 map_b4) {
+  constexpr bool kInt8 = sizeof(T) == 1;
+  constexpr int kBlock = PAIR ? 256 : 128;           // rows of a tile
+  constexpr int kStepElems = 128 / sizeof(T);        // `rows`
+  constexpr int kStepRows = 64;                      // `weights`
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  RaggedHeader* hdr = reinterpret_cast<RaggedHeader*>(smem_raw);
+  int* offsets = reinterpret_cast<int*>(smem_raw + kRaggedHeader);
+  int* starts = reinterpret_cast<int*>(smem_raw + kRaggedHeader + q.table_bytes);      // row blocks before each expert's
+  const uint32_t smem0 = smem_u32(smem_raw);
+  const uint32_t ring0 = (smem0 + kRaggedHeader + 2u * q.table_bytes + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
+  const bool leader = rank == 0;
+  const int columns = PAIR ? q.BN / 2 : q.BN;        // of the right operand, staged by this CTA
+  const uint32_t stage_bytes = kATile + b_tile_bytes(columns);
+  const uint32_t area0 = ring0 + static_cast<uint32_t>(q.stages) * stage_bytes;
+  const uint32_t acc_cols = tmem_cols_for(q.BN);
+  volatile uint32_t* abort_flag = &hdr->abort_flag;
+  const int first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_stride = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+  // ---- set-up ----
+  if (tid == 0) {
+    for (int s = 0; s < kMaxStages; ++s) {
+      mbar_init(smem_u32(&hdr->full[s]), 1);
+      mbar_init(smem_u32(&hdr->empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&hdr->acc_full[b]), 1);
+      mbar_init(smem_u32(&hdr->acc_empty[b]), PAIR ? 2 * kReadWarps : kReadWarps);     // (a pair's: the leader's copy is used)
+    }
+    mbar_init(smem_u32(&hdr->drain), 1);
+    fence_mbar_init();
+  }
+  pdl_wait();
+  if (tid == 0) {
+    hdr->abort_flag = p.status.timed_out() ? 1u : 0u;
+    if (smem_misaligned(smem_raw)) {
+      hdr->abort_flag = 1u;
+      p.status.report(EGS_STATUS_INTERNAL);
+    }
+  }
+  if (p.offsets)
+    for (int e = tid; e <= p.E; e += kRaggedThreads) offsets[e] = p.offsets[e];
+  else if (tid < 2)
+    offsets[tid] = tid ? p.rows : 0;
+  __syncthreads();
+  if (warp == kIssueWarp) {
+    if (PAIR) {
+      tmem_alloc2(smem_u32(&hdr->tmem_base), 2u * acc_cols);
+      tmem_relinquish2();
+    } else {
+      tmem_alloc(smem_u32(&hdr->tmem_base), 2u * acc_cols);
+      tmem_relinquish();
+    }
+  }
+  if (!WEIGHTS) {
+    int carry = 0;
+    for (int e0 = 0; e0 < p.E; e0 += kRaggedThreads) {
+      const int e = e0 + tid;
+      int incl = e < p.E ? (offsets[e + 1] - offsets[e] + kBlock - 1) / kBlock : 0;
+      const int own = incl;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) hdr->warp_sums[warp] = incl;
+      __syncthreads();
+      int before = carry;
+      for (int w = 0; w < kRaggedThreads / 32; ++w) {
+        if (w < warp) before += hdr->warp_sums[w];
+        carry += hdr->warp_sums[w];
+      }
+      if (e < p.E) starts[e] = before + incl - own;
+      if (e == p.E - 1) starts[p.E] = before + incl;
+      __syncthreads();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();                      // both CTAs' barriers are initialised before anything crosses the pair
+  tc_fence_after();
+  const uint32_t tmem_base = hdr->tmem_base;
+  const int units = WEIGHTS ? q.units : starts[p.E] * q.tiles_n;
+  const uint32_t full0 = PAIR ? map_to_cta(smem_u32(&hdr->full[0]), 0) : smem_u32(&hdr->full[0]);
+  RingCursor at;
+  bool alive = true;
+  auto wait_free = [&]() {
+    if (at.round > 0) alive = mbar_wait_all(smem_u32(&hdr->empty[at.slot]), (at.round - 1) & 1, abort_flag, p.status.word);
+    return alive;
+  };
+
+  if (hdr->abort_flag != 0u) {
+    // fall through to the common exit
+  } else if (warp < kGatherWarps) {
+    // =========================== gathered rows ===========================
+    if (q.gathers) {
+      if constexpr (!WEIGHTS) {
+        int e = 0;
+        for (int u = first_unit; u < units && alive; u += unit_stride) {
+          const int block = q.by_n.quotient(u);
+          e = expert_of(starts, p.E, block, e);
+          const int r = offsets[e] + (block - starts[e]) * kBlock + rank * 128 + warp * 32 + lane;
+          const int mine = r < offsets[e + 1] ? p.by_k.quotient(p.slots[r]) : -1;
+          int row[8][4];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) row[i][j] = __shfl_sync(0xffffffffu, mine, i * 4 + j);
+          for (int ks = 0; ks < q.steps; ++ks) {
+            if (!wait_free()) break;
+            const uint32_t bar = full0 + at.slot * 8u;
+            const uint32_t dst = ring0 + static_cast<uint32_t>(at.slot) * stage_bytes + static_cast<uint32_t>(warp) * 4096u;
+            at.next(q.stages);
+            if (elect_one()) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                load_rows4<PAIR>(dst + i * 512u, &map_a4, ks * kStepElems, row[i][0], row[i][1], row[i][2], row[i][3], bar);
+            }
+          }
+        }
+      } else {
+        // a warp has 16 rows of every step; lanes 16..31 look up those of the step behind
+        for (int u = first_unit; u < units && alive; u += unit_stride) {
+          int x = q.by_n.quotient(u);
+          const int c = q.by_c.remainder(x), e = x;
+          const int begin = offsets[e], end = offsets[e + 1];
+          auto look = [&](int step) {                // (an even one)
+            const int r = begin + (step + (lane >> 4)) * kStepRows + warp * 16 + (lane & 15);
+            return r < end ? p.slots[r] : -1;
+          };
+          const int steps = (end - begin + kStepRows - 1) / kStepRows;
+          const int f0 = c * kBlock + rank * 128;
+          int coming = steps ? look(0) : -1, now = -1;
+          for (int ks = 0; ks < steps; ++ks) {
+            if (!(ks & 1)) {
+              now = coming < 0 ? -1 : p.by_k.quotient(coming);
+              coming = ks + 2 < steps ? look(ks + 2) : -1;
+            }
+            int row[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) row[i][j] = __shfl_sync(0xffffffffu, now, (ks & 1) * 16 + i * 4 + j);
+            if (!wait_free()) break;
+            const uint32_t bar = full0 + at.slot * 8u;
+            const uint32_t dst = ring0 + static_cast<uint32_t>(at.slot) * stage_bytes + static_cast<uint32_t>(warp) * 2048u;
+            at.next(q.stages);
+            if (elect_one()) {
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  load_rows4<PAIR>(dst + s * kSegBytes + i * 512u, &map_a4, f0 + s * 64, row[i][0], row[i][1], row[i][2], row[i][3], bar);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kBoxWarp) {
+    // =========================== boxes ===========================
+    const uint32_t bytes = PAIR ? 2u * stage_bytes : stage_bytes;       // announced by the leader for both CTAs
+    int e = 0;
+    for (int u = first_unit; u < units && alive; u += unit_stride) {
+      const int x = q.by_n.quotient(u);
+      const int n0 = (u - x * q.tiles_n) * q.BN + rank * columns;
+      int steps = q.steps, a0 = 0, f0 = 0, begin = 0, end = 0;
+      if constexpr (!WEIGHTS) {
+        e = expert_of(starts, p.E, x, e);
+        a0 = offsets[e] + (x - starts[e]) * kBlock + rank * 128;
+      } else {
+        int y = x;
+        f0 = q.by_c.remainder(y) * kBlock + rank * 128;
+        e = y;
+        begin = offsets[e];
+        end = offsets[e + 1];
+        steps = (end - begin + kStepRows - 1) / kStepRows;
+      }
+      for (int ks = 0; ks < steps; ++ks) {
+        if (!wait_free()) break;
+        const uint32_t own = smem_u32(&hdr->full[at.slot]), bar = full0 + at.slot * 8u;
+        const uint32_t a_dst = ring0 + static_cast<uint32_t>(at.slot) * stage_bytes, b_dst = a_dst + kATile;
+        at.next(q.stages);
+        if (elect_one()) {
+          if (leader) mbar_arrive_expect_tx(own, bytes);
+          if constexpr (!WEIGHTS) {
+            if (!q.gathers) load_box<PAIR>(a_dst, &map_a, ks * kStepElems, a0, 0, bar);
+            if (p.nc) {
+              load_box<PAIR>(b_dst, &map_b, ks * kStepElems, n0, e, bar);
+            } else {
+              for (int s = 0; s * 64 < columns; ++s) load_box<PAIR>(b_dst + s * kSegBytes, &map_b, n0 + s * 64, ks * kStepElems, e, bar);
+            }
+          } else {
+            const int r0 = begin + ks * kStepRows;
+            if (r0 + kStepRows <= end) {
+              if (!q.gathers)
+                for (int s = 0; s < 2; ++s) load_box<PAIR>(a_dst + s * kSegBytes, &map_a, f0 + s * 64, r0, 0, bar);
+              for (int s = 0; s * 64 < columns; ++s) load_box<PAIR>(b_dst + s * kSegBytes, &map_b, n0 + s * 64, r0, 0, bar);
+            } else {                                 // the last rows of the expert, zeros behind them
+              for (int i = 0; i < kStepRows / 4; ++i) {
+                const int r = r0 + i * 4;
+                const int ra = r < end ? r : -1, rb = r + 1 < end ? r + 1 : -1, rc = r + 2 < end ? r + 2 : -1, rd = r + 3 < end ? r + 3 : -1;
+                if (!q.gathers)
+                  for (int s = 0; s < 2; ++s) load_rows4<PAIR>(a_dst + s * kSegBytes + i * 512u, &map_a4, f0 + s * 64, ra, rb, rc, rd, bar);
+                for (int s = 0; s * 64 < columns; ++s)
+                  load_rows4<PAIR>(b_dst + s * kSegBytes + i * 512u, &map_b4, n0 + s * 64, ra, rb, rc, rd, bar);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kIssueWarp) {
+    // =========================== MMA issuer ===========================
+    if (leader) {
+      const bool b_mn = WEIGHTS || !p.nc;
+      const uint64_t a_desc = WEIGHTS ? make_smem_desc(0u, kSegBytes, 1024u) : make_smem_desc(0u, 16u, 1024u);
+      const uint64_t b_desc = (b_mn ? make_smem_desc(0u, kSegBytes, 1024u) : make_smem_desc(0u, 16u, 1024u)) + (kATile >> 4);
+      const uint32_t a_adv = (WEIGHTS ? 16u * 128u : 32u) >> 4, b_adv = (b_mn ? 16u * 128u : 32u) >> 4;
+      // 8-bit integers: signed operands (format 1), int32 accumulator (format 2 in the place of 1)
+      const uint32_t idesc = kInt8 ? make_idesc(1u, 0u, 0u, kBlock, q.BN) + (1u << 4)
+                                   : make_idesc(sizeof(T) == 2 ? Elem<typename std::conditional<kInt8, __half, T>::type>::fmt : 0u, WEIGHTS ? 1u : 0u,
+                                                b_mn ? 1u : 0u, kBlock, q.BN);
+      int t = 0;                                     // tiles with an accumulator
+      for (int u = first_unit; u < units && alive; u += unit_stride) {
+        int steps = q.steps;
+        if constexpr (WEIGHTS) {
+          int x = q.by_n.quotient(u);
+          x = q.by_c.quotient(x);
+          steps = (offsets[x + 1] - offsets[x] + kStepRows - 1) / kStepRows;
+          if (steps == 0) continue;
+        }
+        const int buf = t & 1;
+        if (t >= 2) {
+          alive = mbar_wait_all<PAIR>(smem_u32(&hdr->acc_empty[buf]), ((t >> 1) - 1) & 1, abort_flag, p.status.word);
+          if (!alive) break;
+        }
+        ++t;
+        const uint32_t d = tmem_base + static_cast<uint32_t>(buf) * acc_cols;
+        for (int ks = 0; ks < steps; ++ks) {
+          alive = mbar_wait_all<PAIR>(smem_u32(&hdr->full[at.slot]), at.round & 1, abort_flag, p.status.word);
+          if (!alive) break;
+          const uint32_t empty = smem_u32(&hdr->empty[at.slot]);
+          const uint32_t addr = (ring0 + static_cast<uint32_t>(at.slot) * stage_bytes) >> 4;
+          at.next(q.stages);
+          tc_fence_after();
+          if (elect_one()) {
+            if constexpr (kInt8) umma_i8_x4<PAIR>(d, a_desc + addr, b_desc + addr, idesc, ks > 0 ? 1u : 0u);
+            else umma_f16_x4<PAIR>(d, a_desc + addr, b_desc + addr, a_adv, b_adv, idesc, ks > 0 ? 1u : 0u);
+            umma_done<PAIR>(empty);
+            if (ks + 1 == steps) umma_done<PAIR>(smem_u32(&hdr->acc_full[buf]));
+          }
+        }
+      }
+    }
+    pdl_trigger();
+    __syncwarp();
+  } else if (warp >= kReadWarp0) {
+    // =========================== read-out ===========================
+    const int ew = warp - kReadWarp0, lg = ew & 3, share = ew >> 2;     // TMEM lane group (warp number mod 4), share of the column blocks
+    const uint32_t area = area0 + static_cast<uint32_t>(ew) * kReadArea;
+    const uint32_t lane_base = static_cast<uint32_t>(lg * 32) << 16;
+    OutT* out = static_cast<OutT*>(p.Out);
+    if (!WEIGHTS && p.offsets) {                     // rows that belong to no expert
+      const long long begin = static_cast<long long>(offsets[p.E]) * p.N, end = static_cast<long long>(p.rows) * p.N;
+      const long long step = static_cast<long long>(gridDim.x) * (kReadWarps * 32);
+      for (long long i = begin + blockIdx.x * (kReadWarps * 32) + ew * 32 + lane; i < end; i += step) out[i] = from_f32<OutT>(0.f);
+    }
+    int e = 0, t = 0;
+    for (int u = first_unit; u < units && alive; u += unit_stride) {
+      const int x = q.by_n.quotient(u);
+      const int n0 = (u - x * q.tiles_n) * q.BN, bn = min(q.BN, p.N - n0);
+      long long row0;                                // output row of the warp's first accumulator row
+      int rows;                                      // of its 32 that are stored
+      bool have = true;
+      float scale = 0.f;
+      if constexpr (!WEIGHTS) {
+        e = expert_of(starts, p.E, x, e);
+        const int r = offsets[e] + (x - starts[e]) * kBlock + rank * 128 + lg * 32;
+        row0 = r;
+        rows = min(32, offsets[e + 1] - r);
+        if constexpr (kInt8) {
+          if (lane < rows) scale = p.a_scale[p.slots ? p.by_k.quotient(p.slots[r + lane]) : r + lane];
+        }
+      } else {
+        int y = x;
+        const int f = q.by_c.remainder(y) * kBlock + rank * 128 + lg * 32;
+        e = y;
+        row0 = static_cast<long long>(e) * p.C + f;
+        rows = min(32, p.C - f);
+        have = offsets[e + 1] > offsets[e];
+      }
+      const int buf = t & 1;
+      if (have) {
+        alive = mbar_wait_all(smem_u32(&hdr->acc_full[buf]), (t >> 1) & 1, abort_flag, p.status.word);
+        if (!alive) break;
+        ++t;
+        tc_fence_after();
+      }
+      const uint32_t acc = tmem_base + lane_base + static_cast<uint32_t>(buf) * acc_cols;
+      bool released = false;
+      auto release = [&]() {
+        if (!have || released) return;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&hdr->acc_empty[buf]), 0));
+          else mbar_arrive(smem_u32(&hdr->acc_empty[buf]));
+        }
+        released = true;
+      };
+      // 32 columns of the accumulator in float32
+      auto read = [&](int c, uint32_t (&v)[32]) {
+        if (have) {
+          tmem_ld32(acc + static_cast<uint32_t>(c), v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0u;
+        }
+        if constexpr (kInt8) {
+          const float* ws = p.w_scale + static_cast<long long>(e) * p.N + n0 + c;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float w = c + i < bn ? ws[i] : 0.f;
+            v[i] = __float_as_uint(static_cast<float>(static_cast<int>(v[i])) * (scale * w));
+          }
+        }
+      };
+      if constexpr (sizeof(OutT) == 2) {
+        // 64 columns = 128 bytes of a row at a time, eight lanes to a row
+        for (int c = share * 64; c < bn; c += 128) {
+          const uint32_t srow = area + static_cast<uint32_t>(lane) * 128u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (c + h * 32 < bn) {
+              uint32_t v[32];
+              read(c + h * 32, v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(srow + static_cast<uint32_t>((h * 4 + j) ^ (lane & 7)) * 16u),
+                             "r"(pack_out<OutT>(v[8 * j], v[8 * j + 1])), "r"(pack_out<OutT>(v[8 * j + 2], v[8 * j + 3])),
+                             "r"(pack_out<OutT>(v[8 * j + 4], v[8 * j + 5])), "r"(pack_out<OutT>(v[8 * j + 6], v[8 * j + 7]))
+                             : "memory");
+            }
+          }
+          if (c + 128 >= bn) release();              // the accumulator has been read: the next tile but one may begin
+          __syncwarp();
+          if (q.vectors) {
+            const int j = lane & 7, col = c + j * 8;
+            uint4 y[8];
+#pragma unroll
+            for (int it = 0; it < 8; ++it) {
+              const int row = it * 4 + (lane >> 3);
+              asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(y[it].x), "=r"(y[it].y), "=r"(y[it].z), "=r"(y[it].w)
+                           : "r"(area + row * 128u + (static_cast<uint32_t>(j ^ (row & 7)) << 4))
+                           : "memory");
+            }
+#pragma unroll
+            for (int it = 0; it < 8; ++it) {
+              const int row = it * 4 + (lane >> 3);
+              if (row < rows && col < bn) *reinterpret_cast<uint4*>(out + (row0 + row) * p.N + n0 + col) = y[it];
+            }
+          } else {                                   // rows that begin anywhere: element by element along a row
+            for (int row = 0; row < min(rows, 32); ++row)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int i = h * 32 + lane;
+                unsigned short b;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(area + row * 128u + (static_cast<uint32_t>((i >> 3) ^ (row & 7)) << 4) + (i & 7) * 2u) : "memory");
+                if (c + i < bn) reinterpret_cast<unsigned short*>(out)[(row0 + row) * p.N + n0 + c + i] = b;
+              }
+          }
+          __syncwarp();
+        }
+      } else {
+        for (int c = share * 32; c < bn; c += 64) {
+          uint32_t v[32];
+          read(c, v);
+          if (c + 64 >= bn) release();
+          warp_regs_emit(v, area, lane, [&](int row, int cj, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+            const int col = c + cj;
+            if (row >= rows || col >= bn) return;
+            float* o = reinterpret_cast<float*>(out) + (row0 + row) * p.N + n0 + col;
+            if (q.vectors) {
+              store4(o, x0, x1, x2, x3);
+            } else {
+              o[0] = __uint_as_float(x0);
+              if (col + 1 < bn) o[1] = __uint_as_float(x1);
+              if (col + 2 < bn) o[2] = __uint_as_float(x2);
+              if (col + 3 < bn) o[3] = __uint_as_float(x3);
+            }
+          });
+        }
+      }
+      release();                                     // (warps whose share of the columns is empty)
+    }
+  }
+
+  // ---- common exit (see dense16_kernel) ----
+  tc_fence_before();
+  __syncthreads();
+  if (!PAIR) {
+    if (warp == kIssueWarp) tmem_release(tmem_base, 2u * acc_cols, smem_u32(&hdr->drain), abort_flag, p.status, lane);
+  } else {
+    uint32_t safe = 1u;
+    if (warp == kIssueWarp && *abort_flag) {
+      if (lane == 0) {
+        uint32_t ignore_abort = 0u;
+        p.status.tell_host();
+        umma2_commit(smem_u32(&hdr->drain));
+        safe = mbar_wait(smem_u32(&hdr->drain), 0u, &ignore_abort, nullptr) ? 1u : 0u;
+      }
+      safe = __shfl_sync(0xffffffffu, safe, 0);
+    }
+    cluster_sync_all();
+    if (warp == kIssueWarp && safe) {
+      tc_fence_after();
+      tmem_dealloc2(tmem_base, 2u * acc_cols);
+    }
+  }
+}
+
+size_t smem_before_ring(int E, uint32_t* table_bytes) {
+  *table_bytes = static_cast<uint32_t>((E + 1) * 4 + 15) & ~15u;
+  return (kRaggedHeader + 2u * *table_bytes + 1023u) & ~static_cast<size_t>(1023);
+}
+
+template <typename T, typename OutT, bool WEIGHTS, bool PAIR>
+cudaError_t launch_ragged(const RaggedParams& p, RaggedTiles q, long long most_units, const TensorMap3 (&maps)[4], cudaStream_t st) {
+  const size_t before = smem_before_ring(p.E, &q.table_bytes);
+  const size_t stage = kATile + b_tile_bytes(PAIR ? q.BN / 2 : q.BN);
+  const size_t fixed = before + kReadWarps * kReadArea;
+  q.stages = static_cast<int>((kRaggedSmem - fixed) / stage);
+  if (q.stages > kMaxStages) q.stages = kMaxStages;
+  cudaError_t err = ensure_smem_optin<ragged_kernel<T, OutT, WEIGHTS, PAIR>>(static_cast<int>(kRaggedSmem));
+  if (err != cudaSuccess) return err;
+  const long long workers = PAIR ? kSmCount / 2 : kSmCount;
+  const long long grid = (most_units < workers ? (most_units < 1 ? 1 : most_units) : workers) * (PAIR ? 2 : 1);
+  count_launch();
+  return launch_kernel(ragged_kernel<T, OutT, WEIGHTS, PAIR>, static_cast<unsigned>(grid), kRaggedThreads, fixed + q.stages * stage, st, true, p, q,
+                       maps[0], maps[1], maps[2], maps[3]);
+}
+
+// Maps of a matrix [rows, width] with a pitch: boxes of `box_rows` rows of 128 bytes, and four rows one by one.
+bool row_maps(TensorMap3* box, TensorMap3* four, const void* base, int elem, long long rows, int width, long long pitch, int box_rows) {
+  const unsigned long long dims[3] = {static_cast<unsigned long long>(width), static_cast<unsigned long long>(rows), 1ull};
+  const unsigned long long strides[2] = {static_cast<unsigned long long>(pitch) * elem, static_cast<unsigned long long>(pitch) * elem * rows};
+  const unsigned b3[3] = {static_cast<unsigned>(128 / elem), static_cast<unsigned>(box_rows), 1u}, b2[2] = {static_cast<unsigned>(128 / elem), 1u};
+  return encode_tensor_map_strided(box, base, elem, 3, dims, strides, b3) && encode_tensor_map_strided(four, base, elem, 2, dims, strides, b2);
+}
+
+template <typename T, typename OutT, bool WEIGHTS>
+cudaError_t launch_by_pair(const RaggedParams& p, const RaggedTiles& q, bool pair, long long units, const TensorMap3 (&maps)[4], cudaStream_t st) {
+  return pair ? launch_ragged<T, OutT, WEIGHTS, true>(p, q, units, maps, st) : launch_ragged<T, OutT, WEIGHTS, false>(p, q, units, maps, st);
+}
+
+// Pairs where the experts have 256 rows and more in the mean: their last tiles are half empty otherwise.
+bool wants_pair(const RaggedParams& p) { return p.N > 64 && p.rows >= 256ll * p.E; }
+
+}  // namespace
+
+cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st) {
+  const int elem = dtype == EGS_I8 ? 1 : 2;
+  const int out_elem = out_dtype == EGS_F32 ? 4 : 2;
+  RaggedTiles q{};
+  const bool pair = wants_pair(p);
+  q.BN = p.N > 128 ? 256 : p.N > 64 ? 128 : 64;
+  const int block = pair ? 256 : 128;
+  q.steps = (p.C * elem + 127) / 128;
+  q.tiles_n = (p.N + q.BN - 1) / q.BN;
+  q.by_n = Div(q.tiles_n);
+  q.gathers = p.slots != nullptr;
+  q.vectors = (static_cast<long long>(p.N) * out_elem) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
+  const long long blocks = p.offsets ? p.rows / block + (p.rows < p.E ? p.rows : p.E) : (p.rows + block - 1) / block;
+  const int columns = pair ? q.BN / 2 : q.BN;
+  TensorMap3 maps[4];
+  if (!row_maps(&maps[0], &maps[1], p.A, elem, p.a_rows, p.C, p.a_row, 128)) return cudaErrorInvalidValue;
+  const unsigned long long dims[3] = {static_cast<unsigned long long>(p.nc ? p.C : p.N), static_cast<unsigned long long>(p.nc ? p.N : p.C),
+                                      static_cast<unsigned long long>(p.E)};
+  const unsigned long long strides[2] = {static_cast<unsigned long long>(p.w_row) * elem, static_cast<unsigned long long>(p.w_expert) * elem};
+  const unsigned box[3] = {static_cast<unsigned>(128 / elem), p.nc ? static_cast<unsigned>(columns) : 64u, 1u};
+  if (!encode_tensor_map_strided(&maps[2], p.W, elem, 3, dims, strides, box)) return cudaErrorInvalidValue;
+  maps[3] = maps[2];
+  const long long units = blocks * q.tiles_n;
+  if (dtype == EGS_I8) {
+    if (out_dtype == EGS_F16) return launch_by_pair<int8_t, __half, false>(p, q, pair, units, maps, st);
+    if (out_dtype == EGS_BF16) return launch_by_pair<int8_t, __nv_bfloat16, false>(p, q, pair, units, maps, st);
+    return launch_by_pair<int8_t, float, false>(p, q, pair, units, maps, st);
+  }
+  if (dtype == EGS_F16) return launch_by_pair<__half, __half, false>(p, q, pair, units, maps, st);
+  return launch_by_pair<__nv_bfloat16, __nv_bfloat16, false>(p, q, pair, units, maps, st);
+}
+
+cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, cudaStream_t st) {
+  RaggedTiles q{};
+  const bool pair = wants_pair(p) && p.C > 128;
+  const int block = pair ? 256 : 128;
+  q.BN = p.N > 128 ? 256 : p.N > 64 ? 128 : 64;
+  q.tiles_n = (p.N + q.BN - 1) / q.BN;
+  q.tiles_c = (p.C + block - 1) / block;
+  q.by_n = Div(q.tiles_n);
+  q.by_c = Div(q.tiles_c);
+  q.units = p.E * q.tiles_c * q.tiles_n;
+  q.gathers = p.slots != nullptr;
+  q.vectors = (p.N * 2ll) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
+  TensorMap3 maps[4];
+  if (!row_maps(&maps[0], &maps[1], p.A, 2, p.a_rows, p.C, p.a_row, 64) || !row_maps(&maps[2], &maps[3], p.W, 2, p.rows, p.N, p.w_row, 64))
+    return cudaErrorInvalidValue;
+  if (dtype == EGS_F16) return launch_by_pair<__half, __half, true>(p, q, pair, q.units, maps, st);
+  return launch_by_pair<__nv_bfloat16, __nv_bfloat16, true>(p, q, pair, q.units, maps, st);
+}
+
+}  // namespace egs
