@@ -32,10 +32,14 @@ __device__ __forceinline__ float warp_max(float v) {
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 
 // ------------------------------------------------------------------------------------------------
-// Routing.  A warp has a token, lane l its experts l, l + 32, ...; every choice is a maximum over the lane's own keys, one over the
-// warp (redux on the ordered keys) and the lowest expert that has it.  Softmax and no bias: the logits' order is the scores', so the
-// logits are the keys, and a row's sum is only formed where something needs it.  Renormalised softmax weights are formed from the
-// chosen logits alone.
+// Routing.  A warp has a token, lane l its experts l, l + 32, ...  Softmax and no bias: the logits' order is the scores', so the logits
+// are the keys, and a row's sum is only formed where something needs it.  Renormalised softmax weights are formed from the chosen logits
+// alone.
+//
+// The top k: the k-th highest of the lanes' own maxima is a lower bound of the k-th highest key, and few keys lie at or above it
+// (256 random ones, k = 8: ten in the mean).  Those go through shared memory to one lane each, and a choice is a maximum over the warp
+// (redux) and the first lane that has it.  Where more than 32 keys lie above (many equal ones) every choice looks at all keys of all
+// lanes, as it always did at first: 45 instructions a choice with eight keys a lane instead of 6.
 // ------------------------------------------------------------------------------------------------
 constexpr int kRouteWarps = 8;
 
@@ -50,15 +54,23 @@ struct RouteParams {
   float scale;
   Div by_per;            // experts of a group
   int lanes_log2;        // lanes that look at a group together
+  int pitch;             // of a group's keys in shared memory
+  int warp_words;        // shared memory of a warp
 };
+
+__device__ __forceinline__ float unordered(uint32_t k) {         // (the float of ordered(); any NaN for its 1)
+  return k <= 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
 
 template <typename T, int NPER>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __grid_constant__ RouteParams p) {
-  extern __shared__ float group_values[];
+  extern __shared__ uint32_t route_smem[];
   pdl_wait();
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
   if (t >= p.tokens) return;
+  uint32_t* mem = route_smem + warp * p.warp_words;      // keys in groups, then candidates
   const T* row = static_cast<const T*>(p.logits) + t * p.stride;
   float x[NPER];
 #pragma unroll
@@ -81,59 +93,50 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
       if (i * 32 + lane < p.E) total += m == -INFINITY ? 0.f : expf(x[i] - m);
     total = warp_sum(total);
   }
-  auto score = [&](float v) { return p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total; };
+  // (keys are scores within a few units in the last place; the weights are formed with exact divisions below)
+  const float inverse = 1.f / total;
+  auto score = [&](float v) { return p.sigmoid ? __fdividef(1.f, 1.f + expf(-v)) : m == -INFINITY ? 0.f : expf(v - m) * inverse; };
   uint32_t key[NPER];
-  uint32_t kept = kFull;                       // groups
-  if (!need_scores) {
+  if (p.groups == 1) {
+    if (p.bias) {
 #pragma unroll
-    for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(x[i]) : 0u;
-  }
-  if (need_scores || p.groups > 1) {
-    float* values = group_values + warp * p.E;
+      for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(score(x[i]) + p.bias[i * 32 + lane]) : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(x[i]) : 0u;
+    }
+  } else {
+    int group[NPER];
 #pragma unroll
     for (int i = 0; i < NPER; ++i) {
       const int e = i * 32 + lane;
+      group[i] = p.by_per.quotient(e);
+      key[i] = 0u;
       if (e < p.E) {
-        float v = x[i];
-        if (p.bias) v = score(x[i]) + p.bias[e];
-        key[i] = ordered(v);
-        if (p.groups > 1) values[e] = pairs && !p.bias ? score(x[i]) : v;
-      } else {
-        key[i] = 0u;
+        key[i] = ordered(p.bias ? score(x[i]) + p.bias[e] : x[i]);
+        mem[group[i] * p.pitch + e - group[i] * p.per] = pairs && !p.bias ? ordered(score(x[i])) : key[i];
       }
     }
-  }
-  if (p.groups > 1) {
-    // the lanes of a group look at every 2^lanes_log2-th of its values and join what they found; group g's value ends up in lane g
-    float* values = group_values + warp * p.E;
+    // the lanes of a group look at every 2^lanes_log2-th of its keys and join what they found
     __syncwarp();
     const int lanes = 1 << p.lanes_log2, g = lane >> p.lanes_log2;
     uint32_t k1 = 0u, k2 = 0u;
-    float v1 = 0.f, v2 = 0.f;
-    auto take = [&](uint32_t kk, float v) {
-      if (kk > k1) {
-        k2 = k1; v2 = v1;
-        k1 = kk; v1 = v;
-      } else if (kk > k2) {
-        k2 = kk; v2 = v;
-      }
-    };
     if (g < p.groups)
       for (int i = lane & (lanes - 1); i < p.per; i += lanes) {
-        const float v = values[g * p.per + i];
-        take(ordered(v), v);
+        const uint32_t v = mem[g * p.pitch + i];
+        k2 = max(k2, min(k1, v));
+        k1 = max(k1, v);
       }
     for (int o = 1; o < lanes; o <<= 1) {
       const uint32_t o1 = __shfl_xor_sync(kFull, k1, o), o2 = __shfl_xor_sync(kFull, k2, o);
-      const float w1 = __shfl_xor_sync(kFull, v1, o), w2 = __shfl_xor_sync(kFull, v2, o);
-      take(o1, w1);
-      take(o2, w2);
+      k2 = max(min(k1, o1), max(k2, o2));
+      k1 = max(k1, o1);
     }
-    const float value = p.group_top == 2 && k2 ? v1 + v2 : v1;
-    uint32_t gk = g < p.groups ? ordered(value) : 0u;
-    gk = __shfl_sync(kFull, gk, (lane << p.lanes_log2) & 31);
+    uint32_t gk = k1;
+    if (pairs && k2) gk = ordered(unordered(k1) + unordered(k2));
+    gk = __shfl_sync(kFull, gk, (lane << p.lanes_log2) & 31);      // group g's value in lane g
     if (lane >= p.groups) gk = 0u;
-    kept = 0u;
+    uint32_t kept = 0u;
     for (int i = 0; i < p.top_groups; ++i) {
       const uint32_t best = __reduce_max_sync(kFull, gk);
       const int at = __ffs(__ballot_sync(kFull, gk == best)) - 1;
@@ -142,38 +145,80 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
     }
 #pragma unroll
     for (int i = 0; i < NPER; ++i)
-      if (!((kept >> (p.by_per.quotient(i * 32 + lane) & 31)) & 1u)) key[i] = 0u;
+      if (!((kept >> (group[i] & 31)) & 1u)) key[i] = 0u;
   }
-  int mine = 0;
-  for (int j = 0; j < p.k; ++j) {
-    uint32_t best = key[0];
+  // lower bound, candidates
+  uint32_t top = key[0];
 #pragma unroll
-    for (int i = 1; i < NPER; ++i) best = max(best, key[i]);
-    best = __reduce_max_sync(kFull, best);
-    uint32_t at = kFull;
-#pragma unroll
-    for (int i = NPER - 1; i >= 0; --i)
-      if (key[i] == best) at = i * 32 + lane;
-    at = __reduce_min_sync(kFull, at);
-#pragma unroll
-    for (int i = 0; i < NPER; ++i)
-      if (at == i * 32 + lane) key[i] = 0u;
-    if (lane == j) mine = static_cast<int>(at);
+  for (int i = 1; i < NPER; ++i) top = max(top, key[i]);
+  uint32_t bound = 0u;
+  for (int left = p.k; left > 0;) {
+    bound = __reduce_max_sync(kFull, top);
+    if (bound == 0u) break;
+    left -= __popc(__ballot_sync(kFull, top == bound));
+    if (top == bound) top = 0u;
   }
-  const bool chosen = lane < p.k;
+  bound = max(bound, 1u);
+  int found = 0;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < NPER; ++i) {
+    const unsigned who = __ballot_sync(kFull, key[i] >= bound);
+    if (key[i] >= bound) {
+      const int at = found + __popc(who & ((1u << lane) - 1u));
+      if (at < 32) {
+        mem[at] = key[i];
+        mem[32 + at] = i * 32 + lane;
+      }
+    }
+    found += __popc(who);
+  }
+  __syncwarp();
+  int mine = 0, place = p.k;                   // this lane's chosen expert and its place among them
+  if (found <= 32) {
+    uint32_t own = lane < found ? mem[lane] : 0u;
+    mine = lane < found ? static_cast<int>(mem[32 + lane]) : 0;
+    for (int j = 0; j < p.k; ++j) {
+      const uint32_t best = __reduce_max_sync(kFull, own);
+      if (lane == __ffs(__ballot_sync(kFull, own == best)) - 1) {
+        place = j;
+        own = 0u;
+      }
+    }
+  } else {
+    for (int j = 0; j < p.k; ++j) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < NPER; ++i) best = max(best, key[i]);
+      best = __reduce_max_sync(kFull, best);
+      uint32_t at = kFull;
+#pragma unroll
+      for (int i = NPER - 1; i >= 0; --i)
+        if (key[i] == best) at = i * 32 + lane;
+      at = __reduce_min_sync(kFull, at);
+#pragma unroll
+      for (int i = 0; i < NPER; ++i)
+        if (at == i * 32 + lane) key[i] = 0u;
+      if (lane == j) {
+        mine = static_cast<int>(at);
+        place = j;
+      }
+    }
+  }
+  const bool chosen = place < p.k;
   const float xc = chosen ? to_f32<T>(row[mine]) : -INFINITY;
   float w;
   if (p.renormalize) {
-    const float top = p.sigmoid ? 0.f : warp_max(xc);
-    const float s = !chosen ? 0.f : p.sigmoid ? sigmoid(xc) : top == -INFINITY ? 0.f : expf(xc - top);
+    const float best = p.sigmoid ? 0.f : warp_max(xc);
+    const float s = !chosen ? 0.f : p.sigmoid ? sigmoid(xc) : best == -INFINITY ? 0.f : expf(xc - best);
     const float sum = warp_sum(s);
     w = sum == 0.f ? 0.f : s / sum;
   } else {
-    w = score(xc);
+    w = p.sigmoid ? sigmoid(xc) : m == -INFINITY ? 0.f : expf(xc - m) / total;
   }
   if (chosen) {
-    p.weights[t * p.k + lane] = w * p.scale;
-    p.experts[t * p.k + lane] = mine;
+    p.weights[t * p.k + place] = w * p.scale;
+    p.experts[t * p.k + place] = mine;
   }
 }
 
@@ -255,27 +300,50 @@ struct PlanParams {
   int* offsets;      // [E + 1]
   int* slots;        // [n]
   int* position;     // [n]
-  int* counts;       // [stretches][E + 1], unused with one stretch
+  int* counts;       // [E + 1][stretches], unused with one stretch
   int n, E, part, stretches;      // part: slots of a warp, a multiple of 32; a stretch is kPlanWarps of them
   StatusRef status;
 };
 
+// A warp's slots: the first 128 of them (all, up to half a million slots) in registers, so that their loads are under way together and
+// are made once.
+constexpr int kPlanHeld = 4;
+struct PlanPart {
+  const int* ids;
+  long long first;
+  int n, lane, held[kPlanHeld];
+  __device__ __forceinline__ explicit PlanPart(const PlanParams& p) {
+    first = (static_cast<long long>(blockIdx.x) * kPlanWarps + (threadIdx.x >> 5)) * p.part;
+    n = static_cast<int>(max(0ll, min(static_cast<long long>(p.part), p.n - first)));
+    lane = threadIdx.x & 31;
+    ids = p.experts + first;
+#pragma unroll
+    for (int i = 0; i < kPlanHeld; ++i) held[i] = i * 32 + lane < n ? ids[i * 32 + lane] : -1;
+  }
+  // f(index of the warp's 32 slots, this lane's id) for all of them
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+    for (int i = 0; i < kPlanHeld; ++i)
+      if (i * 32 < n) f(i * 32, held[i]);
+    for (int i = kPlanHeld * 32; i < n; i += 32) f(i, i + lane < n ? ids[i + lane] : -1);
+  }
+};
+
 // smem: [kPlanWarps][E + 1] counts of the warps' parts
-__device__ __forceinline__ void count_parts(const PlanParams& p, int* table, bool report) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E1 = p.E + 1;
+__device__ __forceinline__ void count_parts(const PlanParams& p, const PlanPart& part, int* table, bool report) {
+  const int E1 = p.E + 1;
   for (int i = threadIdx.x; i < kPlanWarps * E1; i += kPlanThreads) table[i] = 0;
   __syncthreads();
-  int* mine = table + warp * E1;
-  const long long first = (static_cast<long long>(blockIdx.x) * kPlanWarps + warp) * p.part;
-  const int n = static_cast<int>(min(static_cast<long long>(p.part), p.n - first));
-  for (int i = lane; i < n; i += 32) {
-    int e = p.experts[first + i];
+  int* mine = table + (threadIdx.x >> 5) * E1;
+  part.each([&](int i, int e) {
+    if (i + part.lane >= part.n) return;
     if (e < 0 || e >= p.E) {
       if (e != -1 && report) p.status.report(EGS_STATUS_INDEX_OUT_OF_RANGE);
       e = p.E;
     }
     atomicAdd(mine + e, 1);
-  }
+  });
   __syncthreads();
 }
 
@@ -283,12 +351,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const __grid_c
   extern __shared__ int table[];
   pdl_wait();
   pdl_trigger();
-  count_parts(p, table, true);
+  const PlanPart part(p);
+  count_parts(p, part, table, true);
   const int E1 = p.E + 1;
   for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
     int sum = 0;
     for (int w = 0; w < kPlanWarps; ++w) sum += table[w * E1 + e];
-    p.counts[blockIdx.x * E1 + e] = sum;
+    p.counts[static_cast<long long>(e) * p.stretches + blockIdx.x] = sum;
   }
 }
 
@@ -299,24 +368,43 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E1 = p.E + 1;
   const bool one = p.stretches == 1;
-  count_parts(p, table, one);
-  // offsets of the experts (exclusive sums over all slots), a part of them at a time, and from them where each warp's slots begin
-  int carry = 0;
-  for (int e0 = 0; e0 < E1; e0 += kPlanThreads) {
-    const int e = e0 + threadIdx.x;
-    int before = 0, all = 0;                   // slots of e in the stretches before this one, in all of them
-    if (e < E1) {
-      if (one) {
-        for (int w = 0; w < kPlanWarps; ++w) all += table[w * E1 + e];
-      } else {
-        for (int s = 0; s < p.stretches; ++s) {
-          const int c = p.counts[s * E1 + e];
-          if (s < static_cast<int>(blockIdx.x)) before += c;
-          all += c;
-        }
+  const PlanPart part(p);
+  // slots of an expert in the stretches before this one, in all of them: a warp has an expert, a lane a stretch (one thread that went
+  // through 64 stretches of an expert took 6 us of the kernel's 12)
+  int* before = table + kPlanWarps * E1;
+  int* all = before + E1;
+  if (!one) {
+#pragma unroll 4
+    for (int e = warp; e < E1; e += kPlanWarps) {
+      int b = 0, a = 0;
+      for (int s = lane; s < p.stretches; s += 32) {
+        const int c = p.counts[static_cast<long long>(e) * p.stretches + s];
+        a += c;
+        if (s < static_cast<int>(blockIdx.x)) b += c;
+      }
+      a = __reduce_add_sync(kFull, a);
+      b = __reduce_add_sync(kFull, b);
+      if (lane == 0) {
+        before[e] = b;
+        all[e] = a;
       }
     }
-    int incl = all;
+  }
+  count_parts(p, part, table, one);
+  if (one) {
+    for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
+      int sum = 0;
+      for (int w = 0; w < kPlanWarps; ++w) sum += table[w * E1 + e];
+      before[e] = 0;
+      all[e] = sum;
+    }
+  }
+  __syncthreads();
+  // offsets of the experts, and from them where each warp's slots begin
+  int carry = 0;
+  for (int e0 = 0; e0 < E1; e0 += kPlanThreads) {
+    const int e = e0 + threadIdx.x, own = e < E1 ? all[e] : 0;
+    int incl = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(kFull, incl, o);
@@ -325,27 +413,29 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
     if (lane == 31) sums[warp] = incl;
     __syncthreads();
     int base = carry;
-    for (int w = 0; w < warp; ++w) base += sums[w];
-    for (int w = 0; w < kPlanWarps; ++w) carry += sums[w];
-    const int offset = base + incl - all;
+#pragma unroll
+    for (int w = 0; w < kPlanWarps; ++w) {
+      const int v = sums[w];
+      if (w < warp) base += v;
+      carry += v;
+    }
+    const int offset = base + incl - own;
     if (e < E1) {
       if (blockIdx.x == 0) p.offsets[e] = offset;
-      int at = offset + before;
+      int c[kPlanWarps], at = offset + before[e];
+#pragma unroll
+      for (int w = 0; w < kPlanWarps; ++w) c[w] = table[w * E1 + e];
+#pragma unroll
       for (int w = 0; w < kPlanWarps; ++w) {
-        const int c = table[w * E1 + e];
         table[w * E1 + e] = at;
-        at += c;
+        at += c[w];
       }
     }
     __syncthreads();
   }
   int* mine = table + warp * E1;
-  const long long first = (static_cast<long long>(blockIdx.x) * kPlanWarps + warp) * p.part;
-  const int n = static_cast<int>(min(static_cast<long long>(p.part), p.n - first));
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const int i = i0 + lane;
-    const bool on = i < n;
-    int e = on ? p.experts[first + i] : p.E;
+  part.each([&](int i0, int e) {
+    const bool on = i0 + lane < part.n;
     const bool real = e >= 0 && e < p.E;
     if (!real) e = p.E;
     const unsigned same = __match_any_sync(kFull, on ? e : -1);
@@ -355,16 +445,21 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
     if (on && rank == 0) mine[e] += __popc(same);
     __syncwarp();
     if (on) {
-      p.slots[at] = static_cast<int>(first + i);
-      p.position[first + i] = real ? at : ~at;
+      const long long slot = part.first + i0 + lane;
+      p.slots[at] = static_cast<int>(slot);
+      p.position[slot] = real ? at : ~at;
     }
-  }
+  });
 }
 
 // ------------------------------------------------------------------------------------------------
-// Weighted sum of a token's rows, float32 in the order of its choices, rounded once.  A thread has V columns of a token.
+// Weighted sum of a token's rows, float32 in the order of its choices, rounded once.
 // ------------------------------------------------------------------------------------------------
 template <typename T, int V> struct Vec;
+// A vector as it lies in memory: loads that wait for one another in this form take half the registers.
+template <typename T, int V> struct alignas(sizeof(T) * V) Packed {
+  T v[V];
+};
 template <typename T> struct Vec<T, 1> {
   static __device__ __forceinline__ void load(const T* p, float (&v)[1]) { v[0] = to_f32<T>(*p); }
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { *p = from_f32<T>(v[0]); }
@@ -399,45 +494,121 @@ struct CombineParams {
   void* out;               // token rows;  backward: dY, sorted rows
   const void* dOut;        // backward: token rows
   void* dweights;          // backward: [tokens, k]
-  int tokens, k, N, vecs;  // vecs: threads of a token (forward), lanes' worth of a row (backward)
+  int tokens, k, N, vecs;  // vecs: vectors of a row
   int w_f32;               // weights (and their gradient) in float32, else in the rows' type
-  Div by_vecs;
-  long long work;          // forward: tokens * vecs
+  Div by_blocks;           // forward: blocks of 32 vectors of a row
+  int work;                // forward: tokens * blocks
 };
 template <typename T>
 __device__ __forceinline__ float weight_of(const CombineParams& p, long long slot) {
   return !p.weights ? 1.f : p.w_f32 ? static_cast<const float*>(p.weights)[slot] : to_f32<T>(static_cast<const T*>(p.weights)[slot]);
 }
 
+// The rows lie anywhere, and what a thread may have in registers is not enough to keep the memory busy (eight loads a thread, 24 warps an
+// SM: 200 us for 131072 rows of 2048 bf16, 3.4 TB/s).  So vectors go to shared memory by cp.async, each to the thread that sums it: a warp
+// has 32 vectors of a token's columns at a time, four choices are a step, three steps are on their way, and positions are asked for a
+// step before that.
+constexpr int kCombineStages = 4, kCombineAhead = kCombineStages - 1, kCombineWarps = 4, kCombineCtas = 148 * 6;
+
 template <typename T, int V>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
+__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __grid_constant__ CombineParams p) {
+  using P = Packed<T, V>;
+  __shared__ P ring[kCombineStages][4][kCombineWarps * 32];
   pdl_wait();
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= p.work) return;
-  const long long t = i / p.vecs;
-  const int c = static_cast<int>(i - t * p.vecs) * V;
-  const T* Y = static_cast<const T*>(p.Y) + c;
-  const int* pos = p.position + t * p.k;
-  float sum[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) sum[v] = 0.f;
-  for (int j0 = 0; j0 < p.k; j0 += 4) {
-    int at[4];
-    float w[4], y[4][V];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      at[j] = j0 + j < p.k ? pos[j0 + j] : -1;
-      if (at[j] >= 0) Vec<T, V>::load(Y + static_cast<long long>(at[j]) * p.N, y[j]);
-      w[j] = at[j] >= 0 ? weight_of<T>(p, t * p.k + j0 + j) : 0.f;
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int first = blockIdx.x * kCombineWarps + (threadIdx.x >> 5), stride = gridDim.x * kCombineWarps;
+  const int items = p.work > first ? static_cast<int>((p.work - 1 - first) / stride) + 1 : 0;
+  const int groups = (p.k + 3) / 4;            // steps of an item
+  const T* Y = static_cast<const T*>(p.Y);
+  // a step further along: the token, its block of columns, the first of the four choices
+  struct Step {
+    int item, group;
+  };
+  auto next = [&](Step& s) {
+    if (++s.group == groups) {
+      s.group = 0;
+      ++s.item;
     }
+  };
+  auto place = [&](const Step& s, int* block) {
+    int i = first + s.item * stride;
+    *block = p.by_blocks.remainder(i);
+    return i;
+  };
+  Step ask{0, 0}, copy{0, 0}, use{0, 0};
+  auto position = [&]() {                      // of choice `lane` of the step asked for
+    int block, pos = -1;
+    if (ask.item < items && lane < 4 && ask.group * 4 + lane < p.k) pos = p.position[static_cast<long long>(place(ask, &block)) * p.k + ask.group * 4 + lane];
+    next(ask);
+    return pos;
+  };
+  auto weight = [&](const Step& s) {
+    int block;
+    if (s.item >= items || lane >= 4 || s.group * 4 + lane >= p.k) return 0.f;
+    return weight_of<T>(p, static_cast<long long>(place(s, &block)) * p.k + s.group * 4 + lane);
+  };
+  unsigned present[kCombineStages];            // choices of a stage that have a row
+  int pos = position();
+  auto fetch = [&](int stage) {
+    unsigned have = 0u;
+    if (copy.item < items) {
+      int block;
+      place(copy, &block);
+      const int c = (block * 32 + lane) * V;
+      have = __ballot_sync(kFull, pos >= 0) & 15u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (at[j] >= 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] = fmaf(w[j], y[j][v], sum[v]);
+      for (int j = 0; j < 4; ++j) {
+        const int at = __shfl_sync(kFull, pos, j);
+        if (at >= 0 && c < p.N) {
+          const P* src = reinterpret_cast<const P*>(Y + static_cast<long long>(at) * p.N + c);
+          if constexpr (sizeof(P) == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[stage][j][threadIdx.x]))), "l"(src) : "memory");
+          else
+            ring[stage][j][threadIdx.x] = *src;
+        }
       }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    next(copy);
+    pos = position();
+    return have;
+  };
+#pragma unroll
+  for (int i = 0; i < kCombineAhead; ++i) present[i] = fetch(i);
+  float w = weight(use), sum[V];
+  while (use.item < items) {
+#pragma unroll
+    for (int stage = 0; stage < kCombineStages; ++stage) {
+      if (use.item >= items) break;
+      present[(stage + kCombineAhead) % kCombineStages] = fetch((stage + kCombineAhead) % kCombineStages);
+      Step after = use;
+      next(after);
+      const float w_next = weight(after);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kCombineAhead) : "memory");
+      if (use.group == 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float wj = __shfl_sync(kFull, w, j);
+        if ((present[stage] >> j) & 1u) {
+          const P y = ring[stage][j][threadIdx.x];
+#pragma unroll
+          for (int v = 0; v < V; ++v) sum[v] = fmaf(wj, to_f32<T>(y.v[v]), sum[v]);
+        }
+      }
+      if (use.group == groups - 1) {
+        int block;
+        const long long t = place(use, &block);
+        const int c = (block * 32 + lane) * V;
+        if (c < p.N) Vec<T, V>::store(static_cast<T*>(p.out) + t * p.N + c, sum);
+      }
+      use = after;
+      w = w_next;
+    }
   }
-  Vec<T, V>::store(static_cast<T*>(p.out) + t * p.N + c, sum);
 }
 
 // A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
@@ -496,64 +667,79 @@ struct QuantizeParams {
 
 template <typename T, int V, int WARPS>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
-  constexpr int kKeep = 4;
-  __shared__ float found[4];
+  using P = Packed<T, V>;
+  constexpr int kKeep = V == 1 ? 16 : 8;
+  __shared__ uint32_t found[4];
   pdl_wait();
   pdl_trigger();
   constexpr int kRowThreads = WARPS * 32;
   const int r = threadIdx.x / kRowThreads, i0 = threadIdx.x % kRowThreads;
   const long long row = static_cast<long long>(blockIdx.x) * (128 / kRowThreads) + r;
   const bool on = row < p.rows;
-  const T* x = static_cast<const T*>(p.X) + row * p.x_stride;
+  const P* x = reinterpret_cast<const P*>(static_cast<const T*>(p.X) + row * p.x_stride);
   const int n = on ? p.C / V : 0;
-  float kept[kKeep][V];
+  P kept[kKeep];
   // the magnitudes' bit patterns have their order, and a NaN lies above infinity
   uint32_t top = 0u;
+  auto look = [&](const P& y) {
 #pragma unroll
-  for (int j = 0; j < kKeep; ++j) {
-    const int i = i0 + j * kRowThreads;
-    if (i < n) {
-      Vec<T, V>::load(x + static_cast<long long>(i) * V, kept[j]);
+    for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(to_f32<T>(y.v[v])) & 0x7fffffffu);
+  };
 #pragma unroll
-      for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(kept[j][v]) & 0x7fffffffu);
-    }
-  }
-  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) {
-    float y[V];
-    Vec<T, V>::load(x + static_cast<long long>(i) * V, y);
+  for (int j = 0; j < kKeep; ++j)
+    if (i0 + j * kRowThreads < n) kept[j] = x[i0 + j * kRowThreads];
 #pragma unroll
-    for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(y[v]) & 0x7fffffffu);
-  }
+  for (int j = 0; j < kKeep; ++j)
+    if (i0 + j * kRowThreads < n) look(kept[j]);
+  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) look(x[i]);
   top = __reduce_max_sync(kFull, top);
   if (WARPS > 1) {
-    if ((threadIdx.x & 31) == 0) found[threadIdx.x >> 5] = __uint_as_float(top);
+    if ((threadIdx.x & 31) == 0) found[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = max(top, __float_as_uint(found[w]));
+    for (int w = 0; w < WARPS; ++w) top = max(top, found[w]);
   }
   const bool finite = top < 0x7f800000u;
   const float scale = finite ? __uint_as_float(top) / 127.f : __uint_as_float(0x7fc00000u);
   const bool zeros = !finite || scale == 0.f;
   if (on && i0 == 0) p.scale[row] = scale;
+  // The nearest integer of x * (1 / scale), which is within 2^-15 of x / scale; where that comes near a half the division decides.  (With a
+  // division for each of 33 million elements the kernel took 44 us.)  kRound: a float32 whose unit is 1, so that adding it rounds and leaves the
+  // integer in the low bits.  Scales below 2^-126 have no reciprocal to work with.
+  constexpr float kRound = 12582912.f;
+  const float inverse = zeros ? 0.f : 1.f / scale;
+  const bool divide = !(inverse < 3e38f);
   int8_t* q = p.q + row * p.q_stride;
-  auto put = [&](int i, const float (&y)[V]) {
-    int8_t b[V];
+  auto put = [&](int i, const P& y) {
+    uint32_t b[V];
+    float far = 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) b[v] = zeros ? 0 : static_cast<int8_t>(max(-127, min(127, __float2int_rn(y[v] / scale))));
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(q + static_cast<long long>(i) * V) = *reinterpret_cast<const uint2*>(b);
-    else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(q + static_cast<long long>(i) * V) = *reinterpret_cast<const uint32_t*>(b);
-    else q[i] = b[0];
+    for (int v = 0; v < V; ++v) {
+      const float z = to_f32<T>(y.v[v]), t = fmaf(z, inverse, kRound);
+      far = fmaxf(far, fabsf(fmaf(z, inverse, kRound - t)));
+      b[v] = __float_as_uint(t);
+    }
+    if (zeros) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[v] = 0u;
+    } else if (divide || far > 0.4999f) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[v] = static_cast<uint32_t>(max(-127, min(127, __float2int_rn(to_f32<T>(y.v[v]) / scale))));
+    }
+    if constexpr (V >= 4) {
+      uint32_t w[V / 4];
+#pragma unroll
+      for (int v = 0; v < V / 4; ++v) w[v] = __byte_perm(__byte_perm(b[4 * v], b[4 * v + 1], 0x0040), __byte_perm(b[4 * v + 2], b[4 * v + 3], 0x0040), 0x5410);
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(q + static_cast<long long>(i) * V) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(q + static_cast<long long>(i) * V) = w[0];
+    } else {
+      q[i] = static_cast<int8_t>(b[0]);
+    }
   };
 #pragma unroll
-  for (int j = 0; j < kKeep; ++j) {
-    const int i = i0 + j * kRowThreads;
-    if (i < n) put(i, kept[j]);
-  }
-  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) {
-    float y[V];
-    Vec<T, V>::load(x + static_cast<long long>(i) * V, y);
-    put(i, y);
-  }
+  for (int j = 0; j < kKeep; ++j)
+    if (i0 + j * kRowThreads < n) put(i0 + j * kRowThreads, kept[j]);
+  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) put(i, x[i]);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -741,7 +927,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short* src
 
 template <typename T, int NPER>
 cudaError_t route_n(const RouteParams& p, cudaStream_t st) {
-  const size_t smem = p.groups > 1 ? sizeof(float) * kRouteWarps * p.E : 0;
+  const size_t smem = sizeof(uint32_t) * kRouteWarps * p.warp_words;
   return launch_kernel(route_tokens_kernel<T, NPER>, (p.tokens + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, smem, st, true, p);
 }
 template <typename T>
@@ -767,8 +953,11 @@ cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
     const long long slots = static_cast<long long>(p.tokens) * p.k;
     return launch_kernel(combine_backward_kernel<T, V>, static_cast<unsigned>((slots + 7) / 8), 256, 0, st, true, p);
   }
-  p.work = static_cast<long long>(p.tokens) * p.vecs;
-  return launch_kernel(combine_kernel<T, V>, static_cast<unsigned>((p.work + 255) / 256), 256, 0, st, true, p);
+  const int blocks = (p.vecs + 31) / 32;
+  p.by_blocks = Div(blocks);
+  p.work = p.tokens * blocks;
+  const int ctas = (p.work + kCombineWarps - 1) / kCombineWarps;
+  return launch_kernel(combine_kernel<T, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
 }
 template <typename T>
 cudaError_t combine_t(CombineParams& p, bool backward, cudaStream_t st) {
@@ -779,7 +968,7 @@ cudaError_t combine_t(CombineParams& p, bool backward, cudaStream_t st) {
 
 template <typename T, int V>
 cudaError_t quantize_v(const QuantizeParams& p, cudaStream_t st) {
-  if (p.C <= 32 * V * 4) return launch_kernel(quantize_rows_kernel<T, V, 1>, (p.rows + 3) / 4, 128, 0, st, true, p);
+  if (p.C <= 32 * V * (V == 1 ? 16 : 8)) return launch_kernel(quantize_rows_kernel<T, V, 1>, (p.rows + 3) / 4, 128, 0, st, true, p);
   return launch_kernel(quantize_rows_kernel<T, V, 4>, p.rows, 128, 0, st, true, p);
 }
 template <typename T>
@@ -800,6 +989,8 @@ cudaError_t launch_route_tokens(const void* logits, const float* bias, float* we
   p.group_top = r.group_top; p.per = r.E / r.groups; p.by_per = Div(p.per);
   p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
   while ((32 >> p.lanes_log2) > 1 && (32 >> (p.lanes_log2 + 1)) >= r.groups) ++p.lanes_log2;
+  p.pitch = p.per + (1 << p.lanes_log2);               // (groups of 32: all lanes in banks of their own)
+  p.warp_words = r.groups > 1 && r.groups * p.pitch > 64 ? r.groups * p.pitch : 64;
   count_launch();
   return by_type(dtype, [&] { return route_t<__half>(p, st); }, [&] { return route_t<__nv_bfloat16>(p, st); }, [&] { return route_t<float>(p, st); });
 }
@@ -833,11 +1024,11 @@ size_t plan_workspace_ints(long long n, int E) { return plan_stretches(n) == 1 ?
 cudaError_t launch_plan_experts(const int* experts, long long n, int E, int* offsets, int* slots, int* position, int* workspace,
                                 StatusRef status, cudaStream_t st) {
   PlanParams p{experts, offsets, slots, position, workspace, static_cast<int>(n), E, plan_part(n), static_cast<int>(plan_stretches(n)), status};
-  const size_t smem = sizeof(int) * kPlanWarps * (E + 1);
-  cudaError_t err = ensure_smem_optin<plan_place_kernel>(sizeof(int) * kPlanWarps * (EGS_MAX_EXPERTS + 1));
+  const size_t smem = sizeof(int) * (kPlanWarps + 2) * (E + 1);
+  cudaError_t err = ensure_smem_optin<plan_place_kernel>(sizeof(int) * (kPlanWarps + 2) * (EGS_MAX_EXPERTS + 1));
   if (err != cudaSuccess) return err;
   if (p.stretches > 1) {
-    err = ensure_smem_optin<plan_count_kernel>(sizeof(int) * kPlanWarps * (EGS_MAX_EXPERTS + 1));
+    err = ensure_smem_optin<plan_count_kernel>(sizeof(int) * (kPlanWarps + 2) * (EGS_MAX_EXPERTS + 1));
     if (err != cudaSuccess) return err;
     err = launch_kernel(plan_count_kernel, p.stretches, kPlanThreads, smem, st, true, p);
     count_launch();

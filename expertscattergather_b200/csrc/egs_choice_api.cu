@@ -173,6 +173,7 @@ int egs_combine(const void* Y, const void* weights, const int32_t* position, voi
   if (int rc = check_ragged(&d)) return rc;
   if (!valid_dtype(dtype) || (weights && weights_dtype != EGS_F32 && weights_dtype != dtype)) return EGS_ERR_INVALID_ARGUMENT;
   if (tokens == 0 || N == 0) return EGS_OK;
+  if (tokens * (N / 32 + 1) > kInt32Max) return EGS_ERR_TOO_LARGE;
   if (!out || (k > 0 && (!Y || !position))) return EGS_ERR_INVALID_ARGUMENT;
   return done(launch_combine(Y, weights, position, out, tokens, static_cast<int>(k), static_cast<int>(N), dtype, weights_dtype == EGS_F32,
                              stream_of(cuda_stream)),
