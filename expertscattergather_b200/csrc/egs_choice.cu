@@ -37,9 +37,11 @@ __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)
 // alone.
 //
 // The top k: the k-th highest of the lanes' own maxima is a lower bound of the k-th highest key, and few keys lie at or above it
-// (256 random ones, k = 8: ten in the mean).  Those go through shared memory to one lane each, and a choice is a maximum over the warp
-// (redux) and the first lane that has it.  Where more than 32 keys lie above (many equal ones) every choice looks at all keys of all
-// lanes, as it always did at first: 45 instructions a choice with eight keys a lane instead of 6.
+// (256 random ones, k = 8: ten in the mean).  Those go through shared memory to one lane each, which counts the candidates before its own.
+// Where more than 32 keys lie above (many equal ones) every choice is a maximum over all keys of all lanes: 45 instructions a choice with
+// eight keys a lane.
+//
+// What bounds it is instructions, half of them the scores'.
 // ------------------------------------------------------------------------------------------------
 constexpr int kRouteWarps = 8;
 
@@ -56,6 +58,7 @@ struct RouteParams {
   int lanes_log2;        // lanes that look at a group together
   int pitch;             // of a group's keys in shared memory
   int warp_words;        // shared memory of a warp
+  int slices;            // groups of that many whole slices of 32 experts; 0: others
 };
 
 __device__ __forceinline__ float unordered(uint32_t k) {         // (the float of ordered(); any NaN for its 1)
@@ -93,9 +96,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
       if (i * 32 + lane < p.E) total += m == -INFINITY ? 0.f : expf(x[i] - m);
     total = warp_sum(total);
   }
-  // (keys are scores within a few units in the last place; the weights are formed with exact divisions below)
-  const float inverse = 1.f / total;
-  auto score = [&](float v) { return p.sigmoid ? __fdividef(1.f, 1.f + expf(-v)) : m == -INFINITY ? 0.f : expf(v - m) * inverse; };
+  auto score = [&](float v) { return p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total; };
   uint32_t key[NPER];
   if (p.groups == 1) {
     if (p.bias) {
@@ -104,6 +105,50 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
     } else {
 #pragma unroll
       for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(x[i]) : 0u;
+    }
+  } else if (p.slices) {
+    // groups of whole slices of 32 experts: the two highest keys of each are maxima over the warp
+    uint32_t k1 = 0u, k2 = 0u, g1 = 0u, g2 = 0u;         // of this lane in the group, of group `lane`
+    int in_group = 0, g = 0;
+#pragma unroll
+    for (int i = 0; i < NPER; ++i) {
+      const int e = i * 32 + lane;
+      const bool on = e < p.E;
+      key[i] = on ? ordered(p.bias ? score(x[i]) + p.bias[e] : x[i]) : 0u;
+      const uint32_t v = on && pairs && !p.bias ? ordered(score(x[i])) : key[i];
+      k2 = max(k2, min(k1, v));
+      k1 = max(k1, v);
+      if (++in_group == p.slices) {
+        const uint32_t first = __reduce_max_sync(kFull, k1);
+        const unsigned who = __ballot_sync(kFull, k1 == first);
+        const uint32_t second = __reduce_max_sync(kFull, lane == __ffs(who) - 1 ? k2 : k1);
+        if (lane == g) {
+          g1 = first;
+          g2 = second;
+        }
+        k1 = k2 = 0u;
+        in_group = 0;
+        ++g;
+      }
+    }
+    uint32_t gk = g1;
+    if (pairs) gk = ordered(unordered(g1) + unordered(g2));
+    if (lane >= p.groups) gk = 0u;
+    uint32_t kept = 0u;
+    for (int i = 0; i < p.top_groups; ++i) {
+      const uint32_t best = __reduce_max_sync(kFull, gk);
+      const int at = __ffs(__ballot_sync(kFull, gk == best)) - 1;
+      kept |= 1u << at;
+      if (lane == at) gk = 0u;
+    }
+    in_group = 0;
+#pragma unroll
+    for (int i = 0; i < NPER; ++i) {
+      if (!(kept & 1u)) key[i] = 0u;
+      if (++in_group == p.slices) {
+        in_group = 0;
+        kept >>= 1;
+      }
     }
   } else {
     int group[NPER];
@@ -152,11 +197,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
 #pragma unroll
   for (int i = 1; i < NPER; ++i) top = max(top, key[i]);
   uint32_t bound = 0u;
-  for (int left = p.k; left > 0;) {
-    bound = __reduce_max_sync(kFull, top);
-    if (bound == 0u) break;
-    left -= __popc(__ballot_sync(kFull, top == bound));
-    if (top == bound) top = 0u;
+  for (int j = 0; j < p.k; ++j) {              // (equal maxima go together: the bound is then lower than it might be)
+    const uint32_t best = __reduce_max_sync(kFull, top);
+    bound = best;
+    if (best == 0u) break;
+    if (top == best) top = 0u;
   }
   bound = max(bound, 1u);
   int found = 0;
@@ -176,14 +221,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
   __syncwarp();
   int mine = 0, place = p.k;                   // this lane's chosen expert and its place among them
   if (found <= 32) {
-    uint32_t own = lane < found ? mem[lane] : 0u;
-    mine = lane < found ? static_cast<int>(mem[32 + lane]) : 0;
-    for (int j = 0; j < p.k; ++j) {
-      const uint32_t best = __reduce_max_sync(kFull, own);
-      if (lane == __ffs(__ballot_sync(kFull, own == best)) - 1) {
-        place = j;
-        own = 0u;
-      }
+    const uint32_t own = lane < found ? mem[lane] : 0u;
+    int before = 0;
+    for (int j = 0; j < found; ++j) {
+      const uint32_t other = mem[j];
+      before += (other > own || (other == own && j < lane)) ? 1 : 0;
+    }
+    if (lane < found) {
+      mine = static_cast<int>(mem[32 + lane]);
+      place = before;
     }
   } else {
     for (int j = 0; j < p.k; ++j) {
@@ -666,7 +712,7 @@ struct QuantizeParams {
 };
 
 template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
+__global__ void __launch_bounds__(128, 8) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
   using P = Packed<T, V>;
   constexpr int kKeep = V == 1 ? 16 : 8;
   __shared__ uint32_t found[4];
@@ -679,11 +725,16 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
   const P* x = reinterpret_cast<const P*>(static_cast<const T*>(p.X) + row * p.x_stride);
   const int n = on ? p.C / V : 0;
   P kept[kKeep];
-  // the magnitudes' bit patterns have their order, and a NaN lies above infinity
+  // the magnitudes' bit patterns have their order, and a NaN lies above infinity; 16-bit ones are compared in pairs
   uint32_t top = 0u;
   auto look = [&](const P& y) {
+    if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(to_f32<T>(y.v[v])) & 0x7fffffffu);
+      for (int v = 0; v < V / 2; ++v) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(&y)[v] & 0x7fff7fffu);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(to_f32<T>(y.v[v])) & 0x7fffffffu);
+    }
   };
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
@@ -692,6 +743,10 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
   for (int j = 0; j < kKeep; ++j)
     if (i0 + j * kRowThreads < n) look(kept[j]);
   for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) look(x[i]);
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    const unsigned short h = static_cast<unsigned short>(max(top & 0xffffu, top >> 16));
+    top = __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&h)));
+  }
   top = __reduce_max_sync(kFull, top);
   if (WARPS > 1) {
     if ((threadIdx.x & 31) == 0) found[threadIdx.x >> 5] = top;
@@ -703,28 +758,29 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
   const float scale = finite ? __uint_as_float(top) / 127.f : __uint_as_float(0x7fc00000u);
   const bool zeros = !finite || scale == 0.f;
   if (on && i0 == 0) p.scale[row] = scale;
-  // The nearest integer of x * (1 / scale), which is within 2^-15 of x / scale; where that comes near a half the division decides.  (With a
-  // division for each of 33 million elements the kernel took 44 us.)  kRound: a float32 whose unit is 1, so that adding it rounds and leaves the
-  // integer in the low bits.  Scales below 2^-126 have no reciprocal to work with.
+  // The nearest integers of x times a little less and a little more than 1 / scale: where they are one it is that of x / scale, else the
+  // division decides (one vector in 500; with a division for each of 33 million elements the kernel took 44 us).  kRound: a float32 whose
+  // unit is 1, so that adding it rounds to nearest even and leaves the integer in the low bits.  Scales below 2^-126 have no reciprocal to
+  // work with.
   constexpr float kRound = 12582912.f;
-  const float inverse = zeros ? 0.f : 1.f / scale;
-  const bool divide = !(inverse < 3e38f);
+  const float inverse = zeros ? 0.f : 1.f / scale, less = inverse * (1.f - 0x1p-20f), more = inverse * (1.f + 0x1p-20f);
+  const bool divide = !zeros && !(inverse < 1e38f);
   int8_t* q = p.q + row * p.q_stride;
   auto put = [&](int i, const P& y) {
-    uint32_t b[V];
-    float far = 0.f;
+    uint32_t b[V], apart = divide;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float z = to_f32<T>(y.v[v]), t = fmaf(z, inverse, kRound);
-      far = fmaxf(far, fabsf(fmaf(z, inverse, kRound - t)));
-      b[v] = __float_as_uint(t);
+      const float z = to_f32<T>(y.v[v]);
+      b[v] = __float_as_uint(fmaf(z, less, kRound));
+      apart |= b[v] ^ __float_as_uint(fmaf(z, more, kRound));
     }
-    if (zeros) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) b[v] = 0u;
-    } else if (divide || far > 0.4999f) {
+    if (apart) {
 #pragma unroll
       for (int v = 0; v < V; ++v) b[v] = static_cast<uint32_t>(max(-127, min(127, __float2int_rn(to_f32<T>(y.v[v]) / scale))));
+    }
+    if (!finite) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[v] = 0u;
     }
     if constexpr (V >= 4) {
       uint32_t w[V / 4];
@@ -990,7 +1046,8 @@ cudaError_t launch_route_tokens(const void* logits, const float* bias, float* we
   p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
   while ((32 >> p.lanes_log2) > 1 && (32 >> (p.lanes_log2 + 1)) >= r.groups) ++p.lanes_log2;
   p.pitch = p.per + (1 << p.lanes_log2);               // (groups of 32: all lanes in banks of their own)
-  p.warp_words = r.groups > 1 && r.groups * p.pitch > 64 ? r.groups * p.pitch : 64;
+  p.slices = r.groups > 1 && p.per % 32 == 0 ? p.per / 32 : 0;
+  p.warp_words = r.groups > 1 && !p.slices && r.groups * p.pitch > 64 ? r.groups * p.pitch : 64;
   count_launch();
   return by_type(dtype, [&] { return route_t<__half>(p, st); }, [&] { return route_t<__nv_bfloat16>(p, st); }, [&] { return route_t<float>(p, st); });
 }
