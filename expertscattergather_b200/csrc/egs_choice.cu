@@ -842,6 +842,19 @@ template <> __device__ __forceinline__ int widen<int8_t>(int8_t v) { return v; }
 __device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ int mac(int a, int b, int c) { return a * b + c; }
 
+// Four elements of a row from `p` on, `left` of which exist (p is not looked at where that is none); `wide`: they may be loaded together.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int left, bool wide, typename Acc<T>::type (&v)[4]) {
+  if (wide && left >= 4) {
+    const Packed<T, 4> x = *reinterpret_cast<const Packed<T, 4>*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = widen<T>(x.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? widen<T>(p[i]) : 0;
+  }
+}
+
 // Rows behind the last expert's: zeros.
 template <typename T>
 __device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int part, int parts) {
@@ -851,10 +864,27 @@ __device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int part, i
   for (long long i = begin + part; i < end; i += parts) out[i] = from_f32<T>(0.f);
 }
 
+// A step in shared memory, contraction by contraction; two of them, so that the next one is written while this one is read.
+template <typename A>
+struct alignas(16) GenericTile {
+  A a[2][kGStep][kGTile + 4], b[2][kGStep][kGTile + 4];
+};
+template <typename A>
+__device__ __forceinline__ void multiply(const GenericTile<A>& s, int buf, int tx, int ty, A (&acc)[4][4]) {
+#pragma unroll
+  for (int c = 0; c < kGStep; ++c) {
+    const Packed<A, 4> a = *reinterpret_cast<const Packed<A, 4>*>(&s.a[buf][c][ty * 4]), b = *reinterpret_cast<const Packed<A, 4>*>(&s.b[buf][c][tx * 4]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mac(a.v[i], b.v[j], acc[i][j]);
+  }
+}
+
 template <typename T, typename OutT>
 __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant__ RaggedParams p) {
   using A = typename Acc<T>::type;
-  __shared__ A As[kGStep][kGTile + 4], Bs[kGStep][kGTile + 4];
+  __shared__ GenericTile<A> s;
   __shared__ int s_expert, s_first, s_end;
   __shared__ int src[kGTile];
   pdl_wait();
@@ -871,41 +901,47 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant_
   const int e = s_expert, first = s_first, end = s_end;
   if (e < 0) return;
   if (tid < kGTile) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
-  const T* X = static_cast<const T*>(p.A);
+  __syncthreads();
   const T* W = static_cast<const T*>(p.W) + e * p.w_expert;
   const int n0 = blockIdx.y * kGTile, tx = tid & 15, ty = tid >> 4;
+  // of A (and of weights [E, N, C]): row tid / 4, elements 4 (tid mod 4) ..;  of weights [E, C, N]: row tid / 16
+  const int lr = tid >> 2, lc = (tid & 3) * 4, row = src[lr];
+  const T* a_row = static_cast<const T*>(p.A) + (row < 0 ? 0 : row) * p.a_row;
+  const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) % sizeof(Packed<T, 4>)) == 0;
+  const bool w_wide = p.w_row % 4 == 0 && p.w_expert % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) % sizeof(Packed<T, 4>)) == 0;
+  A va[4], vb[4];
+  auto fetch = [&](int c0) {
+    load4<T>(a_row + c0 + lc, row < 0 ? 0 : p.C - c0 - lc, a_wide, va);
+    if (p.nc) load4<T>(W + (n0 + lr) * p.w_row + c0 + lc, n0 + lr < p.N ? p.C - c0 - lc : 0, w_wide, vb);
+    else load4<T>(W + (c0 + ty) * p.w_row + n0 + tx * 4, c0 + ty < p.C ? p.N - n0 - tx * 4 : 0, w_wide, vb);
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.a[buf][lc + i][lr] = va[i];
+    if (p.nc) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.b[buf][lc + i][lr] = vb[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.b[buf][ty][tx * 4 + i] = vb[i];
+    }
+  };
   A acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0;
-  for (int c0 = 0; c0 < p.C; c0 += kGStep) {
+  if (p.C > 0) {
+    fetch(0);
+    put(0);
+  }
+  __syncthreads();
+  for (int c0 = 0, buf = 0; c0 < p.C; c0 += kGStep, buf ^= 1) {
+    const bool more = c0 + kGStep < p.C;
+    if (more) fetch(c0 + kGStep);
+    multiply(s, buf, tx, ty, acc);
+    if (more) put(buf ^ 1);
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = (tid >> 4) + 16 * i, c = c0 + (tid & 15);
-      As[tid & 15][m] = src[m] >= 0 && c < p.C ? widen<T>(X[src[m] * p.a_row + c]) : A(0);
-      if (p.nc) {
-        const int n = n0 + m;
-        Bs[tid & 15][m] = n < p.N && c < p.C ? widen<T>(W[n * p.w_row + c]) : A(0);
-      } else {
-        const int cc = c0 + (tid >> 6) + 4 * i, n = n0 + (tid & 63);
-        Bs[(tid >> 6) + 4 * i][tid & 63] = n < p.N && cc < p.C ? widen<T>(W[cc * p.w_row + n]) : A(0);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < kGStep; ++c) {
-      A a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = As[c][ty * 4 + i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = Bs[c][tx * 4 + j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mac(a[i], b[j], acc[i][j]);
-    }
   }
   OutT* out = static_cast<OutT*>(p.Out);
 #pragma unroll
@@ -923,48 +959,80 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant_
   }
 }
 
-// dW[e, c, n] = sum over the rows of e of X[row, c] dY[row, n]
+// dW[e, c, n] = sum over the rows of e of X[row, c] dY[row, n].  The rows of every expert are cut into `splits` ranges, whose sums (where
+// there are several) go to the workspace [E, splits, C, N] and are added in their order by a second kernel.
 template <typename T>
-__global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p) {
-  __shared__ float As[kGStep][kGTile + 4], Bs[kGStep][kGTile + 4];
+__global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p, int splits, float* partial) {
+  __shared__ GenericTile<float> s;
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int e = blockIdx.z, c0 = blockIdx.x * kGTile, n0 = blockIdx.y * kGTile;
-  const int first = p.offsets[e], end = p.offsets[e + 1];
+  const int e = blockIdx.z / splits, split = blockIdx.z - e * splits;
+  const int tiles_n = (p.N + kGTile - 1) / kGTile;
+  const int c0 = blockIdx.x / tiles_n * kGTile, n0 = blockIdx.x % tiles_n * kGTile;
+  int first = p.offsets[e], end = p.offsets[e + 1];
+  const int each = ((end - first + splits - 1) / splits + kGStep - 1) / kGStep * kGStep;
+  first = static_cast<int>(min(static_cast<long long>(end), first + static_cast<long long>(split) * each));
+  end = static_cast<int>(min(static_cast<long long>(end), first + static_cast<long long>(each)));
   const T* X = static_cast<const T*>(p.A);
   const T* Y = static_cast<const T*>(p.W);
-  float acc[4][4] = {};
-  for (int r0 = first; r0 < end; r0 += kGStep) {
-    __syncthreads();
+  const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) % sizeof(Packed<T, 4>)) == 0;
+  const bool w_wide = p.w_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) % sizeof(Packed<T, 4>)) == 0;
+  float va[4], vb[4];
+  int source = -1;                             // row of X in the step to come
+  auto look = [&](int r0) {
+    const int r = r0 + ty;
+    source = r >= end ? -1 : p.slots ? p.slots[r] : r;
+  };
+  auto fetch = [&](int r0) {
+    const long long row = source < 0 ? -1 : p.slots ? p.by_k.quotient(source) : source;
+    load4<T>(X + (row < 0 ? 0 : row) * p.a_row + c0 + tx * 4, row < 0 ? 0 : p.C - c0 - tx * 4, a_wide, va);
+    load4<T>(Y + (r0 + ty < end ? r0 + ty : 0) * p.w_row + n0 + tx * 4, r0 + ty < end ? p.N - n0 - tx * 4 : 0, w_wide, vb);
+    look(r0 + kGStep);
+  };
+  auto put = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = r0 + (tid >> 6) + 4 * i, f = tid & 63;
-      const long long row = r >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[r]) : r;
-      As[(tid >> 6) + 4 * i][f] = row >= 0 && c0 + f < p.C ? to_f32<T>(X[row * p.a_row + c0 + f]) : 0.f;
-      Bs[(tid >> 6) + 4 * i][f] = r < end && n0 + f < p.N ? to_f32<T>(Y[static_cast<long long>(r) * p.w_row + n0 + f]) : 0.f;
+      s.a[buf][ty][tx * 4 + i] = va[i];
+      s.b[buf][ty][tx * 4 + i] = vb[i];
     }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kGStep; ++r) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = As[r][ty * 4 + i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = Bs[r][tx * 4 + j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-    }
+  };
+  float acc[4][4] = {};
+  if (first < end) {
+    look(first);
+    fetch(first);
+    put(0);
   }
-  T* out = static_cast<T*>(p.Out) + static_cast<long long>(e) * p.C * p.N;
+  __syncthreads();
+  for (int r0 = first, buf = 0; r0 < end; r0 += kGStep, buf ^= 1) {
+    const bool more = r0 + kGStep < end;
+    if (more) fetch(r0 + kGStep);
+    multiply(s, buf, tx, ty, acc);
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  const long long size = static_cast<long long>(p.C) * p.N;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = c0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (c < p.C && n < p.N) out[static_cast<long long>(c) * p.N + n] = from_f32<T>(acc[i][j]);
+      if (c >= p.C || n >= p.N) continue;
+      const long long at = static_cast<long long>(c) * p.N + n;
+      if (splits > 1) partial[blockIdx.z * size + at] = acc[i][j];
+      else static_cast<T*>(p.Out)[e * size + at] = from_f32<T>(acc[i][j]);
     }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) dweight_join_kernel(const float* partial, T* out, long long size, int splits) {
+  pdl_wait();
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= size) return;
+  const float* p = partial + blockIdx.y * splits * size + i;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) sum += p[s * size];
+  out[blockIdx.y * size + i] = from_f32<T>(sum);
 }
 
 // Rows of 16-bit elements with another pitch; a thread writes eight elements.
@@ -1147,12 +1215,34 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
                  [&] { return go(ragged_rows_kernel<float, float>); });
 }
 
-cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, cudaStream_t st) {
-  const dim3 grid((p.C + kGTile - 1) / kGTile, (p.N + kGTile - 1) / kGTile, p.E);
-  count_launch();
-  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, 256, 0, st, true, p); };
-  return by_type(dtype, [&] { return go(ragged_dweight_kernel<__half>); }, [&] { return go(ragged_dweight_kernel<__nv_bfloat16>); },
-                 [&] { return go(ragged_dweight_kernel<float>); });
+// Ranges an expert's rows are cut into, so that there are four CTAs for an SM (at most 16 ranges, and none for short lists).
+static int dweight_splits(const RaggedParams& p) {
+  const long long tiles = static_cast<long long>((p.C + kGTile - 1) / kGTile) * ((p.N + kGTile - 1) / kGTile) * p.E;
+  const long long want = 4 * 148 / tiles, most = p.rows / (static_cast<long long>(p.E) * 4 * kGStep);
+  const long long n = want < most ? want : most;
+  return static_cast<int>(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+size_t generic_dweight_workspace(const RaggedParams& p) {
+  const int splits = dweight_splits(p);
+  return splits == 1 ? 0 : static_cast<size_t>(p.E) * splits * p.C * p.N * sizeof(float);
+}
+
+cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st) {
+  const int splits = dweight_splits(p);
+  float* partial = static_cast<float*>(workspace);
+  const long long tiles = static_cast<long long>((p.C + kGTile - 1) / kGTile) * ((p.N + kGTile - 1) / kGTile);
+  const dim3 grid(static_cast<unsigned>(tiles), 1, p.E * splits);
+  const long long size = static_cast<long long>(p.C) * p.N;
+  auto go = [&](auto kernel, auto join, auto* out) {
+    count_launch();
+    cudaError_t err = launch_kernel(kernel, grid, 256, 0, st, true, p, splits, partial);
+    if (err != cudaSuccess || splits == 1) return err;
+    count_launch();
+    return launch_kernel(join, dim3(static_cast<unsigned>((size + 255) / 256), p.E), 256, 0, st, true, partial, out, size, splits);
+  };
+  return by_type(dtype, [&] { return go(ragged_dweight_kernel<__half>, dweight_join_kernel<__half>, static_cast<__half*>(p.Out)); },
+                 [&] { return go(ragged_dweight_kernel<__nv_bfloat16>, dweight_join_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(p.Out)); },
+                 [&] { return go(ragged_dweight_kernel<float>, dweight_join_kernel<float>, static_cast<float*>(p.Out)); });
 }
 
 }  // namespace egs

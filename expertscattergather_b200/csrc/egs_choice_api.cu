@@ -48,7 +48,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // Tiles have 32-bit numbers.
 bool tiles_fit(const RaggedParams& p) {
   const double blocks = p.rows / 128.0 + p.E + 1, wide = p.N / 64.0 + 1, deep = p.C / 128.0 + 1;
-  return blocks * wide < 2e9 && p.E * deep * wide < 2e9;
+  return blocks * wide < 2e9 && (p.E + 1024) * deep * wide < 2e9 && p.rows < kInt32Max - (1 << 22);
 }
 
 // The tensor cores read 16-bit rows that begin on 16 bytes.  Others are copied: bytes of such a copy, 0 where none is needed.
@@ -137,8 +137,13 @@ int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, cons
 }
 
 size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype) {
-  if (dtype == EGS_F32 || check_ragged(dims) != EGS_OK || !valid_rows(rows)) return 0;
-  return copy_bytes(a_rows_of(*dims, rows), dims->C) + copy_bytes(dims->tokens * dims->k, dims->N);
+  if (!valid_dtype(dtype) || check_ragged(dims) != EGS_OK || !valid_rows(rows)) return 0;
+  if (dims->tokens * dims->k == 0 || dims->E * dims->C * dims->N == 0) return 0;
+  const RaggedParams p = ragged(*dims, rows);
+  const size_t generic = generic_dweight_workspace(p);
+  if (dtype == EGS_F32) return generic;
+  const size_t tensor = copy_bytes(a_rows_of(*dims, rows), dims->C) + copy_bytes(p.rows, dims->N) + ragged_dweight_workspace(p);
+  return tensor > generic ? tensor : generic;
 }
 
 int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, const int32_t* slots, void* dW, const egs_ragged* dims, int rows,
@@ -157,14 +162,14 @@ int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, co
   const cudaStream_t st = stream_of(cuda_stream);
   const bool able = device_is_sm100() && dtype != EGS_F32 && aligned16(X) && aligned16(dY) && tiles_fit(p);
   if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
-  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_dweight(p, dtype, st), "expert_dweight launch");
   const size_t need = egs_expert_dweight_workspace_bytes(dims, rows, dtype);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
+  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_dweight(p, dtype, workspace, st), "expert_dweight launch");
   char* ws = static_cast<char*>(workspace);
   cudaError_t err = copy_padded(&p.A, &p.a_row, p.a_rows, p.C, &ws, st);
   if (err == cudaSuccess) err = copy_padded(&p.W, &p.w_row, p.rows, p.N, &ws, st);
   if (err != cudaSuccess) return fail_cuda(err, "expert_dweight copies");
-  return done(launch_ragged_dweight_tensor(p, dtype, st), "expert_dweight launch");
+  return done(launch_ragged_dweight_tensor(p, dtype, ws, st), "expert_dweight launch");
 }
 
 int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,

@@ -267,10 +267,12 @@ cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long lo
                                  cudaStream_t st);
 // dtype EGS_I8: 8-bit operands with scales, products in out_dtype
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
-cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, cudaStream_t st);
+cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
+size_t generic_dweight_workspace(const RaggedParams& p);
 // ... on the tensor cores (egs_ragged.cu): 16-bit or 8-bit operands whose rows begin on 16 bytes, C and N at least 1
 cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
-cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, cudaStream_t st);
+cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
+size_t ragged_dweight_workspace(const RaggedParams& p);
 // Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; what lies behind a row's end is not defined).
 cudaError_t launch_pad_rows(const void* src, void* dst, long long rows, int width, int pitch, cudaStream_t st);
 

@@ -13,6 +13,12 @@
 //   warp  5       tensor-memory allocation; four tcgen05.mma a stage, issued by the leader of a pair for both CTAs
 //   warps 8..15   read-out: tensor memory -> (scales) -> rows of the output; zeros for rows that belong to no expert
 //
+// Experts differ in size, and a weight gradient's tile takes as long as its expert has rows.  So the contraction of a large expert is cut
+// into ranges of at most `range_steps` steps, about half of a CTA's share of all steps; tiles go out largest range first, every second
+// round of the CTAs backwards.  Ranges of a cut expert leave float32 sums in the workspace, which a second kernel adds in the order of
+// the rows: the same bits in every run.  64 experts of 100 to 5000 rows, 1024 x 256 features: tiles in the experts' order, uncut, kept the
+// tensor cores of one pair busy for 61 % of 106 us and those of another for 4 %.
+//
 // Rows of a tile that belong to the next expert are computed and not stored.  In a contraction over rows they would do harm, even where
 // the other operand is 0 (0 * infinity), so the last step of an expert takes the rows behind its end from outside the tensor: zeros.
 #include <type_traits>
@@ -40,14 +46,17 @@ struct __align__(16) RaggedHeader {
   unsigned long long drain;
   uint32_t tmem_base;
   uint32_t abort_flag;
-  int warp_sums[kRaggedThreads / 32];
+  int warp_sums[2 * kRaggedThreads / 32];
+  int ranges;
 };
 static_assert(sizeof(RaggedHeader) <= kRaggedHeader, "header does not fit");
 
 struct RaggedTiles {
   int BN, stages, steps;       // steps: of `rows`
   int tiles_n, tiles_c;        // column tiles; `weights`: tiles over X's features
-  int units;                   // `weights`: all of them
+  int range_steps;             // `weights`: steps of a range at most
+  int most_ranges;             // ... and how many there can be
+  float* partial;              // ... sums of the ranges of cut experts [range, C, N]
   int gathers;                 // X's rows are gathered
   int vectors;                 // rows of the output begin on 16 bytes and are whole 16 bytes
   uint32_t table_bytes;        // of each of the two tables
@@ -114,6 +123,59 @@ __device__ __forceinline__ int expert_of(const int* starts, int E, int block, in
   return lo;
 }
 
+// The row ranges of a weight gradient, in shared memory.
+struct Ranges {
+  int* first;       // rows [first, end)
+  int* end;
+  int* expert;
+  int* partial;     // place among the ranges of cut experts, -1 where the expert is not cut
+  int* order;       // ranges by descending size
+};
+__host__ __device__ constexpr uint32_t range_bytes(int most) { return static_cast<uint32_t>(5 * most * 4 + 15) & ~15u; }
+__device__ __forceinline__ Ranges ranges_at(unsigned char* mem, int most) {
+  int* p = reinterpret_cast<int*>(mem);
+  return {p, p + most, p + 2 * most, p + 3 * most, p + 4 * most};
+}
+constexpr int kStepRows = 64;        // contraction rows of a step of a weight gradient
+__host__ __device__ inline int steps_of(int rows) { return (rows + kStepRows - 1) / kStepRows; }
+// Ranges of an expert with that many rows.
+__device__ __forceinline__ int ranges_of(int rows, int range_steps) {
+  const int steps = steps_of(rows);
+  return steps <= range_steps ? 1 : (steps + range_steps - 1) / range_steps;
+}
+
+// Exclusive sums of `a` and `b` over the threads of the CTA, and the totals; `sums`: an int a warp and quantity.
+__device__ __forceinline__ void scan_two(int& a, int& b, int& total_a, int& total_b, int* sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kRaggedThreads / 32;
+  const int own_a = a, own_b = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int va = __shfl_up_sync(0xffffffffu, a, o), vb = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a += va;
+      b += vb;
+    }
+  }
+  if (lane == 31) {
+    sums[warp] = a;
+    sums[warps + warp] = b;
+  }
+  __syncthreads();
+  total_a = total_b = 0;
+  int before_a = 0, before_b = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) {
+      before_a += sums[w];
+      before_b += sums[warps + w];
+    }
+    total_a += sums[w];
+    total_b += sums[warps + w];
+  }
+  a += before_a - own_a;
+  b += before_b - own_b;
+  __syncthreads();
+}
+
 template <typename OutT>
 __device__ __forceinline__ uint32_t pack_out(uint32_t a, uint32_t b) { return pack2(static_cast<OutT*>(nullptr), a, b); }
 
@@ -125,13 +187,13 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
   constexpr bool kInt8 = sizeof(T) == 1;
   constexpr int kBlock = PAIR ? 256 : 128;           // rows of a tile
   constexpr int kStepElems = 128 / sizeof(T);        // `rows`
-  constexpr int kStepRows = 64;                      // `weights`
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   RaggedHeader* hdr = reinterpret_cast<RaggedHeader*>(smem_raw);
   int* offsets = reinterpret_cast<int*>(smem_raw + kRaggedHeader);
   int* starts = reinterpret_cast<int*>(smem_raw + kRaggedHeader + q.table_bytes);      // row blocks before each expert's
   const uint32_t smem0 = smem_u32(smem_raw);
-  const uint32_t ring0 = (smem0 + kRaggedHeader + 2u * q.table_bytes + 1023u) & ~1023u;
+  const Ranges range = ranges_at(smem_raw + kRaggedHeader + q.table_bytes, q.most_ranges);
+  const uint32_t ring0 = (smem0 + kRaggedHeader + q.table_bytes + (WEIGHTS ? range_bytes(q.most_ranges) : q.table_bytes) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
   const bool leader = rank == 0;
@@ -177,27 +239,43 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
       tmem_relinquish();
     }
   }
-  if (!WEIGHTS) {
-    int carry = 0;
+  {
+    int carry = 0, carry_cut = 0;                    // blocks (ranges), ranges of cut experts
     for (int e0 = 0; e0 < p.E; e0 += kRaggedThreads) {
-      const int e = e0 + tid;
-      int incl = e < p.E ? (offsets[e + 1] - offsets[e] + kBlock - 1) / kBlock : 0;
-      const int own = incl;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+      const int e = e0 + tid, rows = e < p.E ? offsets[e + 1] - offsets[e] : 0;
+      const int own = e >= p.E ? 0 : WEIGHTS ? ranges_of(rows, q.range_steps) : (rows + kBlock - 1) / kBlock;
+      int at = own, cut = WEIGHTS && own > 1 ? own : 0, total, total_cut;
+      scan_two(at, cut, total, total_cut, hdr->warp_sums);
+      at += carry;
+      cut += carry_cut;
+      carry += total;
+      carry_cut += total_cut;
+      if constexpr (!WEIGHTS) {
+        if (e < p.E) starts[e] = at;
+        if (e == p.E - 1) starts[p.E] = carry;
+      } else {
+        const int steps = steps_of(rows), each = own ? (steps + own - 1) / own * kStepRows : 0;
+        for (int i = 0; i < own; ++i) {
+          range.first[at + i] = min(offsets[e] + i * each, offsets[e + 1]);
+          range.end[at + i] = min(offsets[e] + (i + 1) * each, offsets[e + 1]);
+          range.expert[at + i] = e;
+          range.partial[at + i] = own > 1 ? cut + i : -1;
+        }
+        if (tid == 0) hdr->ranges = carry;
       }
-      if (lane == 31) hdr->warp_sums[warp] = incl;
+    }
+    if constexpr (WEIGHTS) {
       __syncthreads();
-      int before = carry;
-      for (int w = 0; w < kRaggedThreads / 32; ++w) {
-        if (w < warp) before += hdr->warp_sums[w];
-        carry += hdr->warp_sums[w];
+      const int n = hdr->ranges;
+      for (int i = tid; i < n; i += kRaggedThreads) {
+        const int size = range.end[i] - range.first[i];
+        int before = 0;
+        for (int j = 0; j < n; ++j) {
+          const int other = range.end[j] - range.first[j];
+          before += other > size || (other == size && j < i) ? 1 : 0;
+        }
+        range.order[before] = i;
       }
-      if (e < p.E) starts[e] = before + incl - own;
-      if (e == p.E - 1) starts[p.E] = before + incl;
-      __syncthreads();
     }
   }
   tc_fence_before();
@@ -205,8 +283,10 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
   if (PAIR) cluster_sync_all();                      // both CTAs' barriers are initialised before anything crosses the pair
   tc_fence_after();
   const uint32_t tmem_base = hdr->tmem_base;
-  const int units = WEIGHTS ? q.units : starts[p.E] * q.tiles_n;
+  const int units = WEIGHTS ? hdr->ranges * q.tiles_n * q.tiles_c : starts[p.E] * q.tiles_n;
   const uint32_t full0 = PAIR ? map_to_cta(smem_u32(&hdr->full[0]), 0) : smem_u32(&hdr->full[0]);
+  // tile `round` of this CTA or pair
+  auto unit_of = [&](int round) { return round * unit_stride + (WEIGHTS && (round & 1) ? unit_stride - 1 - first_unit : first_unit); };
   RingCursor at;
   bool alive = true;
   auto wait_free = [&]() {
@@ -221,7 +301,7 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
     if (q.gathers) {
       if constexpr (!WEIGHTS) {
         int e = 0;
-        for (int u = first_unit; u < units && alive; u += unit_stride) {
+        for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
           const int block = q.by_n.quotient(u);
           e = expert_of(starts, p.E, block, e);
           const int r = offsets[e] + (block - starts[e]) * kBlock + rank * 128 + warp * 32 + lane;
@@ -245,15 +325,15 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
         }
       } else {
         // a warp has 16 rows of every step; lanes 16..31 look up those of the step behind
-        for (int u = first_unit; u < units && alive; u += unit_stride) {
+        for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
           int x = q.by_n.quotient(u);
-          const int c = q.by_c.remainder(x), e = x;
-          const int begin = offsets[e], end = offsets[e + 1];
+          const int c = q.by_c.remainder(x), i = range.order[x];
+          const int begin = range.first[i], end = range.end[i];
           auto look = [&](int step) {                // (an even one)
             const int r = begin + (step + (lane >> 4)) * kStepRows + warp * 16 + (lane & 15);
             return r < end ? p.slots[r] : -1;
           };
-          const int steps = (end - begin + kStepRows - 1) / kStepRows;
+          const int steps = steps_of(end - begin);
           const int f0 = c * kBlock + rank * 128;
           int coming = steps ? look(0) : -1, now = -1;
           for (int ks = 0; ks < steps; ++ks) {
@@ -286,7 +366,7 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
     // =========================== boxes ===========================
     const uint32_t bytes = PAIR ? 2u * stage_bytes : stage_bytes;       // announced by the leader for both CTAs
     int e = 0;
-    for (int u = first_unit; u < units && alive; u += unit_stride) {
+    for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
       const int x = q.by_n.quotient(u);
       const int n0 = (u - x * q.tiles_n) * q.BN + rank * columns;
       int steps = q.steps, a0 = 0, f0 = 0, begin = 0, end = 0;
@@ -296,10 +376,10 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
       } else {
         int y = x;
         f0 = q.by_c.remainder(y) * kBlock + rank * 128;
-        e = y;
-        begin = offsets[e];
-        end = offsets[e + 1];
-        steps = (end - begin + kStepRows - 1) / kStepRows;
+        y = range.order[y];
+        begin = range.first[y];
+        end = range.end[y];
+        steps = steps_of(end - begin);
       }
       for (int ks = 0; ks < steps; ++ks) {
         if (!wait_free()) break;
@@ -348,12 +428,12 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
                                    : make_idesc(sizeof(T) == 2 ? Elem<typename std::conditional<kInt8, __half, T>::type>::fmt : 0u, WEIGHTS ? 1u : 0u,
                                                 b_mn ? 1u : 0u, kBlock, q.BN);
       int t = 0;                                     // tiles with an accumulator
-      for (int u = first_unit; u < units && alive; u += unit_stride) {
+      for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
         int steps = q.steps;
         if constexpr (WEIGHTS) {
           int x = q.by_n.quotient(u);
-          x = q.by_c.quotient(x);
-          steps = (offsets[x + 1] - offsets[x] + kStepRows - 1) / kStepRows;
+          x = range.order[q.by_c.quotient(x)];
+          steps = steps_of(range.end[x] - range.first[x]);
           if (steps == 0) continue;
         }
         const int buf = t & 1;
@@ -393,11 +473,12 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
       for (long long i = begin + blockIdx.x * (kReadWarps * 32) + ew * 32 + lane; i < end; i += step) out[i] = from_f32<OutT>(0.f);
     }
     int e = 0, t = 0;
-    for (int u = first_unit; u < units && alive; u += unit_stride) {
+    for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
       const int x = q.by_n.quotient(u);
       const int n0 = (u - x * q.tiles_n) * q.BN, bn = min(q.BN, p.N - n0);
       long long row0;                                // output row of the warp's first accumulator row
       int rows;                                      // of its 32 that are stored
+      int partial = -1;
       bool have = true;
       float scale = 0.f;
       if constexpr (!WEIGHTS) {
@@ -411,10 +492,11 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
       } else {
         int y = x;
         const int f = q.by_c.remainder(y) * kBlock + rank * 128 + lg * 32;
-        e = y;
-        row0 = static_cast<long long>(e) * p.C + f;
+        y = range.order[y];
+        partial = range.partial[y];
+        row0 = static_cast<long long>(partial >= 0 ? partial : range.expert[y]) * p.C + f;
         rows = min(32, p.C - f);
-        have = offsets[e + 1] > offsets[e];
+        have = range.end[y] > range.first[y];
       }
       const int buf = t & 1;
       if (have) {
@@ -453,7 +535,29 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
           }
         }
       };
-      if constexpr (sizeof(OutT) == 2) {
+      auto store_f32 = [&](float* to, bool vectors) {
+        for (int c = share * 32; c < bn; c += 64) {
+          uint32_t v[32];
+          read(c, v);
+          if (c + 64 >= bn) release();
+          warp_regs_emit(v, area, lane, [&](int row, int cj, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+            const int col = c + cj;
+            if (row >= rows || col >= bn) return;
+            float* o = to + (row0 + row) * p.N + n0 + col;
+            if (vectors) {
+              store4(o, x0, x1, x2, x3);
+            } else {
+              o[0] = __uint_as_float(x0);
+              if (col + 1 < bn) o[1] = __uint_as_float(x1);
+              if (col + 2 < bn) o[2] = __uint_as_float(x2);
+              if (col + 3 < bn) o[3] = __uint_as_float(x3);
+            }
+          });
+        }
+      };
+      if (WEIGHTS && partial >= 0) {
+        store_f32(q.partial, p.N % 4 == 0);
+      } else if constexpr (sizeof(OutT) == 2) {
         // 64 columns = 128 bytes of a row at a time, eight lanes to a row
         for (int c = share * 64; c < bn; c += 128) {
           const uint32_t srow = area + static_cast<uint32_t>(lane) * 128u;
@@ -501,24 +605,7 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
           __syncwarp();
         }
       } else {
-        for (int c = share * 32; c < bn; c += 64) {
-          uint32_t v[32];
-          read(c, v);
-          if (c + 64 >= bn) release();
-          warp_regs_emit(v, area, lane, [&](int row, int cj, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
-            const int col = c + cj;
-            if (row >= rows || col >= bn) return;
-            float* o = reinterpret_cast<float*>(out) + (row0 + row) * p.N + n0 + col;
-            if (q.vectors) {
-              store4(o, x0, x1, x2, x3);
-            } else {
-              o[0] = __uint_as_float(x0);
-              if (col + 1 < bn) o[1] = __uint_as_float(x1);
-              if (col + 2 < bn) o[2] = __uint_as_float(x2);
-              if (col + 3 < bn) o[3] = __uint_as_float(x3);
-            }
-          });
-        }
+        store_f32(reinterpret_cast<float*>(out), q.vectors);
       }
       release();                                     // (warps whose share of the columns is empty)
     }
@@ -548,14 +635,48 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
   }
 }
 
-size_t smem_before_ring(int E, uint32_t* table_bytes) {
-  *table_bytes = static_cast<uint32_t>((E + 1) * 4 + 15) & ~15u;
-  return (kRaggedHeader + 2u * *table_bytes + 1023u) & ~static_cast<size_t>(1023);
+// dW of cut experts: the sums of their ranges, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) ragged_join_kernel(const int* offsets, const float* partial, T* out, long long size, int E, int range_steps) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  long long base = 0;
+  int turn = 0;                                // every gridDim.y-th cut expert is this CTA's
+  for (int e0 = 0; e0 < E; e0 += 32) {         // a lane looks at an expert
+    const int own = e0 + lane < E ? ranges_of(offsets[e0 + lane + 1] - offsets[e0 + lane], range_steps) : 1;
+    for (unsigned cut = __ballot_sync(0xffffffffu, own > 1); cut; cut &= cut - 1) {
+      const int n = __shfl_sync(0xffffffffu, own, __ffs(cut) - 1);
+      const float* p = partial + base * size;
+      base += n;
+      if (turn++ % gridDim.y != blockIdx.y) continue;
+      T* o = out + (e0 + __ffs(cut) - 1) * size;
+      if (size % 4 == 0) {
+        for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4; i < size; i += static_cast<long long>(gridDim.x) * 1024) {
+          float4 sum = *reinterpret_cast<const float4*>(p + i);
+#pragma unroll 4
+          for (int r = 1; r < n; ++r) {
+            const float4 x = *reinterpret_cast<const float4*>(p + r * size + i);
+            sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+          }
+          store4(o + i, __float_as_uint(sum.x), __float_as_uint(sum.y), __float_as_uint(sum.z), __float_as_uint(sum.w));
+        }
+      } else {
+        for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<long long>(gridDim.x) * 256) {
+          float sum = p[i];
+#pragma unroll 4
+          for (int r = 1; r < n; ++r) sum += p[r * size + i];
+          o[i] = from_f32<T>(sum);
+        }
+      }
+    }
+  }
 }
 
 template <typename T, typename OutT, bool WEIGHTS, bool PAIR>
 cudaError_t launch_ragged(const RaggedParams& p, RaggedTiles q, long long most_units, const TensorMap3 (&maps)[4], cudaStream_t st) {
-  const size_t before = smem_before_ring(p.E, &q.table_bytes);
+  q.table_bytes = static_cast<uint32_t>((p.E + 1) * 4 + 15) & ~15u;
+  const size_t before = (kRaggedHeader + q.table_bytes + (WEIGHTS ? range_bytes(q.most_ranges) : q.table_bytes) + 1023u) & ~static_cast<size_t>(1023);
   const size_t stage = kATile + b_tile_bytes(PAIR ? q.BN / 2 : q.BN);
   const size_t fixed = before + kReadWarps * kReadArea;
   q.stages = static_cast<int>((kRaggedSmem - fixed) / stage);
@@ -619,23 +740,52 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
   return launch_by_pair<__nv_bfloat16, __nv_bfloat16, false>(p, q, pair, units, maps, st);
 }
 
-cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, cudaStream_t st) {
-  RaggedTiles q{};
-  const bool pair = wants_pair(p) && p.C > 128;
-  const int block = pair ? 256 : 128;
+// (a range below this takes less time than the kernel that joins ranges)
+constexpr int kLeastRange = 24;
+
+// How a weight gradient is cut: see the top of the file.  Ranges of cut experts have more than half of range_steps steps each.
+struct DweightPlan {
+  bool pair;
+  RaggedTiles q;
+  long long most_partial;
+};
+static DweightPlan dweight_plan(const RaggedParams& p) {
+  DweightPlan d{};
+  RaggedTiles& q = d.q;
+  d.pair = wants_pair(p) && p.C > 128;
+  const int block = d.pair ? 256 : 128, workers = d.pair ? kSmCount / 2 : kSmCount;
   q.BN = p.N > 128 ? 256 : p.N > 64 ? 128 : 64;
   q.tiles_n = (p.N + q.BN - 1) / q.BN;
   q.tiles_c = (p.C + block - 1) / block;
+  const long long steps = steps_of(p.rows), share = steps * q.tiles_n * q.tiles_c / workers;
+  q.range_steps = static_cast<int>(share / 2 < kLeastRange ? kLeastRange : share / 2);
+  d.most_partial = steps <= q.range_steps ? 0 : 2 * (steps / q.range_steps) + 2;
+  q.most_ranges = static_cast<int>(p.E + d.most_partial);
+  return d;
+}
+size_t ragged_dweight_workspace(const RaggedParams& p) { return static_cast<size_t>(dweight_plan(p).most_partial) * p.C * p.N * sizeof(float); }
+
+cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st) {
+  DweightPlan d = dweight_plan(p);
+  RaggedTiles& q = d.q;
   q.by_n = Div(q.tiles_n);
   q.by_c = Div(q.tiles_c);
-  q.units = p.E * q.tiles_c * q.tiles_n;
+  q.partial = static_cast<float*>(workspace);
   q.gathers = p.slots != nullptr;
   q.vectors = (p.N * 2ll) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
   TensorMap3 maps[4];
   if (!row_maps(&maps[0], &maps[1], p.A, 2, p.a_rows, p.C, p.a_row, 64) || !row_maps(&maps[2], &maps[3], p.W, 2, p.rows, p.N, p.w_row, 64))
     return cudaErrorInvalidValue;
-  if (dtype == EGS_F16) return launch_by_pair<__half, __half, true>(p, q, pair, q.units, maps, st);
-  return launch_by_pair<__nv_bfloat16, __nv_bfloat16, true>(p, q, pair, q.units, maps, st);
+  const long long units = static_cast<long long>(q.most_ranges) * q.tiles_c * q.tiles_n, size = static_cast<long long>(p.C) * p.N;
+  cudaError_t err = dtype == EGS_F16 ? launch_by_pair<__half, __half, true>(p, q, d.pair, units, maps, st)
+                                     : launch_by_pair<__nv_bfloat16, __nv_bfloat16, true>(p, q, d.pair, units, maps, st);
+  if (err != cudaSuccess || d.most_partial == 0) return err;
+  const dim3 ctas(static_cast<unsigned>(size / 1024 < 1 ? 1 : size / 1024 > kSmCount ? kSmCount : size / 1024), p.E < 16 ? p.E : 16);
+  count_launch();
+  if (dtype == EGS_F16)
+    return launch_kernel(ragged_join_kernel<__half>, ctas, 256, 0, st, true, p.offsets, q.partial, static_cast<__half*>(p.Out), size, p.E, q.range_steps);
+  return launch_kernel(ragged_join_kernel<__nv_bfloat16>, ctas, 256, 0, st, true, p.offsets, q.partial, static_cast<__nv_bfloat16*>(p.Out), size, p.E,
+                       q.range_steps);
 }
 
 }  // namespace egs
