@@ -502,10 +502,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
 // Weighted sum of a token's rows, float32 in the order of its choices, rounded once.
 // ------------------------------------------------------------------------------------------------
 template <typename T, int V> struct Vec;
-// A vector as it lies in memory: loads that wait for one another in this form take half the registers.
-template <typename T, int V> struct alignas(sizeof(T) * V) Packed {
-  T v[V];
-};
 template <typename T> struct Vec<T, 1> {
   static __device__ __forceinline__ void load(const T* p, float (&v)[1]) { v[0] = to_f32<T>(*p); }
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { *p = from_f32<T>(v[0]); }
@@ -519,10 +515,9 @@ template <> struct Vec<float, 4> {
 };
 template <typename T> struct Vec<T, 8> {
   static __device__ __forceinline__ void load(const T* p, float (&v)[8]) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&x);
+    const Packed<T, 8> x = *reinterpret_cast<const Packed<T, 8>*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(h[i]);
+    for (int i = 0; i < 8; ++i) v[i] = x.get(i);
   }
   static __device__ __forceinline__ void store(T* p, const float (&v)[8]) {
     uint4 x;
@@ -642,7 +637,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
         if ((present[stage] >> j) & 1u) {
           const P y = ring[stage][j][threadIdx.x];
 #pragma unroll
-          for (int v = 0; v < V; ++v) sum[v] = fmaf(wj, to_f32<T>(y.v[v]), sum[v]);
+          for (int v = 0; v < V; ++v) sum[v] = fmaf(wj, y.get(v), sum[v]);
         }
       }
       if (use.group == groups - 1) {
@@ -712,7 +707,7 @@ struct QuantizeParams {
 };
 
 template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(128, 8) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
+__global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
   using P = Packed<T, V>;
   constexpr int kKeep = V == 1 ? 16 : 8;
   __shared__ uint32_t found[4];
@@ -733,7 +728,7 @@ __global__ void __launch_bounds__(128, 8) quantize_rows_kernel(const __grid_cons
       for (int v = 0; v < V / 2; ++v) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(&y)[v] & 0x7fff7fffu);
     } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(to_f32<T>(y.v[v])) & 0x7fffffffu);
+      for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(y.get(v)) & 0x7fffffffu);
     }
   };
 #pragma unroll
@@ -770,13 +765,13 @@ __global__ void __launch_bounds__(128, 8) quantize_rows_kernel(const __grid_cons
     uint32_t b[V], apart = divide;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float z = to_f32<T>(y.v[v]);
+      const float z = y.get(v);
       b[v] = __float_as_uint(fmaf(z, less, kRound));
       apart |= b[v] ^ __float_as_uint(fmaf(z, more, kRound));
     }
     if (apart) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) b[v] = static_cast<uint32_t>(max(-127, min(127, __float2int_rn(to_f32<T>(y.v[v]) / scale))));
+      for (int v = 0; v < V; ++v) b[v] = static_cast<uint32_t>(max(-127, min(127, __float2int_rn(y.get(v) / scale))));
     }
     if (!finite) {
 #pragma unroll
@@ -842,13 +837,16 @@ template <> __device__ __forceinline__ int widen<int8_t>(int8_t v) { return v; }
 __device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ int mac(int a, int b, int c) { return a * b + c; }
 
+template <typename T> __device__ __forceinline__ float four(const Packed<T, 4>& x, int i) { return x.get(i); }
+__device__ __forceinline__ int four(const Packed<int8_t, 4>& x, int i) { return x.raw[i]; }
+
 // Four elements of a row from `p` on, `left` of which exist (p is not looked at where that is none); `wide`: they may be loaded together.
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, int left, bool wide, typename Acc<T>::type (&v)[4]) {
   if (wide && left >= 4) {
     const Packed<T, 4> x = *reinterpret_cast<const Packed<T, 4>*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = widen<T>(x.v[i]);
+    for (int i = 0; i < 4; ++i) v[i] = four(x, i);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = i < left ? widen<T>(p[i]) : 0;
@@ -877,7 +875,7 @@ __device__ __forceinline__ void multiply(const GenericTile<A>& s, int buf, int t
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mac(a.v[i], b.v[j], acc[i][j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mac(a.raw[i], b.raw[j], acc[i][j]);
   }
 }
 

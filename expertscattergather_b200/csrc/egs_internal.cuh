@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/egs_b200.h"
 
 namespace egs {
@@ -28,6 +30,25 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two 16-bit elements of a 32-bit word, the lower first.  (Arrays of 16-bit elements in registers take a register for each.)
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+
+// V elements that are loaded together, as they lie in memory; get(v) with v known at compile time.
+template <typename T, int V> struct alignas(sizeof(T) * V) Packed {
+  static constexpr bool kPairs = sizeof(T) == 2 && V > 1;
+  typename std::conditional<kPairs, uint32_t, T>::type raw[kPairs ? V / 2 : V];
+  __device__ __forceinline__ float get(int v) const {
+    if constexpr (kPairs) {
+      const float2 f = unpack2<T>(raw[v / 2]);
+      return v & 1 ? f.y : f.x;
+    } else {
+      return to_f32<T>(raw[v]);
+    }
+  }
+};
 
 // Reads Ind[pos] for any of the three index widths.
 __device__ __forceinline__ long long load_index(const void* ind, int index_dtype, long long pos) {
@@ -273,6 +294,9 @@ size_t generic_dweight_workspace(const RaggedParams& p);
 cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
 size_t ragged_dweight_workspace(const RaggedParams& p);
+// ... where experts have few rows (egs_few.cu): any type, width and alignment, C at least 1
+bool few_rows_fit(const RaggedParams& p);
+cudaError_t launch_few_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 // Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; what lies behind a row's end is not defined).
 cudaError_t launch_pad_rows(const void* src, void* dst, long long rows, int width, int pitch, cudaStream_t st);
 
