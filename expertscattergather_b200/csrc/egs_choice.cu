@@ -32,16 +32,16 @@ __device__ __forceinline__ float warp_max(float v) {
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 
 // ------------------------------------------------------------------------------------------------
-// Routing.  A warp has a token, lane l its experts l, l + 32, ...  Softmax and no bias: the logits' order is the scores', so the logits
+// Routing.  A warp has a token, lane l the NPER experts from l NPER on.  Softmax and no bias: the logits' order is the scores', so the logits
 // are the keys, and a row's sum is only formed where something needs it.  Renormalised softmax weights are formed from the chosen logits
 // alone.
 //
-// The top k: the k-th highest of the lanes' own maxima is a lower bound of the k-th highest key, and few keys lie at or above it
-// (256 random ones, k = 8: ten in the mean).  Those go through shared memory to one lane each, which counts the candidates before its own.
-// Where more than 32 keys lie above (many equal ones) every choice is a maximum over all keys of all lanes: 45 instructions a choice with
-// eight keys a lane.
-//
-// What bounds it is instructions, half of them the scores'.
+// What bounds it is instructions (32768 tokens of 256 experts in 8 groups, sigmoid and bias: 35 MB, 5 us at the memory's rate), so few keys
+// are formed exactly.  All lanes form keys from the fast exponential and reciprocal, within 2^-21 of a score.  The k-th highest of the
+// lanes' own maxima is a lower bound of the k-th highest key; the keys that lie at most a margin of twice that error below it (256 random
+// ones, k = 8: ten in the mean) go through shared memory to one lane each, where their exact keys are formed and every lane counts the keys
+// before its own.  Where more than 32 lie there (many equal ones), every choice is a maximum over the exact keys of all lanes.
+// Groups are compared by their fast keys.
 // ------------------------------------------------------------------------------------------------
 constexpr int kRouteWarps = 8;
 
@@ -56,13 +56,30 @@ struct RouteParams {
   float scale;
   Div by_per;            // experts of a group
   int lanes_log2;        // lanes that look at a group together
-  int pitch;             // of a group's keys in shared memory
+  int whole_lanes;       // a group is the experts of 2^lanes_log2 lanes
+  int vectors;           // rows (and the bias) begin on 16 bytes and have 32 NPER experts
   int warp_words;        // shared memory of a warp
-  int slices;            // groups of that many whole slices of 32 experts; 0: others
 };
 
-__device__ __forceinline__ float unordered(uint32_t k) {         // (the float of ordered(); any NaN for its 1)
+__device__ __forceinline__ float unordered(uint32_t k) {         // (the float of ordered(); a NaN for its 1)
   return k <= 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+// n elements from `p` on (those that exist: left), in 16-byte loads where `wide`
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, int left, bool wide, float (&v)[N]) {
+  constexpr int V = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < N / V; ++i) {
+      const Packed<T, V> x = reinterpret_cast<const Packed<T, V>*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i * V + j] = x.get(j);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < left ? to_f32<T>(p[i]) : 0.f;
+  }
 }
 
 template <typename T, int NPER>
@@ -71,127 +88,124 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp;
+  const int t = blockIdx.x * kRouteWarps + warp;
   if (t >= p.tokens) return;
-  uint32_t* mem = route_smem + warp * p.warp_words;      // keys in groups, then candidates
+  uint32_t* mem = route_smem + warp * p.warp_words;      // keys (groups that are not whole lanes), then candidates
   const T* row = static_cast<const T*>(p.logits) + t * p.stride;
+  const int e0 = lane * NPER, mine_left = p.E - e0;      // this lane's experts: those of index < mine_left
   float x[NPER];
-#pragma unroll
-  for (int i = 0; i < NPER; ++i) {
-    const int e = i * 32 + lane;
-    x[i] = e < p.E ? to_f32<T>(row[e]) : 0.f;
-  }
+  load_run<T, NPER>(row + e0, mine_left, p.vectors, x);
   const bool pairs = p.groups > 1 && p.group_top == 2;
-  const bool need_scores = p.bias || pairs || (!p.sigmoid && !p.renormalize);
+  const bool sums = !p.sigmoid && (p.bias || pairs || !p.renormalize);
   float m = 0.f, total = 1.f;
-  if (!p.sigmoid && need_scores) {
+  uint32_t key[NPER];
+  if (sums) {                                            // scores of a softmax, in x' place
     m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NPER; ++i)
-      if (i * 32 + lane < p.E) m = fmaxf(m, x[i]);
+      if (i < mine_left) m = fmaxf(m, x[i]);
     m = warp_max(m);
     total = 0.f;
+    float ex[NPER];
 #pragma unroll
-    for (int i = 0; i < NPER; ++i)
-      if (i * 32 + lane < p.E) total += m == -INFINITY ? 0.f : expf(x[i] - m);
+    for (int i = 0; i < NPER; ++i) {
+      ex[i] = i < mine_left && m != -INFINITY ? expf(x[i] - m) : 0.f;
+      total += ex[i];
+    }
     total = warp_sum(total);
-  }
-  auto score = [&](float v) { return p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total; };
-  uint32_t key[NPER];
-  if (p.groups == 1) {
-    if (p.bias) {
+    if (p.bias || pairs) {
+      const float inverse = m == -INFINITY ? 0.f : 1.f / total;
 #pragma unroll
-      for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(score(x[i]) + p.bias[i * 32 + lane]) : 0u;
+      for (int i = 0; i < NPER; ++i) ex[i] *= inverse;
+    }
+    if (p.bias) {
+      float b[NPER];
+      load_run<float, NPER>(p.bias + e0, mine_left, p.vectors, b);
+#pragma unroll
+      for (int i = 0; i < NPER; ++i) key[i] = ordered(ex[i] + b[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NPER; ++i) key[i] = i * 32 + lane < p.E ? ordered(x[i]) : 0u;
+      for (int i = 0; i < NPER; ++i) key[i] = pairs ? ordered(ex[i]) : ordered(x[i]);
     }
-  } else if (p.slices) {
-    // groups of whole slices of 32 experts: the two highest keys of each are maxima over the warp
-    uint32_t k1 = 0u, k2 = 0u, g1 = 0u, g2 = 0u;         // of this lane in the group, of group `lane`
-    int in_group = 0, g = 0;
+  } else if (p.sigmoid && (p.bias || pairs)) {
+    float b[NPER];
+    if (p.bias) load_run<float, NPER>(p.bias + e0, mine_left, p.vectors, b);
 #pragma unroll
     for (int i = 0; i < NPER; ++i) {
-      const int e = i * 32 + lane;
-      const bool on = e < p.E;
-      key[i] = on ? ordered(p.bias ? score(x[i]) + p.bias[e] : x[i]) : 0u;
-      const uint32_t v = on && pairs && !p.bias ? ordered(score(x[i])) : key[i];
-      k2 = max(k2, min(k1, v));
-      k1 = max(k1, v);
-      if (++in_group == p.slices) {
-        const uint32_t first = __reduce_max_sync(kFull, k1);
-        const unsigned who = __ballot_sync(kFull, k1 == first);
-        const uint32_t second = __reduce_max_sync(kFull, lane == __ffs(who) - 1 ? k2 : k1);
-        if (lane == g) {
-          g1 = first;
-          g2 = second;
-        }
-        k1 = k2 = 0u;
-        in_group = 0;
-        ++g;
-      }
-    }
-    uint32_t gk = g1;
-    if (pairs) gk = ordered(unordered(g1) + unordered(g2));
-    if (lane >= p.groups) gk = 0u;
-    uint32_t kept = 0u;
-    for (int i = 0; i < p.top_groups; ++i) {
-      const uint32_t best = __reduce_max_sync(kFull, gk);
-      const int at = __ffs(__ballot_sync(kFull, gk == best)) - 1;
-      kept |= 1u << at;
-      if (lane == at) gk = 0u;
-    }
-    in_group = 0;
-#pragma unroll
-    for (int i = 0; i < NPER; ++i) {
-      if (!(kept & 1u)) key[i] = 0u;
-      if (++in_group == p.slices) {
-        in_group = 0;
-        kept >>= 1;
-      }
+      const float s = __fdividef(1.f, 1.f + __expf(-x[i]));
+      key[i] = ordered(p.bias ? s + b[i] : s);
     }
   } else {
-    int group[NPER];
 #pragma unroll
-    for (int i = 0; i < NPER; ++i) {
-      const int e = i * 32 + lane;
-      group[i] = p.by_per.quotient(e);
-      key[i] = 0u;
-      if (e < p.E) {
-        key[i] = ordered(p.bias ? score(x[i]) + p.bias[e] : x[i]);
-        mem[group[i] * p.pitch + e - group[i] * p.per] = pairs && !p.bias ? ordered(score(x[i])) : key[i];
+    for (int i = 0; i < NPER; ++i) key[i] = ordered(x[i]);
+  }
+  // whether the keys above are fast ones, and the exact key of an expert
+  const bool fast = p.bias || pairs;
+  auto exact = [&](float v, int e) {
+    if (!p.bias) return ordered(v);
+    const float s = p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total;
+    return ordered(s + p.bias[e]);
+  };
+  if (!p.vectors) {
+#pragma unroll
+    for (int i = 0; i < NPER; ++i)
+      if (i >= mine_left) key[i] = 0u;
+  }
+  if (p.groups > 1) {
+    uint32_t k1 = 0u, k2 = 0u;                           // the two highest keys
+    const int g = lane >> p.lanes_log2;
+    if (p.whole_lanes) {
+#pragma unroll
+      for (int i = 0; i < NPER; ++i) {
+        k2 = max(k2, min(k1, key[i]));
+        k1 = max(k1, key[i]);
       }
+    } else {
+      // through shared memory: the lanes of a group look at every 2^lanes_log2-th of its keys
+#pragma unroll
+      for (int i = 0; i < NPER; ++i)
+        if (i < mine_left) mem[e0 + i] = key[i];
+      __syncwarp();
+      if (g < p.groups)
+        for (int i = lane & ((1 << p.lanes_log2) - 1); i < p.per; i += 1 << p.lanes_log2) {
+          const uint32_t v = mem[g * p.per + i];
+          k2 = max(k2, min(k1, v));
+          k1 = max(k1, v);
+        }
+      __syncwarp();
     }
-    // the lanes of a group look at every 2^lanes_log2-th of its keys and join what they found
-    __syncwarp();
-    const int lanes = 1 << p.lanes_log2, g = lane >> p.lanes_log2;
-    uint32_t k1 = 0u, k2 = 0u;
-    if (g < p.groups)
-      for (int i = lane & (lanes - 1); i < p.per; i += lanes) {
-        const uint32_t v = mem[g * p.pitch + i];
-        k2 = max(k2, min(k1, v));
-        k1 = max(k1, v);
-      }
-    for (int o = 1; o < lanes; o <<= 1) {
+    for (int o = 1; o < (1 << p.lanes_log2); o <<= 1) {
       const uint32_t o1 = __shfl_xor_sync(kFull, k1, o), o2 = __shfl_xor_sync(kFull, k2, o);
       k2 = max(min(k1, o1), max(k2, o2));
       k1 = max(k1, o1);
     }
-    uint32_t gk = k1;
-    if (pairs && k2) gk = ordered(unordered(k1) + unordered(k2));
-    gk = __shfl_sync(kFull, gk, (lane << p.lanes_log2) & 31);      // group g's value in lane g
-    if (lane >= p.groups) gk = 0u;
-    uint32_t kept = 0u;
+    // (every lane of a group has its value; the first one stands for it)
+    uint32_t gk = pairs && k2 ? ordered(unordered(k1) + unordered(k2)) : k1;
+    if (g >= p.groups || (lane & ((1 << p.lanes_log2) - 1))) gk = 0u;
+    uint32_t kept = 0u;                                  // by first lanes
     for (int i = 0; i < p.top_groups; ++i) {
       const uint32_t best = __reduce_max_sync(kFull, gk);
       const int at = __ffs(__ballot_sync(kFull, gk == best)) - 1;
       kept |= 1u << at;
       if (lane == at) gk = 0u;
     }
+    if (p.whole_lanes) {
+      if (!((kept >> (g << p.lanes_log2)) & 1u)) {
 #pragma unroll
-    for (int i = 0; i < NPER; ++i)
-      if (!((kept >> (group[i] & 31)) & 1u)) key[i] = 0u;
+        for (int i = 0; i < NPER; ++i) key[i] = 0u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NPER; ++i)
+        if (!((kept >> ((p.by_per.quotient(e0 + i) << p.lanes_log2) & 31)) & 1u)) key[i] = 0u;
+    }
+    if (pairs && !p.bias) {                              // scores have compared the groups; their experts are compared by the logits
+#pragma unroll
+      for (int i = 0; i < NPER; ++i)
+        if (key[i]) key[i] = ordered(x[i]);
+    }
   }
+  const float margin = fast && p.bias ? 1e-6f : 0.f;
   // lower bound, candidates
   uint32_t top = key[0];
 #pragma unroll
@@ -203,50 +217,62 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
     if (best == 0u) break;
     if (top == best) top = 0u;
   }
-  bound = max(bound, 1u);
-  int found = 0;
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < NPER; ++i) {
-    const unsigned who = __ballot_sync(kFull, key[i] >= bound);
-    if (key[i] >= bound) {
-      const int at = found + __popc(who & ((1u << lane) - 1u));
-      if (at < 32) {
-        mem[at] = key[i];
-        mem[32 + at] = i * 32 + lane;
-      }
-    }
-    found += __popc(who);
+  if (margin > 0.f && bound > 1u) {
+    const float b = unordered(bound);
+    bound = ordered(b - margin * (1.f + fabsf(b)));      // (infinities stay where they are)
+    if (b != b || fabsf(b) == INFINITY) bound = 1u;
   }
-  __syncwarp();
+  bound = max(bound, 1u);
+  int own = 0;
+#pragma unroll
+  for (int i = 0; i < NPER; ++i) own += key[i] >= bound ? 1 : 0;
+  int at = own;                                // candidates up to this lane's last: in the order of the experts
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, at, o);
+    if (lane >= o) at += v;
+  }
+  const int found = __shfl_sync(kFull, at, 31);
   int mine = 0, place = p.k;                   // this lane's chosen expert and its place among them
   if (found <= 32) {
-    const uint32_t own = lane < found ? mem[lane] : 0u;
+    at -= own;
+    if (own) {
+#pragma unroll
+      for (int i = 0; i < NPER; ++i)
+        if (key[i] >= bound) mem[at++] = e0 + i;
+    }
+    __syncwarp();
+    mine = lane < found ? static_cast<int>(mem[lane]) : 0;
+    const uint32_t k = lane < found ? exact(to_f32<T>(row[mine]), mine) : 0u;
+    mem[32 + lane] = k;
+    __syncwarp();
     int before = 0;
     for (int j = 0; j < found; ++j) {
-      const uint32_t other = mem[j];
-      before += (other > own || (other == own && j < lane)) ? 1 : 0;
+      const uint32_t other = mem[32 + j];
+      before += (other > k || (other == k && j < lane)) ? 1 : 0;
     }
-    if (lane < found) {
-      mine = static_cast<int>(mem[32 + lane]);
-      place = before;
-    }
+    if (lane < found) place = before;
   } else {
+    if (fast) {
+#pragma unroll
+      for (int i = 0; i < NPER; ++i)
+        if (key[i]) key[i] = exact(x[i], e0 + i);
+    }
     for (int j = 0; j < p.k; ++j) {
       uint32_t best = key[0];
 #pragma unroll
       for (int i = 1; i < NPER; ++i) best = max(best, key[i]);
       best = __reduce_max_sync(kFull, best);
-      uint32_t at = kFull;
+      uint32_t who = kFull;
 #pragma unroll
       for (int i = NPER - 1; i >= 0; --i)
-        if (key[i] == best) at = i * 32 + lane;
-      at = __reduce_min_sync(kFull, at);
+        if (key[i] == best) who = e0 + i;
+      who = __reduce_min_sync(kFull, who);
 #pragma unroll
       for (int i = 0; i < NPER; ++i)
-        if (at == i * 32 + lane) key[i] = 0u;
+        if (who == e0 + i) key[i] = 0u;
       if (lane == j) {
-        mine = static_cast<int>(at);
+        mine = static_cast<int>(who);
         place = j;
       }
     }
@@ -263,8 +289,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
     w = p.sigmoid ? sigmoid(xc) : m == -INFINITY ? 0.f : expf(xc - m) / total;
   }
   if (chosen) {
-    p.weights[t * p.k + place] = w * p.scale;
-    p.experts[t * p.k + place] = mine;
+    p.weights[static_cast<long long>(t) * p.k + place] = w * p.scale;
+    p.experts[static_cast<long long>(t) * p.k + place] = mine;
   }
 }
 
@@ -1047,13 +1073,23 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short* src
   dst[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 template <typename T, int NPER>
-cudaError_t route_n(const RouteParams& p, cudaStream_t st) {
+cudaError_t route_n(RouteParams& p, cudaStream_t st) {
+  const int lanes = p.per / NPER;
+  p.whole_lanes = p.per % NPER == 0 && (lanes & (lanes - 1)) == 0;
+  if (p.whole_lanes) {
+    p.lanes_log2 = 0;
+    while ((1 << p.lanes_log2) < lanes) ++p.lanes_log2;
+  }
+  p.vectors = p.E == 32 * NPER && (p.stride * sizeof(T)) % 16 == 0 && aligned(p.logits) && (!p.bias || aligned(p.bias));
+  p.warp_words = p.groups > 1 && !p.whole_lanes && p.E > 64 ? p.E : 64;
   const size_t smem = sizeof(uint32_t) * kRouteWarps * p.warp_words;
   return launch_kernel(route_tokens_kernel<T, NPER>, (p.tokens + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, smem, st, true, p);
 }
 template <typename T>
-cudaError_t route_t(const RouteParams& p, cudaStream_t st) {
+cudaError_t route_t(RouteParams& p, cudaStream_t st) {
   if (p.E <= 32) return route_n<T, 1>(p, st);
   if (p.E <= 64) return route_n<T, 2>(p, st);
   if (p.E <= 128) return route_n<T, 4>(p, st);
@@ -1066,7 +1102,6 @@ template <class F16, class BF16, class F32>
 cudaError_t by_type(int dtype, F16&& f16, BF16&& bf16, F32&& f32) {
   return dtype == EGS_F16 ? f16() : dtype == EGS_BF16 ? bf16() : f32();
 }
-bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T, int V>
 cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
@@ -1111,9 +1146,6 @@ cudaError_t launch_route_tokens(const void* logits, const float* bias, float* we
   p.group_top = r.group_top; p.per = r.E / r.groups; p.by_per = Div(p.per);
   p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
   while ((32 >> p.lanes_log2) > 1 && (32 >> (p.lanes_log2 + 1)) >= r.groups) ++p.lanes_log2;
-  p.pitch = p.per + (1 << p.lanes_log2);               // (groups of 32: all lanes in banks of their own)
-  p.slices = r.groups > 1 && p.per % 32 == 0 ? p.per / 32 : 0;
-  p.warp_words = r.groups > 1 && !p.slices && r.groups * p.pitch > 64 ? r.groups * p.pitch : 64;
   count_launch();
   return by_type(dtype, [&] { return route_t<__half>(p, st); }, [&] { return route_t<__nv_bfloat16>(p, st); }, [&] { return route_t<float>(p, st); });
 }
