@@ -84,7 +84,7 @@ __device__ __forceinline__ void load_run(const T* p, int left, bool wide, float 
 
 template <typename T, int NPER>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __grid_constant__ RouteParams p) {
-  extern __shared__ uint32_t route_smem[];
+  extern __shared__ __align__(16) uint32_t route_smem[];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
   }
   const int found = __shfl_sync(kFull, at, 31);
   int mine = 0, place = p.k;                   // this lane's chosen expert and its place among them
+  float xc = -INFINITY;                        // ... and its logit
   if (found <= 32) {
     at -= own;
     if (own) {
@@ -243,13 +244,17 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
     }
     __syncwarp();
     mine = lane < found ? static_cast<int>(mem[lane]) : 0;
-    const uint32_t k = lane < found ? exact(to_f32<T>(row[mine]), mine) : 0u;
+    xc = lane < found ? to_f32<T>(row[mine]) : -INFINITY;
+    const uint32_t k = lane < found ? exact(xc, mine) : 0u;
     mem[32 + lane] = k;
     __syncwarp();
     int before = 0;
-    for (int j = 0; j < found; ++j) {
-      const uint32_t other = mem[32 + j];
-      before += (other > k || (other == k && j < lane)) ? 1 : 0;
+    for (int j = 0; j < found; j += 4) {       // (no key is 2^32 - 1, and there are zeros behind the last one)
+      const uint4 other = *reinterpret_cast<const uint4*>(mem + 32 + j);
+      before += other.x + (j < lane) > k;
+      before += other.y + (j + 1 < lane) > k;
+      before += other.z + (j + 2 < lane) > k;
+      before += other.w + (j + 3 < lane) > k;
     }
     if (lane < found) place = before;
   } else {
@@ -276,9 +281,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
         place = j;
       }
     }
+    if (place < p.k) xc = to_f32<T>(row[mine]);
   }
   const bool chosen = place < p.k;
-  const float xc = chosen ? to_f32<T>(row[mine]) : -INFINITY;
+  if (!chosen) xc = -INFINITY;
   float w;
   if (p.renormalize) {
     const float best = p.sigmoid ? 0.f : warp_max(xc);
@@ -1084,7 +1090,7 @@ cudaError_t route_n(RouteParams& p, cudaStream_t st) {
     while ((1 << p.lanes_log2) < lanes) ++p.lanes_log2;
   }
   p.vectors = p.E == 32 * NPER && (p.stride * sizeof(T)) % 16 == 0 && aligned(p.logits) && (!p.bias || aligned(p.bias));
-  p.warp_words = p.groups > 1 && !p.whole_lanes && p.E > 64 ? p.E : 64;
+  p.warp_words = p.groups > 1 && !p.whole_lanes && p.E > 64 ? (p.E + 3) / 4 * 4 : 64;      // (read 16 bytes at a time)
   const size_t smem = sizeof(uint32_t) * kRouteWarps * p.warp_words;
   return launch_kernel(route_tokens_kernel<T, NPER>, (p.tokens + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, smem, st, true, p);
 }

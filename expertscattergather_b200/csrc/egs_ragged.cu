@@ -184,7 +184,7 @@ template <typename T, typename OutT, bool WEIGHTS, bool PAIR>
 __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kRaggedThreads, 1)
 ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ RaggedTiles q, const __grid_constant__ TensorMap3 map_a,
               const __grid_constant__ TensorMap3 map_a4, const __grid_constant__ TensorMap3 map_b, const __grid_constant__ TensorMap3 map_b4) {
-  constexpr bool kInt8 = sizeof(T) == 1;
+  constexpr bool kInt8 = sizeof(T) == 1, kTwoBytes = sizeof(OutT) == 2;
   constexpr int kBlock = PAIR ? 256 : 128;           // rows of a tile
   constexpr int kStepElems = 128 / sizeof(T);        // `rows`
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -472,32 +472,55 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
       const long long step = static_cast<long long>(gridDim.x) * (kReadWarps * 32);
       for (long long i = begin + blockIdx.x * (kReadWarps * 32) + ew * 32 + lane; i < end; i += step) out[i] = from_f32<OutT>(0.f);
     }
-    int e = 0, t = 0;
-    for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
-      const int x = q.by_n.quotient(u);
-      const int n0 = (u - x * q.tiles_n) * q.BN, bn = min(q.BN, p.N - n0);
-      long long row0;                                // output row of the warp's first accumulator row
-      int rows;                                      // of its 32 that are stored
-      int partial = -1;
-      bool have = true;
-      float scale = 0.f;
+    // What is known about a tile before its accumulator is there, asked for while the tile before is read out: the two loads that find a
+    // row's scale took a microsecond of every tile.
+    struct Tile {
+      int e, n0, bn, rows, partial;      // rows: of the warp's 32 that are stored
+      long long row0;                    // output row of the first of them
+      bool have;                         // there is an accumulator (an expert without rows: zeros)
+      float scale, w_scale[4];           // 8-bit operands: of this lane's row, of its columns (32 apart)
+    };
+    int e_last = 0;
+    auto tile_of = [&](int u) {
+      Tile x{};
+      const int block = q.by_n.quotient(u);
+      x.n0 = (u - block * q.tiles_n) * q.BN;
+      x.bn = min(q.BN, p.N - x.n0);
+      x.partial = -1;
       if constexpr (!WEIGHTS) {
-        e = expert_of(starts, p.E, x, e);
-        const int r = offsets[e] + (x - starts[e]) * kBlock + rank * 128 + lg * 32;
-        row0 = r;
-        rows = min(32, offsets[e + 1] - r);
+        x.e = e_last = expert_of(starts, p.E, block, e_last);
+        const int r = offsets[x.e] + (block - starts[x.e]) * kBlock + rank * 128 + lg * 32;
+        x.row0 = r;
+        x.rows = min(32, offsets[x.e + 1] - r);
+        x.have = true;
         if constexpr (kInt8) {
-          if (lane < rows) scale = p.a_scale[p.slots ? p.by_k.quotient(p.slots[r + lane]) : r + lane];
+          if (lane < x.rows) x.scale = p.a_scale[p.slots ? p.by_k.quotient(p.slots[r + lane]) : r + lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = kTwoBytes ? (i >> 1) * 128 + share * 64 + (i & 1) * 32 : i * 64 + share * 32;
+            if (c + lane < x.bn) x.w_scale[i] = p.w_scale[static_cast<long long>(x.e) * p.N + x.n0 + c + lane];
+          }
         }
       } else {
-        int y = x;
+        int y = block;
         const int f = q.by_c.remainder(y) * kBlock + rank * 128 + lg * 32;
         y = range.order[y];
-        partial = range.partial[y];
-        row0 = static_cast<long long>(partial >= 0 ? partial : range.expert[y]) * p.C + f;
-        rows = min(32, p.C - f);
-        have = range.end[y] > range.first[y];
+        x.partial = range.partial[y];
+        x.row0 = static_cast<long long>(x.partial >= 0 ? x.partial : range.expert[y]) * p.C + f;
+        x.rows = min(32, p.C - f);
+        x.have = range.end[y] > range.first[y];
       }
+      return x;
+    };
+    int t = 0;
+    Tile tile{}, coming{};
+    if (unit_of(0) < units) coming = tile_of(unit_of(0));
+    for (int round = 0; unit_of(round) < units && alive; ++round) {
+      tile = coming;
+      if (unit_of(round + 1) < units) coming = tile_of(unit_of(round + 1));
+      const int n0 = tile.n0, bn = tile.bn, rows = tile.rows, partial = tile.partial;
+      const long long row0 = tile.row0;
+      const bool have = tile.have;
       const int buf = t & 1;
       if (have) {
         alive = mbar_wait_all(smem_u32(&hdr->acc_full[buf]), (t >> 1) & 1, abort_flag, p.status.word);
@@ -518,7 +541,7 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
         released = true;
       };
       // 32 columns of the accumulator in float32
-      auto read = [&](int c, uint32_t (&v)[32]) {
+      auto read = [&](int c, int which, uint32_t (&v)[32]) {
         if (have) {
           tmem_ld32(acc + static_cast<uint32_t>(c), v);
           tmem_ld_wait();
@@ -526,19 +549,25 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0u;
         }
-        if constexpr (kInt8) {
-          const float* ws = p.w_scale + static_cast<long long>(e) * p.N + n0 + c;
+        if constexpr (kInt8) {                       // (which: the block's place among those of the warp)
+          const uint32_t scales = area0 + kReadWarps * kReadArea + static_cast<uint32_t>(ew) * 128u;
+          const float own = which == 0 ? tile.w_scale[0] : which == 1 ? tile.w_scale[1] : which == 2 ? tile.w_scale[2] : tile.w_scale[3];
+          __syncwarp();
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + lane * 4u), "f"(own) : "memory");
+          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float w = c + i < bn ? ws[i] : 0.f;
-            v[i] = __float_as_uint(static_cast<float>(static_cast<int>(v[i])) * (scale * w));
+          for (int i = 0; i < 32; i += 4) {
+            float w[4];
+            asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]) : "r"(scales + i * 4u) : "memory");
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i + k] = __float_as_uint(static_cast<float>(static_cast<int>(v[i + k])) * (tile.scale * w[k]));
           }
         }
       };
       auto store_f32 = [&](float* to, bool vectors) {
         for (int c = share * 32; c < bn; c += 64) {
           uint32_t v[32];
-          read(c, v);
+          read(c, c >> 6, v);
           if (c + 64 >= bn) release();
           warp_regs_emit(v, area, lane, [&](int row, int cj, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
             const int col = c + cj;
@@ -565,7 +594,7 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
           for (int h = 0; h < 2; ++h) {
             if (c + h * 32 < bn) {
               uint32_t v[32];
-              read(c + h * 32, v);
+              read(c + h * 32, (c >> 7) * 2 + h, v);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(srow + static_cast<uint32_t>((h * 4 + j) ^ (lane & 7)) * 16u),
@@ -678,7 +707,7 @@ cudaError_t launch_ragged(const RaggedParams& p, RaggedTiles q, long long most_u
   q.table_bytes = static_cast<uint32_t>((p.E + 1) * 4 + 15) & ~15u;
   const size_t before = (kRaggedHeader + q.table_bytes + (WEIGHTS ? range_bytes(q.most_ranges) : q.table_bytes) + 1023u) & ~static_cast<size_t>(1023);
   const size_t stage = kATile + b_tile_bytes(PAIR ? q.BN / 2 : q.BN);
-  const size_t fixed = before + kReadWarps * kReadArea;
+  const size_t fixed = before + kReadWarps * (kReadArea + (sizeof(T) == 1 ? 128 : 0));
   q.stages = static_cast<int>((kRaggedSmem - fixed) / stage);
   if (q.stages > kMaxStages) q.stages = kMaxStages;
   cudaError_t err = ensure_smem_optin<ragged_kernel<T, OutT, WEIGHTS, PAIR>>(static_cast<int>(kRaggedSmem));
