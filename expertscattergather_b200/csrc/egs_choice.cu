@@ -586,6 +586,7 @@ constexpr int kCombineStages = 4, kCombineAhead = kCombineStages - 1, kCombineWa
 template <typename T, int V>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __grid_constant__ CombineParams p) {
   using P = Packed<T, V>;
+  static_assert(sizeof(P) == 16, "cp.async copies 16 bytes");
   __shared__ P ring[kCombineStages][4][kCombineWarps * 32];
   pdl_wait();
   pdl_trigger();
@@ -635,10 +636,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
         const int at = __shfl_sync(kFull, pos, j);
         if (at >= 0 && c < p.N) {
           const P* src = reinterpret_cast<const P*>(Y + static_cast<long long>(at) * p.N + c);
-          if constexpr (sizeof(P) == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[stage][j][threadIdx.x]))), "l"(src) : "memory");
-          else
-            ring[stage][j][threadIdx.x] = *src;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[stage][j][threadIdx.x]))), "l"(src) : "memory");
         }
       }
     }
@@ -682,6 +680,34 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
       w = w_next;
     }
   }
+}
+
+// Rows that do not begin on 16 bytes: a thread has a column of a token.
+template <typename T>
+__global__ void __launch_bounds__(256) combine_columns_kernel(const __grid_constant__ CombineParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<long long>(p.tokens) * p.N) return;
+  const long long t = i / p.N;
+  const int c = static_cast<int>(i - t * p.N);
+  const T* Y = static_cast<const T*>(p.Y) + c;
+  const int* pos = p.position + t * p.k;
+  float sum = 0.f;
+  for (int j0 = 0; j0 < p.k; j0 += 4) {
+    int at[4];
+    float w[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at[j] = j0 + j < p.k ? pos[j0 + j] : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      y[j] = at[j] >= 0 ? to_f32<T>(Y[static_cast<long long>(at[j]) * p.N]) : 0.f;
+      w[j] = at[j] >= 0 ? weight_of<T>(p, t * p.k + j0 + j) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = fmaf(w[j], y[j], sum);
+  }
+  static_cast<T*>(p.out)[i] = from_f32<T>(sum);
 }
 
 // A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
@@ -1065,18 +1091,27 @@ __global__ void __launch_bounds__(256) dweight_join_kernel(const float* partial,
   out[blockIdx.y * size + i] = from_f32<T>(sum);
 }
 
-// Rows of 16-bit elements with another pitch; a thread writes eight elements.
-__global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short* src, uint4* dst, long long vectors, int width, int per_row) {
+// Rows of 16-bit elements with another pitch; a thread writes eight elements.  Two matrices with one launch.
+struct PadMatrix {
+  const unsigned short* src;
+  uint4* dst;
+  long long vectors;
+  int width, per_row;
+};
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ PadMatrix a, const __grid_constant__ PadMatrix b) {
   pdl_wait();
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= vectors) return;
+  long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const bool second = i >= a.vectors;
+  if (second) i -= a.vectors;
+  if (second && i >= b.vectors) return;
+  const int width = second ? b.width : a.width, per_row = second ? b.per_row : a.per_row;
   const long long row = i / per_row;
   const int c = static_cast<int>(i - row * per_row) * 8;
-  const unsigned short* s = src + row * width + c;
+  const unsigned short* s = (second ? b.src : a.src) + row * width + c;
   unsigned short v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = c + j < width ? s[j] : 0;
-  dst[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  (second ? b.dst : a.dst)[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1116,11 +1151,16 @@ cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
     const long long slots = static_cast<long long>(p.tokens) * p.k;
     return launch_kernel(combine_backward_kernel<T, V>, static_cast<unsigned>((slots + 7) / 8), 256, 0, st, true, p);
   }
+  if constexpr (V == 1) {
+    const long long work = static_cast<long long>(p.tokens) * p.N;
+    return launch_kernel(combine_columns_kernel<T>, static_cast<unsigned>((work + 255) / 256), 256, 0, st, true, p);
+  }
   const int blocks = (p.vecs + 31) / 32;
   p.by_blocks = Div(blocks);
   p.work = p.tokens * blocks;
   const int ctas = (p.work + kCombineWarps - 1) / kCombineWarps;
-  return launch_kernel(combine_kernel<T, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
+  if constexpr (V > 1) return launch_kernel(combine_kernel<T, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
+  return cudaErrorInvalidValue;
 }
 template <typename T>
 cudaError_t combine_t(CombineParams& p, bool backward, cudaStream_t st) {
@@ -1226,11 +1266,14 @@ cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long lo
                  [&] { return quantize_t<float>(p, st); });
 }
 
-cudaError_t launch_pad_rows(const void* src, void* dst, long long rows, int width, int pitch, cudaStream_t st) {
-  const long long vectors = rows * (pitch / 8);
+cudaError_t launch_pad_rows(const PadRows (&m)[2], cudaStream_t st) {
+  PadMatrix p[2]{};
+  for (int i = 0; i < 2; ++i)
+    if (m[i].dst) p[i] = {static_cast<const unsigned short*>(m[i].src), static_cast<uint4*>(m[i].dst), m[i].rows * (m[i].pitch / 8), m[i].width, m[i].pitch / 8};
+  const long long vectors = p[0].vectors + p[1].vectors;
+  if (vectors == 0) return cudaSuccess;
   count_launch();
-  return launch_kernel(pad_rows_kernel, static_cast<unsigned>((vectors + 255) / 256), 256, 0, st, true, static_cast<const unsigned short*>(src),
-                       static_cast<uint4*>(dst), vectors, width, pitch / 8);
+  return launch_kernel(pad_rows_kernel, static_cast<unsigned>((vectors + 255) / 256), 256, 0, st, true, p[0], p[1]);
 }
 
 // Row blocks there can be: every expert with rows may have one that is not full.

@@ -56,15 +56,14 @@ long long pitch8(long long width) { return (width + 7) / 8 * 8; }
 size_t copy_bytes(long long rows, long long width) {
   return width % 8 ? (static_cast<size_t>(rows) * pitch8(width) * 2 + 255) & ~static_cast<size_t>(255) : 0;
 }
-// ... of `rows` rows of `width` elements at *src, which *pitch becomes the pitch of; moves `workspace` on
-cudaError_t copy_padded(const void** src, long long* pitch, long long rows, long long width, char** workspace, cudaStream_t st) {
-  if (width % 8 == 0) return cudaSuccess;
-  char* to = *workspace;
+// ... of `rows` rows of `width` elements at *src, which becomes the copy and *pitch its pitch; moves `workspace` on
+PadRows padded(const void** src, long long* pitch, long long rows, long long width, char** workspace) {
+  if (width % 8 == 0) return {};
+  const PadRows m{*src, *workspace, rows, static_cast<int>(width), static_cast<int>(pitch8(width))};
   *workspace += copy_bytes(rows, width);
-  *pitch = pitch8(width);
-  const cudaError_t err = launch_pad_rows(*src, to, rows, static_cast<int>(width), static_cast<int>(*pitch), st);
-  *src = to;
-  return err;
+  *pitch = m.pitch;
+  *src = m.dst;
+  return m;
 }
 long long a_rows_of(const egs_ragged& d, int rows) { return rows == EGS_ROWS_TOKENS ? d.tokens : d.tokens * d.k; }
 
@@ -130,9 +129,9 @@ int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, cons
   const size_t need = egs_expert_matmul_workspace_bytes(dims, rows, w_layout, dtype);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
-  cudaError_t err = copy_padded(&p.A, &p.a_row, p.a_rows, p.C, &ws, st);
-  if (err == cudaSuccess) err = copy_padded(&p.W, &p.w_row, dims->E * (p.nc ? p.N : p.C), p.w_row, &ws, st);
-  if (err != cudaSuccess) return fail_cuda(err, "expert_matmul copies");
+  const PadRows rows_copy = padded(&p.A, &p.a_row, p.a_rows, p.C, &ws);
+  const PadRows copies[2] = {rows_copy, padded(&p.W, &p.w_row, dims->E * (p.nc ? p.N : p.C), p.w_row, &ws)};
+  if (cudaError_t err = launch_pad_rows(copies, st); err != cudaSuccess) return fail_cuda(err, "expert_matmul copies");
   p.w_expert = p.w_row * (p.nc ? p.N : p.C);
   return done(launch_ragged_rows_tensor(p, dtype, dtype, st), "expert_matmul launch");
 }
@@ -167,9 +166,9 @@ int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, co
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
   if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_dweight(p, dtype, workspace, st), "expert_dweight launch");
   char* ws = static_cast<char*>(workspace);
-  cudaError_t err = copy_padded(&p.A, &p.a_row, p.a_rows, p.C, &ws, st);
-  if (err == cudaSuccess) err = copy_padded(&p.W, &p.w_row, p.rows, p.N, &ws, st);
-  if (err != cudaSuccess) return fail_cuda(err, "expert_dweight copies");
+  const PadRows rows_copy = padded(&p.A, &p.a_row, p.a_rows, p.C, &ws);
+  const PadRows copies[2] = {rows_copy, padded(&p.W, &p.w_row, p.rows, p.N, &ws)};
+  if (cudaError_t err = launch_pad_rows(copies, st); err != cudaSuccess) return fail_cuda(err, "expert_dweight copies");
   return done(launch_ragged_dweight_tensor(p, dtype, ws, st), "expert_dweight launch");
 }
 

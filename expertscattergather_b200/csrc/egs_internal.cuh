@@ -297,8 +297,14 @@ size_t ragged_dweight_workspace(const RaggedParams& p);
 // ... where experts have few rows (egs_few.cu): any type, width and alignment, C at least 1
 bool few_rows_fit(const RaggedParams& p);
 cudaError_t launch_few_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
-// Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; what lies behind a row's end is not defined).
-cudaError_t launch_pad_rows(const void* src, void* dst, long long rows, int width, int pitch, cudaStream_t st);
+// Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; zeros behind a row's end); dst NULL: nothing.
+struct PadRows {
+  const void* src;
+  void* dst;
+  long long rows;
+  int width, pitch;
+};
+cudaError_t launch_pad_rows(const PadRows (&m)[2], cudaStream_t st);
 
 // Errors of the C entries (egs_api.cu): remembers the text, returns EGS_ERR_CUDA.
 int fail_cuda(cudaError_t err, const char* where);
