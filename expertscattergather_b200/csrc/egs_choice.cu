@@ -711,7 +711,8 @@ __global__ void __launch_bounds__(256) combine_columns_kernel(const __grid_const
 }
 
 // A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
-// zeros and a gradient of zero.
+// zeros and a gradient of zero.  (A warp for every token, ten loads of four choices under way together: no faster for 512 bf16, 22 us
+// instead of 20 for 65536 slots of 256, 17 instead of 11 for 32768 of 64 float32.)
 template <typename T, int V>
 __global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_constant__ CombineParams p) {
   pdl_wait();
@@ -1015,20 +1016,31 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant_
   }
 }
 
-// dW[e, c, n] = sum over the rows of e of X[row, c] dY[row, n].  The rows of every expert are cut into `splits` ranges, whose sums (where
-// there are several) go to the workspace [E, splits, C, N] and are added in their order by a second kernel.
+// dW[e, c, n] = sum over the rows of e of X[row, c] dY[row, n].  Where `length` is not 0 a CTA has that many rows of an expert at most; the sums of
+// all those ranges go to the workspace [range, C, N] and are added in their order by a second kernel.  (Equal numbers of ranges for all
+// experts left the CTAs of the largest ones at work alone: 44 us for 32 experts of 128 x 64 float32.)
+struct DweightRange {
+  int expert, first, end;
+};
+__device__ __forceinline__ DweightRange range_of(const RaggedParams& p, int length, DweightRange* shared) {
+  if (length == 0) return {static_cast<int>(blockIdx.z), p.offsets[blockIdx.z], p.offsets[blockIdx.z + 1]};
+  if (threadIdx.x < 32) locate_block(p.offsets, p.E, length, blockIdx.z, &shared->expert, &shared->first, &shared->end);
+  __syncthreads();
+  DweightRange r = *shared;
+  r.end = min(r.end, r.first + length);
+  return r;
+}
 template <typename T>
-__global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p, int splits, float* partial) {
+__global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
+  __shared__ DweightRange shared;
   __shared__ GenericTile<float> s;
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int e = blockIdx.z / splits, split = blockIdx.z - e * splits;
+  const DweightRange range = range_of(p, length, &shared);
+  if (range.expert < 0) return;
+  const int e = range.expert, first = range.first, end = range.end;
   const int tiles_n = (p.N + kGTile - 1) / kGTile;
   const int c0 = blockIdx.x / tiles_n * kGTile, n0 = blockIdx.x % tiles_n * kGTile;
-  int first = p.offsets[e], end = p.offsets[e + 1];
-  const int each = ((end - first + splits - 1) / splits + kGStep - 1) / kGStep * kGStep;
-  first = static_cast<int>(min(static_cast<long long>(end), first + static_cast<long long>(split) * each));
-  end = static_cast<int>(min(static_cast<long long>(end), first + static_cast<long long>(each)));
   const T* X = static_cast<const T*>(p.A);
   const T* Y = static_cast<const T*>(p.W);
   const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) % sizeof(Packed<T, 4>)) == 0;
@@ -1074,21 +1086,209 @@ __global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_consta
       const int c = c0 + ty * 4 + i, n = n0 + tx * 4 + j;
       if (c >= p.C || n >= p.N) continue;
       const long long at = static_cast<long long>(c) * p.N + n;
-      if (splits > 1) partial[blockIdx.z * size + at] = acc[i][j];
+      if (length) partial[blockIdx.z * size + at] = acc[i][j];
       else static_cast<T*>(p.Out)[e * size + at] = from_f32<T>(acc[i][j]);
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) dweight_join_kernel(const float* partial, T* out, long long size, int splits) {
+// ------------------------------------------------------------------------------------------------
+// float32, where experts have rows enough: tiles of 128 x 64, 8 x 4 products a thread, two of them an instruction (fma.rn.f32x2, pairs of
+// rows).  A contraction step reads 12 floats a thread from shared memory for 32 products; 4 x 4 tiles read 8 for 16.
+// ------------------------------------------------------------------------------------------------
+constexpr int kWide = 128;
+
+struct alignas(16) WideTile {
+  float a[2][kGStep][kWide + 4], b[2][kGStep][kGTile + 4];
+};
+__device__ __forceinline__ unsigned long long pack(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void fma2(unsigned long long& c, unsigned long long a, unsigned long long b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+// acc[i][j]: rows 8 ty + 2 i and the next one, column 4 tx + j
+__device__ __forceinline__ void multiply_wide(const WideTile& s, int buf, int tx, int ty, unsigned long long (&acc)[4][4]) {
+#pragma unroll
+  for (int c = 0; c < kGStep; ++c) {
+    const ulonglong2 a0 = *reinterpret_cast<const ulonglong2*>(&s.a[buf][c][ty * 8]), a1 = *reinterpret_cast<const ulonglong2*>(&s.a[buf][c][ty * 8 + 4]);
+    const float4 b = *reinterpret_cast<const float4*>(&s.b[buf][c][tx * 4]);
+    const unsigned long long bb[4] = {pack(b.x, b.x), pack(b.y, b.y), pack(b.z, b.z), pack(b.w, b.w)}, aa[4] = {a0.x, a0.y, a1.x, a1.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fma2(acc[i][j], aa[i], bb[j]);
+  }
+}
+__device__ __forceinline__ float half_of(unsigned long long v, int high) { return __uint_as_float(static_cast<uint32_t>(high ? v >> 32 : v)); }
+
+__global__ void __launch_bounds__(256, 2) ragged_rows_f32_kernel(const __grid_constant__ RaggedParams p) {
+  __shared__ WideTile s;
+  __shared__ int s_expert, s_first, s_end;
+  __shared__ int src[kWide];
   pdl_wait();
+  const int tid = threadIdx.x;
+  if (tid < 32) locate_block(p.offsets, p.E, kWide, blockIdx.x, &s_expert, &s_first, &s_end);
+  zero_unrouted<float>(p, (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid, gridDim.x * gridDim.y * 256);
+  __syncthreads();
+  const int e = s_expert, first = s_first, end = s_end;
+  if (e < 0) return;
+  if (tid < kWide) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
+  const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
+  const int n0 = blockIdx.y * kGTile, tx = tid & 15, ty = tid >> 4;
+  const int lr = tid >> 2, lc = (tid & 3) * 4;
+  const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
+  const bool w_wide = p.w_row % 4 == 0 && p.w_expert % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) & 15u) == 0;
+  float va[2][4], vb[4];
+  auto fetch_w = [&](int c0) {
+    if (p.nc) load4<float>(W + (n0 + lr) * p.w_row + c0 + lc, n0 + lr < p.N ? p.C - c0 - lc : 0, w_wide, vb);
+    else load4<float>(W + (c0 + ty) * p.w_row + n0 + tx * 4, c0 + ty < p.C ? p.N - n0 - tx * 4 : 0, w_wide, vb);
+  };
+  fetch_w(0);
+  __syncthreads();
+  const int row[2] = {src[lr], src[lr + 64]};
+  const float* x[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) x[h] = static_cast<const float*>(p.A) + (row[h] < 0 ? 0 : row[h]) * p.a_row + lc;
+  auto fetch_x = [&](int c0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load4<float>(x[h] + c0, row[h] < 0 ? 0 : p.C - c0 - lc, a_wide, va[h]);
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.a[buf][lc + i][lr + 64 * h] = va[h][i];
+    if (p.nc) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.b[buf][lc + i][lr] = vb[i];
+    } else {
+      *reinterpret_cast<float4*>(&s.b[buf][ty][tx * 4]) = make_float4(vb[0], vb[1], vb[2], vb[3]);
+    }
+  };
+  unsigned long long acc[4][4] = {};
+  fetch_x(0);
+  put(0);
+  __syncthreads();
+  for (int c0 = 0, buf = 0; c0 < p.C; c0 += kGStep, buf ^= 1) {
+    const bool more = c0 + kGStep < p.C;
+    if (more) {
+      fetch_x(c0 + kGStep);
+      fetch_w(c0 + kGStep);
+    }
+    multiply_wide(s, buf, tx, ty, acc);
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  float* out = static_cast<float*>(p.Out);
+  const int left = p.N - n0 - tx * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int m = ty * 8 + i;
+    if (src[m] < 0 || left <= 0) continue;
+    float* o = out + static_cast<long long>(first + m) * p.N + n0 + tx * 4;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = half_of(acc[i / 2][j], i & 1);
+    if (p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) o[j] = v[j];
+    }
+  }
+}
+
+// See ragged_dweight_kernel, whose ranges these are.
+__global__ void __launch_bounds__(256, 2) ragged_dweight_f32_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
+  __shared__ DweightRange shared;
+  __shared__ WideTile s;
+  pdl_wait();
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const DweightRange range = range_of(p, length, &shared);
+  if (range.expert < 0) return;
+  const int e = range.expert, first = range.first, end = range.end;
+  const int tiles_n = (p.N + kGTile - 1) / kGTile;
+  const int c0 = blockIdx.x / tiles_n * kWide, n0 = blockIdx.x % tiles_n * kGTile;
+  const float* X = static_cast<const float*>(p.A) + c0;
+  const float* Y = static_cast<const float*>(p.W) + n0;
+  const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
+  const bool w_wide = p.w_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) & 15u) == 0;
+  // X: rows tid / 32 and 8 more of the step, 4 (tid mod 32) ..;  dY: row ty, 4 tx ..
+  const int xr = tid >> 5, xc = (tid & 31) * 4;
+  float va[2][4], vb[4];
+  int source[2];                               // slots (rows) of the step to come
+  auto look = [&](int r0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r0 + xr + 8 * h;
+      source[h] = r >= end ? -1 : p.slots ? p.slots[r] : r;
+    }
+  };
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long row = source[h] < 0 ? -1 : p.slots ? p.by_k.quotient(source[h]) : source[h];
+      load4<float>(X + (row < 0 ? 0 : row) * p.a_row + xc, row < 0 ? 0 : p.C - c0 - xc, a_wide, va[h]);
+    }
+    load4<float>(Y + (r0 + ty < end ? r0 + ty : 0) * p.w_row + tx * 4, r0 + ty < end ? p.N - n0 - tx * 4 : 0, w_wide, vb);
+    look(r0 + kGStep);
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(&s.a[buf][xr + 8 * h][xc]) = make_float4(va[h][0], va[h][1], va[h][2], va[h][3]);
+    *reinterpret_cast<float4*>(&s.b[buf][ty][tx * 4]) = make_float4(vb[0], vb[1], vb[2], vb[3]);
+  };
+  unsigned long long acc[4][4] = {};
+  if (first < end) {
+    look(first);
+    fetch(first);
+    put(0);
+  }
+  __syncthreads();
+  for (int r0 = first, buf = 0; r0 < end; r0 += kGStep, buf ^= 1) {
+    const bool more = r0 + kGStep < end;
+    if (more) fetch(r0 + kGStep);
+    multiply_wide(s, buf, tx, ty, acc);
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  const long long size = static_cast<long long>(p.C) * p.N;
+  float* out = length ? partial + blockIdx.z * size : static_cast<float*>(p.Out) + e * size;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c0 + ty * 8 + i, n = n0 + tx * 4 + j;
+      if (c < p.C && n < p.N) out[static_cast<long long>(c) * p.N + n] = half_of(acc[i / 2][j], i & 1);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) dweight_join_kernel(const int* offsets, const float* partial, T* out, long long size, int length) {
+  __shared__ int s_base, s_count;
+  pdl_wait();
+  const int expert = blockIdx.y, lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    int base = 0;
+    for (int e = lane; e < expert; e += 32) base += (offsets[e + 1] - offsets[e] + length - 1) / length;
+    base = __reduce_add_sync(kFull, base);
+    if (lane == 0) {
+      s_base = base;
+      s_count = (offsets[expert + 1] - offsets[expert] + length - 1) / length;
+    }
+  }
+  __syncthreads();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= size) return;
-  const float* p = partial + blockIdx.y * splits * size + i;
+  const float* p = partial + s_base * size + i;
+  const int n = s_count;
   float sum = 0.f;
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) sum += p[s * size];
-  out[blockIdx.y * size + i] = from_f32<T>(sum);
+  for (int r = 0; r < n; ++r) sum += p[r * size];
+  out[expert * size + i] = from_f32<T>(sum);
 }
 
 // Rows of 16-bit elements with another pitch; a thread writes eight elements.  Two matrices with one launch.
@@ -1281,7 +1481,16 @@ static long long blocks_bound(const RaggedParams& p, int rows) {
   return p.offsets ? p.rows / rows + (p.rows < p.E ? p.rows : p.E) : (p.rows + rows - 1) / rows;
 }
 
+// float32 products in wide tiles: where the mean expert fills most of one, and the features of X most of its rows
+static bool wide_rows(const RaggedParams& p) { return p.offsets && p.rows >= 96ll * p.E && p.C > 0; }
+static bool wide_dweight(const RaggedParams& p) { return p.C > 64; }
+
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st) {
+  if (dtype == EGS_F32 && wide_rows(p)) {
+    const dim3 grid(static_cast<unsigned>(blocks_bound(p, kWide)), (p.N + kGTile - 1) / kGTile);
+    count_launch();
+    return launch_kernel(ragged_rows_f32_kernel, grid, 256, 0, st, true, p);
+  }
   long long blocks = blocks_bound(p, kGTile);
   if (blocks < 1) blocks = 1;
   const dim3 grid(static_cast<unsigned>(blocks), (p.N + kGTile - 1) / kGTile);
@@ -1294,34 +1503,43 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
                  [&] { return go(ragged_rows_kernel<float, float>); });
 }
 
-// Ranges an expert's rows are cut into, so that there are four CTAs for an SM (at most 16 ranges, and none for short lists).
-static int dweight_splits(const RaggedParams& p) {
-  const long long tiles = static_cast<long long>((p.C + kGTile - 1) / kGTile) * ((p.N + kGTile - 1) / kGTile) * p.E;
-  const long long want = 4 * 148 / tiles, most = p.rows / (static_cast<long long>(p.E) * 4 * kGStep);
-  const long long n = want < most ? want : most;
-  return static_cast<int>(n < 1 ? 1 : n > 16 ? 16 : n);
+// Rows of a range, so that there are as many CTAs for an SM as it holds (two with wide tiles, four); 0: whole experts.
+struct DweightCut {
+  bool wide;
+  long long tiles, ranges;
+  int length;
+};
+static DweightCut dweight_cut(const RaggedParams& p, int dtype) {
+  DweightCut c{};
+  c.wide = dtype == EGS_F32 && wide_dweight(p);
+  const int tile = c.wide ? kWide : kGTile;
+  c.tiles = static_cast<long long>((p.C + tile - 1) / tile) * ((p.N + kGTile - 1) / kGTile);
+  const long long length = p.rows * c.tiles / (c.wide ? 2 * 148 : 4 * 148);
+  c.length = static_cast<int>(length < 4 * kGStep ? 4 * kGStep : (length + kGStep - 1) / kGStep * kGStep);
+  if (c.length >= p.rows || c.tiles * p.E >= 4 * 148) c.length = 0;
+  c.ranges = c.length ? p.rows / c.length + p.E : p.E;
+  return c;
 }
-size_t generic_dweight_workspace(const RaggedParams& p) {
-  const int splits = dweight_splits(p);
-  return splits == 1 ? 0 : static_cast<size_t>(p.E) * splits * p.C * p.N * sizeof(float);
+size_t generic_dweight_workspace(const RaggedParams& p, int dtype) {
+  const DweightCut c = dweight_cut(p, dtype);
+  return c.length ? static_cast<size_t>(c.ranges) * p.C * p.N * sizeof(float) : 0;
 }
 
 cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st) {
-  const int splits = dweight_splits(p);
+  const DweightCut c = dweight_cut(p, dtype);
   float* partial = static_cast<float*>(workspace);
-  const long long tiles = static_cast<long long>((p.C + kGTile - 1) / kGTile) * ((p.N + kGTile - 1) / kGTile);
-  const dim3 grid(static_cast<unsigned>(tiles), 1, p.E * splits);
+  const dim3 grid(static_cast<unsigned>(c.tiles), 1, static_cast<unsigned>(c.ranges));
   const long long size = static_cast<long long>(p.C) * p.N;
   auto go = [&](auto kernel, auto join, auto* out) {
     count_launch();
-    cudaError_t err = launch_kernel(kernel, grid, 256, 0, st, true, p, splits, partial);
-    if (err != cudaSuccess || splits == 1) return err;
+    cudaError_t err = launch_kernel(kernel, grid, 256, 0, st, true, p, c.length, partial);
+    if (err != cudaSuccess || c.length == 0) return err;
     count_launch();
-    return launch_kernel(join, dim3(static_cast<unsigned>((size + 255) / 256), p.E), 256, 0, st, true, partial, out, size, splits);
+    return launch_kernel(join, dim3(static_cast<unsigned>((size + 255) / 256), p.E), 256, 0, st, true, p.offsets, partial, out, size, c.length);
   };
   return by_type(dtype, [&] { return go(ragged_dweight_kernel<__half>, dweight_join_kernel<__half>, static_cast<__half*>(p.Out)); },
                  [&] { return go(ragged_dweight_kernel<__nv_bfloat16>, dweight_join_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(p.Out)); },
-                 [&] { return go(ragged_dweight_kernel<float>, dweight_join_kernel<float>, static_cast<float*>(p.Out)); });
+                 [&] { return go(c.wide ? ragged_dweight_f32_kernel : ragged_dweight_kernel<float>, dweight_join_kernel<float>, static_cast<float*>(p.Out)); });
 }
 
 }  // namespace egs

@@ -140,7 +140,7 @@ size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int 
   if (!valid_dtype(dtype) || check_ragged(dims) != EGS_OK || !valid_rows(rows)) return 0;
   if (dims->tokens * dims->k == 0 || dims->E * dims->C * dims->N == 0) return 0;
   const RaggedParams p = ragged(*dims, rows);
-  const size_t generic = generic_dweight_workspace(p);
+  const size_t generic = generic_dweight_workspace(p, dtype);
   if (dtype == EGS_F32) return generic;
   const size_t tensor = copy_bytes(a_rows_of(*dims, rows), dims->C) + copy_bytes(p.rows, dims->N) + ragged_dweight_workspace(p);
   return tensor > generic ? tensor : generic;

@@ -289,7 +289,7 @@ cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long lo
 // dtype EGS_I8: 8-bit operands with scales, products in out_dtype
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
-size_t generic_dweight_workspace(const RaggedParams& p);
+size_t generic_dweight_workspace(const RaggedParams& p, int dtype);
 // ... on the tensor cores (egs_ragged.cu): 16-bit or 8-bit operands whose rows begin on 16 bytes, C and N at least 1
 cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
