@@ -533,30 +533,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------
 // Weighted sum of a token's rows, float32 in the order of its choices, rounded once.
 // ------------------------------------------------------------------------------------------------
-template <typename T, int V> struct Vec;
-template <typename T> struct Vec<T, 1> {
-  static __device__ __forceinline__ void load(const T* p, float (&v)[1]) { v[0] = to_f32<T>(*p); }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { *p = from_f32<T>(v[0]); }
-};
-template <> struct Vec<float, 4> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-};
-template <typename T> struct Vec<T, 8> {
-  static __device__ __forceinline__ void load(const T* p, float (&v)[8]) {
-    const Packed<T, 8> x = *reinterpret_cast<const Packed<T, 8>*>(p);
+// V elements in one store
+template <typename T, int V> struct Vec {
+  static __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+    Packed<T, V> x;
+    T* h = reinterpret_cast<T*>(x.raw);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x.get(i);
-  }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[8]) {
-    uint4 x;
-    T* h = reinterpret_cast<T*>(&x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = x;
+    for (int i = 0; i < V; ++i) h[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<Packed<T, V>*>(p) = x;
   }
 };
 
@@ -579,15 +563,16 @@ __device__ __forceinline__ float weight_of(const CombineParams& p, long long slo
 
 // The rows lie anywhere, and what a thread may have in registers is not enough to keep the memory busy (eight loads a thread, 24 warps an
 // SM: 200 us for 131072 rows of 2048 bf16, 3.4 TB/s).  So vectors go to shared memory by cp.async, each to the thread that sums it: a warp
-// has 32 vectors of a token's columns at a time, four choices are a step, three steps are on their way, and positions are asked for a
+// has 512 bytes of a token's columns at a time, four choices are a step, three steps are on their way, and positions are asked for a
 // step before that.
 constexpr int kCombineStages = 4, kCombineAhead = kCombineStages - 1, kCombineWarps = 4, kCombineCtas = 148 * 6;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __grid_constant__ CombineParams p) {
   using P = Packed<T, V>;
-  static_assert(sizeof(P) == 16, "cp.async copies 16 bytes");
-  __shared__ P ring[kCombineStages][4][kCombineWarps * 32];
+  static_assert(sizeof(P) == 16 || sizeof(P) == 8 || sizeof(P) == 4, "what cp.async copies");
+  constexpr int U = 16 / sizeof(P);            // vectors of a lane, 32 V columns apart
+  __shared__ P ring[kCombineStages][4][U][kCombineWarps * 32];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -629,14 +614,19 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
     if (copy.item < items) {
       int block;
       place(copy, &block);
-      const int c = (block * 32 + lane) * V;
+      const int c = (block * 32 * U + lane) * V;
       have = __ballot_sync(kFull, pos >= 0) & 15u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = __shfl_sync(kFull, pos, j);
-        if (at >= 0 && c < p.N) {
-          const P* src = reinterpret_cast<const P*>(Y + static_cast<long long>(at) * p.N + c);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[stage][j][threadIdx.x]))), "l"(src) : "memory");
+        if (at < 0) continue;
+        const T* src = Y + static_cast<long long>(at) * p.N + c;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (c + u * 32 * V >= p.N) break;
+          const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(&ring[stage][j][u][threadIdx.x]));
+          if constexpr (sizeof(P) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src + u * 32 * V) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src + u * 32 * V), "n"(sizeof(P)) : "memory");
         }
       }
     }
@@ -647,7 +637,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
   };
 #pragma unroll
   for (int i = 0; i < kCombineAhead; ++i) present[i] = fetch(i);
-  float w = weight(use), sum[V];
+  float w = weight(use), sum[U][V];
   while (use.item < items) {
 #pragma unroll
     for (int stage = 0; stage < kCombineStages; ++stage) {
@@ -659,22 +649,29 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
       asm volatile("cp.async.wait_group %0;" ::"n"(kCombineAhead) : "memory");
       if (use.group == 0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] = 0.f;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int v = 0; v < V; ++v) sum[u][v] = 0.f;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float wj = __shfl_sync(kFull, w, j);
         if ((present[stage] >> j) & 1u) {
-          const P y = ring[stage][j][threadIdx.x];
 #pragma unroll
-          for (int v = 0; v < V; ++v) sum[v] = fmaf(wj, y.get(v), sum[v]);
+          for (int u = 0; u < U; ++u) {
+            const P y = ring[stage][j][u][threadIdx.x];
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[u][v] = fmaf(wj, y.get(v), sum[u][v]);
+          }
         }
       }
       if (use.group == groups - 1) {
         int block;
         const long long t = place(use, &block);
-        const int c = (block * 32 + lane) * V;
-        if (c < p.N) Vec<T, V>::store(static_cast<T*>(p.out) + t * p.N + c, sum);
+        const int c = (block * 32 * U + lane) * V;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c + u * 32 * V < p.N) Vec<T, V>::store(static_cast<T*>(p.out) + t * p.N + c + u * 32 * V, sum[u]);
       }
       use = after;
       w = w_next;
@@ -682,32 +679,32 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
   }
 }
 
-// Rows that do not begin on 16 bytes: a thread has a column of a token.
+// Rows that do not even begin on 4 bytes: 64 threads have a token, each every 64th column.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_columns_kernel(const __grid_constant__ CombineParams p) {
   pdl_wait();
   pdl_trigger();
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= static_cast<long long>(p.tokens) * p.N) return;
-  const long long t = i / p.N;
-  const int c = static_cast<int>(i - t * p.N);
-  const T* Y = static_cast<const T*>(p.Y) + c;
+  const long long t = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 64;
+  if (t >= p.tokens) return;
   const int* pos = p.position + t * p.k;
-  float sum = 0.f;
-  for (int j0 = 0; j0 < p.k; j0 += 4) {
-    int at[4];
-    float w[4], y[4];
+  T* out = static_cast<T*>(p.out) + t * p.N;
+  for (int c0 = threadIdx.x & 63; c0 < p.N; c0 += 256) {
+    float sum[4] = {};
+    for (int j = 0; j < p.k; ++j) {
+      const int at = pos[j];
+      if (at < 0) continue;
+      const float w = weight_of<T>(p, t * p.k + j);
+      const T* y = static_cast<const T*>(p.Y) + static_cast<long long>(at) * p.N;
+      float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) at[j] = j0 + j < p.k ? pos[j0 + j] : -1;
+      for (int i = 0; i < 4; ++i) v[i] = c0 + 64 * i < p.N ? to_f32<T>(y[c0 + 64 * i]) : 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      y[j] = at[j] >= 0 ? to_f32<T>(Y[static_cast<long long>(at[j]) * p.N]) : 0.f;
-      w[j] = at[j] >= 0 ? weight_of<T>(p, t * p.k + j0 + j) : 0.f;
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(w, v[i], sum[i]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum = fmaf(w[j], y[j], sum);
+    for (int i = 0; i < 4; ++i)
+      if (c0 + 64 * i < p.N) out[c0 + 64 * i] = from_f32<T>(sum[i]);
   }
-  static_cast<T*>(p.out)[i] = from_f32<T>(sum);
 }
 
 // A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
@@ -728,15 +725,17 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_cons
     const T* y = static_cast<const T*>(p.Y) + static_cast<long long>(at) * p.N;
     T* d = static_cast<T*>(p.out) + static_cast<long long>(at) * p.N;
     for (int c = lane; c < p.vecs; c += 32) {
-      float gv[V], yv[V];
-      Vec<T, V>::load(g + c * V, gv);
-      if (p.dweights) Vec<T, V>::load(y + c * V, yv);
+      const Packed<T, V> gp = *reinterpret_cast<const Packed<T, V>*>(g + c * V);
+      Packed<T, V> yp;
+      if (p.dweights) yp = *reinterpret_cast<const Packed<T, V>*>(y + c * V);
+      float x[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (p.dweights) dot = fmaf(gv[v], yv[v], dot);
-        gv[v] *= w;
+        x[v] = gp.get(v);
+        if (p.dweights) dot = fmaf(x[v], yp.get(v), dot);
+        x[v] *= w;
       }
-      Vec<T, V>::store(d + c * V, gv);
+      Vec<T, V>::store(d + c * V, x);
     }
   }
   if (at < 0) {
@@ -768,7 +767,7 @@ struct QuantizeParams {
 template <typename T, int V, int WARPS>
 __global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
   using P = Packed<T, V>;
-  constexpr int kKeep = V == 1 ? 16 : 8;
+  constexpr int kKeep = V <= 2 ? 16 : 8;
   __shared__ uint32_t found[4];
   pdl_wait();
   pdl_trigger();
@@ -836,7 +835,9 @@ __global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_cons
 #pragma unroll
       for (int v = 0; v < V; ++v) b[v] = 0u;
     }
-    if constexpr (V >= 4) {
+    if constexpr (V == 2) {
+      *reinterpret_cast<unsigned short*>(q + static_cast<long long>(i) * 2) = static_cast<unsigned short>(__byte_perm(b[0], b[1], 0x0040));
+    } else if constexpr (V >= 4) {
       uint32_t w[V / 4];
 #pragma unroll
       for (int v = 0; v < V / 4; ++v) w[v] = __byte_perm(__byte_perm(b[4 * v], b[4 * v + 1], 0x0040), __byte_perm(b[4 * v + 2], b[4 * v + 3], 0x0040), 0x5410);
@@ -858,35 +859,46 @@ __global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_cons
 // ------------------------------------------------------------------------------------------------
 constexpr int kGTile = 64, kGStep = 16;
 
-// The tile-th block of `rows` rows of an expert: its expert and first sorted row, by the first warp; -1 behind the last one.
-__device__ __forceinline__ void locate_block(const int* offsets, int E, int rows, int tile, int* expert, int* first, int* end) {
-  const int lane = threadIdx.x & 31;
-  int seen = 0, e_found = -1, first_found = 0, end_found = 0;
-  for (int e0 = 0; e0 < E && e_found < 0; e0 += 32) {
-    const int e = e0 + lane;
-    const int a = e < E ? offsets[e] : 0, b = e < E ? offsets[e + 1] : 0;
-    const int blocks = (b - a + rows - 1) / rows;
-    int incl = blocks;
+// The tile-th block of `rows` rows of an expert: its expert, its first sorted row and the expert's end; expert -1 behind the last block.  By all
+// threads, with a barrier at the end: the offsets come to shared memory together (warp by warp they were four dependent loads for 111
+// experts, more time than the eight steps of a tile behind them).
+struct Block {
+  int expert, first, end;
+  int offsets[EGS_MAX_EXPERTS + 1];
+};
+__device__ __forceinline__ void locate_block(const int* offsets, int E, int rows, int tile, Block* b) {
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) b->offsets[e] = offsets[e];
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int seen = 0, e_found = -1, first_found = 0, end_found = 0;
+    for (int e0 = 0; e0 < E && e_found < 0; e0 += 32) {
+      const int e = e0 + lane;
+      const int a = e < E ? b->offsets[e] : 0, end = e < E ? b->offsets[e + 1] : 0;
+      const int blocks = (end - a + rows - 1) / rows;
+      int incl = blocks;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(kFull, incl, o);
-      if (lane >= o) incl += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const unsigned hit = __ballot_sync(kFull, seen + incl > tile);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        const int f = a + (tile - seen - (incl - blocks)) * rows;
+        e_found = e0 + src;
+        first_found = __shfl_sync(kFull, f, src);
+        end_found = __shfl_sync(kFull, end, src);
+      }
+      seen += __shfl_sync(kFull, incl, 31);
     }
-    const unsigned hit = __ballot_sync(kFull, seen + incl > tile);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int f = a + (tile - seen - (incl - blocks)) * rows;
-      e_found = e0 + src;
-      first_found = __shfl_sync(kFull, f, src);
-      end_found = __shfl_sync(kFull, b, src);
+    if (lane == 0) {
+      b->expert = e_found;
+      b->first = first_found;
+      b->end = end_found;
     }
-    seen += __shfl_sync(kFull, incl, 31);
   }
-  if (lane == 0) {
-    *expert = e_found;
-    *first = first_found;
-    *end = end_found;
-  }
+  __syncthreads();
 }
 
 template <typename T> struct Acc { using type = float; };
@@ -914,10 +926,9 @@ __device__ __forceinline__ void load4(const T* p, int left, bool wide, typename 
 
 // Rows behind the last expert's: zeros.
 template <typename T>
-__device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int part, int parts) {
-  if (!p.offsets) return;
+__device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int routed, int part, int parts) {
   T* out = static_cast<T*>(p.Out);
-  const long long begin = static_cast<long long>(p.offsets[p.E]) * p.N, end = static_cast<long long>(p.rows) * p.N;
+  const long long begin = static_cast<long long>(routed) * p.N, end = static_cast<long long>(p.rows) * p.N;
   for (long long i = begin + part; i < end; i += parts) out[i] = from_f32<T>(0.f);
 }
 
@@ -942,20 +953,18 @@ template <typename T, typename OutT>
 __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant__ RaggedParams p) {
   using A = typename Acc<T>::type;
   __shared__ GenericTile<A> s;
-  __shared__ int s_expert, s_first, s_end;
+  __shared__ Block block;
   __shared__ int src[kGTile];
   pdl_wait();
   const int tid = threadIdx.x;
-  zero_unrouted<OutT>(p, (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid, gridDim.x * gridDim.y * 256);
+  int e = 0, first = blockIdx.x * kGTile, end = p.rows;
   if (p.offsets) {
-    if (tid < 32) locate_block(p.offsets, p.E, kGTile, blockIdx.x, &s_expert, &s_first, &s_end);
-  } else if (tid == 0) {
-    s_expert = 0;
-    s_first = blockIdx.x * kGTile;
-    s_end = p.rows;
+    locate_block(p.offsets, p.E, kGTile, blockIdx.x, &block);
+    e = block.expert;
+    first = block.first;
+    end = block.end;
+    zero_unrouted<OutT>(p, block.offsets[p.E], (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid, gridDim.x * gridDim.y * 256);
   }
-  __syncthreads();
-  const int e = s_expert, first = s_first, end = s_end;
   if (e < 0) return;
   if (tid < kGTile) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
   __syncthreads();
@@ -1022,21 +1031,18 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant_
 struct DweightRange {
   int expert, first, end;
 };
-__device__ __forceinline__ DweightRange range_of(const RaggedParams& p, int length, DweightRange* shared) {
+__device__ __forceinline__ DweightRange range_of(const RaggedParams& p, int length, Block* block) {
   if (length == 0) return {static_cast<int>(blockIdx.z), p.offsets[blockIdx.z], p.offsets[blockIdx.z + 1]};
-  if (threadIdx.x < 32) locate_block(p.offsets, p.E, length, blockIdx.z, &shared->expert, &shared->first, &shared->end);
-  __syncthreads();
-  DweightRange r = *shared;
-  r.end = min(r.end, r.first + length);
-  return r;
+  locate_block(p.offsets, p.E, length, blockIdx.z, block);
+  return {block->expert, block->first, min(block->end, block->first + length)};
 }
 template <typename T>
 __global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
-  __shared__ DweightRange shared;
+  __shared__ Block block;
   __shared__ GenericTile<float> s;
   pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const DweightRange range = range_of(p, length, &shared);
+  const DweightRange range = range_of(p, length, &block);
   if (range.expert < 0) return;
   const int e = range.expert, first = range.first, end = range.end;
   const int tiles_n = (p.N + kGTile - 1) / kGTile;
@@ -1092,10 +1098,11 @@ __global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------
-// float32, where experts have rows enough: tiles of 128 x 64, 8 x 4 products a thread, two of them an instruction (fma.rn.f32x2, pairs of
-// rows).  A contraction step reads 12 floats a thread from shared memory for 32 products; 4 x 4 tiles read 8 for 16.
+// float32, where experts have rows enough: tiles of 128 x 64, 8 x 8 products a thread, two of them an instruction (fma.rn.f32x2, pairs of
+// rows).  What bounds it is reads of shared memory, which cost by the bytes a lane asks for, equal addresses or not: 16 floats for 64
+// products are as long as the products (8 x 4 products a thread: 36 TFLOP/s, the load unit at 85 %).
 // ------------------------------------------------------------------------------------------------
-constexpr int kWide = 128;
+constexpr int kWide = 128, kWideThreads = 128;
 
 struct alignas(16) WideTile {
   float a[2][kGStep][kWide + 4], b[2][kGStep][kGTile + 4];
@@ -1108,66 +1115,97 @@ __device__ __forceinline__ unsigned long long pack(float a, float b) {
 __device__ __forceinline__ void fma2(unsigned long long& c, unsigned long long a, unsigned long long b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
 }
-// acc[i][j]: rows 8 ty + 2 i and the next one, column 4 tx + j
-__device__ __forceinline__ void multiply_wide(const WideTile& s, int buf, int tx, int ty, unsigned long long (&acc)[4][4]) {
+// acc[i][j]: rows 8 ty + 2 i and the next one; columns 4 tx + j and 32 + 4 tx + j - 4
+__device__ __forceinline__ void multiply_wide(const WideTile& s, int buf, int tx, int ty, unsigned long long (&acc)[4][8]) {
 #pragma unroll
   for (int c = 0; c < kGStep; ++c) {
     const ulonglong2 a0 = *reinterpret_cast<const ulonglong2*>(&s.a[buf][c][ty * 8]), a1 = *reinterpret_cast<const ulonglong2*>(&s.a[buf][c][ty * 8 + 4]);
-    const float4 b = *reinterpret_cast<const float4*>(&s.b[buf][c][tx * 4]);
-    const unsigned long long bb[4] = {pack(b.x, b.x), pack(b.y, b.y), pack(b.z, b.z), pack(b.w, b.w)}, aa[4] = {a0.x, a0.y, a1.x, a1.y};
+    const float4 b0 = *reinterpret_cast<const float4*>(&s.b[buf][c][tx * 4]), b1 = *reinterpret_cast<const float4*>(&s.b[buf][c][32 + tx * 4]);
+    const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+    const unsigned long long aa[4] = {a0.x, a0.y, a1.x, a1.y};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 8; ++j) {
+      const unsigned long long bb = pack(b[j], b[j]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fma2(acc[i][j], aa[i], bb[j]);
+      for (int i = 0; i < 4; ++i) fma2(acc[i][j], aa[i], bb);
+    }
   }
 }
 __device__ __forceinline__ float half_of(unsigned long long v, int high) { return __uint_as_float(static_cast<uint32_t>(high ? v >> 32 : v)); }
+// f(row of the tile, first of four columns, the four values)
+template <class F>
+__device__ __forceinline__ void each_of(const unsigned long long (&acc)[4][8], int tx, int ty, F&& f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = half_of(acc[i / 2][h * 4 + j], i & 1);
+      f(ty * 8 + i, h * 32 + tx * 4, v);
+    }
+}
+__device__ __forceinline__ void store_up_to4(float* to, int left, bool wide, const float (&v)[4]) {
+  if (wide && left >= 4) {
+    *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) to[j] = v[j];
+  }
+}
 
-__global__ void __launch_bounds__(256, 2) ragged_rows_f32_kernel(const __grid_constant__ RaggedParams p) {
+__global__ void __launch_bounds__(kWideThreads, 3) ragged_rows_f32_kernel(const __grid_constant__ RaggedParams p) {
   __shared__ WideTile s;
-  __shared__ int s_expert, s_first, s_end;
+  __shared__ Block block;
   __shared__ int src[kWide];
   pdl_wait();
   const int tid = threadIdx.x;
-  if (tid < 32) locate_block(p.offsets, p.E, kWide, blockIdx.x, &s_expert, &s_first, &s_end);
-  zero_unrouted<float>(p, (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid, gridDim.x * gridDim.y * 256);
-  __syncthreads();
-  const int e = s_expert, first = s_first, end = s_end;
+  locate_block(p.offsets, p.E, kWide, blockIdx.x, &block);
+  const int e = block.expert, first = block.first, end = block.end;
+  zero_unrouted<float>(p, block.offsets[p.E], (blockIdx.y * gridDim.x + blockIdx.x) * kWideThreads + tid, gridDim.x * gridDim.y * kWideThreads);
   if (e < 0) return;
-  if (tid < kWide) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
+  src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
   const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
-  const int n0 = blockIdx.y * kGTile, tx = tid & 15, ty = tid >> 4;
-  const int lr = tid >> 2, lc = (tid & 3) * 4;
+  const int n0 = blockIdx.y * kGTile, tx = tid & 7, ty = tid >> 3;
+  // X (and weights [E, N, C]): rows tid / 4 and every 32nd from there, elements 4 (tid mod 4) ..;  weights [E, C, N]: rows tid / 16 and 8 more
+  const int lr = tid >> 2, lc = (tid & 3) * 4, wr = tid >> 4, wc = (tid & 15) * 4;
   const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
   const bool w_wide = p.w_row % 4 == 0 && p.w_expert % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) & 15u) == 0;
-  float va[2][4], vb[4];
+  float va[4][4], vb[2][4];
   auto fetch_w = [&](int c0) {
-    if (p.nc) load4<float>(W + (n0 + lr) * p.w_row + c0 + lc, n0 + lr < p.N ? p.C - c0 - lc : 0, w_wide, vb);
-    else load4<float>(W + (c0 + ty) * p.w_row + n0 + tx * 4, c0 + ty < p.C ? p.N - n0 - tx * 4 : 0, w_wide, vb);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (p.nc) load4<float>(W + (n0 + lr + 32 * h) * p.w_row + c0 + lc, n0 + lr + 32 * h < p.N ? p.C - c0 - lc : 0, w_wide, vb[h]);
+      else load4<float>(W + (c0 + wr + 8 * h) * p.w_row + n0 + wc, c0 + wr + 8 * h < p.C ? p.N - n0 - wc : 0, w_wide, vb[h]);
+    }
   };
   fetch_w(0);
   __syncthreads();
-  const int row[2] = {src[lr], src[lr + 64]};
-  const float* x[2];
+  int row[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) x[h] = static_cast<const float*>(p.A) + (row[h] < 0 ? 0 : row[h]) * p.a_row + lc;
+  for (int h = 0; h < 4; ++h) row[h] = src[lr + 32 * h];
   auto fetch_x = [&](int c0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) load4<float>(x[h] + c0, row[h] < 0 ? 0 : p.C - c0 - lc, a_wide, va[h]);
+    for (int h = 0; h < 4; ++h)
+      load4<float>(static_cast<const float*>(p.A) + (row[h] < 0 ? 0 : row[h]) * p.a_row + c0 + lc, row[h] < 0 ? 0 : p.C - c0 - lc, a_wide, va[h]);
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 4; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s.a[buf][lc + i][lr + 64 * h] = va[h][i];
-    if (p.nc) {
+      for (int i = 0; i < 4; ++i) s.a[buf][lc + i][lr + 32 * h] = va[h][i];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s.b[buf][lc + i][lr] = vb[i];
-    } else {
-      *reinterpret_cast<float4*>(&s.b[buf][ty][tx * 4]) = make_float4(vb[0], vb[1], vb[2], vb[3]);
+    for (int h = 0; h < 2; ++h) {
+      if (p.nc) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.b[buf][lc + i][lr + 32 * h] = vb[h][i];
+      } else {
+        *reinterpret_cast<float4*>(&s.b[buf][wr + 8 * h][wc]) = make_float4(vb[h][0], vb[h][1], vb[h][2], vb[h][3]);
+      }
     }
   };
-  unsigned long long acc[4][4] = {};
+  unsigned long long acc[4][8] = {};
   fetch_x(0);
   put(0);
   __syncthreads();
@@ -1181,33 +1219,20 @@ __global__ void __launch_bounds__(256, 2) ragged_rows_f32_kernel(const __grid_co
     if (more) put(buf ^ 1);
     __syncthreads();
   }
-  float* out = static_cast<float*>(p.Out);
-  const int left = p.N - n0 - tx * 4;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int m = ty * 8 + i;
-    if (src[m] < 0 || left <= 0) continue;
-    float* o = out + static_cast<long long>(first + m) * p.N + n0 + tx * 4;
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = half_of(acc[i / 2][j], i & 1);
-    if (p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
-      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left) o[j] = v[j];
-    }
-  }
+  float* out = static_cast<float*>(p.Out) + static_cast<long long>(first) * p.N + n0;
+  const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
+  each_of(acc, tx, ty, [&](int m, int n, const float (&v)[4]) {
+    if (src[m] >= 0) store_up_to4(out + static_cast<long long>(m) * p.N + n, p.N - n0 - n, wide, v);
+  });
 }
 
 // See ragged_dweight_kernel, whose ranges these are.
-__global__ void __launch_bounds__(256, 2) ragged_dweight_f32_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
-  __shared__ DweightRange shared;
+__global__ void __launch_bounds__(kWideThreads, 3) ragged_dweight_f32_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
   __shared__ WideTile s;
+  __shared__ Block block;
   pdl_wait();
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const DweightRange range = range_of(p, length, &shared);
+  const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
+  const DweightRange range = range_of(p, length, &block);
   if (range.expert < 0) return;
   const int e = range.expert, first = range.first, end = range.end;
   const int tiles_n = (p.N + kGTile - 1) / kGTile;
@@ -1216,32 +1241,37 @@ __global__ void __launch_bounds__(256, 2) ragged_dweight_f32_kernel(const __grid
   const float* Y = static_cast<const float*>(p.W) + n0;
   const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
   const bool w_wide = p.w_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) & 15u) == 0;
-  // X: rows tid / 32 and 8 more of the step, 4 (tid mod 32) ..;  dY: row ty, 4 tx ..
-  const int xr = tid >> 5, xc = (tid & 31) * 4;
-  float va[2][4], vb[4];
-  int source[2];                               // slots (rows) of the step to come
+  // X: rows tid / 32 and every fourth from there, 4 (tid mod 32) ..;  dY: rows tid / 16 and 8 more, 4 (tid mod 16) ..
+  const int xr = tid >> 5, xc = (tid & 31) * 4, yr = tid >> 4, yc = (tid & 15) * 4;
+  float va[4][4], vb[2][4];
+  int source[4];                               // slots (rows) of the step to come
   auto look = [&](int r0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = r0 + xr + 8 * h;
+    for (int h = 0; h < 4; ++h) {
+      const int r = r0 + xr + 4 * h;
       source[h] = r >= end ? -1 : p.slots ? p.slots[r] : r;
     }
   };
   auto fetch = [&](int r0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 4; ++h) {
       const long long row = source[h] < 0 ? -1 : p.slots ? p.by_k.quotient(source[h]) : source[h];
       load4<float>(X + (row < 0 ? 0 : row) * p.a_row + xc, row < 0 ? 0 : p.C - c0 - xc, a_wide, va[h]);
     }
-    load4<float>(Y + (r0 + ty < end ? r0 + ty : 0) * p.w_row + tx * 4, r0 + ty < end ? p.N - n0 - tx * 4 : 0, w_wide, vb);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r0 + yr + 8 * h;
+      load4<float>(Y + (r < end ? r : 0) * p.w_row + yc, r < end ? p.N - n0 - yc : 0, w_wide, vb[h]);
+    }
     look(r0 + kGStep);
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(&s.a[buf][xr + 8 * h][xc]) = make_float4(va[h][0], va[h][1], va[h][2], va[h][3]);
-    *reinterpret_cast<float4*>(&s.b[buf][ty][tx * 4]) = make_float4(vb[0], vb[1], vb[2], vb[3]);
+    for (int h = 0; h < 4; ++h) *reinterpret_cast<float4*>(&s.a[buf][xr + 4 * h][xc]) = make_float4(va[h][0], va[h][1], va[h][2], va[h][3]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(&s.b[buf][yr + 8 * h][yc]) = make_float4(vb[h][0], vb[h][1], vb[h][2], vb[h][3]);
   };
-  unsigned long long acc[4][4] = {};
+  unsigned long long acc[4][8] = {};
   if (first < end) {
     look(first);
     fetch(first);
@@ -1257,13 +1287,10 @@ __global__ void __launch_bounds__(256, 2) ragged_dweight_f32_kernel(const __grid
   }
   const long long size = static_cast<long long>(p.C) * p.N;
   float* out = length ? partial + blockIdx.z * size : static_cast<float*>(p.Out) + e * size;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + ty * 8 + i, n = n0 + tx * 4 + j;
-      if (c < p.C && n < p.N) out[static_cast<long long>(c) * p.N + n] = half_of(acc[i / 2][j], i & 1);
-    }
+  const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  each_of(acc, tx, ty, [&](int m, int n, const float (&v)[4]) {
+    if (c0 + m < p.C) store_up_to4(out + static_cast<long long>(c0 + m) * p.N + n0 + n, p.N - n0 - n, wide, v);
+  });
 }
 
 template <typename T>
@@ -1351,34 +1378,46 @@ cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
     const long long slots = static_cast<long long>(p.tokens) * p.k;
     return launch_kernel(combine_backward_kernel<T, V>, static_cast<unsigned>((slots + 7) / 8), 256, 0, st, true, p);
   }
-  if constexpr (V == 1) {
-    const long long work = static_cast<long long>(p.tokens) * p.N;
-    return launch_kernel(combine_columns_kernel<T>, static_cast<unsigned>((work + 255) / 256), 256, 0, st, true, p);
+  if constexpr (sizeof(T) * V < 4) {
+    return launch_kernel(combine_columns_kernel<T>, (p.tokens + 3) / 4, 256, 0, st, true, p);
+  } else {
+    const int blocks = (p.vecs * static_cast<int>(sizeof(T) * V) + 511) / 512;
+    p.by_blocks = Div(blocks);
+    p.work = p.tokens * blocks;
+    const int ctas = (p.work + kCombineWarps - 1) / kCombineWarps;
+    return launch_kernel(combine_kernel<T, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
   }
-  const int blocks = (p.vecs + 31) / 32;
-  p.by_blocks = Div(blocks);
-  p.work = p.tokens * blocks;
-  const int ctas = (p.work + kCombineWarps - 1) / kCombineWarps;
-  if constexpr (V > 1) return launch_kernel(combine_kernel<T, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
-  return cudaErrorInvalidValue;
 }
+// The widest vectors that rows of N elements are whole numbers of and begin on.
 template <typename T>
 cudaError_t combine_t(CombineParams& p, bool backward, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  if (p.N % V == 0 && aligned(p.Y) && aligned(p.out) && aligned(p.dOut)) return combine_v<T, V>(p, backward, st);
+  auto fits = [&](int v) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.Y) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.dOut);
+    return p.N % v == 0 && all % (v * sizeof(T)) == 0;
+  };
+  if (fits(V)) return combine_v<T, V>(p, backward, st);
+  if (fits(V / 2)) return combine_v<T, V / 2>(p, backward, st);
+  if constexpr (V > 4) {
+    if (fits(V / 4)) return combine_v<T, V / 4>(p, backward, st);
+  }
   return combine_v<T, 1>(p, backward, st);
 }
 
 template <typename T, int V>
 cudaError_t quantize_v(const QuantizeParams& p, cudaStream_t st) {
-  if (p.C <= 32 * V * (V == 1 ? 16 : 8)) return launch_kernel(quantize_rows_kernel<T, V, 1>, (p.rows + 3) / 4, 128, 0, st, true, p);
+  if (p.C <= 32 * V * (V <= 2 ? 16 : 8)) return launch_kernel(quantize_rows_kernel<T, V, 1>, (p.rows + 3) / 4, 128, 0, st, true, p);
   return launch_kernel(quantize_rows_kernel<T, V, 4>, p.rows, 128, 0, st, true, p);
 }
 template <typename T>
 cudaError_t quantize_t(const QuantizeParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  if (p.C % V == 0 && p.x_stride % V == 0 && aligned(p.X) && p.q_stride % V == 0 && (reinterpret_cast<uintptr_t>(p.q) % V) == 0)
-    return quantize_v<T, V>(p, st);
+  auto fits = [&](int v) {
+    return p.C % v == 0 && p.x_stride % v == 0 && reinterpret_cast<uintptr_t>(p.X) % (v * sizeof(T)) == 0 && p.q_stride % v == 0 &&
+           reinterpret_cast<uintptr_t>(p.q) % v == 0;
+  };
+  if (fits(V)) return quantize_v<T, V>(p, st);
+  if (fits(2)) return quantize_v<T, 2>(p, st);
   return quantize_v<T, 1>(p, st);
 }
 
@@ -1489,7 +1528,7 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
   if (dtype == EGS_F32 && wide_rows(p)) {
     const dim3 grid(static_cast<unsigned>(blocks_bound(p, kWide)), (p.N + kGTile - 1) / kGTile);
     count_launch();
-    return launch_kernel(ragged_rows_f32_kernel, grid, 256, 0, st, true, p);
+    return launch_kernel(ragged_rows_f32_kernel, grid, kWideThreads, 0, st, true, p);
   }
   long long blocks = blocks_bound(p, kGTile);
   if (blocks < 1) blocks = 1;
@@ -1503,7 +1542,7 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
                  [&] { return go(ragged_rows_kernel<float, float>); });
 }
 
-// Rows of a range, so that there are as many CTAs for an SM as it holds (two with wide tiles, four); 0: whole experts.
+// Rows of a range, so that there are as many CTAs for an SM as it holds (three with wide tiles, four); 0: whole experts.
 struct DweightCut {
   bool wide;
   long long tiles, ranges;
@@ -1514,7 +1553,7 @@ static DweightCut dweight_cut(const RaggedParams& p, int dtype) {
   c.wide = dtype == EGS_F32 && wide_dweight(p);
   const int tile = c.wide ? kWide : kGTile;
   c.tiles = static_cast<long long>((p.C + tile - 1) / tile) * ((p.N + kGTile - 1) / kGTile);
-  const long long length = p.rows * c.tiles / (c.wide ? 2 * 148 : 4 * 148);
+  const long long length = p.rows * c.tiles / (c.wide ? 3 * 148 : 4 * 148);
   c.length = static_cast<int>(length < 4 * kGStep ? 4 * kGStep : (length + kGStep - 1) / kGStep * kGStep);
   if (c.length >= p.rows || c.tiles * p.E >= 4 * 148) c.length = 0;
   c.ranges = c.length ? p.rows / c.length + p.E : p.E;
@@ -1532,7 +1571,7 @@ cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, void* worksp
   const long long size = static_cast<long long>(p.C) * p.N;
   auto go = [&](auto kernel, auto join, auto* out) {
     count_launch();
-    cudaError_t err = launch_kernel(kernel, grid, 256, 0, st, true, p, c.length, partial);
+    cudaError_t err = launch_kernel(kernel, grid, c.wide ? kWideThreads : 256, 0, st, true, p, c.length, partial);
     if (err != cudaSuccess || c.length == 0) return err;
     count_launch();
     return launch_kernel(join, dim3(static_cast<unsigned>((size + 255) / 256), p.E), 256, 0, st, true, p.offsets, partial, out, size, c.length);

@@ -59,6 +59,7 @@ struct RaggedTiles {
   float* partial;              // ... sums of the ranges of cut experts [range, C, N]
   int gathers;                 // X's rows are gathered
   int vectors;                 // rows of the output begin on 16 bytes and are whole 16 bytes
+  int words;                   // ... on 4 bytes, whole 4 bytes (16-bit output)
   uint32_t table_bytes;        // of each of the two tables
   Div by_n, by_c;
 };
@@ -621,6 +622,15 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
               const int row = it * 4 + (lane >> 3);
               if (row < rows && col < bn) *reinterpret_cast<uint4*>(out + (row0 + row) * p.N + n0 + col) = y[it];
             }
+          } else if (q.words) {                      // rows of whole words: a row at a time
+            const int col = c + lane * 2;
+            OutT* o = out + row0 * p.N + n0 + col;
+#pragma unroll 8
+            for (int row = 0; row < min(rows, 32); ++row) {
+              uint32_t y;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(area + row * 128u + (static_cast<uint32_t>((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4u) : "memory");
+              if (col < bn) *reinterpret_cast<uint32_t*>(o + static_cast<long long>(row) * p.N) = y;
+            }
           } else {                                   // rows that begin anywhere: element by element along a row
             for (int row = 0; row < min(rows, 32); ++row)
 #pragma unroll
@@ -749,6 +759,7 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
   q.by_n = Div(q.tiles_n);
   q.gathers = p.slots != nullptr;
   q.vectors = (static_cast<long long>(p.N) * out_elem) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
+  q.words = p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 3u) == 0;
   const long long blocks = p.offsets ? p.rows / block + (p.rows < p.E ? p.rows : p.E) : (p.rows + block - 1) / block;
   const int columns = pair ? q.BN / 2 : q.BN;
   TensorMap3 maps[4];
@@ -802,6 +813,7 @@ cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void*
   q.partial = static_cast<float*>(workspace);
   q.gathers = p.slots != nullptr;
   q.vectors = (p.N * 2ll) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
+  q.words = p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 3u) == 0;
   TensorMap3 maps[4];
   if (!row_maps(&maps[0], &maps[1], p.A, 2, p.a_rows, p.C, p.a_row, 64) || !row_maps(&maps[2], &maps[3], p.W, 2, p.rows, p.N, p.w_row, 64))
     return cudaErrorInvalidValue;
