@@ -14,7 +14,7 @@ from expertscattergather_b200 import RoutedExperts, ops  # noqa: E402
 
 def main(steps=30, tokens=4096, E=32, I=256, J=128, top_k=4):
     torch.manual_seed(0)
-    layer = RoutedExperts(E, I, J, top_k, score="sigmoid", groups=4, top_groups=2).cuda().bfloat16()
+    layer = RoutedExperts(E, I, J, top_k, balance=True, score="sigmoid", groups=4, top_groups=2).cuda().bfloat16()
     target = torch.randn(I, I, device="cuda") / I ** 0.5
     opt = torch.optim.AdamW(layer.parameters(), lr=3e-3)
     first = last = None

@@ -124,7 +124,7 @@ int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, cons
   const cudaStream_t st = stream_of(cuda_stream);
   const bool able = device_is_sm100() && dtype != EGS_F32 && p.C > 0 && aligned16(X) && aligned16(W) && tiles_fit(p);
   if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
-  if (path == EGS_PATH_AUTO && p.C > 0 && few_rows_fit(p)) return done(launch_few_rows(p, dtype, dtype, st), "expert_matmul launch");
+  if (path == EGS_PATH_AUTO && p.C > 0 && few_rows_fit(p, dtype)) return done(launch_few_rows(p, dtype, dtype, st), "expert_matmul launch");
   if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_rows(p, dtype, dtype, st), "expert_matmul launch");
   const size_t need = egs_expert_matmul_workspace_bytes(dims, rows, w_layout, dtype);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
@@ -223,7 +223,7 @@ int egs_expert_matmul_int8(const int8_t* q, const float* q_scale, int64_t q_stri
   p.a_row = q_stride; p.w_row = w_stride; p.w_expert = w_stride * p.N;
   const bool able = device_is_sm100() && p.C > 0 && p.a_row % 16 == 0 && p.w_row % 16 == 0 && aligned16(q) && aligned16(Wq) && tiles_fit(p);
   if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
-  if (path == EGS_PATH_AUTO && p.C > 0 && few_rows_fit(p))
+  if (path == EGS_PATH_AUTO && p.C > 0 && few_rows_fit(p, EGS_I8))
     return done(launch_few_rows(p, EGS_I8, out_dtype, stream_of(cuda_stream)), "expert_matmul_int8 launch");
   if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_rows(p, EGS_I8, out_dtype, stream_of(cuda_stream)), "expert_matmul_int8 launch");
   return done(launch_ragged_rows_tensor(p, EGS_I8, out_dtype, stream_of(cuda_stream)), "expert_matmul_int8 launch");

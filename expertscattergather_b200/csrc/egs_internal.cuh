@@ -295,7 +295,7 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
 cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
 size_t ragged_dweight_workspace(const RaggedParams& p);
 // ... where experts have few rows (egs_few.cu): any type, width and alignment, C at least 1
-bool few_rows_fit(const RaggedParams& p);
+bool few_rows_fit(const RaggedParams& p, int dtype);
 cudaError_t launch_few_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 // Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; zeros behind a row's end); dst NULL: nothing.
 struct PadRows {

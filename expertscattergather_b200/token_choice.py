@@ -92,15 +92,23 @@ def combine(Y, weights, plan):
 
 
 class TokenRouter(nn.Module):
-    """``forward(x [..., I]) -> (weights [..., top_k], experts [..., top_k])``.  ``balance`` [E] is added to the keys of the choice;
-    :meth:`adjust` moves it against the load (it is a buffer: no gradient reaches it).  Options as for ``ops.route_tokens``."""
+    """``forward(x [..., I]) -> (weights [..., top_k], experts [..., top_k])``: the logits are ``x @ W.T`` (W [E, I]), options as for
+    ``ops.route_tokens``.  With ``balance`` there is a buffer of that name, [E] in float32 whatever the module's type, that is added to the
+    keys of the choice; no gradient reaches it, :meth:`adjust` moves it against the load."""
 
-    def __init__(self, E: int, I: int, top_k: int, **options):
+    def __init__(self, E: int, I: int, top_k: int, balance: bool = False, **options):
         super().__init__()
         self.E, self.I, self.top_k, self.options = E, I, top_k, options
         self.W = nn.Parameter(torch.empty(E, I))
-        self.register_buffer("balance", None)
+        self.register_buffer("balance", torch.zeros(E) if balance else None)
         nn.init.uniform_(self.W, -1 / math.sqrt(I), 1 / math.sqrt(I))
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = self.balance
+        super()._apply(fn, *args, **kwargs)
+        if kept is not None and self.balance.dtype != torch.float32:      # steps of an adjustment are too small for 16 bits
+            self.balance = kept.to(self.balance.device)
+        return self
 
     def forward(self, x):
         return route_tokens(F.linear(x, self.W), self.top_k, self.balance, **self.options)
@@ -108,15 +116,17 @@ class TokenRouter(nn.Module):
     @torch.no_grad()
     def adjust(self, plan: ops.ExpertPlan, rate: float) -> None:
         """Lowers the keys of experts with more rows than the mean by ``rate``, raises those of the others (no synchronisation)."""
-        counts = plan.counts().float()
         if self.balance is None:
-            self.balance = torch.zeros_like(counts)
+            raise RuntimeError("the router was made without balance")
+        counts = plan.counts().float()
         self.balance += rate * torch.sign(counts.mean() - counts)
 
 
 class RoutedExperts(nn.Module):
     """``out[t] = sum_j weights[t, j] * act(x[t] @ up[e]) @ down[e]`` over the experts ``e`` that the router chose for token t;
-    x [..., I] -> [..., I], up [E, I, J], down [E, J, I], act = SiLU.  No token is dropped, whatever the load of an expert."""
+    x [..., I] -> [..., I], up [E, I, J], down [E, J, I], act = SiLU.  No token is dropped, whatever the load of an expert.  Options go to
+    :class:`TokenRouter`.  In 16 bits the rows between the products are rounded to the tensors' type, each once, as the module's
+    activations are; sums over tokens, experts and features are float32."""
 
     def __init__(self, E: int, I: int, J: int, top_k: int, **options):
         super().__init__()

@@ -294,7 +294,7 @@ def test_plan_types_and_ids_out_of_range(cuda_device):
 
 # tokens, k, E, C, N: one token, tiles and parts of tiles, rows that start anywhere, wide and narrow widths, one expert
 MATMUL_SHAPES = [(1, 1, 1, 1, 1), (1, 8, 64, 256, 128), (2, 3, 5, 17, 9), (40, 2, 3, 64, 64), (129, 1, 1, 72, 136), (257, 2, 4, 128, 264), (500, 4, 13, 330, 201),
-                 (30, 4, 64, 264, 136), (25, 5, 64, 1001, 77), (20, 1, 64, 2600, 300), (1000, 3, 8, 1024, 256), (64, 2, 16, 2050, 70), (2000, 2, 4, 96, 520), (3, 2, 300, 40, 24), (700, 8, 40, 512, 16)]
+                 (6, 4, 64, 264, 136), (4, 5, 64, 1001, 77), (3, 8, 64, 2600, 300), (30, 4, 64, 264, 136), (25, 5, 64, 1001, 77), (20, 1, 64, 2600, 300), (1000, 3, 8, 1024, 256), (64, 2, 16, 2050, 70), (2000, 2, 4, 96, 520), (3, 2, 300, 40, 24), (700, 8, 40, 512, 16)]
 
 
 @pytest.mark.parametrize("tokens,k,E,C,N", MATMUL_SHAPES)
@@ -538,7 +538,7 @@ def test_quantize_rows_extremes(cuda_device):
 
 
 INT8_SHAPES = [(1, 1, 1, 1, 1), (1, 8, 64, 256, 128), (2, 3, 5, 17, 9), (129, 1, 1, 72, 136), (257, 2, 4, 128, 264), (500, 4, 13, 330, 201), (1000, 3, 8, 1024, 256), (3, 2, 300, 40, 24),
-               (30, 4, 64, 264, 136), (25, 5, 64, 1001, 77), (64, 2, 16, 4112, 70), (700, 8, 40, 512, 16)]
+               (6, 4, 64, 264, 136), (4, 5, 64, 1001, 77), (30, 4, 64, 264, 136), (25, 5, 64, 1001, 77), (64, 2, 16, 4112, 70), (700, 8, 40, 512, 16)]
 
 
 def int8_product(q, s, Wq, ws, ids, E, rows):
@@ -624,7 +624,7 @@ def test_layer_trains_and_is_served(cuda_device, dtype):
     g = gen(20)
     torch.manual_seed(2)
     E, I, J, k = 16, 128, 64, 4
-    layer = RoutedExperts(E, I, J, k, score="sigmoid", groups=4, top_groups=2).cuda().to(dtype)
+    layer = RoutedExperts(E, I, J, k, balance=True, score="sigmoid", groups=4, top_groups=2).cuda().to(dtype)
     x = randn(g, 5, 60, I, dtype=dtype)
     out = layer(x)
     w, ids = layer.router(x)
@@ -638,7 +638,10 @@ def test_layer_trains_and_is_served(cuda_device, dtype):
     assert out.shape == x.shape
     assert (out.view(-1, I).double() - ref).norm() <= (4 * HALF[dtype] + 1e-5) * ref.norm()
     layer.router.adjust(layer.plan, 0.01)
-    assert layer.router.balance.shape == (E,) and layer.router.balance.abs().max() <= 0.011
+    assert layer.router.balance.shape == (E,) and layer.router.balance.abs().max() <= 0.011 and layer.router.balance.dtype == torch.float32
+    other = RoutedExperts(E, I, J, k, balance=True).to(dtype)
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other.cuda().router.balance, layer.router.balance)
     out = layer(x)
     out.float().square().sum().backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() and p.grad.abs().sum() > 0 for p in layer.parameters())
