@@ -742,8 +742,33 @@ cudaError_t launch_by_pair(const RaggedParams& p, const RaggedTiles& q, bool pai
   return pair ? launch_ragged<T, OutT, WEIGHTS, true>(p, q, units, maps, st) : launch_ragged<T, OutT, WEIGHTS, false>(p, q, units, maps, st);
 }
 
-// Pairs where the experts have 256 rows and more in the mean: their last tiles are half empty otherwise.
-bool wants_pair(const RaggedParams& p) { return p.N > 64 && p.rows >= 256ll * p.E; }
+// The tile that takes the least time by this estimate, in clocks.  A step of a CTA costs its bytes at 60 a clock (what the L2 gives all SMs) or its
+// MMAs where they take longer; a read-out, under the next tile's steps all but the last, `fixed` and 3000 or 4500 for 256 columns.  blocks(rows of
+// a tile): tiles of one column.  The widest tile on pairs or single CTAs moves the fewest bytes; another has to be a tenth faster.
+struct TileChoice {
+  bool pair;
+  int BN;
+};
+template <class Blocks>
+TileChoice choose_tile(int N, long long steps, int elem, bool pairs, Blocks&& blocks) {
+  constexpr TileChoice kCandidates[] = {{true, 256}, {false, 256}, {true, 128}, {false, 128}, {false, 64}};
+  const double fixed = elem == 1 ? 2500 : 1500, wide = elem == 1 ? 4500 : 3000;
+  TileChoice best{false, 64};
+  double least = -1;
+  for (const TileChoice& c : kCandidates) {
+    if ((c.BN > 64 && N <= c.BN / 2) || (c.pair && !pairs)) continue;
+    const int workers = c.pair ? kSmCount / 2 : kSmCount;
+    const double bytes = kATile + b_tile_bytes(c.pair ? c.BN / 2 : c.BN), mma = elem * c.BN;
+    const double work = (bytes / 60 > mma ? bytes / 60 : mma) * steps, out = fixed + wide * c.BN / 256;
+    const long long units = static_cast<long long>(blocks(c.pair ? 256 : 128) * ((N + c.BN - 1) / c.BN));
+    const double time = static_cast<double>((units + workers - 1) / workers) * (work > out ? work : out) + out;
+    if (least < 0 || time < (best.BN == 256 && c.BN < 256 ? 0.9 : 1.0) * least) {
+      least = time;
+      best = c;
+    }
+  }
+  return best;
+}
 
 }  // namespace
 
@@ -751,10 +776,14 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
   const int elem = dtype == EGS_I8 ? 1 : 2;
   const int out_elem = out_dtype == EGS_F32 ? 4 : 2;
   RaggedTiles q{};
-  const bool pair = wants_pair(p);
-  q.BN = p.N > 128 ? 256 : p.N > 64 ? 128 : 64;
-  const int block = pair ? 256 : 128;
   q.steps = (p.C * elem + 127) / 128;
+  // (an expert's last block is half empty in the mean)
+  const int experts = p.offsets ? (p.rows < p.E ? p.rows : p.E) : 1;
+  const double each = static_cast<double>(p.rows) / experts;
+  const TileChoice tile = choose_tile(p.N, q.steps, elem, true, [&](int rows) { return experts * (each <= rows / 2 ? 1.0 : !p.offsets ? (p.rows + rows - 1) / rows : each / rows + 0.5); });
+  const bool pair = tile.pair;
+  q.BN = tile.BN;
+  const int block = pair ? 256 : 128;
   q.tiles_n = (p.N + q.BN - 1) / q.BN;
   q.by_n = Div(q.tiles_n);
   q.gathers = p.slots != nullptr;
@@ -792,9 +821,14 @@ struct DweightPlan {
 static DweightPlan dweight_plan(const RaggedParams& p) {
   DweightPlan d{};
   RaggedTiles& q = d.q;
-  d.pair = wants_pair(p) && p.C > 128;
+  // where experts are cut, tiles of any size fill the SMs
+  const int each = steps_of(p.rows) / p.E + 1;
+  const bool pairs = p.C > 128 && p.rows >= 256ll * p.E;
+  const TileChoice tile = each > kLeastRange ? TileChoice{pairs && p.N > 64, p.N > 128 ? 256 : p.N > 64 ? 128 : 64}
+                                             : choose_tile(p.N, each, 2, pairs, [&](int features) { return static_cast<double>((p.C + features - 1) / features) * p.E; });
+  d.pair = tile.pair;
   const int block = d.pair ? 256 : 128, workers = d.pair ? kSmCount / 2 : kSmCount;
-  q.BN = p.N > 128 ? 256 : p.N > 64 ? 128 : 64;
+  q.BN = tile.BN;
   q.tiles_n = (p.N + q.BN - 1) / q.BN;
   q.tiles_c = (p.C + block - 1) / block;
   const long long steps = steps_of(p.rows), share = steps * q.tiles_n * q.tiles_c / workers;
