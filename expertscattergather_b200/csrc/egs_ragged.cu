@@ -833,6 +833,22 @@ static DweightPlan dweight_plan(const RaggedParams& p) {
   q.tiles_c = (p.C + block - 1) / block;
   const long long steps = steps_of(p.rows), share = steps * q.tiles_n * q.tiles_c / workers;
   q.range_steps = static_cast<int>(share / 2 < kLeastRange ? kLeastRange : share / 2);
+  if (each > q.range_steps) {
+    // the mean expert is cut: into as many ranges as leave the last round of the CTAs fullest (one of 1024 steps and 20 tiles: 8 ranges are 2.2
+    // rounds, 7 are 1.9), each range costing what its sums take to be written and read
+    const double sums = 8.0 * p.E * p.C * p.N / 2.9e6;           // steps of 0.45 us at 6.5 TB/s
+    double least = -1;
+    for (int n = 1; n <= 16; ++n) {
+      const long long units = static_cast<long long>(p.E) * n * q.tiles_n * q.tiles_c;
+      const int steps_each = (each + n - 1) / n;
+      if (steps_each < kLeastRange) break;
+      const double time = static_cast<double>((units + workers - 1) / workers) * steps_each + (n > 1 ? n * sums : 0.0);
+      if (least < 0 || time < least) {
+        least = time;
+        q.range_steps = steps_each;
+      }
+    }
+  }
   d.most_partial = steps <= q.range_steps ? 0 : 2 * (steps / q.range_steps) + 2;
   q.most_ranges = static_cast<int>(p.E + d.most_partial);
   return d;
