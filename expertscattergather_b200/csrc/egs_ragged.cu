@@ -64,7 +64,10 @@ struct RaggedTiles {
   Div by_n, by_c;
 };
 
-__host__ __device__ constexpr uint32_t b_tile_bytes(int columns) { return static_cast<uint32_t>(columns) * 128u; }
+// The right operand's part of a stage: rows of 128 bytes for its columns (weights [E, N, C]), else column segments of 64.
+__host__ __device__ constexpr uint32_t b_tile_bytes(int columns, bool rows) {
+  return rows ? static_cast<uint32_t>(columns) * 128u : static_cast<uint32_t>((columns + 63) / 64) * kSegBytes;
+}
 
 template <bool PAIR>
 __device__ __forceinline__ void load_box(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
@@ -199,7 +202,7 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
   const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
   const bool leader = rank == 0;
   const int columns = PAIR ? q.BN / 2 : q.BN;        // of the right operand, staged by this CTA
-  const uint32_t stage_bytes = kATile + b_tile_bytes(columns);
+  const uint32_t stage_bytes = kATile + b_tile_bytes(columns, !WEIGHTS && p.nc);
   const uint32_t area0 = ring0 + static_cast<uint32_t>(q.stages) * stage_bytes;
   const uint32_t acc_cols = tmem_cols_for(q.BN);
   volatile uint32_t* abort_flag = &hdr->abort_flag;
@@ -716,7 +719,7 @@ template <typename T, typename OutT, bool WEIGHTS, bool PAIR>
 cudaError_t launch_ragged(const RaggedParams& p, RaggedTiles q, long long most_units, const TensorMap3 (&maps)[4], cudaStream_t st) {
   q.table_bytes = static_cast<uint32_t>((p.E + 1) * 4 + 15) & ~15u;
   const size_t before = (kRaggedHeader + q.table_bytes + (WEIGHTS ? range_bytes(q.most_ranges) : q.table_bytes) + 1023u) & ~static_cast<size_t>(1023);
-  const size_t stage = kATile + b_tile_bytes(PAIR ? q.BN / 2 : q.BN);
+  const size_t stage = kATile + b_tile_bytes(PAIR ? q.BN / 2 : q.BN, !WEIGHTS && p.nc);
   const size_t fixed = before + kReadWarps * (kReadArea + (sizeof(T) == 1 ? 128 : 0));
   q.stages = static_cast<int>((kRaggedSmem - fixed) / stage);
   if (q.stages > kMaxStages) q.stages = kMaxStages;
@@ -758,7 +761,7 @@ TileChoice choose_tile(int N, long long steps, int elem, bool pairs, Blocks&& bl
   for (const TileChoice& c : kCandidates) {
     if ((c.BN > 64 && N <= c.BN / 2) || (c.pair && !pairs)) continue;
     const int workers = c.pair ? kSmCount / 2 : kSmCount;
-    const double bytes = kATile + b_tile_bytes(c.pair ? c.BN / 2 : c.BN), mma = elem * c.BN;
+    const double bytes = kATile + b_tile_bytes(c.pair ? c.BN / 2 : c.BN, false), mma = elem * c.BN;
     const double work = (bytes / 60 > mma ? bytes / 60 : mma) * steps, out = fixed + wide * c.BN / 256;
     const long long units = static_cast<long long>(blocks(c.pair ? 256 : 128) * ((N + c.BN - 1) / c.BN));
     const double time = static_cast<double>((units + workers - 1) / workers) * (work > out ? work : out) + out;
@@ -768,6 +771,12 @@ TileChoice choose_tile(int N, long long steps, int elem, bool pairs, Blocks&& bl
     }
   }
   return best;
+}
+
+// Tiles of one width, no wider than they need be: 776 columns are four of 224, not of 256.  (tcgen05.mma: multiples of 16, of 32 for a pair.)
+int even_width(int N, int BN) {
+  const int tiles = (N + BN - 1) / BN;
+  return ((N + tiles - 1) / tiles + 31) / 32 * 32;
 }
 
 }  // namespace
@@ -782,7 +791,7 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
   const double each = static_cast<double>(p.rows) / experts;
   const TileChoice tile = choose_tile(p.N, q.steps, elem, true, [&](int rows) { return experts * (each <= rows / 2 ? 1.0 : !p.offsets ? (p.rows + rows - 1) / rows : each / rows + 0.5); });
   const bool pair = tile.pair;
-  q.BN = tile.BN;
+  q.BN = even_width(p.N, tile.BN);
   const int block = pair ? 256 : 128;
   q.tiles_n = (p.N + q.BN - 1) / q.BN;
   q.by_n = Div(q.tiles_n);
@@ -828,7 +837,7 @@ static DweightPlan dweight_plan(const RaggedParams& p) {
                                              : choose_tile(p.N, each, 2, pairs, [&](int features) { return static_cast<double>((p.C + features - 1) / features) * p.E; });
   d.pair = tile.pair;
   const int block = d.pair ? 256 : 128, workers = d.pair ? kSmCount / 2 : kSmCount;
-  q.BN = tile.BN;
+  q.BN = even_width(p.N, tile.BN);
   q.tiles_n = (p.N + q.BN - 1) / q.BN;
   q.tiles_c = (p.C + block - 1) / block;
   const long long steps = steps_of(p.rows), share = steps * q.tiles_n * q.tiles_c / workers;
