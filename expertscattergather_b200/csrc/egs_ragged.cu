@@ -13,6 +13,12 @@
 //   warp  5       tensor-memory allocation; four tcgen05.mma a stage, issued by the leader of a pair for both CTAs
 //   warps 8..15   read-out: tensor memory -> (scales) -> rows of the output; zeros for rows that belong to no expert
 //
+// What bounds it: long contractions the MMAs, in a long loop of them the power limit; short ones the read-out, which shares the shared memory with
+// the loads and the MMAs (65536 rows, 256 -> 1024: 43 us, 29 without read-out, 34 without its stores; stores straight from the registers, 32
+// bytes a lane, 49).  16-bit, 64 experts, 2048 -> 512: 65536 rows 110 us = 1.25 PFLOP/s, 131072 rows 210 us = 1.31, weight gradients 136 and
+// 240-260; 8-bit integers 60 and 105-130 us = 2.1-2.6 POP/s, 8192 rows of 4096 -> 4096 76-86 us = 3.2-3.6.
+// Brought to the L2 a tile ahead by bulk prefetches, gathered rows came later, not sooner (131072 rows: 220 -> 259 us).
+//
 // Experts differ in size, and a weight gradient's tile takes as long as its expert has rows.  So the contraction of a large expert is cut
 // into ranges of at most `range_steps` steps, about half of a CTA's share of all steps; tiles go out largest range first, every second
 // round of the CTAs backwards.  Ranges of a cut expert leave float32 sums in the workspace, which a second kernel adds in the order of
@@ -59,7 +65,7 @@ struct RaggedTiles {
   float* partial;              // ... sums of the ranges of cut experts [range, C, N]
   int gathers;                 // X's rows are gathered
   int vectors;                 // rows of the output begin on 16 bytes and are whole 16 bytes
-  int words;                   // ... on 4 bytes, whole 4 bytes (16-bit output)
+  int words;                   // ... on 4 bytes, whole 4 bytes (16-bit output): 1; on 8 and whole 8: 2
   uint32_t table_bytes;        // of each of the two tables
   Div by_n, by_c;
 };
@@ -625,6 +631,15 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
               const int row = it * 4 + (lane >> 3);
               if (row < rows && col < bn) *reinterpret_cast<uint4*>(out + (row0 + row) * p.N + n0 + col) = y[it];
             }
+          } else if (q.words == 2) {                 // rows of whole double words: two at a time
+            const int col = c + (lane & 15) * 4;
+#pragma unroll
+            for (int it = 0; it < 16; ++it) {
+              const int row = it * 2 + (lane >> 4);
+              uint2 y;
+              asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(y.x), "=r"(y.y) : "r"(area + row * 128u + (static_cast<uint32_t>(((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8u) : "memory");
+              if (row < rows && col < bn) *reinterpret_cast<uint2*>(out + (row0 + row) * p.N + n0 + col) = y;
+            }
           } else if (q.words) {                      // rows of whole words: a row at a time
             const int col = c + lane * 2;
             OutT* o = out + row0 * p.N + n0 + col;
@@ -773,6 +788,11 @@ TileChoice choose_tile(int N, long long steps, int elem, bool pairs, Blocks&& bl
   return best;
 }
 
+int words_of(const RaggedParams& p) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.Out);
+  return p.N % 4 == 0 && (at & 7u) == 0 ? 2 : p.N % 2 == 0 && (at & 3u) == 0 ? 1 : 0;
+}
+
 // Tiles of one width, no wider than they need be: 776 columns are four of 224, not of 256.  (tcgen05.mma: multiples of 16, of 32 for a pair.)
 int even_width(int N, int BN) {
   const int tiles = (N + BN - 1) / BN;
@@ -797,7 +817,7 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
   q.by_n = Div(q.tiles_n);
   q.gathers = p.slots != nullptr;
   q.vectors = (static_cast<long long>(p.N) * out_elem) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
-  q.words = p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 3u) == 0;
+  q.words = words_of(p);
   const long long blocks = p.offsets ? p.rows / block + (p.rows < p.E ? p.rows : p.E) : (p.rows + block - 1) / block;
   const int columns = pair ? q.BN / 2 : q.BN;
   TensorMap3 maps[4];
@@ -872,7 +892,7 @@ cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void*
   q.partial = static_cast<float*>(workspace);
   q.gathers = p.slots != nullptr;
   q.vectors = (p.N * 2ll) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
-  q.words = p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 3u) == 0;
+  q.words = words_of(p);
   TensorMap3 maps[4];
   if (!row_maps(&maps[0], &maps[1], p.A, 2, p.a_rows, p.C, p.a_row, 64) || !row_maps(&maps[2], &maps[3], p.W, 2, p.rows, p.N, p.w_row, 64))
     return cudaErrorInvalidValue;

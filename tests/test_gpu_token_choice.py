@@ -293,7 +293,7 @@ def test_plan_types_and_ids_out_of_range(cuda_device):
 # ---- products ------------------------------------------------------------------------------------------
 
 # tokens, k, E, C, N: one token, tiles and parts of tiles, rows that start anywhere, wide and narrow widths, one expert
-MATMUL_SHAPES = [(1, 1, 1, 1, 1), (1, 8, 64, 256, 128), (2, 3, 5, 17, 9), (40, 2, 3, 64, 64), (129, 1, 1, 72, 136), (257, 2, 4, 128, 264), (500, 4, 13, 330, 201),
+MATMUL_SHAPES = [(1, 1, 1, 1, 1), (1, 8, 64, 256, 128), (2, 3, 5, 17, 9), (40, 2, 3, 64, 64), (129, 1, 1, 72, 136), (150, 2, 4, 72, 100), (257, 2, 4, 128, 264), (500, 4, 13, 330, 201),
                  (6, 4, 64, 264, 136), (4, 5, 64, 1001, 77), (3, 8, 64, 2600, 300), (30, 4, 64, 264, 136), (25, 5, 64, 1001, 77), (20, 1, 64, 2600, 300), (1000, 3, 8, 1024, 256), (64, 2, 16, 2050, 70), (2000, 2, 4, 96, 520), (3, 2, 300, 40, 24), (700, 8, 40, 512, 16)]
 
 
@@ -537,7 +537,7 @@ def test_quantize_rows_extremes(cuda_device):
         ops.quantize_rows(wide.cpu())
 
 
-INT8_SHAPES = [(1, 1, 1, 1, 1), (1, 8, 64, 256, 128), (2, 3, 5, 17, 9), (129, 1, 1, 72, 136), (257, 2, 4, 128, 264), (500, 4, 13, 330, 201), (1000, 3, 8, 1024, 256), (3, 2, 300, 40, 24),
+INT8_SHAPES = [(1, 1, 1, 1, 1), (1, 8, 64, 256, 128), (2, 3, 5, 17, 9), (129, 1, 1, 72, 136), (150, 2, 4, 72, 100), (257, 2, 4, 128, 264), (500, 4, 13, 330, 201), (1000, 3, 8, 1024, 256), (3, 2, 300, 40, 24),
                (6, 4, 64, 264, 136), (4, 5, 64, 1001, 77), (30, 4, 64, 264, 136), (25, 5, 64, 1001, 77), (64, 2, 16, 4112, 70), (700, 8, 40, 512, 16)]
 
 
