@@ -1226,6 +1226,166 @@ __global__ void __launch_bounds__(kWideThreads, 3) ragged_rows_f32_kernel(const 
   });
 }
 
+// ------------------------------------------------------------------------------------------------
+// float32, where experts have a few rows or tens: tiles of 32 x 64, whose work is reading weights.  Three steps of 32 contraction elements are on
+// their way by cp.async.  G groups of 64 threads have a part of each step; their sums are joined, in order, at the end (one group alone, five
+// CTAs on an SM, left the load unit waiting: 64 experts of 32 rows, 1024 x 512, 114 us, two groups 82; 16 of 2048 x 1024, of which an SM has
+// fewer than two CTAs: 158, two 121, four 88 - but four 88 in the first case, where there are CTAs enough).  Threads have rows ty, ty + 4, ..
+// and as many of them as the block has.  Weights [E, N, C]: the two halves of a fma.rn.f32x2 are even and odd contraction elements, both operands
+// lie in pairs; [E, C, N]: neighbouring columns.  12 floats of shared memory for 32 products hold it to 36 TFLOP/s.
+// ------------------------------------------------------------------------------------------------
+constexpr int kMidRows = 32, kMidCols = 64, kMidStep = 32, kMidStages = 3;
+constexpr int kMidPitch = kMidStep + 4;      // floats: eight rows are in different banks
+constexpr int kMidStage = kMidRows * kMidPitch + (kMidCols * kMidPitch > kMidStep * (kMidCols + 4) ? kMidCols * kMidPitch : kMidStep * (kMidCols + 4));
+constexpr int kMidSmem = kMidStages * kMidStage * 4;
+
+// Four floats to shared memory, `left` of which exist; zeros for the others.
+__device__ __forceinline__ void copy4(float* dst, const float* src, int left, bool wide) {
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if (wide) {
+    const int bytes = left >= 4 ? 16 : left > 0 ? left * 4 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(bytes) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + i * 4), "l"(i < left ? src + i : src), "r"(i < left ? 4 : 0) : "memory");
+  }
+}
+
+template <bool NC, int G, int R>
+__device__ __forceinline__ void mid_tile(const RaggedParams& p, float* ring, const int* src, int e, int first, int rows) {
+  constexpr int kThreads = 64 * G;
+  constexpr int kX = R * 32 > kThreads ? R * 32 / kThreads : 1, kWn = kMidCols * 8 / kThreads, kWc = kMidStep * 16 / kThreads;
+  const int tid = threadIdx.x, tx = tid & 15, ty = (tid >> 4) & 3, group = tid >> 6, n0 = blockIdx.y * kMidCols;
+  const float* A = static_cast<const float*>(p.A);
+  const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
+  const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
+  const bool w_wide = p.w_row % 4 == 0 && p.w_expert % 4 == 0 && (reinterpret_cast<uintptr_t>(p.W) & 15u) == 0;
+  const int lr = tid >> 3, lc = (tid & 7) * 4;
+  const float* x[kX];
+#pragma unroll
+  for (int i = 0; i < kX; ++i) x[i] = lr + kThreads / 8 * i < rows ? A + src[lr + kThreads / 8 * i] * p.a_row : nullptr;
+  auto issue = [&](int step) {
+    const int c0 = step * kMidStep;
+    if (c0 < p.C) {
+      float* a = ring + step % kMidStages * kMidStage;
+      float* b = a + kMidRows * kMidPitch;
+#pragma unroll
+      for (int i = 0; i < kX; ++i)
+        if (x[i]) copy4(a + (lr + kThreads / 8 * i) * kMidPitch + lc, c0 + lc < p.C ? x[i] + c0 + lc : x[i], p.C - c0 - lc, a_wide);
+#pragma unroll
+      for (int i = 0; i < (NC ? kWn : kWc); ++i) {
+        if (NC) {
+          const int at = lr + kThreads / 8 * i;
+          const float* w = W + (n0 + at) * p.w_row;
+          if (n0 + at < p.N) copy4(b + at * kMidPitch + lc, c0 + lc < p.C ? w + c0 + lc : w, p.C - c0 - lc, w_wide);
+        } else {
+          const int at = (tid >> 4) + kThreads / 16 * i, c = c0 + at, n = n0 + tx * 4;
+          if (n < p.N) copy4(b + at * (kMidCols + 4) + tx * 4, c < p.C ? W + c * p.w_row + n : W, c < p.C ? p.N - n : 0, w_wide);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  unsigned long long acc[R][NC ? 4 : 2] = {};
+#pragma unroll
+  for (int s = 0; s < kMidStages - 1; ++s) issue(s);
+  for (int step = 0; step * kMidStep < p.C; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kMidStages - 2) : "memory");
+    __syncthreads();
+    issue(step + kMidStages - 1);
+    const int part = group * (kMidStep / G);
+    const float* a = ring + step % kMidStages * kMidStage + part;
+    const float* b = ring + step % kMidStages * kMidStage + kMidRows * kMidPitch + (NC ? part : part * (kMidCols + 4));
+#pragma unroll
+    for (int c = 0; c < kMidStep / G; c += 4) {
+      if (NC) {
+        ulonglong2 bv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const ulonglong2*>(b + (tx + 16 * j) * kMidPitch + c);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const ulonglong2 av = *reinterpret_cast<const ulonglong2*>(a + (ty + 4 * i) * kMidPitch + c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            fma2(acc[i][j], av.x, bv[j].x);
+            fma2(acc[i][j], av.y, bv[j].y);
+          }
+        }
+      } else {
+        float4 av[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) av[i] = *reinterpret_cast<const float4*>(a + (ty + 4 * i) * kMidPitch + c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(b + (c + k) * (kMidCols + 4) + tx * 4);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float v = k == 0 ? av[i].x : k == 1 ? av[i].y : k == 2 ? av[i].z : av[i].w;
+            fma2(acc[i][0], pack(v, v), bv.x);
+            fma2(acc[i][1], pack(v, v), bv.y);
+          }
+        }
+      }
+    }
+  }
+  float v[R][4];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[i][j] = NC ? half_of(acc[i][NC ? j : 0], 0) + half_of(acc[i][NC ? j : 0], 1) : half_of(acc[i][NC ? 0 : j / 2], j & 1);
+  __syncthreads();                             // (the ring has been read: the other groups' sums take its place)
+  float4* sums = reinterpret_cast<float4*>(ring) + (tid & 63);
+  if (group > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) sums[((group - 1) * R + i) * 64] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+  }
+  __syncthreads();
+  if (group > 0) return;
+  float* out = static_cast<float*>(p.Out) + static_cast<long long>(first) * p.N + n0;
+  const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 15u) == 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int m = ty + 4 * i;
+    if (m >= rows) break;
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+      const float4 x = sums[((g - 1) * R + i) * 64];
+      v[i][0] += x.x;
+      v[i][1] += x.y;
+      v[i][2] += x.z;
+      v[i][3] += x.w;
+    }
+    float* o = out + static_cast<long long>(m) * p.N;
+    if (NC) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + tx + 16 * j < p.N) o[tx + 16 * j] = v[i][j];
+    } else {
+      store_up_to4(o + tx * 4, p.N - n0 - tx * 4, wide, v[i]);
+    }
+  }
+}
+
+template <bool NC, int G>
+__global__ void __launch_bounds__(64 * G, G == 4 ? 2 : 4) ragged_rows_mid_kernel(const __grid_constant__ RaggedParams p) {
+  extern __shared__ __align__(16) float mid_ring[];
+  static_assert(sizeof(Block) <= kMidSmem, "the offsets, which give way to the ring");
+  __shared__ int src[kMidRows];
+  pdl_wait();
+  const int tid = threadIdx.x;
+  Block* block = reinterpret_cast<Block*>(mid_ring);
+  locate_block(p.offsets, p.E, kMidRows, blockIdx.x, block);
+  const int e = block->expert, first = block->first, rows = min(kMidRows, block->end - first), routed = block->offsets[p.E];
+  zero_unrouted<float>(p, routed, (blockIdx.y * gridDim.x + blockIdx.x) * (64 * G) + tid, gridDim.x * gridDim.y * (64 * G));
+  if (e < 0) return;
+  if (tid < rows) src[tid] = p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
+  __syncthreads();
+  if (rows <= 8) mid_tile<NC, G, 2>(p, mid_ring, src, e, first, rows);
+  else if (rows <= 16) mid_tile<NC, G, 4>(p, mid_ring, src, e, first, rows);
+  else mid_tile<NC, G, 8>(p, mid_ring, src, e, first, rows);
+}
+
 // See ragged_dweight_kernel, whose ranges these are.
 __global__ void __launch_bounds__(kWideThreads, 3) ragged_dweight_f32_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
   __shared__ WideTile s;
@@ -1520,8 +1680,13 @@ static long long blocks_bound(const RaggedParams& p, int rows) {
   return p.offsets ? p.rows / rows + (p.rows < p.E ? p.rows : p.E) : (p.rows + rows - 1) / rows;
 }
 
-// float32 products in wide tiles: where the mean expert fills most of one, and the features of X most of its rows
-static bool wide_rows(const RaggedParams& p) { return p.offsets && p.rows >= 96ll * p.E && p.C > 0; }
+// float32 products in wide tiles: where the mean expert fills most of one, and there are as many as the SMs hold (short contractions, which begin and
+// end most of their time: one for every SM).  128 rows for each of 64 experts, 1024 x 512, 512 wide tiles: 205 us, smaller ones 250;  of 16,
+// 2048 x 1024, 256 tiles: 301 and 254;  1024 rows of 32, 128 x 64, 256 tiles: 20 and 27;  384 of 8, 256 x 128, 48 tiles: 25 and 18.
+static bool wide_rows(const RaggedParams& p) {
+  return p.rows >= 96ll * p.E && p.rows / kWide * ((p.N + kGTile - 1) / kGTile) >= (p.C <= 256 ? 148 : 3 * 148);
+}
+// ... of a weight gradient: where the features of X fill most of its rows
 static bool wide_dweight(const RaggedParams& p) { return p.C > 64; }
 
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st) {
@@ -1529,6 +1694,14 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
     const dim3 grid(static_cast<unsigned>(blocks_bound(p, kWide)), (p.N + kGTile - 1) / kGTile);
     count_launch();
     return launch_kernel(ragged_rows_f32_kernel, grid, kWideThreads, 0, st, true, p);
+  }
+  if (dtype == EGS_F32) {
+    const dim3 grid(static_cast<unsigned>(blocks_bound(p, kMidRows)), (p.N + kMidCols - 1) / kMidCols);
+    count_launch();
+    auto go = [&](auto kernel, int threads) { return launch_kernel(kernel, grid, threads, kMidSmem, st, true, p); };
+    const long long mean = p.rows / kMidRows + p.E / 2, blocks = mean > p.E ? mean : p.rows < p.E ? p.rows : p.E;
+    if (blocks * grid.y < 3 * 148) return p.nc ? go(ragged_rows_mid_kernel<true, 4>, 256) : go(ragged_rows_mid_kernel<false, 4>, 256);
+    return p.nc ? go(ragged_rows_mid_kernel<true, 2>, 128) : go(ragged_rows_mid_kernel<false, 2>, 128);
   }
   long long blocks = blocks_bound(p, kGTile);
   if (blocks < 1) blocks = 1;
@@ -1538,8 +1711,7 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
   if (dtype == EGS_I8)
     return by_type(out_dtype, [&] { return go(ragged_rows_kernel<int8_t, __half>); }, [&] { return go(ragged_rows_kernel<int8_t, __nv_bfloat16>); },
                    [&] { return go(ragged_rows_kernel<int8_t, float>); });
-  return by_type(dtype, [&] { return go(ragged_rows_kernel<__half, __half>); }, [&] { return go(ragged_rows_kernel<__nv_bfloat16, __nv_bfloat16>); },
-                 [&] { return go(ragged_rows_kernel<float, float>); });
+  return dtype == EGS_F16 ? go(ragged_rows_kernel<__half, __half>) : go(ragged_rows_kernel<__nv_bfloat16, __nv_bfloat16>);
 }
 
 // Rows of a range, so that there are as many CTAs for an SM as it holds (three with wide tiles, four); 0: whole experts.

@@ -288,9 +288,10 @@ cudaError_t few_launch(const RaggedParams& p, int segments, cudaStream_t st) {
 // Up to how many rows this is faster than tiles, measured with 1 to 81 experts of 352 x 384 to 2048 x 2048 (whole calls, other kernels in brackets):
 // 16 bits, 64 experts of 1024 x 256: 32 rows 14 us (18), 128 rows 27 (20); of 2048 x 512: 8 rows 19 (24), 32 rows 29 (27), 64 rows 45 (32)
 // 8 bits, 2048 x 512: 32 rows 19 (21), 64 rows 25 (23);  one matrix of 2048 x 2048: 8 rows 16 (17), 16 rows 27 (17)
-// float32, whose tiles run on the CUDA cores, 2048 x 512: 512 rows 180 (284), 1024 rows 295 (285)
+// float32, 64 experts of 1024 x 512: 128 rows 50 (45), 256 rows 55 (45);  16 of 2048 x 1024: 32 rows 47 (57), 64 rows 50 (57);  8 of 256 x 128:
+// 16 rows 10 (12), 64 rows 14 (12)
 bool few_rows_fit(const RaggedParams& p, int dtype) {
-  if (dtype == EGS_F32) return p.rows <= 8ll * p.E || p.rows <= 32;
+  if (dtype == EGS_F32) return p.rows <= 3ll * p.E || p.rows <= 8;
   if (dtype == EGS_I8) return 4ll * p.rows <= 3 * p.E || p.rows <= 8;
   return 8ll * p.rows <= 3 * p.E || p.rows <= 4;
 }

@@ -321,6 +321,26 @@ def test_expert_matmul(cuda_device, tokens, k, E, C, N, dtype, kind):
     ops.check_status()
 
 
+# experts of 0, 1, 2 .. rows up to two blocks of 32 and one more; contractions around the steps of 32, rows that are no whole 16 bytes
+@pytest.mark.parametrize("C,N", [(1, 1), (3, 5), (31, 64), (32, 65), (33, 68), (64, 130), (100, 63), (132, 260), (1027, 66)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_experts_of_every_small_number_of_rows(cuda_device, C, N, dtype):
+    E, g = 66, gen(C * 1000 + N)
+    ids = torch.arange(E, device="cuda", dtype=torch.int32).repeat_interleave(torch.arange(E, device="cuda"))
+    ids = ids[torch.randperm(len(ids), device="cuda", generator=g)].view(-1, 1)
+    tokens = len(ids)
+    plan = ops.plan_experts(ids, E)
+    X, W = randn(g, tokens, C, dtype=dtype), randn(g, E, C, N, dtype=dtype)
+    for rows in ("tokens", "sorted"):
+        ref, size = orc.matmul(X, W, ids, E, rows)
+        for layout, w in (("cn", W), ("nc", W.transpose(1, 2).contiguous())):
+            close(ops.expert_matmul(X, w, plan, rows=rows, w_layout=layout), ref, size, C)
+    wide = randn(g, tokens, C + 5, dtype=dtype)                  # rows that begin anywhere
+    ref, size = orc.matmul(wide[:, 1:C + 1], W, ids, E, "tokens")
+    close(ops.expert_matmul(wide[:, 1:C + 1], W, plan), ref, size, C)
+    ops.check_status()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["one", "none"])
 def test_expert_products_of_one_expert_or_none(cuda_device, dtype, kind):
