@@ -1116,9 +1116,10 @@ __device__ __forceinline__ void fma2(unsigned long long& c, unsigned long long a
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
 }
 // acc[i][j]: rows 8 ty + 2 i and the next one; columns 4 tx + j and 32 + 4 tx + j - 4
+template <int STEP = kGStep>
 __device__ __forceinline__ void multiply_wide(const WideTile& s, int buf, int tx, int ty, unsigned long long (&acc)[4][8]) {
 #pragma unroll
-  for (int c = 0; c < kGStep; ++c) {
+  for (int c = 0; c < STEP; ++c) {
     const ulonglong2 a0 = *reinterpret_cast<const ulonglong2*>(&s.a[buf][c][ty * 8]), a1 = *reinterpret_cast<const ulonglong2*>(&s.a[buf][c][ty * 8 + 4]);
     const float4 b0 = *reinterpret_cast<const float4*>(&s.b[buf][c][tx * 4]), b1 = *reinterpret_cast<const float4*>(&s.b[buf][c][32 + tx * 4]);
     const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
@@ -1255,7 +1256,7 @@ __device__ __forceinline__ void copy4(float* dst, const float* src, int left, bo
 template <bool NC, int G, int R>
 __device__ __forceinline__ void mid_tile(const RaggedParams& p, float* ring, const int* src, int e, int first, int rows) {
   constexpr int kThreads = 64 * G;
-  constexpr int kX = R * 32 > kThreads ? R * 32 / kThreads : 1, kWn = kMidCols * 8 / kThreads, kWc = kMidStep * 16 / kThreads;
+  constexpr int kX = (R * 32 + kThreads - 1) / kThreads, kWn = kMidCols * 8 / kThreads, kWc = kMidStep * 16 / kThreads;
   const int tid = threadIdx.x, tx = tid & 15, ty = (tid >> 4) & 3, group = tid >> 6, n0 = blockIdx.y * kMidCols;
   const float* A = static_cast<const float*>(p.A);
   const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
@@ -1383,6 +1384,7 @@ __global__ void __launch_bounds__(64 * G, G == 4 ? 2 : 4) ragged_rows_mid_kernel
   __syncthreads();
   if (rows <= 8) mid_tile<NC, G, 2>(p, mid_ring, src, e, first, rows);
   else if (rows <= 16) mid_tile<NC, G, 4>(p, mid_ring, src, e, first, rows);
+  else if (rows <= 24) mid_tile<NC, G, 6>(p, mid_ring, src, e, first, rows);
   else mid_tile<NC, G, 8>(p, mid_ring, src, e, first, rows);
 }
 
@@ -1441,7 +1443,8 @@ __global__ void __launch_bounds__(kWideThreads, 3) ragged_dweight_f32_kernel(con
   for (int r0 = first, buf = 0; r0 < end; r0 += kGStep, buf ^= 1) {
     const bool more = r0 + kGStep < end;
     if (more) fetch(r0 + kGStep);
-    multiply_wide(s, buf, tx, ty, acc);
+    if (end - r0 > kGStep / 2) multiply_wide(s, buf, tx, ty, acc);
+    else multiply_wide<kGStep / 2>(s, buf, tx, ty, acc);       // (an expert of 17 rows)
     if (more) put(buf ^ 1);
     __syncthreads();
   }
