@@ -268,6 +268,23 @@ def test_plan(cuda_device, tokens, k, E, kind):
     ops.check_status()
 
 
+# one CTA, clusters of 2 to 16, more of a warp's slots, and stretches counted before; the last stretch with one slot, or whole
+@pytest.mark.parametrize("n", [2048, 2049, 4096, 4097, 6145, 8193, 16384, 16385, 31000, 32768, 32769, 65536, 65537, 131072, 131073, 600001])
+@pytest.mark.parametrize("E", [1, 64, 1024])
+def test_plan_of_every_size_of_cluster(cuda_device, n, E):
+    g = gen(n + E)
+    ids = (torch.rand(n, 1, device="cuda", generator=g) ** 2 * E).int().clamp_(max=E - 1)
+    ids[torch.rand(n, 1, device="cuda", generator=g) < 0.1] = -1
+    plan = ops.plan_experts(ids, E)
+    for mine, ref in zip((plan.offsets, plan.slots, plan.position), orc.plan(ids, E)):
+        assert torch.equal(mine.long(), ref)
+    ops.check_status()
+    ids[n - 1, 0] = E
+    assert ops.plan_experts(ids, E).position[n - 1].item() < 0
+    with pytest.raises(RuntimeError):
+        ops.check_status()
+
+
 def test_plan_types_and_ids_out_of_range(cuda_device):
     ids = torch.tensor([[0, 5], [2, -1], [4, 1]], device="cuda")
     for dtype in (torch.int64, torch.int16, torch.int8, torch.int32):
