@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_backward_kernel(const 
     if (p.sigmoid) {
       const float s = on ? sigmoid(x) : 0.f, slope = s / (1.f + expf(x));          // s (1 - s)
       if (p.renormalize) {
-        const float sum = warp_sum(s), back = sum == 0.f ? 0.f : warp_sum(g * s) / sum;
+        // (the weights, not their sum at the end: one choice has the weight 1 and the gradient 0, exactly)
+        const float sum = warp_sum(s), w = sum == 0.f ? 0.f : s / sum, back = warp_sum(g * w);
         d = sum == 0.f ? 0.f : (g - back) / sum * slope;
       } else {
         d = g * slope;

@@ -252,6 +252,16 @@ def test_route_refusals(cuda_device):
         ops.route_tokens_backward(w, x, ids.float())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_one_choice_of_weight_one_has_no_gradient(cuda_device, dtype, score):
+    g = gen(3)
+    x, d = randn(g, 4000, 24, dtype=dtype), torch.randn(4000, 1, device="cuda", generator=g)
+    w, ids = ops.route_tokens(x, 1, score=score, scale=2.5)
+    assert (w == 2.5).all() and torch.equal(ids[:, 0].long(), x.argmax(-1))
+    assert not ops.route_tokens_backward(d, x, ids, score=score, scale=2.5).any()
+
+
 # ---- the plan ------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("tokens,k,E", [(0, 2, 4), (1, 1, 1), (1, 8, 64), (5, 3, 7), (300, 4, 60), (1024, 2, 33), (4096, 8, 256), (700, 3, 1024), (40000, 4, 64), (150000, 8, 13)])
