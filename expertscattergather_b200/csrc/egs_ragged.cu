@@ -20,7 +20,8 @@
 // Brought to the L2 a tile ahead by bulk prefetches, gathered rows came later, not sooner (131072 rows: 220 -> 259 us).
 //
 // Experts differ in size, and a weight gradient's tile takes as long as its expert has rows.  So the contraction of a large expert is cut
-// into ranges of at most `range_steps` steps, about half of a CTA's share of all steps; tiles go out largest range first, every second
+// into ranges of at most `range_steps` steps, a CTA's share of all steps (half of it: more sums of ranges; 65536 rows of 64 experts, the
+// largest 4858, 1024 x 256: 71 us, the whole share 54); tiles go out largest range first, every second
 // round of the CTAs backwards.  Ranges of a cut expert leave float32 sums in the workspace, which a second kernel adds in the order of
 // the rows: the same bits in every run.  64 experts of 100 to 5000 rows, 1024 x 256 features: tiles in the experts' order, uncut, kept the
 // tensor cores of one pair busy for 61 % of 106 us and those of another for 4 %.
@@ -861,7 +862,7 @@ static DweightPlan dweight_plan(const RaggedParams& p) {
   q.tiles_n = (p.N + q.BN - 1) / q.BN;
   q.tiles_c = (p.C + block - 1) / block;
   const long long steps = steps_of(p.rows), share = steps * q.tiles_n * q.tiles_c / workers;
-  q.range_steps = static_cast<int>(share / 2 < kLeastRange ? kLeastRange : share / 2);
+  q.range_steps = static_cast<int>(share < kLeastRange ? kLeastRange : share < steps ? share : steps);
   if (each > q.range_steps) {
     // the mean expert is cut: into as many ranges as leave the last round of the CTAs fullest (one of 1024 steps and 20 tiles: 8 ranges are 2.2
     // rounds, 7 are 1.9), each range costing what its sums take to be written and read
