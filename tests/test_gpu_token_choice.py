@@ -724,6 +724,50 @@ def test_operators_on_another_stream_and_in_a_graph(cuda_device):
     assert torch.equal(out, served(x))
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+def test_rows_beyond_two_to_the_31_elements(cuda_device, dtype):
+    """70000 sorted rows of 32768: what lies at the end is compared (and a product whose weights end beyond 2^31 elements)."""
+    g = gen(31)
+    tokens, k, E, C, N = 17500, 4, 4, 64, 32768
+    ids = torch.arange(k, device="cuda", dtype=torch.int32).repeat(tokens, 1)
+    plan = ops.plan_experts(ids, E)
+    X, W, w = randn(g, tokens, C, dtype=dtype), randn(g, E, C, N, dtype=dtype), torch.rand(tokens, k, device="cuda", generator=g)
+    Y = ops.expert_matmul(X, W, plan)
+    end = slice(tokens - 200, None)
+    ref, size = X[end].double() @ W[3].double(), X[end].double().abs() @ W[3].double().abs()
+    close(Y[-200:], ref, size, C)
+    out = ops.combine(Y, w, plan)
+    rows = Y.view(k, tokens, N)[:, end].double()                      # (every expert has the tokens in order)
+    want = (rows * w[end].t().unsqueeze(-1).double()).sum(0)
+    close(out[end], want, (rows.abs() * w[end].t().unsqueeze(-1).double()).sum(0), k)
+    del rows, want
+    dY, dw = ops.combine_backward(out, Y, w, plan)
+    want = out[end].double() * w[end, 3:].double()
+    close(dY[-200:], want, want.abs(), 1)
+    want = (out[end].double() * Y[-200:].double()).sum(-1)
+    assert ((dw[end, 3].double() - want).abs() <= N * 2.0 ** -24 * (out[end].double() * Y[-200:].double()).abs().sum(-1)).all()
+    del out, Y
+    dX = ops.expert_matmul(dY, W, plan, rows="sorted", w_layout="nc")
+    close(dX[-200:], dY[-200:].double() @ W[3].double().t(), dY[-200:].double().abs() @ W[3].double().abs().t(), N)
+    dW = ops.expert_dweight(X, dY, plan)
+    last = dY[-tokens:, -300:].double()
+    close(dW[3][:, -300:], X.double().t() @ last, X.double().abs().t() @ last.abs(), tokens)
+    del dY, dX, dW, last
+    E, C, N = 40, 8192, 8192                                          # (one row, and 300 rows of the last expert)
+    W = torch.empty(E, C, N, device="cuda", dtype=dtype)
+    W[-1] = randn(g, C, N, dtype=dtype)
+    for n in (1, 300):
+        X = randn(g, n, C, dtype=dtype)
+        plan = ops.plan_experts(torch.full((n, 1), E - 1, device="cuda"), E)
+        for layout in ("cn", "nc"):
+            V = W[-1] if layout == "cn" else W[-1].t()
+            close(ops.expert_matmul(X, W, plan, w_layout=layout), X.double() @ V.double(), X.double().abs() @ V.double().abs(), C)
+    dW = ops.expert_dweight(X, X, plan)
+    close(dW[-1, -100:], X[:, -100:].double().t() @ X.double(), X[:, -100:].double().abs().t() @ X.double().abs(), 300)
+    assert not dW[:-1].any()
+    ops.check_status()
+
+
 def test_results_do_not_change_from_run_to_run(cuda_device):
     g = gen(22)
     ids = draw_experts(g, 3000, 4, 16, "skewed")
