@@ -45,10 +45,11 @@ def test_plan_entry_and_its_workspace():
     assert lib.egs_plan_experts(one, 4, 1025, one, one, one, None, 0, None, None) == LARGE
     assert lib.egs_plan_experts(one, 1 << 31, 4, one, one, one, None, 0, None, None) == LARGE
     assert lib.egs_plan_experts(None, 4, 4, one, one, one, None, 0, None, None) == BAD
-    assert lib.egs_plan_workspace_bytes(2048, 64) == 0 and lib.egs_plan_workspace_bytes(0, 64) == 0
-    need = lib.egs_plan_workspace_bytes(2049, 64)
-    assert need == 2 * 65 * 4
-    assert lib.egs_plan_experts(one, 2049, 64, one, one, one, one, need - 1, None, None) == WORKSPACE
+    for n in (0, 2048, 2049, 65536):                       # (one launch: nothing between two)
+        assert lib.egs_plan_workspace_bytes(n, 64) == 0
+    need = lib.egs_plan_workspace_bytes(65537, 64)
+    assert need == 33 * 65 * 4
+    assert lib.egs_plan_experts(one, 65537, 64, one, one, one, one, need - 1, None, None) == WORKSPACE
 
 
 def ragged(tokens=10, k=2, E=4, C=8, N=8):
