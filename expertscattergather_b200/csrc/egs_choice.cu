@@ -808,62 +808,46 @@ struct QuantizeParams {
   int rows, C;
 };
 
-template <typename T, int V, int WARPS>
-__global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
-  using P = Packed<T, V>;
-  constexpr int kKeep = V <= 2 ? 16 : 8;
-  __shared__ uint32_t found[4];
-  pdl_wait();
-  pdl_trigger();
-  constexpr int kRowThreads = WARPS * 32;
-  const int r = threadIdx.x / kRowThreads, i0 = threadIdx.x % kRowThreads;
-  const long long row = static_cast<long long>(blockIdx.x) * (128 / kRowThreads) + r;
-  const bool on = row < p.rows;
-  const P* x = reinterpret_cast<const P*>(static_cast<const T*>(p.X) + row * p.x_stride);
-  const int n = on ? p.C / V : 0;
-  P kept[kKeep];
-  // the magnitudes' bit patterns have their order, and a NaN lies above infinity; 16-bit ones are compared in pairs
-  uint32_t top = 0u;
-  auto look = [&](const P& y) {
-    if constexpr (sizeof(T) == 2 && V > 1) {
+// The largest magnitude so far, as a bit pattern: those have the magnitudes' order, and a NaN lies above infinity; 16-bit ones are compared
+// in pairs (top_of makes one float32 pattern of them).
+template <typename T, int V>
+__device__ __forceinline__ void look(uint32_t& top, const Packed<T, V>& y) {
+  if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-      for (int v = 0; v < V / 2; ++v) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(&y)[v] & 0x7fff7fffu);
-    } else {
+    for (int v = 0; v < V / 2; ++v) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(&y)[v] & 0x7fff7fffu);
+  } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(y.get(v)) & 0x7fffffffu);
-    }
-  };
-#pragma unroll
-  for (int j = 0; j < kKeep; ++j)
-    if (i0 + j * kRowThreads < n) kept[j] = x[i0 + j * kRowThreads];
-#pragma unroll
-  for (int j = 0; j < kKeep; ++j)
-    if (i0 + j * kRowThreads < n) look(kept[j]);
-  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) look(x[i]);
+    for (int v = 0; v < V; ++v) top = max(top, __float_as_uint(y.get(v)) & 0x7fffffffu);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ uint32_t top_of(uint32_t top) {
   if constexpr (sizeof(T) == 2 && V > 1) {
     const unsigned short h = static_cast<unsigned short>(max(top & 0xffffu, top >> 16));
     top = __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&h)));
   }
-  top = __reduce_max_sync(kFull, top);
-  if (WARPS > 1) {
-    if ((threadIdx.x & 31) == 0) found[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = max(top, found[w]);
+  return __reduce_max_sync(kFull, top);
+}
+
+// The nearest integers of x times a little less and a little more than 1 / scale: where they are one it is that of x / scale, else the
+// division decides (one vector in 500; with a division for each of 33 million elements the kernel took 44 us).  kRound: a float32 whose
+// unit is 1, so that adding it rounds to nearest even and leaves the integer in the low bits.  Scales below 2^-126 have no reciprocal to
+// work with.
+struct RowScale {
+  bool finite, divide;
+  float scale, less, more;
+  __device__ __forceinline__ explicit RowScale(uint32_t top) {
+    finite = top < 0x7f800000u;
+    scale = finite ? __uint_as_float(top) / 127.f : __uint_as_float(0x7fc00000u);
+    const bool zeros = !finite || scale == 0.f;
+    const float inverse = zeros ? 0.f : 1.f / scale;
+    less = inverse * (1.f - 0x1p-20f);
+    more = inverse * (1.f + 0x1p-20f);
+    divide = !zeros && !(inverse < 1e38f);
   }
-  const bool finite = top < 0x7f800000u;
-  const float scale = finite ? __uint_as_float(top) / 127.f : __uint_as_float(0x7fc00000u);
-  const bool zeros = !finite || scale == 0.f;
-  if (on && i0 == 0) p.scale[row] = scale;
-  // The nearest integers of x times a little less and a little more than 1 / scale: where they are one it is that of x / scale, else the
-  // division decides (one vector in 500; with a division for each of 33 million elements the kernel took 44 us).  kRound: a float32 whose
-  // unit is 1, so that adding it rounds to nearest even and leaves the integer in the low bits.  Scales below 2^-126 have no reciprocal to
-  // work with.
-  constexpr float kRound = 12582912.f;
-  const float inverse = zeros ? 0.f : 1.f / scale, less = inverse * (1.f - 0x1p-20f), more = inverse * (1.f + 0x1p-20f);
-  const bool divide = !zeros && !(inverse < 1e38f);
-  int8_t* q = p.q + row * p.q_stride;
-  auto put = [&](int i, const P& y) {
+  template <typename T, int V>
+  __device__ __forceinline__ void put(int8_t* q, const Packed<T, V>& y) const {
+    constexpr float kRound = 12582912.f;
     uint32_t b[V], apart = divide;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -880,21 +864,94 @@ __global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_cons
       for (int v = 0; v < V; ++v) b[v] = 0u;
     }
     if constexpr (V == 2) {
-      *reinterpret_cast<unsigned short*>(q + static_cast<long long>(i) * 2) = static_cast<unsigned short>(__byte_perm(b[0], b[1], 0x0040));
+      *reinterpret_cast<unsigned short*>(q) = static_cast<unsigned short>(__byte_perm(b[0], b[1], 0x0040));
     } else if constexpr (V >= 4) {
       uint32_t w[V / 4];
 #pragma unroll
       for (int v = 0; v < V / 4; ++v) w[v] = __byte_perm(__byte_perm(b[4 * v], b[4 * v + 1], 0x0040), __byte_perm(b[4 * v + 2], b[4 * v + 3], 0x0040), 0x5410);
-      if constexpr (V == 8) *reinterpret_cast<uint2*>(q + static_cast<long long>(i) * V) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(q + static_cast<long long>(i) * V) = w[0];
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(q) = w[0];
     } else {
-      q[i] = static_cast<int8_t>(b[0]);
+      q[0] = static_cast<int8_t>(b[0]);
     }
-  };
+  }
+};
+
+template <typename T, int V, int WARPS>
+__global__ void __launch_bounds__(128, 7) quantize_rows_kernel(const __grid_constant__ QuantizeParams p) {
+  using P = Packed<T, V>;
+  constexpr int kKeep = V <= 2 ? 16 : 8;
+  __shared__ uint32_t found[4];
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kRowThreads = WARPS * 32;
+  const int r = threadIdx.x / kRowThreads, i0 = threadIdx.x % kRowThreads;
+  const long long row = static_cast<long long>(blockIdx.x) * (128 / kRowThreads) + r;
+  const bool on = row < p.rows;
+  const P* x = reinterpret_cast<const P*>(static_cast<const T*>(p.X) + row * p.x_stride);
+  const int n = on ? p.C / V : 0;
+  P kept[kKeep];
+  uint32_t top = 0u;
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
-    if (i0 + j * kRowThreads < n) put(i0 + j * kRowThreads, kept[j]);
-  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) put(i, x[i]);
+    if (i0 + j * kRowThreads < n) kept[j] = x[i0 + j * kRowThreads];
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (i0 + j * kRowThreads < n) look(top, kept[j]);
+  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) look(top, x[i]);
+  top = top_of<T, V>(top);
+  if (WARPS > 1) {
+    if ((threadIdx.x & 31) == 0) found[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = max(top, found[w]);
+  }
+  const RowScale scale(top);
+  if (on && i0 == 0) p.scale[row] = scale.scale;
+  int8_t* q = p.q + row * p.q_stride;
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (i0 + j * kRowThreads < n) scale.put(q + (i0 + j * kRowThreads) * V, kept[j]);
+  for (int i = i0 + kKeep * kRowThreads; i < n; i += kRowThreads) scale.put(q + static_cast<long long>(i) * V, x[i]);
+}
+
+// Many short rows: a warp has one after the other, with the next one on its way to shared memory (each vector to the thread that reads it)
+// while it looks through this one.  bf16, this and the kernel above: 60000 rows of 128 23 and 31 us, 65536 of 512 35 and 41, 12000 of 128 8 and
+// 10; but 16384 of 2048 29 and 27, 8192 of 4096 37 and 31: longer rows leave too few warps on an SM.
+constexpr int kStreamWarps = 4, kStreamCtas = 148 * 12, kStreamSmem = kStreamWarps * 2 * 2048;
+template <typename T>
+__global__ void __launch_bounds__(kStreamWarps * 32) quantize_stream_kernel(const __grid_constant__ QuantizeParams p) {
+  constexpr int V = 16 / sizeof(T);
+  using P = Packed<T, V>;
+  extern __shared__ __align__(16) unsigned char stream_smem[];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = p.C / V;
+  P* ring = reinterpret_cast<P*>(stream_smem) + warp * 2 * n;
+  const int stride = gridDim.x * kStreamWarps;
+  auto ask = [&](long long row, int half) {
+    if (row < p.rows) {
+      const P* x = reinterpret_cast<const P*>(static_cast<const T*>(p.X) + row * p.x_stride);
+      for (int i = lane; i < n; i += 32)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(ring + half * n + i))), "l"(x + i) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  long long row = blockIdx.x * kStreamWarps + warp;
+  ask(row, 0);
+  for (int half = 0; row < p.rows; row += stride, half ^= 1) {
+    ask(row + stride, half ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const P* x = ring + half * n;
+    uint32_t top = 0u;
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) look(top, x[i]);
+    const RowScale scale(top_of<T, V>(top));
+    if (lane == 0) p.scale[row] = scale.scale;
+    int8_t* q = p.q + row * p.q_stride;
+#pragma unroll 2
+    for (int i = lane; i < n; i += 32) scale.put(q + i * V, x[i]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1623,7 +1680,11 @@ cudaError_t quantize_t(const QuantizeParams& p, cudaStream_t st) {
     return p.C % v == 0 && p.x_stride % v == 0 && reinterpret_cast<uintptr_t>(p.X) % (v * sizeof(T)) == 0 && p.q_stride % v == 0 &&
            reinterpret_cast<uintptr_t>(p.q) % v == 0;
   };
-  if (fits(V)) return quantize_v<T, V>(p, st);
+  if (fits(V)) {
+    const size_t smem = static_cast<size_t>(kStreamWarps) * 2 * p.C * sizeof(T);
+    if (smem <= kStreamSmem && p.rows > kStreamCtas * kStreamWarps) return launch_kernel(quantize_stream_kernel<T>, kStreamCtas, kStreamWarps * 32, smem, st, true, p);
+    return quantize_v<T, V>(p, st);
+  }
   if (fits(2)) return quantize_v<T, 2>(p, st);
   return quantize_v<T, 1>(p, st);
 }

@@ -562,6 +562,24 @@ def test_quantize_rows(cuda_device, rows, C, dtype):
     assert ((s.double() - exact_s).abs() <= U * exact_s).all()
 
 
+# rows enough for warps that have one after the other (beside: too few, rows that are no whole 16 bytes, rows too long)
+@pytest.mark.parametrize("rows,C", [(7104, 64), (7105, 8), (7300, 520), (15000, 1024), (30000, 136), (8000, 132), (7200, 1032), (14209, 512)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_many_rows(cuda_device, rows, C, dtype):
+    g = gen(rows)
+    X = randn(g, rows, C + 16, dtype=dtype)[:, :C]                    # (rows with a pitch)
+    X[5], X[rows - 2, C - 1], X[rows - 1] = 0, float("inf"), X[rows - 1] * 1e-3
+    X[rows // 2, 0] = float("nan")
+    q, s = ops.quantize_rows(X)
+    fine = torch.isfinite(X).all(-1)
+    assert torch.isnan(s[~fine]).all() and not q[~fine].any() and int((~fine).sum()) == 2
+    X, q, s = X[fine], q[fine], s[fine]
+    assert torch.equal(s, (X.double().abs().amax(-1) / 127).float())
+    want = torch.where(s.unsqueeze(-1) == 0, torch.zeros_like(X, dtype=torch.float32), X.float() / s.unsqueeze(-1)).round()
+    assert torch.equal(q.float(), want)
+    ops.check_status()
+
+
 def test_quantize_rows_extremes(cuda_device):
     X = torch.zeros(6, 40, device="cuda")
     X[0, 3] = float("inf")
