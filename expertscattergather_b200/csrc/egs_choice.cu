@@ -598,6 +598,7 @@ struct CombineParams {
   int tokens, k, N, vecs;  // vecs: vectors of a row
   int w_f32;               // weights (and their gradient) in float32, else in the rows' type
   Div by_blocks;           // forward: blocks of 32 vectors of a row
+  Div by_k;                // backward
   int work;                // forward: tokens * blocks
 };
 template <typename T>
@@ -792,6 +793,61 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_cons
   if (lane == 0) {
     if (p.w_f32) static_cast<float*>(p.dweights)[slot] = dot;
     else static_cast<T*>(p.dweights)[slot] = from_f32<T>(dot);
+  }
+}
+
+// ... of rows of at most 16 vectors: 2^lanes_log2 lanes have a slot, one vector each, and slot after slot; the two rows of the next one are on
+// their way and its successor's place is asked for.  bf16, this and a warp for every slot: 240000 slots of 32 16 and 64 us, 32768 of 64 10 and
+// 14 to 16, 24000 of 128 11 and 12; with all 32 lanes 65536 of 256 27 and 27, 171352 of 152 56 and 53.
+constexpr int kNarrowCtas = 148 * 5;
+template <typename T, int V>
+__global__ void __launch_bounds__(256, 5) combine_backward_narrow_kernel(const __grid_constant__ CombineParams p, int lanes_log2) {
+  using P = Packed<T, V>;
+  pdl_wait();
+  const int lane = threadIdx.x & 31, lanes = 1 << lanes_log2, c = lane & (lanes - 1), each = 32 >> lanes_log2;
+  const long long total = static_cast<long long>(p.tokens) * p.k, stride = static_cast<long long>(gridDim.x) * 8 * each;
+  const P* G = static_cast<const P*>(p.dOut) + c;
+  const P* Y = static_cast<const P*>(p.Y) + c;
+  auto place = [&](long long slot) { return slot < total ? p.position[slot] : -1; };
+  struct Held {
+    P g, y;
+    float w;
+  };
+  auto fetch = [&](Held& h, long long slot, int at) {
+    if (at < 0) return;
+    h.w = weight_of<T>(p, slot);
+    if (c >= p.vecs) return;
+    h.g = G[static_cast<long long>(p.by_k.quotient(static_cast<int>(slot))) * p.vecs];
+    if (p.dweights) h.y = Y[static_cast<long long>(at) * p.vecs];
+  };
+  long long slot = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * each + (lane >> lanes_log2);
+  int at = place(slot), at_next = place(slot + stride);
+  Held now, next;
+  fetch(now, slot, at);
+  for (long long first = slot - (lane >> lanes_log2); first < total; first += stride, slot += stride) {
+    fetch(next, slot + stride, at_next);
+    const int at_after = place(slot + 2 * stride);
+    float dot = 0.f;
+    if (slot < total && c < p.vecs) {
+      float x[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        x[v] = at >= 0 ? now.g.get(v) : 0.f;
+        if (p.dweights && at >= 0) dot = fmaf(x[v], now.y.get(v), dot);
+        x[v] = at >= 0 ? x[v] * now.w : 0.f;
+      }
+      Vec<T, V>::store(static_cast<T*>(p.out) + (static_cast<long long>(at >= 0 ? at : ~at) * p.vecs + c) * V, x);
+    }
+    if (p.dweights) {
+      for (int o = lanes >> 1; o; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
+      if (c == 0 && slot < total) {
+        if (p.w_f32) static_cast<float*>(p.dweights)[slot] = dot;
+        else static_cast<T*>(p.dweights)[slot] = from_f32<T>(dot);
+      }
+    }
+    at = at_next;
+    at_next = at_after;
+    now = next;
   }
 }
 
@@ -1640,6 +1696,13 @@ cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
   p.vecs = p.N / V;
   if (backward) {
     const long long slots = static_cast<long long>(p.tokens) * p.k;
+    if (p.vecs <= 16) {
+      int lanes_log2 = 2;
+      while ((1 << lanes_log2) < p.vecs) ++lanes_log2;
+      const long long ctas = ((slots << lanes_log2) + 255) / 256;
+      p.by_k = Div(p.k);
+      return launch_kernel(combine_backward_narrow_kernel<T, V>, static_cast<unsigned>(ctas < kNarrowCtas ? ctas : kNarrowCtas), 256, 0, st, true, p, lanes_log2);
+    }
     return launch_kernel(combine_backward_kernel<T, V>, static_cast<unsigned>((slots + 7) / 8), 256, 0, st, true, p);
   }
   if constexpr (sizeof(T) * V < 4) {

@@ -495,6 +495,14 @@ def test_combine(cuda_device, tokens, k, N, dtype, kind):
         assert dw.dtype == w.dtype
 
 
+# short rows, slots enough for warps that have several one after the other; 4, 8 and 16 lanes to a slot
+@pytest.mark.parametrize("tokens,k,N", [(20000, 4, 8), (30001, 3, 32), (50001, 2, 1), (16000, 4, 60), (9001, 4, 128), (24001, 2, 17)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["skewed", "holes"])
+def test_combine_of_many_short_rows(cuda_device, tokens, k, N, dtype, kind):
+    test_combine(cuda_device, tokens, k, N, dtype, kind)
+
+
 def test_layer_gradients(cuda_device):
     """Products and combine through autograd, float32: the formulas' gradients in float64 (by autograd of the definition)."""
     g = gen(11)
