@@ -752,6 +752,47 @@ __global__ void __launch_bounds__(256) combine_columns_kernel(const __grid_const
   }
 }
 
+// Rows of at most 32 vectors: 2^lanes_log2 threads have a token, one vector each; four rows are on their way, and the next four places.  bf16,
+// this and the kernel above, which leaves lanes without work: 32768 tokens of eight rows of 64 16 and 33 us, of one row 10 and 18; 21419 of eight
+// rows of 152 25 and 27; from 64 vectors on no faster (32768 of four rows of 512: 43 and 42).
+template <typename T, int V>
+__global__ void __launch_bounds__(256) combine_narrow_kernel(const __grid_constant__ CombineParams p, int lanes_log2) {
+  using P = Packed<T, V>;
+  pdl_wait();
+  pdl_trigger();
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, t = i >> lanes_log2;
+  const int c = static_cast<int>(i) & ((1 << lanes_log2) - 1);
+  if (t >= p.tokens || c >= p.vecs) return;
+  const long long slot = t * p.k;
+  const P* Y = static_cast<const P*>(p.Y) + c;
+  int at[4], coming[4];
+  auto places = [&](int j0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) coming[j] = j0 + j < p.k ? p.position[slot + j0 + j] : -1;
+  };
+  places(0);
+  float sum[V] = {};
+  for (int j0 = 0; j0 < p.k; j0 += 4) {
+    P y[4];
+    float w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      at[j] = coming[j];
+      if (at[j] < 0) continue;
+      y[j] = Y[static_cast<long long>(at[j]) * p.vecs];
+      w[j] = weight_of<T>(p, slot + j0 + j);
+    }
+    places(j0 + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (at[j] < 0) continue;
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] = fmaf(w[j], y[j].get(v), sum[v]);
+    }
+  }
+  Vec<T, V>::store(static_cast<T*>(p.out) + (t * p.vecs + c) * V, sum);
+}
+
 // A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
 // zeros and a gradient of zero.  (A warp for every token, ten loads of four choices under way together: no faster for 512 bf16, 22 us
 // instead of 20 for 65536 slots of 256, 17 instead of 11 for 32768 of 64 float32.)
@@ -1708,6 +1749,11 @@ cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
   if constexpr (sizeof(T) * V < 4) {
     return launch_kernel(combine_columns_kernel<T>, (p.tokens + 3) / 4, 256, 0, st, true, p);
   } else {
+    if (p.vecs <= 32) {
+      int lanes_log2 = 2;
+      while ((1 << lanes_log2) < p.vecs) ++lanes_log2;
+      return launch_kernel(combine_narrow_kernel<T, V>, static_cast<unsigned>(((static_cast<long long>(p.tokens) << lanes_log2) + 255) / 256), 256, 0, st, true, p, lanes_log2);
+    }
     const int blocks = (p.vecs * static_cast<int>(sizeof(T) * V) + 511) / 512;
     p.by_blocks = Div(blocks);
     p.work = p.tokens * blocks;
