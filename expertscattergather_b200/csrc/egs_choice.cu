@@ -1052,7 +1052,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32) quantize_stream_kernel(cons
 }
 
 // ------------------------------------------------------------------------------------------------
-// Products over ragged rows on the CUDA cores: any type, width and alignment.  Tiles of 64 x 64, a step of 16 contraction elements,
+// Products over ragged rows on the CUDA cores, any width and alignment: rows of 16 and 8 bits, weight gradients of 16 bits and of few float32
+// features (the other float32 products are below).  Tiles of 64 x 64, a step of 16 contraction elements,
 // 4 x 4 products a thread; float32 (8-bit operands: int32) sums.
 // ------------------------------------------------------------------------------------------------
 constexpr int kGTile = 64, kGStep = 16;
