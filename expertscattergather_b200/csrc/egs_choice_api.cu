@@ -180,6 +180,8 @@ int egs_combine(const void* Y, const void* weights, const int32_t* position, voi
   if (tokens == 0 || N == 0) return EGS_OK;
   if (tokens * (N / 32 + 1) > kInt32Max) return EGS_ERR_TOO_LARGE;
   if (!out || (k > 0 && (!Y || !position))) return EGS_ERR_INVALID_ARGUMENT;
+  // (the kernels go from choice to choice: a token without any is not for them)
+  if (k == 0) return done(launch_fill_zero(out, static_cast<size_t>(tokens) * N * (dtype == EGS_F32 ? 4 : 2), stream_of(cuda_stream)), "combine fill");
   return done(launch_combine(Y, weights, position, out, tokens, static_cast<int>(k), static_cast<int>(N), dtype, weights_dtype == EGS_F32,
                              stream_of(cuda_stream)),
               "combine launch");

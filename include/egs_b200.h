@@ -366,7 +366,7 @@ int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, co
 size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype);
 
 /* out[t] = sum over j of weights[t, j] Y[position[t * k + j]]: token rows [tokens, N] from sorted rows.  weights NULL: ones.  Float32 in
- * the order of j, rounded once.  weights_dtype: EGS_F32 or the rows' type. */
+ * the order of j, rounded once; zeros where k is 0.  weights_dtype: EGS_F32 or the rows' type. */
 int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
                 int weights_dtype, void* cuda_stream);
 /* Its gradients: dY (sorted rows; zeros for slots that were not routed) and, where dweights is given, dweights[t, j] = <dOut[t], Y[..]>. */
