@@ -115,8 +115,10 @@ std::tuple<Tensor, Tensor, Tensor> plan_experts(const Tensor& experts, int64_t E
   return {offsets, slots, position};
 }
 
-// The plan's arrays belong together: [E + 1], [tokens * k], [tokens * k].
-void check_plan(const Tensor& offsets, const Tensor& slots, int64_t E, int64_t n) {
+// The plan's arrays belong together, [E + 1], [tokens * k], [tokens * k], and lie where the tensors do.
+void check_plan(const Call& c, const Tensor& offsets, const Tensor& slots, int64_t E, int64_t n) {
+  for (const Tensor* t : {&offsets, &slots})
+    if (!t->is_cuda() || t->get_device() != c.idx) throw std::runtime_error("the plan must be on the tensors' CUDA device");
   if (offsets.scalar_type() != at::kInt || slots.scalar_type() != at::kInt || offsets.numel() != E + 1 || slots.numel() != n ||
       !offsets.is_contiguous() || !slots.is_contiguous())
     value_error("the plan was made for " + std::to_string(offsets.numel() - 1) + " experts and " + std::to_string(slots.numel()) +
@@ -128,9 +130,9 @@ Tensor expert_matmul(const Tensor& X, const Tensor& W, const Tensor& offsets, co
   if (X.dim() < 1 || W.dim() != 3) value_error("expected X[..., C], W[E,.,.]");
   if (W.scalar_type() != X.scalar_type()) value_error("X and W must have the same dtype");
   const int dt = type_id(X.scalar_type()), rid = rows_id(rows);
-  Call c(X, W, offsets, slots);
+  Call c(X, W);
   const WDims w = w_dims(W, layout);
-  check_plan(offsets, slots, w.E, tokens * k);
+  check_plan(c, offsets, slots, w.E, tokens * k);
   const int64_t want = rid == EGS_ROWS_TOKENS ? tokens : tokens * k;
   if (X.size(-1) != w.C || X.numel() != want * w.C)
     value_error("shape mismatch: X" + shape_of(X) + " W" + shape_of(W) + " (" + layout_name(layout) + ") for " + std::to_string(want) + " rows");
@@ -151,9 +153,9 @@ Tensor expert_dweight(const Tensor& X, const Tensor& dY, const Tensor& offsets, 
   if (X.dim() < 1 || dY.dim() != 2) value_error("expected X[..., C], dY[tokens * k, N]");
   if (dY.scalar_type() != X.scalar_type()) value_error("X and dY must have the same dtype");
   const int dt = type_id(X.scalar_type()), rid = rows_id(rows);
-  Call c(X, dY, offsets, slots);
+  Call c(X, dY);
   const int64_t E = offsets.numel() - 1, C = X.size(-1), N = dY.size(1);
-  check_plan(offsets, slots, E, tokens * k);
+  check_plan(c, offsets, slots, E, tokens * k);
   const int64_t want = rid == EGS_ROWS_TOKENS ? tokens : tokens * k;
   if (X.numel() != want * C || dY.size(0) != tokens * k)
     value_error("shape mismatch: X" + shape_of(X) + " dY" + shape_of(dY) + " for " + std::to_string(want) + " and " + std::to_string(tokens * k) + " rows");
@@ -264,7 +266,7 @@ Tensor matmul_int8(const Tensor& q, const Tensor& q_scale, const Tensor& Wq, con
   const int64_t C = q.size(-1), E = dense ? 1 : Wq.size(0), N = Wq.size(-2), n = C ? q.numel() / C : 0;
   const int64_t row_count = q_scale.numel();
   if (dense) tokens = row_count, k = 1;
-  else check_plan(*offsets, *slots, E, tokens * k);
+  else check_plan(c, *offsets, *slots, E, tokens * k);
   const int64_t want = rid == EGS_ROWS_TOKENS ? tokens : tokens * k;
   if (Wq.size(-1) != C || row_count != want || (C && n != want) || w_scale.numel() != E * N)
     value_error("shape mismatch: q" + shape_of(q) + " scale" + shape_of(q_scale) + " Wq" + shape_of(Wq) + " scale" + shape_of(w_scale) + " for " +

@@ -38,3 +38,28 @@ def test_tokens_without_a_choice(cuda_device, tokens, N, dtype):
         dY, dweights = ops.combine_backward(torch.ones(tokens, N, device="cuda", dtype=dtype), Y, weights, plan)
         assert dY.shape == (0, N) and (dweights is None if weights is None else dweights.shape == (tokens, 0))
     ops.check_status()
+
+
+def test_plans_that_lie_elsewhere_are_refused(cuda_device):
+    """Before any launch: no kernel gets their addresses."""
+    E, k, tokens = 4, 2, 10
+    ids = torch.arange(tokens * k, device="cuda", dtype=torch.int32).view(tokens, k) % E
+    plan = ops.plan_experts(ids, E)
+    arrays = (plan.offsets, plan.slots, plan.position)
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, device="cuda", dtype=dtype)
+    ones = lambda *s: torch.ones(*s, device="cuda")
+    q, Wq = z(tokens, 16, dtype=torch.int8), z(E, 8, 16, dtype=torch.int8)
+    before = ops.launch_count()
+    for away in ((0,), (1,), (2,), (0, 1, 2)):
+        other = ops.ExpertPlan(*(a.cpu() if i in away else a for i, a in enumerate(arrays)), tokens, k, E)
+        calls = [lambda: ops.combine(z(tokens * k, 8), None, other), lambda: ops.combine_backward(z(tokens, 8), z(tokens * k, 8), z(tokens, k), other)] if 2 in away else []
+        if away != (2,):
+            calls += [lambda: ops.expert_matmul(z(tokens, 8), z(E, 8, 8), other), lambda: ops.expert_matmul(z(tokens * k, 8), z(E, 8, 8), other, rows="sorted"),
+                      lambda: ops.expert_dweight(z(tokens, 8), z(tokens * k, 8), other), lambda: ops.expert_matmul_int8(q, ones(tokens), Wq, ones(E, 8), other),
+                      lambda: ops.expert_matmul_int8(z(tokens * k, 16, dtype=torch.int8), ones(tokens * k), Wq, ones(E, 8), other, rows="sorted")]
+        for call in calls:
+            with pytest.raises(RuntimeError):
+                call()
+    assert ops.launch_count() == before
+    ops.expert_matmul_int8(q, ones(tokens), Wq, ones(E, 8), plan)
+    ops.check_status()
