@@ -41,7 +41,8 @@ __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)
 // lanes' own maxima is a lower bound of the k-th highest key; the keys that lie at most a margin of twice that error below it (256 random
 // ones, k = 8: ten in the mean) go through shared memory to one lane each, where their exact keys are formed and every lane counts the keys
 // before its own.  Where more than 32 lie there (many equal ones), every choice is a maximum over the exact keys of all lanes.
-// Groups are compared by their fast keys.
+// Groups are compared by their fast keys too; where a group that is left out comes within the errors of one that is kept, all keys are formed
+// exactly and the groups compared again (the check takes 1.2 us of 32; as a loop around both comparisons it took 3.4).
 // ------------------------------------------------------------------------------------------------
 constexpr int kRouteWarps = 8;
 
@@ -82,8 +83,11 @@ __device__ __forceinline__ void load_run(const T* p, int left, bool wide, float 
   }
 }
 
+// CTAs of an SM, as many as the keys of a thread leave registers for.
+__host__ __device__ constexpr int route_ctas(int nper) { return nper <= 2 ? 8 : nper == 4 ? 6 : nper == 8 ? 5 : nper == 16 ? 3 : 2; }
+
 template <typename T, int NPER>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(kRouteWarps * 32, route_ctas(NPER)) route_tokens_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ __align__(16) uint32_t route_smem[];
   pdl_wait();
   pdl_trigger();
@@ -141,53 +145,77 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens_kernel(const __
   }
   // whether the keys above are fast ones, and the exact key of an expert
   const bool fast = p.bias || pairs;
-  auto exact = [&](float v, int e) {
-    if (!p.bias) return ordered(v);
-    const float s = p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total;
-    return ordered(s + p.bias[e]);
-  };
+  auto score_of = [&](float v) { return p.sigmoid ? sigmoid(v) : m == -INFINITY ? 0.f : expf(v - m) / total; };
+  auto exact = [&](float v, int e) { return ordered(p.bias ? score_of(v) + p.bias[e] : v); };
   if (!p.vectors) {
 #pragma unroll
     for (int i = 0; i < NPER; ++i)
       if (i >= mine_left) key[i] = 0u;
   }
   if (p.groups > 1) {
-    uint32_t k1 = 0u, k2 = 0u;                           // the two highest keys
     const int g = lane >> p.lanes_log2;
-    if (p.whole_lanes) {
+    const bool first_lane = g < p.groups && !(lane & ((1 << p.lanes_log2) - 1));
+    uint32_t kept;                                       // by first lanes
+    // The groups of highest value; whether errors of fast keys may have decided that.
+    auto choose_groups = [&](bool fast_keys) {
+      uint32_t k1 = 0u, k2 = 0u;                         // the two highest keys
+      if (p.whole_lanes) {
 #pragma unroll
-      for (int i = 0; i < NPER; ++i) {
-        k2 = max(k2, min(k1, key[i]));
-        k1 = max(k1, key[i]);
-      }
-    } else {
-      // through shared memory: the lanes of a group look at every 2^lanes_log2-th of its keys
-#pragma unroll
-      for (int i = 0; i < NPER; ++i)
-        if (i < mine_left) mem[e0 + i] = key[i];
-      __syncwarp();
-      if (g < p.groups)
-        for (int i = lane & ((1 << p.lanes_log2) - 1); i < p.per; i += 1 << p.lanes_log2) {
-          const uint32_t v = mem[g * p.per + i];
-          k2 = max(k2, min(k1, v));
-          k1 = max(k1, v);
+        for (int i = 0; i < NPER; ++i) {
+          k2 = max(k2, min(k1, key[i]));
+          k1 = max(k1, key[i]);
         }
+      } else {
+        // through shared memory: the lanes of a group look at every 2^lanes_log2-th of its keys
+#pragma unroll
+        for (int i = 0; i < NPER; ++i)
+          if (i < mine_left) mem[e0 + i] = key[i];
+        __syncwarp();
+        if (g < p.groups)
+          for (int i = lane & ((1 << p.lanes_log2) - 1); i < p.per; i += 1 << p.lanes_log2) {
+            const uint32_t v = mem[g * p.per + i];
+            k2 = max(k2, min(k1, v));
+            k1 = max(k1, v);
+          }
+        __syncwarp();
+      }
+      for (int o = 1; o < (1 << p.lanes_log2); o <<= 1) {
+        const uint32_t o1 = __shfl_xor_sync(kFull, k1, o), o2 = __shfl_xor_sync(kFull, k2, o);
+        k2 = max(min(k1, o1), max(k2, o2));
+        k1 = max(k1, o1);
+      }
+      // (every lane of a group has its value; the first one stands for it)
+      const bool both = pairs && k2;
+      const float a = unordered(k1), b = both ? unordered(k2) : 0.f, value = a + b;
+      uint32_t gk = !first_lane ? 0u : both ? ordered(value) : k1, low = 0u;
+      kept = 0u;
+      for (int i = 0; i < p.top_groups; ++i) {
+        low = __reduce_max_sync(kFull, gk);
+        const int at = __ffs(__ballot_sync(kFull, gk == low)) - 1;
+        kept |= 1u << at;
+        if (lane == at) gk = 0u;
+      }
+      if (!fast_keys || p.top_groups == p.groups) return false;
+      // A value has to be further from the nearest one beyond the cut than twice its error: of a sum of a score and a bias 2^-21 and a unit, of a
+      // score alone 126 units (2 + 1.18 * 88 of the exponential, 2 of the reciprocal, the others the exact ones) and, where the fast reciprocal
+      // gives 0, 2^-126.  (Infinite values have no error, and of equal ones the difference is a NaN.)
+      const float high = unordered(__reduce_max_sync(kFull, gk));
+      const float gap = gk ? unordered(low) - value : value - high;
+      const float slack = p.bias ? 2e-6f * (1.f + fabsf(a) + fabsf(b)) : fmaf(3e-5f, value, 8e-38f);
+      return __any_sync(kFull, first_lane && slack < INFINITY && gap <= slack) != 0;
+    };
+    if (choose_groups(fast)) {
+      // (one after the other: unrolled, they took registers that leave the common way fewer warps, 80 for 48)
+#pragma unroll 1
+      for (int j = 0; j < min(NPER, mine_left); ++j) {
+        const float x_j = to_f32<T>(row[e0 + j]);
+        const uint32_t k = p.bias ? exact(x_j, e0 + j) : ordered(score_of(x_j));
+#pragma unroll
+        for (int i = 0; i < NPER; ++i)
+          if (i == j) key[i] = k;
+      }
       __syncwarp();
-    }
-    for (int o = 1; o < (1 << p.lanes_log2); o <<= 1) {
-      const uint32_t o1 = __shfl_xor_sync(kFull, k1, o), o2 = __shfl_xor_sync(kFull, k2, o);
-      k2 = max(min(k1, o1), max(k2, o2));
-      k1 = max(k1, o1);
-    }
-    // (every lane of a group has its value; the first one stands for it)
-    uint32_t gk = pairs && k2 ? ordered(unordered(k1) + unordered(k2)) : k1;
-    if (g >= p.groups || (lane & ((1 << p.lanes_log2) - 1))) gk = 0u;
-    uint32_t kept = 0u;                                  // by first lanes
-    for (int i = 0; i < p.top_groups; ++i) {
-      const uint32_t best = __reduce_max_sync(kFull, gk);
-      const int at = __ffs(__ballot_sync(kFull, gk == best)) - 1;
-      kept |= 1u << at;
-      if (lane == at) gk = 0u;
+      choose_groups(false);
     }
     if (p.whole_lanes) {
       if (!((kept >> (g << p.lanes_log2)) & 1u)) {

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from expertscattergather_b200 import ops
+from oracle import choice_oracle as orc
 
 pytestmark = pytest.mark.gpu
 
@@ -62,4 +63,80 @@ def test_plans_that_lie_elsewhere_are_refused(cuda_device):
                 call()
     assert ops.launch_count() == before
     ops.expert_matmul_int8(q, ones(tokens), Wq, ones(E, 8), plan)
+    ops.check_status()
+
+
+# ---- groups whose values are almost equal -----------------------------------------------------------------
+
+def kept_groups(key, groups, top_groups, group_top):
+    value = orc.group_values(key, groups, group_top)
+    kept = value.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
+    return torch.zeros_like(value, dtype=torch.bool).scatter_(1, kept, True), value
+
+
+# logits around `at`, where the groups' differ by whole `step`s: scores of a few units' error tell them apart, those of a fast
+# exponential (2 + 1.17 |x| units) need not; at -88 a fast reciprocal gives 0
+@pytest.mark.parametrize("at,step", [(-6.0, 2.0 ** -19), (-15.0, 2.0 ** -19), (-30.0, 2.0 ** -19), (-60.0, 2.0 ** -18), (-80.0, 2.0 ** -17), (-88.0, 2.0 ** -17)])
+@pytest.mark.parametrize("groups,per,top_groups", [(8, 32, 4), (6, 5, 1), (4, 15, 3), (2, 1, 1)])
+def test_groups_of_low_scores_are_compared_exactly(cuda_device, at, step, groups, per, top_groups):
+    """One score is off by at most 2 (exponential) + 1 (sum) + 1 (division) units: two values by 8 of 2^-23, 9.5e-7; a step changes a value
+    by 2^-19 = 1.9e-6 at least."""
+    g = gen(int(-at) + groups)
+    tokens = 4000
+    place = torch.stack([torch.randperm(groups, device="cuda", generator=g) for _ in range(tokens)]).float() * step
+    base = at + torch.randint(0, 64, (tokens, 1), device="cuda", generator=g).float() * step
+    logits = (base + place).unsqueeze(-1) - 0.25 * torch.rand(tokens, groups, per, device="cuda", generator=g).mul(64).floor().div(64) - 0.5
+    where = torch.rand(tokens, groups, per, device="cuda", generator=g).topk(min(2, per), -1).indices
+    logits.scatter_(2, where, (base + place).unsqueeze(-1).expand(-1, -1, where.shape[-1]))            # a group's best two
+    logits = logits.view(tokens, groups * per)
+    k = min(3, per * top_groups)
+    weights, ids = ops.route_tokens(logits, k, score="sigmoid", groups=groups, top_groups=top_groups, group_top=2)
+    kept, _ = kept_groups(orc.scores(logits, "sigmoid"), groups, top_groups, 2)
+    assert kept.gather(1, ids.long() // per).all()
+    # the best of the kept groups are chosen, by their logits
+    masked = logits.masked_fill(~kept.repeat_interleave(per, 1), -float("inf"))
+    assert torch.equal(ids.long(), masked.sort(dim=-1, descending=True, stable=True).indices[:, :k])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("group_top", [1, 2])
+def test_groups_with_a_bias_are_compared_exactly(cuda_device, score, group_top):
+    """Keys of 0.2 to 2 whose groups differ by steps of 2^-20.  A key is off by 4 units of a score below 1 and by half a unit of the key below
+    2, 2^-21 + 2^-24 at most, less than half of what two steps make; values that lie closer are not looked at."""
+    g = gen(group_top)
+    tokens, groups, per, top_groups, k = 4000, 8, 32, 3, 6
+    logits = torch.rand(tokens, groups, per, device="cuda", generator=g) * 0.5
+    place = torch.stack([torch.randperm(groups, device="cuda", generator=g) for _ in range(tokens)])
+    logits[..., 3] = 0.75 + 2.0 ** -17 * place
+    logits[..., 7] = 0.75 + 2.0 ** -17 * place
+    bias = torch.zeros(groups, per, device="cuda")
+    bias[:, (3, 7)] = 0.5
+    logits, bias = logits.view(tokens, -1), bias.flatten()
+    _, ids = ops.route_tokens(logits, k, bias, score=score, groups=groups, top_groups=top_groups, group_top=group_top)
+    kept, value = kept_groups(orc.scores(logits, score) + bias.double(), groups, top_groups, group_top)
+    order = value.sort(-1, descending=True).values
+    clear = order[:, top_groups - 1] - order[:, top_groups] > group_top * (2.0 ** -20 + 2.0 ** -22)
+    if score == "sigmoid":                                 # (a softmax over 256 experts makes the steps smaller than a unit of the key)
+        assert clear.float().mean() > 0.9
+    assert kept.gather(1, ids.long() // per)[clear].all()
+
+
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_groups_that_are_masked_or_equal(cuda_device, with_bias):
+    """Groups of equal values: the lower ones.  A bias of -infinity takes experts, and whole groups, out of the choice."""
+    tokens, groups, per = 70, 8, 4
+    logits = torch.full((tokens, groups * per), -20.0, device="cuda")
+    bias = torch.zeros(groups * per, device="cuda") if with_bias else None
+    for group_top in (1, 2):
+        _, ids = ops.route_tokens(logits, 6, bias, score="sigmoid", groups=groups, top_groups=3, group_top=group_top)
+        assert torch.equal(ids, torch.arange(6, device="cuda", dtype=torch.int32).expand(tokens, 6))
+        if not with_bias:
+            continue
+        masked = bias.clone()
+        masked[:4 * per] = -float("inf")                   # four groups
+        masked[6 * per:6 * per + 3] = -float("inf")        # all but one expert of another
+        _, ids = ops.route_tokens(logits, 9, masked, score="sigmoid", groups=groups, top_groups=3, group_top=group_top)
+        # (two experts of a group: the group with one left counts as lowest, with the masked ones)
+        want = [*range(4 * per, 6 * per), 6 * per + 3] if group_top == 1 else [*range(4 * per, 6 * per), 7 * per]
+        assert torch.equal(ids, torch.tensor(want, device="cuda", dtype=torch.int32).expand(tokens, 9))
     ops.check_status()
