@@ -9,6 +9,7 @@ No counterpart in the reference, whose experts choose their tokens (``ExpertGath
 """
 from __future__ import annotations
 
+import copy
 import math
 
 import torch
@@ -149,17 +150,36 @@ class RoutedExperts(nn.Module):
         return RoutedExpertsInt8(self)
 
 
+def _in_pitch(q):
+    """8-bit rows a multiple of 16 bytes apart, as ``ops.quantize_rows`` lays them out and the products read them without a copy."""
+    pitch = (q.shape[-1] + 15) // 16 * 16
+    if q.stride(-1) == 1 and q.stride(-2) == pitch:
+        return q
+    rows = q.new_zeros((*q.shape[:-1], pitch))[..., :q.shape[-1]]
+    return rows.copy_(q)
+
+
 class RoutedExpertsInt8(nn.Module):
     """A :class:`RoutedExperts` for serving: weights in 8 bits with a scale for each output channel, rows quantised on the way into each
-    product with a scale for each row."""
+    product with a scale for each row.  It has a router of its own, a copy without gradients: what becomes of the layer it was made from,
+    or of its type or device, does not reach it, nor the other way round.  The scales stay in float32 whatever the module is cast to."""
 
     def __init__(self, layer: RoutedExperts):
         super().__init__()
-        self.E, self.router = layer.E, layer.router
+        self.E, self.router = layer.E, copy.deepcopy(layer.router).requires_grad_(False)
         for name in ("up", "down"):
             q, scale = ops.quantize_rows(getattr(layer, name).detach().transpose(1, 2))
             self.register_buffer(name, q)
             self.register_buffer(name + "_scale", scale)
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = {name: getattr(self, name + "_scale") for name in ("up", "down")}
+        super()._apply(fn, *args, **kwargs)
+        for name, scale in kept.items():
+            setattr(self, name, _in_pitch(getattr(self, name)))           # (a copy to another device has its rows together)
+            if getattr(self, name + "_scale").dtype != torch.float32:
+                setattr(self, name + "_scale", scale.to(getattr(self, name).device))
+        return self
 
     @torch.no_grad()
     def forward(self, x):

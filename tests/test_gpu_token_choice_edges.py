@@ -7,7 +7,7 @@ products' magnitudes (u = 2^-24), a rounding to 16 bits by half a unit.
 import pytest
 import torch
 
-from expertscattergather_b200 import ops
+from expertscattergather_b200 import RoutedExperts, ops
 from oracle import choice_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -139,4 +139,28 @@ def test_groups_that_are_masked_or_equal(cuda_device, with_bias):
         # (two experts of a group: the group with one left counts as lowest, with the masked ones)
         want = [*range(4 * per, 6 * per), 6 * per + 3] if group_top == 1 else [*range(4 * per, 6 * per), 7 * per]
         assert torch.equal(ids, torch.tensor(want, device="cuda", dtype=torch.int32).expand(tokens, 9))
+    ops.check_status()
+
+
+# ---- the served layer --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("I,J", [(64, 48), (72, 40)])
+def test_served_layer_after_casts_and_moves(cuda_device, dtype, I, J):
+    torch.manual_seed(0)
+    layer = RoutedExperts(8, I, J, 2, balance=True).cuda()
+    x = randn(gen(1), 30, I)
+    served, full = layer.quantized(), layer(x).detach()
+    small = served(x)
+    assert (small - full).norm() <= 0.04 * full.norm()
+    moved = layer.quantized().cpu().cuda()
+    assert torch.equal(moved(x), small)
+    cast = layer.quantized().to(dtype)
+    assert layer.router.W.dtype == torch.float32 and torch.equal(layer(x), full)
+    out = cast(x.to(dtype))
+    assert out.dtype == dtype and (out.float() - full).norm() <= 0.06 * full.norm()
+    with torch.no_grad():
+        layer.router.W.neg_()
+    assert torch.equal(served(x), small)
+    assert moved.up.stride(-2) % 16 == 0 and moved.down.stride(-2) % 16 == 0
     ops.check_status()

@@ -143,3 +143,39 @@ def test_oracle_against_loops():
     dW, _ = orc.dweight(X, Y, ids, E, "tokens")
     for e in range(E):
         assert torch.allclose(dW[e], sum((torch.outer(X[t].double(), Y[r]) for r, (t, j) in enumerate(rows) if ids[t, j] == e), torch.zeros(C, N, dtype=torch.float64)))
+
+
+def test_served_layer_keeps_its_scales_its_rows_and_its_router(monkeypatch):
+    """Casts, copies and moves of a layer on 8-bit weights, and of the layer it was made from."""
+    import copy
+
+    def quantize(x):                                       # (rows in 8 bits without a GPU, laid out as the operator's)
+        scale = x.float().abs().amax(-1) / 127
+        rows = torch.zeros(*x.shape[:-1], (x.shape[-1] + 15) // 16 * 16, dtype=torch.int8)[..., :x.shape[-1]]
+        return rows.copy_((x.float() / scale.unsqueeze(-1)).round()), scale
+
+    monkeypatch.setattr(ops, "quantize_rows", quantize)
+    layer = egs.RoutedExperts(4, 24, 40, 2, balance=True)
+    served = layer.quantized()
+    before = {n: t.clone() for n, t in served.state_dict().items()}
+    rows = lambda m: [(t.stride(-1), t.stride(-2) % 16) for t in (m.up, m.down)]
+    assert rows(served) == [(1, 0)] * 2 and served.up.shape == (4, 40, 24)
+    served.to(torch.bfloat16)
+    assert served.up_scale.dtype == served.down_scale.dtype == served.router.balance.dtype == torch.float32
+    assert served.router.W.dtype == torch.bfloat16 and layer.router.W.dtype == torch.float32
+    for name in ("up", "down", "up_scale", "down_scale", "router.balance"):
+        assert torch.equal(served.state_dict()[name], before[name])
+    # training on does not move the served router
+    with torch.no_grad():
+        layer.router.W.add_(1.0)
+        layer.router.balance.add_(1.0)
+    assert torch.equal(served.router.W, before["router.W"].bfloat16()) and not served.router.balance.any()
+    assert not any(p.requires_grad for p in served.parameters()) and all(p.requires_grad for p in layer.parameters())
+    # copies that put rows together get their pitch back
+    dense = served._apply(lambda t: t.contiguous().clone())
+    assert dense is served and rows(served) == [(1, 0)] * 2 and torch.equal(served.up, before["up"])
+    other = copy.deepcopy(served)
+    other.load_state_dict(served.state_dict())
+    assert rows(other) == [(1, 0)] * 2 and torch.equal(other.down, served.down)
+    meta = copy.deepcopy(served).to("meta")
+    assert meta.up_scale.dtype == torch.float32 and meta.up_scale.is_meta
