@@ -5,7 +5,8 @@ training and, with 8-bit weights, for serving.
     served = layer.quantized()                          # the same layer on int8 weights, no gradients
 
 No counterpart in the reference, whose experts choose their tokens (``ExpertGather`` / ``ExpertScatter``).  The operators are those of
-``ops``; here they have gradients.
+``ops``; here they have gradients, first ones alone: a second derivative through them raises.  ``torch.compile`` runs the operators as they
+are, between the graphs that it makes of what lies around them; with ``fullgraph=True`` it refuses these layers.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import math
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from . import ops
@@ -34,6 +36,7 @@ class RouteTokensFunction(torch.autograd.Function):
         return weights, experts
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dweights, _):
         logits, experts = ctx.saved_tensors
         return ops.route_tokens_backward(dweights, logits, experts, **ctx.options), None, None, None
@@ -49,6 +52,7 @@ class ExpertMatmulFunction(torch.autograd.Function):
         return ops.expert_matmul(X, W, plan, rows=rows)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dY):
         X, W = ctx.saved_tensors
         dX = dW = None
@@ -72,6 +76,7 @@ class CombineFunction(torch.autograd.Function):
         return ops.combine(Y, weights, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dOut):
         Y, weights = ctx.saved_tensors
         return (*ops.combine_backward(dOut, Y, weights, ctx.plan), None)

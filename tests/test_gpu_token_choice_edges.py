@@ -7,7 +7,7 @@ products' magnitudes (u = 2^-24), a rounding to 16 bits by half a unit.
 import pytest
 import torch
 
-from expertscattergather_b200 import RoutedExperts, ops
+from expertscattergather_b200 import RoutedExperts, ops, token_choice
 from oracle import choice_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -163,4 +163,41 @@ def test_served_layer_after_casts_and_moves(cuda_device, dtype, I, J):
         layer.router.W.neg_()
     assert torch.equal(served(x), small)
     assert moved.up.stride(-2) % 16 == 0 and moved.down.stride(-2) % 16 == 0
+    ops.check_status()
+
+
+# ---- under autograd and torch.compile ----------------------------------------------------------------------
+
+def test_second_derivatives_are_refused(cuda_device):
+    """They are not implemented; a graph of first gradients may be made, and says so where it is differentiated."""
+    g = gen(2)
+    logits, X, W = (t.requires_grad_(True) for t in (randn(g, 20, 6), randn(g, 20, 8), randn(g, 6, 8, 4)))
+    weights, ids = token_choice.route_tokens(logits, 2)
+    plan = ops.plan_experts(ids, 6)
+    Y = randn(g, 40, 4).requires_grad_(True)
+    for out, leaf in ((weights, logits), (token_choice.expert_matmul(X, W, plan), X), (token_choice.combine(Y, weights.detach(), plan), Y)):
+        first, = torch.autograd.grad(out.square().sum(), leaf, create_graph=True, retain_graph=True)
+        plain, = torch.autograd.grad(out.square().sum(), leaf, retain_graph=True)
+        assert torch.equal(first, plain) and not plain.requires_grad
+        # (a penalty on the gradient beside another term of the leaf: without the refusal its part would be missing in silence)
+        with pytest.raises(RuntimeError):
+            (first.square().sum() + leaf.square().sum()).backward()
+
+
+def test_compiled_layer(cuda_device):
+    torch.manual_seed(0)
+    layer = RoutedExperts(8, 64, 32, 2).cuda()
+    x = randn(gen(3), 50, 64)
+    ref = layer(x)
+    ref.square().sum().backward()
+    grads = [p.grad.clone() for p in layer.parameters()]
+    layer.zero_grad()
+    out = torch.compile(layer)(x)
+    out.square().sum().backward()
+    # (what lies between the operators, SiLU above all, may be rounded otherwise)
+    assert torch.allclose(out, ref, rtol=1e-5, atol=1e-6)
+    for p, g in zip(layer.parameters(), grads):
+        assert torch.allclose(p.grad, g, rtol=1e-4, atol=1e-5)
+    served = layer.quantized()
+    assert torch.allclose(torch.compile(served)(x), served(x), rtol=0.02, atol=1e-3)
     ops.check_status()
