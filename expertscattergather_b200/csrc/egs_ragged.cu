@@ -693,9 +693,9 @@ ragged_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ Ra
   }
 }
 
-// dW of cut experts: the sums of their ranges, in order.
+// dW of cut experts: the sums of their ranges, in order.  fours: every expert's begins on four elements and is a whole number of them.
 template <typename T>
-__global__ void __launch_bounds__(256) ragged_join_kernel(const int* offsets, const float* partial, T* out, long long size, int E, int range_steps) {
+__global__ void __launch_bounds__(256) ragged_join_kernel(const int* offsets, const float* partial, T* out, long long size, int E, int range_steps, bool fours) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const int* offsets, co
       base += n;
       if (turn++ % gridDim.y != blockIdx.y) continue;
       T* o = out + (e0 + __ffs(cut) - 1) * size;
-      if (size % 4 == 0) {
+      if (fours) {
         for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4; i < size; i += static_cast<long long>(gridDim.x) * 1024) {
           float4 sum = *reinterpret_cast<const float4*>(p + i);
 #pragma unroll 4
@@ -903,11 +903,12 @@ cudaError_t launch_ragged_dweight_tensor(const RaggedParams& p, int dtype, void*
   if (err != cudaSuccess || d.most_partial == 0) return err;
   // (six CTAs an SM at most: most experts are not cut, and 16 rows of CTAs that find nothing to add took 2 to 6 us more)
   const dim3 ctas(static_cast<unsigned>(size / 1024 < 1 ? 1 : size / 1024 > kSmCount ? kSmCount : size / 1024), p.E < 6 ? p.E : 6);
+  const bool fours = size % 4 == 0 && (reinterpret_cast<uintptr_t>(p.Out) & 7u) == 0;
   count_launch();
   if (dtype == EGS_F16)
-    return launch_kernel(ragged_join_kernel<__half>, ctas, 256, 0, st, true, p.offsets, q.partial, static_cast<__half*>(p.Out), size, p.E, q.range_steps);
+    return launch_kernel(ragged_join_kernel<__half>, ctas, 256, 0, st, true, p.offsets, q.partial, static_cast<__half*>(p.Out), size, p.E, q.range_steps, fours);
   return launch_kernel(ragged_join_kernel<__nv_bfloat16>, ctas, 256, 0, st, true, p.offsets, q.partial, static_cast<__nv_bfloat16*>(p.Out), size, p.E,
-                       q.range_steps);
+                       q.range_steps, fours);
 }
 
 }  // namespace egs

@@ -4,10 +4,12 @@ groups whose values are almost equal, weight gradients in every variant, second 
 Tolerances are those of the tests of the operators: float32 sums of n products are off by at most (n + 2) * 2 * u times the sum of the
 products' magnitudes (u = 2^-24), a rounding to 16 bits by half a unit.
 """
+import ctypes
+
 import pytest
 import torch
 
-from expertscattergather_b200 import RoutedExperts, ops, token_choice
+from expertscattergather_b200 import RoutedExperts, _lib, ops, token_choice
 from oracle import choice_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -200,4 +202,55 @@ def test_compiled_layer(cuda_device):
         assert torch.allclose(p.grad, g, rtol=1e-4, atol=1e-5)
     served = layer.quantized()
     assert torch.allclose(torch.compile(served)(x), served(x), rtol=0.02, atol=1e-3)
+    ops.check_status()
+
+
+# ---- the C entries -----------------------------------------------------------------------------------------
+
+TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def shifted(t, by):
+    """A copy that begins `by` elements into its storage."""
+    store = torch.empty(t.numel() + by + 16, device="cuda", dtype=t.dtype)
+    return store[by:by + t.numel()].view(t.shape).copy_(t)
+
+
+# where a kernel stores several elements together it has to look at where the output begins: the first expert of these is cut into ranges,
+# in the last one a range is a whole expert
+@pytest.mark.parametrize("by", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("tokens,E,C,N", [(7000, 2, 64, 64), (7000, 2, 33, 36), (7000, 2, 35, 33), (60, 6, 64, 72)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_entries_take_outputs_that_begin_anywhere(cuda_device, by, tokens, E, C, N, dtype):
+    lib, g, k = _lib.load(), gen(by + C), 2
+    ids = torch.rand(tokens, E, device="cuda", generator=g).topk(k, -1).indices.int()
+    plan = ops.plan_experts(ids, E)
+    X, W, dY = randn(g, tokens, C, dtype=dtype), randn(g, E, C, N, dtype=dtype), randn(g, tokens * k, N, dtype=dtype)
+    dims = ctypes.byref(_lib.Ragged(tokens, k, E, C, N))
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    space = lambda n: (torch.empty(max(n, 16), device="cuda", dtype=torch.uint8), n)
+    nan = lambda t: shifted(torch.full_like(t, float("nan")), by)
+
+    Y = ops.expert_matmul(X, W, plan)
+    got, (ws, n) = nan(Y), space(lib.egs_expert_matmul_workspace_bytes(dims, 0, 0, TYPES[dtype]))
+    assert lib.egs_expert_matmul(at(X), at(W), at(plan.offsets), at(plan.slots), at(got), dims, 0, 0, TYPES[dtype], 0, at(ws), n, None, stream) == _lib.OK
+    assert torch.equal(got, Y)
+    dW = ops.expert_dweight(X, dY, plan)
+    got, (ws, n) = nan(dW), space(lib.egs_expert_dweight_workspace_bytes(dims, 0, TYPES[dtype]))
+    assert lib.egs_expert_dweight(at(X), at(dY), at(plan.offsets), at(plan.slots), at(got), dims, 0, TYPES[dtype], 0, at(ws), n, None, stream) == _lib.OK
+    assert torch.equal(got, dW)
+    w = torch.rand(tokens, k, device="cuda", generator=g)
+    out = ops.combine(Y, w, plan)
+    got = nan(out)
+    assert lib.egs_combine(at(shifted(Y, by)), at(w), at(plan.position), at(got), tokens, k, N, TYPES[dtype], _lib.F32, stream) == _lib.OK
+    # (the columns of a row are summed in the order of the choices whatever the vectors are)
+    assert torch.equal(got, out)
+    gY, gw = ops.combine_backward(out, Y, w, plan)
+    got, got_w = nan(gY), torch.full_like(gw, float("nan"))
+    assert lib.egs_combine_backward(at(shifted(out, by)), at(shifted(Y, by)), at(w), at(plan.position), at(got), at(got_w), tokens, k, N, TYPES[dtype],
+                                    _lib.F32, stream) == _lib.OK
+    assert torch.equal(got, gY)
+    size = (out.double()[:, None] * Y.double()[plan.position.long()].view(tokens, k, N)).abs().sum(-1)
+    assert ((got_w.double() - gw.double()).abs() <= 2 * (N + 2) * 2.0 ** -24 * size).all()         # (another order of a float32 sum)
     ops.check_status()
