@@ -1102,7 +1102,7 @@ __device__ __forceinline__ void locate_block(const int* offsets, int E, int rows
     for (int e0 = 0; e0 < E && e_found < 0; e0 += 32) {
       const int e = e0 + lane;
       const int a = e < E ? b->offsets[e] : 0, end = e < E ? b->offsets[e + 1] : 0;
-      const int blocks = (end - a + rows - 1) / rows;
+      const int blocks = static_cast<int>((static_cast<unsigned>(end - a) + rows - 1) / rows);     // (`rows` may be nearly all)
       int incl = blocks;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -1261,7 +1261,7 @@ struct DweightRange {
 __device__ __forceinline__ DweightRange range_of(const RaggedParams& p, int length, Block* block) {
   if (length == 0) return {static_cast<int>(blockIdx.z), p.offsets[blockIdx.z], p.offsets[blockIdx.z + 1]};
   locate_block(p.offsets, p.E, length, blockIdx.z, block);
-  return {block->expert, block->first, min(block->end, block->first + length)};
+  return {block->expert, block->first, block->end - block->first > length ? block->first + length : block->end};
 }
 template <typename T>
 __global__ void __launch_bounds__(256) ragged_dweight_kernel(const __grid_constant__ RaggedParams p, int length, float* partial) {
@@ -1690,11 +1690,12 @@ __global__ void __launch_bounds__(256) dweight_join_kernel(const int* offsets, c
   const int expert = blockIdx.y, lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
     int base = 0;
-    for (int e = lane; e < expert; e += 32) base += (offsets[e + 1] - offsets[e] + length - 1) / length;
+    auto ranges = [&](int e) { return static_cast<int>((static_cast<unsigned>(offsets[e + 1] - offsets[e]) + length - 1) / length); };
+    for (int e = lane; e < expert; e += 32) base += ranges(e);
     base = __reduce_add_sync(kFull, base);
     if (lane == 0) {
       s_base = base;
-      s_count = (offsets[expert + 1] - offsets[expert] + length - 1) / length;
+      s_count = ranges(expert);
     }
   }
   __syncthreads();

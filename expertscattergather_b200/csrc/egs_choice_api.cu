@@ -4,7 +4,8 @@
 namespace egs {
 namespace {
 
-constexpr long long kInt32Max = 2147483647LL, kMaxWidth = 1 << 24;
+// Rows are counted in 32 bits, and what lies up to a few tiles behind the last one has to be countable too.
+constexpr long long kInt32Max = 2147483647LL, kMaxRows = EGS_MAX_ROWS, kMaxWidth = 1 << 24;
 
 bool valid_dtype(int d) { return d == EGS_F32 || d == EGS_F16 || d == EGS_BF16; }
 bool valid_path(int p) { return p == EGS_PATH_AUTO || p == EGS_PATH_GENERIC || p == EGS_PATH_TENSOR; }
@@ -20,13 +21,13 @@ int check_route(const egs_route* r, int64_t row_stride, int dtype, bool choice) 
   if (choice && (r->groups < 1 || r->E % r->groups || r->top_groups < 1 || r->top_groups > r->groups || (r->group_top != 1 && r->group_top != 2) ||
                  r->top_k > r->E / r->groups * r->top_groups))
     return EGS_ERR_INVALID_ARGUMENT;
-  if (r->E > EGS_MAX_EXPERTS || r->top_k > EGS_MAX_CHOICES || (choice && r->groups > EGS_MAX_GROUPS) || r->tokens > kInt32Max) return EGS_ERR_TOO_LARGE;
+  if (r->E > EGS_MAX_EXPERTS || r->top_k > EGS_MAX_CHOICES || (choice && r->groups > EGS_MAX_GROUPS) || r->tokens > kMaxRows) return EGS_ERR_TOO_LARGE;
   return EGS_OK;
 }
 
 int check_ragged(const egs_ragged* d) {
   if (!d || d->tokens < 0 || d->k < 0 || d->E < 0 || d->C < 0 || d->N < 0) return EGS_ERR_INVALID_ARGUMENT;
-  if (d->E > EGS_MAX_EXPERTS || d->tokens > kInt32Max || d->k > kInt32Max || d->tokens * d->k > kInt32Max || d->C > kMaxWidth || d->N > kMaxWidth)
+  if (d->E > EGS_MAX_EXPERTS || d->tokens > kMaxRows || d->k > kMaxRows || d->tokens * d->k > kMaxRows || d->C > kMaxWidth || d->N > kMaxWidth)
     return EGS_ERR_TOO_LARGE;
   if (d->E == 0 && d->tokens * d->k > 0) return EGS_ERR_INVALID_ARGUMENT;
   return EGS_OK;
@@ -91,13 +92,13 @@ int egs_route_tokens_backward(const float* dweights, const void* logits, const i
 }
 
 size_t egs_plan_workspace_bytes(int64_t n, int E) {
-  return n <= 0 || n > kInt32Max || E < 0 || E > EGS_MAX_EXPERTS ? 0 : plan_workspace_ints(n, E) * sizeof(int);
+  return n <= 0 || n > kMaxRows || E < 0 || E > EGS_MAX_EXPERTS ? 0 : plan_workspace_ints(n, E) * sizeof(int);
 }
 
 int egs_plan_experts(const int32_t* experts, int64_t n, int E, int32_t* offsets, int32_t* slots, int32_t* position, void* workspace,
                      size_t workspace_bytes, int32_t* status_word, void* cuda_stream) {
   if (n < 0 || E < 1 || !offsets || (n > 0 && (!experts || !slots || !position))) return EGS_ERR_INVALID_ARGUMENT;
-  if (n > kInt32Max || E > EGS_MAX_EXPERTS) return EGS_ERR_TOO_LARGE;
+  if (n > kMaxRows || E > EGS_MAX_EXPERTS) return EGS_ERR_TOO_LARGE;
   const size_t need = egs_plan_workspace_bytes(n, E);
   if (need && (!workspace || workspace_bytes < need)) return EGS_ERR_WORKSPACE;
   return done(launch_plan_experts(experts, n, E, offsets, slots, position, static_cast<int*>(workspace), status_ref(status_word), stream_of(cuda_stream)),
@@ -202,7 +203,7 @@ int egs_combine_backward(const void* dOut, const void* Y, const void* weights, c
 int egs_quantize_rows(const void* X, int8_t* q, float* scale, int64_t rows, int64_t C, int64_t x_stride, int64_t q_stride, int dtype,
                       void* cuda_stream) {
   if (!valid_dtype(dtype) || rows < 0 || C < 0 || x_stride < 0 || q_stride < C) return EGS_ERR_INVALID_ARGUMENT;
-  if (rows > kInt32Max || C > kMaxWidth) return EGS_ERR_TOO_LARGE;
+  if (rows > kMaxRows || C > kMaxWidth) return EGS_ERR_TOO_LARGE;
   if (rows == 0) return EGS_OK;
   if (!scale || (C > 0 && (!X || !q))) return EGS_ERR_INVALID_ARGUMENT;
   return done(launch_quantize_rows(X, q, scale, rows, static_cast<int>(C), x_stride, q_stride, dtype, stream_of(cuda_stream)), "quantize_rows launch");

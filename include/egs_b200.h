@@ -314,6 +314,7 @@ enum { EGS_I8 = 3 };                                     /* element type of the 
 enum { EGS_SCORE_SOFTMAX = 0, EGS_SCORE_SIGMOID = 1 };
 enum { EGS_ROWS_TOKENS = 0 /* row token of a slot */, EGS_ROWS_SORTED = 1 };
 enum { EGS_MAX_EXPERTS = 1024, EGS_MAX_CHOICES = 32, EGS_MAX_GROUPS = 32 };
+enum { EGS_MAX_ROWS = 2147479552 };                      /* tokens, slots and rows: 2^31 - 4096 */
 
 typedef struct egs_route {
   int64_t tokens;

@@ -254,3 +254,21 @@ def test_entries_take_outputs_that_begin_anywhere(cuda_device, by, tokens, E, C,
     size = (out.double()[:, None] * Y.double()[plan.position.long()].view(tokens, k, N)).abs().sum(-1)
     assert ((got_w.double() - gw.double()).abs() <= 2 * (N + 2) * 2.0 ** -24 * size).all()         # (another order of a float32 sum)
     ops.check_status()
+
+
+# ---- as many rows as there can be --------------------------------------------------------------------------
+
+def test_rows_up_to_the_limit(cuda_device):
+    """One expert of 2^31 - 4096 rows of one element."""
+    n = (1 << 31) - 4096
+    X = torch.ones(n, 1, device="cuda")
+    slots = torch.zeros(n, device="cuda", dtype=torch.int32)                   # (sorted rows: nobody reads them)
+    plan = ops.ExpertPlan(torch.tensor([0, n], device="cuda", dtype=torch.int32), slots, slots[:0], n, 1, 1)
+    # sums of at most 3.7 million ones are exact; the ranges' (at most 592 + 1) are added one after the other
+    dW = ops.expert_dweight(X, X, plan, rows="sorted")
+    assert abs(dW.item() - n) <= 593 * 2.0 ** -24 * n
+    Y = ops.expert_matmul(X, torch.full((1, 1, 1), 2.0, device="cuda"), plan, rows="sorted")
+    assert Y[-5000:].eq(2).all() and Y[::4097].eq(2).all()
+    ops.check_status()
+    del X, Y, slots
+    torch.cuda.empty_cache()

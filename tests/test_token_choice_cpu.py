@@ -179,3 +179,22 @@ def test_served_layer_keeps_its_scales_its_rows_and_its_router(monkeypatch):
     assert rows(other) == [(1, 0)] * 2 and torch.equal(other.down, served.down)
     meta = copy.deepcopy(served).to("meta")
     assert meta.up_scale.dtype == torch.float32 and meta.up_scale.is_meta
+
+
+def test_entries_refuse_rows_that_cannot_be_counted():
+    """Up to 2^31 - 4096 rows a few tiles behind the last one can be counted in 32 bits; one more is refused, before a pointer is looked at."""
+    lib, most = _lib.load(), (1 << 31) - 4096
+    for n, code in ((most, BAD), (most + 1, LARGE), ((1 << 31) - 1, LARGE)):          # (BAD: the pointers that are missing)
+        assert lib.egs_route_tokens(None, None, None, None, route(tokens=n), 8, _lib.F32, None) == code
+        assert lib.egs_route_tokens_backward(None, None, None, None, route(tokens=n), 8, _lib.F32, None) == code
+        assert lib.egs_plan_experts(None, n, 4, None, None, None, None, 0, None, None) == BAD
+        assert lib.egs_plan_experts(one, n, 4, one, one, one, None, 0, None, None) == (WORKSPACE if code == BAD else LARGE)
+        assert lib.egs_quantize_rows(None, None, None, n, 1, 1, 1, _lib.F32, None) == code
+        for tokens, k in ((n, 1), (1, n)):
+            d = ragged(tokens=tokens, k=k, E=2, C=1, N=1)
+            for dtype in (_lib.F32, _lib.BF16):
+                assert lib.egs_expert_matmul(None, None, None, None, None, d, 0, 0, dtype, 0, None, 0, None, None) == code
+                assert lib.egs_expert_dweight(None, None, None, None, None, d, 0, dtype, 0, None, 0, None, None) == code
+                assert lib.egs_combine(None, None, None, None, tokens, k, 1, dtype, dtype, None) == code
+                assert lib.egs_combine_backward(None, None, None, None, None, None, tokens, k, 1, dtype, dtype, None) == code
+            assert lib.egs_expert_matmul_int8(None, None, 1, None, None, 1, one, None, None, d, 0, _lib.F32, 0, None, None) == code
