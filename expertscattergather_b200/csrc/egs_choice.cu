@@ -1153,10 +1153,11 @@ __device__ __forceinline__ void load4(const T* p, int left, bool wide, typename 
 
 // Rows behind the last expert's: zeros.
 template <typename T>
-__device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int routed, int part, int parts) {
+__device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int routed) {
   T* out = static_cast<T*>(p.Out);
   const long long begin = static_cast<long long>(routed) * p.N, end = static_cast<long long>(p.rows) * p.N;
-  for (long long i = begin + part; i < end; i += parts) out[i] = from_f32<T>(0.f);
+  const GridThreads threads;
+  for (long long i = begin + threads.mine; i < end; i += threads.all) out[i] = from_f32<T>(0.f);
 }
 
 // A step in shared memory, contraction by contraction; two of them, so that the next one is written while this one is read.
@@ -1190,7 +1191,7 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant_
     e = block.expert;
     first = block.first;
     end = block.end;
-    zero_unrouted<OutT>(p, block.offsets[p.E], (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid, gridDim.x * gridDim.y * 256);
+    zero_unrouted<OutT>(p, block.offsets[p.E]);
   }
   if (e < 0) return;
   if (tid < kGTile) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
@@ -1391,7 +1392,7 @@ __global__ void __launch_bounds__(kWideThreads, 3) ragged_rows_f32_kernel(const 
   const int tid = threadIdx.x;
   locate_block(p.offsets, p.E, kWide, blockIdx.x, &block);
   const int e = block.expert, first = block.first, end = block.end;
-  zero_unrouted<float>(p, block.offsets[p.E], (blockIdx.y * gridDim.x + blockIdx.x) * kWideThreads + tid, gridDim.x * gridDim.y * kWideThreads);
+  zero_unrouted<float>(p, block.offsets[p.E]);
   if (e < 0) return;
   src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
   const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
@@ -1605,7 +1606,7 @@ __global__ void __launch_bounds__(64 * G, G == 4 ? 2 : 4) ragged_rows_mid_kernel
   Block* block = reinterpret_cast<Block*>(mid_ring);
   locate_block(p.offsets, p.E, kMidRows, blockIdx.x, block);
   const int e = block->expert, first = block->first, rows = min(kMidRows, block->end - first), routed = block->offsets[p.E];
-  zero_unrouted<float>(p, routed, (blockIdx.y * gridDim.x + blockIdx.x) * (64 * G) + tid, gridDim.x * gridDim.y * (64 * G));
+  zero_unrouted<float>(p, routed);
   if (e < 0) return;
   if (tid < rows) src[tid] = p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
   __syncthreads();

@@ -58,11 +58,12 @@ __device__ __forceinline__ Segment segment_of(const RaggedParams& p, Segment* sh
   return *shared;
 }
 template <typename OutT>
-__device__ __forceinline__ void few_zero(const RaggedParams& p, int part, int parts) {
+__device__ __forceinline__ void few_zero(const RaggedParams& p) {
   if (!p.offsets) return;
   OutT* out = static_cast<OutT*>(p.Out);
   const long long begin = static_cast<long long>(p.offsets[p.E]) * p.N, end = static_cast<long long>(p.rows) * p.N;
-  for (long long i = begin + part; i < end; i += parts) out[i] = from_f32<OutT>(0.f);
+  const GridThreads threads;
+  for (long long i = begin + threads.mine; i < end; i += threads.all) out[i] = from_f32<OutT>(0.f);
 }
 
 template <typename T, int V>
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_nc_kernel(const __grid_c
   __shared__ Segment shared;
   pdl_wait();
   pdl_trigger();
-  few_zero<OutT>(p, (blockIdx.y * gridDim.x + blockIdx.x) * kFewThreads + threadIdx.x, gridDim.x * gridDim.y * kFewThreads);
+  few_zero<OutT>(p);
   const Segment s = segment_of(p, &shared);
   if (s.expert < 0) return;
   const int n0 = (blockIdx.x * kFewWarps + (threadIdx.x >> 5)) * kFewChannels;
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kFewCnThreads, 1) few_rows_cn_kernel(const __g
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x;
-  few_zero<T>(p, (blockIdx.y * gridDim.x + blockIdx.x) * kFewCnThreads + tid, gridDim.x * gridDim.y * kFewCnThreads);
+  few_zero<T>(p);
   const Segment s = segment_of(p, &sh.segment);
   if (s.expert < 0) return;
   for (int r = s.first; r < s.end; r += kFewRows) {

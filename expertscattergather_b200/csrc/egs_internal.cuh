@@ -50,6 +50,14 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Packed {
   }
 };
 
+// This thread's number among those of a grid, and how many there are (wide outputs have more than 2^31 of them).
+struct GridThreads {
+  long long mine, all;
+  __device__ __forceinline__ GridThreads()
+      : mine((static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x),
+        all(static_cast<long long>(gridDim.x) * gridDim.y * blockDim.x) {}
+};
+
 // Reads Ind[pos] for any of the three index widths.
 __device__ __forceinline__ long long load_index(const void* ind, int index_dtype, long long pos) {
   if (index_dtype == EGS_I64) return static_cast<const long long*>(ind)[pos];

@@ -272,3 +272,28 @@ def test_rows_up_to_the_limit(cuda_device):
     ops.check_status()
     del X, Y, slots
     torch.cuda.empty_cache()
+
+
+# a row for each of many experts, and more that are not routed: grids of more than 2^31 threads, which share the zeros among themselves
+@pytest.mark.parametrize("dtype,E,N", [(torch.float32, 1024, 270000), (torch.bfloat16, 512, 1600000)])
+def test_zeros_of_wide_rows(cuda_device, dtype, E, N):
+    g = gen(N)
+    tokens = E // 6 if dtype != torch.float32 else E
+    ids = torch.stack([torch.randperm(E, device="cuda", generator=g)[:tokens], torch.full((tokens,), -1, device="cuda")], -1)
+    ids[::5, 0] = -1
+    plan = ops.plan_experts(ids, E)
+    X, W = randn(g, tokens, 1, dtype=dtype), torch.rand(E, 1, N, device="cuda", generator=g).to(dtype)
+    torch.full((tokens * 2, N), float("nan"), device="cuda", dtype=dtype)          # (what the output's memory held)
+    for w, layout in ((W, "cn"), (W.view(E, N, 1), "nc")):
+        Y = ops.expert_matmul(X, w, plan, w_layout=layout)
+        routed = plan.offsets[E].item()
+        assert not Y[routed:].any()
+        # one product, rounded once
+        slots = plan.slots[:routed].long()
+        experts = ids.flatten()[slots]
+        for r in range(0, routed, 64):
+            part = slice(r, min(r + 64, routed))
+            assert torch.equal(Y[part], (X[slots[part] // 2].float() * W[experts[part], 0].float()).to(dtype))
+    ops.check_status()
+    del X, W, Y
+    torch.cuda.empty_cache()
