@@ -1197,7 +1197,7 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const __grid_constant_
   if (tid < kGTile) src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
   __syncthreads();
   const T* W = static_cast<const T*>(p.W) + e * p.w_expert;
-  const int n0 = blockIdx.y * kGTile, tx = tid & 15, ty = tid >> 4;
+  const int n0 = column_tile() * kGTile, tx = tid & 15, ty = tid >> 4;
   // of A (and of weights [E, N, C]): row tid / 4, elements 4 (tid mod 4) ..;  of weights [E, C, N]: row tid / 16
   const int lr = tid >> 2, lc = (tid & 3) * 4, row = src[lr];
   const T* a_row = static_cast<const T*>(p.A) + (row < 0 ? 0 : row) * p.a_row;
@@ -1396,7 +1396,7 @@ __global__ void __launch_bounds__(kWideThreads, 3) ragged_rows_f32_kernel(const 
   if (e < 0) return;
   src[tid] = first + tid >= end ? -1 : p.slots ? p.by_k.quotient(p.slots[first + tid]) : first + tid;
   const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
-  const int n0 = blockIdx.y * kGTile, tx = tid & 7, ty = tid >> 3;
+  const int n0 = column_tile() * kGTile, tx = tid & 7, ty = tid >> 3;
   // X (and weights [E, N, C]): rows tid / 4 and every 32nd from there, elements 4 (tid mod 4) ..;  weights [E, C, N]: rows tid / 16 and 8 more
   const int lr = tid >> 2, lc = (tid & 3) * 4, wr = tid >> 4, wc = (tid & 15) * 4;
   const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
@@ -1485,7 +1485,7 @@ template <bool NC, int G, int R>
 __device__ __forceinline__ void mid_tile(const RaggedParams& p, float* ring, const int* src, int e, int first, int rows) {
   constexpr int kThreads = 64 * G;
   constexpr int kX = (R * 32 + kThreads - 1) / kThreads, kWn = kMidCols * 8 / kThreads, kWc = kMidStep * 16 / kThreads;
-  const int tid = threadIdx.x, tx = tid & 15, ty = (tid >> 4) & 3, group = tid >> 6, n0 = blockIdx.y * kMidCols;
+  const int tid = threadIdx.x, tx = tid & 15, ty = (tid >> 4) & 3, group = tid >> 6, n0 = column_tile() * kMidCols;
   const float* A = static_cast<const float*>(p.A);
   const float* W = static_cast<const float*>(p.W) + e * p.w_expert;
   const bool a_wide = p.a_row % 4 == 0 && (reinterpret_cast<uintptr_t>(p.A) & 15u) == 0;
@@ -1957,21 +1957,21 @@ static bool wide_dweight(const RaggedParams& p) { return p.C > 64; }
 
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st) {
   if (dtype == EGS_F32 && wide_rows(p)) {
-    const dim3 grid(static_cast<unsigned>(blocks_bound(p, kWide)), (p.N + kGTile - 1) / kGTile);
+    const dim3 grid = rows_by_columns(blocks_bound(p, kWide), (p.N + kGTile - 1) / kGTile);
     count_launch();
     return launch_kernel(ragged_rows_f32_kernel, grid, kWideThreads, 0, st, true, p);
   }
   if (dtype == EGS_F32) {
-    const dim3 grid(static_cast<unsigned>(blocks_bound(p, kMidRows)), (p.N + kMidCols - 1) / kMidCols);
+    const dim3 grid = rows_by_columns(blocks_bound(p, kMidRows), (p.N + kMidCols - 1) / kMidCols);
     count_launch();
     auto go = [&](auto kernel, int threads) { return launch_kernel(kernel, grid, threads, kMidSmem, st, true, p); };
     const long long mean = p.rows / kMidRows + p.E / 2, blocks = mean > p.E ? mean : p.rows < p.E ? p.rows : p.E;
-    if (blocks * grid.y < 3 * 148) return p.nc ? go(ragged_rows_mid_kernel<true, 4>, 256) : go(ragged_rows_mid_kernel<false, 4>, 256);
+    if (blocks * grid.y * grid.z < 3 * 148) return p.nc ? go(ragged_rows_mid_kernel<true, 4>, 256) : go(ragged_rows_mid_kernel<false, 4>, 256);
     return p.nc ? go(ragged_rows_mid_kernel<true, 2>, 128) : go(ragged_rows_mid_kernel<false, 2>, 128);
   }
   long long blocks = blocks_bound(p, kGTile);
   if (blocks < 1) blocks = 1;
-  const dim3 grid(static_cast<unsigned>(blocks), (p.N + kGTile - 1) / kGTile);
+  const dim3 grid = rows_by_columns(blocks, (p.N + kGTile - 1) / kGTile);
   count_launch();
   auto go = [&](auto kernel) { return launch_kernel(kernel, grid, 256, 0, st, true, p); };
   if (dtype == EGS_I8)

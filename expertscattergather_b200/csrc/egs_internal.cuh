@@ -54,9 +54,15 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Packed {
 struct GridThreads {
   long long mine, all;
   __device__ __forceinline__ GridThreads()
-      : mine((static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x),
-        all(static_cast<long long>(gridDim.x) * gridDim.y * blockDim.x) {}
+      : mine((static_cast<long long>(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x),
+        all(static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z * blockDim.x) {}
 };
+// Grids of row blocks by column tiles, of which y alone holds 65535; this CTA's column tile, which may lie behind the last one.
+inline dim3 rows_by_columns(long long blocks, int tiles) {
+  const int z = (tiles + 65534) / 65535;
+  return dim3(static_cast<unsigned>(blocks), (tiles + z - 1) / z, z);
+}
+__device__ __forceinline__ int column_tile() { return static_cast<int>(blockIdx.z * gridDim.y + blockIdx.y); }
 
 // Reads Ind[pos] for any of the three index widths.
 __device__ __forceinline__ long long load_index(const void* ind, int index_dtype, long long pos) {

@@ -297,3 +297,26 @@ def test_zeros_of_wide_rows(cuda_device, dtype, E, N):
     ops.check_status()
     del X, W, Y
     torch.cuda.empty_cache()
+
+
+# more column tiles than a grid's second dimension holds; few rows an expert, a block of 128 of them, tens
+@pytest.mark.parametrize("tokens,E", [(40, 2), (200, 1), (2, 9)])
+@pytest.mark.parametrize("dtype,path", [(torch.float32, "auto"), (torch.bfloat16, "generic"), (torch.bfloat16, "auto")])
+def test_columns_beyond_65535_tiles(cuda_device, tokens, E, dtype, path):
+    g, N = gen(tokens), 65535 * 64 + 72
+    ids = torch.randint(0, E, (tokens, 1), device="cuda", generator=g)
+    ids[1] = -1
+    plan = ops.plan_experts(ids, E)
+    X, W = randn(g, tokens, 1, dtype=dtype), torch.rand(E, 1, N, device="cuda", generator=g).to(dtype)
+    for w, layout in ((W, "cn"), (W.view(E, N, 1), "nc")):
+        Y = ops.expert_matmul(X, w, plan, w_layout=layout, path=path)
+        assert not Y[-1].any()
+        for r, slot in enumerate(plan.slots[:-1].tolist()):
+            assert torch.equal(Y[r], (X[slot].float() * W[ids[slot, 0], 0].float()).to(dtype))
+        del Y
+    q = torch.ones(tokens, 16, device="cuda", dtype=torch.int8)
+    Wq = torch.randint(-9, 9, (N, 16), device="cuda", generator=g).to(torch.int8)
+    one = torch.ones(N, device="cuda")
+    assert torch.equal(ops.matmul_int8(q, one[:tokens], Wq, one, out_dtype=torch.float32, path=path), Wq.sum(-1).float().expand(tokens, N))
+    ops.check_status()
+    torch.cuda.empty_cache()
