@@ -89,6 +89,7 @@ StatusRef status_ref(int32_t* status_word) {
 
 int fail_cuda(cudaError_t err, const char* where) {
   std::snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", where, cudaGetErrorString(err));
+  cudaGetLastError();            // (reported here, and not by whoever looks at the thread's last error next)
   return EGS_ERR_CUDA;
 }
 

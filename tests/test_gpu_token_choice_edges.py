@@ -320,3 +320,13 @@ def test_columns_beyond_65535_tiles(cuda_device, tokens, E, dtype, path):
     assert torch.equal(ops.matmul_int8(q, one[:tokens], Wq, one, out_dtype=torch.float32, path=path), Wq.sum(-1).float().expand(tokens, N))
     ops.check_status()
     torch.cuda.empty_cache()
+
+
+def test_a_refused_launch_is_reported_once(cuda_device):
+    """Columns of more tiles than a grid's second dimension holds: the launch is refused, and the next operator has nothing to do with it."""
+    N = 1 << 24
+    X, W = torch.ones(1, 4, 1, device="cuda"), torch.ones(1, 1, N, device="cuda")
+    with pytest.raises(RuntimeError, match="invalid"):
+        ops.gather_gemm(X, W, torch.zeros(1, 1, 1, device="cuda", dtype=torch.int32), path="generic")
+    assert (X + 1).sum().item() == 8
+    ops.check_status()
