@@ -1155,9 +1155,7 @@ __device__ __forceinline__ void load4(const T* p, int left, bool wide, typename 
 template <typename T>
 __device__ __forceinline__ void zero_unrouted(const RaggedParams& p, int routed) {
   T* out = static_cast<T*>(p.Out);
-  const long long begin = static_cast<long long>(routed) * p.N, end = static_cast<long long>(p.rows) * p.N;
-  const GridThreads threads;
-  for (long long i = begin + threads.mine; i < end; i += threads.all) out[i] = from_f32<T>(0.f);
+  if (routed < p.rows) zero_by_grid(out + static_cast<long long>(routed) * p.N, out + static_cast<long long>(p.rows) * p.N);
 }
 
 // A step in shared memory, contraction by contraction; two of them, so that the next one is written while this one is read.

@@ -61,9 +61,7 @@ template <typename OutT>
 __device__ __forceinline__ void few_zero(const RaggedParams& p) {
   if (!p.offsets) return;
   OutT* out = static_cast<OutT*>(p.Out);
-  const long long begin = static_cast<long long>(p.offsets[p.E]) * p.N, end = static_cast<long long>(p.rows) * p.N;
-  const GridThreads threads;
-  for (long long i = begin + threads.mine; i < end; i += threads.all) out[i] = from_f32<OutT>(0.f);
+  if (const int routed = p.offsets[p.E]; routed < p.rows) zero_by_grid(out + static_cast<long long>(routed) * p.N, out + static_cast<long long>(p.rows) * p.N);
 }
 
 template <typename T, int V>

@@ -50,13 +50,14 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Packed {
   }
 };
 
-// This thread's number among those of a grid, and how many there are (wide outputs have more than 2^31 of them).
-struct GridThreads {
-  long long mine, all;
-  __device__ __forceinline__ GridThreads()
-      : mine((static_cast<long long>(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x),
-        all(static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z * blockDim.x) {}
-};
+// Zeros in [begin, end), by all threads of a grid (of which wide outputs have more than 2^31).  A function of its own: inlined, its 64-bit
+// counters took registers that the kernels around it then spilled.
+template <typename T>
+__device__ __noinline__ void zero_by_grid(T* begin, T* end) {
+  const long long mine = (static_cast<long long>(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
+  const long long all = static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z * blockDim.x;
+  for (T* p = begin + mine; p < end; p += all) *p = from_f32<T>(0.f);
+}
 // Grids of row blocks by column tiles, of which y alone holds 65535; this CTA's column tile, which may lie behind the last one.
 inline dim3 rows_by_columns(long long blocks, int tiles) {
   const int z = (tiles + 65534) / 65535;
