@@ -762,8 +762,9 @@ cudaError_t launch_by_pair(const RaggedParams& p, const RaggedTiles& q, bool pai
 }
 
 // The tile that takes the least time by this estimate, in clocks.  A step of a CTA costs its bytes at 60 a clock (what the L2 gives all SMs) or its
-// MMAs where they take longer; a read-out, under the next tile's steps all but the last, `fixed` and 3000 or 4500 for 256 columns.  blocks(rows of
-// a tile): tiles of one column.  The widest tile on pairs or single CTAs moves the fewest bytes; another has to be a tenth faster.
+// MMAs where they take longer (two clocks a column in both types: 8-bit steps have twice the elements, at twice the rate); a read-out, under the
+// next tile's steps all but the last, `fixed` and 3000 or 4500 for 256 columns.  blocks(rows of a tile): tiles of one column.  The widest tile on
+// pairs or single CTAs moves the fewest bytes; another has to be a tenth faster.
 struct TileChoice {
   bool pair;
   int BN;
@@ -777,7 +778,7 @@ TileChoice choose_tile(int N, long long steps, int elem, bool pairs, Blocks&& bl
   for (const TileChoice& c : kCandidates) {
     if ((c.BN > 64 && N <= c.BN / 2) || (c.pair && !pairs)) continue;
     const int workers = c.pair ? kSmCount / 2 : kSmCount;
-    const double bytes = kATile + b_tile_bytes(c.pair ? c.BN / 2 : c.BN, false), mma = elem * c.BN;
+    const double bytes = kATile + b_tile_bytes(c.pair ? c.BN / 2 : c.BN, false), mma = 2 * c.BN;
     const double work = (bytes / 60 > mma ? bytes / 60 : mma) * steps, out = fixed + wide * c.BN / 256;
     const long long units = static_cast<long long>(blocks(c.pair ? 256 : 128) * ((N + c.BN - 1) / c.BN));
     const double time = static_cast<double>((units + workers - 1) / workers) * (work > out ? work : out) + out;
