@@ -32,8 +32,8 @@ EXPORTS = (
     "egs_index_csr_scratch_bytes", "egs_index_compact", "egs_gemm_scatter_prepared", "egs_gemm_scatter_csr",
     "egs_set_status_mirror", "egs_expert_row_sum",
     "egs_route_tokens", "egs_route_tokens_backward", "egs_plan_experts", "egs_plan_workspace_bytes", "egs_expert_matmul",
-    "egs_expert_matmul_workspace_bytes", "egs_expert_dweight", "egs_expert_dweight_workspace_bytes", "egs_combine",
-    "egs_combine_backward", "egs_quantize_rows", "egs_expert_matmul_int8",
+    "egs_expert_matmul_out", "egs_expert_matmul_workspace_bytes", "egs_expert_dweight", "egs_expert_dweight_workspace_bytes", "egs_combine",
+    "egs_combine_out", "egs_combine_backward", "egs_quantize_rows", "egs_expert_matmul_int8",
 )
 
 
@@ -127,10 +127,12 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("egs_plan_experts", i, [vp, i64, i, vp, vp, vp, vp, sz, vp, vp]),
             ("egs_plan_workspace_bytes", sz, [i64, i]),
             ("egs_expert_matmul", i, [vp, vp, vp, vp, vp, ragged, i, i, i, i, vp, sz, vp, vp]),
+            ("egs_expert_matmul_out", i, [vp, vp, vp, vp, vp, ragged, i, i, i, i, i, vp, sz, vp, vp]),
             ("egs_expert_matmul_workspace_bytes", sz, [ragged, i, i, i]),
             ("egs_expert_dweight", i, [vp, vp, vp, vp, vp, ragged, i, i, i, vp, sz, vp, vp]),
             ("egs_expert_dweight_workspace_bytes", sz, [ragged, i, i]),
             ("egs_combine", i, [vp, vp, vp, vp, i64, i64, i64, i, i, vp]),
+            ("egs_combine_out", i, [vp, vp, vp, vp, i64, i64, i64, i, i, i, vp]),
             ("egs_combine_backward", i, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i, i, vp]),
             ("egs_quantize_rows", i, [vp, vp, vp, i64, i64, i64, i64, i, vp]),
             ("egs_expert_matmul_int8", i, [vp, vp, i64, vp, vp, i64, vp, vp, vp, ragged, i, i, i, vp, vp])):

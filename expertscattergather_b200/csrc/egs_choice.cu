@@ -624,7 +624,7 @@ struct CombineParams {
   const void* dOut;        // backward: token rows
   void* dweights;          // backward: [tokens, k]
   int tokens, k, N, vecs;  // vecs: vectors of a row
-  int w_f32;               // weights (and their gradient) in float32, else in the rows' type
+  int w_f32;               // weights (and their gradient) in float32, else in the output's type
   Div by_blocks;           // forward: blocks of 32 vectors of a row
   Div by_k;                // backward
   int work;                // forward: tokens * blocks
@@ -640,7 +640,8 @@ __device__ __forceinline__ float weight_of(const CombineParams& p, long long slo
 // step before that.
 constexpr int kCombineStages = 4, kCombineAhead = kCombineStages - 1, kCombineWarps = 4, kCombineCtas = 148 * 6;
 
-template <typename T, int V>
+// T: the rows' type, O: the output's (and the weights', where those are not float32)
+template <typename T, typename O, int V>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __grid_constant__ CombineParams p) {
   using P = Packed<T, V>;
   static_assert(sizeof(P) == 16 || sizeof(P) == 8 || sizeof(P) == 4, "what cp.async copies");
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
   auto weight = [&](const Step& s) {
     int block;
     if (s.item >= items || lane >= 4 || s.group * 4 + lane >= p.k) return 0.f;
-    return weight_of<T>(p, static_cast<long long>(place(s, &block)) * p.k + s.group * 4 + lane);
+    return weight_of<O>(p, static_cast<long long>(place(s, &block)) * p.k + s.group * 4 + lane);
   };
   unsigned present[kCombineStages];            // choices of a stage that have a row
   int pos = position();
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
         const int c = (block * 32 * U + lane) * V;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (c + u * 32 * V < p.N) Vec<T, V>::store(static_cast<T*>(p.out) + t * p.N + c + u * 32 * V, sum[u]);
+          if (c + u * 32 * V < p.N) Vec<O, V>::store(static_cast<O*>(p.out) + t * p.N + c + u * 32 * V, sum[u]);
       }
       use = after;
       w = w_next;
@@ -753,20 +754,20 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
 }
 
 // Rows that do not even begin on 4 bytes: 64 threads have a token, each every 64th column.
-template <typename T>
+template <typename T, typename O>
 __global__ void __launch_bounds__(256) combine_columns_kernel(const __grid_constant__ CombineParams p) {
   pdl_wait();
   pdl_trigger();
   const long long t = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 64;
   if (t >= p.tokens) return;
   const int* pos = p.position + t * p.k;
-  T* out = static_cast<T*>(p.out) + t * p.N;
+  O* out = static_cast<O*>(p.out) + t * p.N;
   for (int c0 = threadIdx.x & 63; c0 < p.N; c0 += 256) {
     float sum[4] = {};
     for (int j = 0; j < p.k; ++j) {
       const int at = pos[j];
       if (at < 0) continue;
-      const float w = weight_of<T>(p, t * p.k + j);
+      const float w = weight_of<O>(p, t * p.k + j);
       const T* y = static_cast<const T*>(p.Y) + static_cast<long long>(at) * p.N;
       float v[4];
 #pragma unroll
@@ -776,14 +777,14 @@ __global__ void __launch_bounds__(256) combine_columns_kernel(const __grid_const
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (c0 + 64 * i < p.N) out[c0 + 64 * i] = from_f32<T>(sum[i]);
+      if (c0 + 64 * i < p.N) out[c0 + 64 * i] = from_f32<O>(sum[i]);
   }
 }
 
 // Rows of at most 32 vectors: 2^lanes_log2 threads have a token, one vector each; four rows are on their way, and the next four places.  bf16,
 // this and the kernel above, which leaves lanes without work: 32768 tokens of eight rows of 64 16 and 33 us, of one row 10 and 18; 21419 of eight
 // rows of 152 25 and 27; from 64 vectors on no faster (32768 of four rows of 512: 43 and 42).
-template <typename T, int V>
+template <typename T, typename O, int V>
 __global__ void __launch_bounds__(256) combine_narrow_kernel(const __grid_constant__ CombineParams p, int lanes_log2) {
   using P = Packed<T, V>;
   pdl_wait();
@@ -808,7 +809,7 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(const __grid_consta
       at[j] = coming[j];
       if (at[j] < 0) continue;
       y[j] = Y[static_cast<long long>(at[j]) * p.vecs];
-      w[j] = weight_of<T>(p, slot + j0 + j);
+      w[j] = weight_of<O>(p, slot + j0 + j);
     }
     places(j0 + 4);
 #pragma unroll
@@ -818,7 +819,7 @@ __global__ void __launch_bounds__(256) combine_narrow_kernel(const __grid_consta
       for (int v = 0; v < V; ++v) sum[v] = fmaf(w[j], y[j].get(v), sum[v]);
     }
   }
-  Vec<T, V>::store(static_cast<T*>(p.out) + (t * p.vecs + c) * V, sum);
+  Vec<O, V>::store(static_cast<O*>(p.out) + (t * p.vecs + c) * V, sum);
 }
 
 // A warp has a slot: dY = weight * dOut of its token, dweight = the product of the two rows.  Slots without an expert have a row of
@@ -1761,7 +1762,7 @@ cudaError_t by_type(int dtype, F16&& f16, BF16&& bf16, F32&& f32) {
   return dtype == EGS_F16 ? f16() : dtype == EGS_BF16 ? bf16() : f32();
 }
 
-template <typename T, int V>
+template <typename T, typename O, int V>
 cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
   p.vecs = p.N / V;
   if (backward) {
@@ -1776,34 +1777,34 @@ cudaError_t combine_v(CombineParams& p, bool backward, cudaStream_t st) {
     return launch_kernel(combine_backward_kernel<T, V>, static_cast<unsigned>((slots + 7) / 8), 256, 0, st, true, p);
   }
   if constexpr (sizeof(T) * V < 4) {
-    return launch_kernel(combine_columns_kernel<T>, (p.tokens + 3) / 4, 256, 0, st, true, p);
+    return launch_kernel(combine_columns_kernel<T, O>, (p.tokens + 3) / 4, 256, 0, st, true, p);
   } else {
     if (p.vecs <= 32) {
       int lanes_log2 = 2;
       while ((1 << lanes_log2) < p.vecs) ++lanes_log2;
-      return launch_kernel(combine_narrow_kernel<T, V>, static_cast<unsigned>(((static_cast<long long>(p.tokens) << lanes_log2) + 255) / 256), 256, 0, st, true, p, lanes_log2);
+      return launch_kernel(combine_narrow_kernel<T, O, V>, static_cast<unsigned>(((static_cast<long long>(p.tokens) << lanes_log2) + 255) / 256), 256, 0, st, true, p, lanes_log2);
     }
     const int blocks = (p.vecs * static_cast<int>(sizeof(T) * V) + 511) / 512;
     p.by_blocks = Div(blocks);
     p.work = p.tokens * blocks;
     const int ctas = (p.work + kCombineWarps - 1) / kCombineWarps;
-    return launch_kernel(combine_kernel<T, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
+    return launch_kernel(combine_kernel<T, O, V>, ctas < kCombineCtas ? ctas : kCombineCtas, kCombineWarps * 32, 0, st, true, p);
   }
 }
 // The widest vectors that rows of N elements are whole numbers of and begin on.
-template <typename T>
+template <typename T, typename O = T>
 cudaError_t combine_t(CombineParams& p, bool backward, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   auto fits = [&](int v) {
-    const uintptr_t all = reinterpret_cast<uintptr_t>(p.Y) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.dOut);
-    return p.N % v == 0 && all % (v * sizeof(T)) == 0;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.Y) | reinterpret_cast<uintptr_t>(p.dOut);
+    return p.N % v == 0 && all % (v * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.out) % (v * sizeof(O)) == 0;
   };
-  if (fits(V)) return combine_v<T, V>(p, backward, st);
-  if (fits(V / 2)) return combine_v<T, V / 2>(p, backward, st);
+  if (fits(V)) return combine_v<T, O, V>(p, backward, st);
+  if (fits(V / 2)) return combine_v<T, O, V / 2>(p, backward, st);
   if constexpr (V > 4) {
-    if (fits(V / 4)) return combine_v<T, V / 4>(p, backward, st);
+    if (fits(V / 4)) return combine_v<T, O, V / 4>(p, backward, st);
   }
-  return combine_v<T, 1>(p, backward, st);
+  return combine_v<T, O, 1>(p, backward, st);
 }
 
 template <typename T, int V>
@@ -1903,10 +1904,12 @@ cudaError_t launch_plan_experts(const int* experts, long long n, int E, int* off
 }
 
 cudaError_t launch_combine(const void* Y, const void* weights, const int* position, void* out, long long tokens, int k, int N, int dtype,
-                           int w_f32, cudaStream_t st) {
+                           int w_f32, int out_dtype, cudaStream_t st) {
   CombineParams p{};
   p.Y = Y; p.weights = weights; p.position = position; p.out = out; p.tokens = static_cast<int>(tokens); p.k = k; p.N = N; p.w_f32 = w_f32;
   count_launch();
+  if (dtype == EGS_F32 && out_dtype != EGS_F32)
+    return out_dtype == EGS_F16 ? combine_t<float, __half>(p, false, st) : combine_t<float, __nv_bfloat16>(p, false, st);
   return by_type(dtype, [&] { return combine_t<__half>(p, false, st); }, [&] { return combine_t<__nv_bfloat16>(p, false, st); },
                  [&] { return combine_t<float>(p, false, st); });
 }
@@ -1975,6 +1978,7 @@ cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, 
   if (dtype == EGS_I8)
     return by_type(out_dtype, [&] { return go(ragged_rows_kernel<int8_t, __half>); }, [&] { return go(ragged_rows_kernel<int8_t, __nv_bfloat16>); },
                    [&] { return go(ragged_rows_kernel<int8_t, float>); });
+  if (out_dtype == EGS_F32) return dtype == EGS_F16 ? go(ragged_rows_kernel<__half, float>) : go(ragged_rows_kernel<__nv_bfloat16, float>);
   return dtype == EGS_F16 ? go(ragged_rows_kernel<__half, __half>) : go(ragged_rows_kernel<__nv_bfloat16, __nv_bfloat16>);
 }
 

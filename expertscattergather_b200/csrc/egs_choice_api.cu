@@ -111,9 +111,10 @@ size_t egs_expert_matmul_workspace_bytes(const egs_ragged* dims, int rows, int w
          (w_layout == EGS_W_NC ? copy_bytes(dims->E * dims->N, dims->C) : copy_bytes(dims->E * dims->C, dims->N));
 }
 
-int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
-                      int w_layout, int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream) {
-  if (!valid_dtype(dtype) || !valid_path(path) || !valid_layout(w_layout) || !valid_rows(rows)) return EGS_ERR_INVALID_ARGUMENT;
+int egs_expert_matmul_out(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
+                          int w_layout, int dtype, int out_dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream) {
+  if (!valid_dtype(dtype) || (out_dtype != dtype && out_dtype != EGS_F32) || !valid_path(path) || !valid_layout(w_layout) || !valid_rows(rows))
+    return EGS_ERR_INVALID_ARGUMENT;
   if (int rc = check_ragged(dims)) return rc;
   RaggedParams p = ragged(*dims, rows);
   if (p.rows == 0 || p.N == 0) return EGS_OK;
@@ -125,8 +126,8 @@ int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, cons
   const cudaStream_t st = stream_of(cuda_stream);
   const bool able = device_is_sm100() && dtype != EGS_F32 && p.C > 0 && aligned16(X) && aligned16(W) && tiles_fit(p);
   if (path == EGS_PATH_TENSOR && !able) return EGS_ERR_UNSUPPORTED;
-  if (path == EGS_PATH_AUTO && p.C > 0 && few_rows_fit(p, dtype)) return done(launch_few_rows(p, dtype, dtype, st), "expert_matmul launch");
-  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_rows(p, dtype, dtype, st), "expert_matmul launch");
+  if (path == EGS_PATH_AUTO && p.C > 0 && few_rows_fit(p, dtype)) return done(launch_few_rows(p, dtype, out_dtype, st), "expert_matmul launch");
+  if (!able || path == EGS_PATH_GENERIC) return done(launch_ragged_rows(p, dtype, out_dtype, st), "expert_matmul launch");
   const size_t need = egs_expert_matmul_workspace_bytes(dims, rows, w_layout, dtype);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return EGS_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
@@ -134,7 +135,12 @@ int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, cons
   const PadRows copies[2] = {rows_copy, padded(&p.W, &p.w_row, dims->E * (p.nc ? p.N : p.C), p.w_row, &ws)};
   if (cudaError_t err = launch_pad_rows(copies, st); err != cudaSuccess) return fail_cuda(err, "expert_matmul copies");
   p.w_expert = p.w_row * (p.nc ? p.N : p.C);
-  return done(launch_ragged_rows_tensor(p, dtype, dtype, st), "expert_matmul launch");
+  return done(launch_ragged_rows_tensor(p, dtype, out_dtype, st), "expert_matmul launch");
+}
+
+int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
+                      int w_layout, int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream) {
+  return egs_expert_matmul_out(X, W, offsets, slots, Y, dims, rows, w_layout, dtype, dtype, path, workspace, workspace_bytes, status_word, cuda_stream);
 }
 
 size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype) {
@@ -173,19 +179,25 @@ int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, co
   return done(launch_ragged_dweight_tensor(p, dtype, ws, st), "expert_dweight launch");
 }
 
-int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
-                int weights_dtype, void* cuda_stream) {
+int egs_combine_out(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
+                    int weights_dtype, int out_dtype, void* cuda_stream) {
   const egs_ragged d{tokens, k, EGS_MAX_EXPERTS, 0, N};
   if (int rc = check_ragged(&d)) return rc;
-  if (!valid_dtype(dtype) || (weights && weights_dtype != EGS_F32 && weights_dtype != dtype)) return EGS_ERR_INVALID_ARGUMENT;
+  if (!valid_dtype(dtype) || !valid_dtype(out_dtype) || (out_dtype != dtype && dtype != EGS_F32) || (weights && weights_dtype != EGS_F32 && weights_dtype != out_dtype))
+    return EGS_ERR_INVALID_ARGUMENT;
   if (tokens == 0 || N == 0) return EGS_OK;
   if (tokens * (N / 32 + 1) > kInt32Max) return EGS_ERR_TOO_LARGE;
   if (!out || (k > 0 && (!Y || !position))) return EGS_ERR_INVALID_ARGUMENT;
   // (the kernels go from choice to choice: a token without any is not for them)
-  if (k == 0) return done(launch_fill_zero(out, static_cast<size_t>(tokens) * N * (dtype == EGS_F32 ? 4 : 2), stream_of(cuda_stream)), "combine fill");
-  return done(launch_combine(Y, weights, position, out, tokens, static_cast<int>(k), static_cast<int>(N), dtype, weights_dtype == EGS_F32,
+  if (k == 0) return done(launch_fill_zero(out, static_cast<size_t>(tokens) * N * (out_dtype == EGS_F32 ? 4 : 2), stream_of(cuda_stream)), "combine fill");
+  return done(launch_combine(Y, weights, position, out, tokens, static_cast<int>(k), static_cast<int>(N), dtype, weights_dtype == EGS_F32, out_dtype,
                              stream_of(cuda_stream)),
               "combine launch");
+}
+
+int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
+                int weights_dtype, void* cuda_stream) {
+  return egs_combine_out(Y, weights, position, out, tokens, k, N, dtype, weights_dtype, dtype, cuda_stream);
 }
 
 int egs_combine_backward(const void* dOut, const void* Y, const void* weights, const int32_t* position, void* dY, void* dweights,

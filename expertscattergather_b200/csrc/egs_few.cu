@@ -159,7 +159,7 @@ struct CnShared {
 };
 
 // Rows first .. first + M - 1 (as in few_nc) times LANES * V columns from n0 on.  sums: [warps][M][LANES * V]
-template <typename T, int V, int LANES, int M>
+template <typename T, typename OutT, int V, int LANES, int M>
 __device__ __forceinline__ void few_cn(const RaggedParams& p, const Segment& s, CnShared<LANES>* sh, float* sums, int first, int n0) {
   using P = Packed<T, V>;
   constexpr int kFewPart = few_part(LANES), kGroups = kFewCnThreads / LANES, kWidth = LANES * V, kWarps = kFewCnThreads / 32;
@@ -216,25 +216,25 @@ __device__ __forceinline__ void few_cn(const RaggedParams& p, const Segment& s, 
       for (int v = 0; v < V; ++v) sums[((tid >> 5) * M + m) * kWidth + l * V + v] = acc[m][v];
   }
   __syncthreads();
-  T* out = static_cast<T*>(p.Out);
+  OutT* out = static_cast<OutT*>(p.Out);
   for (int i = tid; i < M * kWidth; i += kFewCnThreads) {
     const int m = i / kWidth, col = n0 + i % kWidth;
     if (first + m >= s.end || col >= p.N) continue;
     float t = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) t += sums[w * M * kWidth + i];
-    out[static_cast<long long>(first + m) * p.N + col] = from_f32<T>(t);
+    out[static_cast<long long>(first + m) * p.N + col] = from_f32<OutT>(t);
   }
 }
 
-template <typename T, int V, int LANES>
+template <typename T, typename OutT, int V, int LANES>
 __global__ void __launch_bounds__(kFewCnThreads, 1) few_rows_cn_kernel(const __grid_constant__ RaggedParams p) {
   __shared__ CnShared<LANES> sh;
   __shared__ float sums[kFewCnThreads / 32 * kFewRows * LANES * V];
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x;
-  few_zero<T>(p);
+  few_zero<OutT>(p);
   const Segment s = segment_of(p, &sh.segment);
   if (s.expert < 0) return;
   for (int r = s.first; r < s.end; r += kFewRows) {
@@ -244,8 +244,8 @@ __global__ void __launch_bounds__(kFewCnThreads, 1) few_rows_cn_kernel(const __g
       sh.src[tid] = p.slots ? p.by_k.quotient(p.slots[row]) : row;
     }
     __syncthreads();
-    if (r + 1 < s.end) few_cn<T, V, LANES, kFewRows>(p, s, &sh, sums, r, blockIdx.x * LANES * V);
-    else few_cn<T, V, LANES, 1>(p, s, &sh, sums, r, blockIdx.x * LANES * V);
+    if (r + 1 < s.end) few_cn<T, OutT, V, LANES, kFewRows>(p, s, &sh, sums, r, blockIdx.x * LANES * V);
+    else few_cn<T, OutT, V, LANES, 1>(p, s, &sh, sums, r, blockIdx.x * LANES * V);
   }
 }
 
@@ -255,19 +255,19 @@ cudaError_t few_nc_launch(const RaggedParams& p, int segments, cudaStream_t st) 
   return launch_kernel(few_rows_nc_kernel<T, OutT, V>, dim3((p.N + per_cta - 1) / per_cta, segments), kFewThreads, 0, st, true, p);
 }
 
-template <typename T, int V, int LANES>
+template <typename T, typename OutT, int V, int LANES>
 cudaError_t few_cn_lanes(const RaggedParams& p, int segments, cudaStream_t st) {
-  return launch_kernel(few_rows_cn_kernel<T, V, LANES>, dim3((p.N + LANES * V - 1) / (LANES * V), segments), kFewCnThreads, 0, st, true, p);
+  return launch_kernel(few_rows_cn_kernel<T, OutT, V, LANES>, dim3((p.N + LANES * V - 1) / (LANES * V), segments), kFewCnThreads, 0, st, true, p);
 }
-template <typename T, int V>
+template <typename T, typename OutT, int V>
 cudaError_t few_cn_launch(const RaggedParams& p, int segments, cudaStream_t st) {
   if constexpr (V == 1) {
-    return few_cn_lanes<T, 1, 32>(p, segments, st);
+    return few_cn_lanes<T, OutT, 1, 32>(p, segments, st);
   } else {
     auto enough = [&](int lanes) { return (p.N + lanes * V - 1) / (lanes * V) * segments >= 148; };
-    if (enough(16)) return few_cn_lanes<T, V, 16>(p, segments, st);
-    if (enough(8)) return few_cn_lanes<T, V, 8>(p, segments, st);
-    return few_cn_lanes<T, V, 4>(p, segments, st);
+    if (enough(16)) return few_cn_lanes<T, OutT, V, 16>(p, segments, st);
+    if (enough(8)) return few_cn_lanes<T, OutT, V, 8>(p, segments, st);
+    return few_cn_lanes<T, OutT, V, 4>(p, segments, st);
   }
 }
 
@@ -278,7 +278,7 @@ cudaError_t few_launch(const RaggedParams& p, int segments, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool rows_on = p.w_row % V == 0 && p.w_expert % V == 0 && on(p.W, 16);
   if (p.nc) return rows_on && p.a_row % V == 0 && on(p.A, 16) ? few_nc_launch<T, OutT, V>(p, segments, st) : few_nc_launch<T, OutT, 1>(p, segments, st);
-  if constexpr (sizeof(T) > 1) return rows_on && p.N % V == 0 ? few_cn_launch<T, V>(p, segments, st) : few_cn_launch<T, 1>(p, segments, st);
+  if constexpr (sizeof(T) > 1) return rows_on && p.N % V == 0 ? few_cn_launch<T, OutT, V>(p, segments, st) : few_cn_launch<T, OutT, 1>(p, segments, st);
   return cudaErrorInvalidValue;
 }
 
@@ -303,8 +303,9 @@ cudaError_t launch_few_rows(const RaggedParams& p, int dtype, int out_dtype, cud
     if (out_dtype == EGS_BF16) return few_launch<int8_t, __nv_bfloat16>(p, segments, st);
     return few_launch<int8_t, float>(p, segments, st);
   }
-  if (dtype == EGS_F16) return few_launch<__half, __half>(p, segments, st);
-  if (dtype == EGS_BF16) return few_launch<__nv_bfloat16, __nv_bfloat16>(p, segments, st);
+  const bool wide = out_dtype == EGS_F32;
+  if (dtype == EGS_F16) return wide ? few_launch<__half, float>(p, segments, st) : few_launch<__half, __half>(p, segments, st);
+  if (dtype == EGS_BF16) return wide ? few_launch<__nv_bfloat16, float>(p, segments, st) : few_launch<__nv_bfloat16, __nv_bfloat16>(p, segments, st);
   return few_launch<float, float>(p, segments, st);
 }
 

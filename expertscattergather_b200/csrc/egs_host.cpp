@@ -45,8 +45,8 @@ struct Api {
   X(egs_scatter_workspace_bytes) X(egs_dweight) X(egs_dweight_prezeroed) X(egs_dw_workspace_bytes)                          \
   X(egs_gather_scatter_pair) X(egs_fused_pair_eligible) X(egs_route_topk) X(egs_index_csr) X(egs_index_csr_scratch_bytes)   \
   X(egs_fill_zero) X(egs_set_status_mirror) X(egs_expert_row_sum)                                                          \
-  X(egs_route_tokens) X(egs_route_tokens_backward) X(egs_plan_experts) X(egs_plan_workspace_bytes) X(egs_expert_matmul)     \
-  X(egs_expert_matmul_workspace_bytes) X(egs_expert_dweight) X(egs_expert_dweight_workspace_bytes) X(egs_combine)           \
+  X(egs_route_tokens) X(egs_route_tokens_backward) X(egs_plan_experts) X(egs_plan_workspace_bytes) X(egs_expert_matmul_out) \
+  X(egs_expert_matmul_workspace_bytes) X(egs_expert_dweight) X(egs_expert_dweight_workspace_bytes) X(egs_combine_out)       \
   X(egs_combine_backward) X(egs_quantize_rows) X(egs_expert_matmul_int8)
 #define EGS_FIELD(name) decltype(&::name) name = nullptr;
   EGS_API(EGS_FIELD)

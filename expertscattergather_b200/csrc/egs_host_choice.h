@@ -126,10 +126,12 @@ void check_plan(const Call& c, const Tensor& offsets, const Tensor& slots, int64
 }
 
 Tensor expert_matmul(const Tensor& X, const Tensor& W, const Tensor& offsets, const Tensor& slots, int64_t tokens, int64_t k,
-                     const std::string& rows, int layout, int path) {
+                     const std::string& rows, int layout, int path, std::optional<at::ScalarType> out_dtype) {
   if (X.dim() < 1 || W.dim() != 3) value_error("expected X[..., C], W[E,.,.]");
   if (W.scalar_type() != X.scalar_type()) value_error("X and W must have the same dtype");
   const int dt = type_id(X.scalar_type()), rid = rows_id(rows);
+  const at::ScalarType out = out_dtype.value_or(X.scalar_type());
+  if (out != X.scalar_type() && out != at::kFloat) value_error("out_dtype must be X's dtype or float32");
   Call c(X, W);
   const WDims w = w_dims(W, layout);
   check_plan(c, offsets, slots, w.E, tokens * k);
@@ -137,12 +139,12 @@ Tensor expert_matmul(const Tensor& X, const Tensor& W, const Tensor& offsets, co
   if (X.size(-1) != w.C || X.numel() != want * w.C)
     value_error("shape mismatch: X" + shape_of(X) + " W" + shape_of(W) + " (" + layout_name(layout) + ") for " + std::to_string(want) + " rows");
   const Tensor Xc = whole(X), Wc = whole(W);
-  Tensor Y = empty({tokens * k, w.N}, X.scalar_type(), c.idx);
+  Tensor Y = empty({tokens * k, w.N}, out, c.idx);
   const egs_ragged d{tokens, k, w.E, w.C, w.N};
   const size_t bytes = api.egs_expert_matmul_workspace_bytes(&d, rid, layout, dt);
   const Tensor ws = scratch(bytes, c.idx);
-  check(api.egs_expert_matmul(ptr(Xc), ptr(Wc), offsets.data_ptr<int>(), slots.data_ptr<int>(), ptr(Y), &d, rid, layout, dt, path_of(path), ptr(ws),
-                              bytes, c.status(), c.stream),
+  check(api.egs_expert_matmul_out(ptr(Xc), ptr(Wc), offsets.data_ptr<int>(), slots.data_ptr<int>(), ptr(Y), &d, rid, layout, dt, type_id(out),
+                                  path_of(path), ptr(ws), bytes, c.status(), c.stream),
         "egs_expert_matmul");
   c.debug();
   return Y;
@@ -171,26 +173,29 @@ Tensor expert_dweight(const Tensor& X, const Tensor& dY, const Tensor& offsets, 
   return dW;
 }
 
-// weights [.., k] in float32 or the rows' type; undefined for none
-Tensor choice_weights(const OptTensor& weights, const Tensor& Y, int64_t n, int* type) {
+// weights [.., k] in float32 or in `other`; undefined for none
+Tensor choice_weights(const OptTensor& weights, const Tensor& Y, at::ScalarType other, int64_t n, int* type) {
   *type = EGS_F32;
   if (!weights || !weights->defined()) return Tensor();
   if (weights->numel() != n) value_error("weights must have one element a slot (" + std::to_string(n) + "), got " + shape_of(*weights));
-  if (weights->scalar_type() != at::kFloat && weights->scalar_type() != Y.scalar_type()) value_error("weights must be float32 or of the rows' dtype");
+  if (weights->scalar_type() != at::kFloat && weights->scalar_type() != other) value_error("weights must be float32 or of the rows' dtype");
   if (!weights->is_cuda() || weights->get_device() != Y.get_device()) throw std::runtime_error("all tensors must be on the same CUDA device");
   *type = type_id(weights->scalar_type());
   return weights->contiguous();
 }
 
-Tensor combine(const Tensor& Y, const OptTensor& weights, const Tensor& position, int64_t tokens, int64_t k) {
+Tensor combine(const Tensor& Y, const OptTensor& weights, const Tensor& position, int64_t tokens, int64_t k, std::optional<at::ScalarType> out_dtype) {
   if (Y.dim() != 2 || Y.size(0) != tokens * k || position.numel() != tokens * k || position.scalar_type() != at::kInt || !position.is_contiguous())
     value_error("expected Y[" + std::to_string(tokens * k) + ", N], got " + shape_of(Y));
   const int dt = type_id(Y.scalar_type());
+  const at::ScalarType type = out_dtype.value_or(Y.scalar_type());
+  const int ot = type_id(type);
+  if (ot != dt && dt != EGS_F32) value_error("out_dtype must be Y's dtype, or any where Y is float32");
   Call c(Y, position);
   int wt;
-  const Tensor w = choice_weights(weights, Y, tokens * k, &wt), Yc = whole(Y);
-  Tensor out = empty({tokens, Y.size(1)}, Y.scalar_type(), c.idx);
-  check(api.egs_combine(ptr(Yc), ptr(w), position.data_ptr<int>(), ptr(out), tokens, k, Y.size(1), dt, wt, c.stream), "egs_combine");
+  const Tensor w = choice_weights(weights, Y, type, tokens * k, &wt), Yc = whole(Y);
+  Tensor out = empty({tokens, Y.size(1)}, type, c.idx);
+  check(api.egs_combine_out(ptr(Yc), ptr(w), position.data_ptr<int>(), ptr(out), tokens, k, Y.size(1), dt, wt, ot, c.stream), "egs_combine");
   c.debug();
   return out;
 }
@@ -204,7 +209,7 @@ std::tuple<Tensor, OptTensor> combine_backward(const Tensor& dOut, const Tensor&
   const int dt = type_id(Y.scalar_type());
   Call c(Y, dOut, position);
   int wt;
-  const Tensor w = choice_weights(weights, Y, tokens * k, &wt), Yc = whole(Y), g = whole(dOut);
+  const Tensor w = choice_weights(weights, Y, Y.scalar_type(), tokens * k, &wt), Yc = whole(Y), g = whole(dOut);
   Tensor dY = empty({tokens * k, Y.size(1)}, Y.scalar_type(), c.idx);
   OptTensor dw;
   if (w.defined()) dw = empty(weights->sizes(), weights->scalar_type(), c.idx);

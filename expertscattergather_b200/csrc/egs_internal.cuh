@@ -295,13 +295,14 @@ cudaError_t launch_route_backward(const float* dweights, const void* logits, con
 size_t plan_workspace_ints(long long n, int E);
 cudaError_t launch_plan_experts(const int* experts, long long n, int E, int* offsets, int* slots, int* position, int* workspace,
                                 StatusRef status, cudaStream_t st);
+// out_dtype: the rows' type, or 16 bits of float32 rows
 cudaError_t launch_combine(const void* Y, const void* weights, const int* position, void* out, long long tokens, int k, int N, int dtype,
-                           int w_f32, cudaStream_t st);
+                           int w_f32, int out_dtype, cudaStream_t st);
 cudaError_t launch_combine_backward(const void* dOut, const void* Y, const void* weights, const int* position, void* dY, void* dweights,
                                     long long tokens, int k, int N, int dtype, int w_f32, cudaStream_t st);
 cudaError_t launch_quantize_rows(const void* X, int8_t* q, float* scale, long long rows, int C, long long x_stride, long long q_stride, int dtype,
                                  cudaStream_t st);
-// dtype EGS_I8: 8-bit operands with scales, products in out_dtype
+// dtype EGS_I8: 8-bit operands with scales, products in out_dtype; others: products in the operands' type or (16 bits) in float32
 cudaError_t launch_ragged_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
 cudaError_t launch_ragged_dweight(const RaggedParams& p, int dtype, void* workspace, cudaStream_t st);
 size_t generic_dweight_workspace(const RaggedParams& p, int dtype);

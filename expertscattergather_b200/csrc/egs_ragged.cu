@@ -17,6 +17,9 @@
 // the loads and the MMAs (65536 rows, 256 -> 1024: 43 us, 29 without read-out, 34 without its stores; stores straight from the registers, 32
 // bytes a lane, 49).  16-bit, 64 experts, 2048 -> 512: 65536 rows 110 us = 1.25 PFLOP/s, 131072 rows 210 us = 1.31, weight gradients 136 and
 // 240-260; 8-bit integers 60 and 105-130 us = 2.1-2.6 POP/s, 8192 rows of 4096 -> 4096 76-86 us = 3.2-3.6.
+// Rows leave in the operands' 16 bits, rounded once, or in float32 where the caller asks for that: a weighted sum of 16-bit rows is then off by
+// 0.0024 (relative 2-norm, bf16) where one rounding of the sum alone makes 0.0017, and a training step that has its rows in float32 takes half
+// as long again (65536 rows, 1024 x 256: 202 us -> 306; 131072 of 2048 x 512: 895 -> 1235), so the caller decides.
 // Brought to the L2 a tile ahead by bulk prefetches, gathered rows came later, not sooner (131072 rows: 220 -> 259 us).
 //
 // Experts differ in size, and a weight gradient's tile takes as long as its expert has rows.  So the contraction of a large expert is cut
@@ -836,8 +839,11 @@ cudaError_t launch_ragged_rows_tensor(const RaggedParams& p, int dtype, int out_
     if (out_dtype == EGS_BF16) return launch_by_pair<int8_t, __nv_bfloat16, false>(p, q, pair, units, maps, st);
     return launch_by_pair<int8_t, float, false>(p, q, pair, units, maps, st);
   }
-  if (dtype == EGS_F16) return launch_by_pair<__half, __half, false>(p, q, pair, units, maps, st);
-  return launch_by_pair<__nv_bfloat16, __nv_bfloat16, false>(p, q, pair, units, maps, st);
+  const bool wide = out_dtype == EGS_F32;
+  if (dtype == EGS_F16)
+    return wide ? launch_by_pair<__half, float, false>(p, q, pair, units, maps, st) : launch_by_pair<__half, __half, false>(p, q, pair, units, maps, st);
+  return wide ? launch_by_pair<__nv_bfloat16, float, false>(p, q, pair, units, maps, st)
+              : launch_by_pair<__nv_bfloat16, __nv_bfloat16, false>(p, q, pair, units, maps, st);
 }
 
 // (a range below this takes less time than the kernel that joins ranges)

@@ -464,11 +464,12 @@ def plan_experts(experts, E: int) -> ExpertPlan:
     return ExpertPlan(offsets, slots, position, experts.numel() // k, k, E)
 
 
-def expert_matmul(X, W, plan: ExpertPlan, *, rows="tokens", w_layout="cn", path=None):
+def expert_matmul(X, W, plan: ExpertPlan, *, rows="tokens", w_layout="cn", out_dtype=None, path=None):
     """``Y[r] = X[row(r)] @ Wv[expert(r)]`` for every sorted row r of ``plan`` (zeros for slots that were not routed): [tokens*k, N].
     ``rows``: 'tokens' - X holds token rows [..., C], gathered through the plan; 'sorted' - X holds sorted rows [tokens*k, C].
-    ``w_layout`` as in :func:`gather_gemm`.  Sums in float32, rounded once to X's dtype."""
-    return _host().expert_matmul(X, W, plan.offsets, plan.slots, plan.tokens, plan.k, rows, _layout(w_layout), _path(path))
+    ``w_layout`` as in :func:`gather_gemm`.  Sums in float32, rounded once to X's dtype, or with ``out_dtype=torch.float32`` not at all: what
+    is made of the rows (:func:`combine` has an ``out_dtype`` too) is then rounded once, for twice the bytes of 16-bit rows."""
+    return _host().expert_matmul(X, W, plan.offsets, plan.slots, plan.tokens, plan.k, rows, _layout(w_layout), _path(path), out_dtype)
 
 
 def expert_dweight(X, dY, plan: ExpertPlan, *, rows="tokens", path=None):
@@ -477,10 +478,11 @@ def expert_dweight(X, dY, plan: ExpertPlan, *, rows="tokens", path=None):
     return _host().expert_dweight(X, dY, plan.offsets, plan.slots, plan.tokens, plan.k, rows, _path(path))
 
 
-def combine(Y, weights, plan: ExpertPlan):
+def combine(Y, weights, plan: ExpertPlan, *, out_dtype=None):
     """``out[t] = sum_j weights[t, j] * Y[position[t, j]]``: sorted rows [tokens*k, N] -> token rows [tokens, N]; float32 in the order of
-    j, rounded once.  ``weights`` [..., k] in float32 or Y's dtype, None for ones.  Slots that were not routed add nothing."""
-    return _host().combine(Y, weights, plan.position, plan.tokens, plan.k)
+    j, rounded once, to Y's dtype or, where Y is float32, to ``out_dtype``.  ``weights`` [..., k] in float32 or the output's dtype, None for ones.
+    Slots that were not routed add nothing."""
+    return _host().combine(Y, weights, plan.position, plan.tokens, plan.k, out_dtype)
 
 
 def combine_backward(dOut, Y, weights, plan: ExpertPlan):

@@ -43,43 +43,49 @@ class RouteTokensFunction(torch.autograd.Function):
 
 
 class ExpertMatmulFunction(torch.autograd.Function):
-    """``apply(X, W, plan, rows) -> Y`` (``ops.expert_matmul``, W [E, C, N])."""
+    """``apply(X, W, plan, rows, out_dtype=None) -> Y`` (``ops.expert_matmul``, W [E, C, N]).  With float32 rows of 16-bit tensors the rows of
+    dX are float32 too until they have been summed; dY is rounded to the tensors' type, as what the tensor cores multiply."""
 
     @staticmethod
-    def forward(ctx, X, W, plan, rows):
+    def forward(ctx, X, W, plan, rows, out_dtype=None):
         ctx.save_for_backward(X, W)
-        ctx.plan, ctx.rows = plan, rows
-        return ops.expert_matmul(X, W, plan, rows=rows)
+        ctx.plan, ctx.rows, ctx.out_dtype = plan, rows, out_dtype
+        return ops.expert_matmul(X, W, plan, rows=rows, out_dtype=out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dY):
         X, W = ctx.saved_tensors
+        dY = dY.to(X.dtype)
         dX = dW = None
         if ctx.needs_input_grad[0]:
-            dX = ops.expert_matmul(dY, W, ctx.plan, rows="sorted", w_layout="nc")
-            if ctx.rows == "tokens":
-                dX = ops.combine(dX, None, ctx.plan)       # a token's row went to each of its experts
+            if ctx.rows == "tokens":                       # a token's row went to each of its experts
+                dX = ops.combine(ops.expert_matmul(dY, W, ctx.plan, rows="sorted", w_layout="nc", out_dtype=ctx.out_dtype), None, ctx.plan, out_dtype=X.dtype)
+            else:
+                dX = ops.expert_matmul(dY, W, ctx.plan, rows="sorted", w_layout="nc")
             dX = dX.view(X.shape)
         if ctx.needs_input_grad[1]:
             dW = ops.expert_dweight(X, dY, ctx.plan, rows=ctx.rows)
-        return dX, dW, None, None
+        return dX, dW, None, None, None
 
 
 class CombineFunction(torch.autograd.Function):
-    """``apply(Y, weights, plan) -> out`` (``ops.combine``)."""
+    """``apply(Y, weights, plan, out_dtype=None) -> out`` (``ops.combine``)."""
 
     @staticmethod
-    def forward(ctx, Y, weights, plan):
+    def forward(ctx, Y, weights, plan, out_dtype=None):
         ctx.save_for_backward(Y, weights)
         ctx.plan = plan
-        return ops.combine(Y, weights, plan)
+        return ops.combine(Y, weights, plan, out_dtype=out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dOut):
         Y, weights = ctx.saved_tensors
-        return (*ops.combine_backward(dOut, Y, weights, ctx.plan), None)
+        if weights is None or weights.dtype in (torch.float32, Y.dtype):
+            return (*ops.combine_backward(dOut.to(Y.dtype), Y, weights, ctx.plan), None, None)
+        dY, dweights = ops.combine_backward(dOut.to(Y.dtype), Y, weights.to(Y.dtype), ctx.plan)
+        return dY, dweights.to(weights.dtype), None, None
 
 
 def route_tokens(logits, top_k, bias=None, **options):
@@ -87,14 +93,14 @@ def route_tokens(logits, top_k, bias=None, **options):
     return RouteTokensFunction.apply(logits, bias, top_k, options)
 
 
-def expert_matmul(X, W, plan, *, rows="tokens"):
+def expert_matmul(X, W, plan, *, rows="tokens", out_dtype=None):
     """``ops.expert_matmul`` (W [E, C, N]) with gradients for X and W."""
-    return ExpertMatmulFunction.apply(X, W, plan, rows)
+    return ExpertMatmulFunction.apply(X, W, plan, rows, out_dtype)
 
 
-def combine(Y, weights, plan):
+def combine(Y, weights, plan, *, out_dtype=None):
     """``ops.combine`` with gradients for Y and the weights."""
-    return CombineFunction.apply(Y, weights, plan)
+    return CombineFunction.apply(Y, weights, plan, out_dtype)
 
 
 class TokenRouter(nn.Module):
@@ -132,11 +138,13 @@ class RoutedExperts(nn.Module):
     """``out[t] = sum_j weights[t, j] * act(x[t] @ up[e]) @ down[e]`` over the experts ``e`` that the router chose for token t;
     x [..., I] -> [..., I], up [E, I, J], down [E, J, I], act = SiLU.  No token is dropped, whatever the load of an expert.  Options go to
     :class:`TokenRouter`.  In 16 bits the rows between the products are rounded to the tensors' type, each once, as the module's
-    activations are; sums over tokens, experts and features are float32."""
+    activations are; sums over tokens, experts and features are float32.  With ``float32_rows`` products leave float32 rows, so that only what
+    they are made into is rounded (``act(..)``, the output, gradients ahead of their products): about half of the rounding errors' variance,
+    for twice the bytes of those rows."""
 
-    def __init__(self, E: int, I: int, J: int, top_k: int, **options):
+    def __init__(self, E: int, I: int, J: int, top_k: int, *, float32_rows: bool = False, **options):
         super().__init__()
-        self.E, self.I, self.J = E, I, J
+        self.E, self.I, self.J, self.float32_rows = E, I, J, float32_rows
         self.router = TokenRouter(E, I, top_k, **options)
         self.up = nn.Parameter(torch.empty(E, I, J))
         self.down = nn.Parameter(torch.empty(E, J, I))
@@ -147,8 +155,9 @@ class RoutedExperts(nn.Module):
     def forward(self, x):
         weights, experts = self.router(x)
         self.plan = plan = ops.plan_experts(experts, self.E)
-        h = F.silu(expert_matmul(x, self.up, plan))
-        return combine(expert_matmul(h, self.down, plan, rows="sorted"), weights, plan).view(x.shape)
+        wide = torch.float32 if self.float32_rows else None
+        h = F.silu(expert_matmul(x, self.up, plan, out_dtype=wide)).to(x.dtype)
+        return combine(expert_matmul(h, self.down, plan, rows="sorted", out_dtype=wide), weights, plan, out_dtype=x.dtype).view(x.shape)
 
     @torch.no_grad()
     def quantized(self) -> "RoutedExpertsInt8":
@@ -171,7 +180,8 @@ class RoutedExpertsInt8(nn.Module):
 
     def __init__(self, layer: RoutedExperts):
         super().__init__()
-        self.E, self.router = layer.E, copy.deepcopy(layer.router).requires_grad_(False)
+        self.E, self.float32_rows = layer.E, layer.float32_rows
+        self.router = copy.deepcopy(layer.router).requires_grad_(False)
         for name in ("up", "down"):
             q, scale = ops.quantize_rows(getattr(layer, name).detach().transpose(1, 2))
             self.register_buffer(name, q)
@@ -190,6 +200,7 @@ class RoutedExpertsInt8(nn.Module):
     def forward(self, x):
         weights, experts = self.router(x)
         plan = ops.plan_experts(experts, self.E)
-        h = F.silu(ops.expert_matmul_int8(*ops.quantize_rows(x), self.up, self.up_scale, plan, out_dtype=x.dtype))
-        y = ops.expert_matmul_int8(*ops.quantize_rows(h), self.down, self.down_scale, plan, rows="sorted", out_dtype=x.dtype)
-        return ops.combine(y, weights, plan).view(x.shape)
+        rows = torch.float32 if self.float32_rows else x.dtype
+        h = F.silu(ops.expert_matmul_int8(*ops.quantize_rows(x), self.up, self.up_scale, plan, out_dtype=rows))
+        y = ops.expert_matmul_int8(*ops.quantize_rows(h), self.down, self.down_scale, plan, rows="sorted", out_dtype=rows)
+        return ops.combine(y, weights, plan, out_dtype=x.dtype).view(x.shape)

@@ -361,15 +361,22 @@ typedef struct egs_ragged {
 int egs_expert_matmul(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
                       int w_layout, int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
 size_t egs_expert_matmul_workspace_bytes(const egs_ragged* dims, int rows, int w_layout, int dtype);
+/* ... with float32 rows of 16-bit operands (out_dtype EGS_F32), whose rounding is then left to what is made of them; else out_dtype = dtype. */
+int egs_expert_matmul_out(const void* X, const void* W, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
+                          int w_layout, int dtype, int out_dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word,
+                          void* cuda_stream);
 /* dW[e] = sum over the rows r of e of X[row(r)]^T dY[r]: [E, C, N], zero for experts without rows.  dY: sorted rows [tokens * k, N]. */
 int egs_expert_dweight(const void* X, const void* dY, const int32_t* offsets, const int32_t* slots, void* dW, const egs_ragged* dims, int rows,
                        int dtype, int path, void* workspace, size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
 size_t egs_expert_dweight_workspace_bytes(const egs_ragged* dims, int rows, int dtype);
 
 /* out[t] = sum over j of weights[t, j] Y[position[t * k + j]]: token rows [tokens, N] from sorted rows.  weights NULL: ones.  Float32 in
- * the order of j, rounded once; zeros where k is 0.  weights_dtype: EGS_F32 or the rows' type. */
+ * the order of j, rounded once; zeros where k is 0.  weights_dtype: EGS_F32 or the output's type. */
 int egs_combine(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
                 int weights_dtype, void* cuda_stream);
+/* ... in 16 bits from float32 rows (dtype EGS_F32, out_dtype EGS_F16 or EGS_BF16); else out_dtype = dtype. */
+int egs_combine_out(const void* Y, const void* weights, const int32_t* position, void* out, int64_t tokens, int64_t k, int64_t N, int dtype,
+                    int weights_dtype, int out_dtype, void* cuda_stream);
 /* Its gradients: dY (sorted rows; zeros for slots that were not routed) and, where dweights is given, dweights[t, j] = <dOut[t], Y[..]>. */
 int egs_combine_backward(const void* dOut, const void* Y, const void* weights, const int32_t* position, void* dY, void* dweights,
                          int64_t tokens, int64_t k, int64_t N, int dtype, int weights_dtype, void* cuda_stream);

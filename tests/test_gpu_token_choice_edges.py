@@ -11,6 +11,7 @@ import torch
 
 from expertscattergather_b200 import RoutedExperts, _lib, ops, token_choice
 from oracle import choice_oracle as orc
+from test_gpu_token_choice import MATMUL_SHAPES, close, draw_experts
 
 pytestmark = pytest.mark.gpu
 
@@ -329,4 +330,131 @@ def test_a_refused_launch_is_reported_once(cuda_device):
     with pytest.raises(RuntimeError, match="invalid"):
         ops.gather_gemm(X, W, torch.zeros(1, 1, 1, device="cuda", dtype=torch.int32), path="generic")
     assert (X + 1).sum().item() == 8
+    ops.check_status()
+
+
+# ---- float32 rows of 16-bit tensors ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,k,E,C,N", MATMUL_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_float32_rows(cuda_device, tokens, k, E, C, N, dtype):
+    """Products without a rounding, and their weighted sums with one."""
+    g, k = gen(C + N), min(k, E)
+    for kind in ("even", "holes"):
+        ids = draw_experts(g, tokens, k, E, kind)
+        plan = ops.plan_experts(ids, E)
+        W = randn(g, E, C, N, dtype=dtype)
+        for rows, x in (("tokens", randn(g, tokens, C, dtype=dtype)), ("sorted", randn(g, tokens * k, C, dtype=dtype))):
+            ref, size = orc.matmul(x, W, ids, E, rows)
+            for path in ("auto", "generic"):
+                for layout, w in (("cn", W), ("nc", W.transpose(1, 2).contiguous())):
+                    Y = ops.expert_matmul(x, w, plan, rows=rows, w_layout=layout, path=path, out_dtype=torch.float32)
+                    assert Y.dtype == torch.float32
+                    close(Y, ref, size, C)
+            assert torch.equal(ops.expert_matmul(x, W, plan, rows=rows, out_dtype=dtype), ops.expert_matmul(x, W, plan, rows=rows))
+            for weights in (None, torch.rand(tokens, k, device="cuda", generator=g), torch.rand(tokens, k, device="cuda", generator=g).to(dtype)):
+                out = ops.combine(Y, weights, plan, out_dtype=dtype)
+                assert out.dtype == dtype
+                want, many = orc.combine(Y, weights, plan.position, tokens, k)
+                close(out, want, many, k)
+                # the chain: sums of k * C products, one rounding
+                many, _ = orc.combine(size, None if weights is None else weights.abs(), plan.position, tokens, k)
+                want, _ = orc.combine(ref, weights, plan.position, tokens, k)
+                close(out, want, many, C + k)
+    ops.check_status()
+
+
+# rows of 1 to 40 vectors, many of them and few
+@pytest.mark.parametrize("tokens,k,N", [(1, 1, 1), (1, 8, 512), (7, 3, 13), (300, 4, 200), (129, 32, 8), (1000, 2, 1032), (20000, 4, 8), (50001, 2, 3), (2000, 4, 2048)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_combine_of_float32_rows(cuda_device, tokens, k, N, dtype):
+    g = gen(N)
+    ids = draw_experts(g, tokens, k, max(40, k), "holes")
+    plan = ops.plan_experts(ids, max(40, k))
+    Y = randn(g, tokens * k, N)
+    Y[plan.offsets[-1].item():] = float("nan")
+    for weights in (None, torch.rand(tokens, k, device="cuda", generator=g), torch.rand(tokens, k, device="cuda", generator=g).to(dtype)):
+        ref, size = orc.combine(Y, weights, plan.position, tokens, k)
+        close(ops.combine(Y, weights, plan, out_dtype=dtype), ref, size, k)
+    none = ops.ExpertPlan(plan.offsets * 0, plan.slots[:0], plan.position[:0], tokens, 0, max(40, k))
+    out = ops.combine(Y[:0], None, none, out_dtype=dtype)
+    assert out.dtype == dtype and out.shape == (tokens, N) and not out.any()
+
+
+def test_float32_rows_are_refused_where_they_are_not_made(cuda_device):
+    ids = draw_experts(gen(1), 10, 2, 4)
+    plan = ops.plan_experts(ids, 4)
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, device="cuda", dtype=dtype)
+    for out in (torch.float16, torch.float64, torch.int8):
+        with pytest.raises(ValueError):
+            ops.expert_matmul(z(10, 8), z(4, 8, 8), plan, out_dtype=out)
+        with pytest.raises(ValueError):
+            ops.combine(z(20, 8), None, plan, out_dtype=out)
+    with pytest.raises(ValueError):
+        ops.expert_matmul(z(10, 8, dtype=torch.float32), z(4, 8, 8, dtype=torch.float32), plan, out_dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ops.combine(z(20, 8), None, plan, out_dtype=torch.float32)
+    with pytest.raises(ValueError):
+        ops.combine(z(20, 8, dtype=torch.float32), z(10, 2, dtype=torch.float16), plan, out_dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_through_float32_rows(cuda_device, dtype):
+    g = gen(5)
+    tokens, k, E, C, N = 300, 4, 8, 72, 136
+    ids = draw_experts(g, tokens, k, E)
+    plan = ops.plan_experts(ids, E)
+    X, W, w = (t.requires_grad_(True) for t in (randn(g, tokens, C, dtype=dtype), randn(g, E, C, N, dtype=dtype), torch.rand(tokens, k, device="cuda", generator=g).to(dtype)))
+    dOut = randn(g, tokens, N, dtype=dtype)
+    Y = token_choice.expert_matmul(X, W, plan, out_dtype=torch.float32)
+    out = token_choice.combine(Y, w, plan, out_dtype=dtype)
+    assert Y.dtype == torch.float32 and out.dtype == dtype
+    out.backward(dOut)
+    assert all(t.grad.dtype == dtype for t in (X, W, w))
+    # dY is rounded to the tensors' type, once (a product of two of them: exact in float64), and multiplied as it is
+    slots = plan.slots.long()
+    dY = (dOut.double()[slots // k] * w.detach().double().flatten()[slots].unsqueeze(-1)).to(dtype)
+    ref, size = orc.matmul(dY, W.detach().transpose(1, 2), ids, E, "sorted")
+    ref, _ = orc.combine(ref, None, plan.position, tokens, k)
+    size, _ = orc.combine(size, None, plan.position, tokens, k)
+    close(X.grad, ref, size, N + k)
+    ref, size = orc.dweight(X.detach(), dY, ids, E, "tokens")
+    close(W.grad, ref, size, int(plan.counts().max()))
+    rows = Y.detach().double()[plan.position.long()].view(tokens, k, N)
+    ref = (rows * dOut.double().unsqueeze(1)).sum(-1)
+    close(w.grad, ref, (rows * dOut.double().unsqueeze(1)).abs().sum(-1), N)
+    # without the rounding of dY: the gradient of the token rows, gathered, times the weights, summed in float32, rounded once
+    dX = ops.combine(ops.expert_matmul(dOut, W.detach(), plan, w_layout="nc", out_dtype=torch.float32), w.detach(), plan, out_dtype=dtype)
+    ref, size = orc.matmul(dOut, W.detach().transpose(1, 2), ids, E, "tokens")
+    ref, _ = orc.combine(ref, w.detach(), plan.position, tokens, k)
+    size, _ = orc.combine(size, w.detach(), plan.position, tokens, k)
+    close(dX, ref, size, N + k)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_layer_with_float32_rows(cuda_device, dtype):
+    g = gen(6)
+    errors = {}
+    for wide in (False, True):
+        torch.manual_seed(3)
+        layer = RoutedExperts(16, 128, 96, 4, float32_rows=wide).cuda().to(dtype)
+        x = randn(gen(7), 400, 128, dtype=dtype).requires_grad_(True)
+        weights, ids = layer.router(x)
+        out = layer(x)
+        dOut = randn(gen(8), 400, 128, dtype=dtype)
+        out.backward(dOut)
+        xs = x.detach().double().requires_grad_(True)
+        logits = xs @ layer.router.W.detach().double().t()
+        p = torch.softmax(logits, -1).gather(1, ids.long())
+        p = p / p.sum(-1, keepdim=True)
+        ref = 0
+        for j in range(4):
+            h = torch.nn.functional.silu(torch.einsum("tc,tcn->tn", xs, layer.up.detach().double()[ids[:, j].long()]))
+            ref = ref + p[:, j:j + 1] * torch.einsum("tc,tcn->tn", h, layer.down.detach().double()[ids[:, j].long()])
+        ref.backward(dOut.double())
+        errors[wide] = [((a.double() - b).norm() / b.norm()).item() for a, b in ((out, ref.detach()), (x.grad, xs.grad))]
+        served = layer.quantized()
+        assert served.float32_rows == wide and (served(x).double() - ref.detach()).norm() <= 0.05 * ref.norm()
+    assert all(a < b for a, b in zip(errors[True], errors[False])), errors
     ops.check_status()
