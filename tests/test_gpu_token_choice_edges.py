@@ -458,3 +458,85 @@ def test_layer_with_float32_rows(cuda_device, dtype):
         assert served.float32_rows == wide and (served(x).double() - ref.detach()).norm() <= 0.05 * ref.norm()
     assert all(a < b for a, b in zip(errors[True], errors[False])), errors
     ops.check_status()
+
+
+# ---- variants that sizes choose ----------------------------------------------------------------------------
+
+def experts_of(counts, k, g):
+    """Ids of sum(counts) slots in a random order, so many of each expert, -1 for the rest of the last token."""
+    ids = torch.arange(len(counts), device="cuda").repeat_interleave(torch.tensor(counts, device="cuda"))
+    ids = torch.cat([ids, ids.new_full((-len(ids) % k,), -1)])
+    return ids[torch.randperm(len(ids), device="cuda", generator=g)].view(-1, k).int()
+
+
+# rows of the experts; cut into ranges: those of more than 24 steps of 64 rows, on pairs where X has more than 128 features
+LONG = {"one": [5000], "three": [1700, 2000, 4100], "even": [1601] * 40, "skewed": [9000, 1, 0, 700, 2600, 64], "empty first": [0, 0, 6401, 1537]}
+
+
+@pytest.mark.parametrize("counts", LONG.values(), ids=LONG.keys())
+@pytest.mark.parametrize("C,N", [(64, 64), (64, 200), (256, 64), (256, 200), (131, 67), (35, 33), (300, 520)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradients_of_long_experts(cuda_device, counts, C, N, dtype):
+    g, k = gen(C + N), 2
+    ids = experts_of(counts, k, g)
+    E, tokens = len(counts), len(ids)
+    plan = ops.plan_experts(ids, E)
+    dY = randn(g, tokens * k, N, dtype=dtype)
+    for rows, n in (("tokens", tokens), ("sorted", tokens * k)):
+        X = randn(g, n, C, dtype=dtype)
+        ref, size = orc.dweight(X, dY, ids, E, rows)
+        for path in ("auto", "generic"):
+            dW = ops.expert_dweight(X, dY, plan, rows=rows, path=path)
+            close(dW, ref, size, max(counts))
+            assert not any(dW[e].any() for e, c in enumerate(counts) if c == 0)
+    ops.check_status()
+
+
+# more experts than a CTA has threads: the tables of blocks and of ranges take two turns
+@pytest.mark.parametrize("E", [513, 700, 1024])
+@pytest.mark.parametrize("C,N", [(64, 72), (200, 264)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_products_of_many_experts(cuda_device, E, C, N, dtype):
+    g, tokens, k = gen(E + C), 1500, 3
+    ids = draw_experts(g, tokens, k, E, "skewed")
+    ids[:, 2] = E - 1                                      # one of many rows, behind the first turn
+    ids[ids[:, 0] == E - 1, 0] = -1
+    ids[ids[:, 1] == E - 1, 1] = -1
+    plan = ops.plan_experts(ids, E)
+    X, W, dY = randn(g, tokens, C, dtype=dtype), randn(g, E, C, N, dtype=dtype), randn(g, tokens * k, N, dtype=dtype)
+    ref, size = orc.matmul(X, W, ids, E, "tokens")
+    for layout, w in (("cn", W), ("nc", W.transpose(1, 2).contiguous())):
+        close(ops.expert_matmul(X, w, plan, w_layout=layout), ref, size, C)
+    ref, size = orc.dweight(X, dY, ids, E, "tokens")
+    close(ops.expert_dweight(X, dY, plan), ref, size, tokens)
+    q = torch.randint(-127, 128, (tokens, C), device="cuda", generator=g).to(torch.int8)
+    Wq = torch.randint(-127, 128, (E, N, C), device="cuda", generator=g).to(torch.int8)
+    Y = ops.expert_matmul_int8(q, torch.ones(tokens, device="cuda"), Wq, torch.ones(E, N, device="cuda"), plan, out_dtype=torch.float32)
+    ref, _ = orc.matmul(q, Wq.transpose(1, 2), ids, E, "tokens")
+    assert torch.equal(Y.double(), ref)                    # sums below 2^24
+    ops.check_status()
+
+
+@pytest.mark.parametrize("tokens,k,E,C,N", [(300, 2, 6, 128, 192), (9, 2, 6, 128, 192), (301, 3, 5, 130, 67), (5000, 2, 3, 264, 136)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sorted_rows_of_an_expert_stay_with_it(cuda_device, tokens, k, E, C, N, dtype):
+    """Infinities in the sorted rows of one expert, NaN in rows that are not routed: products and gradients of the others are the same bits."""
+    g = gen(C)
+    ids = draw_experts(g, tokens, k, E, "even")
+    ids[::7, 0] = -1
+    plan = ops.plan_experts(ids, E)
+    X, W, dY = randn(g, tokens * k, C, dtype=dtype), randn(g, E, N, C, dtype=dtype), randn(g, tokens * k, N, dtype=dtype)
+    bad = 1
+    a, b, end = plan.offsets[bad].item(), plan.offsets[bad + 1].item(), plan.offsets[E].item()
+    Xn, Yn = X.clone(), dY.clone()
+    Xn[a:b], Xn[end:] = float("inf"), float("nan")
+    Yn[a:b], Yn[end:] = float("-inf"), float("nan")
+    rows = torch.ones(tokens * k, dtype=torch.bool, device="cuda")
+    rows[a:b] = False
+    others = torch.arange(E, device="cuda") != bad
+    for path in ("auto", "generic"):
+        ref, got = (ops.expert_matmul(x, W, plan, rows="sorted", w_layout="nc", path=path) for x in (X, Xn))
+        assert torch.equal(ref[rows], got[rows]) and not got[end:].any() and not torch.isfinite(got[a:b]).any()
+        ref, got = (ops.expert_dweight(x, y, plan, rows="sorted", path=path) for x, y in ((X, dY), (Xn, Yn)))
+        assert torch.equal(ref[others], got[others]) and (a == b or not torch.isfinite(got[bad]).any())
+    ops.check_status()
