@@ -20,6 +20,7 @@ I16, I32, I64 = 0, 1, 2
 PREC_STRICT, PREC_TF32 = 0, 1
 PATH_AUTO, PATH_GENERIC, PATH_TENSOR, PATH_PAIRED = 0, 1, 2, 3
 W_CN, W_NC = 0, 1
+ACT_NONE, ACT_SILU = 0, 1
 DW_GATHERED_ROWS, DW_DIRECT_ROWS = 0, 1
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_TOO_LARGE = range(6)
 STATUS_INDEX_OUT_OF_RANGE, STATUS_PIPELINE_TIMEOUT, STATUS_INTERNAL = 1, 2, 4
@@ -34,6 +35,8 @@ EXPORTS = (
     "egs_route_tokens", "egs_route_tokens_backward", "egs_plan_experts", "egs_plan_workspace_bytes", "egs_expert_matmul",
     "egs_expert_matmul_out", "egs_expert_matmul_workspace_bytes", "egs_expert_dweight", "egs_expert_dweight_workspace_bytes", "egs_combine",
     "egs_combine_out", "egs_combine_backward", "egs_quantize_rows", "egs_expert_matmul_int8",
+    "egs_quantize_rows_fp4", "egs_dequantize_rows_fp4", "egs_expert_matmul_fp4", "egs_expert_matmul_fp4_rows",
+    "egs_expert_matmul_fp4_rows_workspace_bytes",
 )
 
 
@@ -135,7 +138,12 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("egs_combine_out", i, [vp, vp, vp, vp, i64, i64, i64, i, i, i, vp]),
             ("egs_combine_backward", i, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i, i, vp]),
             ("egs_quantize_rows", i, [vp, vp, vp, i64, i64, i64, i64, i, vp]),
-            ("egs_expert_matmul_int8", i, [vp, vp, i64, vp, vp, i64, vp, vp, vp, ragged, i, i, i, vp, vp])):
+            ("egs_expert_matmul_int8", i, [vp, vp, i64, vp, vp, i64, vp, vp, vp, ragged, i, i, i, vp, vp]),
+            ("egs_quantize_rows_fp4", i, [vp, vp, vp, i64, i64, i64, i64, i64, i, i, vp]),
+            ("egs_dequantize_rows_fp4", i, [vp, vp, vp, i64, i64, i64, i64, i, vp]),
+            ("egs_expert_matmul_fp4", i, [vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, ragged, i, i, i, vp, vp]),
+            ("egs_expert_matmul_fp4_rows", i, [vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, i64, i64, ragged, i, i, i, vp, sz, vp, vp]),
+            ("egs_expert_matmul_fp4_rows_workspace_bytes", sz, [ragged, i])):
         getattr(lib, name).restype = result
         getattr(lib, name).argtypes = args
     lib.egs_fused_pair_eligible.restype = i

@@ -24,26 +24,6 @@ constexpr int kFewAhead = 8;           // ... vectors a thread asks for at a tim
 template <typename T> struct Sum { using type = float; };
 template <> struct Sum<int8_t> { using type = int; };
 
-// The `nth` expert with rows, -1 if there are fewer; by a whole warp.
-__device__ __forceinline__ int nth_expert(const int* offsets, int E, int nth, int* first, int* end) {
-  const int lane = threadIdx.x & 31;
-  for (int e0 = 0; e0 < E; e0 += 32) {
-    const int e = e0 + lane;
-    const int a = e < E ? offsets[e] : 0, b = e < E ? offsets[e + 1] : 0;
-    const unsigned has = __ballot_sync(kAll, b > a);
-    if (nth < __popc(has)) {
-      unsigned left = has;
-      while (nth--) left &= left - 1;
-      const int src = __ffs(left) - 1;
-      *first = __shfl_sync(kAll, a, src);
-      *end = __shfl_sync(kAll, b, src);
-      return e0 + src;
-    }
-    nth -= __popc(has);
-  }
-  return -1;
-}
-
 struct Segment {
   int expert, first, end;
 };

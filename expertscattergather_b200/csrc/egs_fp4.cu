@@ -1,0 +1,303 @@
+// Rows in 4 bits and back, and products of few such rows on the CUDA cores.
+#include "egs_fp4.cuh"
+
+namespace egs {
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+
+// ------------------------------------------------------------------------------------------------
+// Rows into 4 bits.  A lane has eight neighbours, four lanes a block, 2^lanes_log2 lanes a row's stretch (short rows share a warp), four such
+// stretches at a time, whose loads go out together.
+// ------------------------------------------------------------------------------------------------
+constexpr int kToWarps = 8, kToAhead = 4;
+
+struct ToFp4 {
+  const void* X;
+  uint8_t* q;
+  uint8_t* scale;
+  long long x_stride, q_stride, s_stride, rows;
+  int C, chunks, lanes_log2;      // chunks: of eight elements, whole blocks
+};
+
+// V: elements that are loaded together
+template <typename T, int V, bool SILU>
+__global__ void __launch_bounds__(kToWarps * 32) to_fp4_kernel(const __grid_constant__ ToFp4 p) {
+  using P = Packed<T, V>;
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = 1 << p.lanes_log2;
+  const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> p.lanes_log2) + (lane >> p.lanes_log2);
+  const int first = blockIdx.y * lanes * kToAhead + (lane & (lanes - 1));
+  const bool on = row < p.rows;
+  const T* x = static_cast<const T*>(p.X) + row * p.x_stride;
+  P y[kToAhead][8 / V];
+  float v[kToAhead][8];
+#pragma unroll
+  for (int u = 0; u < kToAhead; ++u) {
+    const int c = (first + u * lanes) * 8;
+    if (on && c + 8 <= p.C) {
+#pragma unroll
+      for (int i = 0; i < 8 / V; ++i) y[u][i] = reinterpret_cast<const P*>(x + c)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = on && c + i < p.C ? to_f32<T>(x[c + i]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kToAhead; ++u) {
+    const int chunk = first + u * lanes;
+    if (on && chunk * 8 + 8 <= p.C) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = y[u][i / V].get(i % V);
+    }
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (SILU) v[u][i] = silu_exact(v[u][i]);
+      top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
+    }
+    top = max(top, __shfl_xor_sync(kAll, top, 1));
+    top = max(top, __shfl_xor_sync(kAll, top, 2));
+    if (!on || chunk >= p.chunks) continue;
+    const uint32_t byte = fp4_scale(top);
+    const float inverse = fp4_inverse(byte);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[u][i] = fp4_scaled(v[u][i], inverse);
+    *reinterpret_cast<uint32_t*>(p.q + row * p.q_stride + chunk * 4ll) = fp4_pack8(v[u]);
+    if (!(chunk & 3)) p.scale[row * p.s_stride + (chunk >> 2)] = static_cast<uint8_t>(byte);
+  }
+}
+
+template <typename T, int V>
+cudaError_t to_fp4_v(const ToFp4& p, int act, cudaStream_t st) {
+  const long long per_cta = kToWarps * (32 >> p.lanes_log2);
+  const int stretch = kToAhead << p.lanes_log2;
+  const dim3 grid(static_cast<unsigned>((p.rows + per_cta - 1) / per_cta), (p.chunks + stretch - 1) / stretch);
+  return act == EGS_ACT_SILU ? launch_kernel(to_fp4_kernel<T, V, true>, grid, kToWarps * 32, 0, st, true, p)
+                             : launch_kernel(to_fp4_kernel<T, V, false>, grid, kToWarps * 32, 0, st, true, p);
+}
+template <typename T>
+cudaError_t to_fp4_t(const ToFp4& p, int act, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  auto fits = [&](int v) { return p.x_stride % v == 0 && reinterpret_cast<uintptr_t>(p.X) % (v * sizeof(T)) == 0; };
+  if (fits(V)) return to_fp4_v<T, V>(p, act, st);
+  if (fits(2)) return to_fp4_v<T, 2>(p, act, st);
+  return to_fp4_v<T, 1>(p, act, st);
+}
+
+// ------------------------------------------------------------------------------------------------
+// What 4 bits stand for.  A thread has V neighbours, as many as rows of the output begin on.
+// ------------------------------------------------------------------------------------------------
+struct FromFp4 {
+  const uint8_t* q;
+  const uint8_t* scale;
+  void* X;
+  long long q_stride, s_stride, rows;
+  int C;
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256) from_fp4_kernel(const __grid_constant__ FromFp4 p) {
+  pdl_wait();
+  pdl_trigger();
+  const int per_row = p.C / V;
+  const long long all = p.rows * per_row;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * 256) {
+    const long long row = i / per_row;
+    const int c = static_cast<int>(i - row * per_row) * V;
+    const float power = fp4_power(p.scale[row * p.s_stride + c / kFp4Block]) * 0.5f;
+    const uint8_t* q = p.q + row * p.q_stride + c / 2;
+    uint32_t w = 0u;
+#pragma unroll
+    for (int b = 0; b < (V + 1) / 2; ++b) w |= static_cast<uint32_t>(q[b]) << (8 * b);
+    if (V == 1 && (c & 1)) w >>= 4;
+    uint32_t n[2];
+    fp4_integers(w, n[0], n[1]);
+    T out[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = from_f32<T>(static_cast<float>(static_cast<int8_t>(n[v / 4] >> (8 * (v % 4)))) * power);
+    T* x = static_cast<T*>(p.X) + row * p.C + c;
+    if constexpr (V == 8 && sizeof(T) == 2) {
+      uint32_t o[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) o[v] = static_cast<uint32_t>(*reinterpret_cast<unsigned short*>(&out[2 * v])) | static_cast<uint32_t>(*reinterpret_cast<unsigned short*>(&out[2 * v + 1])) << 16;
+      *reinterpret_cast<uint4*>(x) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = out[v];
+    }
+  }
+}
+template <typename T>
+cudaError_t from_fp4_t(const FromFp4& p, cudaStream_t st) {
+  auto go = [&](auto kernel, int v) {
+    const long long ctas = (p.rows * (p.C / v) + 255) / 256;
+    return launch_kernel(kernel, static_cast<unsigned>(ctas < 148 * 64 ? ctas : 148 * 64), 256, 0, st, true, p);
+  };
+  if (p.C % 8 == 0 && (reinterpret_cast<uintptr_t>(p.X) & 15u) == 0) return go(from_fp4_kernel<T, 8>, 8);
+  if (p.C % 2 == 0) return go(from_fp4_kernel<T, 2>, 2);
+  return go(from_fp4_kernel<T, 1>, 1);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Products of few rows: a warp has four channels, its lanes have the blocks of the contraction in turn, up to four rows share a read of the weights.
+// Twice the values are integers, so a block's 32 products are eight dp4a and their sum is exact; it is scaled and added in float32.
+// ------------------------------------------------------------------------------------------------
+constexpr int kFewWarps = 8, kFewRows = 4, kFewChannels = 4;
+
+struct Block4 {
+  uint32_t w[4];
+};
+// Block c of a row of `C` elements (an even number), zeros behind the row's end.
+__device__ __forceinline__ Block4 load_block(const uint8_t* row, int c, int C) {
+  Block4 b;
+  if ((c + 1) * kFp4Block <= C) {
+    const uint4 x = reinterpret_cast<const uint4*>(row)[c];
+    b.w[0] = x.x; b.w[1] = x.y; b.w[2] = x.z; b.w[3] = x.w;
+  } else {
+    const int left = C - c * kFp4Block;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b.w[i] = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (8 * i + 2 * j < left) b.w[i] |= static_cast<uint32_t>(row[c * 16ll + 4 * i + j]) << (8 * j);
+    }
+  }
+  return b;
+}
+
+template <typename OutT, int M>
+__device__ __forceinline__ void few_fp4(const Fp4Params& p, int expert, int first, int end, int n0) {
+  const int lane = threadIdx.x & 31;
+  const uint8_t *w[kFewChannels], *ws[kFewChannels], *x[M], *xs[M];
+#pragma unroll
+  for (int j = 0; j < kFewChannels; ++j) {
+    const int n = min(n0 + j, p.N - 1);
+    w[j] = p.W + expert * p.w_expert + n * p.w_row;
+    ws[j] = p.Ws + expert * p.ws_expert + n * p.ws_row;
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const int r = first + m < end ? first + m : first, src = p.slots ? p.by_k.quotient(p.slots[r]) : r;
+    x[m] = p.A + src * p.a_row;
+    xs[m] = p.As + src * p.as_row;
+  }
+  float acc[M][kFewChannels];
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int j = 0; j < kFewChannels; ++j) acc[m][j] = 0.f;
+  const int blocks = fp4_blocks(p.C);
+#pragma unroll 2
+  for (int c = lane; c < blocks; c += 32) {
+    Block4 wv[kFewChannels], xv[M];
+    uint32_t sw[kFewChannels], sx[M];
+#pragma unroll
+    for (int j = 0; j < kFewChannels; ++j) {
+      wv[j] = load_block(w[j], c, p.C);
+      sw[j] = ws[j][c];
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      xv[m] = load_block(x[m], c, p.C);
+      sx[m] = xs[m][c];
+    }
+    int sum[M][kFewChannels];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < kFewChannels; ++j) sum[m][j] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t xl[M], xh[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) fp4_integers(xv[m].w[i], xl[m], xh[m]);
+#pragma unroll
+      for (int j = 0; j < kFewChannels; ++j) {
+        uint32_t wl, wh;
+        fp4_integers(wv[j].w[i], wl, wh);
+#pragma unroll
+        for (int m = 0; m < M; ++m) sum[m][j] = __dp4a(static_cast<int>(xh[m]), static_cast<int>(wh), __dp4a(static_cast<int>(xl[m]), static_cast<int>(wl), sum[m][j]));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kFewChannels; ++j) {
+      const float f = fp4_power(sw[j]);
+#pragma unroll
+      for (int m = 0; m < M; ++m) acc[m][j] = fmaf(static_cast<float>(sum[m][j]) * (0.25f * fp4_power(sx[m])), f, acc[m][j]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < kFewChannels; ++j) acc[m][j] += __shfl_xor_sync(kAll, acc[m][j], o);
+  OutT* out = static_cast<OutT*>(p.Out);
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int j = 0; j < kFewChannels; ++j)
+      if (lane == m * kFewChannels + j && first + m < end && n0 + j < p.N) out[(first + m) * p.y_row + n0 + j] = from_f32<OutT>(acc[m][j]);
+}
+
+template <typename OutT>
+__global__ void __launch_bounds__(kFewWarps * 32) few_fp4_kernel(const __grid_constant__ Fp4Params p) {
+  __shared__ int segment[3];
+  pdl_wait();
+  pdl_trigger();
+  if (p.offsets) {
+    if (const int routed = p.offsets[p.E]; routed < p.rows) {
+      OutT* out = static_cast<OutT*>(p.Out);
+      zero_by_grid(out + routed * p.y_row, out + p.rows * p.y_row);
+    }
+  }
+  if (threadIdx.x < 32) {                            // the expert with rows that is this CTA's
+    int e = 0, first = 0, end = p.rows;
+    if (p.offsets) e = nth_expert(p.offsets, p.E, blockIdx.z, &first, &end);
+    if (threadIdx.x == 0) segment[0] = e, segment[1] = first, segment[2] = end;
+  }
+  __syncthreads();
+  const int e = segment[0], end = segment[2];
+  const long long tile = static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x;
+  const long long n0 = (tile * kFewWarps + (threadIdx.x >> 5)) * kFewChannels;
+  if (e < 0 || n0 >= p.N) return;
+  int r = segment[1];
+  for (; end - r > 1; r += kFewRows) {
+    few_fp4<OutT, kFewRows>(p, e, r, end, static_cast<int>(n0));
+    if (end - r <= kFewRows) return;
+  }
+  if (r < end) few_fp4<OutT, 1>(p, e, r, end, static_cast<int>(n0));
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_fp4(const void* X, uint8_t* q, uint8_t* scale, long long rows, int C, long long x_stride, long long q_stride,
+                                long long s_stride, int act, int dtype, cudaStream_t st) {
+  ToFp4 p{X, q, scale, x_stride, q_stride, s_stride, rows, C, fp4_blocks(C) * 4, 2};
+  while (p.lanes_log2 < 5 && (1 << p.lanes_log2) < p.chunks) ++p.lanes_log2;
+  count_launch();
+  return dtype == EGS_F16 ? to_fp4_t<__half>(p, act, st) : dtype == EGS_BF16 ? to_fp4_t<__nv_bfloat16>(p, act, st) : to_fp4_t<float>(p, act, st);
+}
+
+cudaError_t launch_dequantize_fp4(const uint8_t* q, const uint8_t* scale, void* X, long long rows, int C, long long q_stride, long long s_stride,
+                                  int dtype, cudaStream_t st) {
+  const FromFp4 p{q, scale, X, q_stride, s_stride, rows, C};
+  count_launch();
+  return dtype == EGS_F16 ? from_fp4_t<__half>(p, st) : dtype == EGS_BF16 ? from_fp4_t<__nv_bfloat16>(p, st) : from_fp4_t<float>(p, st);
+}
+
+bool few_fp4_fit(const Fp4Params& p) { return 4ll * p.rows <= 3 * p.E || p.rows <= 8; }
+
+cudaError_t launch_few_fp4(const Fp4Params& p, int out_dtype, cudaStream_t st) {
+  const int segments = p.offsets ? (p.rows < p.E ? p.rows : p.E) : 1, per_cta = kFewWarps * kFewChannels, tiles = (p.N + per_cta - 1) / per_cta;
+  const dim3 grid(tiles, 1, segments);
+  count_launch();
+  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, kFewWarps * 32, 0, st, true, p); };
+  return out_dtype == EGS_F16 ? go(few_fp4_kernel<__half>) : out_dtype == EGS_BF16 ? go(few_fp4_kernel<__nv_bfloat16>) : go(few_fp4_kernel<float>);
+}
+
+}  // namespace egs

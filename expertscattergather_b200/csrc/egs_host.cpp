@@ -47,7 +47,9 @@ struct Api {
   X(egs_fill_zero) X(egs_set_status_mirror) X(egs_expert_row_sum)                                                          \
   X(egs_route_tokens) X(egs_route_tokens_backward) X(egs_plan_experts) X(egs_plan_workspace_bytes) X(egs_expert_matmul_out) \
   X(egs_expert_matmul_workspace_bytes) X(egs_expert_dweight) X(egs_expert_dweight_workspace_bytes) X(egs_combine_out)       \
-  X(egs_combine_backward) X(egs_quantize_rows) X(egs_expert_matmul_int8)
+  X(egs_combine_backward) X(egs_quantize_rows) X(egs_expert_matmul_int8)                                                   \
+  X(egs_quantize_rows_fp4) X(egs_dequantize_rows_fp4) X(egs_expert_matmul_fp4) X(egs_expert_matmul_fp4_rows)                \
+  X(egs_expert_matmul_fp4_rows_workspace_bytes)
 #define EGS_FIELD(name) decltype(&::name) name = nullptr;
   EGS_API(EGS_FIELD)
 #undef EGS_FIELD
@@ -706,6 +708,7 @@ struct GatherScatterFunction : torch::autograd::Function<GatherScatterFunction> 
 };
 
 #include "egs_host_choice.h"
+#include "egs_host_fp4.h"
 
 // Tensors this path takes as they are: plain tensors outside any tracing, transform or dispatch mode.  (Fake tensors, tensor
 // subclasses and functorch wrappers go through the Python functions and their dispatcher ops.)
@@ -822,4 +825,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("combine_backward", &combine_backward, nogil());
   m.def("quantize_rows", &quantize_rows, nogil());
   m.def("matmul_int8", &matmul_int8, nogil());
+  m.def("quantize_rows_fp4", &quantize_rows_fp4, nogil());
+  m.def("dequantize_rows_fp4", &dequantize_rows_fp4, nogil());
+  m.def("matmul_fp4", &matmul_fp4, nogil());
+  m.def("matmul_fp4_rows", &matmul_fp4_rows, nogil());
 }

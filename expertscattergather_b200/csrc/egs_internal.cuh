@@ -65,6 +65,26 @@ inline dim3 rows_by_columns(long long blocks, int tiles) {
 }
 __device__ __forceinline__ int column_tile() { return static_cast<int>(blockIdx.z * gridDim.y + blockIdx.y); }
 
+// The `nth` expert with rows, -1 if there are fewer; by a whole warp.
+__device__ __forceinline__ int nth_expert(const int* offsets, int E, int nth, int* first, int* end) {
+  const int lane = threadIdx.x & 31;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int e = e0 + lane;
+    const int a = e < E ? offsets[e] : 0, b = e < E ? offsets[e + 1] : 0;
+    const unsigned has = __ballot_sync(0xffffffffu, b > a);
+    if (nth < __popc(has)) {
+      unsigned left = has;
+      while (nth--) left &= left - 1;
+      const int src = __ffs(left) - 1;
+      *first = __shfl_sync(0xffffffffu, a, src);
+      *end = __shfl_sync(0xffffffffu, b, src);
+      return e0 + src;
+    }
+    nth -= __popc(has);
+  }
+  return -1;
+}
+
 // Reads Ind[pos] for any of the three index widths.
 __device__ __forceinline__ long long load_index(const void* ind, int index_dtype, long long pos) {
   if (index_dtype == EGS_I64) return static_cast<const long long*>(ind)[pos];
@@ -209,6 +229,23 @@ struct RaggedParams {
   Div by_k;            // slot -> token row
 };
 
+// Products of rows in 4 bits (egs_fp4.cuh); pitches in bytes, of the output's plain rows in elements.
+struct Fp4Params {
+  const uint8_t* A;          // rows: token rows through `slots`, or sorted rows
+  const uint8_t* As;         // ... their scales
+  const uint8_t* W;          // [E, N, C / 2]
+  const uint8_t* Ws;
+  void* Out;                 // sorted rows
+  uint8_t* OutScale;         // rows of the output in 4 bits: their scales; else NULL
+  const int* offsets;        // [E + 1]; NULL: one expert that has all rows
+  const int* slots;          // slot of a sorted row; NULL: A's rows are the sorted rows
+  StatusRef status;
+  long long a_row, as_row, w_row, ws_row, w_expert, ws_expert, y_row, ys_row;
+  int rows, a_rows, E, C, N; // C is even
+  int act;                   // EGS_ACT_* ahead of 4 bits
+  Div by_k;
+};
+
 // ------------------------------------------------------------------------------------------------
 // launchers implemented in the kernel files; each returns a cudaError_t from the launch
 // ------------------------------------------------------------------------------------------------
@@ -313,6 +350,15 @@ size_t ragged_dweight_workspace(const RaggedParams& p);
 // ... where experts have few rows (egs_few.cu): any type, width and alignment, C at least 1
 bool few_rows_fit(const RaggedParams& p, int dtype);
 cudaError_t launch_few_rows(const RaggedParams& p, int dtype, int out_dtype, cudaStream_t st);
+// Rows in 4 bits (egs_fp4.cu) and products of them: few rows, of any number and alignment; on the tensor cores (egs_fp4_tensor.cu), rows and scales
+// 16 bytes apart
+cudaError_t launch_quantize_fp4(const void* X, uint8_t* q, uint8_t* scale, long long rows, int C, long long x_stride, long long q_stride,
+                                long long s_stride, int act, int dtype, cudaStream_t st);
+cudaError_t launch_dequantize_fp4(const uint8_t* q, const uint8_t* scale, void* X, long long rows, int C, long long q_stride, long long s_stride,
+                                  int dtype, cudaStream_t st);
+bool few_fp4_fit(const Fp4Params& p);
+cudaError_t launch_few_fp4(const Fp4Params& p, int out_dtype, cudaStream_t st);
+cudaError_t launch_fp4_rows_tensor(const Fp4Params& p, int out_dtype, cudaStream_t st);
 // Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; zeros behind a row's end); dst NULL: nothing.
 struct PadRows {
   const void* src;

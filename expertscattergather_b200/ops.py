@@ -17,7 +17,8 @@ from . import _lib
 __all__ = ["gather_gemm", "gemm_scatter", "gather_scatter_pair", "fused_pair_eligible", "fused_pair_preferred", "dweight", "fill_zero", "side_stream", "fill_stream", "set_precision", "get_precision", "set_path", "get_path",
            "check_status", "reset_status", "publish_status", "launch_count", "dtype_to_type_id", "tensor_path_eligible", "describe_plan", "describe_kept_rows", "describe_half_tiles", "route_topk", "build_index_csr", "compact_index", "gemm_scatter_csr", "IndexCSR",
            "route_tokens", "route_tokens_backward", "plan_experts", "ExpertPlan", "expert_matmul", "expert_dweight", "combine", "combine_backward",
-           "quantize_rows", "matmul_int8", "expert_matmul_int8"]
+           "quantize_rows", "matmul_int8", "expert_matmul_int8",
+           "quantize_rows_fp4", "dequantize_rows_fp4", "matmul_fp4", "expert_matmul_fp4", "expert_matmul_fp4_rows"]
 
 _PRECISIONS = {"strict": _lib.PREC_STRICT, "fp32": _lib.PREC_STRICT, "tf32": _lib.PREC_TF32}
 _PATHS = {"auto": _lib.PATH_AUTO, "generic": _lib.PATH_GENERIC, "tensor": _lib.PATH_TENSOR,
@@ -506,3 +507,38 @@ def matmul_int8(q, q_scale, Wq, w_scale, *, out_dtype=torch.bfloat16, path=None)
 def expert_matmul_int8(q, q_scale, Wq, w_scale, plan: ExpertPlan, *, rows="tokens", out_dtype=torch.bfloat16, path=None):
     """:func:`expert_matmul` in 8-bit integers: q [rows, C] with a scale for each row, Wq [E, N, C] with one for each channel [E, N]."""
     return _host().matmul_int8(q, q_scale, Wq, w_scale, plan.offsets, plan.slots, plan.tokens, plan.k, rows, out_dtype, _path(path))
+
+
+# ---- rows in 4 bits ------------------------------------------------------------------------------------
+
+def quantize_rows_fp4(X, *, activation=None):
+    """Rows in 4 bits: blocks of 32 values of sign, two exponent bits and one mantissa bit (magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6) with a power of
+    two for each block.  ``q`` [..., ceil(C / 2)] (uint8: two values a byte, the first in the lower half) and ``scale`` [..., ceil(C / 32)]
+    (uint8: the power's exponent + 127), rows of both a multiple of 16 bytes apart.
+
+    A block's scale is the smallest power of two (from 2^-127 on) whose seven-fold its largest magnitude does not pass; values go to the nearest,
+    ties to an even mantissa, magnitudes beyond 6 to 6.  A block with an infinity or a NaN has the scale 255, which stands for NaN.
+    ``activation='silu'``: of ``x / (1 + exp(-x))``, formed in float32.  Weights [E, N, C] quantised this way are what the products take."""
+    return _host().quantize_rows_fp4(X, activation)
+
+
+def dequantize_rows_fp4(q, scale, C=None, *, dtype=torch.float32):
+    """What the rows of :func:`quantize_rows_fp4` stand for: [..., C] (an even C may be left out), rounded once to ``dtype``."""
+    return _host().dequantize_rows_fp4(q, scale, C, dtype)
+
+
+def matmul_fp4(q, scale, Wq, w_scale, *, out_dtype=torch.bfloat16, path=None):
+    """``Y[r, n] = sum_c x[r, c] w[n, c]`` of rows and weights in 4 bits (see :func:`quantize_rows_fp4`): q [..., C / 2], Wq [N, C / 2] ->
+    [..., N].  float32 sums, rounded once.  Operands whose rows do not lie a multiple of 16 bytes apart are copied first."""
+    return _host().matmul_fp4(q, scale, Wq, w_scale, None, None, 0, 1, "tokens", out_dtype, _path(path))
+
+
+def expert_matmul_fp4(q, scale, Wq, w_scale, plan: ExpertPlan, *, rows="tokens", out_dtype=torch.bfloat16, path=None):
+    """:func:`expert_matmul` of rows and weights in 4 bits: q [rows, C / 2], Wq [E, N, C / 2], scales [rows, C / 32] and [E, N, C / 32]."""
+    return _host().matmul_fp4(q, scale, Wq, w_scale, plan.offsets, plan.slots, plan.tokens, plan.k, rows, out_dtype, _path(path))
+
+
+def expert_matmul_fp4_rows(q, scale, Wq, w_scale, plan: ExpertPlan, *, rows="tokens", activation=None, path=None):
+    """:func:`expert_matmul_fp4` whose sorted rows (with ``activation='silu'`` their activations, formed in float32) leave in 4 bits again, as
+    ``(q, scale)`` for the next product: what lies between two products of a layer is neither stored in full nor read again."""
+    return _host().matmul_fp4_rows(q, scale, Wq, w_scale, plan.offsets, plan.slots, plan.tokens, plan.k, rows, activation, _path(path))

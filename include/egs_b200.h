@@ -392,6 +392,38 @@ int egs_expert_matmul_int8(const int8_t* q, const float* q_scale, int64_t q_stri
                            const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows, int out_dtype, int path,
                            int32_t* status_word, void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Rows in 4 bits.  (No counterpart in the reference.)
+ *
+ * A row is blocks of 32 values of one sign, two exponent and one mantissa bit (magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the first in the
+ * lower half, and a byte s for each block: its values count times 2^(s - 127), and 255 means that they are no numbers.
+ * Rows begin on 16 bytes and so do their scales: bases and strides (in bytes) are multiples of 16.
+ * ------------------------------------------------------------------------------------------------ */
+enum { EGS_ACT_NONE = 0, EGS_ACT_SILU = 1 /* x / (1 + exp(-x)) */ };
+
+/* Rows of X, or of their activations in float32, in 4 bits: a block's scale is the smallest power of two (from 2^-127 on) whose seven-fold its largest
+ * magnitude does not pass, values go to the nearest of 4 bits (ties to an even mantissa), magnitudes beyond 6 to 6.  A block with an infinity or a
+ * NaN has the scale 255 and zeros.  A row's last block is written whole, with zeros behind the row's end: q_stride >= 16 * ceil(C / 32). */
+int egs_quantize_rows_fp4(const void* X, uint8_t* q, uint8_t* scale, int64_t rows, int64_t C, int64_t x_stride, int64_t q_stride, int64_t s_stride,
+                          int activation, int dtype, void* cuda_stream);
+/* What they stand for, X [rows, C], rounded once to its type. */
+int egs_dequantize_rows_fp4(const uint8_t* q, const uint8_t* scale, void* X, int64_t rows, int64_t C, int64_t q_stride, int64_t s_stride, int dtype,
+                            void* cuda_stream);
+/* Y[r, n] = sum over c of row(r)[c] W[e][n][c], float32 sums, in out_dtype: [tokens * k, N], rows behind offsets[E] zero.  q: token rows or sorted
+ * rows (rows: EGS_ROWS_*), Wq [E, N, C / 2] with w_stride bytes from one channel to the next, their scales [E, N, ceil(C / 32)] with ws_stride;
+ * dims->C is even; offsets NULL: one expert that has all tokens (k = 1). */
+int egs_expert_matmul_fp4(const uint8_t* q, const uint8_t* q_scale, int64_t q_stride, int64_t qs_stride, const uint8_t* Wq, const uint8_t* w_scale,
+                          int64_t w_stride, int64_t ws_stride, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
+                          int out_dtype, int path, int32_t* status_word, void* cuda_stream);
+/* ... whose rows, or their activations, leave in 4 bits: y [tokens * k, ceil(N / 2)] and y_scale [tokens * k, ceil(N / 32)], as egs_quantize_rows_fp4
+ * writes them; rows behind offsets[E] are zeros with the scale 0.  workspace (16-byte aligned):
+ * egs_expert_matmul_fp4_rows_workspace_bytes() bytes (float32 rows, where few of them are not for the tensor cores). */
+int egs_expert_matmul_fp4_rows(const uint8_t* q, const uint8_t* q_scale, int64_t q_stride, int64_t qs_stride, const uint8_t* Wq, const uint8_t* w_scale,
+                               int64_t w_stride, int64_t ws_stride, const int32_t* offsets, const int32_t* slots, uint8_t* y, uint8_t* y_scale,
+                               int64_t y_stride, int64_t ys_stride, const egs_ragged* dims, int rows, int activation, int path, void* workspace,
+                               size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
+size_t egs_expert_matmul_fp4_rows_workspace_bytes(const egs_ragged* dims, int path);
+
 /* Number of kernels the library has launched in this process since load (for launch accounting). */
 int64_t egs_launch_count(void);
 

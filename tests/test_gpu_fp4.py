@@ -1,0 +1,194 @@
+"""Rows in 4 bits and their products on the GPU, against the definitions in float64."""
+import pytest
+import torch
+
+from expertscattergather_b200 import ops
+from oracle import choice_oracle as orc
+from oracle import fp4_oracle as fp4
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def randn(*shape, seed=0, dtype=torch.float32):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=gen).to(dtype)
+
+
+def same(a, b):
+    """Equal values, NaN where the other is NaN."""
+    return a.shape == b.shape and bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def check_rows(X, q, scale):
+    C = X.shape[-1]
+    codes, byte = fp4.quantize(X)
+    assert q.dtype == scale.dtype == torch.uint8
+    assert q.shape == (*X.shape[:-1], (C + 1) // 2) and scale.shape == (*X.shape[:-1], (C + 31) // 32)
+    assert torch.equal(scale.int(), byte.int())
+    assert torch.equal(q, fp4.pack(codes)[..., :q.shape[-1]])
+
+
+# ---- rows ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,C", [(1, 1), (3, 2), (5, 31), (1, 32), (7, 33), (130, 64), (33, 330), (9, 1030), (600, 2048), (2, 8200), (4097, 40)])
+def test_quantize(dtype, rows, C):
+    X = (randn(rows, C, seed=C) * torch.exp(3 * randn(rows, 1, seed=1))).to(TYPES[dtype])
+    q, scale = ops.quantize_rows_fp4(X)
+    check_rows(X, q, scale)
+    assert (rows == 1 or q.stride(0) % 16 == 0) and (rows == 1 or scale.stride(0) % 16 == 0)
+    for out in TYPES.values():
+        back = ops.dequantize_rows_fp4(q, scale, C, dtype=out)
+        assert back.dtype == out and same(back.double(), fp4.values(*fp4.quantize(X), C).to(out).double())     # (rows beyond f16 have infinities)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_borders(dtype):
+    """Every border between two values, its neighbours on both sides, at many scales, both signs."""
+    t = TYPES[dtype]
+    base = torch.tensor([0, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, 6, 7, .5, 1, 1.5, 2, 3, 4], device="cuda")
+    e = torch.arange(-12 if dtype == "f16" else -120, 12 if dtype == "f16" else 120, device="cuda").float()
+    at = (base * torch.exp2(e).unsqueeze(-1)).to(t)
+    up, down = (torch.nextafter(at, torch.full_like(at, s)) for s in (float("inf"), 0.0))
+    X = torch.stack([torch.cat((v, -v), -1) for v in (at, up, down)], 1)          # [e, 3, 32]: a border is the block's largest, or not
+    small = X.clone()
+    small[..., 8:10] = 0
+    small[..., 24:26] = 0
+    for x in (X, small, X.flatten(1)):
+        check_rows(x, *ops.quantize_rows_fp4(x))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_specials(dtype):
+    t = TYPES[dtype]
+    inf, nan, top, tiny = float("inf"), float("nan"), torch.finfo(t).max, torch.finfo(t).smallest_normal
+    X = randn(9, 96, seed=3).to(t)
+    X[0] = 0
+    X[1] = -0.0
+    X[2, 40] = inf
+    X[3, 95] = -inf
+    X[4, 0] = nan
+    X[5] = top
+    X[6] = torch.linspace(-1, 1, 96, device="cuda").to(t) * tiny
+    X[7, 5:] = 0
+    X[8] = torch.linspace(-1, 1, 96, device="cuda").to(t) * top
+    q, scale = ops.quantize_rows_fp4(X)
+    check_rows(X, q, scale)
+    back = ops.dequantize_rows_fp4(q, scale)
+    assert back[2, 32:64].isnan().all() and not back[2, :32].isnan().any() and back[4, :32].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_strides(dtype):
+    t = TYPES[dtype]
+    big = randn(40, 7, 200, seed=5).to(t)
+    for X in (big[:, 1], big[:, :, 3:99], big[::2, 2, 1:], big.transpose(0, 2), big[3, 4], big[:, 2, ::2], big[:0], big[:, :, :0], big[:1, :1, 5:38], big[0, 0, 7]):
+        if X.dim() == 0:
+            with pytest.raises(ValueError):
+                ops.quantize_rows_fp4(X)
+            continue
+        q, scale = ops.quantize_rows_fp4(X)
+        check_rows(X, q, scale)
+        assert torch.equal(ops.dequantize_rows_fp4(q, scale, X.shape[-1]).double(), fp4.values(*fp4.quantize(X), X.shape[-1]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_silu_is_torchs(dtype):
+    X = (3 * randn(700, 1030, seed=2)).to(TYPES[dtype])
+    X[0, :8] = torch.tensor([-200.0, -104, -88, -87, 0, 88, 200, -1e-6], device="cuda").to(X.dtype)
+    x = X.float()
+    check_rows(x / (1 + torch.exp(-x)), *ops.quantize_rows_fp4(X, activation="silu"))
+
+
+def test_quantize_many_rows_and_far_ones():
+    """More rows than a dimension of a grid has CTAs for, and elements beyond 2^31."""
+    X = randn(600011, 2, seed=7, dtype=torch.bfloat16)
+    check_rows(X, *ops.quantize_rows_fp4(X))
+    X = torch.zeros(2 ** 21 + 5, 1056, device="cuda", dtype=torch.bfloat16)
+    X[-3:] = randn(3, 1056, seed=8)
+    q, scale = ops.quantize_rows_fp4(X)
+    check_rows(X[-5:], q[-5:], scale[-5:])
+    assert torch.equal(ops.dequantize_rows_fp4(q, scale, dtype=torch.bfloat16)[-5:].double(), fp4.rows(q[-5:], scale[-5:]))
+
+
+# ---- products -----------------------------------------------------------------------------------------
+
+def product_bound(size, Y, C, out):
+    """A block's 32 products are exact and so is their sum; sums of blocks are float32: four truncations for two blocks at most, each by 2^-23 of what has
+    been summed, and the result is rounded once."""
+    return size * ((C / 64 + 2) * 4 * 2.0 ** -23) + Y.abs() * (torch.finfo(out).eps / 2 if out != torch.float32 else 0) + 1e-30
+
+
+def operands(rows, E, C, N, seed=0):
+    X = randn(rows, C, seed=seed) * torch.exp(randn(rows, 1, seed=seed + 1))
+    W = randn(E, N, C, seed=seed + 2) / C ** 0.5
+    return ops.quantize_rows_fp4(X), ops.quantize_rows_fp4(W)
+
+
+def even(C):
+    return (C + 1) // 2 * 2
+
+
+SHAPES = [(1, 32, 32), (5, 64, 33), (130, 256, 224), (128, 2048, 512), (700, 330, 201), (300, 1030, 777), (257, 96, 450), (64, 4100, 64), (1500, 512, 1000), (3, 1, 1)]
+
+
+@pytest.mark.parametrize("path", ["tensor", "generic"])
+@pytest.mark.parametrize("rows,C,N", SHAPES)
+def test_matmul(path, rows, C, N):
+    (q, s), (wq, ws) = operands(rows, 1, C, N)
+    x, w = fp4.rows(q, s), fp4.rows(wq[0], ws[0])
+    Y, size = x @ w.t(), x.abs() @ w.abs().t()
+    for out in TYPES.values():
+        got = ops.matmul_fp4(q, s, wq[0], ws[0], out_dtype=out, path=path)
+        assert got.shape == (rows, N) and got.dtype == out
+        worst = ((got.double() - Y).abs() - product_bound(size, Y, C, out)).max().item()
+        assert worst <= 0, (out, worst, (got.double() - Y).abs().max().item())
+
+
+def choose(tokens, E, k, seed, skew=0.5, idle=0, lost=0.0):
+    popular = skew * randn(E, seed=seed)
+    if idle:
+        popular[:idle] = -1e4
+    ids = (randn(tokens, E, seed=seed + 1) + popular).topk(k, -1).indices.int()
+    if lost:
+        ids[randn(tokens, k, seed=seed + 2).abs() < lost] = -1
+    return ids
+
+
+ROUTED = [(1, 64, 8, 256, 64, 0), (3, 64, 8, 2048, 512, 0), (200, 13, 3, 330, 201, 0.3), (1000, 8, 2, 512, 480, 0.1), (4000, 16, 4, 288, 512, 0), (50, 1, 1, 64, 32, 0.5), (6, 4, 2, 64, 64, 9.0), (900, 200, 2, 128, 96, 0)]
+
+
+@pytest.mark.parametrize("path", ["auto", "tensor", "generic"])
+@pytest.mark.parametrize("tokens,E,k,C,N,lost", ROUTED)
+def test_expert_matmul(path, tokens, E, k, C, N, lost):
+    ids = choose(tokens, E, k, seed=tokens, lost=lost, idle=E // 8)
+    plan = ops.plan_experts(ids, E)
+    for rows in ("tokens", "sorted"):
+        (q, s), (wq, ws) = operands(tokens if rows == "tokens" else tokens * k, E, C, N, seed=3)
+        Y, size = orc.matmul(fp4.rows(q, s), fp4.rows(wq, ws).transpose(1, 2), ids, E, rows)
+        for out in TYPES.values():
+            got = ops.expert_matmul_fp4(q, s, wq, ws, plan, rows=rows, out_dtype=out, path=path)
+            worst = ((got.double() - Y).abs() - product_bound(size, Y, C, out)).max().item()
+            assert worst <= 0, (rows, out, worst)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("path", ["tensor", "generic"])
+@pytest.mark.parametrize("tokens,E,k,C,N,lost", ROUTED)
+def test_expert_matmul_into_4_bits(path, tokens, E, k, C, N, lost):
+    """The rows that leave in 4 bits are those of the product in float32."""
+    ids = choose(tokens, E, k, seed=tokens, lost=lost)
+    plan = ops.plan_experts(ids, E)
+    (q, s), (wq, ws) = operands(tokens, E, C, N, seed=4)
+    full = ops.expert_matmul_fp4(q, s, wq, ws, plan, out_dtype=torch.float32, path=path)
+    check_rows(full, *ops.expert_matmul_fp4_rows(q, s, wq, ws, plan, path=path))
+    y, ys = ops.expert_matmul_fp4_rows(q, s, wq, ws, plan, activation="silu", path=path)
+    got = fp4.values(fp4.codes_of(y), ys, N)
+    want = fp4.values(*fp4.quantize(full / (1 + torch.exp(-full))), N)
+    # the tensor cores' read-out forms the activation within 2^-20: a value that lies so near a border may go the other way, one step, or its block's scale
+    off = got != want
+    assert off.double().mean().item() <= (0 if path == "generic" else 2e-4)
+    step = torch.exp2(torch.maximum(ys.double(), fp4.quantize(full / (1 + torch.exp(-full)))[1].double()) - 127).repeat_interleave(32, -1)[..., :N]
+    assert ((got - want).abs() <= 2 * step).all()
+    ops.check_status()
