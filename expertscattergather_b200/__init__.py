@@ -13,11 +13,11 @@ import sys
 
 from .torch_interface import ExpertGather, ExpertGatherScatter, ExpertScatter
 from .kernels import ExpertGatherFunction, ExpertScatterFunction, create_kernels
-from .token_choice import RoutedExperts, RoutedExpertsInt8, TokenRouter
+from .token_choice import RoutedExperts, RoutedExpertsFp4, RoutedExpertsInt8, TokenRouter
 from . import ops, token_choice
 
 __all__ = ["ExpertGather", "ExpertScatter", "ExpertGatherScatter", "ExpertGatherFunction", "ExpertScatterFunction", "create_kernels",
-           "TokenRouter", "RoutedExperts", "RoutedExpertsInt8", "token_choice", "ops", "install_as_egs"]
+           "TokenRouter", "RoutedExperts", "RoutedExpertsInt8", "RoutedExpertsFp4", "token_choice", "ops", "install_as_egs"]
 __version__ = "0.1.0"
 
 

@@ -36,7 +36,7 @@ EXPORTS = (
     "egs_expert_matmul_out", "egs_expert_matmul_workspace_bytes", "egs_expert_dweight", "egs_expert_dweight_workspace_bytes", "egs_combine",
     "egs_combine_out", "egs_combine_backward", "egs_quantize_rows", "egs_expert_matmul_int8",
     "egs_quantize_rows_fp4", "egs_dequantize_rows_fp4", "egs_expert_matmul_fp4", "egs_expert_matmul_fp4_rows",
-    "egs_expert_matmul_fp4_rows_workspace_bytes",
+    "egs_expert_matmul_fp4_rows_workspace_bytes", "egs_routed_experts_few", "egs_routed_experts_few_fp4", "egs_routed_experts_few_workspace_bytes",
 )
 
 
@@ -143,7 +143,10 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("egs_dequantize_rows_fp4", i, [vp, vp, vp, i64, i64, i64, i64, i, vp]),
             ("egs_expert_matmul_fp4", i, [vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, ragged, i, i, i, vp, vp]),
             ("egs_expert_matmul_fp4_rows", i, [vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, i64, i64, ragged, i, i, i, vp, sz, vp, vp]),
-            ("egs_expert_matmul_fp4_rows_workspace_bytes", sz, [ragged, i])):
+            ("egs_expert_matmul_fp4_rows_workspace_bytes", sz, [ragged, i]),
+            ("egs_routed_experts_few", i, [vp] * 8 + [route, i64, i64, i64, i, vp, sz, vp]),
+            ("egs_routed_experts_few_fp4", i, [vp, vp, vp, vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, route, i64, i64, i64, i, vp, sz, vp]),
+            ("egs_routed_experts_few_workspace_bytes", sz, [route, i64, i64])):
         getattr(lib, name).restype = result
         getattr(lib, name).argtypes = args
     lib.egs_fused_pair_eligible.restype = i

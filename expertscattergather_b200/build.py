@@ -21,7 +21,7 @@ OBJ_DIR = os.path.join(OUT_DIR, "obj")
 LIB_PATH = os.path.join(OUT_DIR, "libegs_b200.so")
 HOST_PATH = os.path.join(OUT_DIR, "_egs_host.so")
 SOURCES = ["egs_api.cu", "egs_generic.cu", "egs_tensor.cu", "egs_strict.cu", "egs_dense16.cu", "egs_pair16.cu", "egs_gather2.cu", "egs_index.cu", "egs_choice.cu", "egs_ragged.cu", "egs_few.cu",
-           "egs_choice_api.cu", "egs_fp4.cu", "egs_fp4_tensor.cu", "egs_fp4_api.cu"]
+           "egs_choice_api.cu", "egs_fp4.cu", "egs_fp4_tensor.cu", "egs_layer.cu", "egs_fp4_api.cu"]
 HOST_SOURCE = os.path.join(CSRC, "egs_host.cpp")
 API_HEADER = os.path.join(PKG, "..", "include", "egs_b200.h")
 HEADERS = [os.path.join(CSRC, "egs_internal.cuh"), os.path.join(CSRC, "egs_tcgen05.cuh"), os.path.join(CSRC, "egs_fp4.cuh"), API_HEADER]

@@ -147,28 +147,6 @@ cudaError_t from_fp4_t(const FromFp4& p, cudaStream_t st) {
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewWarps = 8, kFewRows = 4, kFewChannels = 4;
 
-struct Block4 {
-  uint32_t w[4];
-};
-// Block c of a row of `C` elements (an even number), zeros behind the row's end.
-__device__ __forceinline__ Block4 load_block(const uint8_t* row, int c, int C) {
-  Block4 b;
-  if ((c + 1) * kFp4Block <= C) {
-    const uint4 x = reinterpret_cast<const uint4*>(row)[c];
-    b.w[0] = x.x; b.w[1] = x.y; b.w[2] = x.z; b.w[3] = x.w;
-  } else {
-    const int left = C - c * kFp4Block;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      b.w[i] = 0u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (8 * i + 2 * j < left) b.w[i] |= static_cast<uint32_t>(row[c * 16ll + 4 * i + j]) << (8 * j);
-    }
-  }
-  return b;
-}
-
 template <typename OutT, int M>
 __device__ __forceinline__ void few_fp4(const Fp4Params& p, int expert, int first, int end, int n0) {
   const int lane = threadIdx.x & 31;

@@ -46,6 +46,28 @@ __device__ __forceinline__ void fp4_integers(uint32_t w, uint32_t& low, uint32_t
   high = __byte_perm(__byte_perm(p0, p1, m >> 16), __byte_perm(n0, n1, m >> 16), 0x3210u + (s >> 16));
 }
 
+struct Block4 {
+  uint32_t w[4];
+};
+// Block c of a row of `C` elements (an even number), zeros behind the row's end.
+__device__ __forceinline__ Block4 load_block(const uint8_t* row, int c, int C) {
+  Block4 b;
+  if ((c + 1) * kFp4Block <= C) {
+    const uint4 x = reinterpret_cast<const uint4*>(row)[c];
+    b.w[0] = x.x; b.w[1] = x.y; b.w[2] = x.z; b.w[3] = x.w;
+  } else {
+    const int left = C - c * kFp4Block;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b.w[i] = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (8 * i + 2 * j < left) b.w[i] |= static_cast<uint32_t>(row[c * 16ll + 4 * i + j]) << (8 * j);
+    }
+  }
+  return b;
+}
+
 // x / (1 + exp(-x)) as torch's elementary operations form it, bit by bit (the sum is not joined with the exponential's last product).
 __device__ __forceinline__ float silu_exact(float x) { return x / __fadd_rn(1.f, expf(-x)); }
 // The same from the fast exponential and division: within 2^-20 of it, relative (of results above 2^-100).

@@ -1,4 +1,4 @@
-// C entries of the operators in 4 bits: checks of arguments, choice of kernels.
+// C entries of the operators in 4 bits and of the whole layer for a few tokens: checks of arguments, choice of kernels.
 #include "egs_fp4.cuh"
 
 namespace egs {
@@ -63,6 +63,25 @@ int product(const Operands& o, const egs_ragged* dims, int rows, int path, int32
 // Whether the kernel for few rows takes this, by the caller's wish or because it is faster; `able`: the tensor cores could.
 bool takes_few(const Fp4Params& p, int path, bool able) { return !able || path == EGS_PATH_GENERIC || (path == EGS_PATH_AUTO && few_fp4_fit(p)); }
 bool tensor_able(const egs_ragged& d) { return device_is_sm100() && d.C > 0 && tiles_fit(d); }
+
+int check_layer(const egs_route* r, int64_t I, int64_t J) {
+  if (!r || r->tokens < 0 || r->E < 1 || r->top_k < 1 || r->groups < 1 || r->E % r->groups || r->top_groups < 1 || r->top_groups > r->groups ||
+      (r->group_top != 1 && r->group_top != 2) || r->top_k > r->E / r->groups * r->top_groups || (r->score != EGS_SCORE_SOFTMAX && r->score != EGS_SCORE_SIGMOID) ||
+      I < 1 || J < 1)
+    return EGS_ERR_INVALID_ARGUMENT;
+  if (r->E > EGS_MAX_EXPERTS || r->top_k > EGS_MAX_CHOICES || r->groups > EGS_MAX_GROUPS || r->tokens > EGS_MAX_FEW_TOKENS || r->tokens * r->top_k > EGS_MAX_FEW_SLOTS ||
+      I > kMaxWidth || J > kMaxWidth)
+    return EGS_ERR_TOO_LARGE;
+  return EGS_OK;
+}
+int layer(const FewLayer& f, const egs_route* r, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype) || f.x_row < 0) return EGS_ERR_INVALID_ARGUMENT;
+  if (int rc = check_layer(r, f.I, f.J)) return rc;
+  if (r->tokens == 0) return EGS_OK;
+  if (!f.X || !f.router || !f.up || !f.down || !f.out || !f.weights || !f.experts) return EGS_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < few_layer_workspace(*r, f.J) || !on16(workspace)) return EGS_ERR_WORKSPACE;
+  return done(launch_few_layer(f, *r, dtype, workspace, stream_of(stream)), "routed_experts_few launch");
+}
 
 }  // namespace
 }  // namespace egs
@@ -139,6 +158,29 @@ int egs_expert_matmul_fp4_rows(const uint8_t* q, const uint8_t* q_scale, int64_t
   p.y_row = p.N;
   if (cudaError_t err = launch_few_fp4(p, EGS_F32, st); err != cudaSuccess) return fail_cuda(err, "expert_matmul_fp4_rows launch");
   return done(launch_quantize_fp4(workspace, y, y_scale, p.rows, p.N, p.N, y_stride, ys_stride, activation, EGS_F32, st), "expert_matmul_fp4_rows in 4 bits");
+}
+
+size_t egs_routed_experts_few_workspace_bytes(const egs_route* route, int64_t I, int64_t J) {
+  return check_layer(route, I, J) == EGS_OK && route->tokens ? few_layer_workspace(*route, J) : 0;
+}
+
+int egs_routed_experts_few(const void* X, const void* router, const float* bias, const void* up, const void* down, void* out, float* weights,
+                           int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype, void* workspace,
+                           size_t workspace_bytes, void* cuda_stream) {
+  if (int rc = check_layer(route, I, J)) return rc;
+  const FewLayer f{X, router, bias, up, down, nullptr, nullptr, out, weights, experts, x_stride, 0, 0, 0, 0, static_cast<int>(I), static_cast<int>(J)};
+  return layer(f, route, dtype, workspace, workspace_bytes, cuda_stream);
+}
+
+int egs_routed_experts_few_fp4(const void* X, const void* router, const float* bias, const uint8_t* up, const uint8_t* up_scale, int64_t up_stride,
+                               int64_t us_stride, const uint8_t* down, const uint8_t* down_scale, int64_t down_stride, int64_t ds_stride, void* out,
+                               float* weights, int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype,
+                               void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  if (int rc = check_layer(route, I, J)) return rc;
+  if (!strides_hold(up_stride, us_stride, I, false) || !strides_hold(down_stride, ds_stride, J, false)) return EGS_ERR_INVALID_ARGUMENT;
+  if (route->tokens && (!up_scale || !down_scale || !on16(up) || !on16(down))) return EGS_ERR_INVALID_ARGUMENT;
+  const FewLayer f{X, router, bias, up, down, up_scale, down_scale, out, weights, experts, x_stride, up_stride, us_stride, down_stride, ds_stride, static_cast<int>(I), static_cast<int>(J)};
+  return layer(f, route, dtype, workspace, workspace_bytes, cuda_stream);
 }
 
 }  // extern "C"

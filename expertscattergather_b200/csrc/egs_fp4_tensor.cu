@@ -27,7 +27,6 @@ constexpr uint32_t kATile = 16384;                 // 128 rows x 128 bytes
 constexpr uint32_t kReadArea = 4096;               // transpose of a read-out warp
 constexpr size_t kFp4Smem = 227 * 1024;
 constexpr int kSmCount = 148;
-constexpr int kWidest = 224;
 constexpr int kStepElems = 256, kStepBlocks = 8;
 constexpr int kChunkSteps = 4;                     // steps whose scales come together
 constexpr uint32_t kAtom = 512;                    // scales of 128 rows and four blocks: [32 rows][4 x 32 rows][4 blocks]

@@ -49,7 +49,8 @@ struct Api {
   X(egs_expert_matmul_workspace_bytes) X(egs_expert_dweight) X(egs_expert_dweight_workspace_bytes) X(egs_combine_out)       \
   X(egs_combine_backward) X(egs_quantize_rows) X(egs_expert_matmul_int8)                                                   \
   X(egs_quantize_rows_fp4) X(egs_dequantize_rows_fp4) X(egs_expert_matmul_fp4) X(egs_expert_matmul_fp4_rows)                \
-  X(egs_expert_matmul_fp4_rows_workspace_bytes)
+  X(egs_expert_matmul_fp4_rows_workspace_bytes) X(egs_routed_experts_few) X(egs_routed_experts_few_fp4)                     \
+  X(egs_routed_experts_few_workspace_bytes)
 #define EGS_FIELD(name) decltype(&::name) name = nullptr;
   EGS_API(EGS_FIELD)
 #undef EGS_FIELD
@@ -829,4 +830,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dequantize_rows_fp4", &dequantize_rows_fp4, nogil());
   m.def("matmul_fp4", &matmul_fp4, nogil());
   m.def("matmul_fp4_rows", &matmul_fp4_rows, nogil());
+  m.def("routed_experts_few", &routed_experts_few, nogil());
 }

@@ -1,4 +1,4 @@
-// Operators on rows in 4 bits (included by egs_host.cpp behind egs_host_choice.h, whose helpers it uses).
+// Operators on rows in 4 bits and the whole layer for a few tokens (included by egs_host.cpp behind egs_host_choice.h, whose helpers it uses).
 
 int activation_id(const std::optional<std::string>& s) {
   if (!s) return EGS_ACT_NONE;
@@ -130,4 +130,62 @@ std::tuple<Tensor, Tensor> matmul_fp4_rows(const Tensor& q, const Tensor& q_scal
         "egs_expert_matmul_fp4_rows");
   c.debug();
   return {y.q, y.scale};
+}
+
+// The whole layer for a few tokens; up_scale and down_scale given: weights in 4 bits.
+std::tuple<Tensor, Tensor, Tensor> routed_experts_few(const Tensor& x, const Tensor& router, const Tensor& up, const Tensor& down, int64_t k, const OptTensor& bias,
+                                                      const OptTensor& up_scale, const OptTensor& down_scale, const std::string& score, int64_t groups,
+                                                      int64_t top_groups, int64_t group_top, bool renormalize, double scale) {
+  const bool fp4 = up_scale && up_scale->defined();
+  if (fp4 != (down_scale && down_scale->defined())) value_error("up_scale and down_scale belong together");
+  if (x.dim() < 1 || router.dim() != 2 || up.dim() != 3 || down.dim() != 3) value_error("expected x[..., I], router[E, I], up and down [E, ., .]");
+  const int dt = type_id(x.scalar_type()), sc = score_id(score);
+  if (router.scalar_type() != x.scalar_type() || (!fp4 && (up.scalar_type() != x.scalar_type() || down.scalar_type() != x.scalar_type())))
+    value_error("x, router and weights must have the same dtype");
+  Call c(x, router, up, down);
+  const int64_t I = x.size(-1), E = router.size(0), J = fp4 ? up.size(1) : up.size(2), tokens = rows_ahead(x);
+  const auto wrong = [&] {
+    value_error("shape mismatch: x" + shape_of(x) + " router" + shape_of(router) + " up" + shape_of(up) + " down" + shape_of(down) +
+                (fp4 ? " ([E, J, I / 2] and [E, I, J / 2] in 4 bits)" : " ([E, I, J] and [E, J, I])"));
+  };
+  if (router.size(1) != I || up.size(0) != E || down.size(0) != E) wrong();
+  if (fp4 ? up.size(2) != (I + 1) / 2 || down.size(1) != I || down.size(2) != (J + 1) / 2 : up.size(1) != I || down.size(1) != J || down.size(2) != I) wrong();
+  if (E < 1 || groups < 1 || E % groups || top_groups < 1 || top_groups > groups || (group_top != 1 && group_top != 2) || k < 1 || k > E / groups * top_groups)
+    value_error("routed_experts_few: E = " + std::to_string(E) + " experts in " + std::to_string(groups) + " groups, " + std::to_string(top_groups) +
+                " of them kept, do not give " + std::to_string(k) + " experts (group_top is 1 or 2)");
+  if (E > EGS_MAX_EXPERTS || k > EGS_MAX_CHOICES || groups > EGS_MAX_GROUPS || tokens > EGS_MAX_FEW_TOKENS || tokens * k > EGS_MAX_FEW_SLOTS)
+    value_error("routed_experts_few: at most " + std::to_string(int(EGS_MAX_FEW_TOKENS)) + " tokens, " + std::to_string(int(EGS_MAX_FEW_SLOTS)) + " of tokens * top_k, " +
+                std::to_string(int(EGS_MAX_EXPERTS)) + " experts, " + std::to_string(int(EGS_MAX_CHOICES)) + " choices and " + std::to_string(int(EGS_MAX_GROUPS)) + " groups");
+  Tensor b;
+  if (bias && bias->defined()) {
+    if (bias->numel() != E || !bias->is_floating_point()) value_error("bias must be a floating tensor of E elements");
+    if (!bias->is_cuda() || bias->get_device() != c.idx) throw std::runtime_error("bias must be on x's CUDA device");
+    b = bias->reshape({E}).to(at::kFloat).contiguous();
+  }
+  const Rows r = rows_of(x);
+  const Tensor w = router.contiguous();
+  auto shape = x.sizes().vec();
+  Tensor out = empty(shape, x.scalar_type(), c.idx);
+  shape.back() = k;
+  Tensor weights = empty(shape, at::kFloat, c.idx), experts = empty(shape, at::kInt, c.idx);
+  if (I == 0 || J == 0) value_error("routed_experts_few: no features");
+  const egs_route spec{tokens, int(E), int(k), int(groups), int(top_groups), int(group_top), sc, renormalize ? 1 : 0, float(scale)};
+  const size_t bytes = api.egs_routed_experts_few_workspace_bytes(&spec, I, J);
+  const Tensor ws = scratch(bytes, c.idx);
+  if (fp4) {
+    for (const Tensor* t : {&*up_scale, &*down_scale})
+      if (!t->is_cuda() || t->get_device() != c.idx) throw std::runtime_error("all tensors must be on the same CUDA device");
+    const Given4 u = given_rows4(up, *up_scale, "weights"), d = given_rows4(down, *down_scale, "weights");
+    check(api.egs_routed_experts_few_fp4(ptr(r.t), ptr(w), static_cast<const float*>(ptr(b)), bytes_of(u.q), bytes_of(u.scale), u.q.pitch, u.scale.pitch, bytes_of(d.q),
+                                         bytes_of(d.scale), d.q.pitch, d.scale.pitch, ptr(out), weights.data_ptr<float>(), experts.data_ptr<int>(), &spec, I, J, r.stride, dt,
+                                         ptr(ws), bytes, c.stream),
+          "egs_routed_experts_few_fp4");
+  } else {
+    const Tensor u = whole(up), d = whole(down);
+    check(api.egs_routed_experts_few(ptr(r.t), ptr(w), static_cast<const float*>(ptr(b)), ptr(u), ptr(d), ptr(out), weights.data_ptr<float>(), experts.data_ptr<int>(), &spec, I, J,
+                                     r.stride, dt, ptr(ws), bytes, c.stream),
+          "egs_routed_experts_few");
+  }
+  c.debug();
+  return {out, weights, experts};
 }

@@ -359,6 +359,21 @@ cudaError_t launch_dequantize_fp4(const uint8_t* q, const uint8_t* scale, void* 
 bool few_fp4_fit(const Fp4Params& p);
 cudaError_t launch_few_fp4(const Fp4Params& p, int out_dtype, cudaStream_t st);
 cudaError_t launch_fp4_rows_tensor(const Fp4Params& p, int out_dtype, cudaStream_t st);
+// A whole routed layer for a few tokens (egs_layer.cu); the scales NULL: weights [E, I, J] and [E, J, I] of the rows' type, else in 4 bits, [E, J, I / 2]
+// and [E, I, J / 2], with strides in bytes.
+struct FewLayer {
+  const void *X, *router;
+  const float* bias;
+  const void *up, *down;
+  const uint8_t *up_scale, *down_scale;
+  void* out;
+  float* weights;
+  int* experts;
+  long long x_row, up_row, us_row, down_row, ds_row;
+  int I, J;
+};
+size_t few_layer_workspace(const egs_route& r, long long J);
+cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st);
 // Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; zeros behind a row's end); dst NULL: nothing.
 struct PadRows {
   const void* src;

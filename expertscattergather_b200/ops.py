@@ -18,7 +18,8 @@ __all__ = ["gather_gemm", "gemm_scatter", "gather_scatter_pair", "fused_pair_eli
            "check_status", "reset_status", "publish_status", "launch_count", "dtype_to_type_id", "tensor_path_eligible", "describe_plan", "describe_kept_rows", "describe_half_tiles", "route_topk", "build_index_csr", "compact_index", "gemm_scatter_csr", "IndexCSR",
            "route_tokens", "route_tokens_backward", "plan_experts", "ExpertPlan", "expert_matmul", "expert_dweight", "combine", "combine_backward",
            "quantize_rows", "matmul_int8", "expert_matmul_int8",
-           "quantize_rows_fp4", "dequantize_rows_fp4", "matmul_fp4", "expert_matmul_fp4", "expert_matmul_fp4_rows"]
+           "quantize_rows_fp4", "dequantize_rows_fp4", "matmul_fp4", "expert_matmul_fp4", "expert_matmul_fp4_rows",
+           "routed_experts_few", "FEW_TOKENS", "FEW_SLOTS"]
 
 _PRECISIONS = {"strict": _lib.PREC_STRICT, "fp32": _lib.PREC_STRICT, "tf32": _lib.PREC_TF32}
 _PATHS = {"auto": _lib.PATH_AUTO, "generic": _lib.PATH_GENERIC, "tensor": _lib.PATH_TENSOR,
@@ -542,3 +543,22 @@ def expert_matmul_fp4_rows(q, scale, Wq, w_scale, plan: ExpertPlan, *, rows="tok
     """:func:`expert_matmul_fp4` whose sorted rows (with ``activation='silu'`` their activations, formed in float32) leave in 4 bits again, as
     ``(q, scale)`` for the next product: what lies between two products of a layer is neither stored in full nor read again."""
     return _host().matmul_fp4_rows(q, scale, Wq, w_scale, plan.offsets, plan.slots, plan.tokens, plan.k, rows, activation, _path(path))
+
+
+# ---- a whole routed layer for a few tokens ----------------------------------------------------------------
+
+FEW_TOKENS, FEW_SLOTS = 32, 256          # most tokens of a call of routed_experts_few, most tokens * top_k
+
+
+def routed_experts_few(x, router, up, down, top_k, bias=None, *, up_scale=None, down_scale=None, score="softmax", groups=1, top_groups=1,
+                       group_top=2, renormalize=True, scale=1.0):
+    """A routed layer for a few tokens, as a decoding step has them: ``out[t] = sum_j weights[t, j] * silu(x[t] @ up[e]) @ down[e]`` with
+    ``e = experts[t, j]``.  Returns ``(out [..., I], weights [..., top_k], experts [..., top_k])``.
+
+    ``x`` [..., I] of at most ``FEW_TOKENS`` tokens and ``FEW_SLOTS`` of tokens * top_k, ``router`` [E, I], ``up`` [E, I, J], ``down`` [E, J, I] of
+    one type; or, with their scales, weights in 4 bits as :func:`quantize_rows_fp4` makes them of the transposed ones, ``up`` [E, J, I / 2] and ``down``
+    [E, I, J / 2]: the rows ahead of both products are then rounded to 4 bits as well, and sums are those of :func:`expert_matmul_fp4`.
+    Choice and weights are those of :func:`route_tokens`, of logits that stay float32 (a module's are rounded to its type).  All sums and what
+    lies between the products are float32; ``out`` is rounded once.  No gradients.  The same bits in every run."""
+    return _host().routed_experts_few(x, router, up, down, int(top_k), bias, up_scale, down_scale, score, int(groups), int(top_groups), int(group_top),
+                                      bool(renormalize), float(scale))

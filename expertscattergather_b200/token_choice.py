@@ -1,8 +1,10 @@
 """Layers whose tokens choose their experts: the router, the experts' products with their gradients, and the layer made of them, for
-training and, with 8-bit weights, for serving.
+training and, with weights in 8 or 4 bits, for serving.
 
     layer = RoutedExperts(E, I, J, top_k).cuda()        # x [..., I] -> [..., I]
     served = layer.quantized()                          # the same layer on int8 weights, no gradients
+    served = layer.quantized(bits=4)                    # ... on weights in 4 bits
+    y = layer.few(x)                                    # a decoding step's few tokens, no gradients
 
 No counterpart in the reference, whose experts choose their tokens (``ExpertGather`` / ``ExpertScatter``).  The operators are those of
 ``ops``; here they have gradients, first ones alone: a second derivative through them raises.  ``torch.compile`` runs the operators as they
@@ -21,7 +23,7 @@ from torch.nn import functional as F
 from . import ops
 
 __all__ = ["RouteTokensFunction", "ExpertMatmulFunction", "CombineFunction", "route_tokens", "expert_matmul", "combine", "TokenRouter",
-           "RoutedExperts", "RoutedExpertsInt8"]
+           "RoutedExperts", "RoutedExpertsInt8", "RoutedExpertsFp4"]
 
 
 class RouteTokensFunction(torch.autograd.Function):
@@ -160,12 +162,21 @@ class RoutedExperts(nn.Module):
         return combine(expert_matmul(h, self.down, plan, rows="sorted", out_dtype=wide), weights, plan, out_dtype=x.dtype).view(x.shape)
 
     @torch.no_grad()
-    def quantized(self) -> "RoutedExpertsInt8":
-        return RoutedExpertsInt8(self)
+    def few(self, x):
+        """The layer for a decoding step's few tokens (``ops.routed_experts_few``, and its limits), without gradients.  Logits and what lies between
+        the products stay float32 here, so that results are nearer to the definition than :meth:`forward`'s."""
+        return ops.routed_experts_few(x, self.router.W, self.up, self.down, self.router.top_k, self.router.balance, **self.router.options)[0]
+
+    @torch.no_grad()
+    def quantized(self, bits: int = 8):
+        """The layer for serving, on weights in 8 bits (:class:`RoutedExpertsInt8`) or 4 (:class:`RoutedExpertsFp4`)."""
+        if bits not in (8, 4):
+            raise ValueError("bits must be 8 or 4")
+        return RoutedExpertsInt8(self) if bits == 8 else RoutedExpertsFp4(self)
 
 
 def _in_pitch(q):
-    """8-bit rows a multiple of 16 bytes apart, as ``ops.quantize_rows`` lays them out and the products read them without a copy."""
+    """Rows of bytes a multiple of 16 apart, as ``ops.quantize_rows`` lays them out and the products read them without a copy."""
     pitch = (q.shape[-1] + 15) // 16 * 16
     if q.stride(-1) == 1 and q.stride(-2) == pitch:
         return q
@@ -203,4 +214,37 @@ class RoutedExpertsInt8(nn.Module):
         rows = torch.float32 if self.float32_rows else x.dtype
         h = F.silu(ops.expert_matmul_int8(*ops.quantize_rows(x), self.up, self.up_scale, plan, out_dtype=rows))
         y = ops.expert_matmul_int8(*ops.quantize_rows(h), self.down, self.down_scale, plan, rows="sorted", out_dtype=rows)
+        return ops.combine(y, weights, plan, out_dtype=x.dtype).view(x.shape)
+
+
+class RoutedExpertsFp4(nn.Module):
+    """A :class:`RoutedExperts` for serving: weights in 4 bits (``ops.quantize_rows_fp4`` along their contractions), rows rounded to 4 bits on the way
+    into each product.  A call of a few tokens (``ops.FEW_TOKENS``, ``ops.FEW_SLOTS``) is one of ``ops.routed_experts_few``, whose logits stay float32;
+    in others the router is the module's own.  It has a router of its own, as :class:`RoutedExpertsInt8` has."""
+
+    def __init__(self, layer: RoutedExperts):
+        super().__init__()
+        self.E, self.I, self.float32_rows = layer.E, layer.I, layer.float32_rows
+        self.router = copy.deepcopy(layer.router).requires_grad_(False)
+        for name in ("up", "down"):
+            q, scale = ops.quantize_rows_fp4(getattr(layer, name).detach().transpose(1, 2))
+            self.register_buffer(name, q)
+            self.register_buffer(name + "_scale", scale)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        for name in ("up", "down", "up_scale", "down_scale"):
+            setattr(self, name, _in_pitch(getattr(self, name)))           # (a copy to another device has its rows together)
+        return self
+
+    @torch.no_grad()
+    def forward(self, x):
+        tokens, k = x.numel() // max(self.I, 1), self.router.top_k
+        if tokens <= ops.FEW_TOKENS and tokens * k <= ops.FEW_SLOTS:
+            return ops.routed_experts_few(x, self.router.W, self.up, self.down, k, self.router.balance, up_scale=self.up_scale, down_scale=self.down_scale,
+                                          **self.router.options)[0]
+        weights, experts = self.router(x)
+        plan = ops.plan_experts(experts, self.E)
+        h = ops.expert_matmul_fp4_rows(*ops.quantize_rows_fp4(x), self.up, self.up_scale, plan, activation="silu")
+        y = ops.expert_matmul_fp4(*h, self.down, self.down_scale, plan, rows="sorted", out_dtype=torch.float32 if self.float32_rows else x.dtype)
         return ops.combine(y, weights, plan, out_dtype=x.dtype).view(x.shape)

@@ -424,6 +424,25 @@ int egs_expert_matmul_fp4_rows(const uint8_t* q, const uint8_t* q_scale, int64_t
                                size_t workspace_bytes, int32_t* status_word, void* cuda_stream);
 size_t egs_expert_matmul_fp4_rows_workspace_bytes(const egs_ragged* dims, int path);
 
+/* ------------------------------------------------------------------------------------------------
+ * A whole routed layer for a few tokens.  (No counterpart in the reference.)
+ *
+ * out[t] = sum over j of weights[t, j] * silu(X[t] up[e]) down[e], e = experts[t, j]: weights and experts [tokens, top_k] are those of egs_route_tokens for the
+ * logits X[t] . router[e] [E, I], which stay float32, as do all sums; out [tokens, I] is rounded once.  X's rows lie x_stride elements apart.
+ * up [E, I, J], down [E, J, I]; or in 4 bits (egs_quantize_rows_fp4), up [E, J, I / 2] and down [E, I, J / 2], where X's rows and silu(..) are rounded to
+ * 4 bits ahead of their products too.  At most EGS_MAX_FEW_TOKENS tokens and EGS_MAX_FEW_SLOTS = tokens * top_k.
+ * workspace (16-byte aligned): egs_routed_experts_few_workspace_bytes() bytes.  The same bits in every run.
+ * ------------------------------------------------------------------------------------------------ */
+enum { EGS_MAX_FEW_TOKENS = 32, EGS_MAX_FEW_SLOTS = 256 };
+int egs_routed_experts_few(const void* X, const void* router, const float* bias, const void* up, const void* down, void* out, float* weights,
+                           int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype, void* workspace,
+                           size_t workspace_bytes, void* cuda_stream);
+int egs_routed_experts_few_fp4(const void* X, const void* router, const float* bias, const uint8_t* up, const uint8_t* up_scale, int64_t up_stride,
+                               int64_t us_stride, const uint8_t* down, const uint8_t* down_scale, int64_t down_stride, int64_t ds_stride, void* out,
+                               float* weights, int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype,
+                               void* workspace, size_t workspace_bytes, void* cuda_stream);
+size_t egs_routed_experts_few_workspace_bytes(const egs_route* route, int64_t I, int64_t J);
+
 /* Number of kernels the library has launched in this process since load (for launch accounting). */
 int64_t egs_launch_count(void);
 
