@@ -4,15 +4,16 @@
 // Persistent CTAs, or pairs of them, walk tiles of 128 (256) sorted rows of one expert x BN columns.  A step is 256 elements, 128 bytes of a row:
 // four MMAs.  Their scales lie in tensor memory beside two accumulators, which leaves 224 columns for each: a tile is no wider.
 //
-//   warps 0..3    gathered rows of X (tile::gather4), where they are gathered
-//   warp  4       boxes of rows that follow one another and of weights; announces the bytes of a stage
-//   warp  5       tensor-memory allocation; copies a step's scales to tensor memory and issues its MMAs, by the leader of a pair for both CTAs
-//   warps 6, 7    scales: of four steps at a time, from rows to the order in which tensor memory takes them
+//   warps 0, 1    gathered rows of X (tile::gather4), where they are gathered
+//   warp  2       boxes of rows that follow one another and of weights; announces the bytes of a stage
+//   warp  3       tensor-memory allocation; copies a step's scales to tensor memory and issues its MMAs, by the leader of a pair for both CTAs
+//   warps 4..7    scales: of two steps at a time, from rows to the order in which tensor memory takes them
 //   warps 8..15   read-out: tensor memory -> rows of the output, in float32, 16 bits or (activated) in 4 bits with their scales
 //
 // Scales cannot come by TMA: of a row there are 8 bytes a step, and tensor memory wants four bytes of four rows beside one another.  Both CTAs of a pair
-// need the scales of all columns.  A pair's second CTA tells the leader by a releasing arrival, once for four steps: such an arrival waits behind a
-// memory barrier for longer than a step takes.
+// need the scales of all columns.  What the second one's warps have stored is made visible to its tensor core by their proxy fence; their
+// arrival at the leader's barrier says no more than that this has happened, and a release of everything at cluster scope, which waits behind a memory
+// barrier, made the kernel wait for it (8192 x 4096 -> 4096: 94 us for 74; word by word with cp.async 106; no scales at all 61, no products 47).
 #include "egs_fp4.cuh"
 #include "egs_tcgen05.cuh"
 
@@ -20,7 +21,7 @@ namespace egs {
 
 namespace {
 
-constexpr int kGatherWarps = 4, kBoxWarp = 4, kIssueWarp = 5, kScaleWarp0 = 6, kScaleWarps = 2, kReadWarp0 = 8, kReadWarps = 8;
+constexpr int kGatherWarps = 2, kBoxWarp = 2, kIssueWarp = 3, kScaleWarp0 = 4, kScaleWarps = 4, kReadWarp0 = 8, kReadWarps = 8;
 constexpr int kFp4Threads = (kReadWarp0 + kReadWarps) * 32;
 constexpr uint32_t kFp4Header = 512;
 constexpr uint32_t kATile = 16384;                 // 128 rows x 128 bytes
@@ -33,11 +34,13 @@ constexpr uint32_t kAtom = 512;                    // scales of 128 rows and fou
 constexpr uint32_t kChunkA = kChunkSteps * 2 * kAtom, kChunkB = 2 * kChunkA, kChunkBytes = kChunkA + kChunkB;
 constexpr uint32_t kScaleCols = 24;                // tensor-memory columns of a step's scales: 2 x 4 of rows, 2 x 8 of columns
 
+constexpr int kScaleRing = 2;                      // chunks that are on their way
+
 struct __align__(16) Fp4Header {
   unsigned long long full[kMaxStages];
   unsigned long long empty[kMaxStages];
-  unsigned long long scale_full[2];
-  unsigned long long scale_empty[2];
+  unsigned long long scale_full[kScaleRing];
+  unsigned long long scale_empty[kScaleRing];
   unsigned long long acc_full[2];
   unsigned long long acc_empty[2];
   unsigned long long drain;
@@ -122,22 +125,111 @@ __device__ __forceinline__ int expert_of(const int* starts, int E, int block, in
   return lo;
 }
 
-// Up to 32 bytes of a row's scales from block `b` on as words; zeros behind the row's end and for rows that are not there.
-__device__ __forceinline__ void load_scales(const uint8_t* row, int b, int blocks, uint32_t (&w)[8]) {
+// 16 bytes of a row's scales from block `b` on as words; zeros behind the row's end and for rows that are not there.
+__device__ __forceinline__ void load_scales(const uint8_t* row, int b, int blocks, uint32_t (&w)[4]) {
+  if (row && b + 16 <= blocks) {
+    const uint4 x = *reinterpret_cast<const uint4*>(row + b);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int first = b + h * 16;
-    if (row && first + 16 <= blocks) {
-      const uint4 x = *reinterpret_cast<const uint4*>(row + first);
-      w[4 * h] = x.x; w[4 * h + 1] = x.y; w[4 * h + 2] = x.z; w[4 * h + 3] = x.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[4 * h + i] = 0u;
-        for (int j = 0; j < 4; ++j)
-          if (row && first + 4 * i + j < blocks) w[4 * h + i] |= static_cast<uint32_t>(row[first + 4 * i + j]) << (8 * j);
-      }
+    for (int i = 0; i < 4; ++i) {
+      w[i] = 0u;
+      for (int j = 0; j < 4; ++j)
+        if (row && b + 4 * i + j < blocks) w[i] |= static_cast<uint32_t>(row[b + 4 * i + j]) << (8 * j);
     }
+  }
+}
+
+// The warps that bring scales.  P neighbouring lanes have 16 P bytes of a row, 16 each, and a lane hands its words over when their two steps come, with four steps'; what is behind is
+// asked for `kSets` such stretches ahead.  A request of the L2 takes as long for 16 bytes as for 64: 16 or 32 bytes of a row at a time, scales held up the operands (8192 x
+// 4096 -> 4096: 80 us, 64 bytes 70), while stretches longer than a contraction leave nothing on its way under a tile (512 -> 2048: 64 bytes 197 us, 16 86).
+struct ScaleTiles {
+  const int *offsets, *starts;
+  int units, first, stride, block, row0;
+  uint32_t scales, full, empty;
+  volatile uint32_t* abort_flag;
+};
+template <int P, bool PAIR>
+__device__ __forceinline__ void scale_warps(const Fp4Params& p, const Fp4Tiles& q, const ScaleTiles& t, bool second) {
+  constexpr int kSets = P == 1 ? 3 : P == 2 ? 2 : 1, kTurn = 128 / P, kColTurns = P == 4 ? 7 : 2 * P;      // (a tile has 224 columns at most)
+  struct Words {
+    uint32_t a[P][4], b[kColTurns][4];
+    int chunks;
+  };
+  const int lane = threadIdx.x & 31, piece = lane % P, mine = (threadIdx.x / 32 - kScaleWarp0) * (32 / P) + lane / P;
+  int round = 0, s0 = 0, e = 0;
+  int row[P], coming[P], columns_here = 0;           // rows of X of the tile and (their slots) of the next one
+  const uint8_t* b_rows = nullptr;
+  auto unit_of = [&](int r) { return r * t.stride + t.first; };
+  auto rows_of = [&](int u) {
+    if (u >= t.units) return;
+    const int block = q.by_n.quotient(u);
+    e = expert_of(t.starts, p.E, block, e);
+    const int r = t.offsets[e] + (block - t.starts[e]) * t.block + t.row0 + mine, end = t.offsets[e + 1];
+#pragma unroll
+    for (int i = 0; i < P; ++i) coming[i] = r + i * kTurn < end ? p.slots ? p.slots[r + i * kTurn] : r + i * kTurn : -1;
+  };
+  auto ask = [&](Words& w) {
+    const int u = unit_of(round);
+    w.chunks = 0;
+    if (u >= t.units) return;
+    if (s0 == 0) {
+      const int block = q.by_n.quotient(u), n0 = (u - block * q.tiles_n) * q.BN;
+      columns_here = min(q.BN, p.N - n0);
+#pragma unroll
+      for (int i = 0; i < P; ++i) row[i] = coming[i] >= 0 && p.slots ? p.by_k.quotient(coming[i]) : coming[i];
+      b_rows = p.Ws + e * p.ws_expert + (n0 + mine) * p.ws_row;
+      rows_of(unit_of(round + 1));
+    }
+    const int first = s0 * kStepBlocks + piece * 16;
+#pragma unroll
+    for (int i = 0; i < P; ++i) load_scales(row[i] >= 0 ? p.As + row[i] * p.as_row : nullptr, first, q.blocks, w.a[i]);
+#pragma unroll
+    for (int i = 0; i < kColTurns; ++i) load_scales(mine + i * kTurn < columns_here ? b_rows + i * kTurn * p.ws_row : nullptr, first, q.blocks, w.b[i]);
+    w.chunks = min((P + 1) / 2, (q.steps - s0 + kChunkSteps - 1) / kChunkSteps);
+    s0 += 2 * P;
+    if (s0 >= q.steps) {
+      s0 = 0;
+      ++round;
+    }
+  };
+  RingCursor chunk;
+  auto turn = [&](Words& w) {
+    if (w.chunks == 0) return false;
+#pragma unroll 1
+    for (int c = 0; c < w.chunks; ++c) {
+      if (chunk.round > 0 && !mbar_wait_all(t.empty + chunk.slot * 8u, (chunk.round - 1) & 1, t.abort_flag, p.status.word)) return false;
+      if (piece >> 1 == c) {
+        const uint32_t to = t.scales + static_cast<uint32_t>(chunk.slot) * kChunkBytes, half = static_cast<uint32_t>(piece & 1) * 4u;      // (four words of a chunk's eight)
+        auto put = [&](uint32_t base, uint32_t stride, int r, const uint32_t (&x)[4]) {
+          const uint32_t at = base + static_cast<uint32_t>(r & 31) * 16u + static_cast<uint32_t>(r >> 5 & 3) * 4u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + static_cast<uint32_t>(j) * stride), "r"(x[j]) : "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < P; ++i) put(to + half * kAtom, kAtom, i * kTurn + mine, w.a[i]);
+#pragma unroll
+        for (int i = 0; i < kColTurns; ++i) put(to + kChunkA + (half * 2u + static_cast<uint32_t>(i * kTurn >> 7)) * kAtom, 2u * kAtom, i * kTurn + mine, w.b[i]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR && second) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_cta(t.full + chunk.slot * 8u, 0)) : "memory");
+        else mbar_arrive(t.full + chunk.slot * 8u);
+      }
+      chunk.next(kScaleRing);
+    }
+    ask(w);
+    return true;
+  };
+  Words w[kSets];
+  rows_of(unit_of(0));
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) ask(w[i]);
+  bool more = true;
+  while (more) {
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) more = more && turn(w[i]);
   }
 }
 
@@ -162,7 +254,7 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
   const int columns = PAIR ? q.BN / 2 : q.BN;        // of the right operand, staged by this CTA
   const uint32_t stage_bytes = kATile + static_cast<uint32_t>(columns) * 128u;
   const uint32_t scales0 = ring0 + static_cast<uint32_t>(q.stages) * stage_bytes;      // (rows of 128 bytes, eight at a time: whole 1024 bytes)
-  const uint32_t area0 = scales0 + 2u * kChunkBytes;
+  const uint32_t area0 = scales0 + kScaleRing * kChunkBytes;                 // (rows in 4 bits need none)
   const uint32_t acc_cols = static_cast<uint32_t>(q.BN), scale_cols = 2u * acc_cols, all_cols = tmem_cols_for(2 * q.BN + 2 * static_cast<int>(kScaleCols));
   volatile uint32_t* abort_flag = &hdr->abort_flag;
   const int first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_stride = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -173,9 +265,11 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
       mbar_init(smem_u32(&hdr->full[s]), 1);
       mbar_init(smem_u32(&hdr->empty[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kScaleRing; ++b) {
       mbar_init(smem_u32(&hdr->scale_full[b]), PAIR ? 2 * kScaleWarps : kScaleWarps);  // (a pair's: the leader's copy is used)
       mbar_init(smem_u32(&hdr->scale_empty[b]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&hdr->acc_full[b]), 1);
       mbar_init(smem_u32(&hdr->acc_empty[b]), PAIR ? 2 * kReadWarps : kReadWarps);     // (the leader's too)
     }
@@ -248,21 +342,21 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
       for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
         const int block = q.by_n.quotient(u);
         e = expert_of(starts, p.E, block, e);
-        const int r = offsets[e] + (block - starts[e]) * kBlock + rank * 128 + warp * 32 + lane;
-        const int mine = r < offsets[e + 1] ? p.by_k.quotient(p.slots[r]) : -1;
-        int row[8][4];
+        const int r = offsets[e] + (block - starts[e]) * kBlock + rank * 128 + warp * 64 + lane, end = offsets[e + 1];
+        const int low = r < end ? p.by_k.quotient(p.slots[r]) : -1, high = r + 32 < end ? p.by_k.quotient(p.slots[r + 32]) : -1;
+        int row[16][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 16; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) row[i][j] = __shfl_sync(0xffffffffu, mine, i * 4 + j);
+          for (int j = 0; j < 4; ++j) row[i][j] = __shfl_sync(0xffffffffu, i < 8 ? low : high, i % 8 * 4 + j);
         for (int ks = 0; ks < q.steps; ++ks) {
           if (!wait_free()) break;
           const uint32_t bar = full0 + at.slot * 8u;
-          const uint32_t dst = ring0 + static_cast<uint32_t>(at.slot) * stage_bytes + static_cast<uint32_t>(warp) * 4096u;
+          const uint32_t dst = ring0 + static_cast<uint32_t>(at.slot) * stage_bytes + static_cast<uint32_t>(warp) * 8192u;
           at.next(q.stages);
           if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) load_rows4<PAIR>(dst + i * 512u, &map_a4, ks * 128, row[i], bar);
+            for (int i = 0; i < 16; ++i) load_rows4<PAIR>(dst + i * 512u, &map_a4, ks * 128, row[i], bar);
           }
         }
       }
@@ -297,7 +391,8 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
       // E2M1 operands (format 1), scales as powers of two, K-major; places of the scales' bytes come with the MMAs
       const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(q.BN >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(kBlock >> 4) << 24);
       const bool wide = q.BN > 128;
-      int t = 0, chunk = 0;
+      int t = 0;
+      RingCursor chunk;
       uint32_t parity = 0u;
       for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
         const int buf = t & 1;
@@ -310,19 +405,19 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
         for (int ks = 0; ks < q.steps; ++ks) {
           const int part = ks % kChunkSteps;
           if (part == 0) {
-            alive = mbar_wait_all<PAIR>(smem_u32(&hdr->scale_full[chunk & 1]), (chunk >> 1) & 1, abort_flag, p.status.word);
+            alive = mbar_wait_all<PAIR>(smem_u32(&hdr->scale_full[chunk.slot]), chunk.round & 1, abort_flag, p.status.word);
             if (!alive) break;
           }
           alive = mbar_wait_all<PAIR>(smem_u32(&hdr->full[at.slot]), at.round & 1, abort_flag, p.status.word);
           if (!alive) break;
-          const uint32_t empty = smem_u32(&hdr->empty[at.slot]), scale_empty = smem_u32(&hdr->scale_empty[chunk & 1]);
+          const uint32_t empty = smem_u32(&hdr->empty[at.slot]), scale_empty = smem_u32(&hdr->scale_empty[chunk.slot]);
           const uint32_t addr = (ring0 + static_cast<uint32_t>(at.slot) * stage_bytes) >> 4;
-          const uint32_t scales = scales0 + static_cast<uint32_t>(chunk & 1) * kChunkBytes + static_cast<uint32_t>(part) * 2u * kAtom;
+          const uint32_t scales = scales0 + static_cast<uint32_t>(chunk.slot) * kChunkBytes + static_cast<uint32_t>(part) * 2u * kAtom;
           const uint32_t sa = tmem_base + scale_cols + parity * kScaleCols, sb = sa + 8u;
           const bool last = ks + 1 == q.steps, last_of_chunk = last || part + 1 == kChunkSteps;
           at.next(q.stages);
           parity ^= 1u;
-          if (last_of_chunk) ++chunk;
+          if (last_of_chunk) chunk.next(kScaleRing);
           tc_fence_after();
           if (elect_one()) {
             const uint64_t from_a = s_desc + (scales >> 4), from_b = s_desc + ((scales + kChunkA + static_cast<uint32_t>(part) * 2u * kAtom) >> 4);
@@ -344,73 +439,10 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
     __syncwarp();
   } else if (warp < kReadWarp0) {
     // =========================== scales ===========================
-    // A thread has two of the tile's rows and up to four of its columns.  What comes next is asked for before this is handed over.
-    const int mine = (warp - kScaleWarp0) * 32 + lane;
-    const uint8_t *a_row[2], *b_row[4];
-    uint32_t wa[2][8], wb[4][8];
-    int round = 0, ks = 0, e = 0;
-    int coming[2];                                   // rows of X of the next tile
-    auto rows_of = [&](int u) {
-      if (u >= units) return;
-      const int block = q.by_n.quotient(u);
-      e = expert_of(starts, p.E, block, e);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = offsets[e] + (block - starts[e]) * kBlock + rank * 128 + i * 64 + mine;
-        coming[i] = r < offsets[e + 1] ? p.slots ? p.by_k.quotient(p.slots[r]) : r : -1;
-      }
-    };
-    auto begin_tile = [&](int u) {
-      const int block = q.by_n.quotient(u), n0 = (u - block * q.tiles_n) * q.BN;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) a_row[i] = coming[i] >= 0 ? p.As + coming[i] * p.as_row : nullptr;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = i * 64 + mine;
-        b_row[i] = n < q.BN && n0 + n < p.N ? p.Ws + e * p.ws_expert + (n0 + n) * p.ws_row : nullptr;
-      }
-      rows_of(unit_of(round + 1));
-    };
-    auto ask = [&]() {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) load_scales(a_row[i], ks * kStepBlocks, q.blocks, wa[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i * 64 < q.BN) load_scales(b_row[i], ks * kStepBlocks, q.blocks, wb[i]);
-    };
-    rows_of(unit_of(0));
-    if (unit_of(0) < units) {
-      begin_tile(unit_of(0));
-      ask();
-    }
-    for (int chunk = 0; unit_of(round) < units; ++chunk) {
-      if (chunk >= 2 && !mbar_wait_all(smem_u32(&hdr->scale_empty[chunk & 1]), ((chunk >> 1) - 1) & 1, abort_flag, p.status.word)) break;
-      const uint32_t to = scales0 + static_cast<uint32_t>(chunk & 1) * kChunkBytes;
-      auto put = [&](uint32_t base, uint32_t stride, int row, const uint32_t (&w)[8]) {
-        const uint32_t at0 = base + static_cast<uint32_t>(row & 31) * 16u + static_cast<uint32_t>(row >> 5 & 3) * 4u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at0 + static_cast<uint32_t>(i) * stride), "r"(w[i]) : "memory");
-      };
-#pragma unroll
-      for (int i = 0; i < 2; ++i) put(to, kAtom, i * 64 + mine, wa[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i * 64 < q.BN) put(to + kChunkA + static_cast<uint32_t>(i >> 1) * kAtom, 2u * kAtom, (i & 1) * 64 + mine, wb[i]);
-      ks += kChunkSteps;
-      if (ks >= q.steps) {
-        ks = 0;
-        ++round;
-        if (unit_of(round) < units) begin_tile(unit_of(round));
-      }
-      if (unit_of(round) < units) ask();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        const uint32_t bar = smem_u32(&hdr->scale_full[chunk & 1]);
-        if (PAIR && !leader) mbar_arrive_cluster(map_to_cta(bar, 0));
-        else mbar_arrive(bar);
-      }
-    }
+    const ScaleTiles tiles{offsets, starts, units, first_unit, unit_stride, kBlock, rank * 128, scales0, smem_u32(&hdr->scale_full[0]), smem_u32(&hdr->scale_empty[0]), abort_flag};
+    if (q.steps > 4) scale_warps<4, PAIR>(p, q, tiles, !leader);
+    else if (q.steps > 2) scale_warps<2, PAIR>(p, q, tiles, !leader);
+    else scale_warps<1, PAIR>(p, q, tiles, !leader);
     __syncwarp();
   } else {
     // =========================== read-out ===========================
@@ -601,7 +633,7 @@ cudaError_t launch_fp4(const Fp4Params& p, Fp4Tiles q, long long most_units, con
   q.table_bytes = static_cast<uint32_t>((p.E + 1) * 4 + 15) & ~15u;
   const size_t before = (kFp4Header + 2 * q.table_bytes + 1023u) & ~static_cast<size_t>(1023);
   const size_t stage = kATile + static_cast<size_t>(PAIR ? q.BN / 2 : q.BN) * 128;
-  const size_t fixed = before + 2 * kChunkBytes + kReadWarps * kReadArea;
+  const size_t fixed = before + kScaleRing * kChunkBytes + (std::is_same<OutT, Fp4Out>::value ? 0 : kReadWarps * kReadArea);
   q.stages = static_cast<int>((kFp4Smem - fixed) / stage);
   if (q.stages > kMaxStages) q.stages = kMaxStages;
   cudaError_t err = ensure_smem_optin<fp4_rows_kernel<OutT, PAIR>>(static_cast<int>(kFp4Smem));
