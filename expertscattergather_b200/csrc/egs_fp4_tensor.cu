@@ -405,10 +405,10 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
         for (int ks = 0; ks < q.steps; ++ks) {
           const int part = ks % kChunkSteps;
           if (part == 0) {
-            alive = mbar_wait_all<PAIR>(smem_u32(&hdr->scale_full[chunk.slot]), chunk.round & 1, abort_flag, p.status.word);
+            alive = mbar_wait_all(smem_u32(&hdr->scale_full[chunk.slot]), chunk.round & 1, abort_flag, p.status.word);
             if (!alive) break;
           }
-          alive = mbar_wait_all<PAIR>(smem_u32(&hdr->full[at.slot]), at.round & 1, abort_flag, p.status.word);
+          alive = mbar_wait_all(smem_u32(&hdr->full[at.slot]), at.round & 1, abort_flag, p.status.word);
           if (!alive) break;
           const uint32_t empty = smem_u32(&hdr->empty[at.slot]), scale_empty = smem_u32(&hdr->scale_empty[chunk.slot]);
           const uint32_t addr = (ring0 + static_cast<uint32_t>(at.slot) * stage_bytes) >> 4;
