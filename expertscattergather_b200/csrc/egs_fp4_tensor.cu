@@ -14,6 +14,8 @@
 // need the scales of all columns.  What the second one's warps have stored is made visible to its tensor core by their proxy fence; their
 // arrival at the leader's barrier says no more than that this has happened, and a release of everything at cluster scope, which waits behind a memory
 // barrier, made the kernel wait for it (8192 x 4096 -> 4096: 94 us for 74; word by word with cp.async 106; no scales at all 61, no products 47).
+#include <cstddef>
+
 #include "egs_fp4.cuh"
 #include "egs_tcgen05.cuh"
 
@@ -75,32 +77,42 @@ __device__ __forceinline__ void load_rows4(uint32_t dst, const void* map, int x,
         : "memory");
 }
 
-// 512 bytes of scales to four columns of tensor memory, for all four groups of lanes
-template <bool PAIR>
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-// Four contraction steps of 64 elements; scales of the first two at sa, sb, of the others four (eight) columns on.
-#define EGS_FP4_X4(GROUP)                                                                                           \
+// A step: its scales to tensor memory (512 bytes to four columns of all four groups of lanes: those of the rows at sa, of the columns at sa + 8, the second half of the step's
+// four and eight columns on), then four contraction steps of 64 elements.  One block of PTX: the warp's own instructions between them cost more than they.
+#define EGS_FP4_STEP(GROUP, WIDE)                                                                                   \
   asm volatile(                                                                                                     \
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t.reg .b32 i, s, t;\n\t"                                          \
-      "setp.ne.b32 p, %6, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"                                                           \
-      "or.b32 i, %3, 0x40000020;\n\tadd.u32 s, %4, 4;\n\tadd.u32 t, %5, 8;\n\t"                                     \
-      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"  \
-      "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 2;\n\t"                                                                  \
-      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, i, [%4], [%5], q;\n\t"     \
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t"                                                                    \
-      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [s], [t], q;\n\t"      \
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t"                                                                    \
-      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, i, [s], [t], q;\n\t}"      \
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                          \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t.reg .b32 i, s, t, u, v;\n\t"                                     \
+      "add.u32 s, %4, 4;\n\tadd.u32 t, %4, 8;\n\tadd.u32 u, %4, 16;\n\tadd.u32 v, %4, 12;\n\t"                       \
+      "add.u64 a, %5, 32;\n\tadd.u64 b, %6, 64;\n\t"                                                               \
+      "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%4], %5;\n\t"                                                \
+      "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [s], a;\n\t"                                                  \
+      "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [t], %6;\n\t"                                                 \
+      "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [u], b;\n\t" WIDE                                             \
+      "setp.ne.b32 p, %7, 0;\n\tsetp.eq.b32 q, 0, 0;\n\tor.b32 i, %3, 0x40000020;\n\t"                              \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [t], p;\n\t"   \
+      "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 2;\n\t"                                                                 \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, i, [%4], [t], q;\n\t"      \
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t"                                                                   \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [s], [u], q;\n\t"      \
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t"                                                                   \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, i, [s], [u], q;\n\t}"      \
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa), "l"(from_a), "l"(from_b), "r"(accumulate)         \
       : "memory")
+// (more than 128 columns: another 512 bytes for each half)
+#define EGS_FP4_WIDE(GROUP)                                            \
+  "add.u64 a, %6, 32;\n\tadd.u64 b, %6, 96;\n\t"                      \
+  "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [v], a;\n\t"         \
+  "add.u32 v, %4, 20;\n\t"                                            \
+  "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [v], b;\n\t"
 template <bool PAIR>
-__device__ __forceinline__ void umma_fp4_x4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  if (PAIR) EGS_FP4_X4("2");
-  else EGS_FP4_X4("1");
+__device__ __forceinline__ void step_fp4(bool wide, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sa, uint64_t from_a, uint64_t from_b, uint32_t accumulate) {
+  if (wide) {
+    if (PAIR) EGS_FP4_STEP("2", EGS_FP4_WIDE("2"));
+    else EGS_FP4_STEP("1", EGS_FP4_WIDE("1"));
+  } else {
+    if (PAIR) EGS_FP4_STEP("2", "");
+    else EGS_FP4_STEP("1", "");
+  }
 }
 
 struct RingCursor {
@@ -125,18 +137,14 @@ __device__ __forceinline__ int expert_of(const int* starts, int E, int block, in
   return lo;
 }
 
-// 16 bytes of a row's scales from block `b` on as words; zeros behind the row's end and for rows that are not there.
+// 16 bytes of a row's scales from block `b` on as words; zeros behind the row's end (whose 16 bytes may be read to their end) and for rows that are not there.
 __device__ __forceinline__ void load_scales(const uint8_t* row, int b, int blocks, uint32_t (&w)[4]) {
-  if (row && b + 16 <= blocks) {
-    const uint4 x = *reinterpret_cast<const uint4*>(row + b);
-    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-  } else {
+  const uint4 x = row && b < blocks ? *reinterpret_cast<const uint4*>(row + b) : make_uint4(0u, 0u, 0u, 0u);
+  w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  if (b + 16 > blocks) {
+    const int left = 8 * (blocks - b);               // bits
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = 0u;
-      for (int j = 0; j < 4; ++j)
-        if (row && b + 4 * i + j < blocks) w[i] |= static_cast<uint32_t>(row[b + 4 * i + j]) << (8 * j);
-    }
+    for (int i = 0; i < 4; ++i) w[i] &= left >= 32 * (i + 1) ? 0xffffffffu : left > 32 * i ? (1u << (left - 32 * i)) - 1u : 0u;
   }
 }
 
@@ -387,13 +395,20 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
   } else if (warp == kIssueWarp) {
     // =========================== MMA issuer ===========================
     if (leader) {
-      const uint64_t a_desc = make_smem_desc(0u, 16u, 1024u), b_desc = a_desc + (kATile >> 4), s_desc = make_smem_desc(0u, 16u, 128u, 0u);
+      const uint64_t a_desc = make_smem_desc(0u, 16u, 1024u), s_desc = make_smem_desc(0u, 16u, 128u, 0u);
       // E2M1 operands (format 1), scales as powers of two, K-major; places of the scales' bytes come with the MMAs
       const uint32_t idesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(q.BN >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(kBlock >> 4) << 24);
       const bool wide = q.BN > 128;
+      // What a step needs moves on by additions: multiplications and remainders between two steps' MMAs left the tensor cores waiting.
       int t = 0;
       RingCursor chunk;
       uint32_t parity = 0u;
+      const uint32_t sa0 = tmem_base + scale_cols;
+      const uint64_t b_far = static_cast<uint64_t>(kATile >> 4), stage_units = static_cast<uint64_t>(stage_bytes >> 4);
+      const uint64_t a_first = a_desc + (ring0 >> 4);
+      uint64_t a_now = a_first;
+      uint32_t full = smem_u32(&hdr->full[0]);
+      constexpr uint32_t kEmptyFar = static_cast<uint32_t>(offsetof(Fp4Header, empty) - offsetof(Fp4Header, full));
       for (int round = 0, u; (u = unit_of(round)) < units && alive; ++round) {
         const int buf = t & 1;
         if (t >= 2) {
@@ -402,36 +417,35 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
         }
         ++t;
         const uint32_t d = tmem_base + static_cast<uint32_t>(buf) * acc_cols;
-        for (int ks = 0; ks < q.steps; ++ks) {
-          const int part = ks % kChunkSteps;
-          if (part == 0) {
-            alive = mbar_wait_all(smem_u32(&hdr->scale_full[chunk.slot]), chunk.round & 1, abort_flag, p.status.word);
+        for (int ks = 0; ks < q.steps && alive;) {
+          const uint32_t scale_full = smem_u32(&hdr->scale_full[chunk.slot]), scale_empty = smem_u32(&hdr->scale_empty[chunk.slot]);
+          const uint32_t scales = (scales0 + static_cast<uint32_t>(chunk.slot) * kChunkBytes) >> 4;
+          uint64_t from_a = s_desc + scales, from_b = s_desc + scales + (kChunkA >> 4);
+          alive = mbar_wait_all(scale_full, chunk.round & 1, abort_flag, p.status.word);
+          const int end = min(q.steps, ks + kChunkSteps);
+          for (; ks < end && alive; ++ks) {
+            alive = mbar_wait_all(full, at.round & 1, abort_flag, p.status.word);
             if (!alive) break;
+            tc_fence_after();
+            if (elect_one()) {
+              step_fp4<PAIR>(wide, d, a_now, a_now + b_far, idesc, sa0 + parity, from_a, from_b, ks > 0 ? 1u : 0u);
+              umma_done<PAIR>(full + kEmptyFar);
+              if (ks + 1 == end) umma_done<PAIR>(scale_empty);
+              if (ks + 1 == q.steps) umma_done<PAIR>(smem_u32(&hdr->acc_full[buf]));
+            }
+            parity ^= kScaleCols;
+            from_a += 2u * kAtom >> 4;
+            from_b += 4u * kAtom >> 4;
+            a_now += stage_units;
+            full += 8u;
+            if (++at.slot == q.stages) {
+              at.slot = 0;
+              ++at.round;
+              a_now = a_first;
+              full = smem_u32(&hdr->full[0]);
+            }
           }
-          alive = mbar_wait_all(smem_u32(&hdr->full[at.slot]), at.round & 1, abort_flag, p.status.word);
-          if (!alive) break;
-          const uint32_t empty = smem_u32(&hdr->empty[at.slot]), scale_empty = smem_u32(&hdr->scale_empty[chunk.slot]);
-          const uint32_t addr = (ring0 + static_cast<uint32_t>(at.slot) * stage_bytes) >> 4;
-          const uint32_t scales = scales0 + static_cast<uint32_t>(chunk.slot) * kChunkBytes + static_cast<uint32_t>(part) * 2u * kAtom;
-          const uint32_t sa = tmem_base + scale_cols + parity * kScaleCols, sb = sa + 8u;
-          const bool last = ks + 1 == q.steps, last_of_chunk = last || part + 1 == kChunkSteps;
-          at.next(q.stages);
-          parity ^= 1u;
-          if (last_of_chunk) chunk.next(kScaleRing);
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t from_a = s_desc + (scales >> 4), from_b = s_desc + ((scales + kChunkA + static_cast<uint32_t>(part) * 2u * kAtom) >> 4);
-            copy_scales<PAIR>(sa, from_a);
-            copy_scales<PAIR>(sa + 4u, from_a + (kAtom >> 4));
-            copy_scales<PAIR>(sb, from_b);
-            if (wide) copy_scales<PAIR>(sb + 4u, from_b + (kAtom >> 4));
-            copy_scales<PAIR>(sb + 8u, from_b + (2u * kAtom >> 4));
-            if (wide) copy_scales<PAIR>(sb + 12u, from_b + (3u * kAtom >> 4));
-            umma_fp4_x4<PAIR>(d, a_desc + addr, b_desc + addr, idesc, sa, sb, ks > 0 ? 1u : 0u);
-            umma_done<PAIR>(empty);
-            if (last_of_chunk) umma_done<PAIR>(scale_empty);
-            if (last) umma_done<PAIR>(smem_u32(&hdr->acc_full[buf]));
-          }
+          chunk.next(kScaleRing);
         }
       }
     }
@@ -488,36 +502,31 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
       };
       if constexpr (kFp4Out) {
         // a lane has a row's 32 columns: a block
-        for (int c = share * 64; c < bn; c += 128) {
+        for (int c = share * 32; c < bn; c += 64) {
+          uint32_t v[32];
+          tmem_ld32(acc + static_cast<uint32_t>(c), v);
+          tmem_ld_wait();
+          if (c + 64 >= bn) release();
+          uint32_t top = 0u;
+          if (p.act == EGS_ACT_SILU) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int col = c + h * 32;
-            if (col >= bn) break;
-            uint32_t v[32];
-            tmem_ld32(acc + static_cast<uint32_t>(col), v);
-            tmem_ld_wait();
-            if (col + 32 >= bn || (h == 1 && c + 128 >= bn)) release();
-            uint32_t top = 0u;
-            if (p.act == EGS_ACT_SILU) {
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(silu_fast(__uint_as_float(v[i])));
+          }
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(silu_fast(__uint_as_float(v[i])));
-            }
+          for (int i = 0; i < 32; ++i) top = max(top, v[i] & 0x7fffffffu);
+          const uint32_t byte = fp4_scale(top);
+          const float inverse = fp4_inverse(byte);
+          uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = max(top, v[i] & 0x7fffffffu);
-            const uint32_t byte = fp4_scale(top);
-            const float inverse = fp4_inverse(byte);
-            uint32_t w[4];
+          for (int i = 0; i < 4; ++i) {
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float x[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = fp4_scaled(__uint_as_float(v[8 * i + j]), inverse);
-              w[i] = fp4_pack8(x);
-            }
-            if (lane < rows) {
-              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.Out) + (row0 + lane) * p.y_row + (n0 + col) / 2) = make_uint4(w[0], w[1], w[2], w[3]);
-              p.OutScale[(row0 + lane) * p.ys_row + (n0 + col) / kFp4Block] = static_cast<uint8_t>(byte);
-            }
+            for (int j = 0; j < 8; ++j) x[j] = fp4_scaled(__uint_as_float(v[8 * i + j]), inverse);
+            w[i] = fp4_pack8(x);
+          }
+          if (lane < rows) {
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.Out) + (row0 + lane) * p.y_row + (n0 + c) / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+            p.OutScale[(row0 + lane) * p.ys_row + (n0 + c) / kFp4Block] = static_cast<uint8_t>(byte);
           }
         }
       } else if constexpr (sizeof(OutT) == 2) {

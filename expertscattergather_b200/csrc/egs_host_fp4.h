@@ -40,7 +40,17 @@ Given4 given_rows4(const Tensor& q, const Tensor& scale, const char* name) {
       scale.size(-1) != (q.size(-1) + 15) / 16)
     value_error(std::string(name) + " in 4 bits are [..., C / 2] with scales [..., ceil(C / 32)], got " + shape_of(q) + " and " + shape_of(scale));
   if (q.scalar_type() != at::kByte || scale.scalar_type() != at::kByte) value_error(std::string(name) + " in 4 bits and their scales must be uint8");
-  return {rows8_of(q), rows8_of(scale), 2 * q.size(-1), rows_ahead(q)};
+  Given4 g{rows8_of(q), rows8_of(scale), 2 * q.size(-1), rows_ahead(q)};
+  // the products read a row's scales 16 bytes at a time, to the end of the last of them
+  const Tensor& s = g.scale.t;
+  if (s.data_ptr() == scale.data_ptr() && g.rows > 0 &&
+      static_cast<size_t>(s.storage_offset() + (g.rows - 1) * g.scale.pitch + up16(s.size(-1))) > s.storage().nbytes()) {
+    auto shape = scale.sizes().vec();
+    shape.back() = g.scale.pitch = up16(scale.size(-1));
+    g.scale.t = at::empty(shape, scale.options());
+    g.scale.t.narrow(-1, 0, scale.size(-1)).copy_(scale);
+  }
+  return g;
 }
 const uint8_t* bytes_of(const Rows8& r) { return static_cast<const uint8_t*>(ptr(r.t)); }
 

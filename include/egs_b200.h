@@ -397,7 +397,8 @@ int egs_expert_matmul_int8(const int8_t* q, const float* q_scale, int64_t q_stri
  *
  * A row is blocks of 32 values of one sign, two exponent and one mantissa bit (magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the first in the
  * lower half, and a byte s for each block: its values count times 2^(s - 127), and 255 means that they are no numbers.
- * Rows begin on 16 bytes and so do their scales: bases and strides (in bytes) are multiples of 16.
+ * Rows begin on 16 bytes and so do their scales: bases and strides (in bytes) are multiples of 16.  The products read a row's scales up to a multiple
+ * of 16 bytes, the last row's too, and make nothing of those behind its end.
  * ------------------------------------------------------------------------------------------------ */
 enum { EGS_ACT_NONE = 0, EGS_ACT_SILU = 1 /* x / (1 + exp(-x)) */ };
 
