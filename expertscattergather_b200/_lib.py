@@ -145,7 +145,7 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("egs_expert_matmul_fp4_rows", i, [vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, i64, i64, ragged, i, i, i, vp, sz, vp, vp]),
             ("egs_expert_matmul_fp4_rows_workspace_bytes", sz, [ragged, i]),
             ("egs_routed_experts_few", i, [vp] * 8 + [route, i64, i64, i64, i, vp, sz, vp]),
-            ("egs_routed_experts_few_fp4", i, [vp, vp, vp, vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, route, i64, i64, i64, i, vp, sz, vp]),
+            ("egs_routed_experts_few_fp4", i, [vp, vp, vp, vp, vp, i64, i64, i64, i, vp, vp, i64, i64, i64, i, vp, vp, vp, route, i64, i64, i64, i, vp, sz, vp]),
             ("egs_routed_experts_few_workspace_bytes", sz, [route, i64, i64])):
         getattr(lib, name).restype = result
         getattr(lib, name).argtypes = args

@@ -168,18 +168,25 @@ int egs_routed_experts_few(const void* X, const void* router, const float* bias,
                            int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype, void* workspace,
                            size_t workspace_bytes, void* cuda_stream) {
   if (int rc = check_layer(route, I, J)) return rc;
-  const FewLayer f{X, router, bias, up, down, nullptr, nullptr, out, weights, experts, x_stride, 0, 0, 0, 0, static_cast<int>(I), static_cast<int>(J)};
+  const FewLayer f{X, router, bias, up, down, nullptr, nullptr, out, weights, experts, x_stride, 0, 0, 0, 0, static_cast<int>(I), static_cast<int>(J), 0, 0, false, false};
   return layer(f, route, dtype, workspace, workspace_bytes, cuda_stream);
 }
 
 int egs_routed_experts_few_fp4(const void* X, const void* router, const float* bias, const uint8_t* up, const uint8_t* up_scale, int64_t up_stride,
-                               int64_t us_stride, const uint8_t* down, const uint8_t* down_scale, int64_t down_stride, int64_t ds_stride, void* out,
+                               int64_t up_far, int64_t us_stride, int up_layout, const uint8_t* down, const uint8_t* down_scale, int64_t down_stride,
+                               int64_t down_far, int64_t ds_stride, int down_layout, void* out,
                                float* weights, int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype,
                                void* workspace, size_t workspace_bytes, void* cuda_stream) {
   if (int rc = check_layer(route, I, J)) return rc;
-  if (!strides_hold(up_stride, us_stride, I, false) || !strides_hold(down_stride, ds_stride, J, false)) return EGS_ERR_INVALID_ARGUMENT;
-  if (route->tokens && (!up_scale || !down_scale || !on16(up) || !on16(down))) return EGS_ERR_INVALID_ARGUMENT;
-  const FewLayer f{X, router, bias, up, down, up_scale, down_scale, out, weights, experts, x_stride, up_stride, us_stride, down_stride, ds_stride, static_cast<int>(I), static_cast<int>(J)};
+  // an expert's [N, C / 2], or [C / 2, N]
+  auto holds = [&](const uint8_t* w, int64_t stride, int64_t far, int64_t s_stride, int layout, int64_t C, int64_t N) {
+    if (layout == EGS_W_NC) return strides_hold(stride, s_stride, C, false) && far >= stride * (N - 1) + (C + 1) / 2 && far % 16 == 0 && on16(w);
+    return layout == EGS_W_CN && s_stride >= (C + 31) / 32 && stride >= N && far >= stride * ((C + 1) / 2 - 1) + N;
+  };
+  if (!holds(up, up_stride, up_far, us_stride, up_layout, I, J) || !holds(down, down_stride, down_far, ds_stride, down_layout, J, I)) return EGS_ERR_INVALID_ARGUMENT;
+  if (route->tokens && (!up_scale || !down_scale)) return EGS_ERR_INVALID_ARGUMENT;
+  const FewLayer f{X, router, bias, up, down, up_scale, down_scale, out, weights, experts, x_stride, up_stride, us_stride, down_stride, ds_stride, static_cast<int>(I), static_cast<int>(J),
+                   up_far, down_far, up_layout == EGS_W_CN, down_layout == EGS_W_CN};
   return layer(f, route, dtype, workspace, workspace_bytes, cuda_stream);
 }
 

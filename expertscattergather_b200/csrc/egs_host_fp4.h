@@ -142,6 +142,25 @@ std::tuple<Tensor, Tensor> matmul_fp4_rows(const Tensor& q, const Tensor& q_scal
   return {y.q, y.scale};
 }
 
+// An expert's weights in 4 bits for the layer below, [E, N, C / 2] with the bytes of a channel or those of all channels together; others are copied.
+struct Matrices4 {
+  Tensor q;
+  Rows8 scale;
+  int64_t stride, far;
+  int layout;
+  const uint8_t* bytes() const { return static_cast<const uint8_t*>(ptr(q)); }
+};
+Matrices4 matrices4(const Tensor& q, const Tensor& scale) {
+  if (q.scalar_type() == at::kByte && q.size(2) > 1 && q.size(1) > 1 && q.stride(1) == 1 && q.stride(2) >= q.size(1) &&
+      q.stride(0) >= q.stride(2) * (q.size(2) - 1) + q.size(1)) {
+    if (scale.dim() != 3 || scale.scalar_type() != at::kByte || scale.size(0) != q.size(0) || scale.size(1) != q.size(1) || scale.size(2) != (q.size(2) + 15) / 16)
+      value_error("weights in 4 bits are [E, N, C / 2] with scales [E, N, ceil(C / 32)], got " + shape_of(q) + " and " + shape_of(scale));
+    return {q, rows8_of(scale), q.stride(2), q.stride(0), EGS_W_CN};
+  }
+  const Given4 g = given_rows4(q, scale, "weights");
+  return {g.q.t, g.scale, g.q.pitch, g.q.pitch * q.size(1), EGS_W_NC};
+}
+
 // The whole layer for a few tokens; up_scale and down_scale given: weights in 4 bits.
 std::tuple<Tensor, Tensor, Tensor> routed_experts_few(const Tensor& x, const Tensor& router, const Tensor& up, const Tensor& down, int64_t k, const OptTensor& bias,
                                                       const OptTensor& up_scale, const OptTensor& down_scale, const std::string& score, int64_t groups,
@@ -185,10 +204,10 @@ std::tuple<Tensor, Tensor, Tensor> routed_experts_few(const Tensor& x, const Ten
   if (fp4) {
     for (const Tensor* t : {&*up_scale, &*down_scale})
       if (!t->is_cuda() || t->get_device() != c.idx) throw std::runtime_error("all tensors must be on the same CUDA device");
-    const Given4 u = given_rows4(up, *up_scale, "weights"), d = given_rows4(down, *down_scale, "weights");
-    check(api.egs_routed_experts_few_fp4(ptr(r.t), ptr(w), static_cast<const float*>(ptr(b)), bytes_of(u.q), bytes_of(u.scale), u.q.pitch, u.scale.pitch, bytes_of(d.q),
-                                         bytes_of(d.scale), d.q.pitch, d.scale.pitch, ptr(out), weights.data_ptr<float>(), experts.data_ptr<int>(), &spec, I, J, r.stride, dt,
-                                         ptr(ws), bytes, c.stream),
+    const Matrices4 u = matrices4(up, *up_scale), d = matrices4(down, *down_scale);
+    check(api.egs_routed_experts_few_fp4(ptr(r.t), ptr(w), static_cast<const float*>(ptr(b)), u.bytes(), bytes_of(u.scale), u.stride, u.far, u.scale.pitch, u.layout, d.bytes(),
+                                         bytes_of(d.scale), d.stride, d.far, d.scale.pitch, d.layout, ptr(out), weights.data_ptr<float>(), experts.data_ptr<int>(), &spec, I, J,
+                                         r.stride, dt, ptr(ws), bytes, c.stream),
           "egs_routed_experts_few_fp4");
   } else {
     const Tensor u = whole(up), d = whole(down);

@@ -371,6 +371,8 @@ struct FewLayer {
   int* experts;
   long long x_row, up_row, us_row, down_row, ds_row;
   int I, J;
+  long long up_far, down_far;  // bytes from one expert to the next
+  bool up_cn, down_cn;         // bytes lie along the columns: [E, I / 2, J] and [E, J / 2, I]
 };
 size_t few_layer_workspace(const egs_route& r, long long J);
 cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st);

@@ -1,9 +1,10 @@
 // A whole routed layer for a few tokens: out[t] = sum over j of w[t, j] silu(x[t] up[e]) down[e], e the j-th expert that token t chose.  Its work is
 // reading the weights of the experts that were chosen, each of them once, with all SMs.
 //
-//   logits   a warp has an expert's row of the router and all tokens
-//   choice   egs_choice.cu's kernel
-//   up       units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round the CTAs; float32 sums of parts
+//   logits   a warp has an expert's row of the router and the tokens in fours: in `up`, by each cluster of CTAs for itself, where tokens and router are few
+//            and small, else by a kernel of its own
+//   up       every CTA makes the choice for itself; units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round
+//            the CTAs; float32 sums of parts.  The other product's weights are brought to the L2 meanwhile.
 //   down     a cluster has a tile of the output's columns, its CTAs the contraction in parts; warps have the experts' tokens in turn.  The parts' sums
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
 //            CTAs' in theirs: the same bits in every run.
@@ -16,12 +17,16 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMost = EGS_MAX_FEW_SLOTS, kRows = 4;      // slots; tokens that share a read of the weights
 constexpr int kUpThreads = 256, kUpWarps = kUpThreads / 32, kUpGrid = 296, kUpPart = 1024;
+constexpr int kUpCluster = 4;                // CTAs that form logits together (two SMs: clusters of eight leave SMs of a processing cluster without any)
 constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
 constexpr int kMostParts = 8;
+constexpr int kFixedRows = 128, kFixedRows4 = 512;       // of a unit, in rows of its tile: 16 KB of weights
 
+struct LayerList;
 struct LayerParams {
   const void* X;
   const void* router;
+  const float* bias;
   const void* up;            // [E, I, J], in 4 bits [E, J, I / 2]
   const void* down;          // [E, J, I], in 4 bits [E, I, J / 2]
   const uint8_t* up_scale;
@@ -31,13 +36,23 @@ struct LayerParams {
   int* experts;
   float* logits;
   float* h;                  // [parts][tokens * k][J]
+  LayerList* list;    // what `up` has found out
   long long x_row, up_row, us_row, down_row, ds_row;       // elements; in 4 bits bytes
+  long long up_far;          // in 4 bits: bytes from one expert of `up` to the next
   int tokens, E, k, I, J;
+  int groups, top_groups, group_top, sigmoid, renormalize;
+  float scale;
+  int own_logits;            // `up` forms them
+  int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
+  long long down_far;        // bytes from one expert of `down` to the next
+  int down_bytes;            // ... of one, to bring to the L2 ahead; 0: not
+  int pieces;                // ... in so many pieces
   int act_floats;            // down: room for activations
+  Div by_pieces, by_tiles, by_k, by_E4;
 };
 
 // An expert's tokens, up to four at a time.
-struct Item {
+struct alignas(16) Item {
   int expert, rows;
   short slot[kRows];
 };
@@ -45,59 +60,57 @@ struct Items {
   Item item[kMost];
   int ids[kMost];
   unsigned tokens[EGS_MAX_EXPERTS];
+  int first[EGS_MAX_EXPERTS];    // an expert's first item
   int count;
 };
-// From the chosen experts; by all threads.
+struct LayerList {
+  int count, parts;              // items, parts that sums of `up` are in
+  int pad[2];
+  Item item[kMost];
+};
+// From the chosen experts (s->ids); by all threads, which have synchronised behind the ids and s->tokens = 0.
 __device__ __forceinline__ void list_items(const LayerParams& p, Items* s) {
   const int tid = threadIdx.x, n = p.tokens * p.k;
-  for (int e = tid; e < p.E; e += blockDim.x) s->tokens[e] = 0u;
-  __syncthreads();
-  for (int i = tid; i < n; i += blockDim.x) {
-    const int e = p.experts[i];
-    s->ids[i] = e;
-    atomicOr(&s->tokens[e], 1u << (i / p.k));
-  }
+  for (int i = tid; i < n; i += blockDim.x) atomicOr(&s->tokens[s->ids[i]], 1u << p.by_k.quotient(i));
   __syncthreads();
   if (tid < 32) {
     int before = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + tid;
-      unsigned mask = e < p.E ? s->tokens[e] : 0u;
-      const int own = (__popc(mask) + kRows - 1) / kRows;
-      int at = own;
+      const int e = e0 + tid, own = e < p.E ? (__popc(s->tokens[e]) + kRows - 1) / kRows : 0;
+      int at = before;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(kAll, at, o);
-        if (tid >= o) at += v;
+      for (int bit = 0; bit < 4; ++bit) {        // (eight items at most)
+        const unsigned has = __ballot_sync(kAll, own >> bit & 1);
+        at += __popc(has & ((1u << tid) - 1u)) << bit;
+        before += __popc(has) << bit;
       }
-      const int total = __shfl_sync(kAll, at, 31);
-      at += before - own;
-      before += total;
-      for (int i = 0; i < own; ++i) {
-        Item& x = s->item[at + i];
-        x.expert = e;
-        x.rows = min(kRows, __popc(mask));
-        for (int r = 0; r < x.rows; ++r) {
-          const int t = __ffs(mask) - 1;
-          mask &= mask - 1;
-          int j = 0;
-          while (j < p.k - 1 && s->ids[t * p.k + j] != e) ++j;
-          x.slot[r] = static_cast<short>(t * p.k + j);
-        }
-        for (int r = x.rows; r < kRows; ++r) x.slot[r] = x.slot[0];
-      }
+      if (e < p.E) s->first[e] = at;
     }
     if (tid == 0) s->count = before;
   }
   __syncthreads();
+  for (int i = tid; i < n; i += blockDim.x) {
+    const int e = s->ids[i];
+    const unsigned tokens = s->tokens[e];
+    const int place = __popc(tokens & ((1u << p.by_k.quotient(i)) - 1u)), rows = min(kRows, __popc(tokens) - place / kRows * kRows);
+    Item& x = s->item[s->first[e] + place / kRows];
+    x.slot[place % kRows] = static_cast<short>(i);
+    if (place % kRows == 0) {
+      x.expert = e;
+      x.rows = rows;
+      for (int r = rows; r < kRows; ++r) x.slot[r] = static_cast<short>(i);
+    }
+  }
+  __syncthreads();
 }
 
-// Parts that the contraction of `up` is cut into: the fewest rounds of the CTAs, a unit costing as much as 128 rows beside its own.
-__device__ __forceinline__ int parts_of(int units, int length) {
+// Parts that the contraction of `up` is cut into: the fewest rounds of the CTAs, a unit costing as much as `fixed` rows beside its own.
+__device__ __forceinline__ int parts_of(int units, int length, int fixed) {
   int best = 1, least = 0x7fffffff;
-  for (int s = 1; s <= kMostParts && (s == 1 || length / s >= 64); s *= 2) {
-    const int cost = (units * s + kUpGrid - 1) / kUpGrid * ((length + s - 1) / s + 128);
-    if (cost < least) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = 1 << i, cost = (units * s + kUpGrid - 1) / kUpGrid * (((length + s - 1) >> i) + fixed);
+    if (cost < least && (i == 0 || length >> i >= 64)) {
       least = cost;
       best = s;
     }
@@ -105,39 +118,292 @@ __device__ __forceinline__ int parts_of(int units, int length) {
   return best;
 }
 
-// ---- logits ---------------------------------------------------------------------------------------------------------
-template <typename T, int V>
-__global__ void __launch_bounds__(256) few_logits_kernel(const __grid_constant__ LayerParams p) {
-  using P = Packed<T, V>;
-  pdl_wait();
-  pdl_trigger();
-  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t0 = blockIdx.y * kRows;
-  if (e >= p.E) return;
-  const T* w = static_cast<const T*>(p.router) + static_cast<long long>(e) * p.I;
-  const T* x[kRows];
-  float acc[kRows];
+// ---- the choice -------------------------------------------------------------------------------------------------------
+// Floats as unsigned numbers of the same order; NaN lies below everything and above 0, which stands for "no candidate".
+__device__ __forceinline__ uint32_t ordered(float x) {
+  x += 0.f;                                    // -0 and 0 are equal
+  const uint32_t b = __float_as_uint(x);
+  return x != x ? 1u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return k <= 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int m = 0; m < kRows; ++m) {
-    x[m] = static_cast<const T*>(p.X) + min(t0 + m, p.tokens - 1) * p.x_row;
-    acc[m] = 0.f;
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+
+// The choice as route_tokens_kernel defines it.  A warp forms a token's keys; logits, keys: shared memory.
+struct Softmax {
+  float m, total;
+};
+__device__ __forceinline__ float score_of(const LayerParams& p, const Softmax& soft, float x) {
+  return p.sigmoid ? 1.f / (1.f + expf(-x)) : soft.m == -INFINITY ? 0.f : expf(x - soft.m) / soft.total;
+}
+__device__ __forceinline__ Softmax form_keys(const LayerParams& p, const float* logits, uint32_t* keys, int E4) {
+  const int lane = threadIdx.x & 31;
+  const bool pairs = p.groups > 1 && p.group_top == 2, scores = p.bias || pairs;
+  Softmax soft{0.f, 1.f};
+  if (!p.sigmoid && (scores || !p.renormalize)) {
+    soft.m = -INFINITY;
+    for (int e = lane; e < p.E; e += 32) soft.m = fmaxf(soft.m, logits[e]);
+    soft.m = warp_max(soft.m);
+    soft.total = 0.f;
+    for (int e = lane; e < p.E; e += 32) soft.total += soft.m == -INFINITY ? 0.f : expf(logits[e] - soft.m);
+    soft.total = warp_sum(soft.total);
   }
-#pragma unroll 4
-  for (int i = lane; i < p.I / V; i += 32) {
-    const P a = reinterpret_cast<const P*>(w)[i];
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      const P b = reinterpret_cast<const P*>(x[m])[i];
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[m] = fmaf(a.get(v), b.get(v), acc[m]);
+  for (int e = lane; e < E4; e += 32) {
+    const float x = e < p.E ? logits[e] : 0.f;
+    keys[e] = e >= p.E ? 0u : ordered(!scores ? x : p.bias ? score_of(p, soft, x) + p.bias[e] : score_of(p, soft, x));
+  }
+  __syncwarp();
+  if (p.groups > 1) {
+    const int per = p.E / p.groups;
+    uint32_t value = 0u;                       // of lane's group
+    if (lane < p.groups) {
+      uint32_t k1 = 0u, k2 = 0u;
+      for (int i = 0; i < per; ++i) {
+        const uint32_t v = keys[lane * per + i];
+        k2 = max(k2, min(k1, v));
+        k1 = max(k1, v);
+      }
+      value = pairs && k2 ? ordered(unordered(k1) + unordered(k2)) : k1;
     }
+    unsigned kept = 0u;
+    for (int i = 0; i < p.top_groups; ++i) {
+      const int at = __ffs(__ballot_sync(kAll, value == __reduce_max_sync(kAll, value))) - 1;
+      kept |= 1u << at;
+      if (lane == at) value = 0u;
+    }
+    __syncwarp();
+    for (int e = lane; e < p.E; e += 32) keys[e] = !(kept >> (e / per) & 1u) ? 0u : p.bias ? keys[e] : ordered(logits[e]);
+    __syncwarp();
+  }
+  return soft;
+}
+// Many experts: the k highest keys one after the other, by a warp.
+__device__ __forceinline__ void choose_in_turn(const LayerParams& p, uint32_t* keys, int* ids) {
+  const int lane = threadIdx.x & 31;
+  uint32_t best = 0u;                          // of this lane's experts
+  int who = 0;
+  auto look = [&]() {
+    best = 0u;
+    for (int e = lane; e < p.E; e += 32)
+      if (keys[e] > best) {
+        best = keys[e];
+        who = e;
+      }
+  };
+  look();
+  for (int j = 0; j < p.k; ++j) {
+    const uint32_t top = __reduce_max_sync(kAll, best);
+    const int e = __reduce_min_sync(kAll, best == top && top ? who : 0x7fffffff);
+    if (lane == j) ids[j] = e;
+    if (best == top && who == e) {
+      keys[e] = 0u;
+      look();
+    }
+  }
+}
+// Few: a thread counts the keys before its expert's (equal ones: those of lower experts).
+constexpr int kCounted = 256;
+__device__ __forceinline__ void choose_by_count(const LayerParams& p, const uint32_t* keys, int tokens, int E4, int* ids) {
+  for (int i = threadIdx.x; i < tokens * E4; i += kUpThreads) {
+    const int w = p.by_E4.quotient(i), e = i - w * E4;
+    const uint32_t* row = keys + w * E4;
+    const uint32_t key = row[e];
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < E4; j += 4) {          // (no key is 2^32 - 1, and there are zeros behind the last one)
+      const uint4 other = *reinterpret_cast<const uint4*>(row + j);
+      before += other.x + (j < e) > key;
+      before += other.y + (j + 1 < e) > key;
+      before += other.z + (j + 2 < e) > key;
+      before += other.w + (j + 3 < e) > key;
+    }
+    if (key && before < p.k) ids[w * p.k + before] = e;
+  }
+}
+// A token's weights, lane j < k has the j-th.
+__device__ __forceinline__ float weight_of(const LayerParams& p, const Softmax& soft, const float* logits, const int* ids) {
+  const int lane = threadIdx.x & 31;
+  const bool chosen = lane < p.k;
+  const float x = chosen ? logits[ids[lane]] : -INFINITY;
+  if (!p.renormalize) return score_of(p, soft, x) * p.scale;
+  const float high = p.sigmoid ? 0.f : warp_max(x);
+  const float s = !chosen ? 0.f : p.sigmoid ? score_of(p, soft, x) : high == -INFINITY ? 0.f : expf(x - high);
+  const float sum = warp_sum(s);
+  return (sum == 0.f ? 0.f : s / sum) * p.scale;
+}
+
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int cluster_size() {
+  int r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(const void* mine, int rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float of_cta(const float* mine, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(in_cta(mine, rank)) : "memory");
+  return v;
+}
+
+// Dot products of two experts' rows of the router with M tokens' rows from t0 on (the last ones' for those that are not there); all lanes have them.  Loads
+// of AHEAD steps go out together.
+template <typename T, int V, int M, int AHEAD>
+__device__ __forceinline__ void dots(const LayerParams& p, int e0, int e1, int t0, float (&acc)[2][M]) {
+  using P = Packed<T, V>;
+  const int lane = threadIdx.x & 31, n = p.I / V;
+  const P* w0 = reinterpret_cast<const P*>(static_cast<const T*>(p.router) + static_cast<long long>(e0) * p.I);
+  const P* w1 = reinterpret_cast<const P*>(static_cast<const T*>(p.router) + static_cast<long long>(min(e1, p.E - 1)) * p.I);
+  const P* x[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    x[m] = reinterpret_cast<const P*>(static_cast<const T*>(p.X) + min(t0 + m, p.tokens - 1) * p.x_row);
+    acc[0][m] = acc[1][m] = 0.f;
+  }
+  for (int i0 = lane; i0 < n; i0 += 32 * AHEAD) {
+    P a[2][AHEAD], b[M][AHEAD];
+#pragma unroll
+    for (int h = 0; h < AHEAD; ++h) {
+      const bool there = i0 + h * 32 < n;
+      a[0][h] = there ? w0[i0 + h * 32] : P{};
+      a[1][h] = there ? w1[i0 + h * 32] : P{};
+#pragma unroll
+      for (int m = 0; m < M; ++m) b[m][h] = there ? x[m][i0 + h * 32] : P{};
+    }
+#pragma unroll
+    for (int h = 0; h < AHEAD; ++h)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          acc[0][m] = fmaf(a[0][h].get(v), b[m][h].get(v), acc[0][m]);
+          acc[1][m] = fmaf(a[1][h].get(v), b[m][h].get(v), acc[1][m]);
+        }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1)
 #pragma unroll
-    for (int m = 0; m < kRows; ++m) acc[m] += __shfl_xor_sync(kAll, acc[m], o);
+    for (int m = 0; m < M; ++m) {
+      acc[0][m] += __shfl_xor_sync(kAll, acc[0][m], o);
+      acc[1][m] += __shfl_xor_sync(kAll, acc[1][m], o);
+    }
+}
+// ... by a warp for tokens from t0 to t1, in fours: emit(token, expert, logit)
+template <typename T, class Emit>
+__device__ __forceinline__ void logits_of(const LayerParams& p, int e0, int e1, int t0, int t1, Emit&& emit) {
+  constexpr int V = 16 / sizeof(T);
+  for (; t0 < t1; t0 += kRows) {
+    if (t1 - t0 == 1) {
+      float acc[2][1];
+      if (p.x_vectors) dots<T, V, 1, 8>(p, e0, e1, t0, acc);
+      else dots<T, 1, 1, 16>(p, e0, e1, t0, acc);
+      emit(t0, e0, acc[0][0]);
+      if (e1 < p.E) emit(t0, e1, acc[1][0]);
+    } else {
+      float acc[2][kRows];
+      if (p.x_vectors) dots<T, V, kRows, 2>(p, e0, e1, t0, acc);
+      else dots<T, 1, kRows, 8>(p, e0, e1, t0, acc);
 #pragma unroll
-  for (int m = 0; m < kRows; ++m)
-    if (lane == m && t0 + m < p.tokens) p.logits[(t0 + m) * p.E + e] = acc[m];
+      for (int m = 0; m < kRows; ++m)
+        if (t0 + m < t1) {
+          emit(t0 + m, e0, acc[0][m]);
+          if (e1 < p.E) emit(t0 + m, e1, acc[1][m]);
+        }
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__ LayerParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int e = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2, lane = threadIdx.x & 31, t0 = blockIdx.y * kRows;
+  if (e >= p.E) return;
+  logits_of<T>(p, e, e + 1, t0, min(p.tokens, t0 + kRows), [&](int t, int expert, float v) {
+    if (lane == 0) p.logits[t * p.E + expert] = v;
+  });
+}
+
+// What both `up` kernels begin with: logits (or those that are there), the choice, the items, the parts; the CTAs of a cluster share the logits.
+// table: 2 * 8 rows of E4 words, logits and keys.  `tiles`: of columns.
+template <typename T>
+__device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint32_t* table, int tiles, int fixed) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, E4 = p.by_E4.d;
+  float* logits = reinterpret_cast<float*>(table);
+  uint32_t* keys = table + kUpWarps * E4;
+  if (p.own_logits) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  pdl_wait();
+  pdl_trigger();
+  for (int e = tid; e < p.E; e += kUpThreads) s->tokens[e] = 0u;
+  if (p.own_logits) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // all CTAs of the cluster have begun
+    constexpr int kAll8 = kUpCluster * kUpWarps;
+    for (int e = cluster_rank() * kUpWarps + warp; e < p.E; e += 2 * kAll8)
+      logits_of<T>(p, e, e + kAll8, 0, p.tokens, [&](int t, int expert, float v) {
+        if (lane < kUpCluster) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(logits + t * E4 + expert, lane)), "f"(v) : "memory");
+      });
+    cluster_sync();
+  }
+  for (int t0 = 0; t0 < p.tokens; t0 += kUpWarps) {
+    const int t = t0 + warp, here = min(kUpWarps, p.tokens - t0);
+    float* row = logits + warp * E4;
+    Softmax soft{};
+    if (t < p.tokens) {
+      if (!p.own_logits) {
+        for (int e = lane; e < p.E; e += 32) row[e] = p.logits[t * p.E + e];
+        __syncwarp();
+      }
+      soft = form_keys(p, row, keys + warp * E4, E4);
+      if (p.E > kCounted) choose_in_turn(p, keys + warp * E4, s->ids + t * p.k);
+    }
+    __syncthreads();
+    if (p.E <= kCounted) {
+      choose_by_count(p, keys, here, E4, s->ids + t0 * p.k);
+      __syncthreads();
+    }
+    if (blockIdx.x == 0 && t < p.tokens) {
+      const float w = weight_of(p, soft, row, s->ids + t * p.k);
+      if (lane < p.k) {
+        p.weights[t * p.k + lane] = w;
+        p.experts[t * p.k + lane] = s->ids[t * p.k + lane];
+      }
+    }
+    if (t0 + kUpWarps < p.tokens) __syncthreads();
+  }
+  list_items(p, s);
+  const int parts = parts_of(s->count * tiles, p.I, fixed);
+  if (blockIdx.x == 0) {
+    for (int i = tid; i < s->count; i += kUpThreads) p.list->item[i] = s->item[i];
+    if (tid == 0) {
+      p.list->count = s->count;
+      p.list->parts = parts;
+    }
+  }
+  // the other product's weights to the L2, in pieces that go round the CTAs
+  constexpr int kPiece = 8192;
+  for (int i = blockIdx.x + tid * gridDim.x; i < s->count * p.pieces; i += kUpThreads * gridDim.x) {
+    const int which = p.by_pieces.quotient(i), from = (i - which * p.pieces) * kPiece;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char*>(p.down) + s->item[which].expert * p.down_far + from), "r"(min(kPiece, p.down_bytes - from)) : "memory");
+  }
+  return parts;
 }
 
 // ---- products along rows of the weights ([contraction, columns]) -----------------------------------------------------
@@ -215,7 +481,7 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
       __syncthreads();                         // what was in shared memory has been read
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        const T* x = static_cast<const T*>(p.X) + item.slot[m] / p.k * p.x_row;
+        const T* x = static_cast<const T*>(p.X) + p.by_k.quotient(item.slot[m]) * p.x_row;
         for (int i = tid; i < ((c1 - c0 + 3) & ~3); i += kUpThreads) s->x[m][i] = c0 + i < c1 ? to_f32<T>(x[c0 + i]) : 0.f;
       }
       __syncthreads();
@@ -242,13 +508,11 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
 template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_constant__ LayerParams p) {
   constexpr int kTile = LANES * V;
+  extern __shared__ uint32_t layer_table[];
   __shared__ UpShared<T, V, LANES> s;
-  pdl_wait();
-  pdl_trigger();
-  list_items(p, &s.items);
-  const int tiles = (p.J + kTile - 1) / kTile, all = s.items.count * tiles, parts = parts_of(all, p.I), length = ((p.I + parts - 1) / parts + 3) & ~3;
+  const int tiles = p.by_tiles.d, parts = begin_layer<T>(p, &s.items, layer_table, tiles, kFixedRows), all = s.items.count * tiles, length = ((p.I + parts - 1) / parts + 3) & ~3;
   for (int u = blockIdx.x; u < all * parts; u += gridDim.x) {
-    const int part = u / all, x = u - part * all, i = x / tiles, n0 = (x - i * tiles) * kTile, begin = min(p.I, part * length), end = min(p.I, begin + length);
+    const int part = u / all, x = u - part * all, i = p.by_tiles.quotient(x), n0 = (x - i * tiles) * kTile, begin = min(p.I, part * length), end = min(p.I, begin + length);
     const Item item = s.items.item[i];
     float* to = p.h + static_cast<long long>(part) * p.tokens * p.k * p.J;
     if (item.rows == 1) up_unit<T, V, LANES, 1>(p, &s, item, n0, begin, end, to);
@@ -256,57 +520,84 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
   }
 }
 
-// Sum of a slot's parts, activated.
-__device__ __forceinline__ float activation(const LayerParams& p, int parts, long long at) {
-  float v = p.h[at];
-  for (int s = 1; s < parts; ++s) v += p.h[at + static_cast<long long>(s) * p.tokens * p.k * p.J];
-  return v / (1.f + expf(-v));
+// What `up` has found out, and the weights, in shared memory.
+struct DownShared {
+  Item item[kMost];
+  float weights[kMost];
+  int count, parts;
+};
+__device__ __forceinline__ void begin_down(const LayerParams& p, DownShared* s) {
+  const int tid = threadIdx.x, slots = p.tokens * p.k;       // (items are no more than slots)
+  if (tid < slots) {
+    s->item[tid] = p.list->item[tid];
+    s->weights[tid] = p.weights[tid];
+  }
+  if (tid == 0) {
+    s->count = p.list->count;
+    s->parts = p.list->parts;
+  }
+  __syncthreads();
 }
 
-__device__ __forceinline__ int cluster_rank() {
-  int r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ int cluster_size() {
-  int r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float of_cta(const float* mine, int rank) {
-  uint32_t at;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
+// N neighbouring sums of a slot's parts from h[at] on (those that exist: left), activated.  All loads go out before the first sum.
+template <int N>
+__device__ __forceinline__ void activation(const LayerParams& p, int parts, long long at, int left, float (&v)[N]) {
+  const long long far = static_cast<long long>(p.tokens) * p.k * p.J;
+  float x[kMostParts][N];
+  const bool vectors = N % 4 == 0 && left >= N && p.J % 4 == 0;
+#pragma unroll
+  for (int s = 0; s < kMostParts; ++s) {
+    const float* h = p.h + at + s * far;
+    if (vectors) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        const float4 y = s < parts ? reinterpret_cast<const float4*>(h)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[s][4 * i] = y.x; x[s][4 * i + 1] = y.y; x[s][4 * i + 2] = y.z; x[s][4 * i + 3] = y.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[s][i] = s < parts && i < left ? h[i] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float sum = x[0][i];
+#pragma unroll
+    for (int s = 1; s < kMostParts; ++s) sum += x[s][i];
+    v[i] = i < left ? sum / (1.f + expf(-sum)) : 0.f;
+  }
 }
 
-// out[t, n0 + n] from the slots' products: part [shares][slots][tile]; `sums` [tokens][tile] of shared memory
-template <typename T>
-__device__ __forceinline__ void put_out(const LayerParams& p, const float* part, float* sums, int shares, int tile, int n0) {
-  const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size();
-  for (int i = threadIdx.x; i < p.tokens * tile; i += kDownThreads) {
-    const int t = i / tile, n = i - t * tile;
+// out[t, n0 + n] from the slots' products, part [shares][slots][tile].  Every CTA of a cluster has a share of the outputs, and the others hand it their
+// sums: to, room for them, [CTAs][outputs of a share] of shared memory.
+template <typename T, int TILE>
+__device__ __forceinline__ void put_out(const LayerParams& p, const float* part, float* to, int shares, int n0) {
+  const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = all / size;
+  if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all have begun
+  for (int i = threadIdx.x; i < all; i += kDownThreads) {
+    const int t = i / TILE, n = i % TILE;
     float v = 0.f;
     for (int j = 0; j < p.k; ++j)
-      for (int s = 0; s < shares; ++s) v += part[(s * slots + t * p.k + j) * tile + n];
-    sums[i] = v;
+      for (int s = 0; s < shares; ++s) v += part[(s * slots + t * p.k + j) * TILE + n];
+    if (size == 1) {
+      if (n0 + n < p.I) static_cast<T*>(p.out)[static_cast<long long>(t) * p.I + n0 + n] = from_f32<T>(v);
+    } else {
+      const int owner = i / own;
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(to + rank * own + i - owner * own, owner)), "f"(v) : "memory");
+    }
   }
+  if (size == 1) return;
   cluster_sync();
-  for (int i = threadIdx.x + rank * kDownThreads; i < p.tokens * tile; i += kDownThreads * size) {
-    const int t = i / tile, n = i - t * tile;
-    float v = of_cta(sums + i, 0);
-    for (int r = 1; r < size; ++r) v += of_cta(sums + i, r);
+  for (int i = threadIdx.x; i < own; i += kDownThreads) {
+    const int x = rank * own + i, t = x / TILE, n = x % TILE;
+    float v = to[i];
+    for (int r = 1; r < size; ++r) v += to[r * own + i];
     if (n0 + n < p.I) static_cast<T*>(p.out)[static_cast<long long>(t) * p.I + n0 + n] = from_f32<T>(v);
   }
-  cluster_sync();
 }
 
-template <typename T, int V, int LANES, int M>
-__device__ __forceinline__ void down_item(const LayerParams& p, const Item& item, const float* act, int pitch, int base, int begin, int end, int n0, float* part, bool first) {
+template <typename T, int V, int LANES, int M, class Ready>
+__device__ __forceinline__ void down_item(const LayerParams& p, const Item& item, const float* act, int pitch, int base, int begin, int end, int n0, float* part, bool first, Ready&& ready) {
   constexpr int kTile = LANES * V;
   const int lane = threadIdx.x & 31, l = lane % LANES, n = n0 + l * V;
   float acc[M][V];
@@ -317,7 +608,7 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[m][v] = 0.f;
   }
-  accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, p.down_row, begin + lane / LANES * 4, 32 / LANES * 4, end, n < p.I, a, base, []() {});
+  accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, p.down_row, begin + lane / LANES * 4, 32 / LANES * 4, end, n < p.I, a, base, ready);
   join_groups<LANES, V, M>(acc);
   if (lane < LANES) {
 #pragma unroll
@@ -336,194 +627,334 @@ template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_constant__ LayerParams p) {
   constexpr int kTile = LANES * V;
   extern __shared__ __align__(16) float layer_smem[];
-  __shared__ Items items;
+  __shared__ DownShared items;
+  if (cluster_size() > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_trigger();
-  list_items(p, &items);
+  begin_down(p, &items);
   const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5;
   const int n0 = blockIdx.x / size * kTile;
   float* act = layer_smem;
   float* part = layer_smem + p.act_floats;
-  const int up_tiles = (p.J + kTile - 1) / kTile, parts = parts_of(items.count * up_tiles, p.I);
+  const int parts = items.parts;
   const int length = ((p.J + size - 1) / size + 3) & ~3, begin = min(p.J, rank * length), end = min(p.J, begin + length);
   const int room = min(length, p.act_floats / slots & ~3);
   int shares = 1;                              // warps that have an item's contraction in turn
   while (items.count * shares * 2 <= kDownWarps && length / shares >= 64) shares *= 2;
   for (int c0 = begin; c0 == begin || c0 < end; c0 += room) {
     const int c1 = min(end, c0 + room), width = (c1 - c0 + 3) & ~3;
-    __syncthreads();
-    for (int slot = warp; slot < slots; slot += kDownWarps) {
-      const float w = p.weights[slot];
-      for (int i = tid & 31; i < width; i += 32) act[slot * room + i] = c0 + i < c1 ? w * activation(p, parts, static_cast<long long>(slot) * p.J + c0 + i) : 0.f;
-    }
-    __syncthreads();
+    // activations, four at a time; a warp's first weights are on their way meanwhile
+    bool staged = false;
+    auto stage = [&]() {
+      if (staged) return;
+      staged = true;
+      __syncthreads();
+      for (int i = tid; i < slots * (width / 4); i += kDownThreads) {
+        const int slot = i / (width / 4), c = (i - slot * (width / 4)) * 4;
+        const float w = items.weights[slot];
+        float v[4];
+        activation<4>(p, parts, static_cast<long long>(slot) * p.J + c0 + c, c1 - c0 - c, v);
+        *reinterpret_cast<float4*>(act + slot * room + c) = make_float4(w * v[0], w * v[1], w * v[2], w * v[3]);
+      }
+      __syncthreads();
+    };
     const int each = (width / 4 + shares - 1) / shares * 4;
     for (int x = warp; x < items.count * shares; x += kDownWarps) {
       const int i = x / shares, share = x - i * shares, b = min(c1, c0 + share * each), e = min(c1, b + each);
       const Item item = items.item[i];
       float* to = part + share * slots * kTile;
-      if (item.rows == 1) down_item<T, V, LANES, 1>(p, item, act, room, c0, b, e, n0, to, c0 == begin);
-      else down_item<T, V, LANES, kRows>(p, item, act, room, c0, b, e, n0, to, c0 == begin);
+      if (item.rows == 1) down_item<T, V, LANES, 1>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
+      else down_item<T, V, LANES, kRows>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
     }
+    stage();
   }
   __syncthreads();
-  put_out<T>(p, part, act, shares, kTile, n0);
+  put_out<T, kTile>(p, part, part + max(4 * kDownWarps, slots) * kTile, shares, n0);
 }
 
-// ---- products along the contraction, weights in 4 bits ([columns, contraction]) ---------------------------------------
-constexpr int kChannels = 8;                   // columns of a warp
-constexpr int kTile4 = 64;
+// ---- weights in 4 bits -------------------------------------------------------------------------------------------------
+// Four columns of an expert times M rows, a block of 32 contraction elements at a time: the weights' bytes lie along the contraction (NC, a lane has 16 of a column) or along
+// the columns (CN, a lane has four of each of 16 rows, or one where rows begin anywhere).  Twice the values are integers, so that a block's sum is exact.
+constexpr int kTile4 = 64;                     // NC: columns of a tile
+__host__ __device__ constexpr int tile4(int layout) { return layout == 0 ? kTile4 : layout == 4 ? 128 : 32; }      // layout: 0 NC, 4 or 1 CN with so many columns a lane
+constexpr int kColumns = 4;
+struct Weights4 {
+  Block4 w[kColumns];
+  uint32_t s[kColumns];
+};
+struct Matrix4 {
+  const uint8_t *w, *s;        // of an expert
+  long long row, s_row;        // NC: bytes from one column to the next, CN: from one pair of contraction elements to the next; scales: from one column to the next
+  int C, N;
+};
 
-// Eight columns of an expert from n0 on times M rows, blocks [begin, end): a[m] + b * 32: twice the rows' 4 bits as bytes, f[m] + b: their scales.  Lanes
-// go along the blocks, 4 to 32 of them; those that are left have other columns.  emit(column, row, sum) for the lanes that have the sums.
-template <int M, class Emit>
-__device__ __forceinline__ void columns4(const uint8_t* W, long long w_row, const uint8_t* S, long long s_row, int C, int N, int n0, int begin, int end, const uint8_t* const (&a)[M],
-                                         const float* const (&f)[M], int base, Emit&& emit) {
-  const int lane = threadIdx.x & 31;
-  int lanes_log2 = 2;
-  while (lanes_log2 < 5 && (1 << lanes_log2) < end - begin) ++lanes_log2;
-  const int along = lane & ((1 << lanes_log2) - 1), group = lane >> lanes_log2, groups = 32 >> lanes_log2;
-  constexpr int kAtOnce = 2;
-  for (int j0 = 0; j0 < kChannels / groups; j0 += kAtOnce) {
-    float acc[kAtOnce][M];
+// acc[j][m] += the block's products; a[m]: twice the rows' 4 bits as bytes, f[m]: a quarter of their scale.
+template <int M, int COLUMNS>
+__device__ __forceinline__ void add_block(const Weights4& x, const uint8_t* const (&a)[M], const float (&f)[M], float (&acc)[COLUMNS][M]) {
+  uint32_t y[M][8];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
+  for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int m = 0; m < M; ++m) acc[j][m] = 0.f;
-#pragma unroll 2
-    for (int b = begin + along; b < end; b += 1 << lanes_log2) {
-      Block4 w[kAtOnce];
-      uint32_t s[kAtOnce];
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const long long n = min(n0 + (j0 + j) * groups + group, N - 1);
-        w[j] = load_block(W + n * w_row, b, C);
-        s[j] = S[n * s_row + b];
-      }
-      uint32_t x[M][8];
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 y = *reinterpret_cast<const uint4*>(a[m] + (b - base) * 32 + i * 16);
-          x[m][4 * i] = y.x; x[m][4 * i + 1] = y.y; x[m][4 * i + 2] = y.z; x[m][4 * i + 3] = y.w;
-        }
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        int sum[M];
-#pragma unroll
-        for (int m = 0; m < M; ++m) sum[m] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t low, high;
-          fp4_integers(w[j].w[i], low, high);
-#pragma unroll
-          for (int m = 0; m < M; ++m) sum[m] = __dp4a(static_cast<int>(x[m][2 * i + 1]), static_cast<int>(high), __dp4a(static_cast<int>(x[m][2 * i]), static_cast<int>(low), sum[m]));
-        }
-        const float power = fp4_power(s[j]);
-#pragma unroll
-        for (int m = 0; m < M; ++m) acc[j][m] = fmaf(static_cast<float>(sum[m]) * f[m][b - base], power, acc[j][m]);
-      }
+    for (int h = 0; h < 2; ++h) {
+      const uint4 z = *reinterpret_cast<const uint4*>(a[m] + h * 16);
+      y[m][4 * h] = z.x; y[m][4 * h + 1] = z.y; y[m][4 * h + 2] = z.z; y[m][4 * h + 3] = z.w;
     }
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
+  for (int j = 0; j < COLUMNS; ++j) {
+    int sum[M];
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-        for (int o = 1; o < 1 << lanes_log2; o <<= 1) acc[j][m] += __shfl_xor_sync(kAll, acc[j][m], o);
+    for (int m = 0; m < M; ++m) sum[m] = 0;
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int c = (j0 + j) * groups + group;
-      if (j0 + j < kChannels / groups && along == 0 && n0 + c < N) {
+    for (int h = 0; h < 4; ++h) {
+      uint32_t low, high;
+      fp4_integers(x.w[j].w[h], low, high);
 #pragma unroll
-        for (int m = 0; m < M; ++m) emit(n0 + c, m, acc[j][m]);
+      for (int m = 0; m < M; ++m) sum[m] = __dp4a(static_cast<int>(y[m][2 * h + 1]), static_cast<int>(high), __dp4a(static_cast<int>(y[m][2 * h]), static_cast<int>(low), sum[m]));
+    }
+    const float power = fp4_power(x.s[j]);
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[j][m] = fmaf(static_cast<float>(sum[m]) * f[m], power, acc[j][m]);
+  }
+}
+
+// CN: a block of four columns from n on; the words of four rows become four columns' words.
+template <int V>
+__device__ __forceinline__ void load_columns(Weights4& x, const Matrix4& t, int n, int b) {
+  const bool there = n < t.N;
+  const uint8_t* from = t.w + b * 16ll * t.row + n;
+  const int rows = min(16, t.C / 2 - b * 16);
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (V == 4) r[i] = there && i < rows ? *reinterpret_cast<const uint32_t*>(from + i * t.row) : 0u;
+    else r[i] = there && i < rows ? from[i * t.row] : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) x.s[j] = n + j < t.N ? t.s[(n + j) * t.s_row + b] : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t p0 = __byte_perm(r[4 * i], r[4 * i + 1], 0x5140), p1 = __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x5140);
+    x.w[0].w[i] = __byte_perm(p0, p1, 0x5410);
+    if constexpr (V == 4) {
+      const uint32_t p2 = __byte_perm(r[4 * i], r[4 * i + 1], 0x7362), p3 = __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x7362);
+      x.w[1].w[i] = __byte_perm(p0, p1, 0x7632);
+      x.w[2].w[i] = __byte_perm(p2, p3, 0x5410);
+      x.w[3].w[i] = __byte_perm(p2, p3, 0x7632);
+    }
+  }
+}
+// Columns n .. n + V - 1 of a lane over the blocks begin, begin + step, .. below end.  `ready` is called when the first weights have been asked for.
+template <int V, int M, class Ready>
+__device__ __forceinline__ void along_columns(const Matrix4& t, int n, int begin, int step, int end, const uint8_t* const (&a)[M], const float* const (&f)[M], int base, float (&acc)[V][M], Ready&& ready) {
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[j][m] = 0.f;
+  Weights4 next;
+  if (begin < end) load_columns<V>(next, t, n, begin);
+  ready();
+  for (int b = begin; b < end; b += step) {
+    const Weights4 now = next;
+    if (b + step < end) load_columns<V>(next, t, n, b + step);
+    const uint8_t* at[M];
+    float g[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      at[m] = a[m] + (b - base) * 32;
+      g[m] = f[m][b - base];
+    }
+    add_block<M, V>(now, at, g, acc);
+  }
+}
+
+// NC: columns [n0, n0 + columns), blocks [begin, end).  Lanes go along the blocks, 4 to 32 of them; those that are left have other columns, four at a time.
+// emit(column, row, sum) by the lanes that have the sums.
+template <int M, class Ready, class Emit>
+__device__ __forceinline__ void along_rows(const Matrix4& t, int n0, int columns, int begin, int end, const uint8_t* const (&a)[M], const float* const (&f)[M], int base, Ready&& ready, Emit&& emit) {
+  int log2 = 2;
+  while (log2 < 5 && (1 << log2) < end - begin) ++log2;
+  const int lane = threadIdx.x & 31, along = lane & ((1 << log2) - 1), group = lane >> log2, groups = 32 >> log2;
+  Weights4 next;
+  auto load = [&](int first, int b) {
+#pragma unroll
+    for (int j = 0; j < kColumns; ++j) {
+      const int n = n0 + first + j * groups + group;
+      const bool there = first + j * groups < columns && n < t.N && b < end;
+      next.w[j] = there ? load_block(t.w + n * t.row, b, t.C) : Block4{};
+      next.s[j] = there ? t.s[n * t.s_row + b] : 0u;
+    }
+  };
+  int first = 0, b = begin + along;            // of the weights that come next
+  load(first, b);
+  ready();
+  while (first < columns) {
+    float acc[kColumns][M];
+#pragma unroll
+    for (int j = 0; j < kColumns; ++j)
+#pragma unroll
+      for (int m = 0; m < M; ++m) acc[j][m] = 0.f;
+    const int now_first = first;
+    for (int steps = max(1, (end - begin + (1 << log2) - 1) >> log2); steps; --steps) {
+      const Weights4 now = next;
+      const int at_block = max(min(b, end - 1) - base, 0);
+      const bool on = b < end;
+      b += 1 << log2;
+      if (steps == 1) {
+        first += kColumns * groups;
+        b = begin + along;
+      }
+      if (first < columns) load(first, b);
+      const uint8_t* at[M];
+      float g[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        at[m] = a[m] + at_block * 32;
+        g[m] = on ? f[m][at_block] : 0.f;
+      }
+      add_block<M, kColumns>(now, at, g, acc);
+    }
+    for (int o = 1; o < 1 << log2; o <<= 1)
+#pragma unroll
+      for (int j = 0; j < kColumns; ++j)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[j][m] += __shfl_xor_sync(kAll, acc[j][m], o);
+#pragma unroll
+    for (int j = 0; j < kColumns; ++j) {
+      const int c = now_first + j * groups;
+      if (along == 0 && c < columns && n0 + c + group < t.N) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) emit(n0 + c + group, m, acc[j][m]);
       }
     }
   }
 }
 
-// A block of 32 values in 4 bits, as twice their values in bytes; a quarter of its scale.
-__device__ __forceinline__ float block4(float (&v)[32], uint8_t* to) {
+// Eight of a block's 32 values by each of four neighbouring lanes, in 4 bits, as twice their values in bytes; a quarter of the block's scale.
+__device__ __forceinline__ float block4(const float (&v)[8], uint8_t* to) {
   uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(kAll, top, 1));
+  top = max(top, __shfl_xor_sync(kAll, top, 2));
   const uint32_t byte = fp4_scale(top);
   const float inverse = fp4_inverse(byte);
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = fp4_scaled(v[8 * i + j], inverse);
+  for (int i = 0; i < 8; ++i) x[i] = fp4_scaled(v[i], inverse);
+  if (to) {
     uint2 w;
     fp4_integers(fp4_pack8(x), w.x, w.y);
-    *reinterpret_cast<uint2*>(to + 8 * i) = w;
+    *reinterpret_cast<uint2*>(to) = w;
   }
   return 0.25f * fp4_power(byte);
 }
 
+constexpr int kUpBlocks = 2 * kUpPart / kFp4Block;       // blocks in shared memory at a time
+template <int LAYOUT>
 struct Up4Shared {
   Items items;
   alignas(16) uint8_t x[kRows][2 * kUpPart];
-  float f[kRows][2 * kUpPart / kFp4Block];
+  float f[kRows][kUpBlocks];
+  float sums[LAYOUT ? kUpWarps : 1][kRows][LAYOUT ? tile4(LAYOUT) : 1];
 };
 
-template <typename T, int M>
-__device__ __forceinline__ void up4_unit(const LayerParams& p, Up4Shared* s, const Item& item, int n0, int begin, int end, float* to) {
-  const int tid = threadIdx.x;
+// An item's rows of X, blocks [b0, b0 + n), into shared memory; by all threads.
+template <typename T>
+__device__ __noinline__ void stage_rows4(const LayerParams& p, const Item& item, int rows, int b0, int n, uint8_t* x, float* f) {
+  constexpr int kVec = 16 / sizeof(T);
+  __syncthreads();                             // what was in shared memory has been read
+  for (int m = 0; m < rows; ++m) {
+    const T* from = static_cast<const T*>(p.X) + p.by_k.quotient(item.slot[m]) * p.x_row;
+    for (int i0 = 0; i0 < n * 4; i0 += kUpThreads) {       // (whole warps)
+      const int i = i0 + threadIdx.x, c = b0 * 32 + i * 8;
+      const bool there = i < n * 4;
+      float v[8];
+      if (p.x_vectors && there && c + 8 <= p.I) {
+#pragma unroll
+        for (int h = 0; h < 8 / kVec; ++h) {
+          const Packed<T, kVec> y = reinterpret_cast<const Packed<T, kVec>*>(from + c)[h];
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) v[h * kVec + j] = y.get(j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = there && c + j < p.I ? to_f32<T>(from[c + j]) : 0.f;
+      }
+      const float g = block4(v, there ? x + m * (2 * kUpPart) + i * 8 : nullptr);
+      if (there && i % 4 == 0) f[m * kUpBlocks + i / 4] = g;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int LAYOUT, int M>
+__device__ __forceinline__ void up4_unit(const LayerParams& p, Up4Shared<LAYOUT>* s, const Item& item, int n0, int begin, int end, float* to) {
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const Matrix4 t{static_cast<const uint8_t*>(p.up) + item.expert * p.up_far, p.up_scale + item.expert * (p.us_row * p.J), p.up_row, p.us_row, (p.I + 1) / 2 * 2, p.J};
   const uint8_t* a[M];
   const float* f[M];
-  const T* x[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     a[m] = s->x[m];
     f[m] = s->f[m];
-    x[m] = static_cast<const T*>(p.X) + item.slot[m] / p.k * p.x_row;
   }
-  const int C = (p.I + 1) / 2 * 2, chunk = 2 * kUpPart / kFp4Block;
-  for (int b0 = begin; b0 < end; b0 += chunk) {
-    const int b1 = min(end, b0 + chunk), n = b1 - b0;
-    __syncthreads();
-    for (int i = tid; i < M * n; i += kUpThreads) {
-      const int m = i / n, b = b0 + i - m * n;
-      float v[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = b * 32 + c < p.I ? to_f32<T>(x[m][b * 32 + c]) : 0.f;
-      s->f[m][b - b0] = block4(v, s->x[m] + (b - b0) * 32);
-    }
-    __syncthreads();
+  for (int b0 = begin; b0 < end; b0 += kUpBlocks) {
+    const int b1 = min(end, b0 + kUpBlocks);
     const bool first = b0 == begin;
-    columns4<M>(static_cast<const uint8_t*>(p.up) + item.expert * (p.up_row * p.J), p.up_row, p.up_scale + item.expert * (p.us_row * p.J), p.us_row, C, p.J,
-                n0 + (tid >> 5) * kChannels, b0, b1, a, f, b0, [&](int col, int m, float v) {
-                  if (m >= item.rows) return;
-                  float* o = to + static_cast<long long>(item.slot[m]) * p.J + col;
-                  *o = first ? v : *o + v;
-                });
+    auto stage = [&]() { stage_rows4<T>(p, item, M, b0, b1 - b0, s->x[0], s->f[0]); };
+    auto put = [&](int col, int m, float v) {
+      if (m >= item.rows || col >= p.J) return;
+      float* o = to + static_cast<long long>(item.slot[m]) * p.J + col;
+      *o = first ? v : *o + v;
+    };
+    if constexpr (LAYOUT == 0) {
+      along_rows<M>(t, n0 + warp * (kTile4 / kUpWarps), kTile4 / kUpWarps, b0, b1, a, f, b0, stage, put);
+    } else {
+      constexpr int kTile = tile4(LAYOUT);
+      const int n = (tid & 31) * LAYOUT;
+      float acc[LAYOUT][M];
+      along_columns<LAYOUT, M>(t, n0 + n, b0 + warp, kUpWarps, b1, a, f, b0, acc, stage);
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int j = 0; j < LAYOUT; ++j) s->sums[warp][m][n + j] = acc[j][m];
+      __syncthreads();
+      for (int i = tid; i < M * kTile; i += kUpThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kUpWarps; ++w) v += s->sums[w][i / kTile][i % kTile];
+        put(n0 + i % kTile, i / kTile, v);
+      }
+    }
   }
 }
 
-template <typename T>
+template <typename T, int LAYOUT>
 __global__ void __launch_bounds__(kUpThreads, 2) few_up4_kernel(const __grid_constant__ LayerParams p) {
-  __shared__ Up4Shared s;
-  pdl_wait();
-  pdl_trigger();
-  list_items(p, &s.items);
-  const int tiles = (p.J + kTile4 - 1) / kTile4, all = s.items.count * tiles, parts = parts_of(all, p.I), blocks = fp4_blocks(p.I), length = (blocks + parts - 1) / parts;
+  constexpr int kTile = tile4(LAYOUT);
+  extern __shared__ uint32_t layer_table[];
+  __shared__ Up4Shared<LAYOUT> s;
+  const int tiles = p.by_tiles.d, parts = begin_layer<T>(p, &s.items, layer_table, tiles, kFixedRows4 * kTile4 / kTile), all = s.items.count * tiles, blocks = fp4_blocks(p.I), length = (blocks + parts - 1) / parts;
   for (int u = blockIdx.x; u < all * parts; u += gridDim.x) {
-    const int part = u / all, x = u - part * all, i = x / tiles, n0 = (x - i * tiles) * kTile4, begin = min(blocks, part * length), end = min(blocks, begin + length);
+    const int part = u / all, x = u - part * all, i = p.by_tiles.quotient(x), n0 = (x - i * tiles) * kTile, begin = min(blocks, part * length), end = min(blocks, begin + length);
     const Item item = s.items.item[i];
     float* to = p.h + static_cast<long long>(part) * p.tokens * p.k * p.J;
     if (begin == end) {                        // (nothing is left for the last parts of a short contraction)
-      for (int c = threadIdx.x; c < item.rows * kTile4; c += kUpThreads)
-        if (n0 + c % kTile4 < p.J) to[static_cast<long long>(item.slot[c / kTile4]) * p.J + n0 + c % kTile4] = 0.f;
+      for (int c = threadIdx.x; c < item.rows * kTile; c += kUpThreads)
+        if (n0 + c % kTile < p.J) to[static_cast<long long>(item.slot[c / kTile]) * p.J + n0 + c % kTile] = 0.f;
     } else if (item.rows == 1) {
-      up4_unit<T, 1>(p, &s, item, n0, begin, end, to);
+      up4_unit<T, LAYOUT, 1>(p, &s, item, n0, begin, end, to);
     } else {
-      up4_unit<T, kRows>(p, &s, item, n0, begin, end, to);
+      up4_unit<T, LAYOUT, kRows>(p, &s, item, n0, begin, end, to);
     }
   }
 }
 
-template <int M>
-__device__ __forceinline__ void down4_item(const LayerParams& p, const Item& item, const uint8_t* act, const float* scale, int pitch, int b0, int b1, int n0, int base_n, float* part, bool first) {
+template <int LAYOUT, int M, class Ready>
+__device__ __forceinline__ void down4_item(const LayerParams& p, const Item& item, const uint8_t* act, const float* scale, int pitch, int b0, int b1, int n0, int share, int shares, float* part,
+                                           bool first, Ready&& ready) {
+  constexpr int kTile = tile4(LAYOUT);
+  const Matrix4 t{static_cast<const uint8_t*>(p.down) + item.expert * p.down_far, p.down_scale + item.expert * (p.ds_row * p.I), p.down_row, p.ds_row, (p.J + 1) / 2 * 2, p.I};
   const uint8_t* a[M];
   const float* f[M];
 #pragma unroll
@@ -531,50 +962,78 @@ __device__ __forceinline__ void down4_item(const LayerParams& p, const Item& ite
     a[m] = act + item.slot[m] * pitch * 32;
     f[m] = scale + item.slot[m] * pitch;
   }
-  columns4<M>(static_cast<const uint8_t*>(p.down) + item.expert * (p.down_row * p.I), p.down_row, p.down_scale + item.expert * (p.ds_row * p.I), p.ds_row, (p.J + 1) / 2 * 2, p.I, n0, b0, b1, a, f,
-              b0, [&](int col, int m, float v) {
-                if (m >= item.rows) return;
-                float* o = part + item.slot[m] * kTile4 + col - base_n;
-                *o = first ? v : *o + v;
-              });
+  auto put = [&](float* row, int m, float v) {
+    if (m >= item.rows) return;
+    float* o = row + item.slot[m] * kTile;
+    *o = first ? v : *o + v;
+  };
+  if constexpr (LAYOUT == 0) {                 // (shares: of the columns)
+    const int columns = kTile / shares;
+    along_rows<M>(t, n0 + share * columns, columns, b0, b1, a, f, b0, ready, [&](int col, int m, float v) { put(part + col - n0, m, v); });
+  } else {                                     // (of the blocks)
+    const int n = (threadIdx.x & 31) * LAYOUT;
+    float acc[LAYOUT][M];
+    along_columns<LAYOUT, M>(t, n0 + n, b0 + share, shares, b1, a, f, b0, acc, ready);
+    float* row = part + share * p.tokens * p.k * kTile + n;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < LAYOUT; ++j) put(row + j, m, acc[j][m]);
+  }
 }
 
-template <typename T>
+// The activations of all slots, blocks [b0, b0 + n), in 4 bits into shared memory; by all threads.
+__device__ __noinline__ void stage_activations4(const LayerParams& p, const DownShared& items, int b0, int n, int room, uint8_t* act, float* scale) {
+  const int slots = p.tokens * p.k, tid = threadIdx.x, all = slots * n * 4;
+  __syncthreads();
+  for (int i0 = 0; i0 < all; i0 += kDownThreads) {       // (whole warps)
+    const int i = min(i0 + tid, all - 1), slot = i / (n * 4), b = i / 4 - slot * n, c = (b0 + b) * 32 + i % 4 * 8;
+    float v[8];
+    activation<8>(p, items.parts, static_cast<long long>(slot) * p.J + c, p.J - c, v);
+    const bool there = i0 + tid < all;
+    const float f = items.weights[slot] * block4(v, there ? act + (slot * room + b) * 32 + i % 4 * 8 : nullptr);
+    if (there && i % 4 == 0) scale[slot * room + b] = f;
+  }
+  __syncthreads();
+}
+
+template <typename T, int LAYOUT>
 __global__ void __launch_bounds__(kDownThreads, 1) few_down4_kernel(const __grid_constant__ LayerParams p) {
+  constexpr int kTile = tile4(LAYOUT);
   extern __shared__ __align__(16) float layer_smem[];
-  __shared__ Items items;
+  __shared__ DownShared items;
+  if (cluster_size() > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_trigger();
-  list_items(p, &items);
+  begin_down(p, &items);
   const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5;
-  const int n0 = blockIdx.x / size * kTile4;
+  const int n0 = blockIdx.x / size * kTile;
   float* part = layer_smem + p.act_floats;
-  const int up_tiles = (p.J + kTile4 - 1) / kTile4, parts = parts_of(items.count * up_tiles, p.I), blocks = fp4_blocks(p.J);
+  const int blocks = fp4_blocks(p.J);
   const int length = (blocks + size - 1) / size, begin = min(blocks, rank * length), end = min(blocks, begin + length);
   const int room = min(length, p.act_floats / (9 * slots));            // blocks: eight words of bytes and a scale
   uint8_t* act = reinterpret_cast<uint8_t*>(layer_smem);
   float* scale = layer_smem + static_cast<long long>(slots) * room * 8;
+  int shares = 1;                              // warps that have an item's columns or blocks apart
+  while (items.count * shares * 2 <= kDownWarps && shares < (LAYOUT ? length : 8)) shares *= 2;
   for (int b0 = begin; b0 == begin || b0 < end; b0 += room) {
-    const int b1 = min(end, b0 + room), n = b1 - b0;
-    __syncthreads();
-    for (int i = tid; i < slots * n; i += kDownThreads) {
-      const int slot = i / n, b = b0 + i - slot * n;
-      float v[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = b * 32 + c < p.J ? activation(p, parts, static_cast<long long>(slot) * p.J + b * 32 + c) : 0.f;
-      scale[slot * room + b - b0] = p.weights[slot] * block4(v, act + (slot * room + b - b0) * 32);
+    const int b1 = min(end, b0 + room);
+    bool staged = false;
+    auto stage = [&]() {
+      if (staged) return;
+      staged = true;
+      stage_activations4(p, items, b0, b1 - b0, room, act, scale);
+    };
+    for (int x = warp; x < items.count * shares; x += kDownWarps) {
+      const Item item = items.item[x / shares];
+      const int share = x % shares;
+      if (item.rows == 1) down4_item<LAYOUT, 1>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
+      else down4_item<LAYOUT, kRows>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
     }
-    __syncthreads();
-    constexpr int kSets = kTile4 / kChannels;
-    for (int x = warp; x < items.count * kSets; x += kDownWarps) {
-      const Item item = items.item[x / kSets];
-      const int first_n = n0 + x % kSets * kChannels;
-      if (item.rows == 1) down4_item<1>(p, item, act, scale, room, b0, b1, first_n, n0, part, b0 == begin);
-      else down4_item<kRows>(p, item, act, scale, room, b0, b1, first_n, n0, part, b0 == begin);
-    }
+    stage();
   }
   __syncthreads();
-  put_out<T>(p, part, layer_smem, 1, kTile4, n0);
+  put_out<T, kTile>(p, part, part + max(4 * kDownWarps, slots) * kTile, LAYOUT ? shares : 1, n0);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
@@ -598,10 +1057,12 @@ cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned bl
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// CTAs of a cluster: as many as leave a CTA for every SM at most, each with 32 contraction elements at least.
+// CTAs of a cluster, each with 32 contraction elements at least and an SM of its own: of the processing clusters, 16 to 20 SMs, clusters of eight and
+// of four leave some SMs unused.
 unsigned cluster_of(int tiles, int J) {
   unsigned size = 8;
-  while (size > 1 && (tiles * static_cast<int>(size) > 148 || J / static_cast<int>(size) < 32)) size /= 2;
+  auto fit = [](unsigned n) { return n == 8 ? 16 : n == 4 ? 32 : 74; };
+  while (size > 1 && (tiles > fit(size) || J / static_cast<int>(size) < 32)) size /= 2;
   return size;
 }
 
@@ -610,10 +1071,9 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   const int tiles = (p.I + tile - 1) / tile, slots = p.tokens * p.k;
   cudaError_t err = ensure_smem_optin<kernel>(static_cast<int>(kDownSmem));
   if (err != cudaSuccess) return err;
-  const size_t part = static_cast<size_t>(slots < 4 * kDownWarps ? 4 * kDownWarps : slots) * tile * sizeof(float);
   const unsigned size = cluster_of(tiles, p.J);
+  const size_t part = static_cast<size_t>((slots < 4 * kDownWarps ? 4 * kDownWarps : slots) + (size > 1 ? p.tokens : 0)) * tile * sizeof(float);
   size_t act = static_cast<size_t>(slots) * (p.J / size + 36) * sizeof(float);
-  if (act < static_cast<size_t>(p.tokens) * tile * sizeof(float)) act = static_cast<size_t>(p.tokens) * tile * sizeof(float);
   act = (act + 15) & ~static_cast<size_t>(15);
   if (act > kDownSmem - part) act = kDownSmem - part;
   p.act_floats = static_cast<int>(act / sizeof(float));
@@ -621,29 +1081,63 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   return launch_cluster(kernel, tiles * size, kDownThreads, size, act + part, st, p);
 }
 
+template <auto kernel>
+cudaError_t up_launch(const LayerParams& p, cudaStream_t st) {
+  constexpr int kMostTable = 2 * kUpWarps * EGS_MAX_EXPERTS * 4;
+  cudaError_t err = ensure_smem_optin<kernel>(kMostTable);
+  if (err != cudaSuccess) return err;
+  count_launch();
+  return launch_cluster(kernel, kUpGrid, kUpThreads, kUpCluster, static_cast<size_t>(2 * kUpWarps) * ((p.E + 3) / 4 * 4) * 4, st, p);
+}
+
 bool on(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// An expert's weights of `down` that are brought to the L2 ahead: all, where those of all experts that can be chosen leave half of it to others.
+void ahead(LayerParams* p, long long bytes) {
+  const long long most = p->tokens * p->k < p->E ? p->tokens * p->k : p->E;
+  p->down_bytes = bytes * most <= (64ll << 20) ? static_cast<int>(bytes) : 0;
+  p->pieces = (p->down_bytes + 8191) / 8192;
+  p->by_pieces = Div(p->pieces > 0 ? p->pieces : 1);
+}
+
 template <typename T>
-cudaError_t layer_t(const LayerParams& p, bool fp4, const egs_route& r, const float* bias, cudaStream_t st) {
+cudaError_t layer_t(LayerParams p, bool fp4, bool up_cn, bool down_cn, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T), kLanes = 8;
-  const dim3 grid((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows);
-  const bool vectors = p.I % V == 0 && p.x_row % V == 0 && on(p.X, 16) && on(p.router, 16);
-  count_launch();
-  cudaError_t err = vectors ? launch_kernel(few_logits_kernel<T, V>, grid, 256, 0, st, true, p) : launch_kernel(few_logits_kernel<T, 1>, grid, 256, 0, st, true, p);
-  if (err != cudaSuccess) return err;
-  if ((err = launch_route_tokens(p.logits, bias, p.weights, p.experts, r, p.E, EGS_F32, st)) != cudaSuccess) return err;
-  count_launch();
+  p.x_vectors = p.I % V == 0 && p.x_row % V == 0 && on(p.X, 16) && on(p.router, 16);
+  // Logits by every cluster for itself where that is little: 64 KB of the router and 64 Ki products for a CTA.
+  const long long router = static_cast<long long>(p.E) * p.I;
+  p.by_k = Div(p.k);
+  p.by_E4 = Div((p.E + 3) / 4 * 4);
+  p.own_logits = p.tokens <= kUpWarps && router * static_cast<long long>(sizeof(T)) <= (256 << 10) && router * p.tokens <= (256 << 10);
+  cudaError_t err = cudaSuccess;
+  if (!p.own_logits) {
+    count_launch();
+    err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
+    if (err != cudaSuccess) return err;
+  }
   if (fp4) {
-    if ((err = launch_kernel(few_up4_kernel<T>, kUpGrid, kUpThreads, 0, st, true, p)) != cudaSuccess) return err;
-    return down_launch<few_down4_kernel<T>, T>(p, kTile4, st);
+    // (what lies behind the last row may be nobody's)
+    ahead(&p, down_cn ? p.down_row * ((p.J + 1) / 2 - 1) + p.I / 16 * 16 : p.down_row * (p.I - 1) + (p.J + 1) / 2 / 16 * 16);
+    if (p.down_far % 16 || !on(p.down, 16)) p.pieces = 0;
+    auto fours = [](const void* w, long long row, long long far, int N) { return row % 4 == 0 && far % 4 == 0 && N % 4 == 0 && on(w, 4); };
+    const int up = !up_cn ? 0 : fours(p.up, p.up_row, p.up_far, p.J) ? 4 : 1, down = !down_cn ? 0 : fours(p.down, p.down_row, p.down_far, p.I) ? 4 : 1;
+    p.by_tiles = Div((p.J + tile4(up) - 1) / tile4(up));
+    err = up == 0 ? up_launch<few_up4_kernel<T, 0>>(p, st) : up == 4 ? up_launch<few_up4_kernel<T, 4>>(p, st) : up_launch<few_up4_kernel<T, 1>>(p, st);
+    if (err != cudaSuccess) return err;
+    return down == 0 ? down_launch<few_down4_kernel<T, 0>, T>(p, tile4(0), st) : down == 4 ? down_launch<few_down4_kernel<T, 4>, T>(p, tile4(4), st) : down_launch<few_down4_kernel<T, 1>, T>(p, tile4(1), st);
   }
   // (one width for both: the parts of `up` are counted by it)
   const bool wide = p.I % V == 0 && p.J % V == 0 && on(p.up, 16) && on(p.down, 16);
   if (wide) {
-    if ((err = launch_kernel(few_up_kernel<T, V, kLanes>, kUpGrid, kUpThreads, 0, st, true, p)) != cudaSuccess) return err;
+    const long long bytes = static_cast<long long>(p.I) * p.J * sizeof(T);
+    p.down_far = bytes;
+    ahead(&p, bytes);
+    p.by_tiles = Div((p.J + V * kLanes - 1) / (V * kLanes));
+    if ((err = up_launch<few_up_kernel<T, V, kLanes>>(p, st)) != cudaSuccess) return err;
     return down_launch<few_down_kernel<T, V, kLanes>, T>(p, V * kLanes, st);
   }
-  if ((err = launch_kernel(few_up_kernel<T, 1, 32>, kUpGrid, kUpThreads, 0, st, true, p)) != cudaSuccess) return err;
+  p.by_tiles = Div((p.J + 31) / 32);
+  if ((err = up_launch<few_up_kernel<T, 1, 32>>(p, st)) != cudaSuccess) return err;
   return down_launch<few_down_kernel<T, 1, 32>, T>(p, 32, st);
 }
 
@@ -651,20 +1145,24 @@ cudaError_t layer_t(const LayerParams& p, bool fp4, const egs_route& r, const fl
 
 size_t few_layer_workspace(const egs_route& r, long long J) {
   const size_t logits = (static_cast<size_t>(r.tokens) * r.E + 3) / 4 * 4;
-  return (logits + static_cast<size_t>(kMostParts) * r.tokens * r.top_k * J) * sizeof(float);
+  return sizeof(LayerList) + (logits + static_cast<size_t>(kMostParts) * r.tokens * r.top_k * J) * sizeof(float);
 }
 
 cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st) {
   LayerParams p{};
   p.X = f.X; p.router = f.router; p.up = f.up; p.down = f.down; p.up_scale = f.up_scale; p.down_scale = f.down_scale;
   p.out = f.out; p.weights = f.weights; p.experts = f.experts;
-  p.logits = static_cast<float*>(workspace);
+  p.list = static_cast<LayerList*>(workspace);
+  p.logits = reinterpret_cast<float*>(p.list + 1);
   p.h = p.logits + (static_cast<size_t>(r.tokens) * r.E + 3) / 4 * 4;
   p.x_row = f.x_row;
   p.tokens = static_cast<int>(r.tokens); p.E = r.E; p.k = r.top_k; p.I = f.I; p.J = f.J;
+  p.bias = f.bias; p.groups = r.groups; p.top_groups = r.top_groups; p.group_top = r.group_top;
+  p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
   const bool fp4 = f.up_scale != nullptr;
   p.up_row = fp4 ? f.up_row : p.J; p.us_row = f.us_row; p.down_row = fp4 ? f.down_row : p.I; p.ds_row = f.ds_row;
-  return dtype == EGS_F16 ? layer_t<__half>(p, fp4, r, f.bias, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, fp4, r, f.bias, st) : layer_t<float>(p, fp4, r, f.bias, st);
+  p.up_far = f.up_far; p.down_far = f.down_far;
+  return dtype == EGS_F16 ? layer_t<__half>(p, fp4, f.up_cn, f.down_cn, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, fp4, f.up_cn, f.down_cn, st) : layer_t<float>(p, fp4, f.up_cn, f.down_cn, st);
 }
 
 }  // namespace egs

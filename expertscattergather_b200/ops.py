@@ -557,7 +557,8 @@ def routed_experts_few(x, router, up, down, top_k, bias=None, *, up_scale=None, 
 
     ``x`` [..., I] of at most ``FEW_TOKENS`` tokens and ``FEW_SLOTS`` of tokens * top_k, ``router`` [E, I], ``up`` [E, I, J], ``down`` [E, J, I] of
     one type; or, with their scales, weights in 4 bits as :func:`quantize_rows_fp4` makes them of the transposed ones, ``up`` [E, J, I / 2] and ``down``
-    [E, I, J / 2]: the rows ahead of both products are then rounded to 4 bits as well, and sums are those of :func:`expert_matmul_fp4`.
+    [E, I, J / 2]: the rows ahead of both products are then rounded to 4 bits as well, and sums are those of :func:`expert_matmul_fp4`.  (Their bytes
+    may lie along either of the last two dimensions; others are copied first.)
     Choice and weights are those of :func:`route_tokens`, of logits that stay float32 (a module's are rounded to its type).  All sums and what
     lies between the products are float32; ``out`` is rounded once.  No gradients.  The same bits in every run."""
     return _host().routed_experts_few(x, router, up, down, int(top_k), bias, up_scale, down_scale, score, int(groups), int(top_groups), int(group_top),

@@ -430,8 +430,9 @@ size_t egs_expert_matmul_fp4_rows_workspace_bytes(const egs_ragged* dims, int pa
  *
  * out[t] = sum over j of weights[t, j] * silu(X[t] up[e]) down[e], e = experts[t, j]: weights and experts [tokens, top_k] are those of egs_route_tokens for the
  * logits X[t] . router[e] [E, I], which stay float32, as do all sums; out [tokens, I] is rounded once.  X's rows lie x_stride elements apart.
- * up [E, I, J], down [E, J, I]; or in 4 bits (egs_quantize_rows_fp4), up [E, J, I / 2] and down [E, I, J / 2], where X's rows and silu(..) are rounded to
- * 4 bits ahead of their products too.  At most EGS_MAX_FEW_TOKENS tokens and EGS_MAX_FEW_SLOTS = tokens * top_k.
+ * up [E, I, J], down [E, J, I]; or in 4 bits (egs_quantize_rows_fp4), where X's rows and silu(..) are rounded to 4 bits ahead of their products too: with the
+ * layout EGS_W_NC up [E, J, I / 2] and down [E, I, J / 2], rows as everywhere; with EGS_W_CN the same bytes with the columns together, up [E, I / 2, J] and
+ * down [E, J / 2, I], from any address and stride on; experts up_far and down_far bytes apart, scales always [E, J, I / 32] and [E, I, J / 32].  At most EGS_MAX_FEW_TOKENS tokens and EGS_MAX_FEW_SLOTS = tokens * top_k.
  * workspace (16-byte aligned): egs_routed_experts_few_workspace_bytes() bytes.  The same bits in every run.
  * ------------------------------------------------------------------------------------------------ */
 enum { EGS_MAX_FEW_TOKENS = 32, EGS_MAX_FEW_SLOTS = 256 };
@@ -439,7 +440,8 @@ int egs_routed_experts_few(const void* X, const void* router, const float* bias,
                            int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype, void* workspace,
                            size_t workspace_bytes, void* cuda_stream);
 int egs_routed_experts_few_fp4(const void* X, const void* router, const float* bias, const uint8_t* up, const uint8_t* up_scale, int64_t up_stride,
-                               int64_t us_stride, const uint8_t* down, const uint8_t* down_scale, int64_t down_stride, int64_t ds_stride, void* out,
+                               int64_t up_far, int64_t us_stride, int up_layout, const uint8_t* down, const uint8_t* down_scale, int64_t down_stride,
+                               int64_t down_far, int64_t ds_stride, int down_layout, void* out,
                                float* weights, int32_t* experts, const egs_route* route, int64_t I, int64_t J, int64_t x_stride, int dtype,
                                void* workspace, size_t workspace_bytes, void* cuda_stream);
 size_t egs_routed_experts_few_workspace_bytes(const egs_route* route, int64_t I, int64_t J);

@@ -23,8 +23,8 @@ def plain(spec=None, I=64, J=64, x_stride=64, dtype=0, ws=one, size=1 << 40, **h
                                               dtype, ws, size, None)
 
 
-def fp4_call(spec=None, I=64, J=64, up=one, us=one, upp=32, usp=16, down=one, ds=one, dp=32, dsp=16, ws=one, size=1 << 40):
-    return _lib.load().egs_routed_experts_few_fp4(one, one, None, up, us, upp, usp, down, ds, dp, dsp, one, one, one, spec if spec is not None else route(), I, J, 64, 0, ws, size, None)
+def fp4_call(spec=None, I=64, J=64, up=one, us=one, upp=32, upf=2048, usp=16, upl=_lib.W_NC, down=one, ds=one, dp=32, df=2048, dsp=16, dl=_lib.W_NC, ws=one, size=1 << 40):
+    return _lib.load().egs_routed_experts_few_fp4(one, one, None, up, us, upp, upf, usp, upl, down, ds, dp, df, dsp, dl, one, one, one, spec if spec is not None else route(), I, J, 64, 0, ws, size, None)
 
 
 @pytest.mark.parametrize("spec,code", [({"E": 0}, BAD), ({"top_k": 0}, BAD), ({"top_k": 9}, BAD), ({"groups": 3}, BAD), ({"groups": 4, "top_groups": 5}, BAD), ({"group_top": 3}, BAD), ({"score": 2}, BAD),
@@ -43,8 +43,11 @@ def test_entries_sizes_pointers_and_workspaces():
     assert plain(dtype=3) == BAD and plain(x_stride=-1) == BAD
     for name in ("X", "router", "up", "down", "out", "weights", "experts"):
         assert plain(**{name: None}) == BAD
-    for bad in ({"upp": 24}, {"upp": 16}, {"usp": 1}, {"dp": 8}, {"dsp": 0}, {"us": None}, {"ds": None}, {"up": off}, {"down": off}, {"up": None}):
+    for bad in ({"upp": 24}, {"upp": 16}, {"usp": 1}, {"dp": 8}, {"dsp": 0}, {"us": None}, {"ds": None}, {"up": off}, {"down": off}, {"up": None}, {"upl": 2}, {"upf": 2000}, {"upf": 2040},
+                {"df": 2008}, {"upl": _lib.W_CN}, {"upl": _lib.W_CN, "upp": 64, "upf": 2047}, {"upl": _lib.W_CN, "upp": 63}, {"dl": _lib.W_CN, "dp": 64, "df": 2047}, {"dl": _lib.W_CN, "dp": 64, "dsp": 1}):
         assert fp4_call(**bad) == BAD
+    for good in ({"upl": _lib.W_CN, "upp": 64}, {"dl": _lib.W_CN, "dp": 64, "down": off}, {"upl": _lib.W_CN, "upp": 65, "upf": 31 * 65 + 64, "usp": 2}):
+        assert fp4_call(**good, size=0) == WORKSPACE
     assert _lib.load().egs_routed_experts_few_workspace_bytes(route(tokens=33), 64, 64) == 0
     assert _lib.load().egs_routed_experts_few_workspace_bytes(route(tokens=0), 64, 64) == 0
     assert _lib.load().egs_routed_experts_few_workspace_bytes(None, 64, 64) == 0

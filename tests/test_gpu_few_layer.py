@@ -128,8 +128,15 @@ def test_layer_on_4_bits(dtype, tokens, E, k, I, J):
     gen = torch.Generator(device="cuda").manual_seed(5)
     x = (torch.randint(-6, 7, (tokens, I), device="cuda", generator=gen).float() * 0.5).to(t)
     router = (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    others = []
     out, w, ids = ops.routed_experts_few(x, router, u, d, k, up_scale=us, down_scale=ds)
     check_choice(x, router, None, k, w, ids)
+    across = [q.transpose(1, 2).contiguous().transpose(1, 2) for q in (u, d)]             # the bytes of all channels together
+    spare = torch.nn.functional.pad(across[1].transpose(1, 2), (0, 3, 0, 2))[:, :d.shape[2], :I].transpose(1, 2)      # ... experts and rows apart, rows that begin anywhere
+    for uu, dd in ((across[0], d), (u, across[1]), (across[0], across[1]), (u, spare)):
+        other = ops.routed_experts_few(x, router, uu, dd, k, up_scale=us, down_scale=ds)
+        assert torch.equal(other[1], w) and torch.equal(other[2], ids)
+        others.append(other[0])
     xq = fp4.values(*fp4.quantize(x), I)
     up, down = fp4.rows(u, us)[..., :I].transpose(1, 2), fp4.rows(d, ds)[..., :J].transpose(1, 2)
     want = torch.zeros(tokens, I, dtype=torch.float64, device="cuda")
@@ -144,8 +151,9 @@ def test_layer_on_4_bits(dtype, tokens, E, k, I, J):
             size.index_put_((tt,), we * (a.abs() @ down[e].abs()), accumulate=True)
     # a block's products are exact; chains of at most J / 32 blocks, the joins, the CTAs and the choices
     off = size * ((J / 32 + k + 24) * 2.0 ** -24) + want.abs() * (torch.finfo(t).eps / 2) + (2.0 ** -25 if dtype == "f16" else 0)
-    worst = ((out.double() - want).abs() - off).max().item()
-    assert worst <= 0, (worst, (out.double() - want).abs().max().item())
+    for got in (out, *others):
+        worst = ((got.double() - want).abs() - off).max().item()
+        assert worst <= 0, (worst, (got.double() - want).abs().max().item())
 
 
 def test_strides_and_shapes():
