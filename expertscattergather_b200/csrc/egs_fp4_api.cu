@@ -180,6 +180,7 @@ int egs_routed_experts_few_fp4(const void* X, const void* router, const float* b
   if (int rc = check_layer(route, I, J)) return rc;
   // an expert's [N, C / 2], or [C / 2, N]
   auto holds = [&](const uint8_t* w, int64_t stride, int64_t far, int64_t s_stride, int layout, int64_t C, int64_t N) {
+    if (stride > 0xffffffffll || s_stride > 0xffffffffll) return false;
     if (layout == EGS_W_NC) return strides_hold(stride, s_stride, C, false) && far >= stride * (N - 1) + (C + 1) / 2 && far % 16 == 0 && on16(w);
     return layout == EGS_W_CN && s_stride >= (C + 31) / 32 && stride >= N && far >= stride * ((C + 1) / 2 - 1) + N;
   };

@@ -1,9 +1,9 @@
 // A whole routed layer for a few tokens: out[t] = sum over j of w[t, j] silu(x[t] up[e]) down[e], e the j-th expert that token t chose.  Its work is
 // reading the weights of the experts that were chosen, each of them once, with all SMs.
 //
-//   logits   a warp has an expert's row of the router and the tokens in fours: in `up`, by each cluster of CTAs for itself, where tokens and router are few
-//            and small, else by a kernel of its own
-//   up       every CTA makes the choice for itself; units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round
+//   choice   where tokens and router are few and small, in `up`: each cluster of CTAs forms the logits, each CTA makes the choice for itself; else two kernels,
+//            the logits, in which a warp has two experts' rows of the router and four tokens, and egs_choice.cu's
+//   up       units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round
 //            the CTAs; float32 sums of parts.  The other product's weights are brought to the L2 meanwhile.
 //   down     a cluster has a tile of the output's columns, its CTAs the contraction in parts; warps have the experts' tokens in turn.  The parts' sums
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__
   });
 }
 
-// What both `up` kernels begin with: logits (or those that are there), the choice, the items, the parts; the CTAs of a cluster share the logits.
+// What both `up` kernels begin with: logits and the choice (or that which is there), the items, the parts; the CTAs of a cluster share the logits.
 // table: 2 * 8 rows of E4 words, logits and keys.  `tiles`: of columns.
 template <typename T>
 __device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint32_t* table, int tiles, int fixed) {
@@ -362,21 +362,17 @@ __device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint3
       });
     cluster_sync();
   }
-  for (int t0 = 0; t0 < p.tokens; t0 += kUpWarps) {
-    const int t = t0 + warp, here = min(kUpWarps, p.tokens - t0);
+  if (p.own_logits) {
+    const int t = warp;
     float* row = logits + warp * E4;
     Softmax soft{};
     if (t < p.tokens) {
-      if (!p.own_logits) {
-        for (int e = lane; e < p.E; e += 32) row[e] = p.logits[t * p.E + e];
-        __syncwarp();
-      }
       soft = form_keys(p, row, keys + warp * E4, E4);
       if (p.E > kCounted) choose_in_turn(p, keys + warp * E4, s->ids + t * p.k);
     }
     __syncthreads();
     if (p.E <= kCounted) {
-      choose_by_count(p, keys, here, E4, s->ids + t0 * p.k);
+      choose_by_count(p, keys, p.tokens, E4, s->ids);
       __syncthreads();
     }
     if (blockIdx.x == 0 && t < p.tokens) {
@@ -386,7 +382,9 @@ __device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint3
         p.experts[t * p.k + lane] = s->ids[t * p.k + lane];
       }
     }
-    if (t0 + kUpWarps < p.tokens) __syncthreads();
+  } else {
+    for (int i = tid; i < p.tokens * p.k; i += kUpThreads) s->ids[i] = p.experts[i];
+    __syncthreads();
   }
   list_items(p, s);
   const int parts = parts_of(s->count * tiles, p.I, fixed);
@@ -407,20 +405,53 @@ __device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint3
 }
 
 // ---- products along rows of the weights ([contraction, columns]) -----------------------------------------------------
+// Sums of V columns, two to a 64-bit register where V is even: one instruction adds two products.
+template <int V> struct Sums {
+  static constexpr bool kPairs = V % 2 == 0;
+  using Word = typename std::conditional<kPairs, unsigned long long, float>::type;
+  Word raw[kPairs ? V / 2 : V];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (auto& x : raw) x = 0;
+  }
+  __device__ __forceinline__ float get(int v) const {
+    if constexpr (kPairs) return __uint_as_float(static_cast<uint32_t>(v & 1 ? raw[v / 2] >> 32 : raw[v / 2]));
+    else return raw[v];
+  }
+  __device__ __forceinline__ void set(int v, float a, float b) {          // of v and v + 1
+    raw[v / 2] = pair(a, b);
+  }
+  static __device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+  }
+  template <class P>
+  __device__ __forceinline__ void add(float x, const P& w) {
+    if constexpr (kPairs) {
+      const unsigned long long xx = pair(x, x);
+#pragma unroll
+      for (int v = 0; v < V; v += 2) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(raw[v / 2]) : "l"(xx), "l"(pair(w.get(v), w.get(v + 1))));
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) raw[v] = fmaf(x, w.get(v), raw[v]);
+    }
+  }
+};
+
 // A group of lanes has four neighbouring rows at a time, every `step`-th such four from c on; a[m] + c - base: the other operand, zeros up to whole
 // fours.  `ready` is called when the first weights have been asked for.
 template <typename T, int V, int M, int AHEAD, class Ready>
-__device__ __forceinline__ void accumulate(float (&acc)[M][V], const T* W, long long w_row, int c, int step, int end, bool on, const float* const (&a)[M], int base, Ready&& ready) {
+__device__ __forceinline__ void accumulate(Sums<V> (&acc)[M], const T* W, int w_row, int c, int step, int end, bool on, const float* const (&a)[M], int base, Ready&& ready) {
   using P = Packed<T, V>;
   P w[AHEAD][4];
   auto load = [&]() {
+    const T* from = W + static_cast<long long>(c) * w_row;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = c + i * step + r;
-        w[i][r] = on && row < end ? *reinterpret_cast<const P*>(W + row * w_row) : P{};
-      }
+      for (int r = 0; r < 4; ++r)
+        w[i][r] = on && c + i * step + r < end ? *reinterpret_cast<const P*>(from + static_cast<long long>(i * step + r) * w_row) : P{};
   };
   load();
   ready();
@@ -431,27 +462,28 @@ __device__ __forceinline__ void accumulate(float (&acc)[M][V], const T* W, long 
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const float4 x = *reinterpret_cast<const float4*>(a[m] + c + i * step - base);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          acc[m][v] = fmaf(x.x, w[i][0].get(v), acc[m][v]);
-          acc[m][v] = fmaf(x.y, w[i][1].get(v), acc[m][v]);
-          acc[m][v] = fmaf(x.z, w[i][2].get(v), acc[m][v]);
-          acc[m][v] = fmaf(x.w, w[i][3].get(v), acc[m][v]);
-        }
+        acc[m].add(x.x, w[i][0]);
+        acc[m].add(x.y, w[i][1]);
+        acc[m].add(x.z, w[i][2]);
+        acc[m].add(x.w, w[i][3]);
       }
     }
     c += AHEAD * step;
     if (c < end) load();
   }
 }
+// Sums over the groups of lanes: all lanes have them.
 template <int LANES, int V, int M>
-__device__ __forceinline__ void join_groups(float (&acc)[M][V]) {
+__device__ __forceinline__ void join_groups(const Sums<V> (&acc)[M], float (&sum)[M][V]) {
 #pragma unroll
-  for (int o = LANES; o < 32; o <<= 1)
+  for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+    for (int v = 0; v < V; ++v) {
+      float x = acc[m].get(v);
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[m][v] += __shfl_xor_sync(kAll, acc[m][v], o);
+      for (int o = LANES; o < 32; o <<= 1) x += __shfl_xor_sync(kAll, x, o);
+      sum[m][v] = x;
+    }
 }
 __host__ __device__ constexpr int ahead_of(int V) { return V >= 4 ? 2 : 4; }
 
@@ -467,17 +499,16 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
   constexpr int kGroups = kUpThreads / LANES, kTile = LANES * V;
   const int tid = threadIdx.x, l = tid % LANES, n = n0 + l * V;
   const T* W = static_cast<const T*>(p.up) + item.expert * (p.up_row * p.I) + n;
-  float acc[M][V];
+  Sums<V> acc[M];
   const float* a[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     a[m] = s->x[m];
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[m][v] = 0.f;
+    acc[m].zero();
   }
   for (int c0 = begin; c0 < end; c0 += kUpPart) {
     const int c1 = min(end, c0 + kUpPart);
-    accumulate<T, V, M, ahead_of(V)>(acc, W, p.up_row, c0 + tid / LANES * 4, kGroups * 4, c1, n < p.J, a, c0, [&]() {
+    accumulate<T, V, M, ahead_of(V)>(acc, W, static_cast<int>(p.up_row), c0 + tid / LANES * 4, kGroups * 4, c1, n < p.J, a, c0, [&]() {
       __syncthreads();                         // what was in shared memory has been read
 #pragma unroll
       for (int m = 0; m < M; ++m) {
@@ -487,12 +518,13 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
       __syncthreads();
     });
   }
-  join_groups<LANES, V, M>(acc);
+  float sum[M][V];
+  join_groups<LANES, V, M>(acc, sum);
   if ((tid & 31) < LANES) {
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int v = 0; v < V; ++v) s->sums[tid >> 5][m][l * V + v] = acc[m][v];
+      for (int v = 0; v < V; ++v) s->sums[tid >> 5][m][l * V + v] = sum[m][v];
   }
   __syncthreads();
   for (int i = tid; i < M * kTile; i += kUpThreads) {
@@ -516,6 +548,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
     const Item item = s.items.item[i];
     float* to = p.h + static_cast<long long>(part) * p.tokens * p.k * p.J;
     if (item.rows == 1) up_unit<T, V, LANES, 1>(p, &s, item, n0, begin, end, to);
+    else if (item.rows == 2) up_unit<T, V, LANES, 2>(p, &s, item, n0, begin, end, to);
     else up_unit<T, V, LANES, kRows>(p, &s, item, n0, begin, end, to);
   }
 }
@@ -574,16 +607,23 @@ template <typename T, int TILE>
 __device__ __forceinline__ void put_out(const LayerParams& p, const float* part, float* to, int shares, int n0) {
   const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = all / size;
   if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all have begun
-  for (int i = threadIdx.x; i < all; i += kDownThreads) {
+  for (int i = threadIdx.x * 4; i < all; i += kDownThreads * 4) {
     const int t = i / TILE, n = i % TILE;
-    float v = 0.f;
-    for (int j = 0; j < p.k; ++j)
-      for (int s = 0; s < shares; ++s) v += part[(s * slots + t * p.k + j) * TILE + n];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < p.k * shares; ++j) {
+      const int choice = shares == 1 ? j : j / shares, s = j - choice * shares;
+      const float4 x = *reinterpret_cast<const float4*>(part + (s * slots + t * p.k + choice) * TILE + n);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
     if (size == 1) {
-      if (n0 + n < p.I) static_cast<T*>(p.out)[static_cast<long long>(t) * p.I + n0 + n] = from_f32<T>(v);
+      T* out = static_cast<T*>(p.out) + static_cast<long long>(t) * p.I + n0 + n;
+      if (n0 + n < p.I) out[0] = from_f32<T>(v.x);
+      if (n0 + n + 1 < p.I) out[1] = from_f32<T>(v.y);
+      if (n0 + n + 2 < p.I) out[2] = from_f32<T>(v.z);
+      if (n0 + n + 3 < p.I) out[3] = from_f32<T>(v.w);
     } else {
-      const int owner = i / own;
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(to + rank * own + i - owner * own, owner)), "f"(v) : "memory");
+      const int owner = i / own;               // (shares are whole fours: a tile has at least 32 columns, a cluster eight CTAs)
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(in_cta(to + rank * own + i - owner * own, owner)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
     }
   }
   if (size == 1) return;
@@ -600,16 +640,16 @@ template <typename T, int V, int LANES, int M, class Ready>
 __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item, const float* act, int pitch, int base, int begin, int end, int n0, float* part, bool first, Ready&& ready) {
   constexpr int kTile = LANES * V;
   const int lane = threadIdx.x & 31, l = lane % LANES, n = n0 + l * V;
-  float acc[M][V];
+  Sums<V> acc[M];
   const float* a[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     a[m] = act + item.slot[m] * pitch;
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[m][v] = 0.f;
+    acc[m].zero();
   }
-  accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, p.down_row, begin + lane / LANES * 4, 32 / LANES * 4, end, n < p.I, a, base, ready);
-  join_groups<LANES, V, M>(acc);
+  accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, static_cast<int>(p.down_row), begin + lane / LANES * 4, 32 / LANES * 4, end, n < p.I, a, base, ready);
+  float sum[M][V];
+  join_groups<LANES, V, M>(acc, sum);
   if (lane < LANES) {
 #pragma unroll
     for (int m = 0; m < M; ++m)
@@ -617,7 +657,7 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float* to = part + item.slot[m] * kTile + l * V + v;
-          *to = first ? acc[m][v] : *to + acc[m][v];
+          *to = first ? sum[m][v] : *to + sum[m][v];
         }
       }
   }
@@ -664,6 +704,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
       const Item item = items.item[i];
       float* to = part + share * slots * kTile;
       if (item.rows == 1) down_item<T, V, LANES, 1>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
+      else if (item.rows == 2) down_item<T, V, LANES, 2>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
       else down_item<T, V, LANES, kRows>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
     }
     stage();
@@ -684,7 +725,7 @@ struct Weights4 {
 };
 struct Matrix4 {
   const uint8_t *w, *s;        // of an expert
-  long long row, s_row;        // NC: bytes from one column to the next, CN: from one pair of contraction elements to the next; scales: from one column to the next
+  uint32_t row, s_row;         // NC: bytes from one column to the next, CN: from one pair of contraction elements to the next; scales: from one column to the next
   int C, N;
 };
 
@@ -721,16 +762,16 @@ __device__ __forceinline__ void add_block(const Weights4& x, const uint8_t* cons
 template <int V>
 __device__ __forceinline__ void load_columns(Weights4& x, const Matrix4& t, int n, int b) {
   const bool there = n < t.N;
-  const uint8_t* from = t.w + b * 16ll * t.row + n;
+  const uint8_t* from = t.w + static_cast<unsigned long long>(b * 16) * t.row + n;
   const int rows = min(16, t.C / 2 - b * 16);
   uint32_t r[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    if constexpr (V == 4) r[i] = there && i < rows ? *reinterpret_cast<const uint32_t*>(from + i * t.row) : 0u;
-    else r[i] = there && i < rows ? from[i * t.row] : 0u;
+    if constexpr (V == 4) r[i] = there && i < rows ? *reinterpret_cast<const uint32_t*>(from + static_cast<unsigned long long>(i) * t.row) : 0u;
+    else r[i] = there && i < rows ? from[static_cast<unsigned long long>(i) * t.row] : 0u;
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) x.s[j] = n + j < t.N ? t.s[(n + j) * t.s_row + b] : 0u;
+  for (int j = 0; j < V; ++j) x.s[j] = n + j < t.N ? t.s[static_cast<unsigned long long>(n + j) * t.s_row + b] : 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t p0 = __byte_perm(r[4 * i], r[4 * i + 1], 0x5140), p1 = __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x5140);
@@ -780,8 +821,8 @@ __device__ __forceinline__ void along_rows(const Matrix4& t, int n0, int columns
     for (int j = 0; j < kColumns; ++j) {
       const int n = n0 + first + j * groups + group;
       const bool there = first + j * groups < columns && n < t.N && b < end;
-      next.w[j] = there ? load_block(t.w + n * t.row, b, t.C) : Block4{};
-      next.s[j] = there ? t.s[n * t.s_row + b] : 0u;
+      next.w[j] = there ? load_block(t.w + static_cast<unsigned long long>(n) * t.row, b, t.C) : Block4{};
+      next.s[j] = there ? t.s[static_cast<unsigned long long>(n) * t.s_row + b] : 0u;
     }
   };
   int first = 0, b = begin + along;            // of the weights that come next
@@ -890,7 +931,7 @@ __device__ __noinline__ void stage_rows4(const LayerParams& p, const Item& item,
 template <typename T, int LAYOUT, int M>
 __device__ __forceinline__ void up4_unit(const LayerParams& p, Up4Shared<LAYOUT>* s, const Item& item, int n0, int begin, int end, float* to) {
   const int tid = threadIdx.x, warp = tid >> 5;
-  const Matrix4 t{static_cast<const uint8_t*>(p.up) + item.expert * p.up_far, p.up_scale + item.expert * (p.us_row * p.J), p.up_row, p.us_row, (p.I + 1) / 2 * 2, p.J};
+  const Matrix4 t{static_cast<const uint8_t*>(p.up) + item.expert * p.up_far, p.up_scale + item.expert * (p.us_row * p.J), static_cast<uint32_t>(p.up_row), static_cast<uint32_t>(p.us_row), (p.I + 1) / 2 * 2, p.J};
   const uint8_t* a[M];
   const float* f[M];
 #pragma unroll
@@ -944,6 +985,8 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up4_kernel(const __grid_con
         if (n0 + c % kTile < p.J) to[static_cast<long long>(item.slot[c / kTile]) * p.J + n0 + c % kTile] = 0.f;
     } else if (item.rows == 1) {
       up4_unit<T, LAYOUT, 1>(p, &s, item, n0, begin, end, to);
+    } else if (item.rows == 2) {
+      up4_unit<T, LAYOUT, 2>(p, &s, item, n0, begin, end, to);
     } else {
       up4_unit<T, LAYOUT, kRows>(p, &s, item, n0, begin, end, to);
     }
@@ -954,7 +997,7 @@ template <int LAYOUT, int M, class Ready>
 __device__ __forceinline__ void down4_item(const LayerParams& p, const Item& item, const uint8_t* act, const float* scale, int pitch, int b0, int b1, int n0, int share, int shares, float* part,
                                            bool first, Ready&& ready) {
   constexpr int kTile = tile4(LAYOUT);
-  const Matrix4 t{static_cast<const uint8_t*>(p.down) + item.expert * p.down_far, p.down_scale + item.expert * (p.ds_row * p.I), p.down_row, p.ds_row, (p.J + 1) / 2 * 2, p.I};
+  const Matrix4 t{static_cast<const uint8_t*>(p.down) + item.expert * p.down_far, p.down_scale + item.expert * (p.ds_row * p.I), static_cast<uint32_t>(p.down_row), static_cast<uint32_t>(p.ds_row), (p.J + 1) / 2 * 2, p.I};
   const uint8_t* a[M];
   const float* f[M];
 #pragma unroll
@@ -1028,6 +1071,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down4_kernel(const __grid
       const Item item = items.item[x / shares];
       const int share = x % shares;
       if (item.rows == 1) down4_item<LAYOUT, 1>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
+      else if (item.rows == 2) down4_item<LAYOUT, 2>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
       else down4_item<LAYOUT, kRows>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
     }
     stage();
@@ -1087,7 +1131,7 @@ cudaError_t up_launch(const LayerParams& p, cudaStream_t st) {
   cudaError_t err = ensure_smem_optin<kernel>(kMostTable);
   if (err != cudaSuccess) return err;
   count_launch();
-  return launch_cluster(kernel, kUpGrid, kUpThreads, kUpCluster, static_cast<size_t>(2 * kUpWarps) * ((p.E + 3) / 4 * 4) * 4, st, p);
+  return launch_cluster(kernel, kUpGrid, kUpThreads, kUpCluster, p.own_logits ? static_cast<size_t>(2 * kUpWarps) * ((p.E + 3) / 4 * 4) * 4 : 0, st, p);
 }
 
 bool on(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -1101,7 +1145,7 @@ void ahead(LayerParams* p, long long bytes) {
 }
 
 template <typename T>
-cudaError_t layer_t(LayerParams p, bool fp4, bool up_cn, bool down_cn, cudaStream_t st) {
+cudaError_t layer_t(LayerParams p, const egs_route& route, bool fp4, bool up_cn, bool down_cn, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T), kLanes = 8;
   p.x_vectors = p.I % V == 0 && p.x_row % V == 0 && on(p.X, 16) && on(p.router, 16);
   // Logits by every cluster for itself where that is little: 64 KB of the router and 64 Ki products for a CTA.
@@ -1114,6 +1158,7 @@ cudaError_t layer_t(LayerParams p, bool fp4, bool up_cn, bool down_cn, cudaStrea
     count_launch();
     err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
     if (err != cudaSuccess) return err;
+    if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
   }
   if (fp4) {
     // (what lies behind the last row may be nobody's)
@@ -1162,7 +1207,7 @@ cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, v
   const bool fp4 = f.up_scale != nullptr;
   p.up_row = fp4 ? f.up_row : p.J; p.us_row = f.us_row; p.down_row = fp4 ? f.down_row : p.I; p.ds_row = f.ds_row;
   p.up_far = f.up_far; p.down_far = f.down_far;
-  return dtype == EGS_F16 ? layer_t<__half>(p, fp4, f.up_cn, f.down_cn, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, fp4, f.up_cn, f.down_cn, st) : layer_t<float>(p, fp4, f.up_cn, f.down_cn, st);
+  return dtype == EGS_F16 ? layer_t<__half>(p, r, fp4, f.up_cn, f.down_cn, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, r, fp4, f.up_cn, f.down_cn, st) : layer_t<float>(p, r, fp4, f.up_cn, f.down_cn, st);
 }
 
 }  // namespace egs
