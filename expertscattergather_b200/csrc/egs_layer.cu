@@ -47,6 +47,7 @@ struct LayerParams {
   long long down_far;        // bytes from one expert of `down` to the next
   int down_bytes;            // ... of one, to bring to the L2 ahead; 0: not
   int pieces;                // ... in so many pieces
+  int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
   Div by_pieces, by_tiles, by_k, by_E4;
 };
@@ -342,6 +343,15 @@ __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__
   });
 }
 
+// The other product's weights to the L2, in pieces that go round the CTAs.
+__device__ __forceinline__ void bring_down(const LayerParams& p, const Items& items) {
+  constexpr int kPiece = 8192;
+  for (int i = blockIdx.x + threadIdx.x * gridDim.x; i < items.count * p.pieces; i += kUpThreads * gridDim.x) {
+    const int which = p.by_pieces.quotient(i), from = (i - which * p.pieces) * kPiece;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char*>(p.down) + items.item[which].expert * p.down_far + from), "r"(min(kPiece, p.down_bytes - from)) : "memory");
+  }
+}
+
 // What both `up` kernels begin with: logits and the choice (or that which is there), the items, the parts; the CTAs of a cluster share the logits.
 // table: 2 * 8 rows of E4 words, logits and keys.  `tiles`: of columns.
 template <typename T>
@@ -394,12 +404,6 @@ __device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint3
       p.list->count = s->count;
       p.list->parts = parts;
     }
-  }
-  // the other product's weights to the L2, in pieces that go round the CTAs
-  constexpr int kPiece = 8192;
-  for (int i = blockIdx.x + tid * gridDim.x; i < s->count * p.pieces; i += kUpThreads * gridDim.x) {
-    const int which = p.by_pieces.quotient(i), from = (i - which * p.pieces) * kPiece;
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char*>(p.down) + s->item[which].expert * p.down_far + from), "r"(min(kPiece, p.down_bytes - from)) : "memory");
   }
   return parts;
 }
@@ -472,6 +476,49 @@ __device__ __forceinline__ void accumulate(Sums<V> (&acc)[M], const T* W, int w_
     if (c < end) load();
   }
 }
+// Weights on their way to shared memory, kDepth pieces of 64 bytes a thread, each thread's its own: what it asked for it reads, so that nobody waits for
+// others, and the next unit's weights come while this one's sums are joined.  (Into registers, with a wait for all that had been asked for before
+// more was, 43 MB came at 3.4 TB/s.)
+template <int THREADS, int DEPTH>
+struct Ring {
+  uint32_t base;
+  int slot = 0;
+  __device__ __forceinline__ explicit Ring(const void* smem) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16u) {}
+  __device__ __forceinline__ uint32_t at(int r) const { return base + static_cast<uint32_t>(slot * 4 + r) * (THREADS * 16u); }
+  __device__ __forceinline__ void ask(int r, const void* from, bool there) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(r)), "l"(from), "r"(there ? 16 : 0) : "memory");
+  }
+  __device__ __forceinline__ void asked() {        // (the slot that has been read is the one that is asked for anew)
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++slot == DEPTH) slot = 0;
+  }
+  __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory"); }
+  template <class P>
+  __device__ __forceinline__ P get(int r) const {
+    static_assert(sizeof(P) == 16, "pieces are of 16 bytes");
+    union {
+      uint4 raw;
+      P value;
+    } x{};
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.raw.x), "=r"(x.raw.y), "=r"(x.raw.z), "=r"(x.raw.w) : "r"(at(r)) : "memory");
+    return x.value;
+  }
+};
+// Four rows of weights times M rows of the other operand at x.
+template <typename T, int V, int M, class R>
+__device__ __forceinline__ void add_four(Sums<V> (&acc)[M], const R& ring, const float* const (&a)[M], int at) {
+  Packed<T, V> w[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) w[r] = ring.template get<Packed<T, V>>(r);
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const float4 x = *reinterpret_cast<const float4*>(a[m] + at);
+    acc[m].add(x.x, w[0]);
+    acc[m].add(x.y, w[1]);
+    acc[m].add(x.z, w[2]);
+    acc[m].add(x.w, w[3]);
+  }
+}
 // Sums over the groups of lanes: all lanes have them.
 template <int LANES, int V, int M>
 __device__ __forceinline__ void join_groups(const Sums<V> (&acc)[M], float (&sum)[M][V]) {
@@ -494,10 +541,26 @@ struct UpShared {
   float sums[kUpWarps][kRows][LANES * V];
 };
 
-template <typename T, int V, int LANES, int M>
-__device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LANES>* s, const Item& item, int n0, int begin, int end, float* to) {
-  constexpr int kGroups = kUpThreads / LANES, kTile = LANES * V;
-  const int tid = threadIdx.x, l = tid % LANES, n = n0 + l * V;
+struct UpUnit {
+  int item, part, n0, begin, end;
+};
+__device__ __forceinline__ UpUnit up_unit_of(const LayerParams& p, int u, int all, int length, int whole, int tile) {
+  UpUnit x;
+  x.part = u / all;
+  const int rest = u - x.part * all;
+  x.item = p.by_tiles.quotient(rest);
+  x.n0 = (rest - x.item * p.by_tiles.d) * tile;
+  x.begin = min(whole, x.part * length);
+  x.end = min(whole, x.begin + length);
+  return x;
+}
+
+// A unit's products; ring: has its weights (16-byte vectors), `next` asks for more; without it (narrow ones) they are asked for here.
+template <typename T, int V, int LANES, int M, class R, class Next>
+__device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LANES>* s, const UpUnit& u, float* to, R& ring, Next&& next) {
+  constexpr int kStep = kUpThreads / LANES * 4, kTile = LANES * V;
+  const int tid = threadIdx.x, l = tid % LANES, n = u.n0 + l * V;
+  const Item item = s->items.item[u.item];
   const T* W = static_cast<const T*>(p.up) + item.expert * (p.up_row * p.I) + n;
   Sums<V> acc[M];
   const float* a[M];
@@ -506,9 +569,9 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
     a[m] = s->x[m];
     acc[m].zero();
   }
-  for (int c0 = begin; c0 < end; c0 += kUpPart) {
-    const int c1 = min(end, c0 + kUpPart);
-    accumulate<T, V, M, ahead_of(V)>(acc, W, static_cast<int>(p.up_row), c0 + tid / LANES * 4, kGroups * 4, c1, n < p.J, a, c0, [&]() {
+  for (int c0 = u.begin; c0 < u.end; c0 += kUpPart) {
+    const int c1 = min(u.end, c0 + kUpPart), first = c0 + tid / LANES * 4;
+    auto stage = [&]() {
       __syncthreads();                         // what was in shared memory has been read
 #pragma unroll
       for (int m = 0; m < M; ++m) {
@@ -516,7 +579,17 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
         for (int i = tid; i < ((c1 - c0 + 3) & ~3); i += kUpThreads) s->x[m][i] = c0 + i < c1 ? to_f32<T>(x[c0 + i]) : 0.f;
       }
       __syncthreads();
-    });
+    };
+    if constexpr (V == 16 / sizeof(T)) {
+      stage();
+      for (int c = first, left = (c1 - c0 + kStep - 1) / kStep; left; --left, c += kStep) {
+        ring.wait();
+        if (c < c1) add_four<T, V, M>(acc, ring, a, c - c0);
+        next();
+      }
+    } else {
+      accumulate<T, V, M, ahead_of(V)>(acc, W, static_cast<int>(p.up_row), first, kStep, c1, n < p.J, a, c0, stage);
+    }
   }
   float sum[M][V];
   join_groups<LANES, V, M>(acc, sum);
@@ -529,27 +602,64 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
   __syncthreads();
   for (int i = tid; i < M * kTile; i += kUpThreads) {
     const int m = i / kTile, col = i % kTile;
-    if (m >= item.rows || n0 + col >= p.J) continue;
+    if (m >= item.rows || u.n0 + col >= p.J) continue;
     float t = 0.f;
 #pragma unroll
     for (int w = 0; w < kUpWarps; ++w) t += s->sums[w][m][col];
-    to[static_cast<long long>(item.slot[m]) * p.J + n0 + col] = t;
+    to[static_cast<long long>(item.slot[m]) * p.J + u.n0 + col] = t;
   }
 }
 
+constexpr int kUpDepth = 4, kDownDepth = 3;
+constexpr size_t ring_bytes(int threads, int depth) { return static_cast<size_t>(threads) * depth * 64; }
+
 template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_constant__ LayerParams p) {
-  constexpr int kTile = LANES * V;
-  extern __shared__ uint32_t layer_table[];
+  constexpr int kTile = LANES * V, kStep = kUpThreads / LANES * 4;
+  constexpr bool kRing = V == 16 / sizeof(T);
+  extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ UpShared<T, V, LANES> s;
-  const int tiles = p.by_tiles.d, parts = begin_layer<T>(p, &s.items, layer_table, tiles, kFixedRows), all = s.items.count * tiles, length = ((p.I + parts - 1) / parts + 3) & ~3;
-  for (int u = blockIdx.x; u < all * parts; u += gridDim.x) {
-    const int part = u / all, x = u - part * all, i = p.by_tiles.quotient(x), n0 = (x - i * tiles) * kTile, begin = min(p.I, part * length), end = min(p.I, begin + length);
-    const Item item = s.items.item[i];
-    float* to = p.h + static_cast<long long>(part) * p.tokens * p.k * p.J;
-    if (item.rows == 1) up_unit<T, V, LANES, 1>(p, &s, item, n0, begin, end, to);
-    else if (item.rows == 2) up_unit<T, V, LANES, 2>(p, &s, item, n0, begin, end, to);
-    else up_unit<T, V, LANES, kRows>(p, &s, item, n0, begin, end, to);
+  const int parts = begin_layer<T>(p, &s.items, layer_table + p.ring_words, p.by_tiles.d, kFixedRows), all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
+  Ring<kUpThreads, kUpDepth> ring(layer_table);
+  // what is asked for next: rows c .. c + 3 of unit `coming`
+  int coming = blockIdx.x, c = 0, end = 0, left = 0;
+  bool on = false;
+  const T* from = static_cast<const T*>(p.up);
+  auto next = [&]() {
+    if (left == 0 && coming < units) {
+      const UpUnit x = up_unit_of(p, coming, all, length, p.I, kTile);
+      const int n = x.n0 + threadIdx.x % LANES * V;
+      on = n < p.J;
+      c = x.begin + threadIdx.x / LANES * 4;
+      end = x.end;
+      left = (x.end - x.begin + kStep - 1) / kStep;
+      from = static_cast<const T*>(p.up) + s.items.item[x.item].expert * (p.up_row * p.I) + c * p.up_row + n;
+      coming += gridDim.x;
+    }
+    if (left) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool there = on && c + r < end;
+        ring.ask(r, there ? from + r * p.up_row : static_cast<const T*>(p.up), there);
+      }
+      c += kStep;
+      from += kStep * p.up_row;
+      --left;
+    }
+    ring.asked();
+  };
+  if constexpr (kRing) {
+#pragma unroll 1
+    for (int d = 0; d < kUpDepth; ++d) next();
+  }
+  bring_down(p, s.items);
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const UpUnit x = up_unit_of(p, u, all, length, p.I, kTile);
+    float* to = p.h + static_cast<long long>(x.part) * p.tokens * p.k * p.J;
+    const int rows = s.items.item[x.item].rows;
+    if (rows == 1) up_unit<T, V, LANES, 1>(p, &s, x, to, ring, next);
+    else if (rows == 2) up_unit<T, V, LANES, 2>(p, &s, x, to, ring, next);
+    else up_unit<T, V, LANES, kRows>(p, &s, x, to, ring, next);
   }
 }
 
@@ -636,9 +746,9 @@ __device__ __forceinline__ void put_out(const LayerParams& p, const float* part,
   }
 }
 
-template <typename T, int V, int LANES, int M, class Ready>
-__device__ __forceinline__ void down_item(const LayerParams& p, const Item& item, const float* act, int pitch, int base, int begin, int end, int n0, float* part, bool first, Ready&& ready) {
-  constexpr int kTile = LANES * V;
+template <typename T, int V, int LANES, int M, class R, class Next>
+__device__ __forceinline__ void down_item(const LayerParams& p, const Item& item, const float* act, int pitch, int base, int begin, int end, int n0, float* part, bool first, R& ring, Next&& next) {
+  constexpr int kTile = LANES * V, kStep = 32 / LANES * 4;
   const int lane = threadIdx.x & 31, l = lane % LANES, n = n0 + l * V;
   Sums<V> acc[M];
   const float* a[M];
@@ -647,7 +757,15 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
     a[m] = act + item.slot[m] * pitch;
     acc[m].zero();
   }
-  accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, static_cast<int>(p.down_row), begin + lane / LANES * 4, 32 / LANES * 4, end, n < p.I, a, base, ready);
+  if constexpr (V == 16 / sizeof(T)) {
+    for (int c = begin + lane / LANES * 4, left = (end - begin + kStep - 1) / kStep; left; --left, c += kStep) {
+      ring.wait();
+      if (c < end) add_four<T, V, M>(acc, ring, a, c - base);
+      next();
+    }
+  } else {
+    accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, static_cast<int>(p.down_row), begin + lane / LANES * 4, kStep, end, n < p.I, a, base, []() {});
+  }
   float sum[M][V];
   join_groups<LANES, V, M>(acc, sum);
   if (lane < LANES) {
@@ -665,52 +783,82 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
 
 template <typename T, int V, int LANES>
 __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_constant__ LayerParams p) {
-  constexpr int kTile = LANES * V;
+  constexpr int kTile = LANES * V, kStep = 32 / LANES * 4;
+  constexpr bool kRing = V == 16 / sizeof(T);
   extern __shared__ __align__(16) float layer_smem[];
   __shared__ DownShared items;
   if (cluster_size() > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_trigger();
   begin_down(p, &items);
-  const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5;
+  const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n0 = blockIdx.x / size * kTile;
-  float* act = layer_smem;
-  float* part = layer_smem + p.act_floats;
+  float* act = layer_smem + p.ring_words;
+  float* part = act + p.act_floats;
   const int parts = items.parts;
   const int length = ((p.J + size - 1) / size + 3) & ~3, begin = min(p.J, rank * length), end = min(p.J, begin + length);
   const int room = min(length, p.act_floats / slots & ~3);
-  int shares = 1;                              // warps that have an item's contraction in turn
-  while (items.count * shares * 2 <= kDownWarps && length / shares >= 64) shares *= 2;
+  int shares_log2 = 0;                         // warps that have an item's contraction in turn
+  while (items.count << (shares_log2 + 1) <= kDownWarps && length >> shares_log2 >= 64) ++shares_log2;
+  const int turns = items.count << shares_log2;
+  Ring<kDownThreads, kDownDepth> ring(layer_smem);
   for (int c0 = begin; c0 == begin || c0 < end; c0 += room) {
-    const int c1 = min(end, c0 + room), width = (c1 - c0 + 3) & ~3;
-    // activations, four at a time; a warp's first weights are on their way meanwhile
-    bool staged = false;
-    auto stage = [&]() {
-      if (staged) return;
-      staged = true;
-      __syncthreads();
-      for (int i = tid; i < slots * (width / 4); i += kDownThreads) {
-        const int slot = i / (width / 4), c = (i - slot * (width / 4)) * 4;
-        const float w = items.weights[slot];
-        float v[4];
-        activation<4>(p, parts, static_cast<long long>(slot) * p.J + c0 + c, c1 - c0 - c, v);
-        *reinterpret_cast<float4*>(act + slot * room + c) = make_float4(w * v[0], w * v[1], w * v[2], w * v[3]);
-      }
-      __syncthreads();
+    const int c1 = min(end, c0 + room), width = (c1 - c0 + 3) & ~3, each = ((width / 4 + (1 << shares_log2) - 1) >> shares_log2) * 4;
+    auto share_of = [&](int x, int* to) {      // first row, and the one behind the last
+      const int b = min(c1, c0 + (x & ((1 << shares_log2) - 1)) * each);
+      *to = min(c1, b + each);
+      return b;
     };
-    const int each = (width / 4 + shares - 1) / shares * 4;
-    for (int x = warp; x < items.count * shares; x += kDownWarps) {
-      const int i = x / shares, share = x - i * shares, b = min(c1, c0 + share * each), e = min(c1, b + each);
-      const Item item = items.item[i];
-      float* to = part + share * slots * kTile;
-      if (item.rows == 1) down_item<T, V, LANES, 1>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
-      else if (item.rows == 2) down_item<T, V, LANES, 2>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
-      else down_item<T, V, LANES, kRows>(p, item, act, room, c0, b, e, n0, to, c0 == begin, stage);
+    // what is asked for next: rows c .. c + 3 of turn `coming`
+    int coming = warp, c = 0, stop = 0, left = 0;
+    const T* from = static_cast<const T*>(p.down);
+    const bool on = n0 + lane % LANES * V < p.I;
+    auto next = [&]() {
+      while (left == 0 && coming < turns) {
+        const int b = share_of(coming, &stop);
+        c = b + lane / LANES * 4;
+        left = (stop - b + kStep - 1) / kStep;
+        from = static_cast<const T*>(p.down) + items.item[coming >> shares_log2].expert * (p.down_row * p.J) + c * p.down_row + n0 + lane % LANES * V;
+        coming += kDownWarps;
+      }
+      if (left) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool there = on && c + r < stop;
+          ring.ask(r, there ? from + r * p.down_row : static_cast<const T*>(p.down), there);
+        }
+        c += kStep;
+        from += kStep * p.down_row;
+        --left;
+      }
+      ring.asked();
+    };
+    if constexpr (kRing) {
+#pragma unroll 1
+      for (int d = 0; d < kDownDepth; ++d) next();
     }
-    stage();
+    // activations, four at a time; the first weights are on their way meanwhile
+    __syncthreads();
+    for (int i = tid; i < slots * (width / 4); i += kDownThreads) {
+      const int slot = i / (width / 4), at = (i - slot * (width / 4)) * 4;
+      const float w = items.weights[slot];
+      float v[4];
+      activation<4>(p, parts, static_cast<long long>(slot) * p.J + c0 + at, c1 - c0 - at, v);
+      *reinterpret_cast<float4*>(act + slot * room + at) = make_float4(w * v[0], w * v[1], w * v[2], w * v[3]);
+    }
+    __syncthreads();
+    for (int x = warp; x < turns; x += kDownWarps) {
+      int e;
+      const int b = share_of(x, &e);
+      const Item item = items.item[x >> shares_log2];
+      float* to = part + (x & ((1 << shares_log2) - 1)) * slots * kTile;
+      if (item.rows == 1) down_item<T, V, LANES, 1>(p, item, act, room, c0, b, e, n0, to, c0 == begin, ring, next);
+      else if (item.rows == 2) down_item<T, V, LANES, 2>(p, item, act, room, c0, b, e, n0, to, c0 == begin, ring, next);
+      else down_item<T, V, LANES, kRows>(p, item, act, room, c0, b, e, n0, to, c0 == begin, ring, next);
+    }
   }
   __syncthreads();
-  put_out<T, kTile>(p, part, part + max(4 * kDownWarps, slots) * kTile, shares, n0);
+  put_out<T, kTile>(p, part, part + max(4 * kDownWarps, slots) * kTile, 1 << shares_log2, n0);
 }
 
 // ---- weights in 4 bits -------------------------------------------------------------------------------------------------
@@ -976,6 +1124,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up4_kernel(const __grid_con
   extern __shared__ uint32_t layer_table[];
   __shared__ Up4Shared<LAYOUT> s;
   const int tiles = p.by_tiles.d, parts = begin_layer<T>(p, &s.items, layer_table, tiles, kFixedRows4 * kTile4 / kTile), all = s.items.count * tiles, blocks = fp4_blocks(p.I), length = (blocks + parts - 1) / parts;
+  bring_down(p, s.items);
   for (int u = blockIdx.x; u < all * parts; u += gridDim.x) {
     const int part = u / all, x = u - part * all, i = p.by_tiles.quotient(x), n0 = (x - i * tiles) * kTile, begin = min(blocks, part * length), end = min(blocks, begin + length);
     const Item item = s.items.item[i];
@@ -1081,7 +1230,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down4_kernel(const __grid
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
-constexpr size_t kDownSmem = 200 * 1024;
+constexpr size_t kDownSmem = 220 * 1024;
 
 template <class... Params, class... Args>
 cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, unsigned cluster, size_t smem, cudaStream_t st, Args... args) {
@@ -1116,22 +1265,23 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   cudaError_t err = ensure_smem_optin<kernel>(static_cast<int>(kDownSmem));
   if (err != cudaSuccess) return err;
   const unsigned size = cluster_of(tiles, p.J);
+  const size_t ring = static_cast<size_t>(p.ring_words) * 4;
   const size_t part = static_cast<size_t>((slots < 4 * kDownWarps ? 4 * kDownWarps : slots) + (size > 1 ? p.tokens : 0)) * tile * sizeof(float);
   size_t act = static_cast<size_t>(slots) * (p.J / size + 36) * sizeof(float);
   act = (act + 15) & ~static_cast<size_t>(15);
-  if (act > kDownSmem - part) act = kDownSmem - part;
+  if (act > kDownSmem - part - ring) act = kDownSmem - part - ring;
   p.act_floats = static_cast<int>(act / sizeof(float));
   count_launch();
-  return launch_cluster(kernel, tiles * size, kDownThreads, size, act + part, st, p);
+  return launch_cluster(kernel, tiles * size, kDownThreads, size, ring + act + part, st, p);
 }
 
 template <auto kernel>
 cudaError_t up_launch(const LayerParams& p, cudaStream_t st) {
-  constexpr int kMostTable = 2 * kUpWarps * EGS_MAX_EXPERTS * 4;
+  constexpr int kMostTable = 2 * kUpWarps * EGS_MAX_EXPERTS * 4 + static_cast<int>(ring_bytes(kUpThreads, kUpDepth));
   cudaError_t err = ensure_smem_optin<kernel>(kMostTable);
   if (err != cudaSuccess) return err;
   count_launch();
-  return launch_cluster(kernel, kUpGrid, kUpThreads, kUpCluster, p.own_logits ? static_cast<size_t>(2 * kUpWarps) * ((p.E + 3) / 4 * 4) * 4 : 0, st, p);
+  return launch_cluster(kernel, kUpGrid, kUpThreads, kUpCluster, (p.own_logits ? static_cast<size_t>(2 * kUpWarps) * ((p.E + 3) / 4 * 4) * 4 : 0) + static_cast<size_t>(p.ring_words) * 4, st, p);
 }
 
 bool on(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -1178,7 +1328,9 @@ cudaError_t layer_t(LayerParams p, const egs_route& route, bool fp4, bool up_cn,
     p.down_far = bytes;
     ahead(&p, bytes);
     p.by_tiles = Div((p.J + V * kLanes - 1) / (V * kLanes));
+    p.ring_words = static_cast<int>(ring_bytes(kUpThreads, kUpDepth) / 4);
     if ((err = up_launch<few_up_kernel<T, V, kLanes>>(p, st)) != cudaSuccess) return err;
+    p.ring_words = static_cast<int>(ring_bytes(kDownThreads, kDownDepth) / 4);
     return down_launch<few_down_kernel<T, V, kLanes>, T>(p, V * kLanes, st);
   }
   p.by_tiles = Div((p.J + 31) / 32);
