@@ -79,7 +79,7 @@ int layer(const FewLayer& f, const egs_route* r, int dtype, void* workspace, siz
   if (int rc = check_layer(r, f.I, f.J)) return rc;
   if (r->tokens == 0) return EGS_OK;
   if (!f.X || !f.router || !f.up || !f.down || !f.out || !f.weights || !f.experts) return EGS_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < few_layer_workspace(*r, f.J) || !on16(workspace)) return EGS_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < few_layer_workspace(*r, f.I, f.J) || !on16(workspace)) return EGS_ERR_WORKSPACE;
   return done(launch_few_layer(f, *r, dtype, workspace, stream_of(stream)), "routed_experts_few launch");
 }
 
@@ -161,7 +161,7 @@ int egs_expert_matmul_fp4_rows(const uint8_t* q, const uint8_t* q_scale, int64_t
 }
 
 size_t egs_routed_experts_few_workspace_bytes(const egs_route* route, int64_t I, int64_t J) {
-  return check_layer(route, I, J) == EGS_OK && route->tokens ? few_layer_workspace(*route, J) : 0;
+  return check_layer(route, I, J) == EGS_OK && route->tokens ? few_layer_workspace(*route, static_cast<int>(I), static_cast<int>(J)) : 0;
 }
 
 int egs_routed_experts_few(const void* X, const void* router, const float* bias, const void* up, const void* down, void* out, float* weights,

@@ -374,7 +374,7 @@ struct FewLayer {
   long long up_far, down_far;  // bytes from one expert to the next
   bool up_cn, down_cn;         // bytes lie along the columns: [E, I / 2, J] and [E, J / 2, I]
 };
-size_t few_layer_workspace(const egs_route& r, long long J);
+size_t few_layer_workspace(const egs_route& r, int I, int J);
 cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st);
 // Copies [rows, width] of 16-bit elements to rows `pitch` elements apart (a multiple of 8; zeros behind a row's end); dst NULL: nothing.
 struct PadRows {

@@ -4,7 +4,7 @@
 //   choice   where tokens and router are few and small, in `up`: each cluster of CTAs forms the logits, each CTA makes the choice for itself; else two kernels,
 //            the logits, in which a warp has two experts' rows of the router and four tokens, and egs_choice.cu's
 //   up       units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round
-//            the CTAs; float32 sums of parts.  The other product's weights are brought to the L2 meanwhile.
+//            the CTAs; float32 sums of parts.
 //   down     a cluster has a tile of the output's columns, its CTAs the contraction in parts; warps have the experts' tokens in turn.  The parts' sums
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
 //            CTAs' in theirs: the same bits in every run.
@@ -20,7 +20,7 @@ constexpr int kUpThreads = 256, kUpWarps = kUpThreads / 32, kUpGrid = 296, kUpPa
 constexpr int kUpCluster = 4;                // CTAs that form logits together (two SMs: clusters of eight leave SMs of a processing cluster without any)
 constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
 constexpr int kMostParts = 8;
-constexpr int kFixedRows = 128, kFixedRows4 = 512;       // of a unit, in rows of its tile: 16 KB of weights
+constexpr int kFixedRows = 128;              // of a unit, in rows of its tile: 16 KB of weights
 
 struct LayerList;
 struct LayerParams {
@@ -38,18 +38,16 @@ struct LayerParams {
   float* h;                  // [parts][tokens * k][J]
   LayerList* list;    // what `up` has found out
   long long x_row, up_row, us_row, down_row, ds_row;       // elements; in 4 bits bytes
-  long long up_far;          // in 4 bits: bytes from one expert of `up` to the next
+  long long up_far, down_far;      // in 4 bits: bytes from one expert to the next
   int tokens, E, k, I, J;
   int groups, top_groups, group_top, sigmoid, renormalize;
   float scale;
   int own_logits;            // `up` forms them
   int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
-  long long down_far;        // bytes from one expert of `down` to the next
-  int down_bytes;            // ... of one, to bring to the L2 ahead; 0: not
-  int pieces;                // ... in so many pieces
+  bool up_words, down_words; // 4 bits: scales can be read four at a time
   int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
-  Div by_pieces, by_tiles, by_k, by_E4;
+  Div by_tiles, by_k, by_E4;
 };
 
 // An expert's tokens, up to four at a time.
@@ -105,12 +103,22 @@ __device__ __forceinline__ void list_items(const LayerParams& p, Items* s) {
   __syncthreads();
 }
 
-// Parts that the contraction of `up` is cut into: the fewest rounds of the CTAs, a unit costing as much as `fixed` rows beside its own.
-__device__ __forceinline__ int parts_of(int units, int length, int fixed) {
+// ... for `down`
+__device__ __forceinline__ void publish(const LayerParams& p, const Items& s, int parts) {
+  if (blockIdx.x) return;
+  for (int i = threadIdx.x; i < s.count; i += blockDim.x) p.list->item[i] = s.item[i];
+  if (threadIdx.x == 0) {
+    p.list->count = s.count;
+    p.list->parts = parts;
+  }
+}
+
+// Parts that the contraction of `up` is cut into: the fewest rounds of the CTAs, a unit costing as much as kFixedRows beside its own.
+__device__ __forceinline__ int parts_of(int units, int length) {
   int best = 1, least = 0x7fffffff;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int s = 1 << i, cost = (units * s + kUpGrid - 1) / kUpGrid * (((length + s - 1) >> i) + fixed);
+    const int s = 1 << i, cost = (units * s + kUpGrid - 1) / kUpGrid * (((length + s - 1) >> i) + kFixedRows);
     if (cost < least && (i == 0 || length >> i >= 64)) {
       least = cost;
       best = s;
@@ -259,12 +267,6 @@ __device__ __forceinline__ uint32_t in_cta(const void* mine, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
   return at;
 }
-__device__ __forceinline__ float of_cta(const float* mine, int rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(in_cta(mine, rank)) : "memory");
-  return v;
-}
-
 // Dot products of two experts' rows of the router with M tokens' rows from t0 on (the last ones' for those that are not there); all lanes have them.  Loads
 // of AHEAD steps go out together.
 template <typename T, int V, int M, int AHEAD>
@@ -333,29 +335,23 @@ __device__ __forceinline__ void logits_of(const LayerParams& p, int e0, int e1, 
 }
 
 template <typename T>
+__device__ __forceinline__ void logits_by_warps(const LayerParams& p, int e, int t0) {
+  if (e >= p.E) return;
+  logits_of<T>(p, e, e + 1, t0, min(p.tokens, t0 + kRows), [&](int t, int expert, float v) {
+    if ((threadIdx.x & 31) == 0) p.logits[t * p.E + expert] = v;
+  });
+}
+template <typename T>
 __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__ LayerParams p) {
   pdl_wait();
   pdl_trigger();
-  const int e = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2, lane = threadIdx.x & 31, t0 = blockIdx.y * kRows;
-  if (e >= p.E) return;
-  logits_of<T>(p, e, e + 1, t0, min(p.tokens, t0 + kRows), [&](int t, int expert, float v) {
-    if (lane == 0) p.logits[t * p.E + expert] = v;
-  });
+  logits_by_warps<T>(p, (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2, blockIdx.y * kRows);
 }
 
-// The other product's weights to the L2, in pieces that go round the CTAs.
-__device__ __forceinline__ void bring_down(const LayerParams& p, const Items& items) {
-  constexpr int kPiece = 8192;
-  for (int i = blockIdx.x + threadIdx.x * gridDim.x; i < items.count * p.pieces; i += kUpThreads * gridDim.x) {
-    const int which = p.by_pieces.quotient(i), from = (i - which * p.pieces) * kPiece;
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char*>(p.down) + items.item[which].expert * p.down_far + from), "r"(min(kPiece, p.down_bytes - from)) : "memory");
-  }
-}
-
-// What both `up` kernels begin with: logits and the choice (or that which is there), the items, the parts; the CTAs of a cluster share the logits.
+// What `up` begins with: logits and the choice (or that which is there), the items, the parts; the CTAs of a cluster share the logits.
 // table: 2 * 8 rows of E4 words, logits and keys.  `tiles`: of columns.
 template <typename T>
-__device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint32_t* table, int tiles, int fixed) {
+__device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint32_t* table, int tiles) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, E4 = p.by_E4.d;
   float* logits = reinterpret_cast<float*>(table);
   uint32_t* keys = table + kUpWarps * E4;
@@ -397,14 +393,8 @@ __device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint3
     __syncthreads();
   }
   list_items(p, s);
-  const int parts = parts_of(s->count * tiles, p.I, fixed);
-  if (blockIdx.x == 0) {
-    for (int i = tid; i < s->count; i += kUpThreads) p.list->item[i] = s->item[i];
-    if (tid == 0) {
-      p.list->count = s->count;
-      p.list->parts = parts;
-    }
-  }
+  const int parts = parts_of(s->count * tiles, p.I);
+  publish(p, *s, parts);
   return parts;
 }
 
@@ -619,7 +609,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
   constexpr bool kRing = V == 16 / sizeof(T);
   extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ UpShared<T, V, LANES> s;
-  const int parts = begin_layer<T>(p, &s.items, layer_table + p.ring_words, p.by_tiles.d, kFixedRows), all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
+  const int parts = begin_layer<T>(p, &s.items, layer_table + p.ring_words, p.by_tiles.d), all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
   Ring<kUpThreads, kUpDepth> ring(layer_table);
   // what is asked for next: rows c .. c + 3 of unit `coming`
   int coming = blockIdx.x, c = 0, end = 0, left = 0;
@@ -652,7 +642,6 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
 #pragma unroll 1
     for (int d = 0; d < kUpDepth; ++d) next();
   }
-  bring_down(p, s.items);
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const UpUnit x = up_unit_of(p, u, all, length, p.I, kTile);
     float* to = p.h + static_cast<long long>(x.part) * p.tokens * p.k * p.J;
@@ -711,20 +700,16 @@ __device__ __forceinline__ void activation(const LayerParams& p, int parts, long
   }
 }
 
-// out[t, n0 + n] from the slots' products, part [shares][slots][tile].  Every CTA of a cluster has a share of the outputs, and the others hand it their
+// out[t, n0 + n] from this CTA's sums: sum(t, n, v) adds four of them to v.  Every CTA of a cluster has a share of the outputs, and the others hand it their
 // sums: to, room for them, [CTAs][outputs of a share] of shared memory.
-template <typename T, int TILE>
-__device__ __forceinline__ void put_out(const LayerParams& p, const float* part, float* to, int shares, int n0) {
-  const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = all / size;
+template <typename T, int TILE, class Sum>
+__device__ __forceinline__ void put_out(const LayerParams& p, float* to, int n0, Sum&& sum) {
+  const int rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = all / size;
   if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all have begun
-  for (int i = threadIdx.x * 4; i < all; i += kDownThreads * 4) {
+  for (int i = threadIdx.x * 4; i < all; i += blockDim.x * 4) {
     const int t = i / TILE, n = i % TILE;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = 0; j < p.k * shares; ++j) {
-      const int choice = shares == 1 ? j : j / shares, s = j - choice * shares;
-      const float4 x = *reinterpret_cast<const float4*>(part + (s * slots + t * p.k + choice) * TILE + n);
-      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-    }
+    sum(t, n, v);
     if (size == 1) {
       T* out = static_cast<T*>(p.out) + static_cast<long long>(t) * p.I + n0 + n;
       if (n0 + n < p.I) out[0] = from_f32<T>(v.x);
@@ -738,7 +723,7 @@ __device__ __forceinline__ void put_out(const LayerParams& p, const float* part,
   }
   if (size == 1) return;
   cluster_sync();
-  for (int i = threadIdx.x; i < own; i += kDownThreads) {
+  for (int i = threadIdx.x; i < own; i += blockDim.x) {
     const int x = rank * own + i, t = x / TILE, n = x % TILE;
     float v = to[i];
     for (int r = 1; r < size; ++r) v += to[r * own + i];
@@ -858,168 +843,208 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
     }
   }
   __syncthreads();
-  put_out<T, kTile>(p, part, part + max(4 * kDownWarps, slots) * kTile, 1 << shares_log2, n0);
+  put_out<T, kTile>(p, part + max(4 * kDownWarps, slots) * kTile, n0, [&](int t, int n, float4& v) {
+    for (int j = 0; j < p.k << shares_log2; ++j) {
+      const float4 x = *reinterpret_cast<const float4*>(part + ((j & ((1 << shares_log2) - 1)) * slots + t * p.k + (j >> shares_log2)) * kTile + n);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+  });
 }
 
 // ---- weights in 4 bits -------------------------------------------------------------------------------------------------
-// Four columns of an expert times M rows, a block of 32 contraction elements at a time: the weights' bytes lie along the contraction (NC, a lane has 16 of a column) or along
-// the columns (CN, a lane has four of each of 16 rows, or one where rows begin anywhere).  Twice the values are integers, so that a block's sum is exact.
-constexpr int kTile4 = 64;                     // NC: columns of a tile
-__host__ __device__ constexpr int tile4(int layout) { return layout == 0 ? kTile4 : layout == 4 ? 128 : 32; }      // layout: 0 NC, 4 or 1 CN with so many columns a lane
-constexpr int kColumns = 4;
-struct Weights4 {
-  Block4 w[kColumns];
-  uint32_t s[kColumns];
-};
+// Rows and weights become 16-bit floats, which hold them exactly, and go through the tensor cores (mma.sync: 16 columns, 16 contraction elements, up to eight
+// rows); a block's sums are exact, then times both scales into float32 sums.  (As integers through dp4a four columns and a block took 980
+// instructions a warp, and 85 us went by at 43 MB of weights, which are read in 7.)  The weights' bytes lie along the contraction (NC) or along the columns (CN).
+// A warp's stage: 4 blocks of the contraction x a tile of 32 columns, 2 KB of weights; kDepth4 stages are on their way, each warp's its own.  Lane (g, q) = (lane / 4,
+// lane % 4) multiplies columns 4 g .. 4 g + 3 and of each block the eight elements from 8 q on; their order is the same in both operands.
+constexpr int kTile4 = 32, kStage4 = 4, kDepth4 = 3, kThreads4 = 256, kWarps4 = kThreads4 / 32;
+constexpr int kRowPitch4 = 320;                // a row's 256 bytes, in other banks than the next one's
+constexpr int kStageRows4 = 2048, kStageScale4 = kStageRows4 + kRows * kRowPitch4, kStageF4 = kStageScale4 + 128, kStageBytes4 = kStageF4 + kRows * 16;
+constexpr int kWarpBytes4 = kDepth4 * kStageBytes4 + 512;      // ... and the scales of a stage as floats
+constexpr size_t kRing4 = static_cast<size_t>(kWarps4) * kWarpBytes4;
+__host__ __device__ constexpr int stages_of(int C) { return (fp4_blocks(C) + kStage4 - 1) / kStage4; }
+enum Layout4 { kNC, kCN16, kCN4, kCN1 };       // CN: rows, counted from the tensor's begin, are whole pieces of so many bytes
+
 struct Matrix4 {
   const uint8_t *w, *s;        // of an expert
-  uint32_t row, s_row;         // NC: bytes from one column to the next, CN: from one pair of contraction elements to the next; scales: from one column to the next
+  long long row;               // NC: bytes from one column to the next, CN: from one pair of contraction elements to the next
+  long long s_row;             // from one column's scales to the next
   int C, N;
+  bool words;                  // scales can be read four at a time
+};
+// Rows in 16-bit floats, whole blocks, and their scales, whole stages.
+struct Rows4 {
+  __half* x;
+  float* f;
+  int C;
+  __device__ __forceinline__ const __half* row(int i) const { return x + static_cast<long long>(i) * fp4_blocks(C) * kFp4Block; }
+  __device__ __forceinline__ const float* scale(int i) const { return f + i * stages_of(C) * kStage4; }
 };
 
-// acc[j][m] += the block's products; a[m]: twice the rows' 4 bits as bytes, f[m]: a quarter of their scale.
-template <int M, int COLUMNS>
-__device__ __forceinline__ void add_block(const Weights4& x, const uint8_t* const (&a)[M], const float (&f)[M], float (&acc)[COLUMNS][M]) {
-  uint32_t y[M][8];
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 z = *reinterpret_cast<const uint4*>(a[m] + h * 16);
-      y[m][4 * h] = z.x; y[m][4 * h + 1] = z.y; y[m][4 * h + 2] = z.z; y[m][4 * h + 3] = z.w;
-    }
-#pragma unroll
-  for (int j = 0; j < COLUMNS; ++j) {
-    int sum[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) sum[m] = 0;
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      uint32_t low, high;
-      fp4_integers(x.w[j].w[h], low, high);
-#pragma unroll
-      for (int m = 0; m < M; ++m) sum[m] = __dp4a(static_cast<int>(y[m][2 * h + 1]), static_cast<int>(high), __dp4a(static_cast<int>(y[m][2 * h]), static_cast<int>(low), sum[m]));
-    }
-    const float power = fp4_power(x.s[j]);
-#pragma unroll
-    for (int m = 0; m < M; ++m) acc[j][m] = fmaf(static_cast<float>(sum[m]) * f[m], power, acc[j][m]);
-  }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-
-// CN: a block of four columns from n on; the words of four rows become four columns' words.
-template <int V>
-__device__ __forceinline__ void load_columns(Weights4& x, const Matrix4& t, int n, int b) {
-  const bool there = n < t.N;
-  const uint8_t* from = t.w + static_cast<unsigned long long>(b * 16) * t.row + n;
-  const int rows = min(16, t.C / 2 - b * 16);
-  uint32_t r[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (V == 4) r[i] = there && i < rows ? *reinterpret_cast<const uint32_t*>(from + static_cast<unsigned long long>(i) * t.row) : 0u;
-    else r[i] = there && i < rows ? from[static_cast<unsigned long long>(i) * t.row] : 0u;
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) x.s[j] = n + j < t.N ? t.s[static_cast<unsigned long long>(n + j) * t.s_row + b] : 0u;
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t word_at(uint32_t at) {
+  uint32_t x;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ uint4 words_at(uint32_t at) {
+  uint4 x;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+  return x;
+}
+// Eight values in 4 bits as 16-bit floats, the first in the lowest half.
+__device__ __forceinline__ void fp4_halves(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+// Eight floats to the nearest of 4 bits, as 16-bit floats.  (By way of integers: with the conversion above right behind the one into 4 bits, CUDA 12.9's
+// compiler left zeros.)
+__device__ __forceinline__ uint4 fp4_rounded(const float (&v)[8]) {
+  uint32_t twice[2];
+  fp4_integers(fp4_pack8(v), twice[0], twice[1]);
+  alignas(16) __half2 h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t p0 = __byte_perm(r[4 * i], r[4 * i + 1], 0x5140), p1 = __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x5140);
-    x.w[0].w[i] = __byte_perm(p0, p1, 0x5410);
-    if constexpr (V == 4) {
-      const uint32_t p2 = __byte_perm(r[4 * i], r[4 * i + 1], 0x7362), p3 = __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x7362);
-      x.w[1].w[i] = __byte_perm(p0, p1, 0x7632);
-      x.w[2].w[i] = __byte_perm(p2, p3, 0x5410);
-      x.w[3].w[i] = __byte_perm(p2, p3, 0x7632);
-    }
+    const int two = static_cast<int>(twice[i / 2] >> (i % 2 * 16));
+    h[i] = __floats2half2_rn(0.5f * static_cast<signed char>(two), 0.5f * static_cast<signed char>(two >> 8));
   }
+  return *reinterpret_cast<const uint4*>(h);
 }
-// Columns n .. n + V - 1 of a lane over the blocks begin, begin + step, .. below end.  `ready` is called when the first weights have been asked for.
-template <int V, int M, class Ready>
-__device__ __forceinline__ void along_columns(const Matrix4& t, int n, int begin, int step, int end, const uint8_t* const (&a)[M], const float* const (&f)[M], int base, float (&acc)[V][M], Ready&& ready) {
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int m = 0; m < M; ++m) acc[j][m] = 0.f;
-  Weights4 next;
-  if (begin < end) load_columns<V>(next, t, n, begin);
-  ready();
-  for (int b = begin; b < end; b += step) {
-    const Weights4 now = next;
-    if (b + step < end) load_columns<V>(next, t, n, b + step);
-    const uint8_t* at[M];
-    float g[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      at[m] = a[m] + (b - base) * 32;
-      g[m] = f[m][b - base];
-    }
-    add_block<M, V>(now, at, g, acc);
-  }
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NC: columns [n0, n0 + columns), blocks [begin, end).  Lanes go along the blocks, 4 to 32 of them; those that are left have other columns, four at a time.
-// emit(column, row, sum) by the lanes that have the sums.
-template <int M, class Ready, class Emit>
-__device__ __forceinline__ void along_rows(const Matrix4& t, int n0, int columns, int begin, int end, const uint8_t* const (&a)[M], const float* const (&f)[M], int base, Ready&& ready, Emit&& emit) {
-  int log2 = 2;
-  while (log2 < 5 && (1 << log2) < end - begin) ++log2;
-  const int lane = threadIdx.x & 31, along = lane & ((1 << log2) - 1), group = lane >> log2, groups = 32 >> log2;
-  Weights4 next;
-  auto load = [&](int first, int b) {
-#pragma unroll
-    for (int j = 0; j < kColumns; ++j) {
-      const int n = n0 + first + j * groups + group;
-      const bool there = first + j * groups < columns && n < t.N && b < end;
-      next.w[j] = there ? load_block(t.w + static_cast<unsigned long long>(n) * t.row, b, t.C) : Block4{};
-      next.s[j] = there ? t.s[static_cast<unsigned long long>(n) * t.s_row + b] : 0u;
-    }
-  };
-  int first = 0, b = begin + along;            // of the weights that come next
-  load(first, b);
-  ready();
-  while (first < columns) {
-    float acc[kColumns][M];
-#pragma unroll
-    for (int j = 0; j < kColumns; ++j)
-#pragma unroll
-      for (int m = 0; m < M; ++m) acc[j][m] = 0.f;
-    const int now_first = first;
-    for (int steps = max(1, (end - begin + (1 << log2) - 1) >> log2); steps; --steps) {
-      const Weights4 now = next;
-      const int at_block = max(min(b, end - 1) - base, 0);
-      const bool on = b < end;
-      b += 1 << log2;
-      if (steps == 1) {
-        first += kColumns * groups;
-        b = begin + along;
-      }
-      if (first < columns) load(first, b);
-      const uint8_t* at[M];
-      float g[M];
-#pragma unroll
-      for (int m = 0; m < M; ++m) {
-        at[m] = a[m] + at_block * 32;
-        g[m] = on ? f[m][at_block] : 0.f;
-      }
-      add_block<M, kColumns>(now, at, g, acc);
-    }
-    for (int o = 1; o < 1 << log2; o <<= 1)
-#pragma unroll
-      for (int j = 0; j < kColumns; ++j)
-#pragma unroll
-        for (int m = 0; m < M; ++m) acc[j][m] += __shfl_xor_sync(kAll, acc[j][m], o);
-#pragma unroll
-    for (int j = 0; j < kColumns; ++j) {
-      const int c = now_first + j * groups;
-      if (along == 0 && c < columns && n0 + c + group < t.N) {
-#pragma unroll
-        for (int m = 0; m < M; ++m) emit(n0 + c + group, m, acc[j][m]);
-      }
-    }
+template <int LAYOUT>
+struct Stages {
+  uint32_t base;
+  int ask_slot = 0, get_slot = 0;
+  uint32_t late[kStage4];      // scales that are read byte by byte, stored when the next stage is asked for
+  uint32_t late_at = 0;
+  __device__ __forceinline__ explicit Stages(const void* smem) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * kWarpBytes4) {}
+  __device__ __forceinline__ void store_late() {
+    if (late_at == 0) return;
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(late_at), "r"(late[0] | late[1] << 8 | late[2] << 16 | late[3] << 24) : "memory");
+    late_at = 0;
   }
-}
+  // Stage `stage` of columns [n0, n0 + 32) and of `rows` rows; which(m): the m-th one's place.
+  template <class Which>
+  __device__ __forceinline__ void ask(const Matrix4& t, int n0, int stage, const Rows4& x, int rows, Which&& which) {
+    const int lane = threadIdx.x & 31, b0 = stage * kStage4, half = (t.C + 1) / 2;
+    const uint32_t to = base + ask_slot * kStageBytes4;
+    store_late();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (LAYOUT == kNC) {
+        const int col = r * 8 + (lane >> 2), kk = lane & 3, byte = (b0 + kk) * 16, left = n0 + col < t.N ? max(min(half - byte, 16), 0) : 0;
+        copy16(to + (((col & 3) * 8 + (col >> 2)) * 4 + (kk ^ (col >> 3))) * 16, left ? t.w + (n0 + col) * t.row + byte : t.w, left);
+      } else if constexpr (LAYOUT == kCN1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int pair = (b0 + r) * 16 + i;
+          const uint32_t v = pair < half && n0 + lane < t.N ? t.w[pair * t.row + n0 + lane] : 0u;
+          asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (r * 16 + (i & 3) * 4 + (i >> 2)) * 32 + lane), "r"(v) : "memory");
+        }
+      } else {
+        const int i = lane >> 1, pair = (b0 + r) * 16 + i, n = n0 + (lane & 1) * 16, left = pair < half ? max(min(t.N - n, 16), 0) : 0;
+        const uint8_t* from = left ? t.w + pair * t.row + n : t.w;
+        const uint32_t at = to + (r * 16 + (i & 3) * 4 + (i >> 2)) * 32 + (lane & 1) * 16;
+        if constexpr (LAYOUT == kCN16) {
+          copy16(at, from, left);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) copy4(at + 4 * j, j * 4 < left ? from + 4 * j : t.w, max(min(left - j * 4, 4), 0));
+        }
+      }
+    }
+    const int blocks = n0 + lane < t.N ? min(fp4_blocks(t.C) - b0, kStage4) : 0;
+    const uint8_t* scale = blocks ? t.s + (n0 + lane) * t.s_row + b0 : t.s;
+    if (t.words) {
+      copy4(to + kStageScale4 + lane * 4, scale, blocks);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kStage4; ++i) late[i] = i < blocks ? scale[i] : 0;
+      late_at = to + kStageScale4 + lane * 4;
+    }
+    const int blocks_x = fp4_blocks(x.C) - b0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int m = h * 2 + (lane >> 4), piece = lane & 15;
+      if (m < rows) copy16(to + kStageRows4 + m * kRowPitch4 + piece * 16, piece / 4 < blocks_x ? x.row(which(m)) + b0 * kFp4Block + piece * 8 : x.x, piece / 4 < blocks_x ? 16 : 0);
+    }
+    if (lane < rows) copy16(to + kStageF4 + lane * 16, x.scale(which(lane)) + b0, min(blocks_x, kStage4) * 4);
+  }
+  __device__ __forceinline__ void asked() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++ask_slot == kDepth4) ask_slot = 0;
+  }
+  // acc[i]: columns 4 g + i, rows 2 q and 2 q + 1 (of q < 2); f: what the rows' scales are times
+  __device__ __forceinline__ void add(float2 (&acc)[4], int rows, float f0, float f1) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const uint32_t from = base + get_slot * kStageBytes4, powers = base + kDepth4 * kStageBytes4;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth4 - 1) : "memory");
+    __syncwarp();
+    const uint32_t bytes = word_at(from + kStageScale4 + lane * 4);
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(powers + ((lane & 3) * 8 + g) * 16), "f"(fp4_power(bytes & 255u)), "f"(fp4_power(bytes >> 8 & 255u)), "f"(fp4_power(bytes >> 16 & 255u)),
+                 "f"(fp4_power(bytes >> 24)) : "memory");
+    __syncwarp();
+    float s[4][kStage4], f[2][kStage4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = words_at(powers + (i * 8 + g) * 16);
+      s[i][0] = __uint_as_float(v.x); s[i][1] = __uint_as_float(v.y); s[i][2] = __uint_as_float(v.z); s[i][3] = __uint_as_float(v.w);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 v = words_at(from + kStageF4 + ((q & 1) * 2 + i) * 16);
+      const float times = i ? f1 : f0;
+      f[i][0] = __uint_as_float(v.x) * times; f[i][1] = __uint_as_float(v.y) * times; f[i][2] = __uint_as_float(v.z) * times; f[i][3] = __uint_as_float(v.w) * times;
+    }
+#pragma unroll
+    for (int kk = 0; kk < kStage4; ++kk) {
+      uint32_t w[4];
+      if constexpr (LAYOUT == kNC) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = word_at(from + ((i * 8 + g) * 4 + (kk ^ (g >> 1))) * 16 + q * 4);
+      } else {
+        uint32_t r[4];                         // four columns of a pair of elements each: to four pairs of a column each
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = word_at(from + (kk * 16 + i * 4 + q) * 32 + g * 4);
+        const uint32_t p0 = __byte_perm(r[0], r[1], 0x5140), p1 = __byte_perm(r[2], r[3], 0x5140), p2 = __byte_perm(r[0], r[1], 0x7362), p3 = __byte_perm(r[2], r[3], 0x7362);
+        w[0] = __byte_perm(p0, p1, 0x5410);
+        w[1] = __byte_perm(p0, p1, 0x7632);
+        w[2] = __byte_perm(p2, p3, 0x5410);
+        w[3] = __byte_perm(p2, p3, 0x7632);
+      }
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (g < rows) x = words_at(from + kStageRows4 + g * kRowPitch4 + kk * 64 + q * 16);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        uint32_t a[4], b[4];
+        fp4_halves(w[i], a);
+        fp4_halves(w[i + 1], b);
+        float d[4] = {};
+        mma16(d, a[0], b[0], a[1], b[1], x.x, x.y);
+        mma16(d, a[2], b[2], a[3], b[3], x.z, x.w);
+        acc[i].x = fmaf(d[0] * f[0][kk], s[i][kk], acc[i].x);
+        acc[i].y = fmaf(d[1] * f[1][kk], s[i][kk], acc[i].y);
+        acc[i + 1].x = fmaf(d[2] * f[0][kk], s[i + 1][kk], acc[i + 1].x);
+        acc[i + 1].y = fmaf(d[3] * f[1][kk], s[i + 1][kk], acc[i + 1].y);
+      }
+    }
+    __syncwarp();                              // the slot may be asked for anew, the powers written
+    if (++get_slot == kDepth4) get_slot = 0;
+  }
+};
 
-// Eight of a block's 32 values by each of four neighbouring lanes, in 4 bits, as twice their values in bytes; a quarter of the block's scale.
-__device__ __forceinline__ float block4(const float (&v)[8], uint8_t* to) {
+// Eight of a block's 32 values by each of four neighbouring lanes, in 4 bits, as 16-bit floats; the block's scale.
+__device__ __forceinline__ float block4(const float (&v)[8], __half* to) {
   uint32_t top = 0u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -1030,203 +1055,169 @@ __device__ __forceinline__ float block4(const float (&v)[8], uint8_t* to) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = fp4_scaled(v[i], inverse);
-  if (to) {
-    uint2 w;
-    fp4_integers(fp4_pack8(x), w.x, w.y);
-    *reinterpret_cast<uint2*>(to) = w;
-  }
-  return 0.25f * fp4_power(byte);
+  if (to) *reinterpret_cast<uint4*>(to) = fp4_rounded(x);
+  return fp4_power(byte);
 }
 
-constexpr int kUpBlocks = 2 * kUpPart / kFp4Block;       // blocks in shared memory at a time
-template <int LAYOUT>
+// The logits, as few_logits_kernel's, and behind their CTAs those that bring X into 4 bits.
+template <typename T>
+__global__ void __launch_bounds__(128) few_logits4_kernel(const __grid_constant__ LayerParams p, const Rows4 to, int logits_ctas) {
+  pdl_wait();
+  pdl_trigger();
+  const int t0 = blockIdx.y * kRows;
+  if (blockIdx.x < logits_ctas) {
+    logits_by_warps<T>(p, (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2, t0);
+    return;
+  }
+  constexpr int kVec = 16 / sizeof(T);
+  const int blocks = fp4_blocks(p.I), i = (blockIdx.x - logits_ctas) * 128 + threadIdx.x, c = i * 8;
+  float v[kRows][8];
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+    const T* from = static_cast<const T*>(p.X) + min(t0 + m, p.tokens - 1) * p.x_row + c;
+    if (p.x_vectors && c + 8 <= p.I) {
+#pragma unroll
+      for (int h = 0; h < 8 / kVec; ++h) {
+        const Packed<T, kVec> y = reinterpret_cast<const Packed<T, kVec>*>(from)[h];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[m][h * kVec + j] = y.get(j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[m][j] = c + j < p.I ? to_f32<T>(from[j]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+    const bool there = i / 4 < blocks && t0 + m < p.tokens;
+    const float f = block4(v[m], there ? const_cast<__half*>(to.row(t0 + m)) + c : nullptr);
+    if (there && i % 4 == 0) const_cast<float*>(to.scale(t0 + m))[i / 4] = f;
+  }
+}
+
+// Units go round the CTAs: an item's products with a tile of columns, its warps the contraction in turn.  What the warps' sums add up to is activated and, one block of
+// the other product's contraction, brought into 4 bits.
 struct Up4Shared {
   Items items;
-  alignas(16) uint8_t x[kRows][2 * kUpPart];
-  float f[kRows][kUpBlocks];
-  float sums[LAYOUT ? kUpWarps : 1][kRows][LAYOUT ? tile4(LAYOUT) : 1];
+  float sums[2][kWarps4][kRows][kTile4];
 };
-
-// An item's rows of X, blocks [b0, b0 + n), into shared memory; by all threads.
-template <typename T>
-__device__ __noinline__ void stage_rows4(const LayerParams& p, const Item& item, int rows, int b0, int n, uint8_t* x, float* f) {
-  constexpr int kVec = 16 / sizeof(T);
-  __syncthreads();                             // what was in shared memory has been read
-  for (int m = 0; m < rows; ++m) {
-    const T* from = static_cast<const T*>(p.X) + p.by_k.quotient(item.slot[m]) * p.x_row;
-    for (int i0 = 0; i0 < n * 4; i0 += kUpThreads) {       // (whole warps)
-      const int i = i0 + threadIdx.x, c = b0 * 32 + i * 8;
-      const bool there = i < n * 4;
-      float v[8];
-      if (p.x_vectors && there && c + 8 <= p.I) {
-#pragma unroll
-        for (int h = 0; h < 8 / kVec; ++h) {
-          const Packed<T, kVec> y = reinterpret_cast<const Packed<T, kVec>*>(from + c)[h];
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) v[h * kVec + j] = y.get(j);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = there && c + j < p.I ? to_f32<T>(from[c + j]) : 0.f;
-      }
-      const float g = block4(v, there ? x + m * (2 * kUpPart) + i * 8 : nullptr);
-      if (there && i % 4 == 0) f[m * kUpBlocks + i / 4] = g;
-    }
-  }
+template <int LAYOUT>
+__global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_constant__ LayerParams p, const Rows4 x, const Rows4 to) {
+  extern __shared__ __align__(16) uint32_t layer_table[];
+  __shared__ Up4Shared s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_trigger();
+  for (int e = tid; e < p.E; e += kThreads4) s.items.tokens[e] = 0u;
+  for (int i = tid; i < p.tokens * p.k; i += kThreads4) s.items.ids[i] = p.experts[i];
   __syncthreads();
-}
-
-template <typename T, int LAYOUT, int M>
-__device__ __forceinline__ void up4_unit(const LayerParams& p, Up4Shared<LAYOUT>* s, const Item& item, int n0, int begin, int end, float* to) {
-  const int tid = threadIdx.x, warp = tid >> 5;
-  const Matrix4 t{static_cast<const uint8_t*>(p.up) + item.expert * p.up_far, p.up_scale + item.expert * (p.us_row * p.J), static_cast<uint32_t>(p.up_row), static_cast<uint32_t>(p.us_row), (p.I + 1) / 2 * 2, p.J};
-  const uint8_t* a[M];
-  const float* f[M];
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-    a[m] = s->x[m];
-    f[m] = s->f[m];
-  }
-  for (int b0 = begin; b0 < end; b0 += kUpBlocks) {
-    const int b1 = min(end, b0 + kUpBlocks);
-    const bool first = b0 == begin;
-    auto stage = [&]() { stage_rows4<T>(p, item, M, b0, b1 - b0, s->x[0], s->f[0]); };
-    auto put = [&](int col, int m, float v) {
-      if (m >= item.rows || col >= p.J) return;
-      float* o = to + static_cast<long long>(item.slot[m]) * p.J + col;
-      *o = first ? v : *o + v;
-    };
-    if constexpr (LAYOUT == 0) {
-      along_rows<M>(t, n0 + warp * (kTile4 / kUpWarps), kTile4 / kUpWarps, b0, b1, a, f, b0, stage, put);
-    } else {
-      constexpr int kTile = tile4(LAYOUT);
-      const int n = (tid & 31) * LAYOUT;
-      float acc[LAYOUT][M];
-      along_columns<LAYOUT, M>(t, n0 + n, b0 + warp, kUpWarps, b1, a, f, b0, acc, stage);
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int j = 0; j < LAYOUT; ++j) s->sums[warp][m][n + j] = acc[j][m];
-      __syncthreads();
-      for (int i = tid; i < M * kTile; i += kUpThreads) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kUpWarps; ++w) v += s->sums[w][i / kTile][i % kTile];
-        put(n0 + i % kTile, i / kTile, v);
-      }
+  list_items(p, &s.items);
+  publish(p, s.items, 1);
+  const int tiles = p.by_tiles.d, units = s.items.count * tiles, stages = stages_of(p.I);
+  Stages<LAYOUT> ring(layer_table);
+  int coming = blockIdx.x, stage = warp;
+  auto next = [&]() {
+    while (coming < units && stage >= stages) {
+      coming += gridDim.x;
+      stage = warp;
+      if (warp >= stages) break;
     }
-  }
-}
-
-template <typename T, int LAYOUT>
-__global__ void __launch_bounds__(kUpThreads, 2) few_up4_kernel(const __grid_constant__ LayerParams p) {
-  constexpr int kTile = tile4(LAYOUT);
-  extern __shared__ uint32_t layer_table[];
-  __shared__ Up4Shared<LAYOUT> s;
-  const int tiles = p.by_tiles.d, parts = begin_layer<T>(p, &s.items, layer_table, tiles, kFixedRows4 * kTile4 / kTile), all = s.items.count * tiles, blocks = fp4_blocks(p.I), length = (blocks + parts - 1) / parts;
-  bring_down(p, s.items);
-  for (int u = blockIdx.x; u < all * parts; u += gridDim.x) {
-    const int part = u / all, x = u - part * all, i = p.by_tiles.quotient(x), n0 = (x - i * tiles) * kTile, begin = min(blocks, part * length), end = min(blocks, begin + length);
-    const Item item = s.items.item[i];
-    float* to = p.h + static_cast<long long>(part) * p.tokens * p.k * p.J;
-    if (begin == end) {                        // (nothing is left for the last parts of a short contraction)
-      for (int c = threadIdx.x; c < item.rows * kTile; c += kUpThreads)
-        if (n0 + c % kTile < p.J) to[static_cast<long long>(item.slot[c / kTile]) * p.J + n0 + c % kTile] = 0.f;
-    } else if (item.rows == 1) {
-      up4_unit<T, LAYOUT, 1>(p, &s, item, n0, begin, end, to);
-    } else if (item.rows == 2) {
-      up4_unit<T, LAYOUT, 2>(p, &s, item, n0, begin, end, to);
+    if (coming < units && stage < stages) {
+      const int which = p.by_tiles.quotient(coming);
+      const Item& item = s.items.item[which];
+      const Matrix4 t{static_cast<const uint8_t*>(p.up) + item.expert * p.up_far, p.up_scale + item.expert * (p.us_row * p.J), p.up_row, p.us_row, p.I, p.J, p.up_words};
+      ring.ask(t, (coming - which * tiles) * kTile4, stage, x, item.rows, [&](int m) { return p.by_k.quotient(item.slot[m]); });
+      stage += kWarps4;
     } else {
-      up4_unit<T, LAYOUT, kRows>(p, &s, item, n0, begin, end, to);
+      ring.store_late();
     }
-  }
-}
-
-template <int LAYOUT, int M, class Ready>
-__device__ __forceinline__ void down4_item(const LayerParams& p, const Item& item, const uint8_t* act, const float* scale, int pitch, int b0, int b1, int n0, int share, int shares, float* part,
-                                           bool first, Ready&& ready) {
-  constexpr int kTile = tile4(LAYOUT);
-  const Matrix4 t{static_cast<const uint8_t*>(p.down) + item.expert * p.down_far, p.down_scale + item.expert * (p.ds_row * p.I), static_cast<uint32_t>(p.down_row), static_cast<uint32_t>(p.ds_row), (p.J + 1) / 2 * 2, p.I};
-  const uint8_t* a[M];
-  const float* f[M];
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-    a[m] = act + item.slot[m] * pitch * 32;
-    f[m] = scale + item.slot[m] * pitch;
-  }
-  auto put = [&](float* row, int m, float v) {
-    if (m >= item.rows) return;
-    float* o = row + item.slot[m] * kTile;
-    *o = first ? v : *o + v;
+    ring.asked();
   };
-  if constexpr (LAYOUT == 0) {                 // (shares: of the columns)
-    const int columns = kTile / shares;
-    along_rows<M>(t, n0 + share * columns, columns, b0, b1, a, f, b0, ready, [&](int col, int m, float v) { put(part + col - n0, m, v); });
-  } else {                                     // (of the blocks)
-    const int n = (threadIdx.x & 31) * LAYOUT;
-    float acc[LAYOUT][M];
-    along_columns<LAYOUT, M>(t, n0 + n, b0 + share, shares, b1, a, f, b0, acc, ready);
-    float* row = part + share * p.tokens * p.k * kTile + n;
+#pragma unroll 1
+  for (int d = 0; d < kDepth4 - 1; ++d) next();
+  int buffer = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x, buffer ^= 1) {
+    const int which = p.by_tiles.quotient(u), n0 = (u - which * tiles) * kTile4;
+    const Item item = s.items.item[which];
+    float2 acc[4] = {};
+    for (int i = warp; i < stages; i += kWarps4) {
+      next();
+      ring.add(acc, item.rows, 1.f, 1.f);
+    }
+    const int g = lane >> 2, q = lane & 3;
+    if (q < 2) {
+      *reinterpret_cast<float4*>(&s.sums[buffer][warp][2 * q][4 * g]) = make_float4(acc[0].x, acc[1].x, acc[2].x, acc[3].x);
+      *reinterpret_cast<float4*>(&s.sums[buffer][warp][2 * q + 1][4 * g]) = make_float4(acc[0].y, acc[1].y, acc[2].y, acc[3].y);
+    }
+    __syncthreads();                           // (and when all have come here again the other buffer has been read)
+    if (warp < item.rows) {
+      float v = 0.f;
 #pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int j = 0; j < LAYOUT; ++j) put(row + j, m, acc[j][m]);
+      for (int w = 0; w < kWarps4; ++w) v += s.sums[buffer][w][warp][lane];
+      v = n0 + lane < p.J ? v / (1.f + expf(-v)) : 0.f;
+      const uint32_t byte = fp4_scale(__reduce_max_sync(kAll, __float_as_uint(v) & 0x7fffffffu));
+      const float y[8] = {fp4_scaled(v, fp4_inverse(byte))};
+      const_cast<__half*>(to.row(item.slot[warp]))[n0 + lane] = __ushort_as_half(static_cast<unsigned short>(fp4_rounded(y).x));
+      if (lane == 0) const_cast<float*>(to.scale(item.slot[warp]))[n0 / kTile4] = fp4_power(byte);
+    }
   }
 }
 
-// The activations of all slots, blocks [b0, b0 + n), in 4 bits into shared memory; by all threads.
-__device__ __noinline__ void stage_activations4(const LayerParams& p, const DownShared& items, int b0, int n, int room, uint8_t* act, float* scale) {
-  const int slots = p.tokens * p.k, tid = threadIdx.x, all = slots * n * 4;
-  __syncthreads();
-  for (int i0 = 0; i0 < all; i0 += kDownThreads) {       // (whole warps)
-    const int i = min(i0 + tid, all - 1), slot = i / (n * 4), b = i / 4 - slot * n, c = (b0 + b) * 32 + i % 4 * 8;
-    float v[8];
-    activation<8>(p, items.parts, static_cast<long long>(slot) * p.J + c, p.J - c, v);
-    const bool there = i0 + tid < all;
-    const float f = items.weights[slot] * block4(v, there ? act + (slot * room + b) * 32 + i % 4 * 8 : nullptr);
-    if (there && i % 4 == 0) scale[slot * room + b] = f;
-  }
-  __syncthreads();
-}
-
+// A cluster has a tile of the output's columns, its warps the items' stages in turn; each warp adds up the tokens' outputs for itself, then they are joined.
 template <typename T, int LAYOUT>
-__global__ void __launch_bounds__(kDownThreads, 1) few_down4_kernel(const __grid_constant__ LayerParams p) {
-  constexpr int kTile = tile4(LAYOUT);
+__global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_constant__ LayerParams p, const Rows4 x) {
   extern __shared__ __align__(16) float layer_smem[];
   __shared__ DownShared items;
-  if (cluster_size() > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n0 = blockIdx.x / size * kTile4;
+  if (size > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  float* part = layer_smem + kRing4 / 4;       // [warp][token][column]
+  for (int i = tid; i < kWarps4 * p.tokens * kTile4; i += kThreads4) part[i] = 0.f;
   pdl_wait();
   pdl_trigger();
   begin_down(p, &items);
-  const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5;
-  const int n0 = blockIdx.x / size * kTile;
-  float* part = layer_smem + p.act_floats;
-  const int blocks = fp4_blocks(p.J);
-  const int length = (blocks + size - 1) / size, begin = min(blocks, rank * length), end = min(blocks, begin + length);
-  const int room = min(length, p.act_floats / (9 * slots));            // blocks: eight words of bytes and a scale
-  uint8_t* act = reinterpret_cast<uint8_t*>(layer_smem);
-  float* scale = layer_smem + static_cast<long long>(slots) * room * 8;
-  int shares = 1;                              // warps that have an item's columns or blocks apart
-  while (items.count * shares * 2 <= kDownWarps && shares < (LAYOUT ? length : 8)) shares *= 2;
-  for (int b0 = begin; b0 == begin || b0 < end; b0 += room) {
-    const int b1 = min(end, b0 + room);
-    bool staged = false;
-    auto stage = [&]() {
-      if (staged) return;
-      staged = true;
-      stage_activations4(p, items, b0, b1 - b0, room, act, scale);
-    };
-    for (int x = warp; x < items.count * shares; x += kDownWarps) {
-      const Item item = items.item[x / shares];
-      const int share = x % shares;
-      if (item.rows == 1) down4_item<LAYOUT, 1>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
-      else if (item.rows == 2) down4_item<LAYOUT, 2>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
-      else down4_item<LAYOUT, kRows>(p, item, act, scale, room, b0, b1, n0, share, shares, part, b0 == begin, stage);
+  const int stages = stages_of(p.J), all = items.count * stages, step = size * kWarps4;
+  Stages<LAYOUT> ring(layer_smem);
+  int coming = rank * kWarps4 + warp;
+  auto next = [&]() {
+    if (coming < all) {
+      const int which = coming / stages;
+      const Item& item = items.item[which];
+      const Matrix4 t{static_cast<const uint8_t*>(p.down) + item.expert * p.down_far, p.down_scale + item.expert * (p.ds_row * p.I), p.down_row, p.ds_row, p.J, p.I, p.down_words};
+      ring.ask(t, n0, coming - which * stages, x, item.rows, [&](int m) { return static_cast<int>(item.slot[m]); });
+      coming += step;
+    } else {
+      ring.store_late();
     }
-    stage();
+    ring.asked();
+  };
+#pragma unroll 1
+  for (int d = 0; d < kDepth4 - 1; ++d) next();
+  const int g = lane >> 2, q = lane & 3;
+  for (int i = rank * kWarps4 + warp; i < all; i += step) {
+    const Item item = items.item[i / stages];
+    const int slot0 = item.slot[(q & 1) * 2], slot1 = item.slot[(q & 1) * 2 + 1];
+    float2 acc[4] = {};
+    next();
+    ring.add(acc, item.rows, items.weights[slot0], items.weights[slot1]);
+    float4* to = reinterpret_cast<float4*>(part + (warp * p.tokens + p.by_k.quotient(slot0)) * kTile4 + 4 * g);
+    if (q * 2 < item.rows) {
+      const float4 o = *to;
+      *to = make_float4(o.x + acc[0].x, o.y + acc[1].x, o.z + acc[2].x, o.w + acc[3].x);
+    }
+    to = reinterpret_cast<float4*>(part + (warp * p.tokens + p.by_k.quotient(slot1)) * kTile4 + 4 * g);
+    if (q * 2 + 1 < item.rows) {
+      const float4 o = *to;
+      *to = make_float4(o.x + acc[0].y, o.y + acc[1].y, o.z + acc[2].y, o.w + acc[3].y);
+    }
   }
   __syncthreads();
-  put_out<T, kTile>(p, part, part + max(4 * kDownWarps, slots) * kTile, LAYOUT ? shares : 1, n0);
+  put_out<T, kTile4>(p, part + kWarps4 * p.tokens * kTile4, n0, [&](int t, int n, float4& v) {
+#pragma unroll
+    for (int w = 0; w < kWarps4; ++w) {
+      const float4 y = *reinterpret_cast<const float4*>(part + (w * p.tokens + t) * kTile4 + n);
+      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+    }
+  });
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
@@ -1286,22 +1277,69 @@ cudaError_t up_launch(const LayerParams& p, cudaStream_t st) {
 
 bool on(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// An expert's weights of `down` that are brought to the L2 ahead: all, where those of all experts that can be chosen leave half of it to others.
-void ahead(LayerParams* p, long long bytes) {
-  const long long most = p->tokens * p->k < p->E ? p->tokens * p->k : p->E;
-  p->down_bytes = bytes * most <= (64ll << 20) ? static_cast<int>(bytes) : 0;
-  p->pieces = (p->down_bytes + 8191) / 8192;
-  p->by_pieces = Div(p->pieces > 0 ? p->pieces : 1);
+template <typename T>
+void prepare(LayerParams* p) {
+  constexpr int V = 16 / sizeof(T);
+  p->x_vectors = p->I % V == 0 && p->x_row % V == 0 && on(p->X, 16) && on(p->router, 16);
+  p->by_k = Div(p->k);
+  p->by_E4 = Div((p->E + 3) / 4 * 4);
+}
+
+Layout4 layout4(const void* w, bool cn, long long row, long long far) {
+  auto whole = [&](int n) { return row % n == 0 && far % n == 0 && on(w, n); };
+  return !cn ? kNC : whole(16) ? kCN16 : whole(4) ? kCN4 : kCN1;
+}
+template <int LAYOUT>
+cudaError_t up4_launch(const LayerParams& p, const Rows4& x, const Rows4& to, cudaStream_t st) {
+  cudaError_t err = ensure_smem_optin<few_up4_kernel<LAYOUT>>(static_cast<int>(kRing4));
+  if (err != cudaSuccess) return err;
+  count_launch();
+  return launch_kernel(few_up4_kernel<LAYOUT>, dim3(kUpGrid), kThreads4, kRing4, st, true, p, x, to);
+}
+// CTAs of a cluster: as many as two an SM leave room for, a stage for a warp at least.
+template <typename T, int LAYOUT>
+cudaError_t down4_launch(const LayerParams& p, const Rows4& x, cudaStream_t st) {
+  const int tiles = (p.I + kTile4 - 1) / kTile4, turns = p.tokens * p.k * stages_of(p.J);
+  unsigned size = 8;
+  while (size > 1 && (tiles * size > 256 || turns < static_cast<int>(size / 2) * kWarps4)) size /= 2;
+  const size_t smem = kRing4 + static_cast<size_t>(kWarps4 + 1) * p.tokens * kTile4 * sizeof(float);
+  cudaError_t err = ensure_smem_optin<few_down4_kernel<T, LAYOUT>>(static_cast<int>(kRing4 + (kWarps4 + 1) * 32 * kTile4 * sizeof(float)));
+  if (err != cudaSuccess) return err;
+  count_launch();
+  return launch_cluster(few_down4_kernel<T, LAYOUT>, tiles * size, kThreads4, size, smem, st, p, x);
+}
+template <typename T>
+cudaError_t layer4_t(LayerParams p, const egs_route& route, bool up_cn, bool down_cn, const Rows4& x, const Rows4& h, cudaStream_t st) {
+  prepare<T>(&p);
+  const int logits_ctas = (p.E + 7) / 8;
+  count_launch();
+  cudaError_t err = launch_kernel(few_logits4_kernel<T>, dim3(logits_ctas + (fp4_blocks(p.I) + 31) / 32, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p, x, logits_ctas);
+  if (err != cudaSuccess) return err;
+  if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
+  p.by_tiles = Div((p.J + kTile4 - 1) / kTile4);
+  p.up_words = p.us_row % 4 == 0 && on(p.up_scale, 4);
+  p.down_words = p.ds_row % 4 == 0 && on(p.down_scale, 4);
+  switch (layout4(p.up, up_cn, p.up_row, p.up_far)) {
+    case kNC: err = up4_launch<kNC>(p, x, h, st); break;
+    case kCN16: err = up4_launch<kCN16>(p, x, h, st); break;
+    case kCN4: err = up4_launch<kCN4>(p, x, h, st); break;
+    default: err = up4_launch<kCN1>(p, x, h, st);
+  }
+  if (err != cudaSuccess) return err;
+  switch (layout4(p.down, down_cn, p.down_row, p.down_far)) {
+    case kNC: return down4_launch<T, kNC>(p, h, st);
+    case kCN16: return down4_launch<T, kCN16>(p, h, st);
+    case kCN4: return down4_launch<T, kCN4>(p, h, st);
+    default: return down4_launch<T, kCN1>(p, h, st);
+  }
 }
 
 template <typename T>
-cudaError_t layer_t(LayerParams p, const egs_route& route, bool fp4, bool up_cn, bool down_cn, cudaStream_t st) {
+cudaError_t layer_t(LayerParams p, const egs_route& route, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T), kLanes = 8;
-  p.x_vectors = p.I % V == 0 && p.x_row % V == 0 && on(p.X, 16) && on(p.router, 16);
+  prepare<T>(&p);
   // Logits by every cluster for itself where that is little: 64 KB of the router and 64 Ki products for a CTA.
   const long long router = static_cast<long long>(p.E) * p.I;
-  p.by_k = Div(p.k);
-  p.by_E4 = Div((p.E + 3) / 4 * 4);
   p.own_logits = p.tokens <= kUpWarps && router * static_cast<long long>(sizeof(T)) <= (256 << 10) && router * p.tokens <= (256 << 10);
   cudaError_t err = cudaSuccess;
   if (!p.own_logits) {
@@ -1310,23 +1348,9 @@ cudaError_t layer_t(LayerParams p, const egs_route& route, bool fp4, bool up_cn,
     if (err != cudaSuccess) return err;
     if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
   }
-  if (fp4) {
-    // (what lies behind the last row may be nobody's)
-    ahead(&p, down_cn ? p.down_row * ((p.J + 1) / 2 - 1) + p.I / 16 * 16 : p.down_row * (p.I - 1) + (p.J + 1) / 2 / 16 * 16);
-    if (p.down_far % 16 || !on(p.down, 16)) p.pieces = 0;
-    auto fours = [](const void* w, long long row, long long far, int N) { return row % 4 == 0 && far % 4 == 0 && N % 4 == 0 && on(w, 4); };
-    const int up = !up_cn ? 0 : fours(p.up, p.up_row, p.up_far, p.J) ? 4 : 1, down = !down_cn ? 0 : fours(p.down, p.down_row, p.down_far, p.I) ? 4 : 1;
-    p.by_tiles = Div((p.J + tile4(up) - 1) / tile4(up));
-    err = up == 0 ? up_launch<few_up4_kernel<T, 0>>(p, st) : up == 4 ? up_launch<few_up4_kernel<T, 4>>(p, st) : up_launch<few_up4_kernel<T, 1>>(p, st);
-    if (err != cudaSuccess) return err;
-    return down == 0 ? down_launch<few_down4_kernel<T, 0>, T>(p, tile4(0), st) : down == 4 ? down_launch<few_down4_kernel<T, 4>, T>(p, tile4(4), st) : down_launch<few_down4_kernel<T, 1>, T>(p, tile4(1), st);
-  }
   // (one width for both: the parts of `up` are counted by it)
   const bool wide = p.I % V == 0 && p.J % V == 0 && on(p.up, 16) && on(p.down, 16);
   if (wide) {
-    const long long bytes = static_cast<long long>(p.I) * p.J * sizeof(T);
-    p.down_far = bytes;
-    ahead(&p, bytes);
     p.by_tiles = Div((p.J + V * kLanes - 1) / (V * kLanes));
     p.ring_words = static_cast<int>(ring_bytes(kUpThreads, kUpDepth) / 4);
     if ((err = up_launch<few_up_kernel<T, V, kLanes>>(p, st)) != cudaSuccess) return err;
@@ -1340,9 +1364,18 @@ cudaError_t layer_t(LayerParams p, const egs_route& route, bool fp4, bool up_cn,
 
 }  // namespace
 
-size_t few_layer_workspace(const egs_route& r, long long J) {
-  const size_t logits = (static_cast<size_t>(r.tokens) * r.E + 3) / 4 * 4;
-  return sizeof(LayerList) + (logits + static_cast<size_t>(kMostParts) * r.tokens * r.top_k * J) * sizeof(float);
+namespace {
+size_t logits_words(const egs_route& r) { return (static_cast<size_t>(r.tokens) * r.E + 3) / 4 * 4; }
+size_t rows4_bytes(long long rows, int C) { return static_cast<size_t>(rows) * (fp4_blocks(C) * 64 + stages_of(C) * 16); }
+Rows4 rows4_at(void* from, long long rows, int C) {
+  return {static_cast<__half*>(from), reinterpret_cast<float*>(static_cast<char*>(from) + static_cast<size_t>(rows) * fp4_blocks(C) * 64), C};
+}
+}  // namespace
+
+size_t few_layer_workspace(const egs_route& r, int I, int J) {
+  const long long slots = static_cast<long long>(r.tokens) * r.top_k;
+  const size_t parts = static_cast<size_t>(kMostParts) * slots * J * sizeof(float), fp4 = rows4_bytes(r.tokens, I) + rows4_bytes(slots, J);
+  return sizeof(LayerList) + logits_words(r) * sizeof(float) + (parts > fp4 ? parts : fp4);
 }
 
 cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st) {
@@ -1351,15 +1384,20 @@ cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, v
   p.out = f.out; p.weights = f.weights; p.experts = f.experts;
   p.list = static_cast<LayerList*>(workspace);
   p.logits = reinterpret_cast<float*>(p.list + 1);
-  p.h = p.logits + (static_cast<size_t>(r.tokens) * r.E + 3) / 4 * 4;
+  p.h = p.logits + logits_words(r);
   p.x_row = f.x_row;
   p.tokens = static_cast<int>(r.tokens); p.E = r.E; p.k = r.top_k; p.I = f.I; p.J = f.J;
   p.bias = f.bias; p.groups = r.groups; p.top_groups = r.top_groups; p.group_top = r.group_top;
   p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
-  const bool fp4 = f.up_scale != nullptr;
-  p.up_row = fp4 ? f.up_row : p.J; p.us_row = f.us_row; p.down_row = fp4 ? f.down_row : p.I; p.ds_row = f.ds_row;
-  p.up_far = f.up_far; p.down_far = f.down_far;
-  return dtype == EGS_F16 ? layer_t<__half>(p, r, fp4, f.up_cn, f.down_cn, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, r, fp4, f.up_cn, f.down_cn, st) : layer_t<float>(p, r, fp4, f.up_cn, f.down_cn, st);
+  if (f.up_scale) {
+    p.up_row = f.up_row; p.us_row = f.us_row; p.down_row = f.down_row; p.ds_row = f.ds_row;
+    p.up_far = f.up_far; p.down_far = f.down_far;
+    const Rows4 x = rows4_at(p.h, r.tokens, f.I), h = rows4_at(reinterpret_cast<char*>(p.h) + rows4_bytes(r.tokens, f.I), static_cast<long long>(p.tokens) * p.k, f.J);
+    return dtype == EGS_F16 ? layer4_t<__half>(p, r, f.up_cn, f.down_cn, x, h, st) : dtype == EGS_BF16 ? layer4_t<__nv_bfloat16>(p, r, f.up_cn, f.down_cn, x, h, st) : layer4_t<float>(p, r, f.up_cn, f.down_cn, x, h, st);
+  }
+  p.up_row = p.J;
+  p.down_row = p.I;
+  return dtype == EGS_F16 ? layer_t<__half>(p, r, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, r, st) : layer_t<float>(p, r, st);
 }
 
 }  // namespace egs
