@@ -916,9 +916,9 @@ __device__ __forceinline__ uint4 fp4_rounded(const float (&v)[8]) {
   }
   return *reinterpret_cast<const uint4*>(h);
 }
-__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 template <int LAYOUT>
@@ -927,7 +927,13 @@ struct Stages {
   int ask_slot = 0, get_slot = 0;
   uint32_t late[kStage4];      // scales that are read byte by byte, stored when the next stage is asked for
   uint32_t late_at = 0;
-  __device__ __forceinline__ explicit Stages(const void* smem) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * kWarpBytes4) {}
+  uint32_t own;                // where this lane's first piece of a stage goes
+  long long lane_offset;       // ... and comes from
+  __device__ __forceinline__ Stages(const void* smem, long long row) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * kWarpBytes4) {
+    const int lane = threadIdx.x & 31, i = lane >> 1, col = lane >> 2;
+    own = LAYOUT == kNC ? (((col & 3) * 8 + (col >> 2)) * 4) * 16 : ((i & 3) * 4 + (i >> 2)) * 32 + (lane & 1) * 16;
+    lane_offset = LAYOUT == kNC ? col * row + (lane & 3) * 16 : i * row + (lane & 1) * 16;
+  }
   __device__ __forceinline__ void store_late() {
     if (late_at == 0) return;
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(late_at), "r"(late[0] | late[1] << 8 | late[2] << 16 | late[3] << 24) : "memory");
@@ -939,27 +945,41 @@ struct Stages {
     const int lane = threadIdx.x & 31, b0 = stage * kStage4, half = (t.C + 1) / 2;
     const uint32_t to = base + ask_slot * kStageBytes4;
     store_late();
+    const bool whole = (b0 + kStage4) * 16 <= half && n0 + kTile4 <= t.N;
+    if constexpr (LAYOUT == kNC) {
+      const uint8_t* from = t.w + n0 * t.row + b0 * 16 + lane_offset;
+      const int left = half - (b0 + (lane & 3)) * 16;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (LAYOUT == kNC) {
-        const int col = r * 8 + (lane >> 2), kk = lane & 3, byte = (b0 + kk) * 16, left = n0 + col < t.N ? max(min(half - byte, 16), 0) : 0;
-        copy16(to + (((col & 3) * 8 + (col >> 2)) * 4 + (kk ^ (col >> 3))) * 16, left ? t.w + (n0 + col) * t.row + byte : t.w, left);
-      } else if constexpr (LAYOUT == kCN1) {
+      for (int r = 0; r < 4; ++r, from += 8 * t.row) {
+        const uint32_t at = to + own + r * 128 + (((lane & 3) ^ r) << 4);       // column c = 8 r + lane / 4 to the place (c % 4, c / 4), its pieces in turns
+        if (whole) {
+          copy16(at, from, 16);
+        } else {
+          const int bytes = n0 + r * 8 + (lane >> 2) < t.N ? max(min(left, 16), 0) : 0;
+          copy16(at, bytes ? from : t.w, bytes);
+        }
+      }
+    } else if constexpr (LAYOUT == kCN1) {
+#pragma unroll 1
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int pair = (b0 + r) * 16 + i;
           const uint32_t v = pair < half && n0 + lane < t.N ? t.w[pair * t.row + n0 + lane] : 0u;
           asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (r * 16 + (i & 3) * 4 + (i >> 2)) * 32 + lane), "r"(v) : "memory");
         }
-      } else {
-        const int i = lane >> 1, pair = (b0 + r) * 16 + i, n = n0 + (lane & 1) * 16, left = pair < half ? max(min(t.N - n, 16), 0) : 0;
-        const uint8_t* from = left ? t.w + pair * t.row + n : t.w;
-        const uint32_t at = to + (r * 16 + (i & 3) * 4 + (i >> 2)) * 32 + (lane & 1) * 16;
+    } else {
+      const uint8_t* from = t.w + b0 * 16 * t.row + n0 + lane_offset;
+      const int left = t.N - n0 - (lane & 1) * 16;
+#pragma unroll
+      for (int r = 0; r < 4; ++r, from += 16 * t.row) {
+        const uint32_t at = to + own + r * 512;
+        const int bytes = whole ? 16 : (b0 + r) * 16 + (lane >> 1) < half ? max(min(left, 16), 0) : 0;
         if constexpr (LAYOUT == kCN16) {
-          copy16(at, from, left);
+          copy16(at, bytes ? from : t.w, bytes);
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) copy4(at + 4 * j, j * 4 < left ? from + 4 * j : t.w, max(min(left - j * 4, 4), 0));
+          for (int j = 0; j < 4; ++j) copy4(at + 4 * j, j * 4 < bytes ? from + 4 * j : t.w, max(min(bytes - j * 4, 4), 0));
         }
       }
     }
@@ -1029,9 +1049,9 @@ struct Stages {
         uint32_t a[4], b[4];
         fp4_halves(w[i], a);
         fp4_halves(w[i + 1], b);
-        float d[4] = {};
-        mma16(d, a[0], b[0], a[1], b[1], x.x, x.y);
-        mma16(d, a[2], b[2], a[3], b[3], x.z, x.w);
+        float d[4];
+        mma16(d, a[0], b[0], a[1], b[1], x.x, x.y, 0.f, 0.f, 0.f, 0.f);
+        mma16(d, a[2], b[2], a[3], b[3], x.z, x.w, d[0], d[1], d[2], d[3]);
         acc[i].x = fmaf(d[0] * f[0][kk], s[i][kk], acc[i].x);
         acc[i].y = fmaf(d[1] * f[1][kk], s[i][kk], acc[i].y);
         acc[i + 1].x = fmaf(d[2] * f[0][kk], s[i + 1][kk], acc[i + 1].x);
@@ -1114,7 +1134,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_cons
   list_items(p, &s.items);
   publish(p, s.items, 1);
   const int tiles = p.by_tiles.d, units = s.items.count * tiles, stages = stages_of(p.I);
-  Stages<LAYOUT> ring(layer_table);
+  Stages<LAYOUT> ring(layer_table, p.up_row);
   int coming = blockIdx.x, stage = warp;
   auto next = [&]() {
     while (coming < units && stage >= stages) {
@@ -1176,7 +1196,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
   pdl_trigger();
   begin_down(p, &items);
   const int stages = stages_of(p.J), all = items.count * stages, step = size * kWarps4;
-  Stages<LAYOUT> ring(layer_smem);
+  Stages<LAYOUT> ring(layer_smem, p.down_row);
   int coming = rank * kWarps4 + warp;
   auto next = [&]() {
     if (coming < all) {
