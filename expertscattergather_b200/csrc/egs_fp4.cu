@@ -8,7 +8,7 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 
 // ------------------------------------------------------------------------------------------------
-// Rows into 4 bits.  A lane has eight neighbours, four lanes a block, 2^lanes_log2 lanes a row's stretch (short rows share a warp), four such
+// Rows into 4 bits.  A lane has eight neighbours, four lanes a block, 2^lanes_log2 lanes a row's stretch (short rows share a warp), up to four such
 // stretches at a time, whose loads go out together.
 // ------------------------------------------------------------------------------------------------
 constexpr int kToWarps = 8, kToAhead = 4;
@@ -21,42 +21,53 @@ struct ToFp4 {
   int C, chunks, lanes_log2;      // chunks: of eight elements, whole blocks
 };
 
-// V: elements that are loaded together
-template <typename T, int V, bool SILU>
+// V: elements that are loaded together; AHEAD: stretches whose loads go out together
+template <typename T, int V, bool SILU, int AHEAD>
 __global__ void __launch_bounds__(kToWarps * 32) to_fp4_kernel(const __grid_constant__ ToFp4 p) {
   using P = Packed<T, V>;
+  union Eight {
+    P packs[8 / V];
+    T each[8];
+    uint32_t words[2 * sizeof(T)];
+    __device__ Eight() {}
+  };
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = 1 << p.lanes_log2;
   const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> p.lanes_log2) + (lane >> p.lanes_log2);
-  const int first = blockIdx.y * lanes * kToAhead + (lane & (lanes - 1));
+  const int first = blockIdx.y * lanes * AHEAD + (lane & (lanes - 1));
   const bool on = row < p.rows;
   const T* x = static_cast<const T*>(p.X) + row * p.x_stride;
-  P y[kToAhead][8 / V];
-  float v[kToAhead][8];
+  Eight y[AHEAD];
 #pragma unroll
-  for (int u = 0; u < kToAhead; ++u) {
+  for (int u = 0; u < AHEAD; ++u) {
     const int c = (first + u * lanes) * 8;
     if (on && c + 8 <= p.C) {
 #pragma unroll
-      for (int i = 0; i < 8 / V; ++i) y[u][i] = reinterpret_cast<const P*>(x + c)[i];
+      for (int i = 0; i < 8 / V; ++i) y[u].packs[i] = reinterpret_cast<const P*>(x + c)[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = on && c + i < p.C ? to_f32<T>(x[c + i]) : 0.f;
+      for (int i = 0; i < 8; ++i) y[u].each[i] = on && c + i < p.C ? x[c + i] : from_f32<T>(0.f);
     }
   }
 #pragma unroll
-  for (int u = 0; u < kToAhead; ++u) {
+  for (int u = 0; u < AHEAD; ++u) {
     const int chunk = first + u * lanes;
-    if (on && chunk * 8 + 8 <= p.C) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = y[u][i / V].get(i % V);
-    }
-    uint32_t top = 0u;
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if constexpr (SILU) v[u][i] = silu_exact(v[u][i]);
-      top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
+      v[i] = to_f32<T>(y[u].each[i]);
+      if constexpr (SILU) v[i] = silu_exact(v[i]);
+    }
+    uint32_t top = 0u;
+    if constexpr (!SILU && sizeof(T) == 2) {   // 16-bit magnitudes in pairs
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = __vmaxu2(top, y[u].words[i] & 0x7fff7fffu);
+      const unsigned short most = static_cast<unsigned short>(max(top >> 16, top & 0xffffu));
+      top = __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&most)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     }
     top = max(top, __shfl_xor_sync(kAll, top, 1));
     top = max(top, __shfl_xor_sync(kAll, top, 2));
@@ -64,19 +75,24 @@ __global__ void __launch_bounds__(kToWarps * 32) to_fp4_kernel(const __grid_cons
     const uint32_t byte = fp4_scale(top);
     const float inverse = fp4_inverse(byte);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[u][i] = fp4_scaled(v[u][i], inverse);
-    *reinterpret_cast<uint32_t*>(p.q + row * p.q_stride + chunk * 4ll) = fp4_pack8(v[u]);
+    for (int i = 0; i < 8; ++i) v[i] *= inverse;
+    const uint32_t q = fp4_pack8(v);
+    *reinterpret_cast<uint32_t*>(p.q + row * p.q_stride + chunk * 4ll) = inverse == 0.f ? 0u : q;
     if (!(chunk & 3)) p.scale[row * p.s_stride + (chunk >> 2)] = static_cast<uint8_t>(byte);
   }
 }
 
 template <typename T, int V>
 cudaError_t to_fp4_v(const ToFp4& p, int act, cudaStream_t st) {
-  const long long per_cta = kToWarps * (32 >> p.lanes_log2);
-  const int stretch = kToAhead << p.lanes_log2;
-  const dim3 grid(static_cast<unsigned>((p.rows + per_cta - 1) / per_cta), (p.chunks + stretch - 1) / stretch);
-  return act == EGS_ACT_SILU ? launch_kernel(to_fp4_kernel<T, V, true>, grid, kToWarps * 32, 0, st, true, p)
-                             : launch_kernel(to_fp4_kernel<T, V, false>, grid, kToWarps * 32, 0, st, true, p);
+  const long long per_cta = kToWarps * (32 >> p.lanes_log2), ctas = (p.rows + per_cta - 1) / per_cta;
+  auto go = [&](auto kernel, int ahead) {
+    const int stretch = ahead << p.lanes_log2;
+    return launch_kernel(kernel, dim3(static_cast<unsigned>(ctas), (p.chunks + stretch - 1) / stretch), kToWarps * 32, 0, st, true, p);
+  };
+  // Few rows: a stretch a CTA, so that all SMs have some (1003 x 1030 with SiLU, and back: 8.8 us, with four of them 13.7).
+  const bool spread = ctas * ((p.chunks >> p.lanes_log2) + 3) / 4 < 148 * 4;
+  if (act == EGS_ACT_SILU) return spread ? go(to_fp4_kernel<T, V, true, 1>, 1) : go(to_fp4_kernel<T, V, true, kToAhead>, kToAhead);
+  return spread ? go(to_fp4_kernel<T, V, false, 1>, 1) : go(to_fp4_kernel<T, V, false, kToAhead>, kToAhead);
 }
 template <typename T>
 cudaError_t to_fp4_t(const ToFp4& p, int act, cudaStream_t st) {
@@ -88,56 +104,100 @@ cudaError_t to_fp4_t(const ToFp4& p, int act, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// What 4 bits stand for.  A thread has V neighbours, as many as rows of the output begin on.
+// What 4 bits stand for.  A lane has V neighbours, as many as rows of the output begin on, so that a warp's stores are of whole lines; lanes and stretches as above.
 // ------------------------------------------------------------------------------------------------
 struct FromFp4 {
   const uint8_t* q;
   const uint8_t* scale;
   void* X;
   long long q_stride, s_stride, rows;
-  int C;
+  int C, chunks, lanes_log2;      // chunks: of V elements
 };
+// V / 2 pairs to where V elements begin on (16 bytes at most).
+template <typename T, int V>
+__device__ __forceinline__ void store_pairs(T* to, const float2 (&f)[V / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 2) *reinterpret_cast<float2*>(to) = f[0];
+    else
+#pragma unroll
+      for (int i = 0; i < V / 2; i += 2) reinterpret_cast<float4*>(to)[i / 2] = make_float4(f[i].x, f[i].y, f[i + 1].x, f[i + 1].y);
+  } else {
+    uint32_t o[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(f[i].x, f[i].y);
+        o[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[i].x, f[i].y);
+        o[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    if constexpr (V == 2) *reinterpret_cast<uint32_t*>(to) = o[0];
+    else *reinterpret_cast<uint4*>(to) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+__host__ __device__ constexpr int from_ahead(int V) { return V == 8 ? 4 : 8; }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) from_fp4_kernel(const __grid_constant__ FromFp4 p) {
+__global__ void __launch_bounds__(kToWarps * 32) from_fp4_kernel(const __grid_constant__ FromFp4 p) {
+  using Q = typename std::conditional<V == 8, uint32_t, uint8_t>::type;
+  constexpr int kAhead = from_ahead(V);
   pdl_wait();
   pdl_trigger();
-  const int per_row = p.C / V;
-  const long long all = p.rows * per_row;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * 256) {
-    const long long row = i / per_row;
-    const int c = static_cast<int>(i - row * per_row) * V;
-    const float power = fp4_power(p.scale[row * p.s_stride + c / kFp4Block]) * 0.5f;
-    const uint8_t* q = p.q + row * p.q_stride + c / 2;
-    uint32_t w = 0u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = 1 << p.lanes_log2;
+  const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> p.lanes_log2) + (lane >> p.lanes_log2);
+  if (row >= p.rows) return;
+  const uint8_t *q = p.q + row * p.q_stride, *scale = p.scale + row * p.s_stride;
+  T* x = static_cast<T*>(p.X) + row * p.C;
+  for (int first = blockIdx.y * lanes * kAhead + (lane & (lanes - 1)); first < p.chunks; first += gridDim.y * lanes * kAhead) {
+    uint32_t w[kAhead], s[kAhead];
 #pragma unroll
-    for (int b = 0; b < (V + 1) / 2; ++b) w |= static_cast<uint32_t>(q[b]) << (8 * b);
-    if (V == 1 && (c & 1)) w >>= 4;
-    uint32_t n[2];
-    fp4_integers(w, n[0], n[1]);
-    T out[V];
+    for (int u = 0; u < kAhead; ++u) {
+      const int c = (first + u * lanes) * V;
+      w[u] = c < p.C ? *reinterpret_cast<const Q*>(q + c / 2) : 0u;
+      s[u] = c < p.C ? scale[c / kFp4Block] : 0u;
+    }
 #pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = from_f32<T>(static_cast<float>(static_cast<int8_t>(n[v / 4] >> (8 * (v % 4)))) * power);
-    T* x = static_cast<T*>(p.X) + row * p.C + c;
-    if constexpr (V == 8 && sizeof(T) == 2) {
-      uint32_t o[4];
+    for (int u = 0; u < kAhead; ++u) {
+      const int c = (first + u * lanes) * V;
+      if (c >= p.C) break;
+      const float power = fp4_power(s[u]);
+      if constexpr (V == 8) {
+        uint32_t h[4];
+        fp4_halves(w[u], h);
+        float2 f[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) o[v] = static_cast<uint32_t>(*reinterpret_cast<unsigned short*>(&out[2 * v])) | static_cast<uint32_t>(*reinterpret_cast<unsigned short*>(&out[2 * v + 1])) << 16;
-      *reinterpret_cast<uint4*>(x) = make_uint4(o[0], o[1], o[2], o[3]);
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = out[v];
+        for (int i = 0; i < 4; ++i) {
+          f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+          f[i].x *= power;
+          f[i].y *= power;
+        }
+        store_pairs<T, 8>(x + c, f);
+      } else {
+        const float even = fp4_value(w[u]) * power, odd = fp4_value(w[u] >> 4) * power;
+        if constexpr (V == 1) {
+          x[c] = from_f32<T>(c & 1 ? odd : even);
+        } else {
+          const float2 f[1] = {make_float2(even, odd)};
+          store_pairs<T, 2>(x + c, f);
+        }
+      }
     }
   }
 }
 template <typename T>
-cudaError_t from_fp4_t(const FromFp4& p, cudaStream_t st) {
+cudaError_t from_fp4_t(FromFp4 p, cudaStream_t st) {
   auto go = [&](auto kernel, int v) {
-    const long long ctas = (p.rows * (p.C / v) + 255) / 256;
-    return launch_kernel(kernel, static_cast<unsigned>(ctas < 148 * 64 ? ctas : 148 * 64), 256, 0, st, true, p);
+    p.chunks = (p.C + v - 1) / v;
+    p.lanes_log2 = 0;
+    while (p.lanes_log2 < 5 && (1 << p.lanes_log2) < p.chunks) ++p.lanes_log2;
+    const long long per_cta = kToWarps * (32 >> p.lanes_log2);
+    const int stretch = from_ahead(v) << p.lanes_log2, stretches = (p.chunks + stretch - 1) / stretch;
+    return launch_kernel(kernel, dim3(static_cast<unsigned>((p.rows + per_cta - 1) / per_cta), stretches < 65535 ? stretches : 65535), kToWarps * 32, 0, st, true, p);
   };
   if (p.C % 8 == 0 && (reinterpret_cast<uintptr_t>(p.X) & 15u) == 0) return go(from_fp4_kernel<T, 8>, 8);
-  if (p.C % 2 == 0) return go(from_fp4_kernel<T, 2>, 2);
+  if (p.C % 2 == 0 && reinterpret_cast<uintptr_t>(p.X) % (2 * sizeof(T)) == 0) return go(from_fp4_kernel<T, 2>, 2);
   return go(from_fp4_kernel<T, 1>, 1);
 }
 
@@ -263,7 +323,7 @@ cudaError_t launch_quantize_fp4(const void* X, uint8_t* q, uint8_t* scale, long 
 
 cudaError_t launch_dequantize_fp4(const uint8_t* q, const uint8_t* scale, void* X, long long rows, int C, long long q_stride, long long s_stride,
                                   int dtype, cudaStream_t st) {
-  const FromFp4 p{q, scale, X, q_stride, s_stride, rows, C};
+  const FromFp4 p{q, scale, X, q_stride, s_stride, rows, C, 0, 0};
   count_launch();
   return dtype == EGS_F16 ? from_fp4_t<__half>(p, st) : dtype == EGS_BF16 ? from_fp4_t<__nv_bfloat16>(p, st) : from_fp4_t<float>(p, st);
 }

@@ -46,6 +46,16 @@ __device__ __forceinline__ void fp4_integers(uint32_t w, uint32_t& low, uint32_t
   high = __byte_perm(__byte_perm(p0, p1, m >> 16), __byte_perm(n0, n1, m >> 16), 0x3210u + (s >> 16));
 }
 
+// What the lowest 4 bits stand for.
+__device__ __forceinline__ float fp4_value(uint32_t w) { return __uint_as_float((w & 7u) << 22 | (w & 8u) << 28) * 0x1p126f; }
+// Eight values in 4 bits as 16-bit floats, the first in the lowest half.  (Of a word in 32-bit registers: from what the compiler can see to have been bytes, a
+// byte's load or a conversion into 4 bits, CUDA 12.9's leaves zeros.)
+__device__ __forceinline__ void fp4_halves(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+
 struct Block4 {
   uint32_t w[4];
 };

@@ -897,14 +897,7 @@ __device__ __forceinline__ uint4 words_at(uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
   return x;
 }
-// Eight values in 4 bits as 16-bit floats, the first in the lowest half.
-__device__ __forceinline__ void fp4_halves(uint32_t w, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
-}
-// Eight floats to the nearest of 4 bits, as 16-bit floats.  (By way of integers: with the conversion above right behind the one into 4 bits, CUDA 12.9's
-// compiler left zeros.)
+// Eight floats to the nearest of 4 bits, as 16-bit floats.  (By way of integers: see fp4_halves.)
 __device__ __forceinline__ uint4 fp4_rounded(const float (&v)[8]) {
   uint32_t twice[2];
   fp4_integers(fp4_pack8(v), twice[0], twice[1]);
