@@ -1258,7 +1258,7 @@ cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned bl
 // of four leave some SMs unused.
 unsigned cluster_of(int tiles, int J) {
   unsigned size = 8;
-  auto fit = [](unsigned n) { return n == 8 ? 16 : n == 4 ? 32 : 74; };
+  auto fit = [](unsigned n) { return n == 8 ? 15 : n == 4 ? 33 : 74; };
   while (size > 1 && (tiles > fit(size) || J / static_cast<int>(size) < 32)) size /= 2;
   return size;
 }
