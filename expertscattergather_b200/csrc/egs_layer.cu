@@ -1,10 +1,10 @@
 // A whole routed layer for a few tokens: out[t] = sum over j of w[t, j] silu(x[t] up[e]) down[e], e the j-th expert that token t chose.  Its work is
 // reading the weights of the experts that were chosen, each of them once, with all SMs.
 //
-//   choice   where tokens and router are few and small, in `up`: each cluster of CTAs forms the logits, each CTA makes the choice for itself; else two kernels,
-//            the logits, in which a warp has two experts' rows of the router and four tokens, and egs_choice.cu's
+//   choice   two kernels: the logits, a warp two experts' rows of the router and four tokens, and egs_choice.cu's.  (In one kernel with `up`, each CTA
+//            choosing for itself, or in one with each other, by a cluster of eight CTAs, they took 1 to 6 us more.)
 //   up       units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round
-//            the CTAs; float32 sums of parts.
+//            the CTAs; float32 sums of parts
 //   down     a cluster has a tile of the output's columns, its CTAs the contraction in parts; warps have the experts' tokens in turn.  The parts' sums
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
 //            CTAs' in theirs: the same bits in every run.
@@ -17,7 +17,6 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMost = EGS_MAX_FEW_SLOTS, kRows = 4;      // slots; tokens that share a read of the weights
 constexpr int kUpThreads = 256, kUpWarps = kUpThreads / 32, kUpGrid = 296, kUpPart = 1024;
-constexpr int kUpCluster = 4;                // CTAs that form logits together (two SMs: clusters of eight leave SMs of a processing cluster without any)
 constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
 constexpr int kMostParts = 8;
 constexpr int kFixedRows = 128;              // of a unit, in rows of its tile: 16 KB of weights
@@ -42,12 +41,11 @@ struct LayerParams {
   int tokens, E, k, I, J;
   int groups, top_groups, group_top, sigmoid, renormalize;
   float scale;
-  int own_logits;            // `up` forms them
   int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
   bool up_words, down_words; // 4 bits: scales can be read four at a time
   int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
-  Div by_tiles, by_k, by_E4;
+  Div by_tiles, by_k;
 };
 
 // An expert's tokens, up to four at a time.
@@ -127,128 +125,7 @@ __device__ __forceinline__ int parts_of(int units, int length) {
   return best;
 }
 
-// ---- the choice -------------------------------------------------------------------------------------------------------
-// Floats as unsigned numbers of the same order; NaN lies below everything and above 0, which stands for "no candidate".
-__device__ __forceinline__ uint32_t ordered(float x) {
-  x += 0.f;                                    // -0 and 0 are equal
-  const uint32_t b = __float_as_uint(x);
-  return x != x ? 1u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float unordered(uint32_t k) { return k <= 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
-  return v;
-}
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
-  return v;
-}
-
-// The choice as route_tokens_kernel defines it.  A warp forms a token's keys; logits, keys: shared memory.
-struct Softmax {
-  float m, total;
-};
-__device__ __forceinline__ float score_of(const LayerParams& p, const Softmax& soft, float x) {
-  return p.sigmoid ? 1.f / (1.f + expf(-x)) : soft.m == -INFINITY ? 0.f : expf(x - soft.m) / soft.total;
-}
-__device__ __forceinline__ Softmax form_keys(const LayerParams& p, const float* logits, uint32_t* keys, int E4) {
-  const int lane = threadIdx.x & 31;
-  const bool pairs = p.groups > 1 && p.group_top == 2, scores = p.bias || pairs;
-  Softmax soft{0.f, 1.f};
-  if (!p.sigmoid && (scores || !p.renormalize)) {
-    soft.m = -INFINITY;
-    for (int e = lane; e < p.E; e += 32) soft.m = fmaxf(soft.m, logits[e]);
-    soft.m = warp_max(soft.m);
-    soft.total = 0.f;
-    for (int e = lane; e < p.E; e += 32) soft.total += soft.m == -INFINITY ? 0.f : expf(logits[e] - soft.m);
-    soft.total = warp_sum(soft.total);
-  }
-  for (int e = lane; e < E4; e += 32) {
-    const float x = e < p.E ? logits[e] : 0.f;
-    keys[e] = e >= p.E ? 0u : ordered(!scores ? x : p.bias ? score_of(p, soft, x) + p.bias[e] : score_of(p, soft, x));
-  }
-  __syncwarp();
-  if (p.groups > 1) {
-    const int per = p.E / p.groups;
-    uint32_t value = 0u;                       // of lane's group
-    if (lane < p.groups) {
-      uint32_t k1 = 0u, k2 = 0u;
-      for (int i = 0; i < per; ++i) {
-        const uint32_t v = keys[lane * per + i];
-        k2 = max(k2, min(k1, v));
-        k1 = max(k1, v);
-      }
-      value = pairs && k2 ? ordered(unordered(k1) + unordered(k2)) : k1;
-    }
-    unsigned kept = 0u;
-    for (int i = 0; i < p.top_groups; ++i) {
-      const int at = __ffs(__ballot_sync(kAll, value == __reduce_max_sync(kAll, value))) - 1;
-      kept |= 1u << at;
-      if (lane == at) value = 0u;
-    }
-    __syncwarp();
-    for (int e = lane; e < p.E; e += 32) keys[e] = !(kept >> (e / per) & 1u) ? 0u : p.bias ? keys[e] : ordered(logits[e]);
-    __syncwarp();
-  }
-  return soft;
-}
-// Many experts: the k highest keys one after the other, by a warp.
-__device__ __forceinline__ void choose_in_turn(const LayerParams& p, uint32_t* keys, int* ids) {
-  const int lane = threadIdx.x & 31;
-  uint32_t best = 0u;                          // of this lane's experts
-  int who = 0;
-  auto look = [&]() {
-    best = 0u;
-    for (int e = lane; e < p.E; e += 32)
-      if (keys[e] > best) {
-        best = keys[e];
-        who = e;
-      }
-  };
-  look();
-  for (int j = 0; j < p.k; ++j) {
-    const uint32_t top = __reduce_max_sync(kAll, best);
-    const int e = __reduce_min_sync(kAll, best == top && top ? who : 0x7fffffff);
-    if (lane == j) ids[j] = e;
-    if (best == top && who == e) {
-      keys[e] = 0u;
-      look();
-    }
-  }
-}
-// Few: a thread counts the keys before its expert's (equal ones: those of lower experts).
-constexpr int kCounted = 256;
-__device__ __forceinline__ void choose_by_count(const LayerParams& p, const uint32_t* keys, int tokens, int E4, int* ids) {
-  for (int i = threadIdx.x; i < tokens * E4; i += kUpThreads) {
-    const int w = p.by_E4.quotient(i), e = i - w * E4;
-    const uint32_t* row = keys + w * E4;
-    const uint32_t key = row[e];
-    int before = 0;
-#pragma unroll 4
-    for (int j = 0; j < E4; j += 4) {          // (no key is 2^32 - 1, and there are zeros behind the last one)
-      const uint4 other = *reinterpret_cast<const uint4*>(row + j);
-      before += other.x + (j < e) > key;
-      before += other.y + (j + 1 < e) > key;
-      before += other.z + (j + 2 < e) > key;
-      before += other.w + (j + 3 < e) > key;
-    }
-    if (key && before < p.k) ids[w * p.k + before] = e;
-  }
-}
-// A token's weights, lane j < k has the j-th.
-__device__ __forceinline__ float weight_of(const LayerParams& p, const Softmax& soft, const float* logits, const int* ids) {
-  const int lane = threadIdx.x & 31;
-  const bool chosen = lane < p.k;
-  const float x = chosen ? logits[ids[lane]] : -INFINITY;
-  if (!p.renormalize) return score_of(p, soft, x) * p.scale;
-  const float high = p.sigmoid ? 0.f : warp_max(x);
-  const float s = !chosen ? 0.f : p.sigmoid ? score_of(p, soft, x) : high == -INFINITY ? 0.f : expf(x - high);
-  const float sum = warp_sum(s);
-  return (sum == 0.f ? 0.f : s / sum) * p.scale;
-}
-
+// ---- clusters -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int cluster_rank() {
   int r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -348,54 +225,14 @@ __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__
   logits_by_warps<T>(p, (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2, blockIdx.y * kRows);
 }
 
-// What `up` begins with: logits and the choice (or that which is there), the items, the parts; the CTAs of a cluster share the logits.
-// table: 2 * 8 rows of E4 words, logits and keys.  `tiles`: of columns.
-template <typename T>
-__device__ __forceinline__ int begin_layer(const LayerParams& p, Items* s, uint32_t* table, int tiles) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, E4 = p.by_E4.d;
-  float* logits = reinterpret_cast<float*>(table);
-  uint32_t* keys = table + kUpWarps * E4;
-  if (p.own_logits) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+// What both `up` kernels begin with: the items from the choice.
+__device__ __forceinline__ void begin_up(const LayerParams& p, Items* s) {
   pdl_wait();
   pdl_trigger();
-  for (int e = tid; e < p.E; e += kUpThreads) s->tokens[e] = 0u;
-  if (p.own_logits) {
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // all CTAs of the cluster have begun
-    constexpr int kAll8 = kUpCluster * kUpWarps;
-    for (int e = cluster_rank() * kUpWarps + warp; e < p.E; e += 2 * kAll8)
-      logits_of<T>(p, e, e + kAll8, 0, p.tokens, [&](int t, int expert, float v) {
-        if (lane < kUpCluster) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(logits + t * E4 + expert, lane)), "f"(v) : "memory");
-      });
-    cluster_sync();
-  }
-  if (p.own_logits) {
-    const int t = warp;
-    float* row = logits + warp * E4;
-    Softmax soft{};
-    if (t < p.tokens) {
-      soft = form_keys(p, row, keys + warp * E4, E4);
-      if (p.E > kCounted) choose_in_turn(p, keys + warp * E4, s->ids + t * p.k);
-    }
-    __syncthreads();
-    if (p.E <= kCounted) {
-      choose_by_count(p, keys, p.tokens, E4, s->ids);
-      __syncthreads();
-    }
-    if (blockIdx.x == 0 && t < p.tokens) {
-      const float w = weight_of(p, soft, row, s->ids + t * p.k);
-      if (lane < p.k) {
-        p.weights[t * p.k + lane] = w;
-        p.experts[t * p.k + lane] = s->ids[t * p.k + lane];
-      }
-    }
-  } else {
-    for (int i = tid; i < p.tokens * p.k; i += kUpThreads) s->ids[i] = p.experts[i];
-    __syncthreads();
-  }
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) s->tokens[e] = 0u;
+  for (int i = threadIdx.x; i < p.tokens * p.k; i += blockDim.x) s->ids[i] = p.experts[i];
+  __syncthreads();
   list_items(p, s);
-  const int parts = parts_of(s->count * tiles, p.I);
-  publish(p, *s, parts);
-  return parts;
 }
 
 // ---- products along rows of the weights ([contraction, columns]) -----------------------------------------------------
@@ -609,7 +446,10 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
   constexpr bool kRing = V == 16 / sizeof(T);
   extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ UpShared<T, V, LANES> s;
-  const int parts = begin_layer<T>(p, &s.items, layer_table + p.ring_words, p.by_tiles.d), all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
+  begin_up(p, &s.items);
+  const int parts = parts_of(s.items.count * p.by_tiles.d, p.I);
+  publish(p, s.items, parts);
+  const int all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
   Ring<kUpThreads, kUpDepth> ring(layer_table);
   // what is asked for next: rows c .. c + 3 of unit `coming`
   int coming = blockIdx.x, c = 0, end = 0, left = 0;
@@ -1119,12 +959,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_cons
   extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ Up4Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_wait();
-  pdl_trigger();
-  for (int e = tid; e < p.E; e += kThreads4) s.items.tokens[e] = 0u;
-  for (int i = tid; i < p.tokens * p.k; i += kThreads4) s.items.ids[i] = p.experts[i];
-  __syncthreads();
-  list_items(p, &s.items);
+  begin_up(p, &s.items);
   publish(p, s.items, 1);
   const int tiles = p.by_tiles.d, units = s.items.count * tiles, stages = stages_of(p.I);
   Stages<LAYOUT> ring(layer_table, p.up_row);
@@ -1281,11 +1116,10 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
 
 template <auto kernel>
 cudaError_t up_launch(const LayerParams& p, cudaStream_t st) {
-  constexpr int kMostTable = 2 * kUpWarps * EGS_MAX_EXPERTS * 4 + static_cast<int>(ring_bytes(kUpThreads, kUpDepth));
-  cudaError_t err = ensure_smem_optin<kernel>(kMostTable);
+  cudaError_t err = ensure_smem_optin<kernel>(static_cast<int>(ring_bytes(kUpThreads, kUpDepth)));
   if (err != cudaSuccess) return err;
   count_launch();
-  return launch_cluster(kernel, kUpGrid, kUpThreads, kUpCluster, (p.own_logits ? static_cast<size_t>(2 * kUpWarps) * ((p.E + 3) / 4 * 4) * 4 : 0) + static_cast<size_t>(p.ring_words) * 4, st, p);
+  return launch_kernel(kernel, dim3(kUpGrid), kUpThreads, static_cast<size_t>(p.ring_words) * 4, st, true, p);
 }
 
 bool on(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -1295,7 +1129,6 @@ void prepare(LayerParams* p) {
   constexpr int V = 16 / sizeof(T);
   p->x_vectors = p->I % V == 0 && p->x_row % V == 0 && on(p->X, 16) && on(p->router, 16);
   p->by_k = Div(p->k);
-  p->by_E4 = Div((p->E + 3) / 4 * 4);
 }
 
 Layout4 layout4(const void* w, bool cn, long long row, long long far) {
@@ -1351,16 +1184,10 @@ template <typename T>
 cudaError_t layer_t(LayerParams p, const egs_route& route, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T), kLanes = 8;
   prepare<T>(&p);
-  // Logits by every cluster for itself where that is little: 64 KB of the router and 64 Ki products for a CTA.
-  const long long router = static_cast<long long>(p.E) * p.I;
-  p.own_logits = p.tokens <= kUpWarps && router * static_cast<long long>(sizeof(T)) <= (256 << 10) && router * p.tokens <= (256 << 10);
-  cudaError_t err = cudaSuccess;
-  if (!p.own_logits) {
-    count_launch();
-    err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
-    if (err != cudaSuccess) return err;
-    if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
-  }
+  count_launch();
+  cudaError_t err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
+  if (err != cudaSuccess) return err;
+  if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
   // (one width for both: the parts of `up` are counted by it)
   const bool wide = p.I % V == 0 && p.J % V == 0 && on(p.up, 16) && on(p.down, 16);
   if (wide) {
