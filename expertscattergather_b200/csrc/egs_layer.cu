@@ -42,10 +42,9 @@ struct LayerParams {
   int groups, top_groups, group_top, sigmoid, renormalize;
   float scale;
   int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
-  bool up_words, down_words; // 4 bits: scales can be read four at a time
   int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
-  Div by_tiles, by_k;
+  Div by_tiles, by_k, by_stages;
 };
 
 // An expert's tokens, up to four at a time.
@@ -706,12 +705,14 @@ __host__ __device__ constexpr int stages_of(int C) { return (fp4_blocks(C) + kSt
 enum Layout4 { kNC, kCN16, kCN4, kCN1 };       // CN: rows, counted from the tensor's begin, are whole pieces of so many bytes
 
 struct Matrix4 {
-  const uint8_t *w, *s;        // of an expert
-  long long row;               // NC: bytes from one column to the next, CN: from one pair of contraction elements to the next
-  long long s_row;             // from one column's scales to the next
+  const uint8_t *w, *s;
+  long long far, s_far;        // bytes from one expert to the next
+  uint32_t row;                // NC: from one column to the next, CN: from one pair of contraction elements to the next
+  uint32_t s_row;              // from one column's scales to the next
   int C, N;
   bool words;                  // scales can be read four at a time
 };
+__device__ __forceinline__ unsigned long long wide(uint32_t a, uint32_t b) { return static_cast<unsigned long long>(a) * b; }
 // Rows in 16-bit floats, whole blocks, and their scales, whole stages.
 struct Rows4 {
   __half* x;
@@ -756,89 +757,113 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
 
 template <int LAYOUT>
 struct Stages {
+  const Matrix4& t;
   uint32_t base;
   int ask_slot = 0, get_slot = 0;
   uint32_t late[kStage4];      // scales that are read byte by byte, stored when the next stage is asked for
   uint32_t late_at = 0;
   uint32_t own;                // where this lane's first piece of a stage goes
-  long long lane_offset;       // ... and comes from
-  __device__ __forceinline__ Stages(const void* smem, long long row) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * kWarpBytes4) {
+  // of the unit that is asked for: where this lane's pieces of its first stage are
+  const uint8_t *w, *s;
+  const char *x0, *x1, *f;
+  int n0, rows, whole;         // whole: stages that need no bounds
+
+  __device__ __forceinline__ Stages(const void* smem, const Matrix4& m) : t(m), base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * kWarpBytes4) {
     const int lane = threadIdx.x & 31, i = lane >> 1, col = lane >> 2;
     own = LAYOUT == kNC ? (((col & 3) * 8 + (col >> 2)) * 4) * 16 : ((i & 3) * 4 + (i >> 2)) * 32 + (lane & 1) * 16;
-    lane_offset = LAYOUT == kNC ? col * row + (lane & 3) * 16 : i * row + (lane & 1) * 16;
+  }
+  // Columns [column, column + 32) of an expert and `m` rows; which(i): the i-th one's place in x.
+  template <class Which>
+  __device__ __forceinline__ void begin(int expert, int column, const Rows4& x, int m, Which&& which) {
+    const int lane = threadIdx.x & 31;
+    n0 = column;
+    rows = m;
+    w = t.w + expert * t.far;
+    if constexpr (LAYOUT == kNC) w += wide(n0 + (lane >> 2), t.row) + (lane & 3) * 16;
+    else if constexpr (LAYOUT == kCN1) w += n0 + lane;
+    else w += n0 + (lane & 1) * 16 + wide(lane >> 1, t.row);
+    s = t.s + expert * t.s_far + wide(n0 + lane, t.s_row);
+    const uint32_t pitch = fp4_blocks(x.C) * kFp4Block * 2, piece = (lane & 15) * 16;
+    x0 = reinterpret_cast<const char*>(x.x) + wide(which(lane >> 4), pitch) + piece;
+    x1 = reinterpret_cast<const char*>(x.x) + wide(which(2 + (lane >> 4)), pitch) + piece;
+    f = reinterpret_cast<const char*>(x.f) + wide(which(lane & 3), stages_of(x.C) * kStage4 * 4);
+    whole = t.words && LAYOUT != kCN1 && n0 + kTile4 <= t.N ? (t.C + 1) / 2 / (kStage4 * 16) : 0;
   }
   __device__ __forceinline__ void store_late() {
     if (late_at == 0) return;
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(late_at), "r"(late[0] | late[1] << 8 | late[2] << 16 | late[3] << 24) : "memory");
     late_at = 0;
   }
-  // Stage `stage` of columns [n0, n0 + 32) and of `rows` rows; which(m): the m-th one's place.
-  template <class Which>
-  __device__ __forceinline__ void ask(const Matrix4& t, int n0, int stage, const Rows4& x, int rows, Which&& which) {
-    const int lane = threadIdx.x & 31, b0 = stage * kStage4, half = (t.C + 1) / 2;
+  __device__ __forceinline__ void ask(int stage) {
+    const int lane = threadIdx.x & 31;
     const uint32_t to = base + ask_slot * kStageBytes4;
+    const uint8_t* from = w + (LAYOUT == kNC ? wide(stage, kStage4 * 16) : wide(stage * (kStage4 * 16), t.row));
+    const unsigned long long step = wide(LAYOUT == kNC ? 8 : 16, t.row);
+    const uint32_t x_to = to + kStageRows4 + (lane >> 4) * kRowPitch4 + (lane & 15) * 16, x_from = stage * (kStage4 * kFp4Block * 2);
+    if (stage < whole) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r, from += step) {
+        if constexpr (LAYOUT == kNC) copy16(to + own + r * 128 + (((lane & 3) ^ r) << 4), from, 16);
+        else if constexpr (LAYOUT == kCN16) copy16(to + own + r * 512, from, 16);
+        else
+#pragma unroll
+          for (int j = 0; j < 4; ++j) copy4(to + own + r * 512 + 4 * j, from + 4 * j, 4);
+      }
+      copy4(to + kStageScale4 + lane * 4, s + stage * kStage4, 4);
+      if ((lane >> 4) < rows) copy16(x_to, x0 + x_from, 16);
+      if (2 + (lane >> 4) < rows) copy16(x_to + 2 * kRowPitch4, x1 + x_from, 16);
+      if (lane < rows) copy16(to + kStageF4 + lane * 16, f + stage * (kStage4 * 4), 16);
+      return;
+    }
     store_late();
-    const bool whole = (b0 + kStage4) * 16 <= half && n0 + kTile4 <= t.N;
+    const int b0 = stage * kStage4, half = (t.C + 1) / 2, left_blocks = min(fp4_blocks(t.C) - b0, kStage4);
     if constexpr (LAYOUT == kNC) {
-      const uint8_t* from = t.w + n0 * t.row + b0 * 16 + lane_offset;
       const int left = half - (b0 + (lane & 3)) * 16;
 #pragma unroll
-      for (int r = 0; r < 4; ++r, from += 8 * t.row) {
-        const uint32_t at = to + own + r * 128 + (((lane & 3) ^ r) << 4);       // column c = 8 r + lane / 4 to the place (c % 4, c / 4), its pieces in turns
-        if (whole) {
-          copy16(at, from, 16);
-        } else {
-          const int bytes = n0 + r * 8 + (lane >> 2) < t.N ? max(min(left, 16), 0) : 0;
-          copy16(at, bytes ? from : t.w, bytes);
-        }
+      for (int r = 0; r < 4; ++r, from += step) {       // column c = 8 r + lane / 4 to the place (c % 4, c / 4), its pieces in turns
+        const int bytes = n0 + r * 8 + (lane >> 2) < t.N ? max(min(left, 16), 0) : 0;
+        copy16(to + own + r * 128 + (((lane & 3) ^ r) << 4), bytes ? from : t.w, bytes);
       }
     } else if constexpr (LAYOUT == kCN1) {
 #pragma unroll 1
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int pair = (b0 + r) * 16 + i;
-          const uint32_t v = pair < half && n0 + lane < t.N ? t.w[pair * t.row + n0 + lane] : 0u;
+        for (int i = 0; i < 16; ++i, from += t.row) {
+          const uint32_t v = (b0 + r) * 16 + i < half && n0 + lane < t.N ? *from : 0u;
           asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (r * 16 + (i & 3) * 4 + (i >> 2)) * 32 + lane), "r"(v) : "memory");
         }
     } else {
-      const uint8_t* from = t.w + b0 * 16 * t.row + n0 + lane_offset;
       const int left = t.N - n0 - (lane & 1) * 16;
 #pragma unroll
-      for (int r = 0; r < 4; ++r, from += 16 * t.row) {
-        const uint32_t at = to + own + r * 512;
-        const int bytes = whole ? 16 : (b0 + r) * 16 + (lane >> 1) < half ? max(min(left, 16), 0) : 0;
+      for (int r = 0; r < 4; ++r, from += step) {
+        const int bytes = (b0 + r) * 16 + (lane >> 1) < half ? max(min(left, 16), 0) : 0;
         if constexpr (LAYOUT == kCN16) {
-          copy16(at, bytes ? from : t.w, bytes);
+          copy16(to + own + r * 512, bytes ? from : t.w, bytes);
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) copy4(at + 4 * j, j * 4 < bytes ? from + 4 * j : t.w, max(min(bytes - j * 4, 4), 0));
+          for (int j = 0; j < 4; ++j) copy4(to + own + r * 512 + 4 * j, j * 4 < bytes ? from + 4 * j : t.w, max(min(bytes - j * 4, 4), 0));
         }
       }
     }
-    const int blocks = n0 + lane < t.N ? min(fp4_blocks(t.C) - b0, kStage4) : 0;
-    const uint8_t* scale = blocks ? t.s + (n0 + lane) * t.s_row + b0 : t.s;
+    const int blocks = n0 + lane < t.N ? left_blocks : 0;
     if (t.words) {
-      copy4(to + kStageScale4 + lane * 4, scale, blocks);
+      copy4(to + kStageScale4 + lane * 4, blocks ? s + b0 : t.s, blocks);
     } else {
 #pragma unroll
-      for (int i = 0; i < kStage4; ++i) late[i] = i < blocks ? scale[i] : 0;
+      for (int i = 0; i < kStage4; ++i) late[i] = i < blocks ? s[b0 + i] : 0;
       late_at = to + kStageScale4 + lane * 4;
     }
-    const int blocks_x = fp4_blocks(x.C) - b0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int m = h * 2 + (lane >> 4), piece = lane & 15;
-      if (m < rows) copy16(to + kStageRows4 + m * kRowPitch4 + piece * 16, piece / 4 < blocks_x ? x.row(which(m)) + b0 * kFp4Block + piece * 8 : x.x, piece / 4 < blocks_x ? 16 : 0);
-    }
-    if (lane < rows) copy16(to + kStageF4 + lane * 16, x.scale(which(lane)) + b0, min(blocks_x, kStage4) * 4);
+    const bool there = (lane & 15) / 4 < left_blocks;
+    if ((lane >> 4) < rows) copy16(x_to, there ? x0 + x_from : x0, there ? 16 : 0);
+    if (2 + (lane >> 4) < rows) copy16(x_to + 2 * kRowPitch4, there ? x1 + x_from : x1, there ? 16 : 0);
+    if (lane < rows) copy16(to + kStageF4 + lane * 16, f + b0 * 4, left_blocks * 4);
   }
   __device__ __forceinline__ void asked() {
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (++ask_slot == kDepth4) ask_slot = 0;
   }
-  // acc[i]: columns 4 g + i, rows 2 q and 2 q + 1 (of q < 2); f: what the rows' scales are times
-  __device__ __forceinline__ void add(float2 (&acc)[4], int rows, float f0, float f1) {
+  // acc[i]: columns 4 g + i of `count` rows, 2 q and 2 q + 1 (of q < 2); f0, f1: what those rows' scales are times
+  __device__ __forceinline__ void add(float2 (&acc)[4], int count, float f0, float f1) {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t from = base + get_slot * kStageBytes4, powers = base + kDepth4 * kStageBytes4;
     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth4 - 1) : "memory");
@@ -847,17 +872,17 @@ struct Stages {
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(powers + ((lane & 3) * 8 + g) * 16), "f"(fp4_power(bytes & 255u)), "f"(fp4_power(bytes >> 8 & 255u)), "f"(fp4_power(bytes >> 16 & 255u)),
                  "f"(fp4_power(bytes >> 24)) : "memory");
     __syncwarp();
-    float s[4][kStage4], f[2][kStage4];
+    float power[4][kStage4], scale[2][kStage4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 v = words_at(powers + (i * 8 + g) * 16);
-      s[i][0] = __uint_as_float(v.x); s[i][1] = __uint_as_float(v.y); s[i][2] = __uint_as_float(v.z); s[i][3] = __uint_as_float(v.w);
+      power[i][0] = __uint_as_float(v.x); power[i][1] = __uint_as_float(v.y); power[i][2] = __uint_as_float(v.z); power[i][3] = __uint_as_float(v.w);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint4 v = words_at(from + kStageF4 + ((q & 1) * 2 + i) * 16);
       const float times = i ? f1 : f0;
-      f[i][0] = __uint_as_float(v.x) * times; f[i][1] = __uint_as_float(v.y) * times; f[i][2] = __uint_as_float(v.z) * times; f[i][3] = __uint_as_float(v.w) * times;
+      scale[i][0] = __uint_as_float(v.x) * times; scale[i][1] = __uint_as_float(v.y) * times; scale[i][2] = __uint_as_float(v.z) * times; scale[i][3] = __uint_as_float(v.w) * times;
     }
 #pragma unroll
     for (int kk = 0; kk < kStage4; ++kk) {
@@ -876,7 +901,7 @@ struct Stages {
         w[3] = __byte_perm(p2, p3, 0x7632);
       }
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (g < rows) x = words_at(from + kStageRows4 + g * kRowPitch4 + kk * 64 + q * 16);
+      if (g < count) x = words_at(from + kStageRows4 + g * kRowPitch4 + kk * 64 + q * 16);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         uint32_t a[4], b[4];
@@ -885,10 +910,10 @@ struct Stages {
         float d[4];
         mma16(d, a[0], b[0], a[1], b[1], x.x, x.y, 0.f, 0.f, 0.f, 0.f);
         mma16(d, a[2], b[2], a[3], b[3], x.z, x.w, d[0], d[1], d[2], d[3]);
-        acc[i].x = fmaf(d[0] * f[0][kk], s[i][kk], acc[i].x);
-        acc[i].y = fmaf(d[1] * f[1][kk], s[i][kk], acc[i].y);
-        acc[i + 1].x = fmaf(d[2] * f[0][kk], s[i + 1][kk], acc[i + 1].x);
-        acc[i + 1].y = fmaf(d[3] * f[1][kk], s[i + 1][kk], acc[i + 1].y);
+        acc[i].x = fmaf(d[0] * scale[0][kk], power[i][kk], acc[i].x);
+        acc[i].y = fmaf(d[1] * scale[1][kk], power[i][kk], acc[i].y);
+        acc[i + 1].x = fmaf(d[2] * scale[0][kk], power[i + 1][kk], acc[i + 1].x);
+        acc[i + 1].y = fmaf(d[3] * scale[1][kk], power[i + 1][kk], acc[i + 1].y);
       }
     }
     __syncwarp();                              // the slot may be asked for anew, the powers written
@@ -955,26 +980,25 @@ struct Up4Shared {
   float sums[2][kWarps4][kRows][kTile4];
 };
 template <int LAYOUT>
-__global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_constant__ LayerParams p, const Rows4 x, const Rows4 to) {
+__global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_constant__ LayerParams p, const __grid_constant__ Matrix4 t, const Rows4 x, const Rows4 to) {
   extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ Up4Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   begin_up(p, &s.items);
   publish(p, s.items, 1);
   const int tiles = p.by_tiles.d, units = s.items.count * tiles, stages = stages_of(p.I);
-  Stages<LAYOUT> ring(layer_table, p.up_row);
-  int coming = blockIdx.x, stage = warp;
+  Stages<LAYOUT> ring(layer_table, t);
+  int coming = warp < stages ? blockIdx.x : units, stage = stages;       // of what is asked for next; (a contraction of few stages leaves warps idle)
   auto next = [&]() {
-    while (coming < units && stage >= stages) {
-      coming += gridDim.x;
-      stage = warp;
-      if (warp >= stages) break;
-    }
-    if (coming < units && stage < stages) {
+    if (stage >= stages && coming < units) {
       const int which = p.by_tiles.quotient(coming);
       const Item& item = s.items.item[which];
-      const Matrix4 t{static_cast<const uint8_t*>(p.up) + item.expert * p.up_far, p.up_scale + item.expert * (p.us_row * p.J), p.up_row, p.us_row, p.I, p.J, p.up_words};
-      ring.ask(t, (coming - which * tiles) * kTile4, stage, x, item.rows, [&](int m) { return p.by_k.quotient(item.slot[m]); });
+      ring.begin(item.expert, (coming - which * tiles) * kTile4, x, item.rows, [&](int m) { return p.by_k.quotient(item.slot[m]); });
+      stage = warp;
+      coming += gridDim.x;
+    }
+    if (stage < stages) {
+      ring.ask(stage);
       stage += kWarps4;
     } else {
       ring.store_late();
@@ -1013,7 +1037,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_cons
 
 // A cluster has a tile of the output's columns, its warps the items' stages in turn; each warp adds up the tokens' outputs for itself, then they are joined.
 template <typename T, int LAYOUT>
-__global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_constant__ LayerParams p, const Rows4 x) {
+__global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_constant__ LayerParams p, const __grid_constant__ Matrix4 t, const Rows4 x) {
   extern __shared__ __align__(16) float layer_smem[];
   __shared__ DownShared items;
   const int rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n0 = blockIdx.x / size * kTile4;
@@ -1024,14 +1048,14 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
   pdl_trigger();
   begin_down(p, &items);
   const int stages = stages_of(p.J), all = items.count * stages, step = size * kWarps4;
-  Stages<LAYOUT> ring(layer_smem, p.down_row);
+  Stages<LAYOUT> ring(layer_smem, t);
   int coming = rank * kWarps4 + warp;
   auto next = [&]() {
     if (coming < all) {
-      const int which = coming / stages;
+      const int which = p.by_stages.quotient(coming);
       const Item& item = items.item[which];
-      const Matrix4 t{static_cast<const uint8_t*>(p.down) + item.expert * p.down_far, p.down_scale + item.expert * (p.ds_row * p.I), p.down_row, p.ds_row, p.J, p.I, p.down_words};
-      ring.ask(t, n0, coming - which * stages, x, item.rows, [&](int m) { return static_cast<int>(item.slot[m]); });
+      ring.begin(item.expert, n0, x, item.rows, [&](int m) { return static_cast<int>(item.slot[m]); });
+      ring.ask(coming - which * stages);
       coming += step;
     } else {
       ring.store_late();
@@ -1042,7 +1066,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
   for (int d = 0; d < kDepth4 - 1; ++d) next();
   const int g = lane >> 2, q = lane & 3;
   for (int i = rank * kWarps4 + warp; i < all; i += step) {
-    const Item item = items.item[i / stages];
+    const Item item = items.item[p.by_stages.quotient(i)];
     const int slot0 = item.slot[(q & 1) * 2], slot1 = item.slot[(q & 1) * 2 + 1];
     float2 acc[4] = {};
     next();
@@ -1136,15 +1160,15 @@ Layout4 layout4(const void* w, bool cn, long long row, long long far) {
   return !cn ? kNC : whole(16) ? kCN16 : whole(4) ? kCN4 : kCN1;
 }
 template <int LAYOUT>
-cudaError_t up4_launch(const LayerParams& p, const Rows4& x, const Rows4& to, cudaStream_t st) {
+cudaError_t up4_launch(const LayerParams& p, const Matrix4& t, const Rows4& x, const Rows4& to, cudaStream_t st) {
   cudaError_t err = ensure_smem_optin<few_up4_kernel<LAYOUT>>(static_cast<int>(kRing4));
   if (err != cudaSuccess) return err;
   count_launch();
-  return launch_kernel(few_up4_kernel<LAYOUT>, dim3(kUpGrid), kThreads4, kRing4, st, true, p, x, to);
+  return launch_kernel(few_up4_kernel<LAYOUT>, dim3(kUpGrid), kThreads4, kRing4, st, true, p, t, x, to);
 }
 // CTAs of a cluster: as many as two an SM leave room for, a stage for a warp at least.
 template <typename T, int LAYOUT>
-cudaError_t down4_launch(const LayerParams& p, const Rows4& x, cudaStream_t st) {
+cudaError_t down4_launch(const LayerParams& p, const Matrix4& t, const Rows4& x, cudaStream_t st) {
   const int tiles = (p.I + kTile4 - 1) / kTile4, turns = p.tokens * p.k * stages_of(p.J);
   unsigned size = 8;
   while (size > 1 && (tiles * size > 256 || turns < static_cast<int>(size / 2) * kWarps4)) size /= 2;
@@ -1152,7 +1176,7 @@ cudaError_t down4_launch(const LayerParams& p, const Rows4& x, cudaStream_t st) 
   cudaError_t err = ensure_smem_optin<few_down4_kernel<T, LAYOUT>>(static_cast<int>(kRing4 + (kWarps4 + 1) * 32 * kTile4 * sizeof(float)));
   if (err != cudaSuccess) return err;
   count_launch();
-  return launch_cluster(few_down4_kernel<T, LAYOUT>, tiles * size, kThreads4, size, smem, st, p, x);
+  return launch_cluster(few_down4_kernel<T, LAYOUT>, tiles * size, kThreads4, size, smem, st, p, t, x);
 }
 template <typename T>
 cudaError_t layer4_t(LayerParams p, const egs_route& route, bool up_cn, bool down_cn, const Rows4& x, const Rows4& h, cudaStream_t st) {
@@ -1163,20 +1187,22 @@ cudaError_t layer4_t(LayerParams p, const egs_route& route, bool up_cn, bool dow
   if (err != cudaSuccess) return err;
   if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
   p.by_tiles = Div((p.J + kTile4 - 1) / kTile4);
-  p.up_words = p.us_row % 4 == 0 && on(p.up_scale, 4);
-  p.down_words = p.ds_row % 4 == 0 && on(p.down_scale, 4);
+  p.by_stages = Div(stages_of(p.J));
+  auto words = [](const uint8_t* scale, long long row) { return row % 4 == 0 && on(scale, 4); };
+  const Matrix4 up{static_cast<const uint8_t*>(p.up), p.up_scale, p.up_far, p.us_row * p.J, static_cast<uint32_t>(p.up_row), static_cast<uint32_t>(p.us_row), p.I, p.J, words(p.up_scale, p.us_row)};
+  const Matrix4 down{static_cast<const uint8_t*>(p.down), p.down_scale, p.down_far, p.ds_row * p.I, static_cast<uint32_t>(p.down_row), static_cast<uint32_t>(p.ds_row), p.J, p.I, words(p.down_scale, p.ds_row)};
   switch (layout4(p.up, up_cn, p.up_row, p.up_far)) {
-    case kNC: err = up4_launch<kNC>(p, x, h, st); break;
-    case kCN16: err = up4_launch<kCN16>(p, x, h, st); break;
-    case kCN4: err = up4_launch<kCN4>(p, x, h, st); break;
-    default: err = up4_launch<kCN1>(p, x, h, st);
+    case kNC: err = up4_launch<kNC>(p, up, x, h, st); break;
+    case kCN16: err = up4_launch<kCN16>(p, up, x, h, st); break;
+    case kCN4: err = up4_launch<kCN4>(p, up, x, h, st); break;
+    default: err = up4_launch<kCN1>(p, up, x, h, st);
   }
   if (err != cudaSuccess) return err;
   switch (layout4(p.down, down_cn, p.down_row, p.down_far)) {
-    case kNC: return down4_launch<T, kNC>(p, h, st);
-    case kCN16: return down4_launch<T, kCN16>(p, h, st);
-    case kCN4: return down4_launch<T, kCN4>(p, h, st);
-    default: return down4_launch<T, kCN1>(p, h, st);
+    case kNC: return down4_launch<T, kNC>(p, down, h, st);
+    case kCN16: return down4_launch<T, kCN16>(p, down, h, st);
+    case kCN4: return down4_launch<T, kCN4>(p, down, h, st);
+    default: return down4_launch<T, kCN1>(p, down, h, st);
   }
 }
 
