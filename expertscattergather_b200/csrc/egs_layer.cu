@@ -543,7 +543,7 @@ __device__ __forceinline__ void activation(const LayerParams& p, int parts, long
 // sums: to, room for them, [CTAs][outputs of a share] of shared memory.
 template <typename T, int TILE, class Sum>
 __device__ __forceinline__ void put_out(const LayerParams& p, float* to, int n0, Sum&& sum) {
-  const int rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = all / size;
+  const int rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = (all / 4 + size - 1) / size * 4;
   if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all have begun
   for (int i = threadIdx.x * 4; i < all; i += blockDim.x * 4) {
     const int t = i / TILE, n = i % TILE;
@@ -556,13 +556,13 @@ __device__ __forceinline__ void put_out(const LayerParams& p, float* to, int n0,
       if (n0 + n + 2 < p.I) out[2] = from_f32<T>(v.z);
       if (n0 + n + 3 < p.I) out[3] = from_f32<T>(v.w);
     } else {
-      const int owner = i / own;               // (shares are whole fours: a tile has at least 32 columns, a cluster eight CTAs)
+      const int owner = i / own;
       asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(in_cta(to + rank * own + i - owner * own, owner)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
     }
   }
   if (size == 1) return;
   cluster_sync();
-  for (int i = threadIdx.x; i < own; i += blockDim.x) {
+  for (int i = threadIdx.x; i < min(own, all - rank * own); i += blockDim.x) {
     const int x = rank * own + i, t = x / TILE, n = x % TILE;
     float v = to[i];
     for (int r = 1; r < size; ++r) v += to[r * own + i];
@@ -1113,12 +1113,12 @@ cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned bl
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// CTAs of a cluster, each with 32 contraction elements at least and an SM of its own: of the processing clusters, 16 to 20 SMs, clusters of eight and
-// of four leave some SMs unused.
+// CTAs of a cluster, each with 32 contraction elements at least and an SM of its own: as many as leave room for all clusters at once.  (Of clusters of eight
+// 15 fit, of seven as many, of six 22: clusters lie in processing clusters of 14 to 20 SMs.  16 tiles: a cluster that waits for the others took 5 us.)
 unsigned cluster_of(int tiles, int J) {
+  constexpr int kFit[] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
   unsigned size = 8;
-  auto fit = [](unsigned n) { return n == 8 ? 15 : n == 4 ? 33 : 74; };
-  while (size > 1 && (tiles > fit(size) || J / static_cast<int>(size) < 32)) size /= 2;
+  while (size > 1 && (tiles > kFit[size] || J / static_cast<int>(size) < 32)) --size;
   return size;
 }
 
@@ -1129,7 +1129,7 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   if (err != cudaSuccess) return err;
   const unsigned size = cluster_of(tiles, p.J);
   const size_t ring = static_cast<size_t>(p.ring_words) * 4;
-  const size_t part = static_cast<size_t>((slots < 4 * kDownWarps ? 4 * kDownWarps : slots) + (size > 1 ? p.tokens : 0)) * tile * sizeof(float);
+  const size_t part = static_cast<size_t>((slots < 4 * kDownWarps ? 4 * kDownWarps : slots) + (size > 1 ? p.tokens : 0)) * tile * sizeof(float) + 4 * size * sizeof(float);
   size_t act = static_cast<size_t>(slots) * (p.J / size + 36) * sizeof(float);
   act = (act + 15) & ~static_cast<size_t>(15);
   if (act > kDownSmem - part - ring) act = kDownSmem - part - ring;
