@@ -42,6 +42,7 @@ struct LayerParams {
   int groups, top_groups, group_top, sigmoid, renormalize;
   float scale;
   int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
+  long long weight_bytes;    // of all experts' matrices, of either product
   int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
   Div by_tiles, by_k, by_stages;
@@ -305,37 +306,81 @@ __device__ __forceinline__ void accumulate(Sums<V> (&acc)[M], const T* W, int w_
 // Weights on their way to shared memory, kDepth pieces of 64 bytes a thread, each thread's its own: what it asked for it reads, so that nobody waits for
 // others, and the next unit's weights come while this one's sums are joined.  (Into registers, with a wait for all that had been asked for before
 // more was, 43 MB came at 3.4 TB/s.)
-template <int THREADS, int DEPTH>
+// SHIFT: rows that begin anywhere.  What comes are the 16-byte pieces of memory that a row's tile lies in, one more than it has, and a thread shifts its elements
+// together from its piece and the next thread's.
+template <int THREADS, int DEPTH, int LANES, bool SHIFT>
 struct Ring {
+  enum : bool { kShift = SHIFT };
   uint32_t base;
   int slot = 0;
-  __device__ __forceinline__ explicit Ring(const void* smem) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16u) {}
-  __device__ __forceinline__ uint32_t at(int r) const { return base + static_cast<uint32_t>(slot * 4 + r) * (THREADS * 16u); }
-  __device__ __forceinline__ void ask(int r, const void* from, bool there) const {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(r)), "l"(from), "r"(there ? 16 : 0) : "memory");
+  __device__ __forceinline__ explicit Ring(const void* smem) : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem))) {}
+  __device__ __forceinline__ uint32_t at(int r) const { return base + static_cast<uint32_t>(slot * 4 + r) * (THREADS * 16u) + threadIdx.x * 16u; }
+  __device__ __forceinline__ uint32_t behind(int r) const {        // the piece that a group of threads has beyond theirs
+    return base + static_cast<uint32_t>(DEPTH * THREADS * 64) + (static_cast<uint32_t>(slot * 4 + r) * (THREADS / LANES) + threadIdx.x / LANES) * 16u;
+  }
+  __device__ __forceinline__ void ask(uint32_t to, const void* from, int bytes) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
   }
   __device__ __forceinline__ void asked() {        // (the slot that has been read is the one that is asked for anew)
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (++slot == DEPTH) slot = 0;
   }
-  __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory"); }
+  __device__ __forceinline__ void wait() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    if constexpr (SHIFT) __syncwarp();
+  }
+  __device__ __forceinline__ void read() const {   // all that is in the slot
+    if constexpr (SHIFT) __syncwarp();
+  }
+  __device__ __forceinline__ static uint4 load(uint32_t from) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(from) : "memory");
+    return x;
+  }
+  // first: bytes of this thread's piece that are before its elements
   template <class P>
-  __device__ __forceinline__ P get(int r) const {
+  __device__ __forceinline__ P get(int r, uint32_t first) const {
     static_assert(sizeof(P) == 16, "pieces are of 16 bytes");
     union {
       uint4 raw;
       P value;
     } x{};
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.raw.x), "=r"(x.raw.y), "=r"(x.raw.z), "=r"(x.raw.w) : "r"(at(r)) : "memory");
+    x.raw = load(at(r));
+    if constexpr (SHIFT) {
+      const uint4 y = load(threadIdx.x % LANES == LANES - 1 ? behind(r) : at(r) + 16u);
+      uint32_t w[8] = {x.raw.x, x.raw.y, x.raw.z, x.raw.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = first & 8u ? w[i + 2] : w[i];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = first & 4u ? w[i + 1] : w[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (first & 2u) * 8u);
+      x.raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
     return x.value;
   }
 };
-// Four rows of weights times M rows of the other operand at x.
+// Shifted rows: `left` of four from `row` on (of all experts' rows), from column n0 on; all: bytes of the weights.
+template <typename T, int LANES, class R>
+__device__ __forceinline__ void ask_shifted(const R& ring, const void* W, int N, long long row, int left, int n0, long long all) {
+  const int lane = threadIdx.x % LANES;
+  long long begin = (row * N + n0) * static_cast<long long>(sizeof(T));
+  auto ask = [&](uint32_t to, long long at, int r) {
+    const int there = r < left ? static_cast<int>(max(min(all - at, 16ll), 0ll)) : 0;
+    ring.ask(to, there ? static_cast<const char*>(W) + at : W, there);
+  };
+#pragma unroll
+  for (int r = 0; r < 4; ++r, begin += N * static_cast<long long>(sizeof(T))) {
+    ask(ring.at(r), (begin & ~15ll) + lane * 16, r);
+    if (lane == r) ask(ring.behind(r), (begin & ~15ll) + LANES * 16, r);
+  }
+}
+// Four rows of weights times M rows of the other operand at `at`.  Shifted rows: element `first` of all is the first row's first, they are N apart.
 template <typename T, int V, int M, class R>
-__device__ __forceinline__ void add_four(Sums<V> (&acc)[M], const R& ring, const float* const (&a)[M], int at) {
+__device__ __forceinline__ void add_four(Sums<V> (&acc)[M], const R& ring, const float* const (&a)[M], int at, uint32_t first, uint32_t N) {
   Packed<T, V> w[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) w[r] = ring.template get<Packed<T, V>>(r);
+  for (int r = 0; r < 4; ++r, first += N) w[r] = ring.template get<Packed<T, V>>(r, first * sizeof(T));
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     const float4 x = *reinterpret_cast<const float4*>(a[m] + at);
@@ -410,7 +455,8 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
       stage();
       for (int c = first, left = (c1 - c0 + kStep - 1) / kStep; left; --left, c += kStep) {
         ring.wait();
-        if (c < c1) add_four<T, V, M>(acc, ring, a, c - c0);
+        if (c < c1) add_four<T, V, M>(acc, ring, a, c - c0, R::kShift ? (static_cast<uint32_t>(item.expert) * p.I + c) * p.J + u.n0 : 0u, p.J);
+        ring.read();
         next();
       }
     } else {
@@ -437,9 +483,9 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
 }
 
 constexpr int kUpDepth = 4, kDownDepth = 3;
-constexpr size_t ring_bytes(int threads, int depth) { return static_cast<size_t>(threads) * depth * 64; }
+constexpr size_t ring_bytes(int threads, int depth, int lanes) { return static_cast<size_t>(threads) * depth * 64 + (lanes ? static_cast<size_t>(threads / lanes) * depth * 64 : 0); }
 
-template <typename T, int V, int LANES>
+template <typename T, int V, int LANES, bool SHIFT>
 __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_constant__ LayerParams p) {
   constexpr int kTile = LANES * V, kStep = kUpThreads / LANES * 4;
   constexpr bool kRing = V == 16 / sizeof(T);
@@ -449,11 +495,13 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
   const int parts = parts_of(s.items.count * p.by_tiles.d, p.I);
   publish(p, s.items, parts);
   const int all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
-  Ring<kUpThreads, kUpDepth> ring(layer_table);
+  Ring<kUpThreads, kUpDepth, LANES, SHIFT> ring(layer_table);
   // what is asked for next: rows c .. c + 3 of unit `coming`
   int coming = blockIdx.x, c = 0, end = 0, left = 0;
   bool on = false;
   const T* from = static_cast<const T*>(p.up);
+  long long first_row = 0;
+  int n0 = 0;
   auto next = [&]() {
     if (left == 0 && coming < units) {
       const UpUnit x = up_unit_of(p, coming, all, length, p.I, kTile);
@@ -463,13 +511,19 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
       end = x.end;
       left = (x.end - x.begin + kStep - 1) / kStep;
       from = static_cast<const T*>(p.up) + s.items.item[x.item].expert * (p.up_row * p.I) + c * p.up_row + n;
+      first_row = static_cast<long long>(s.items.item[x.item].expert) * p.I;
+      n0 = x.n0;
       coming += gridDim.x;
     }
     if (left) {
+      if constexpr (SHIFT) {
+        ask_shifted<T, LANES>(ring, p.up, p.J, first_row + c, end - c, n0, p.weight_bytes);
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool there = on && c + r < end;
-        ring.ask(r, there ? from + r * p.up_row : static_cast<const T*>(p.up), there);
+        for (int r = 0; r < 4; ++r) {
+          const bool there = on && c + r < end;
+          ring.ask(ring.at(r), there ? from + r * p.up_row : static_cast<const T*>(p.up), there ? 16 : 0);
+        }
       }
       c += kStep;
       from += kStep * p.up_row;
@@ -584,7 +638,8 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
   if constexpr (V == 16 / sizeof(T)) {
     for (int c = begin + lane / LANES * 4, left = (end - begin + kStep - 1) / kStep; left; --left, c += kStep) {
       ring.wait();
-      if (c < end) add_four<T, V, M>(acc, ring, a, c - base);
+      if (c < end) add_four<T, V, M>(acc, ring, a, c - base, R::kShift ? (static_cast<uint32_t>(item.expert) * p.J + c) * p.I + n0 : 0u, p.I);
+      ring.read();
       next();
     }
   } else {
@@ -605,7 +660,7 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
   }
 }
 
-template <typename T, int V, int LANES>
+template <typename T, int V, int LANES, bool SHIFT>
 __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_constant__ LayerParams p) {
   constexpr int kTile = LANES * V, kStep = 32 / LANES * 4;
   constexpr bool kRing = V == 16 / sizeof(T);
@@ -625,7 +680,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
   int shares_log2 = 0;                         // warps that have an item's contraction in turn
   while (items.count << (shares_log2 + 1) <= kDownWarps && length >> shares_log2 >= 64) ++shares_log2;
   const int turns = items.count << shares_log2;
-  Ring<kDownThreads, kDownDepth> ring(layer_smem);
+  Ring<kDownThreads, kDownDepth, LANES, SHIFT> ring(layer_smem);
   for (int c0 = begin; c0 == begin || c0 < end; c0 += room) {
     const int c1 = min(end, c0 + room), width = (c1 - c0 + 3) & ~3, each = ((width / 4 + (1 << shares_log2) - 1) >> shares_log2) * 4;
     auto share_of = [&](int x, int* to) {      // first row, and the one behind the last
@@ -637,19 +692,25 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
     int coming = warp, c = 0, stop = 0, left = 0;
     const T* from = static_cast<const T*>(p.down);
     const bool on = n0 + lane % LANES * V < p.I;
+    long long first_row = 0;
     auto next = [&]() {
       while (left == 0 && coming < turns) {
         const int b = share_of(coming, &stop);
         c = b + lane / LANES * 4;
         left = (stop - b + kStep - 1) / kStep;
         from = static_cast<const T*>(p.down) + items.item[coming >> shares_log2].expert * (p.down_row * p.J) + c * p.down_row + n0 + lane % LANES * V;
+        first_row = static_cast<long long>(items.item[coming >> shares_log2].expert) * p.J;
         coming += kDownWarps;
       }
       if (left) {
+        if constexpr (SHIFT) {
+          ask_shifted<T, LANES>(ring, p.down, p.I, first_row + c, stop - c, n0, p.weight_bytes);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool there = on && c + r < stop;
-          ring.ask(r, there ? from + r * p.down_row : static_cast<const T*>(p.down), there);
+          for (int r = 0; r < 4; ++r) {
+            const bool there = on && c + r < stop;
+            ring.ask(ring.at(r), there ? from + r * p.down_row : static_cast<const T*>(p.down), there ? 16 : 0);
+          }
         }
         c += kStep;
         from += kStep * p.down_row;
@@ -1140,7 +1201,7 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
 
 template <auto kernel>
 cudaError_t up_launch(const LayerParams& p, cudaStream_t st) {
-  cudaError_t err = ensure_smem_optin<kernel>(static_cast<int>(ring_bytes(kUpThreads, kUpDepth)));
+  cudaError_t err = ensure_smem_optin<kernel>(static_cast<int>(ring_bytes(kUpThreads, kUpDepth, 8)));
   if (err != cudaSuccess) return err;
   count_launch();
   return launch_kernel(kernel, dim3(kUpGrid), kUpThreads, static_cast<size_t>(p.ring_words) * 4, st, true, p);
@@ -1214,18 +1275,29 @@ cudaError_t layer_t(LayerParams p, const egs_route& route, cudaStream_t st) {
   cudaError_t err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
   if (err != cudaSuccess) return err;
   if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
-  // (one width for both: the parts of `up` are counted by it)
-  const bool wide = p.I % V == 0 && p.J % V == 0 && on(p.up, 16) && on(p.down, 16);
-  if (wide) {
+  // One width for both products: the parts of `up` are counted by it.  16-byte vectors where rows begin on them.  Rows that do not are shifted together in 16 bits from
+  // 128 Ki elements of an expert's matrix on, and else come element by element (us a call, shifted and not: 8 tokens, 2047 x 511, 62 and 102; 4 tokens, 500 x 301,
+  // 18.8 and 19.5, 330 x 201, 18.0 and 16.9; 4 tokens in float32, 1001 x 500, 34.3 and 34.1).
+  const bool whole = p.I % V == 0 && p.J % V == 0;
+  const long long elements = static_cast<long long>(p.I) * p.J;
+  if (on(p.up, 16) && on(p.down, 16) && (whole || (sizeof(T) == 2 && elements >= 128 << 10))) {
     p.by_tiles = Div((p.J + V * kLanes - 1) / (V * kLanes));
-    p.ring_words = static_cast<int>(ring_bytes(kUpThreads, kUpDepth) / 4);
-    if ((err = up_launch<few_up_kernel<T, V, kLanes>>(p, st)) != cudaSuccess) return err;
-    p.ring_words = static_cast<int>(ring_bytes(kDownThreads, kDownDepth) / 4);
-    return down_launch<few_down_kernel<T, V, kLanes>, T>(p, V * kLanes, st);
+    p.weight_bytes = p.E * elements * static_cast<long long>(sizeof(T));
+    auto both = [&](auto up, auto down, int lanes) {
+      p.ring_words = static_cast<int>(ring_bytes(kUpThreads, kUpDepth, lanes) / 4);
+      if (cudaError_t e = up(); e != cudaSuccess) return e;
+      p.ring_words = static_cast<int>(ring_bytes(kDownThreads, kDownDepth, lanes) / 4);
+      return down();
+    };
+    if constexpr (sizeof(T) == 2) {
+      if (!whole)
+        return both([&] { return up_launch<few_up_kernel<T, V, kLanes, true>>(p, st); }, [&] { return down_launch<few_down_kernel<T, V, kLanes, true>, T>(p, V * kLanes, st); }, kLanes);
+    }
+    return both([&] { return up_launch<few_up_kernel<T, V, kLanes, false>>(p, st); }, [&] { return down_launch<few_down_kernel<T, V, kLanes, false>, T>(p, V * kLanes, st); }, 0);
   }
   p.by_tiles = Div((p.J + 31) / 32);
-  if ((err = up_launch<few_up_kernel<T, 1, 32>>(p, st)) != cudaSuccess) return err;
-  return down_launch<few_down_kernel<T, 1, 32>, T>(p, 32, st);
+  if ((err = up_launch<few_up_kernel<T, 1, 32, false>>(p, st)) != cudaSuccess) return err;
+  return down_launch<few_down_kernel<T, 1, 32, false>, T>(p, 32, st);
 }
 
 }  // namespace

@@ -175,6 +175,21 @@ def test_strides_and_shapes():
         assert torch.equal(ops.routed_experts_few(x, router, u, d, k)[0], want[0])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,E,k,I,J", [(1, 3, 3, 2047, 511), (9, 5, 3, 515, 771), (4, 6, 2, 1031, 257), (32, 3, 2, 266, 1001), (2, 2, 2, 37, 7001), (3, 4, 1, 9000, 15)])
+@pytest.mark.parametrize("begin", [8, 3])
+def test_wide_rows_that_begin_anywhere(dtype, tokens, E, k, I, J, begin):
+    """Rows of no whole vectors, all experts among the chosen ones, NaN before and behind the weights; weights that begin on 16 bytes, or not."""
+    t = TYPES[dtype]
+    x, router = randn(tokens, I, seed=1, dtype=t), (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    up, down = (torch.full((begin + E * I * J + 9,), float("nan"), device="cuda", dtype=t)[begin:begin + E * I * J] for _ in range(2))
+    up, down = up.view(E, I, J).copy_(randn(E, I, J, seed=3) * 2 / I ** 0.5), down.view(E, J, I).copy_(randn(E, J, I, seed=4) / J ** 0.5)
+    out, w, ids = ops.routed_experts_few(x, router, up, down, k)
+    want, off = layer64(x.double(), w.double(), ids.long(), up.double(), down.double())
+    worst = ((out.double() - want).abs() - off - want.abs() * (torch.finfo(t).eps / 2) - (2.0 ** -25 if dtype == "f16" else 0)).max().item()
+    assert worst <= 0, (worst, (out.double() - want).abs().max().item())
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)
