@@ -21,8 +21,17 @@ struct ToFp4 {
   int C, chunks, lanes_log2;      // chunks: of eight elements, whole blocks
 };
 
-// V: elements that are loaded together; AHEAD: stretches whose loads go out together
-template <typename T, int V, bool SILU, int AHEAD>
+// The largest magnitude of eight 16-bit elements in pairs, as float32's bits (a NaN where there is one).
+template <typename T>
+__device__ __forceinline__ uint32_t most_of(const uint32_t (&w)[4]) {
+  using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const P* x = reinterpret_cast<const P*>(w);
+  const P most = __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])), __hmax2_nan(__habs2(x[2]), __habs2(x[3])));
+  return __float_as_uint(to_f32<T>(__hmax_nan(most.x, most.y)));
+}
+// V: elements that are loaded together; AHEAD: stretches whose loads go out together; WIDE: of 32 lanes, which makes their distances known (74
+// instructions for eight elements, 101 with addresses and bounds of each: 33.5 million elements 17.0 us and 17.6, 1 million 2.9 and 4.4).
+template <typename T, int V, bool SILU, int AHEAD, bool WIDE>
 __global__ void __launch_bounds__(kToWarps * 32) to_fp4_kernel(const __grid_constant__ ToFp4 p) {
   using P = Packed<T, V>;
   union Eight {
@@ -33,53 +42,57 @@ __global__ void __launch_bounds__(kToWarps * 32) to_fp4_kernel(const __grid_cons
   };
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = 1 << p.lanes_log2;
-  const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> p.lanes_log2) + (lane >> p.lanes_log2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes_log2 = WIDE ? 5 : p.lanes_log2, lanes = 1 << lanes_log2;
+  const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> lanes_log2) + (lane >> lanes_log2);
   const int first = blockIdx.y * lanes * AHEAD + (lane & (lanes - 1));
   const bool on = row < p.rows;
-  const T* x = static_cast<const T*>(p.X) + row * p.x_stride;
-  Eight y[AHEAD];
+  const T* x = static_cast<const T*>(p.X) + row * p.x_stride + first * 8ll;
+  uint32_t* q = reinterpret_cast<uint32_t*>(p.q + row * p.q_stride) + first;
+  uint8_t* scale = p.scale + row * p.s_stride;
+  auto pass = [&](auto whole) {                // whole: all of it is there
+    constexpr bool kWhole = decltype(whole)::value;
+    Eight y[AHEAD];
 #pragma unroll
-  for (int u = 0; u < AHEAD; ++u) {
-    const int c = (first + u * lanes) * 8;
-    if (on && c + 8 <= p.C) {
+    for (int u = 0; u < AHEAD; ++u) {
+      const int c = (first + u * lanes) * 8;
+      if (kWhole || (on && c + 8 <= p.C)) {
 #pragma unroll
-      for (int i = 0; i < 8 / V; ++i) y[u].packs[i] = reinterpret_cast<const P*>(x + c)[i];
-    } else {
+        for (int i = 0; i < 8 / V; ++i) y[u].packs[i] = reinterpret_cast<const P*>(x + u * lanes * 8)[i];
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[u].each[i] = on && c + i < p.C ? x[c + i] : from_f32<T>(0.f);
+        for (int i = 0; i < 8; ++i) y[u].each[i] = on && c + i < p.C ? x[u * lanes * 8 + i] : from_f32<T>(0.f);
+      }
     }
-  }
 #pragma unroll
-  for (int u = 0; u < AHEAD; ++u) {
-    const int chunk = first + u * lanes;
-    float v[8];
+    for (int u = 0; u < AHEAD; ++u) {
+      const int chunk = first + u * lanes;
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = to_f32<T>(y[u].each[i]);
-      if constexpr (SILU) v[i] = silu_exact(v[i]);
+      for (int i = 0; i < 8; ++i) {
+        v[i] = to_f32<T>(y[u].each[i]);
+        if constexpr (SILU) v[i] = silu_exact(v[i]);
+      }
+      uint32_t top = 0u;
+      if constexpr (!SILU && sizeof(T) == 2) {
+        top = most_of<T>(y[u].words);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      }
+      top = max(top, __shfl_xor_sync(kAll, top, 1));
+      top = max(top, __shfl_xor_sync(kAll, top, 2));
+      if (!kWhole && (!on || chunk >= p.chunks)) continue;
+      const uint32_t byte = fp4_scale(top);
+      const float inverse = fp4_inverse(byte);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= inverse;
+      const uint32_t w = fp4_pack8(v);
+      q[u * lanes] = inverse == 0.f ? 0u : w;
+      if (!(lane & 3)) scale[chunk >> 2] = static_cast<uint8_t>(byte);
     }
-    uint32_t top = 0u;
-    if constexpr (!SILU && sizeof(T) == 2) {   // 16-bit magnitudes in pairs
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = __vmaxu2(top, y[u].words[i] & 0x7fff7fffu);
-      const unsigned short most = static_cast<unsigned short>(max(top >> 16, top & 0xffffu));
-      top = __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&most)));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    }
-    top = max(top, __shfl_xor_sync(kAll, top, 1));
-    top = max(top, __shfl_xor_sync(kAll, top, 2));
-    if (!on || chunk >= p.chunks) continue;
-    const uint32_t byte = fp4_scale(top);
-    const float inverse = fp4_inverse(byte);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inverse;
-    const uint32_t q = fp4_pack8(v);
-    *reinterpret_cast<uint32_t*>(p.q + row * p.q_stride + chunk * 4ll) = inverse == 0.f ? 0u : q;
-    if (!(chunk & 3)) p.scale[row * p.s_stride + (chunk >> 2)] = static_cast<uint8_t>(byte);
-  }
+  };
+  if (WIDE && __all_sync(kAll, on && (first + (AHEAD - 1) * lanes + 1) * 8 <= p.C)) pass(std::true_type{});
+  else pass(std::false_type{});
 }
 
 template <typename T, int V>
@@ -89,10 +102,14 @@ cudaError_t to_fp4_v(const ToFp4& p, int act, cudaStream_t st) {
     const int stretch = ahead << p.lanes_log2;
     return launch_kernel(kernel, dim3(static_cast<unsigned>(ctas), (p.chunks + stretch - 1) / stretch), kToWarps * 32, 0, st, true, p);
   };
-  // Few rows: a stretch a CTA, so that all SMs have some (1003 x 1030 with SiLU, and back: 8.8 us, with four of them 13.7).
+  // Few rows: a stretch a CTA, so that all SMs have some (1003 x 1030 with SiLU, and back: 8.8 us, with four of them 13.7; now 5.8).
   const bool spread = ctas * ((p.chunks >> p.lanes_log2) + 3) / 4 < 148 * 4;
-  if (act == EGS_ACT_SILU) return spread ? go(to_fp4_kernel<T, V, true, 1>, 1) : go(to_fp4_kernel<T, V, true, kToAhead>, kToAhead);
-  return spread ? go(to_fp4_kernel<T, V, false, 1>, 1) : go(to_fp4_kernel<T, V, false, kToAhead>, kToAhead);
+  auto by_width = [&](auto silu) {
+    constexpr bool kSilu = decltype(silu)::value;
+    if (spread) return p.lanes_log2 == 5 ? go(to_fp4_kernel<T, V, kSilu, 1, true>, 1) : go(to_fp4_kernel<T, V, kSilu, 1, false>, 1);
+    return p.lanes_log2 == 5 ? go(to_fp4_kernel<T, V, kSilu, kToAhead, true>, kToAhead) : go(to_fp4_kernel<T, V, kSilu, kToAhead, false>, kToAhead);
+  };
+  return act == EGS_ACT_SILU ? by_width(std::true_type{}) : by_width(std::false_type{});
 }
 template <typename T>
 cudaError_t to_fp4_t(const ToFp4& p, int act, cudaStream_t st) {
@@ -139,51 +156,60 @@ __device__ __forceinline__ void store_pairs(T* to, const float2 (&f)[V / 2]) {
 }
 __host__ __device__ constexpr int from_ahead(int V) { return V == 8 ? 4 : 8; }
 
-template <typename T, int V>
+template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(kToWarps * 32) from_fp4_kernel(const __grid_constant__ FromFp4 p) {
   using Q = typename std::conditional<V == 8, uint32_t, uint8_t>::type;
   constexpr int kAhead = from_ahead(V);
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = 1 << p.lanes_log2;
-  const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> p.lanes_log2) + (lane >> p.lanes_log2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes_log2 = WIDE ? 5 : p.lanes_log2, lanes = 1 << lanes_log2;
+  const long long row = (static_cast<long long>(blockIdx.x) * kToWarps + warp) * (32 >> lanes_log2) + (lane >> lanes_log2);
   if (row >= p.rows) return;
   const uint8_t *q = p.q + row * p.q_stride, *scale = p.scale + row * p.s_stride;
   T* x = static_cast<T*>(p.X) + row * p.C;
   for (int first = blockIdx.y * lanes * kAhead + (lane & (lanes - 1)); first < p.chunks; first += gridDim.y * lanes * kAhead) {
-    uint32_t w[kAhead], s[kAhead];
+    const Q* q1 = reinterpret_cast<const Q*>(q + first * V / 2);         // (V = 1: of an even element and of the one behind it the same)
+    const uint8_t* scale1 = scale + first * V / kFp4Block;
+    T* x1 = x + first * V;
+    auto pass = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;      // all of it is there, and lanes * V are whole blocks
+      uint32_t w[kAhead], s[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int c = (first + u * lanes) * V;
-      w[u] = c < p.C ? *reinterpret_cast<const Q*>(q + c / 2) : 0u;
-      s[u] = c < p.C ? scale[c / kFp4Block] : 0u;
-    }
+      for (int u = 0; u < kAhead; ++u) {
+        const int c = (first + u * lanes) * V;
+        w[u] = kWhole ? q1[u * 32 * V / 2 / sizeof(Q)] : c < p.C ? *reinterpret_cast<const Q*>(q + c / 2) : 0u;
+        s[u] = kWhole ? scale1[u * 32 * V / kFp4Block] : c < p.C ? scale[c / kFp4Block] : 0u;
+      }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int c = (first + u * lanes) * V;
-      if (c >= p.C) break;
-      const float power = fp4_power(s[u]);
-      if constexpr (V == 8) {
-        uint32_t h[4];
-        fp4_halves(w[u], h);
-        float2 f[4];
+      for (int u = 0; u < kAhead; ++u) {
+        const int c = (first + u * lanes) * V;
+        if (!kWhole && c >= p.C) break;
+        T* to = kWhole ? x1 + u * 32 * V : x + c;
+        const float power = fp4_power(s[u]);
+        if constexpr (V == 8) {
+          uint32_t h[4];
+          fp4_halves(w[u], h);
+          float2 f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-          f[i].x *= power;
-          f[i].y *= power;
-        }
-        store_pairs<T, 8>(x + c, f);
-      } else {
-        const float even = fp4_value(w[u]) * power, odd = fp4_value(w[u] >> 4) * power;
-        if constexpr (V == 1) {
-          x[c] = from_f32<T>(c & 1 ? odd : even);
+          for (int i = 0; i < 4; ++i) {
+            f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+            f[i].x *= power;
+            f[i].y *= power;
+          }
+          store_pairs<T, 8>(to, f);
         } else {
-          const float2 f[1] = {make_float2(even, odd)};
-          store_pairs<T, 2>(x + c, f);
+          const float even = fp4_value(w[u]) * power, odd = fp4_value(w[u] >> 4) * power;
+          if constexpr (V == 1) {
+            *to = from_f32<T>(c & 1 ? odd : even);
+          } else {
+            const float2 f[1] = {make_float2(even, odd)};
+            store_pairs<T, 2>(to, f);
+          }
         }
       }
-    }
+    };
+    if (WIDE && (first + (kAhead - 1) * lanes + 1) * V <= p.C) pass(std::true_type{});
+    else pass(std::false_type{});
   }
 }
 template <typename T>
@@ -196,9 +222,13 @@ cudaError_t from_fp4_t(FromFp4 p, cudaStream_t st) {
     const int stretch = from_ahead(v) << p.lanes_log2, stretches = (p.chunks + stretch - 1) / stretch;
     return launch_kernel(kernel, dim3(static_cast<unsigned>((p.rows + per_cta - 1) / per_cta), stretches < 65535 ? stretches : 65535), kToWarps * 32, 0, st, true, p);
   };
-  if (p.C % 8 == 0 && (reinterpret_cast<uintptr_t>(p.X) & 15u) == 0) return go(from_fp4_kernel<T, 8>, 8);
-  if (p.C % 2 == 0 && reinterpret_cast<uintptr_t>(p.X) % (2 * sizeof(T)) == 0) return go(from_fp4_kernel<T, 2>, 2);
-  return go(from_fp4_kernel<T, 1>, 1);
+  auto by_width = [&](auto vector) {
+    constexpr int V = decltype(vector)::value;
+    return p.C > 16 * V ? go(from_fp4_kernel<T, V, true>, V) : go(from_fp4_kernel<T, V, false>, V);      // (more than 16 of them: 32 lanes)
+  };
+  if (p.C % 8 == 0 && (reinterpret_cast<uintptr_t>(p.X) & 15u) == 0) return by_width(std::integral_constant<int, 8>{});
+  if (p.C % 2 == 0 && reinterpret_cast<uintptr_t>(p.X) % (2 * sizeof(T)) == 0) return by_width(std::integral_constant<int, 2>{});
+  return by_width(std::integral_constant<int, 1>{});
 }
 
 // ------------------------------------------------------------------------------------------------
