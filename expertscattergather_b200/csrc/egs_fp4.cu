@@ -358,7 +358,10 @@ cudaError_t launch_dequantize_fp4(const uint8_t* q, const uint8_t* scale, void* 
   return dtype == EGS_F16 ? from_fp4_t<__half>(p, st) : dtype == EGS_BF16 ? from_fp4_t<__nv_bfloat16>(p, st) : from_fp4_t<float>(p, st);
 }
 
-bool few_fp4_fit(const Fp4Params& p) { return 4ll * p.rows <= 3 * p.E || p.rows <= 8; }
+// Where experts have one row each, or nearly all: a token's choices differ.  (us, this kernel and tiles of 128 rows: 1 token, 8 of 64 experts, 2048 x 512, 4.8 and 8.4;
+// 1 row, 4096 x 4096, 6.4 and 10.6; 2 tokens, 4 of 64, 1024 x 1024, 5.8 and 8.4; two rows an expert cost as much as four: 3 tokens, 8 of 64, 2048 x 512, 12.7 and 9.5;
+// 16 tokens, 2 of 64, 512 x 512, 11.1 and 6.5; 8 rows, 2048 x 512, 11.3 and 7.4.)
+bool few_fp4_fit(const Fp4Params& p) { return p.rows <= p.by_k.d || 8ll * p.rows <= p.E; }
 
 cudaError_t launch_few_fp4(const Fp4Params& p, int out_dtype, cudaStream_t st) {
   const int segments = p.offsets ? (p.rows < p.E ? p.rows : p.E) : 1, per_cta = kFewWarps * kFewChannels, tiles = (p.N + per_cta - 1) / per_cta;

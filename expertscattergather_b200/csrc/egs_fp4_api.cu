@@ -132,6 +132,7 @@ size_t egs_expert_matmul_fp4_rows_workspace_bytes(const egs_ragged* dims, int pa
   Fp4Params p{};
   p.rows = static_cast<int>(dims->tokens * dims->k);
   p.E = static_cast<int>(dims->E);
+  p.by_k = Div(static_cast<int>(dims->k));
   return takes_few(p, path, tensor_able(*dims)) ? static_cast<size_t>(p.rows) * dims->N * sizeof(float) : 0;
 }
 
