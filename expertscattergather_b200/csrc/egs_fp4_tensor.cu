@@ -7,13 +7,17 @@
 //   warps 0, 1    gathered rows of X (tile::gather4), where they are gathered
 //   warp  2       boxes of rows that follow one another and of weights; announces the bytes of a stage
 //   warp  3       tensor-memory allocation; copies a step's scales to tensor memory and issues its MMAs, by the leader of a pair for both CTAs
-//   warps 4..7    scales: of two steps at a time, from rows to the order in which tensor memory takes them
+//   warps 4..7    scales: of four steps at a time, from rows to the order in which tensor memory takes them
 //   warps 8..15   read-out: tensor memory -> rows of the output, in float32, 16 bits or (activated) in 4 bits with their scales
 //
 // Scales cannot come by TMA: of a row there are 8 bytes a step, and tensor memory wants four bytes of four rows beside one another.  Both CTAs of a pair
 // need the scales of all columns.  What the second one's warps have stored is made visible to its tensor core by their proxy fence; their
-// arrival at the leader's barrier says no more than that this has happened, and a release of everything at cluster scope, which waits behind a memory
-// barrier, made the kernel wait for it (8192 x 4096 -> 4096: 94 us for 74; word by word with cp.async 106; no scales at all 61, no products 47).
+// arrival at the leader's barrier says no more than that this has happened: a release of everything at cluster scope, which waits behind a memory
+// barrier, made the kernel wait for it (94 us for 74 at 8192 x 4096 -> 4096).  Scales word by word with cp.async: 106; 16 bytes of a row (two steps) at a time for 64: 80 for 70.
+//
+// 8192 x 4096 -> 4096: 63.5 us, 4.3 PFLOP/s (2.6 times the 16-bit rate; loads alone 47, all but the scales 61).  Bound by what the L2 gives all SMs, 9.6 TB/s of tiles and scales.
+// 65536 rows of 64 experts, 2048 -> 512: 59, of which 53 without the read-out; 512 -> 2048, two steps a tile: 86, without stores 70, without the read-out 55: 268 MB of
+// output (41) share the memory with the loads.  Rows of a block kept in shared memory for all column tiles: 72 for 55; a read-out of both halves at once: no gain.
 #include <cstddef>
 
 #include "egs_fp4.cuh"

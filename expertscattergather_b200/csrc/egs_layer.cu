@@ -8,6 +8,11 @@
 //   down     a cluster has a tile of the output's columns, its CTAs the contraction in parts; warps have the experts' tokens in turn.  The parts' sums
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
 //            CTAs' in theirs: the same bits in every run.
+//
+// us a call in a graph, new weights each time: 1 token, 8 of 64 experts, 2048 x 512 bf16 (33.8 MB, 5.2 at the copy's rate) 18.0, of which logits 2, choice 2, `up` 4.2 and `down`
+// 6.7 on the device, the rest between them; 16 tokens, 4 of 64, 1024 x 256 (43 MB) 27.7.  Products run at 4 to 5 TB/s once weights come; what is left is latency: four
+// launches, the list, the first weights, the join of a cluster.  Tried: the other product's weights to the L2 ahead (no gain), 16-bit products on mma.sync (1 us more; float32 sums by
+// packed FMA are not what bounds it), weights through registers (3.4 TB/s), rings of 2, 4 and 6 steps (equal, equal, slower), tiles of 128 columns (20 us -> 24.6).
 #include "egs_fp4.cuh"
 
 namespace egs {
@@ -218,6 +223,7 @@ __device__ __forceinline__ void logits_by_warps(const LayerParams& p, int e, int
     if ((threadIdx.x & 31) == 0) p.logits[t * p.E + expert] = v;
   });
 }
+// The logits in float32; 2.0 to 2.6 us, the latency of a router's row.
 template <typename T>
 __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__ LayerParams p) {
   pdl_wait();
@@ -485,6 +491,7 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
 constexpr int kUpDepth = 4, kDownDepth = 3;
 constexpr size_t ring_bytes(int threads, int depth, int lanes) { return static_cast<size_t>(threads) * depth * 64 + (lanes ? static_cast<size_t>(threads / lanes) * depth * 64 : 0); }
 
+// Parts of the first product.  Two CTAs an SM, so that one loads while the other joins its sums; a tile is 128 bytes of a row (eight lanes), of which 32 rows come at a time.
 template <typename T, int V, int LANES, bool SHIFT>
 __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_constant__ LayerParams p) {
   constexpr int kTile = LANES * V, kStep = kUpThreads / LANES * 4;
@@ -660,6 +667,8 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
   }
 }
 
+// The second product and the sum over the choices.  Clusters, because the contraction is short and the columns are few: a token's sums of all CTAs meet in shared memory instead of
+// in another launch.  16 warps have items of their own, so that no two write the same sums.
 template <typename T, int V, int LANES, bool SHIFT>
 __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_constant__ LayerParams p) {
   constexpr int kTile = LANES * V, kStep = 32 / LANES * 4;
@@ -754,7 +763,8 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
 // ---- weights in 4 bits -------------------------------------------------------------------------------------------------
 // Rows and weights become 16-bit floats, which hold them exactly, and go through the tensor cores (mma.sync: 16 columns, 16 contraction elements, up to eight
 // rows); a block's sums are exact, then times both scales into float32 sums.  (As integers through dp4a four columns and a block took 980
-// instructions a warp, and 85 us went by at 43 MB of weights, which are read in 7.)  The weights' bytes lie along the contraction (NC) or along the columns (CN).
+// instructions a warp: 83 us a call, 8 tokens, 8 of 64 experts, 2048 x 512, 47 MB.  Now 35: 4.7 million warp instructions a product, a third of which ask for weights in pieces
+// of 32 bytes a row; with cold caches a product took 20 us, 16 without its arithmetic and 12 without its loads, and takes 17 now.)  The weights' bytes lie along the contraction (NC) or along the columns (CN).
 // A warp's stage: 4 blocks of the contraction x a tile of 32 columns, 2 KB of weights; kDepth4 stages are on their way, each warp's its own.  Lane (g, q) = (lane / 4,
 // lane % 4) multiplies columns 4 g .. 4 g + 3 and of each block the eight elements from 8 q on; their order is the same in both operands.
 constexpr int kTile4 = 32, kStage4 = 4, kDepth4 = 3, kThreads4 = 256, kWarps4 = kThreads4 / 32;
