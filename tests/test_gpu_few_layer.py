@@ -190,6 +190,65 @@ def test_wide_rows_that_begin_anywhere(dtype, tokens, E, k, I, J, begin):
     assert worst <= 0, (worst, (out.double() - want).abs().max().item())
 
 
+@pytest.mark.parametrize("tokens,k", [(8, 32), (32, 8), (1, 32)])
+@pytest.mark.parametrize("dtype,I,J", [("bf16", 96, 64), ("f16", 2049, 67), ("f32", 33, 20)])
+def test_most_slots_and_experts(tokens, k, dtype, I, J):
+    """1024 experts, 256 of tokens * top_k, in 16 and 32 bits and on weights in 4."""
+    t, E = TYPES[dtype], 1024
+    x, router = randn(tokens, I, seed=1, dtype=t), (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    up, down = (randn(E, I, J, seed=3) * 2 / I ** 0.5).to(t), (randn(E, J, I, seed=4) / J ** 0.5).to(t)
+    out, w, ids = ops.routed_experts_few(x, router, up, down, k)
+    check_choice(x, router, None, k, w, ids)
+    want, off = layer64(x.double(), w.double(), ids.long(), up.double(), down.double())
+    assert ((out.double() - want).abs() - off - want.abs() * (torch.finfo(t).eps / 2) - (2.0 ** -25 if dtype == "f16" else 0)).max().item() <= 0
+    (u, us), (d, ds) = grid4(E, J, I, seed=3, low=120, high=124), grid4(E, I, J, seed=4)
+    out, w4, ids4 = ops.routed_experts_few(x, router, u, d, k, up_scale=us, down_scale=ds)
+    assert torch.equal(w4, w) and torch.equal(ids4, ids)
+    # the experts that were chosen alone, in another order: the same products, sums over the choices in their order
+    used, place = ids.long().unique(return_inverse=True)
+    again = torch.zeros(tokens, I, dtype=torch.float64, device="cuda")
+    xq = fp4.values(*fp4.quantize(x), I)
+    upq, downq = fp4.rows(u[used], us[used])[..., :I].transpose(1, 2), fp4.rows(d[used], ds[used])[..., :J].transpose(1, 2)
+    size = torch.zeros_like(again)
+    for e in range(used.numel()):
+        tt, j = (place == e).nonzero(as_tuple=True)
+        h = (xq[tt] @ upq[e]).float()                        # sums of 2049 products of multiples of 2^-9 below 2^4 * 2^-4 * 2049 < 2^12: below 2^24 steps of float32, to 2^-12
+        a = fp4.values(*fp4.quantize(h / (1 + torch.exp(-h))), J)
+        we = w[tt, j].double().unsqueeze(-1)
+        again.index_put_((tt,), we * (a @ downq[e]), accumulate=True)
+        size.index_put_((tt,), we * (a.abs() @ downq[e].abs()), accumulate=True)
+    # where a value lies on a border between two of 4 bits up to the float32 sums' last bits the other one may be taken: a step of it, at most a third of the largest
+    off = size * ((J / 32 + k + 24) * 2.0 ** -24) + again.abs() * (torch.finfo(t).eps / 2) + (2.0 ** -25 if dtype == "f16" else 0)
+    wrong = (out.double() - again).abs() > off
+    assert wrong.double().mean().item() <= (0.02 if I > 1000 else 0.0), wrong.double().mean().item()
+    assert ((out.double() - again).abs() <= off + size / 3).all()
+
+
+def test_blocks_that_are_not_numbers():
+    """A block with the scale 255 makes NaN of what uses it and of nothing else; so does a row with a NaN."""
+    tokens, E, k, I, J = 5, 4, 2, 160, 96
+    (u, us), (d, ds) = grid4(E, J, I, seed=3, low=120, high=124), grid4(E, I, J, seed=4)
+    x, router = randn(tokens, I, seed=1, dtype=torch.bfloat16), randn(E, I, seed=2, dtype=torch.bfloat16)
+    good, _, ids = ops.routed_experts_few(x, router, u, d, k, up_scale=us, down_scale=ds)
+    e = int(ids[0, 0])
+    bad = ds.clone()
+    bad[e, 7, 1] = 255
+    bad[e, 133, 2] = 255
+    out = ops.routed_experts_few(x, router, u, d, k, up_scale=us, down_scale=bad)[0]
+    users = (ids == e).any(-1)
+    gone = users.unsqueeze(-1) & torch.isin(torch.arange(I, device="cuda"), torch.tensor([7, 133], device="cuda"))
+    assert torch.equal(out.isnan(), gone) and torch.equal(out[~gone], good[~gone])
+    bad = us.clone()
+    bad[e, 40, 0] = 255                                     # one activation, so a block of them, so all outputs
+    out = ops.routed_experts_few(x, router, u, d, k, up_scale=bad, down_scale=ds)[0]
+    assert torch.equal(out.isnan().all(-1), users) and torch.equal(out[~users], good[~users])
+    y = x.clone()
+    y[2, 50] = float("nan")
+    out, _, other = ops.routed_experts_few(y, router, u, d, k, up_scale=us, down_scale=ds)
+    rest = torch.arange(tokens, device="cuda") != 2
+    assert out[2].isnan().all() and torch.equal(out[rest], good[rest]) and torch.equal(other[rest], ids[rest])
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)

@@ -192,3 +192,24 @@ def test_expert_matmul_into_4_bits(path, tokens, E, k, C, N, lost):
     step = torch.exp2(torch.maximum(ys.double(), fp4.quantize(full / (1 + torch.exp(-full)))[1].double()) - 127).repeat_interleave(32, -1)[..., :N]
     assert ((got - want).abs() <= 2 * step).all()
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_smallest_numbers_and_no_numbers(dtype):
+    """Blocks of subnormal numbers, zeros, infinities and NaN beside ordinary ones, in rows of all three forms of the kernels."""
+    t = TYPES[dtype]
+    small = torch.finfo(t).smallest_normal if dtype != "f16" else 2.0 ** -14
+    for C in (32, 31, 40, 264, 1030, 1056):
+        X = randn(12, C, seed=C).to(t)
+        X[0] = (X[0].float() * small).to(t)
+        X[1] = (X[1].float() * small / 8).to(t)
+        X[2] = 0
+        X[3, C // 2] = float("inf")
+        X[4, 0] = float("-inf")
+        X[5, C - 1] = float("nan")
+        X[6] = torch.finfo(t).max
+        q, scale = ops.quantize_rows_fp4(X)
+        check_rows(X, q, scale)
+        back = ops.dequantize_rows_fp4(q, scale, C, dtype=torch.float32)
+        want = fp4.values(*fp4.quantize(X), C).to(torch.float32)             # (6 * 2^126, what float32's largest number becomes, is beyond it)
+        assert bool(same(back, want))
