@@ -30,7 +30,6 @@ struct LayerList;
 struct LayerParams {
   const void* X;
   const void* router;
-  const float* bias;
   const void* up;            // [E, I, J], in 4 bits [E, J, I / 2]
   const void* down;          // [E, J, I], in 4 bits [E, I, J / 2]
   const uint8_t* up_scale;
@@ -40,12 +39,10 @@ struct LayerParams {
   int* experts;
   float* logits;
   float* h;                  // [parts][tokens * k][J]
-  LayerList* list;    // what `up` has found out
+  LayerList* list;           // what `up` has found out
   long long x_row, up_row, us_row, down_row, ds_row;       // elements; in 4 bits bytes
   long long up_far, down_far;      // in 4 bits: bytes from one expert to the next
   int tokens, E, k, I, J;
-  int groups, top_groups, group_top, sigmoid, renormalize;
-  float scale;
   int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
   long long weight_bytes;    // of all experts' matrices, of either product
   int ring_words;            // of weights on their way, in shared memory
@@ -409,7 +406,7 @@ __device__ __forceinline__ void join_groups(const Sums<V> (&acc)[M], float (&sum
       sum[m][v] = x;
     }
 }
-__host__ __device__ constexpr int ahead_of(int V) { return V >= 4 ? 2 : 4; }
+constexpr int kAhead = 4;                    // steps of single elements whose loads go out together
 
 template <typename T, int V, int LANES>
 struct UpShared {
@@ -466,7 +463,7 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
         next();
       }
     } else {
-      accumulate<T, V, M, ahead_of(V)>(acc, W, static_cast<int>(p.up_row), first, kStep, c1, n < p.J, a, c0, stage);
+      accumulate<T, V, M, kAhead>(acc, W, static_cast<int>(p.up_row), first, kStep, c1, n < p.J, a, c0, stage);
     }
   }
   float sum[M][V];
@@ -650,7 +647,7 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
       next();
     }
   } else {
-    accumulate<T, V, M, ahead_of(V)>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, static_cast<int>(p.down_row), begin + lane / LANES * 4, kStep, end, n < p.I, a, base, []() {});
+    accumulate<T, V, M, kAhead>(acc, static_cast<const T*>(p.down) + item.expert * (p.down_row * p.J) + n, static_cast<int>(p.down_row), begin + lane / LANES * 4, kStep, end, n < p.I, a, base, []() {});
   }
   float sum[M][V];
   join_groups<LANES, V, M>(acc, sum);
@@ -1250,13 +1247,13 @@ cudaError_t down4_launch(const LayerParams& p, const Matrix4& t, const Rows4& x,
   return launch_cluster(few_down4_kernel<T, LAYOUT>, tiles * size, kThreads4, size, smem, st, p, t, x);
 }
 template <typename T>
-cudaError_t layer4_t(LayerParams p, const egs_route& route, bool up_cn, bool down_cn, const Rows4& x, const Rows4& h, cudaStream_t st) {
+cudaError_t layer4_t(LayerParams p, const float* bias, const egs_route& route, bool up_cn, bool down_cn, const Rows4& x, const Rows4& h, cudaStream_t st) {
   prepare<T>(&p);
   const int logits_ctas = (p.E + 7) / 8;
   count_launch();
   cudaError_t err = launch_kernel(few_logits4_kernel<T>, dim3(logits_ctas + (fp4_blocks(p.I) + 31) / 32, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p, x, logits_ctas);
   if (err != cudaSuccess) return err;
-  if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
+  if ((err = launch_route_tokens(p.logits, bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
   p.by_tiles = Div((p.J + kTile4 - 1) / kTile4);
   p.by_stages = Div(stages_of(p.J));
   auto words = [](const uint8_t* scale, long long row) { return row % 4 == 0 && on(scale, 4); };
@@ -1278,13 +1275,13 @@ cudaError_t layer4_t(LayerParams p, const egs_route& route, bool up_cn, bool dow
 }
 
 template <typename T>
-cudaError_t layer_t(LayerParams p, const egs_route& route, cudaStream_t st) {
+cudaError_t layer_t(LayerParams p, const float* bias, const egs_route& route, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T), kLanes = 8;
   prepare<T>(&p);
   count_launch();
   cudaError_t err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
   if (err != cudaSuccess) return err;
-  if ((err = launch_route_tokens(p.logits, p.bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
+  if ((err = launch_route_tokens(p.logits, bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
   // One width for both products: the parts of `up` are counted by it.  16-byte vectors where rows begin on them.  Rows that do not are shifted together in 16 bits from
   // 128 Ki elements of an expert's matrix on, and else come element by element (us a call, shifted and not: 8 tokens, 2047 x 511, 62 and 102; 4 tokens, 500 x 301,
   // 18.8 and 19.5, 330 x 201, 18.0 and 16.9; 4 tokens in float32, 1001 x 500, 34.3 and 34.1).
@@ -1335,17 +1332,15 @@ cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, v
   p.h = p.logits + logits_words(r);
   p.x_row = f.x_row;
   p.tokens = static_cast<int>(r.tokens); p.E = r.E; p.k = r.top_k; p.I = f.I; p.J = f.J;
-  p.bias = f.bias; p.groups = r.groups; p.top_groups = r.top_groups; p.group_top = r.group_top;
-  p.sigmoid = r.score == EGS_SCORE_SIGMOID; p.renormalize = r.renormalize; p.scale = r.scale;
   if (f.up_scale) {
     p.up_row = f.up_row; p.us_row = f.us_row; p.down_row = f.down_row; p.ds_row = f.ds_row;
     p.up_far = f.up_far; p.down_far = f.down_far;
     const Rows4 x = rows4_at(p.h, r.tokens, f.I), h = rows4_at(reinterpret_cast<char*>(p.h) + rows4_bytes(r.tokens, f.I), static_cast<long long>(p.tokens) * p.k, f.J);
-    return dtype == EGS_F16 ? layer4_t<__half>(p, r, f.up_cn, f.down_cn, x, h, st) : dtype == EGS_BF16 ? layer4_t<__nv_bfloat16>(p, r, f.up_cn, f.down_cn, x, h, st) : layer4_t<float>(p, r, f.up_cn, f.down_cn, x, h, st);
+    return dtype == EGS_F16 ? layer4_t<__half>(p, f.bias, r, f.up_cn, f.down_cn, x, h, st) : dtype == EGS_BF16 ? layer4_t<__nv_bfloat16>(p, f.bias, r, f.up_cn, f.down_cn, x, h, st) : layer4_t<float>(p, f.bias, r, f.up_cn, f.down_cn, x, h, st);
   }
   p.up_row = p.J;
   p.down_row = p.I;
-  return dtype == EGS_F16 ? layer_t<__half>(p, r, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, r, st) : layer_t<float>(p, r, st);
+  return dtype == EGS_F16 ? layer_t<__half>(p, f.bias, r, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, f.bias, r, st) : layer_t<float>(p, f.bias, r, st);
 }
 
 }  // namespace egs
