@@ -23,7 +23,7 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMost = EGS_MAX_FEW_SLOTS, kRows = 4;      // slots; tokens that share a read of the weights
 constexpr int kUpThreads = 256, kUpWarps = kUpThreads / 32, kUpGrid = 296, kUpPart = 1024;
 constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
-constexpr int kMostParts = 8;
+constexpr int kMostParts = 8, kMostSplits = 4;
 constexpr int kFixedRows = 128;              // of a unit, in rows of its tile: 16 KB of weights
 
 struct LayerList;
@@ -47,6 +47,8 @@ struct LayerParams {
   long long weight_bytes;    // of all experts' matrices, of either product
   int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
+  int splits;                // ... clusters that a tile's contraction is cut into beside their CTAs
+  float* sums;               // ... theirs, [splits][tokens][I], where there are several
   Div by_tiles, by_k, by_stages;
 };
 
@@ -600,19 +602,24 @@ __device__ __forceinline__ void activation(const LayerParams& p, int parts, long
 // out[t, n0 + n] from this CTA's sums: sum(t, n, v) adds four of them to v.  Every CTA of a cluster has a share of the outputs, and the others hand it their
 // sums: to, room for them, [CTAs][outputs of a share] of shared memory.
 template <typename T, int TILE, class Sum>
-__device__ __forceinline__ void put_out(const LayerParams& p, float* to, int n0, Sum&& sum) {
+__device__ __forceinline__ void put_out(const LayerParams& p, float* to, int n0, int split, Sum&& sum) {
   const int rank = cluster_rank(), size = cluster_size(), all = p.tokens * TILE, own = (all / 4 + size - 1) / size * 4;
+  auto put = [&](int t, int n, float v) {
+    if (n0 + n >= p.I) return;
+    const long long at = static_cast<long long>(t) * p.I + n0 + n;
+    if (gridDim.y > 1) p.sums[split * (static_cast<long long>(p.tokens) * p.I) + at] = v;
+    else static_cast<T*>(p.out)[at] = from_f32<T>(v);
+  };
   if (size > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all have begun
   for (int i = threadIdx.x * 4; i < all; i += blockDim.x * 4) {
     const int t = i / TILE, n = i % TILE;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     sum(t, n, v);
     if (size == 1) {
-      T* out = static_cast<T*>(p.out) + static_cast<long long>(t) * p.I + n0 + n;
-      if (n0 + n < p.I) out[0] = from_f32<T>(v.x);
-      if (n0 + n + 1 < p.I) out[1] = from_f32<T>(v.y);
-      if (n0 + n + 2 < p.I) out[2] = from_f32<T>(v.z);
-      if (n0 + n + 3 < p.I) out[3] = from_f32<T>(v.w);
+      put(t, n, v.x);
+      put(t, n + 1, v.y);
+      put(t, n + 2, v.z);
+      put(t, n + 3, v.w);
     } else {
       const int owner = i / own;
       asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(in_cta(to + rank * own + i - owner * own, owner)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
@@ -624,7 +631,7 @@ __device__ __forceinline__ void put_out(const LayerParams& p, float* to, int n0,
     const int x = rank * own + i, t = x / TILE, n = x % TILE;
     float v = to[i];
     for (int r = 1; r < size; ++r) v += to[r * own + i];
-    if (n0 + n < p.I) static_cast<T*>(p.out)[static_cast<long long>(t) * p.I + n0 + n] = from_f32<T>(v);
+    put(t, n, v);
   }
 }
 
@@ -677,11 +684,11 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
   pdl_trigger();
   begin_down(p, &items);
   const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n0 = blockIdx.x / size * kTile;
+  const int split = blockIdx.y, n0 = blockIdx.x / size * kTile;
   float* act = layer_smem + p.ring_words;
   float* part = act + p.act_floats;
   const int parts = items.parts;
-  const int length = ((p.J + size - 1) / size + 3) & ~3, begin = min(p.J, rank * length), end = min(p.J, begin + length);
+  const int ctas = size * p.splits, length = ((p.J + ctas - 1) / ctas + 3) & ~3, begin = min(p.J, (split * size + rank) * length), end = min(p.J, begin + length);
   const int room = min(length, p.act_floats / slots & ~3);
   int shares_log2 = 0;                         // warps that have an item's contraction in turn
   while (items.count << (shares_log2 + 1) <= kDownWarps && length >> shares_log2 >= 64) ++shares_log2;
@@ -749,12 +756,27 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
     }
   }
   __syncthreads();
-  put_out<T, kTile>(p, part + max(4 * kDownWarps, slots) * kTile, n0, [&](int t, int n, float4& v) {
+  put_out<T, kTile>(p, part + max(4 * kDownWarps, slots) * kTile, n0, split, [&](int t, int n, float4& v) {
     for (int j = 0; j < p.k << shares_log2; ++j) {
       const float4 x = *reinterpret_cast<const float4*>(part + ((j & ((1 << shares_log2) - 1)) * slots + t * p.k + (j >> shares_log2)) * kTile + n);
       v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
     }
   });
+}
+
+// The splits' sums, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ LayerParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const long long all = static_cast<long long>(p.tokens) * p.I, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= all) return;
+  float v[kMostSplits];
+#pragma unroll
+  for (int s = 0; s < kMostSplits; ++s) v[s] = s < p.splits ? p.sums[s * all + i] : 0.f;
+#pragma unroll
+  for (int s = 1; s < kMostSplits; ++s) v[0] += v[s];
+  static_cast<T*>(p.out)[i] = from_f32<T>(v[0]);
 }
 
 // ---- weights in 4 bits -------------------------------------------------------------------------------------------------
@@ -1151,7 +1173,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
     }
   }
   __syncthreads();
-  put_out<T, kTile4>(p, part + kWarps4 * p.tokens * kTile4, n0, [&](int t, int n, float4& v) {
+  put_out<T, kTile4>(p, part + kWarps4 * p.tokens * kTile4, n0, 0, [&](int t, int n, float4& v) {
 #pragma unroll
     for (int w = 0; w < kWarps4; ++w) {
       const float4 y = *reinterpret_cast<const float4*>(part + (w * p.tokens + t) * kTile4 + n);
@@ -1161,10 +1183,10 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
-constexpr size_t kDownSmem = 220 * 1024;
+constexpr size_t kDownSmem = 220 * 1024, kHalfSmem = 104 * 1024;      // (227 KB an SM, of which static ones and a KB a CTA take some)
 
 template <class... Params, class... Args>
-cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, unsigned cluster, size_t smem, cudaStream_t st, Args... args) {
+cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, unsigned block, unsigned cluster, size_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -1190,20 +1212,41 @@ unsigned cluster_of(int tiles, int J) {
   return size;
 }
 
+// Clusters for a tile: several where one leaves half of the SMs or more unused and there is enough to read to pay for another launch.  (us a call, one cluster
+// and several: 19 tokens, 3 of 10 experts, 256 x 1792, 38.3 and 28.0; 8 tokens, 4 of 64, 512 x 2048, 41.1 and 37.5; 9 tokens, 2 of 22, 160 x 1760 in float32, 22.6 and 20.7; 4 tokens,
+// 2 of 10, 128 x 960, which is less, 14.0 and 14.5.)
+int splits_of(int tiles, const LayerParams& p) {
+  const int experts = p.tokens * p.k < p.E ? p.tokens * p.k : p.E;
+  if (static_cast<long long>(experts) * p.I * p.J < 2 << 20) return 1;
+  int best = 1;
+  unsigned most = tiles * cluster_of(tiles, p.J);
+  for (int n = 2; n <= kMostSplits && most <= 74; ++n) {
+    const unsigned ctas = tiles * n * cluster_of(tiles * n, p.J / (2 * n));      // (64 contraction elements a CTA at least)
+    if (2 * ctas >= 3 * most) {
+      most = ctas;
+      best = n;
+    }
+  }
+  return best;
+}
+
 template <auto kernel, typename T>
 cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   const int tiles = (p.I + tile - 1) / tile, slots = p.tokens * p.k;
   cudaError_t err = ensure_smem_optin<kernel>(static_cast<int>(kDownSmem));
   if (err != cudaSuccess) return err;
-  const unsigned size = cluster_of(tiles, p.J);
+  p.splits = splits_of(tiles, p);
+  const unsigned size = p.splits > 1 ? cluster_of(tiles * p.splits, p.J / (2 * p.splits)) : cluster_of(tiles, p.J);
   const size_t ring = static_cast<size_t>(p.ring_words) * 4;
   const size_t part = static_cast<size_t>((slots < 4 * kDownWarps ? 4 * kDownWarps : slots) + (size > 1 ? p.tokens : 0)) * tile * sizeof(float) + 4 * size * sizeof(float);
-  size_t act = static_cast<size_t>(slots) * (p.J / size + 36) * sizeof(float);
+  size_t act = static_cast<size_t>(slots) * (p.J / (size * p.splits) + 36) * sizeof(float);
   act = (act + 15) & ~static_cast<size_t>(15);
   if (act > kDownSmem - part - ring) act = kDownSmem - part - ring;
   p.act_floats = static_cast<int>(act / sizeof(float));
-  count_launch();
-  return launch_cluster(kernel, tiles * size, kDownThreads, size, ring + act + part, st, p);
+  count_launch(p.splits > 1 ? 2 : 1);
+  err = launch_cluster(kernel, dim3(tiles * size, p.splits), kDownThreads, size, ring + act + part, st, p);
+  if (err != cudaSuccess || p.splits == 1) return err;
+  return launch_kernel(few_join_kernel<T>, dim3(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.I + 255) / 256)), 256, 0, st, true, p);
 }
 
 template <auto kernel>
@@ -1234,17 +1277,24 @@ cudaError_t up4_launch(const LayerParams& p, const Matrix4& t, const Rows4& x, c
   count_launch();
   return launch_kernel(few_up4_kernel<LAYOUT>, dim3(kUpGrid), kThreads4, kRing4, st, true, p, t, x, to);
 }
-// CTAs of a cluster: as many as two an SM leave room for, a stage for a warp at least.
+// CTAs of a cluster: as many as two an SM leave room for (33 clusters of eight, 71 of four, 148 of two), a stage for a warp at least; one an SM where the tokens' sums take
+// more shared memory.
 template <typename T, int LAYOUT>
-cudaError_t down4_launch(const LayerParams& p, const Matrix4& t, const Rows4& x, cudaStream_t st) {
+cudaError_t down4_launch(LayerParams p, const Matrix4& t, const Rows4& x, cudaStream_t st) {
   const int tiles = (p.I + kTile4 - 1) / kTile4, turns = p.tokens * p.k * stages_of(p.J);
+  const size_t smem = kRing4 + static_cast<size_t>(kWarps4 + 1) * p.tokens * kTile4 * sizeof(float) + 128;
   unsigned size = 8;
-  while (size > 1 && (tiles * size > 256 || turns < static_cast<int>(size / 2) * kWarps4)) size /= 2;
-  const size_t smem = kRing4 + static_cast<size_t>(kWarps4 + 1) * p.tokens * kTile4 * sizeof(float);
-  cudaError_t err = ensure_smem_optin<few_down4_kernel<T, LAYOUT>>(static_cast<int>(kRing4 + (kWarps4 + 1) * 32 * kTile4 * sizeof(float)));
+  if (smem > kHalfSmem) {
+    size = cluster_of(tiles, 32 * 8);
+  } else {
+    while (size > 1 && tiles * size > 256) size /= 2;
+  }
+  while (size > 1 && turns <= static_cast<int>(size / 2) * kWarps4) size /= 2;
+  p.splits = 1;
+  cudaError_t err = ensure_smem_optin<few_down4_kernel<T, LAYOUT>>(static_cast<int>(kRing4 + (kWarps4 + 1) * 32 * kTile4 * sizeof(float) + 128));
   if (err != cudaSuccess) return err;
   count_launch();
-  return launch_cluster(few_down4_kernel<T, LAYOUT>, tiles * size, kThreads4, size, smem, st, p, t, x);
+  return launch_cluster(few_down4_kernel<T, LAYOUT>, dim3(tiles * size), kThreads4, size, smem, st, p, t, x);
 }
 template <typename T>
 cudaError_t layer4_t(LayerParams p, const float* bias, const egs_route& route, bool up_cn, bool down_cn, const Rows4& x, const Rows4& h, cudaStream_t st) {
@@ -1320,7 +1370,8 @@ Rows4 rows4_at(void* from, long long rows, int C) {
 size_t few_layer_workspace(const egs_route& r, int I, int J) {
   const long long slots = static_cast<long long>(r.tokens) * r.top_k;
   const size_t parts = static_cast<size_t>(kMostParts) * slots * J * sizeof(float), fp4 = rows4_bytes(r.tokens, I) + rows4_bytes(slots, J);
-  return sizeof(LayerList) + logits_words(r) * sizeof(float) + (parts > fp4 ? parts : fp4);
+  const size_t sums = static_cast<size_t>(kMostSplits) * r.tokens * I * sizeof(float);
+  return sizeof(LayerList) + logits_words(r) * sizeof(float) + (parts + sums > fp4 ? parts + sums : fp4);
 }
 
 cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st) {
@@ -1340,6 +1391,7 @@ cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, v
   }
   p.up_row = p.J;
   p.down_row = p.I;
+  p.sums = p.h + static_cast<size_t>(kMostParts) * p.tokens * p.k * p.J;
   return dtype == EGS_F16 ? layer_t<__half>(p, f.bias, r, st) : dtype == EGS_BF16 ? layer_t<__nv_bfloat16>(p, f.bias, r, st) : layer_t<float>(p, f.bias, r, st);
 }
 

@@ -249,6 +249,20 @@ def test_blocks_that_are_not_numbers():
     assert out[2].isnan().all() and torch.equal(out[rest], good[rest]) and torch.equal(other[rest], ids[rest])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,E,k,I,J", [(19, 10, 3, 256, 1792), (19, 10, 3, 250, 1793), (2, 4, 4, 64, 9000), (32, 3, 1, 40, 20000), (8, 16, 4, 520, 2048)])
+def test_wide_contraction_of_the_last_product(dtype, tokens, E, k, I, J):
+    """Few columns and a long contraction: several clusters for a tile of columns."""
+    t = TYPES[dtype]
+    x, router = randn(tokens, I, seed=1, dtype=t), (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    up, down = (randn(E, I, J, seed=3) * 2 / I ** 0.5).to(t), (randn(E, J, I, seed=4) / J ** 0.5).to(t)
+    out, w, ids = ops.routed_experts_few(x, router, up, down, k)
+    want, off = layer64(x.double(), w.double(), ids.long(), up.double(), down.double())
+    worst = ((out.double() - want).abs() - off - want.abs() * (torch.finfo(t).eps / 2) - (2.0 ** -25 if dtype == "f16" else 0)).max().item()
+    assert worst <= 0, (worst, (out.double() - want).abs().max().item())
+    assert torch.equal(out, ops.routed_experts_few(x, router, up, down, k)[0])
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)
