@@ -2,7 +2,7 @@
 // reading the weights of the experts that were chosen, each of them once, with all SMs.
 //
 //   choice   two kernels: the logits, a warp two experts' rows of the router and four tokens, and egs_choice.cu's.  (In one kernel with `up`, each CTA
-//            choosing for itself, or in one with each other, by a cluster of eight CTAs, they took 1 to 6 us more.)
+//            choosing for itself, or in one with each other, by a cluster of eight CTAs or one, they took 0.5 to 6 us more.)
 //   up       units of (an expert's up to four tokens) x (a tile of columns) x (a part of the contraction) go round
 //            the CTAs; float32 sums of parts
 //   down     a cluster has a tile of the output's columns, its CTAs the contraction in parts; warps have the experts' tokens in turn.  The parts' sums
@@ -234,6 +234,18 @@ __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__
 __device__ __forceinline__ void begin_up(const LayerParams& p, Items* s) {
   pdl_wait();
   pdl_trigger();
+  if (p.tokens == 1) {                         // its experts differ
+    const int i = threadIdx.x;
+    if (i < p.k) {
+      Item x{p.experts[i], 1};
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) x.slot[r] = static_cast<short>(i);
+      s->item[i] = x;
+    }
+    if (i == 0) s->count = p.k;
+    __syncthreads();
+    return;
+  }
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) s->tokens[e] = 0u;
   for (int i = threadIdx.x; i < p.tokens * p.k; i += blockDim.x) s->ids[i] = p.experts[i];
   __syncthreads();
