@@ -9,9 +9,9 @@
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
 //            CTAs' in theirs: the same bits in every run.
 //
-// us a call in a graph, new weights each time: 1 token, 8 of 64 experts, 2048 x 512 bf16 (33.8 MB, 5.2 at the copy's rate) 18.0, of which logits 2, choice 2, `up` 4.2 and `down`
-// 6.7 on the device, the rest between them; 16 tokens, 4 of 64, 1024 x 256 (43 MB) 27.7.  Products run at 4 to 5 TB/s once weights come; what is left is latency: four
-// launches, the list, the first weights, the join of a cluster.  Tried: the other product's weights to the L2 ahead (no gain), 16-bit products on mma.sync (1 us more; float32 sums by
+// us a call in a graph, new weights each time: 1 token, 8 of 64 experts, 2048 x 512 bf16 (33.8 MB, 5.2 at the copy's rate) 17.5, of which logits 2, choice 2, `up` 4.2 and `down`
+// 6.7 on the device, the rest between them; 16 tokens, 4 of 64, 1024 x 256 (43 MB) 28.1.  Products run at 4 to 5 TB/s once weights come; what is left is latency: four
+// launches, the list, the first weights, the join of a cluster.  Tried: the other product's weights to the L2 ahead (no gain), 16-bit products on mma.sync (1 us more: float32 sums by
 // packed FMA are not what bounds it), weights through registers (3.4 TB/s), rings of 2, 4 and 6 steps (equal, equal, slower), tiles of 128 columns (20 us -> 24.6).
 #include "egs_fp4.cuh"
 

@@ -263,6 +263,42 @@ def test_wide_contraction_of_the_last_product(dtype, tokens, E, k, I, J):
     assert torch.equal(out, ops.routed_experts_few(x, router, up, down, k)[0])
 
 
+def test_two_streams_and_two_graphs_at_once():
+    """Calls on two streams, and replays of two graphs on them, that run beside each other: each has a workspace of its own."""
+    E, k, I, J = 24, 3, 512, 320
+    router, up, down = randn(E, I, seed=2, dtype=torch.bfloat16), randn(E, I, J, seed=3, dtype=torch.bfloat16), randn(E, J, I, seed=4, dtype=torch.bfloat16)
+    (u, us), (d, ds) = grid4(E, J, I, seed=3, low=120, high=124), grid4(E, I, J, seed=4)
+    xs = [randn(t, I, seed=10 + t, dtype=torch.bfloat16) for t in (1, 5, 16, 32)]
+
+    def both(x):
+        return ops.routed_experts_few(x, router, up, down, k)[0], ops.routed_experts_few(x, router, u, d, k, up_scale=us, down_scale=ds)[0]
+
+    want = [both(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for n in range(12):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[s].append(both(xs[(n + s) % 4]))
+    graphs = []
+    for s in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[s]):
+            graphs.append((g, [both(x) for x in xs]))
+    torch.cuda.synchronize()
+    for n in range(6):
+        for (g, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+    torch.cuda.synchronize()
+    for s in range(2):
+        for n in range(12):
+            assert all(torch.equal(a, b) for a, b in zip(got[s][n], want[(n + s) % 4]))
+        for out, ref in zip(graphs[s][1], want):
+            assert all(torch.equal(a, b) for a, b in zip(out, ref))
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)
