@@ -9,8 +9,9 @@
 //            are joined, activated and weighted on the way into shared memory; a token's products are added in the order of its choices, the
 //            CTAs' in theirs: the same bits in every run.
 //
-// us a call in a graph, new weights each time: 1 token, 8 of 64 experts, 2048 x 512 bf16 (33.8 MB, 5.2 at the copy's rate) 17.5, of which logits 2, choice 2, `up` 4.2 and `down`
-// 6.7 on the device, the rest between them; 16 tokens, 4 of 64, 1024 x 256 (43 MB) 28.1.  Products run at 4 to 5 TB/s once weights come; what is left is latency: four
+// us a call in a graph, new weights each time: 1 token, 8 of 64 experts, 2048 x 512 bf16 (33.8 MB, 5.2 at the copy's rate) 17.2, of which logits 2, choice 2, `up` 4.2 and `down`
+// 6.7 on the device, the rest between them; 16 tokens, 4 of 64, 1024 x 256 (43 MB) 26.0
+// (28.2 with a last product that waited before it listed the items and asked for weights).  Products run at 4 to 5 TB/s once weights come; what is left is latency: four
 // launches, the list, the first weights, the join of a cluster.  Tried: the other product's weights to the L2 ahead (no gain), 16-bit products on mma.sync (1 us more: float32 sums by
 // packed FMA are not what bounds it), weights through registers (3.4 TB/s), rings of 2, 4 and 6 steps (equal, equal, slower), tiles of 128 columns (20 us -> 24.6).
 #include "egs_fp4.cuh"
@@ -26,7 +27,7 @@ constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
 constexpr int kMostParts = 8, kMostSplits = 4;
 constexpr int kFixedRows = 128;              // of a unit, in rows of its tile: 16 KB of weights
 
-struct LayerList;
+struct Items;
 struct LayerParams {
   const void* X;
   const void* router;
@@ -39,7 +40,7 @@ struct LayerParams {
   int* experts;
   float* logits;
   float* h;                  // [parts][tokens * k][J]
-  LayerList* list;           // what `up` has found out
+  Items* list;               // in 4 bits: from `up`
   long long x_row, up_row, us_row, down_row, ds_row;       // elements; in 4 bits bytes
   long long up_far, down_far;      // in 4 bits: bytes from one expert to the next
   int tokens, E, k, I, J;
@@ -57,27 +58,25 @@ struct alignas(16) Item {
   int expert, rows;
   short slot[kRows];
 };
-struct Items {
+struct alignas(16) Items {
   Item item[kMost];
+  int count;
+};
+// What is needed while they are listed.
+struct Scratch {
   int ids[kMost];
   unsigned tokens[EGS_MAX_EXPERTS];
   int first[EGS_MAX_EXPERTS];    // an expert's first item
-  int count;
 };
-struct LayerList {
-  int count, parts;              // items, parts that sums of `up` are in
-  int pad[2];
-  Item item[kMost];
-};
-// From the chosen experts (s->ids); by all threads, which have synchronised behind the ids and s->tokens = 0.
-__device__ __forceinline__ void list_items(const LayerParams& p, Items* s) {
+// From the chosen experts (w->ids); by all threads, which have synchronised behind the ids and w->tokens = 0.
+__device__ __forceinline__ void list_chosen(const LayerParams& p, Items* s, Scratch* w) {
   const int tid = threadIdx.x, n = p.tokens * p.k;
-  for (int i = tid; i < n; i += blockDim.x) atomicOr(&s->tokens[s->ids[i]], 1u << p.by_k.quotient(i));
+  for (int i = tid; i < n; i += blockDim.x) atomicOr(&w->tokens[w->ids[i]], 1u << p.by_k.quotient(i));
   __syncthreads();
   if (tid < 32) {
     int before = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + tid, own = e < p.E ? (__popc(s->tokens[e]) + kRows - 1) / kRows : 0;
+      const int e = e0 + tid, own = e < p.E ? (__popc(w->tokens[e]) + kRows - 1) / kRows : 0;
       int at = before;
 #pragma unroll
       for (int bit = 0; bit < 4; ++bit) {        // (eight items at most)
@@ -85,16 +84,16 @@ __device__ __forceinline__ void list_items(const LayerParams& p, Items* s) {
         at += __popc(has & ((1u << tid) - 1u)) << bit;
         before += __popc(has) << bit;
       }
-      if (e < p.E) s->first[e] = at;
+      if (e < p.E) w->first[e] = at;
     }
     if (tid == 0) s->count = before;
   }
   __syncthreads();
   for (int i = tid; i < n; i += blockDim.x) {
-    const int e = s->ids[i];
-    const unsigned tokens = s->tokens[e];
+    const int e = w->ids[i];
+    const unsigned tokens = w->tokens[e];
     const int place = __popc(tokens & ((1u << p.by_k.quotient(i)) - 1u)), rows = min(kRows, __popc(tokens) - place / kRows * kRows);
-    Item& x = s->item[s->first[e] + place / kRows];
+    Item& x = s->item[w->first[e] + place / kRows];
     x.slot[place % kRows] = static_cast<short>(i);
     if (place % kRows == 0) {
       x.expert = e;
@@ -105,14 +104,24 @@ __device__ __forceinline__ void list_items(const LayerParams& p, Items* s) {
   __syncthreads();
 }
 
-// ... for `down`
-__device__ __forceinline__ void publish(const LayerParams& p, const Items& s, int parts) {
-  if (blockIdx.x) return;
-  for (int i = threadIdx.x; i < s.count; i += blockDim.x) p.list->item[i] = s.item[i];
-  if (threadIdx.x == 0) {
-    p.list->count = s.count;
-    p.list->parts = parts;
+// The items of the choice; by all threads.
+__device__ __forceinline__ void list_items(const LayerParams& p, Items* s, Scratch* w) {
+  if (p.tokens == 1) {                         // its experts differ
+    const int i = threadIdx.x;
+    if (i < p.k) {
+      Item x{__ldcg(p.experts + i), 1};
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) x.slot[r] = static_cast<short>(i);
+      s->item[i] = x;
+    }
+    if (i == 0) s->count = p.k;
+    __syncthreads();
+    return;
   }
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) w->tokens[e] = 0u;
+  for (int i = threadIdx.x; i < p.tokens * p.k; i += blockDim.x) w->ids[i] = __ldcg(p.experts + i);
+  __syncthreads();
+  list_chosen(p, s, w);
 }
 
 // Parts that the contraction of `up` is cut into: the fewest rounds of the CTAs, a unit costing as much as kFixedRows beside its own.
@@ -228,28 +237,6 @@ __global__ void __launch_bounds__(128) few_logits_kernel(const __grid_constant__
   pdl_wait();
   pdl_trigger();
   logits_by_warps<T>(p, (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2, blockIdx.y * kRows);
-}
-
-// What both `up` kernels begin with: the items from the choice.
-__device__ __forceinline__ void begin_up(const LayerParams& p, Items* s) {
-  pdl_wait();
-  pdl_trigger();
-  if (p.tokens == 1) {                         // its experts differ
-    const int i = threadIdx.x;
-    if (i < p.k) {
-      Item x{p.experts[i], 1};
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) x.slot[r] = static_cast<short>(i);
-      s->item[i] = x;
-    }
-    if (i == 0) s->count = p.k;
-    __syncthreads();
-    return;
-  }
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) s->tokens[e] = 0u;
-  for (int i = threadIdx.x; i < p.tokens * p.k; i += blockDim.x) s->ids[i] = p.experts[i];
-  __syncthreads();
-  list_items(p, s);
 }
 
 // ---- products along rows of the weights ([contraction, columns]) -----------------------------------------------------
@@ -425,6 +412,7 @@ constexpr int kAhead = 4;                    // steps of single elements whose l
 template <typename T, int V, int LANES>
 struct UpShared {
   Items items;
+  Scratch scratch;
   alignas(16) float x[kRows][kUpPart];
   float sums[kUpWarps][kRows][LANES * V];
 };
@@ -509,9 +497,10 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
   constexpr bool kRing = V == 16 / sizeof(T);
   extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ UpShared<T, V, LANES> s;
-  begin_up(p, &s.items);
+  pdl_wait();
+  pdl_trigger();
+  list_items(p, &s.items, &s.scratch);
   const int parts = parts_of(s.items.count * p.by_tiles.d, p.I);
-  publish(p, s.items, parts);
   const int all = s.items.count * p.by_tiles.d, units = all * parts, length = ((p.I + parts - 1) / parts + 3) & ~3;
   Ring<kUpThreads, kUpDepth, LANES, SHIFT> ring(layer_table);
   // what is asked for next: rows c .. c + 3 of unit `coming`
@@ -563,23 +552,15 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
   }
 }
 
-// What `up` has found out, and the weights, in shared memory.
-struct DownShared {
-  Item item[kMost];
+// The items and the choice's weights, in shared memory.  `down` calls this ahead of its wait: what the choice has written is there, since `up` lets its dependents begin when all of its
+// CTAs have waited for the choice, and with it for all that came before.  So are weights of the layer.
+struct DownShared : Items {
   float weights[kMost];
-  int count, parts;
 };
-__device__ __forceinline__ void begin_down(const LayerParams& p, DownShared* s) {
-  const int tid = threadIdx.x, slots = p.tokens * p.k;       // (items are no more than slots)
-  if (tid < slots) {
-    s->item[tid] = p.list->item[tid];
-    s->weights[tid] = p.weights[tid];
-  }
-  if (tid == 0) {
-    s->count = p.list->count;
-    s->parts = p.list->parts;
-  }
-  __syncthreads();
+__device__ __forceinline__ void begin_down(const LayerParams& p, DownShared* s, void* scratch) {
+  for (int i = threadIdx.x; i < p.tokens * p.k; i += blockDim.x) s->weights[i] = __ldcg(p.weights + i);
+  list_items(p, s, static_cast<Scratch*>(scratch));
+  __syncthreads();                             // (and the scratch is free)
 }
 
 // N neighbouring sums of a slot's parts from h[at] on (those that exist: left), activated.  All loads go out before the first sum.
@@ -692,14 +673,12 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
   extern __shared__ __align__(16) float layer_smem[];
   __shared__ DownShared items;
   if (cluster_size() > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  pdl_wait();
-  pdl_trigger();
-  begin_down(p, &items);
+  begin_down(p, &items, layer_smem);
   const int slots = p.tokens * p.k, rank = cluster_rank(), size = cluster_size(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.y, n0 = blockIdx.x / size * kTile;
   float* act = layer_smem + p.ring_words;
   float* part = act + p.act_floats;
-  const int parts = items.parts;
+  const int parts = parts_of(items.count * p.by_tiles.d, p.I);
   const int ctas = size * p.splits, length = ((p.J + ctas - 1) / ctas + 3) & ~3, begin = min(p.J, (split * size + rank) * length), end = min(p.J, begin + length);
   const int room = min(length, p.act_floats / slots & ~3);
   int shares_log2 = 0;                         // warps that have an item's contraction in turn
@@ -747,7 +726,11 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
 #pragma unroll 1
       for (int d = 0; d < kDownDepth; ++d) next();
     }
-    // activations, four at a time; the first weights are on their way meanwhile
+    if (c0 == begin) {                         // the first weights are on their way
+      pdl_wait();
+      pdl_trigger();
+    }
+    // activations, four at a time
     __syncthreads();
     for (int i = tid; i < slots * (width / 4); i += kDownThreads) {
       const int slot = i / (width / 4), at = (i - slot * (width / 4)) * 4;
@@ -1079,6 +1062,7 @@ __global__ void __launch_bounds__(128) few_logits4_kernel(const __grid_constant_
 // the other product's contraction, brought into 4 bits.
 struct Up4Shared {
   Items items;
+  Scratch scratch;
   float sums[2][kWarps4][kRows][kTile4];
 };
 template <int LAYOUT>
@@ -1086,8 +1070,13 @@ __global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_cons
   extern __shared__ __align__(16) uint32_t layer_table[];
   __shared__ Up4Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  begin_up(p, &s.items);
-  publish(p, s.items, 1);
+  pdl_wait();
+  pdl_trigger();
+  list_items(p, &s.items, &s.scratch);
+  if (blockIdx.x == 0) {
+    for (int i = tid; i < s.items.count; i += kThreads4) p.list->item[i] = s.items.item[i];
+    if (tid == 0) p.list->count = s.items.count;
+  }
   const int tiles = p.by_tiles.d, units = s.items.count * tiles, stages = stages_of(p.I);
   Stages<LAYOUT> ring(layer_table, t);
   int coming = warp < stages ? blockIdx.x : units, stage = stages;       // of what is asked for next; (a contraction of few stages leaves warps idle)
@@ -1148,7 +1137,12 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
   for (int i = tid; i < kWarps4 * p.tokens * kTile4; i += kThreads4) part[i] = 0.f;
   pdl_wait();
   pdl_trigger();
-  begin_down(p, &items);
+  for (int i = tid; i < p.tokens * p.k; i += kThreads4) {       // (items are no more than slots)
+    items.item[i] = p.list->item[i];
+    items.weights[i] = p.weights[i];
+  }
+  if (tid == 0) items.count = p.list->count;
+  __syncthreads();
   const int stages = stages_of(p.J), all = items.count * stages, step = size * kWarps4;
   Stages<LAYOUT> ring(layer_smem, t);
   int coming = rank * kWarps4 + warp;
@@ -1195,7 +1189,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------
-constexpr size_t kDownSmem = 220 * 1024, kHalfSmem = 104 * 1024;      // (227 KB an SM, of which static ones and a KB a CTA take some)
+constexpr size_t kDownSmem = 218 * 1024, kHalfSmem = 104 * 1024;      // (227 KB an SM, of which static ones and a KB a CTA take some)
 
 template <class... Params, class... Args>
 cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, unsigned block, unsigned cluster, size_t smem, cudaStream_t st, Args... args) {
@@ -1256,7 +1250,8 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   if (act > kDownSmem - part - ring) act = kDownSmem - part - ring;
   p.act_floats = static_cast<int>(act / sizeof(float));
   count_launch(p.splits > 1 ? 2 : 1);
-  err = launch_cluster(kernel, dim3(tiles * size, p.splits), kDownThreads, size, ring + act + part, st, p);
+  const size_t smem = ring + act + part;       // (what the items are listed with lies at its begin first)
+  err = launch_cluster(kernel, dim3(tiles * size, p.splits), kDownThreads, size, smem > sizeof(Scratch) ? smem : sizeof(Scratch), st, p);
   if (err != cudaSuccess || p.splits == 1) return err;
   return launch_kernel(few_join_kernel<T>, dim3(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.I + 255) / 256)), 256, 0, st, true, p);
 }
@@ -1383,14 +1378,14 @@ size_t few_layer_workspace(const egs_route& r, int I, int J) {
   const long long slots = static_cast<long long>(r.tokens) * r.top_k;
   const size_t parts = static_cast<size_t>(kMostParts) * slots * J * sizeof(float), fp4 = rows4_bytes(r.tokens, I) + rows4_bytes(slots, J);
   const size_t sums = static_cast<size_t>(kMostSplits) * r.tokens * I * sizeof(float);
-  return sizeof(LayerList) + logits_words(r) * sizeof(float) + (parts + sums > fp4 ? parts + sums : fp4);
+  return sizeof(Items) + logits_words(r) * sizeof(float) + (parts + sums > fp4 ? parts + sums : fp4);
 }
 
 cudaError_t launch_few_layer(const FewLayer& f, const egs_route& r, int dtype, void* workspace, cudaStream_t st) {
   LayerParams p{};
   p.X = f.X; p.router = f.router; p.up = f.up; p.down = f.down; p.up_scale = f.up_scale; p.down_scale = f.down_scale;
   p.out = f.out; p.weights = f.weights; p.experts = f.experts;
-  p.list = static_cast<LayerList*>(workspace);
+  p.list = static_cast<Items*>(workspace);
   p.logits = reinterpret_cast<float*>(p.list + 1);
   p.h = p.logits + logits_words(r);
   p.x_row = f.x_row;

@@ -299,6 +299,19 @@ def test_two_streams_and_two_graphs_at_once():
             assert all(torch.equal(a, b) for a, b in zip(out, ref))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,k", [(2, 1), (3, 2), (32, 1)])
+@pytest.mark.parametrize("I,J", [(3, 1), (32, 32), (65, 31)])
+def test_many_experts_of_a_small_layer(dtype, tokens, k, I, J):
+    """1024 experts and next to no products: the list of the items needs more room than they do."""
+    t, E = TYPES[dtype], 1024
+    x, router = randn(tokens, I, seed=1, dtype=t), (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    up, down = (randn(E, I, J, seed=3) * 2 / I ** 0.5).to(t), (randn(E, J, I, seed=4) / J ** 0.5).to(t)
+    out, w, ids = ops.routed_experts_few(x, router, up, down, k)
+    want, off = layer64(x.double(), w.double(), ids.long(), up.double(), down.double())
+    assert ((out.double() - want).abs() - off - want.abs() * (torch.finfo(t).eps / 2) - (2.0 ** -25 if dtype == "f16" else 0)).max().item() <= 0
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)
