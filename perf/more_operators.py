@@ -240,11 +240,12 @@ def _run_own(state):
     if case["E"] == 1:
         return (ops.matmul_fp4(q, s, state["up"][0], state["up_scale"][0], out_dtype=X.dtype),)
     plan = ops.plan_experts(state["experts"], case["E"])
+    # rows stay float32 until a token's sum has been formed, which is rounded once
     if case["op"] == "product":
-        Y = ops.expert_matmul_fp4(q, s, state["up"], state["up_scale"], plan, out_dtype=X.dtype)
+        Y = ops.expert_matmul_fp4(q, s, state["up"], state["up_scale"], plan, out_dtype=torch.float32)
     else:
         h, hs = ops.expert_matmul_fp4_rows(q, s, state["up"], state["up_scale"], plan, activation="silu")
-        Y = ops.expert_matmul_fp4(h, hs, state["down"], state["down_scale"], plan, rows="sorted", out_dtype=X.dtype)
+        Y = ops.expert_matmul_fp4(h, hs, state["down"], state["down_scale"], plan, rows="sorted", out_dtype=torch.float32)
     return (ops.combine(Y, state["weights"], plan, out_dtype=X.dtype),)
 
 
