@@ -6,14 +6,15 @@
 //
 //   warps 0, 1    gathered rows of X (tile::gather4), where they are gathered
 //   warp  2       boxes of rows that follow one another and of weights; announces the bytes of a stage
-//   warp  3       tensor-memory allocation; copies a step's scales to tensor memory and issues its MMAs, by the leader of a pair for both CTAs
+//   warp  3       tensor-memory allocation; copies a step's scales to tensor memory and issues its MMAs, by the leader of a pair for both CTAs; the
+//                 second one's tells the leader of scales that are there
 //   warps 4..7    scales: of four steps at a time, from rows to the order in which tensor memory takes them
 //   warps 8..15   read-out: tensor memory -> rows of the output, in float32, 16 bits or (activated) in 4 bits with their scales
 //
 // Scales cannot come by TMA: of a row there are 8 bytes a step, and tensor memory wants four bytes of four rows beside one another.  Both CTAs of a pair
-// need the scales of all columns.  What the second one's warps have stored is made visible to its tensor core by their proxy fence; their
-// arrival at the leader's barrier says no more than that this has happened: a release of everything at cluster scope, which waits behind a memory
-// barrier, made the kernel wait for it (94 us for 74 at 8192 x 4096 -> 4096).  Scales word by word with cp.async: 106; 16 bytes of a row (two steps) at a time for 64: 80 for 70.
+// need the scales of all columns.  What the second one's warps have stored and fenced for the async proxy they hand to a warp of their CTA that has nothing on its way, and that
+// one hands it over to the leader with a release at cluster scope, which the leader's wait acquires: releases by the storing warps themselves wait
+// for the scales that they have asked for behind a memory barrier (94 us for 74 at 8192 x 4096 -> 4096).  Scales word by word with cp.async: 106; 16 bytes of a row (two steps) at a time for 64: 80 for 70.
 //
 // 8192 x 4096 -> 4096: 63.5 us, 4.3 PFLOP/s (2.6 times the 16-bit rate; loads alone 47, all but the scales 61).  Bound by what the L2 gives all SMs, 9.6 TB/s of tiles and scales.
 // 65536 rows of 64 experts, 2048 -> 512: 59, of which 53 without the read-out; 512 -> 2048, two steps a tile: 86, without stores 70, without the read-out 55: 268 MB of
@@ -46,6 +47,7 @@ struct __align__(16) Fp4Header {
   unsigned long long full[kMaxStages];
   unsigned long long empty[kMaxStages];
   unsigned long long scale_full[kScaleRing];
+  unsigned long long scale_stored[kScaleRing];       // of the second CTA of a pair, before the leader knows
   unsigned long long scale_empty[kScaleRing];
   unsigned long long acc_full[2];
   unsigned long long acc_empty[2];
@@ -158,11 +160,11 @@ __device__ __forceinline__ void load_scales(const uint8_t* row, int b, int block
 struct ScaleTiles {
   const int *offsets, *starts;
   int units, first, stride, block, row0;
-  uint32_t scales, full, empty;
+  uint32_t scales, stored, empty;      // stored: the barrier of this CTA's warps
   volatile uint32_t* abort_flag;
 };
-template <int P, bool PAIR>
-__device__ __forceinline__ void scale_warps(const Fp4Params& p, const Fp4Tiles& q, const ScaleTiles& t, bool second) {
+template <int P>
+__device__ __forceinline__ void scale_warps(const Fp4Params& p, const Fp4Tiles& q, const ScaleTiles& t) {
   constexpr int kSets = P == 1 ? 3 : P == 2 ? 2 : 1, kTurn = 128 / P, kColTurns = P == 4 ? 7 : 2 * P;      // (a tile has 224 columns at most)
   struct Words {
     uint32_t a[P][4], b[kColTurns][4];
@@ -225,10 +227,7 @@ __device__ __forceinline__ void scale_warps(const Fp4Params& p, const Fp4Tiles& 
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        if (PAIR && second) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_cta(t.full + chunk.slot * 8u, 0)) : "memory");
-        else mbar_arrive(t.full + chunk.slot * 8u);
-      }
+      if (lane == 0) mbar_arrive(t.stored + chunk.slot * 8u);
       chunk.next(kScaleRing);
     }
     ask(w);
@@ -278,7 +277,8 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
       mbar_init(smem_u32(&hdr->empty[s]), 1);
     }
     for (int b = 0; b < kScaleRing; ++b) {
-      mbar_init(smem_u32(&hdr->scale_full[b]), PAIR ? 2 * kScaleWarps : kScaleWarps);  // (a pair's: the leader's copy is used)
+      mbar_init(smem_u32(&hdr->scale_full[b]), PAIR ? kScaleWarps + 1 : kScaleWarps);  // (a pair's: the leader's copy is used)
+      mbar_init(smem_u32(&hdr->scale_stored[b]), kScaleWarps);
       mbar_init(smem_u32(&hdr->scale_empty[b]), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -425,10 +425,10 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
           const uint32_t scale_full = smem_u32(&hdr->scale_full[chunk.slot]), scale_empty = smem_u32(&hdr->scale_empty[chunk.slot]);
           const uint32_t scales = (scales0 + static_cast<uint32_t>(chunk.slot) * kChunkBytes) >> 4;
           uint64_t from_a = s_desc + scales, from_b = s_desc + scales + (kChunkA >> 4);
-          alive = mbar_wait_all(scale_full, chunk.round & 1, abort_flag, p.status.word);
+          alive = mbar_wait_all<PAIR>(scale_full, chunk.round & 1, abort_flag, p.status.word);
           const int end = min(q.steps, ks + kChunkSteps);
           for (; ks < end && alive; ++ks) {
-            alive = mbar_wait_all(full, at.round & 1, abort_flag, p.status.word);
+            alive = mbar_wait_all<PAIR>(full, at.round & 1, abort_flag, p.status.word);
             if (!alive) break;
             tc_fence_after();
             if (elect_one()) {
@@ -452,15 +452,24 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
           chunk.next(kScaleRing);
         }
       }
+    } else {
+      // scales that this CTA's warps have stored: what the wait has acquired of them the arrival releases to the leader
+      RingCursor chunk;
+      for (int round = 0; unit_of(round) < units && alive; ++round)
+        for (int ks = 0; ks < q.steps && alive; ks += kChunkSteps) {
+          alive = mbar_wait_all(smem_u32(&hdr->scale_stored[chunk.slot]), chunk.round & 1, abort_flag, p.status.word);
+          if (alive && elect_one()) mbar_arrive_cluster(map_to_cta(smem_u32(&hdr->scale_full[chunk.slot]), 0));
+          chunk.next(kScaleRing);
+        }
     }
     pdl_trigger();
     __syncwarp();
   } else if (warp < kReadWarp0) {
     // =========================== scales ===========================
-    const ScaleTiles tiles{offsets, starts, units, first_unit, unit_stride, kBlock, rank * 128, scales0, smem_u32(&hdr->scale_full[0]), smem_u32(&hdr->scale_empty[0]), abort_flag};
-    if (q.steps > 4) scale_warps<4, PAIR>(p, q, tiles, !leader);
-    else if (q.steps > 2) scale_warps<2, PAIR>(p, q, tiles, !leader);
-    else scale_warps<1, PAIR>(p, q, tiles, !leader);
+    const ScaleTiles tiles{offsets, starts, units, first_unit, unit_stride, kBlock, rank * 128, scales0, smem_u32(leader ? &hdr->scale_full[0] : &hdr->scale_stored[0]), smem_u32(&hdr->scale_empty[0]), abort_flag};
+    if (q.steps > 4) scale_warps<4>(p, q, tiles);
+    else if (q.steps > 2) scale_warps<2>(p, q, tiles);
+    else scale_warps<1>(p, q, tiles);
     __syncwarp();
   } else {
     // =========================== read-out ===========================

@@ -47,3 +47,23 @@ def test_ctas_that_count_for_themselves_are_resident_together():
     text = open(os.path.join(CSRC, "egs_generic.cu")).read()
     assert re.search(r"__launch_bounds__\(kPrepThreads, 4\)\s+scatter_prepare_kernel", text)
     assert "size_t grid = 4 * 148;" in text
+
+
+def test_arrivals_at_another_ctas_barrier_name_their_scope():
+    """An arrival without one orders memory for its own CTA alone; what it announces to another CTA may not be there yet."""
+    found = 0
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu*"))):
+        for at in re.findall(r"mbarrier\.arrive[\w.:]*", re.sub(r"//[^\n]*", "", open(path).read())):
+            if "shared::cluster" in at:
+                found += 1
+                assert ".release.cluster." in at or ".relaxed.cluster." in at, f"{os.path.basename(path)}: {at}"
+    assert found >= 2
+
+
+def test_scales_of_a_pair_are_waited_for_at_the_scope_they_are_released_at():
+    """The leader's tensor core reads both CTAs' scales and tiles: its waits for them acquire what the other CTA has released."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, "egs_fp4_tensor.cu")).read())
+    issuer = text[text.index("warp == kIssueWarp", text.index("warp == kBoxWarp")):text.index("warp < kReadWarp0")]
+    for barrier in ("scale_full", "full", "smem_u32(&hdr->acc_empty[buf])"):
+        assert f"mbar_wait_all<PAIR>({barrier}," in issuer
+    assert re.search(r"mbar_wait_all\(smem_u32\(&hdr->scale_stored\[.*\n.*mbar_arrive_cluster\(map_to_cta\(smem_u32\(&hdr->scale_full", issuer)
