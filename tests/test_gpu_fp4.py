@@ -213,3 +213,25 @@ def test_smallest_numbers_and_no_numbers(dtype):
         back = ops.dequantize_rows_fp4(q, scale, C, dtype=torch.float32)
         want = fp4.values(*fp4.quantize(X), C).to(torch.float32)             # (6 * 2^126, what float32's largest number becomes, is beyond it)
         assert bool(same(back, want))
+
+
+# ---- sums over a token's experts ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,E,k,C,N", [(40, 8, 2, 256, 96), (300, 16, 4, 520, 330)])
+def test_projection_of_experts_is_rounded_once(dtype, tokens, E, k, C, N):
+    """A token's sum over its experts as a workload forms it: off by half a step of its type, and by float32 sums."""
+    from perf import more_operators as workloads
+    case = workloads._product("", tokens, E, k, C, N, dtype)
+    state = workloads.prepare(case, 5)
+    out, = workloads._run_own(state)
+    up, w, ids = fp4.rows(state["up"], state["up_scale"])[..., :C], state["weights"].double(), state["experts"].long()
+    xq = fp4.values(*fp4.quantize(state["X"]), C)
+    want, size = (torch.zeros(tokens, N, dtype=torch.float64, device="cuda") for _ in range(2))
+    for e in range(E):
+        t, j = (ids == e).nonzero(as_tuple=True)
+        want.index_put_((t,), w[t, j].unsqueeze(-1) * (xq[t] @ up[e].t()), accumulate=True)
+        size.index_put_((t,), w[t, j].unsqueeze(-1) * (xq[t].abs() @ up[e].abs().t()), accumulate=True)
+    # a product's float32 sums (product_bound), then k products with weights and their sums, 2^-24 of what has been summed each
+    off = product_bound(size, want, C, TYPES[dtype]) + size * (2 * k * 2.0 ** -24) + (2.0 ** -25 if dtype == "f16" else 0)
+    assert ((out.double() - want).abs() - off).max().item() <= 0
