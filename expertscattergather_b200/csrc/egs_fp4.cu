@@ -294,11 +294,14 @@ __device__ __forceinline__ void few_fp4(const Fp4Params& p, int expert, int firs
         for (int m = 0; m < M; ++m) sum[m][j] = __dp4a(static_cast<int>(xh[m]), static_cast<int>(wh), __dp4a(static_cast<int>(xl[m]), static_cast<int>(wl), sum[m][j]));
       }
     }
+    float low[M], high[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) fp4_factors(fp4_power(sx[m]), low[m], high[m]);
 #pragma unroll
     for (int j = 0; j < kFewChannels; ++j) {
       const float f = fp4_power(sw[j]);
 #pragma unroll
-      for (int m = 0; m < M; ++m) acc[m][j] = fmaf(static_cast<float>(sum[m][j]) * (0.25f * fp4_power(sx[m])), f, acc[m][j]);
+      for (int m = 0; m < M; ++m) acc[m][j] = fmaf(static_cast<float>(sum[m][j]) * (0.25f * low[m]) * f, high[m], acc[m][j]);
     }
   }
 #pragma unroll

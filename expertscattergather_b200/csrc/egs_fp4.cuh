@@ -23,6 +23,12 @@ __device__ __forceinline__ float fp4_inverse(uint32_t byte) { return byte == 255
 __device__ __forceinline__ float fp4_power(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
 }
+// A scale as two factors, `low` at most 1 and `high` at least 1 (both NaN of one that is not a number).  A block's sum times `low`, times the other operand's scale,
+// times `high` leaves float32's range no earlier than the product itself: sums are multiples of 1/4 up to 1152, so that all but the last factor give
+// exact numbers from 2^-129 on, or the last one is 1.  (Times one scale and then the other, rows from 2^118 on gave infinities whatever the weights.)
+__device__ __forceinline__ void fp4_factors(float power, float& low, float& high) {
+  asm("min.NaN.f32 %0, %2, 0f3F800000;\n\tmax.NaN.f32 %1, %2, 0f3F800000;" : "=f"(low), "=f"(high) : "f"(power));
+}
 
 // Eight values to the nearest of 4 bits (ties to an even mantissa, beyond 6: 6).
 __device__ __forceinline__ uint32_t fp4_pack8(const float (&v)[8]) {

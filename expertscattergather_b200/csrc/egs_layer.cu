@@ -840,6 +840,13 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
+// acc += d * low * power * high of two rows, in this order (see fp4_factors).
+__device__ __forceinline__ void add_scaled(float2& acc, float2 d, float2 low, float power, float2 high) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 b, {%6, %6};\n\tmul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 b, {%7, %8};\n\tmov.b64 c, {%0, %1};\n\tfma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(acc.x), "+f"(acc.y) : "f"(d.x), "f"(d.y), "f"(low.x), "f"(low.y), "f"(power), "f"(high.x), "f"(high.y));
+}
+
 template <int LAYOUT>
 struct Stages {
   const Matrix4& t;
@@ -947,8 +954,8 @@ struct Stages {
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (++ask_slot == kDepth4) ask_slot = 0;
   }
-  // acc[i]: columns 4 g + i of `count` rows, 2 q and 2 q + 1 (of q < 2); f0, f1: what those rows' scales are times
-  __device__ __forceinline__ void add(float2 (&acc)[4], int count, float f0, float f1) {
+  // acc[i]: columns 4 g + i of `count` rows, 2 q and 2 q + 1 (of q < 2)
+  __device__ __forceinline__ void add(float2 (&acc)[4], int count) {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t from = base + get_slot * kStageBytes4, powers = base + kDepth4 * kStageBytes4;
     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth4 - 1) : "memory");
@@ -966,8 +973,7 @@ struct Stages {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint4 v = words_at(from + kStageF4 + ((q & 1) * 2 + i) * 16);
-      const float times = i ? f1 : f0;
-      scale[i][0] = __uint_as_float(v.x) * times; scale[i][1] = __uint_as_float(v.y) * times; scale[i][2] = __uint_as_float(v.z) * times; scale[i][3] = __uint_as_float(v.w) * times;
+      scale[i][0] = __uint_as_float(v.x); scale[i][1] = __uint_as_float(v.y); scale[i][2] = __uint_as_float(v.z); scale[i][3] = __uint_as_float(v.w);
     }
 #pragma unroll
     for (int kk = 0; kk < kStage4; ++kk) {
@@ -987,6 +993,10 @@ struct Stages {
       }
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
       if (g < count) x = words_at(from + kStageRows4 + g * kRowPitch4 + kk * 64 + q * 16);
+      float low0, low1, high0, high1;
+      fp4_factors(scale[0][kk], low0, high0);
+      fp4_factors(scale[1][kk], low1, high1);
+      const float2 low = make_float2(low0, low1), high = make_float2(high0, high1);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         uint32_t a[4], b[4];
@@ -995,10 +1005,8 @@ struct Stages {
         float d[4];
         mma16(d, a[0], b[0], a[1], b[1], x.x, x.y, 0.f, 0.f, 0.f, 0.f);
         mma16(d, a[2], b[2], a[3], b[3], x.z, x.w, d[0], d[1], d[2], d[3]);
-        acc[i].x = fmaf(d[0] * scale[0][kk], power[i][kk], acc[i].x);
-        acc[i].y = fmaf(d[1] * scale[1][kk], power[i][kk], acc[i].y);
-        acc[i + 1].x = fmaf(d[2] * scale[0][kk], power[i + 1][kk], acc[i + 1].x);
-        acc[i + 1].y = fmaf(d[3] * scale[1][kk], power[i + 1][kk], acc[i + 1].y);
+        add_scaled(acc[i], make_float2(d[0], d[1]), low, power[i][kk], high);
+        add_scaled(acc[i + 1], make_float2(d[2], d[3]), low, power[i + 1][kk], high);
       }
     }
     __syncwarp();                              // the slot may be asked for anew, the powers written
@@ -1105,7 +1113,7 @@ __global__ void __launch_bounds__(kThreads4, 2) few_up4_kernel(const __grid_cons
     float2 acc[4] = {};
     for (int i = warp; i < stages; i += kWarps4) {
       next();
-      ring.add(acc, item.rows, 1.f, 1.f);
+      ring.add(acc, item.rows);
     }
     const int g = lane >> 2, q = lane & 3;
     if (q < 2) {
@@ -1166,16 +1174,17 @@ __global__ void __launch_bounds__(kThreads4, 2) few_down4_kernel(const __grid_co
     const int slot0 = item.slot[(q & 1) * 2], slot1 = item.slot[(q & 1) * 2 + 1];
     float2 acc[4] = {};
     next();
-    ring.add(acc, item.rows, items.weights[slot0], items.weights[slot1]);
+    ring.add(acc, item.rows);
+    const float w0 = items.weights[slot0], w1 = items.weights[slot1];
     float4* to = reinterpret_cast<float4*>(part + (warp * p.tokens + p.by_k.quotient(slot0)) * kTile4 + 4 * g);
     if (q * 2 < item.rows) {
       const float4 o = *to;
-      *to = make_float4(o.x + acc[0].x, o.y + acc[1].x, o.z + acc[2].x, o.w + acc[3].x);
+      *to = make_float4(fmaf(w0, acc[0].x, o.x), fmaf(w0, acc[1].x, o.y), fmaf(w0, acc[2].x, o.z), fmaf(w0, acc[3].x, o.w));
     }
     to = reinterpret_cast<float4*>(part + (warp * p.tokens + p.by_k.quotient(slot1)) * kTile4 + 4 * g);
     if (q * 2 + 1 < item.rows) {
       const float4 o = *to;
-      *to = make_float4(o.x + acc[0].y, o.y + acc[1].y, o.z + acc[2].y, o.w + acc[3].y);
+      *to = make_float4(fmaf(w1, acc[0].y, o.x), fmaf(w1, acc[1].y, o.y), fmaf(w1, acc[2].y, o.z), fmaf(w1, acc[3].y, o.w));
     }
   }
   __syncthreads();

@@ -411,3 +411,32 @@ def test_served_in_4_bits_on_another_stream():
         got = [served(x) for x in xs]
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens,E,k,I,J", [(1, 8, 2, 256, 96), (7, 5, 3, 330, 201), (32, 4, 2, 96, 1032)])
+@pytest.mark.parametrize("x_far,up_far,down_far", [(120, -118, 0), (-118, 120, 0), (0, 118, -118), (0, 60, 40), (100, -40, -60), (-110, 118, 90)])
+def test_layer_on_4_bits_of_far_scales(dtype, tokens, E, k, I, J, x_far, up_far, down_far):
+    """Rows, weights and activations of magnitudes at the ends of float32 whose products are ordinary numbers."""
+    t = TYPES[dtype]
+    (u, us), (d, ds) = grid4(E, J, I, seed=3, low=124 + up_far, high=128 + up_far), grid4(E, I, J, seed=4, low=125 + down_far, high=129 + down_far)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.ldexp(torch.randint(-6, 7, (tokens, I), device="cuda", generator=gen).float() * 0.5, torch.tensor(x_far, device="cuda")).to(t)
+    router = torch.ldexp(randn(E, I, seed=2) * 1.5 / I ** 0.5, torch.tensor(-x_far, device="cuda")).to(t)
+    xq = fp4.values(*fp4.quantize(x), I)
+    up, down = fp4.rows(u, us)[..., :I].transpose(1, 2), fp4.rows(d, ds)[..., :J].transpose(1, 2)
+    for uu, dd in ((u, d), tuple(q.transpose(1, 2).contiguous().transpose(1, 2) for q in (u, d))):
+        out, w, ids = ops.routed_experts_few(x, router, uu, dd, k, up_scale=us, down_scale=ds)
+        want = torch.zeros(tokens, I, dtype=torch.float64, device="cuda")
+        size = torch.zeros_like(want)
+        for e in range(E):
+            tt, j = (ids.long() == e).nonzero(as_tuple=True)
+            if tt.numel():
+                h = (xq[tt] @ up[e]).float()                 # exact: see grid4
+                a = fp4.values(*fp4.quantize(h / (1 + torch.exp(-h))), J)
+                we = w[tt, j].double().unsqueeze(-1)
+                want.index_put_((tt,), we * (a @ down[e]), accumulate=True)
+                size.index_put_((tt,), we * (a.abs() @ down[e].abs()), accumulate=True)
+        assert want.isfinite().all() and want.abs().max() < 2.0 ** 126
+        off = size * ((J / 32 + k + 24) * 2.0 ** -24) + want.abs() * (torch.finfo(t).eps / 2)      # (as test_layer_on_4_bits)
+        assert ((out.double() - want).abs() - off).max().item() <= 0

@@ -235,3 +235,25 @@ def test_projection_of_experts_is_rounded_once(dtype, tokens, E, k, C, N):
     # a product's float32 sums (product_bound), then k products with weights and their sums, 2^-24 of what has been summed each
     off = product_bound(size, want, C, TYPES[dtype]) + size * (2 * k * 2.0 ** -24) + (2.0 ** -25 if dtype == "f16" else 0)
     assert ((out.double() - want).abs() - off).max().item() <= 0
+
+
+# ---- far scales ---------------------------------------------------------------------------------------
+
+FAR = [(123, -20), (-20, 123), (124, -130), (-130, 124), (110, 8), (8, 110), (-100, 20), (20, -100), (100, -100), (-149, 110)]
+
+
+@pytest.mark.parametrize("path", ["auto", "tensor", "generic"])
+@pytest.mark.parametrize("up,down", FAR)
+@pytest.mark.parametrize("rows,C,N", [(1, 4096, 64), (1, 70, 33), (130, 512, 96)])
+def test_products_of_far_scales(path, up, down, rows, C, N):
+    """Rows and weights of magnitudes at the ends of float32 whose products are ordinary numbers."""
+    X, W = torch.ldexp(randn(rows, C, seed=1), torch.tensor(up, device="cuda")), torch.ldexp(randn(N, C, seed=2), torch.tensor(down, device="cuda"))
+    (q, s), (wq, ws) = ops.quantize_rows_fp4(X), ops.quantize_rows_fp4(W)
+    x, w = fp4.rows(q, s), fp4.rows(wq, ws)
+    Y, size = x @ w.t(), x.abs() @ w.abs().t()
+    plan = ops.plan_experts(torch.zeros(rows, 1, dtype=torch.int32, device="cuda"), 1)
+    for out in (torch.float32, torch.bfloat16):
+        for got in (ops.matmul_fp4(q, s, wq, ws, out_dtype=out, path=path), ops.expert_matmul_fp4(q, s, wq[None], ws[None], plan, out_dtype=out, path=path)):
+            # relative to the magnitudes, which product_bound's smallest term would hide: 2^-149 is float32's
+            off = product_bound(size, Y, C, out) - 1e-30 + 2.0 ** -148
+            assert ((got.double() - Y).abs() - off).max().item() <= 0
