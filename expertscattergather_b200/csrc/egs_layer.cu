@@ -1257,6 +1257,9 @@ cudaError_t down_launch(LayerParams p, int tile, cudaStream_t st) {
   size_t act = static_cast<size_t>(slots) * (p.J / (size * p.splits) + 36) * sizeof(float);
   act = (act + 15) & ~static_cast<size_t>(15);
   if (act > kDownSmem - part - ring) act = kDownSmem - part - ring;
+  // What other CTAs write of their sums lies behind what this one lists its items with: they may be through before it has begun to.
+  const size_t sums = ring + act + static_cast<size_t>(slots < 4 * kDownWarps ? 4 * kDownWarps : slots) * tile * sizeof(float);
+  if (size > 1 && sums < sizeof(Scratch)) act += (sizeof(Scratch) - sums + 15) & ~static_cast<size_t>(15);
   p.act_floats = static_cast<int>(act / sizeof(float));
   count_launch(p.splits > 1 ? 2 : 1);
   const size_t smem = ring + act + part;       // (what the items are listed with lies at its begin first)

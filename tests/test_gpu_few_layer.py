@@ -312,6 +312,21 @@ def test_many_experts_of_a_small_layer(dtype, tokens, k, I, J):
     assert ((out.double() - want).abs() - off - want.abs() * (torch.finfo(t).eps / 2) - (2.0 ** -25 if dtype == "f16" else 0)).max().item() <= 0
 
 
+@pytest.mark.parametrize("E", [905, 1024])
+@pytest.mark.parametrize("dtype,tokens,k,I,J", [("f32", 2, 1, 33, 70), ("f32", 3, 1, 65, 130), ("bf16", 2, 2, 31, 259), ("f16", 1, 3, 97, 65)])
+def test_clusters_of_a_layer_with_many_experts(E, dtype, tokens, k, I, J):
+    """Several CTAs to a tile and a list of items that is longer than all they add up: the sums that they hand to each other lie behind it."""
+    t = TYPES[dtype]
+    x, router = randn(tokens, I, seed=1, dtype=t), (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    up, down = (randn(E, I, J, seed=3) * 2 / I ** 0.5).to(t), (randn(E, J, I, seed=4) / J ** 0.5).to(t)
+    out, w, ids = ops.routed_experts_few(x, router, up, down, k)
+    want, off = layer64(x.double(), w.double(), ids.long(), up.double(), down.double())
+    off = off + want.abs() * (torch.finfo(t).eps / 2) + (2.0 ** -25 if dtype == "f16" else 0)
+    for _ in range(8):
+        assert ((out.double() - want).abs() - off).max().item() <= 0
+        out = ops.routed_experts_few(x, router, up, down, k)[0]
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)
