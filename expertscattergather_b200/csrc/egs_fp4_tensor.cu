@@ -523,7 +523,7 @@ fp4_rows_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ Fp4
           uint32_t top = 0u;
           if (p.act == EGS_ACT_SILU) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(silu_fast(__uint_as_float(v[i])));
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(silu_near(__uint_as_float(v[i])));
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) top = max(top, v[i] & 0x7fffffffu);

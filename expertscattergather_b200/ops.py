@@ -541,7 +541,8 @@ def expert_matmul_fp4(q, scale, Wq, w_scale, plan: ExpertPlan, *, rows="tokens",
 
 def expert_matmul_fp4_rows(q, scale, Wq, w_scale, plan: ExpertPlan, *, rows="tokens", activation=None, path=None):
     """:func:`expert_matmul_fp4` whose sorted rows (with ``activation='silu'`` their activations, formed in float32) leave in 4 bits again, as
-    ``(q, scale)`` for the next product: what lies between two products of a layer is neither stored in full nor read again."""
+    ``(q, scale)`` for the next product: what lies between two products of a layer is neither stored in full nor read again.  The tensor cores' rows are activated
+    within 2^-20 of what :func:`quantize_rows_fp4` forms, so that a value so near to the border between two of 4 bits may go to the other one."""
     return _host().matmul_fp4_rows(q, scale, Wq, w_scale, plan.offsets, plan.slots, plan.tokens, plan.k, rows, activation, _path(path))
 
 

@@ -417,7 +417,7 @@ int egs_expert_matmul_fp4(const uint8_t* q, const uint8_t* q_scale, int64_t q_st
                           int64_t w_stride, int64_t ws_stride, const int32_t* offsets, const int32_t* slots, void* Y, const egs_ragged* dims, int rows,
                           int out_dtype, int path, int32_t* status_word, void* cuda_stream);
 /* ... whose rows, or their activations, leave in 4 bits: y [tokens * k, ceil(N / 2)] and y_scale [tokens * k, ceil(N / 32)], as egs_quantize_rows_fp4
- * writes them; rows behind offsets[E] are zeros with the scale 0.  workspace (16-byte aligned):
+ * writes them, activations of the tensor cores' rows within 2^-20 of its own; rows behind offsets[E] are zeros with the scale 0.  workspace (16-byte aligned):
  * egs_expert_matmul_fp4_rows_workspace_bytes() bytes (float32 rows, where few of them are not for the tensor cores). */
 int egs_expert_matmul_fp4_rows(const uint8_t* q, const uint8_t* q_scale, int64_t q_stride, int64_t qs_stride, const uint8_t* Wq, const uint8_t* w_scale,
                                int64_t w_stride, int64_t ws_stride, const int32_t* offsets, const int32_t* slots, uint8_t* y, uint8_t* y_scale,

@@ -257,3 +257,31 @@ def test_products_of_far_scales(path, up, down, rows, C, N):
             # relative to the magnitudes, which product_bound's smallest term would hide: 2^-149 is float32's
             off = product_bound(size, Y, C, out) - 1e-30 + 2.0 ** -148
             assert ((got.double() - Y).abs() - off).max().item() <= 0
+
+
+# ---- activations ahead of 4 bits ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("path", ["auto", "tensor", "generic"])
+@pytest.mark.parametrize("tokens,E,k,C,N", [(1, 8, 2, 96, 70), (300, 6, 2, 128, 256), (2000, 4, 1, 64, 224)])
+@pytest.mark.parametrize("low,high", [(-110, -86), (-90, -60), (-70, -10), (-12, 0), (-1, 1), (0, 100)])
+def test_activations_ahead_of_4_bits_are_the_exact_ones(path, tokens, E, k, C, N, low, high):
+    """Rows that leave activated are those of the same product in float32, activated and brought into 4 bits by themselves, whatever kernel has them: whole
+    blocks of sums between `low` and `high`.  The tensor cores' read-out forms activations within 2^-20 of the elementary form (relative; infinite
+    exponentials give 0 in both), so there a value may go the other way where a border between two lies as near."""
+    plan = ops.plan_experts(choose(tokens, E, k, seed=7), E)
+    q, s = ops.quantize_rows_fp4(1 + 0.2 * randn(tokens, C, seed=1))
+    wq, ws = ops.quantize_rows_fp4((low + (high - low) * torch.rand(E, N, 1, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))) * (1 + 0.1 * randn(E, N, C, seed=3)) / C)
+    full = ops.expert_matmul_fp4(q, s, wq, ws, plan, out_dtype=torch.float32, path=path)
+    y, ys = ops.expert_matmul_fp4_rows(q, s, wq, ws, plan, activation="silu", path=path)
+    elementary = full / (1 + torch.exp(-full))
+    if path == "generic" or tokens == 1 and path == "auto":
+        check_rows(elementary, y, ys)
+    v = elementary.double()
+    (_, least), (_, most) = (fp4.quantize(v * f) for f in (1 - 2.0 ** -20, 1 + 2.0 ** -20))
+    assert ((ys >= least) & (ys <= most)).all()
+    power = torch.exp2(ys.double() - 127).repeat_interleave(32, -1)[..., :N]
+    edges = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5], dtype=torch.float64, device="cuda")
+    level = torch.tensor(fp4.LEVELS, dtype=torch.float64, device="cuda")
+    size, got = v.abs() / power, fp4.values(fp4.codes_of(y), ys, N) / power
+    low_level, high_level = (level[torch.bucketize(size * f, edges)] for f in (1 - 2.0 ** -20, 1 + 2.0 ** -20))
+    assert ((got.abs() >= low_level) & (got.abs() <= high_level) & ((got == 0) | (torch.sign(got) == torch.sign(v)))).all()
