@@ -240,7 +240,8 @@ class RoutedExpertsFp4(nn.Module):
     @torch.no_grad()
     def forward(self, x):
         tokens, k = x.numel() // max(self.I, 1), self.router.top_k
-        if tokens <= ops.FEW_TOKENS and tokens * k <= ops.FEW_SLOTS:
+        # (under autocast rows may come in another type than the router's, which its product takes and the layer in one call does not)
+        if tokens <= ops.FEW_TOKENS and tokens * k <= ops.FEW_SLOTS and x.dtype == self.router.W.dtype:
             return ops.routed_experts_few(x, self.router.W, self.up, self.down, k, self.router.balance, up_scale=self.up_scale, down_scale=self.down_scale,
                                           **self.router.options)[0]
         weights, experts = self.router(x)

@@ -110,3 +110,26 @@ def test_served_layer_in_4_bits(monkeypatch):
     with pytest.raises(StopIteration):
         served(torch.zeros(ops.FEW_TOKENS + 1, 24, dtype=torch.bfloat16))
     assert len(calls) == 2
+
+
+def served_calls(monkeypatch, E, I, J, k, dtype=torch.float32):
+    """A served layer in 4 bits without weights to speak of, and the list of the calls that it makes: 'few' or 'separate'."""
+    monkeypatch.setattr(ops, "quantize_rows_fp4", lambda x, **_: (torch.zeros(*x.shape[:-1], 16 * ((x.shape[-1] + 31) // 32), dtype=torch.uint8)[..., :(x.shape[-1] + 1) // 2],
+                                                                torch.zeros(*x.shape[:-1], (x.shape[-1] + 511) // 512 * 16, dtype=torch.uint8)[..., :(x.shape[-1] + 31) // 32]))
+    served = egs.RoutedExperts(E, I, J, k).to(dtype).quantized(bits=4)
+    calls = []
+    monkeypatch.setattr(ops, "routed_experts_few", lambda x, *a, **o: calls.append("few") or (x, None, None))
+    monkeypatch.setattr(egs.TokenRouter, "forward", lambda self, x: calls.append("separate") or (None, None))
+    monkeypatch.setattr(ops, "plan_experts", lambda *a: None)
+    monkeypatch.setattr(ops, "expert_matmul_fp4_rows", lambda *a, **o: (None, None))
+    monkeypatch.setattr(ops, "expert_matmul_fp4", lambda *a, **o: None)
+    monkeypatch.setattr(ops, "combine", lambda y, w, plan, out_dtype: torch.zeros(0))
+    return lambda x: (calls.clear(), served(x), calls[:])[2]
+
+
+def test_rows_of_another_type_go_through_the_router(monkeypatch):
+    """As autocast hands them over: few tokens are taken as many are."""
+    run = served_calls(monkeypatch, 4, 24, 70, 2)
+    assert run(torch.zeros(3, 24)) == ["few"]
+    monkeypatch.setattr(torch.Tensor, "view", lambda self, *a: self)
+    assert run(torch.zeros(3, 24, dtype=torch.bfloat16)) == ["separate"] and run(torch.zeros(40, 24, dtype=torch.bfloat16)) == ["separate"]

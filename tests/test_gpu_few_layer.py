@@ -455,3 +455,16 @@ def test_layer_on_4_bits_of_far_scales(dtype, tokens, E, k, I, J, x_far, up_far,
         assert want.isfinite().all() and want.abs().max() < 2.0 ** 126
         off = size * ((J / 32 + k + 24) * 2.0 ** -24) + want.abs() * (torch.finfo(t).eps / 2)      # (as test_layer_on_4_bits)
         assert ((out.double() - want).abs() - off).max().item() <= 0
+
+
+def test_served_in_4_bits_under_autocast():
+    """A float32 layer whose rows come in 16 bits: few tokens give what they give among many."""
+    import expertscattergather_b200 as egs
+    torch.manual_seed(6)
+    served = egs.RoutedExperts(8, 128, 96, 2).cuda().quantized(bits=4)
+    x = randn(40, 128, seed=2, dtype=torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        many, few = served(x), served(x[:5])
+    assert few.dtype == many.dtype == torch.bfloat16
+    # the router's product may be summed in another order: logits are off by a step of bf16 at most, 2^-8 of themselves (which are below 2), weights by as much
+    assert (few.float() - many[:5].float()).norm() <= 2e-2 * many[:5].float().norm()
