@@ -219,8 +219,10 @@ class RoutedExpertsInt8(nn.Module):
 
 class RoutedExpertsFp4(nn.Module):
     """A :class:`RoutedExperts` for serving: weights in 4 bits (``ops.quantize_rows_fp4`` along their contractions), rows rounded to 4 bits on the way
-    into each product.  A call of a few tokens (``ops.FEW_TOKENS``, ``ops.FEW_SLOTS``) is one of ``ops.routed_experts_few``, whose logits stay float32;
-    in others the router is the module's own.  It has a router of its own, as :class:`RoutedExpertsInt8` has."""
+    into each product.  A call of a few tokens (``ops.FEW_TOKENS``, ``ops.FEW_SLOTS``) that need not read weights over and over is one of
+    ``ops.routed_experts_few``, whose logits stay float32; in others the router is the module's own.  Rows that are summed over a token's experts are float32 up to
+    ``ops.FEW_TOKENS`` tokens, and beyond, as :class:`RoutedExperts` has them, of x's type unless the layer had ``float32_rows``.  It has a router of its own, as
+    :class:`RoutedExpertsInt8` has."""
 
     def __init__(self, layer: RoutedExperts):
         super().__init__()
@@ -237,15 +239,26 @@ class RoutedExpertsFp4(nn.Module):
             setattr(self, name, _in_pitch(getattr(self, name)))           # (a copy to another device has its rows together)
         return self
 
+    def _in_one_call(self, x) -> bool:
+        """Whether ``ops.routed_experts_few`` takes x, and sooner than the separate operators.  It shares a read of an expert's weights among four tokens: with no more
+        nothing is read twice.  With more its time goes with the slots and a matrix's size, that of the operators, 30 to 45 us of launches aside, with the experts that are used.
+        us in a graph, one call and five: 32 tokens, 4 of 8 experts, 2048 x 512 33 and 32, 2048 x 2048 85 and 39, 4096 x 4096 273 and 75; 16 tokens, 8 of 64, 2048 x 512 52 and 55,
+        2048 x 2048 140 and 90; 8 tokens, 2 of 8, 4096 x 4096 73 and 77, 8 of 8, 124 and 76; 4 tokens, 8 of 8, 77 and 81.  (Of 150 sizes the choice costs 0.4 % over the better one in the
+        mean, the host's 14 and 46 us counted for half of them.)"""
+        tokens = x.numel() // max(self.I, 1)
+        slots = tokens * self.router.top_k
+        if tokens > ops.FEW_TOKENS or slots > ops.FEW_SLOTS or x.dtype != self.router.W.dtype:       # (autocast hands over rows of another type, which the router's product takes)
+            return False
+        return tokens <= 4 or slots * self.I * self.up.shape[1] <= 200_000_000
+
     @torch.no_grad()
     def forward(self, x):
-        tokens, k = x.numel() // max(self.I, 1), self.router.top_k
-        # (under autocast rows may come in another type than the router's, which its product takes and the layer in one call does not)
-        if tokens <= ops.FEW_TOKENS and tokens * k <= ops.FEW_SLOTS and x.dtype == self.router.W.dtype:
-            return ops.routed_experts_few(x, self.router.W, self.up, self.down, k, self.router.balance, up_scale=self.up_scale, down_scale=self.down_scale,
+        if self._in_one_call(x):
+            return ops.routed_experts_few(x, self.router.W, self.up, self.down, self.router.top_k, self.router.balance, up_scale=self.up_scale, down_scale=self.down_scale,
                                           **self.router.options)[0]
         weights, experts = self.router(x)
         plan = ops.plan_experts(experts, self.E)
         h = ops.expert_matmul_fp4_rows(*ops.quantize_rows_fp4(x), self.up, self.up_scale, plan, activation="silu")
-        y = ops.expert_matmul_fp4(*h, self.down, self.down_scale, plan, rows="sorted", out_dtype=torch.float32 if self.float32_rows else x.dtype)
+        wide = self.float32_rows or x.numel() <= ops.FEW_TOKENS * self.I
+        y = ops.expert_matmul_fp4(*h, self.down, self.down_scale, plan, rows="sorted", out_dtype=torch.float32 if wide else x.dtype)
         return ops.combine(y, weights, plan, out_dtype=x.dtype).view(x.shape)

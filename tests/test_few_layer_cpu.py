@@ -133,3 +133,14 @@ def test_rows_of_another_type_go_through_the_router(monkeypatch):
     assert run(torch.zeros(3, 24)) == ["few"]
     monkeypatch.setattr(torch.Tensor, "view", lambda self, *a: self)
     assert run(torch.zeros(3, 24, dtype=torch.bfloat16)) == ["separate"] and run(torch.zeros(40, 24, dtype=torch.bfloat16)) == ["separate"]
+
+
+@pytest.mark.parametrize("E,I,J,k,one,many", [(8, 24, 70, 2, (0, 1, 4, 5, 32), (33, 700)), (8, 24, 70, 8, (1, 32), (33,)), (64, 24, 70, 9, (1, 28), (29, 32)), (8, 512, 1000, 4, (1, 4, 32), (33,)),
+                                              (8, 2048, 1024, 8, (1, 2, 4, 8, 11), (12, 16, 32)), (2, 4096, 4096, 2, (1, 3, 4), (6, 32)), (1, 4096, 4096, 1, (4, 11), (12, 32))])
+def test_which_calls_the_served_layer_makes(monkeypatch, E, I, J, k, one, many):
+    """Few tokens in one call; those whose experts' weights would be read over and over by the operators for many."""
+    run = served_calls(monkeypatch, E, I, J, k)
+    monkeypatch.setattr(torch.Tensor, "view", lambda self, *a: self)
+    assert [run(torch.zeros(n, I)) for n in one] == [["few"]] * len(one)
+    assert [run(torch.zeros(n, I)) for n in many] == [["separate"]] * len(many)
+    assert run(torch.zeros(many[0], 1, I)) == ["separate"] and run(torch.zeros(1, one[1], I)) == ["few"]

@@ -468,3 +468,27 @@ def test_served_in_4_bits_under_autocast():
     assert few.dtype == many.dtype == torch.bfloat16
     # the router's product may be summed in another order: logits are off by a step of bf16 at most, 2^-8 of themselves (which are below 2), weights by as much
     assert (few.float() - many[:5].float()).norm() <= 2e-2 * many[:5].float().norm()
+
+
+@pytest.mark.parametrize("tokens,E,I,J,k", [(4, 4, 1024, 3000, 4), (32, 4, 1024, 3000, 4), (12, 8, 2048, 1030, 8), (33, 8, 2048, 1030, 8)])
+def test_served_large_layer_in_4_bits(tokens, E, I, J, k):
+    """Few tokens of a large layer go through the operators for many, with float32 rows ahead of the sum."""
+    import expertscattergather_b200 as egs
+    torch.manual_seed(8)
+    served = egs.RoutedExperts(E, I, J, k).cuda().bfloat16().quantized(bits=4)
+    x = randn(tokens, I, seed=tokens, dtype=torch.bfloat16)
+    ops.check_status()
+    y = served(x)
+    one_call = tokens <= 4
+    w, ids = ops.routed_experts_few(x, served.router.W, served.up, served.down, k, up_scale=served.up_scale, down_scale=served.down_scale)[1:] if one_call else served.router(x)
+    up, down = fp4.rows(served.up, served.up_scale).transpose(1, 2), fp4.rows(served.down, served.down_scale).transpose(1, 2)
+    xq = fp4.values(*fp4.quantize(x), I)
+    want = torch.zeros(tokens, I, dtype=torch.float64, device="cuda")
+    for e in range(E):
+        t, j = (ids.long() == e).nonzero(as_tuple=True)
+        h = (xq[t] @ up[e]).float()
+        a = fp4.values(*fp4.quantize(h / (1 + torch.exp(-h))), J)[:, :J]
+        want.index_put_((t,), w[t, j].double().unsqueeze(-1) * (a @ down[e][:J]), accumulate=True)
+    # (as test_served_in_4_bits; one rounding to bf16 where rows are float32)
+    assert (y.double() - want).norm() <= (2.5e-3 if tokens <= ops.FEW_TOKENS else 4e-3) * want.norm()
+    ops.check_status()
