@@ -79,6 +79,8 @@ int layer(const FewLayer& f, const egs_route* r, int dtype, void* workspace, siz
   if (int rc = check_layer(r, f.I, f.J)) return rc;
   if (r->tokens == 0) return EGS_OK;
   if (!f.X || !f.router || !f.up || !f.down || !f.out || !f.weights || !f.experts) return EGS_ERR_INVALID_ARGUMENT;
+  const uintptr_t element = dtype == EGS_F32 ? 4 : 2, addresses = reinterpret_cast<uintptr_t>(f.X) | reinterpret_cast<uintptr_t>(f.router) | reinterpret_cast<uintptr_t>(f.out);
+  if ((addresses | (f.up_scale ? 0u : reinterpret_cast<uintptr_t>(f.up) | reinterpret_cast<uintptr_t>(f.down))) % element) return EGS_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < few_layer_workspace(*r, f.I, f.J) || !on16(workspace)) return EGS_ERR_WORKSPACE;
   return done(launch_few_layer(f, *r, dtype, workspace, stream_of(stream)), "routed_experts_few launch");
 }

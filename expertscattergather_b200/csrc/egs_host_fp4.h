@@ -218,7 +218,7 @@ std::tuple<Tensor, Tensor, Tensor> routed_experts_few(const Tensor& x, const Ten
                                          r.stride, dt, ptr(ws), bytes, c.stream),
           "egs_routed_experts_few_fp4");
   } else {
-    const Tensor u = whole(up), d = whole(down);
+    const Tensor u = up.contiguous(), d = down.contiguous();
     check(api.egs_routed_experts_few(ptr(r.t), ptr(w), static_cast<const float*>(ptr(b)), ptr(u), ptr(d), ptr(out), weights.data_ptr<float>(), experts.data_ptr<int>(), &spec, I, J,
                                      r.stride, dt, ptr(ws), bytes, c.stream),
           "egs_routed_experts_few");

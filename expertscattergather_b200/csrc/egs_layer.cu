@@ -46,6 +46,7 @@ struct LayerParams {
   int tokens, E, k, I, J;
   int x_vectors;             // rows of X and of the router begin on 16 bytes and are whole 16 bytes
   long long weight_bytes;    // of all experts' matrices, of either product
+  uint32_t up_first, down_first;   // shifted rows: `up` and `down` are the 16 bytes that the weights begin in, this many elements on
   int ring_words;            // of weights on their way, in shared memory
   int act_floats;            // down: room for activations
   int splits;                // ... clusters that a tile's contraction is cut into beside their CTAs
@@ -364,11 +365,12 @@ struct Ring {
     return x.value;
   }
 };
-// Shifted rows: `left` of four from `row` on (of all experts' rows), from column n0 on; all: bytes of the weights.
+// Shifted rows: `left` of four from `row` on (of all experts' rows), from column n0 on; all: bytes of the weights, which begin `first` elements behind W.
 template <typename T, int LANES, class R>
-__device__ __forceinline__ void ask_shifted(const R& ring, const void* W, int N, long long row, int left, int n0, long long all) {
+__device__ __forceinline__ void ask_shifted(const R& ring, const void* W, uint32_t first, int N, long long row, int left, int n0, long long all) {
   const int lane = threadIdx.x % LANES;
-  long long begin = (row * N + n0) * static_cast<long long>(sizeof(T));
+  long long begin = (row * N + n0 + first) * static_cast<long long>(sizeof(T));
+  all += first * static_cast<long long>(sizeof(T));
   auto ask = [&](uint32_t to, long long at, int r) {
     const int there = r < left ? static_cast<int>(max(min(all - at, 16ll), 0ll)) : 0;
     ring.ask(to, there ? static_cast<const char*>(W) + at : W, there);
@@ -460,7 +462,7 @@ __device__ __forceinline__ void up_unit(const LayerParams& p, UpShared<T, V, LAN
       stage();
       for (int c = first, left = (c1 - c0 + kStep - 1) / kStep; left; --left, c += kStep) {
         ring.wait();
-        if (c < c1) add_four<T, V, M>(acc, ring, a, c - c0, R::kShift ? (static_cast<uint32_t>(item.expert) * p.I + c) * p.J + u.n0 : 0u, p.J);
+        if (c < c1) add_four<T, V, M>(acc, ring, a, c - c0, R::kShift ? (static_cast<uint32_t>(item.expert) * p.I + c) * p.J + u.n0 + p.up_first : 0u, p.J);
         ring.read();
         next();
       }
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) few_up_kernel(const __grid_cons
     }
     if (left) {
       if constexpr (SHIFT) {
-        ask_shifted<T, LANES>(ring, p.up, p.J, first_row + c, end - c, n0, p.weight_bytes);
+        ask_shifted<T, LANES>(ring, p.up, p.up_first, p.J, first_row + c, end - c, n0, p.weight_bytes);
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -642,7 +644,7 @@ __device__ __forceinline__ void down_item(const LayerParams& p, const Item& item
   if constexpr (V == 16 / sizeof(T)) {
     for (int c = begin + lane / LANES * 4, left = (end - begin + kStep - 1) / kStep; left; --left, c += kStep) {
       ring.wait();
-      if (c < end) add_four<T, V, M>(acc, ring, a, c - base, R::kShift ? (static_cast<uint32_t>(item.expert) * p.J + c) * p.I + n0 : 0u, p.I);
+      if (c < end) add_four<T, V, M>(acc, ring, a, c - base, R::kShift ? (static_cast<uint32_t>(item.expert) * p.J + c) * p.I + n0 + p.down_first : 0u, p.I);
       ring.read();
       next();
     }
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) few_down_kernel(const __grid_
       }
       if (left) {
         if constexpr (SHIFT) {
-          ask_shifted<T, LANES>(ring, p.down, p.I, first_row + c, stop - c, n0, p.weight_bytes);
+          ask_shifted<T, LANES>(ring, p.down, p.down_first, p.I, first_row + c, stop - c, n0, p.weight_bytes);
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -1351,12 +1353,13 @@ cudaError_t layer_t(LayerParams p, const float* bias, const egs_route& route, cu
   cudaError_t err = launch_kernel(few_logits_kernel<T>, dim3((p.E + 7) / 8, (p.tokens + kRows - 1) / kRows), 128, 0, st, true, p);
   if (err != cudaSuccess) return err;
   if ((err = launch_route_tokens(p.logits, bias, p.weights, p.experts, route, p.E, EGS_F32, st)) != cudaSuccess) return err;
-  // One width for both products: the parts of `up` are counted by it.  16-byte vectors where rows begin on them.  Rows that do not are shifted together in 16 bits from
-  // 128 Ki elements of an expert's matrix on, and else come element by element (us a call, shifted and not: 8 tokens, 2047 x 511, 62 and 102; 4 tokens, 500 x 301,
+  // One width for both products: the parts of `up` are counted by it.  16-byte vectors where rows begin on them.  Rows of whole vectors that do not, as a slice of a larger
+  // buffer has them, are shifted together (8 tokens, 4 of 16 experts, 2048 x 512: 45 us, from 16 bytes on 32, and a copy of all experts' weights ahead of it 78).
+  // So are rows of other widths in 16 bits from 128 Ki elements of an expert's matrix on; else they come element by element (us a call, shifted and not: 8 tokens, 2047 x 511, 62 and 102; 4 tokens, 500 x 301,
   // 18.8 and 19.5, 330 x 201, 18.0 and 16.9; 4 tokens in float32, 1001 x 500, 34.3 and 34.1).
   const bool whole = p.I % V == 0 && p.J % V == 0;
   const long long elements = static_cast<long long>(p.I) * p.J;
-  if (on(p.up, 16) && on(p.down, 16) && (whole || (sizeof(T) == 2 && elements >= 128 << 10))) {
+  if (whole || (sizeof(T) == 2 && elements >= 128 << 10)) {
     p.by_tiles = Div((p.J + V * kLanes - 1) / (V * kLanes));
     p.weight_bytes = p.E * elements * static_cast<long long>(sizeof(T));
     auto both = [&](auto up, auto down, int lanes) {
@@ -1365,9 +1368,15 @@ cudaError_t layer_t(LayerParams p, const float* bias, const egs_route& route, cu
       p.ring_words = static_cast<int>(ring_bytes(kDownThreads, kDownDepth, lanes) / 4);
       return down();
     };
-    if constexpr (sizeof(T) == 2) {
-      if (!whole)
-        return both([&] { return up_launch<few_up_kernel<T, V, kLanes, true>>(p, st); }, [&] { return down_launch<few_down_kernel<T, V, kLanes, true>, T>(p, V * kLanes, st); }, kLanes);
+    if (!whole || !on(p.up, 16) || !on(p.down, 16)) {
+      auto piece = [](const void*& w) {            // the 16 bytes that w lies in
+        const uintptr_t behind = reinterpret_cast<uintptr_t>(w) & 15u;
+        w = static_cast<const char*>(w) - behind;
+        return static_cast<uint32_t>(behind / sizeof(T));
+      };
+      p.up_first = piece(p.up);
+      p.down_first = piece(p.down);
+      return both([&] { return up_launch<few_up_kernel<T, V, kLanes, true>>(p, st); }, [&] { return down_launch<few_down_kernel<T, V, kLanes, true>, T>(p, V * kLanes, st); }, kLanes);
     }
     return both([&] { return up_launch<few_up_kernel<T, V, kLanes, false>>(p, st); }, [&] { return down_launch<few_down_kernel<T, V, kLanes, false>, T>(p, V * kLanes, st); }, 0);
   }

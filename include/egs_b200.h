@@ -430,7 +430,7 @@ size_t egs_expert_matmul_fp4_rows_workspace_bytes(const egs_ragged* dims, int pa
  *
  * out[t] = sum over j of weights[t, j] * silu(X[t] up[e]) down[e], e = experts[t, j]: weights and experts [tokens, top_k] are those of egs_route_tokens for the
  * logits X[t] . router[e] [E, I], which stay float32, as do all sums; out [tokens, I] is rounded once.  X's rows lie x_stride elements apart.
- * up [E, I, J], down [E, J, I]; or in 4 bits (egs_quantize_rows_fp4), where X's rows and silu(..) are rounded to 4 bits ahead of their products too: with the
+ * up [E, I, J], down [E, J, I], from any element's address on (16 bytes are read soonest; up to 14 ahead of weights that begin inside 16, of those 16, are read too); or in 4 bits (egs_quantize_rows_fp4), where X's rows and silu(..) are rounded to 4 bits ahead of their products too: with the
  * layout EGS_W_NC up [E, J, I / 2] and down [E, I, J / 2], rows as everywhere; with EGS_W_CN the same bytes with the columns together, up [E, I / 2, J] and
  * down [E, J / 2, I], from any address and stride on; experts up_far and down_far bytes apart, scales always [E, J, I / 32] and [E, I, J / 32].  At most EGS_MAX_FEW_TOKENS tokens and EGS_MAX_FEW_SLOTS = tokens * top_k.
  * workspace (16-byte aligned): egs_routed_experts_few_workspace_bytes() bytes.  The same bits in every run.

@@ -144,3 +144,9 @@ def test_which_calls_the_served_layer_makes(monkeypatch, E, I, J, k, one, many):
     assert [run(torch.zeros(n, I)) for n in one] == [["few"]] * len(one)
     assert [run(torch.zeros(n, I)) for n in many] == [["separate"]] * len(many)
     assert run(torch.zeros(many[0], 1, I)) == ["separate"] and run(torch.zeros(1, one[1], I)) == ["few"]
+
+
+def test_entries_refuse_addresses_inside_an_element():
+    for name in ("X", "router", "up", "down", "out"):
+        assert plain(**{name: ctypes.c_void_p(18)}) == BAD and plain(**{name: ctypes.c_void_p(17)}, dtype=1) == BAD
+        assert plain(**{name: ctypes.c_void_p(20)}, size=0) == WORKSPACE and plain(**{name: ctypes.c_void_p(18)}, dtype=1, size=0) == WORKSPACE

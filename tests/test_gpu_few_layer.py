@@ -327,6 +327,26 @@ def test_clusters_of_a_layer_with_many_experts(E, dtype, tokens, k, I, J):
         out = ops.routed_experts_few(x, router, up, down, k)[0]
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,E,k,I,J", [(1, 5, 3, 2048, 512), (9, 6, 2, 264, 520), (4, 3, 2, 48, 40), (20, 2, 1, 8, 4096), (3, 33, 4, 512, 8)])
+@pytest.mark.parametrize("up_begin,down_begin", [(1, 0), (0, 3), (2, 1), (5, 7)])
+def test_weights_that_begin_anywhere(dtype, tokens, E, k, I, J, up_begin, down_begin):
+    """Slices of a larger buffer, NaN right before and behind them: the bits that weights on 16 bytes give, and no copy of them."""
+    t = TYPES[dtype]
+    x, router = randn(tokens, I, seed=1, dtype=t), (randn(E, I, seed=2) * 1.5 / I ** 0.5).to(t)
+    whole = [(randn(E, I, J, seed=3) * 2 / I ** 0.5).to(t), (randn(E, J, I, seed=4) / J ** 0.5).to(t)]
+    up, down = (torch.full((n + w.numel() + 9,), float("nan"), device="cuda", dtype=t)[n:n + w.numel()].view(w.shape).copy_(w) for n, w in zip((up_begin, down_begin), whole))
+    want = ops.routed_experts_few(x, router, *whole, k)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = ops.routed_experts_few(x, router, up, down, k)
+    grown = torch.cuda.max_memory_allocated() - before
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if I * J > 100000:                                       # (the workspace is eight parts of the first product, the sums of the second, logits and outputs)
+        assert grown < up.numel() * t.itemsize
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)
