@@ -62,7 +62,7 @@ struct Fp4Tiles {
   int BN, stages, steps, blocks;
   int tiles_n;
   int gathers;                 // X's rows are gathered
-  int vectors, words;          // rows of the output begin on 16 bytes and are whole 16 bytes; on 8: words 2, on 4: words 1
+  int vectors, words;          // rows of the output begin on 16 bytes and are whole 16 bytes; of 16-bit elements, on four bytes and whole words
   uint32_t table_bytes;        // of each of the two tables
   Div by_n;
 };

@@ -200,37 +200,29 @@ __device__ __forceinline__ void dots(const LayerParams& p, int e0, int e1, int t
       acc[1][m] += __shfl_xor_sync(kAll, acc[1][m], o);
     }
 }
-// ... by a warp for tokens from t0 to t1, in fours: emit(token, expert, logit)
-template <typename T, class Emit>
-__device__ __forceinline__ void logits_of(const LayerParams& p, int e0, int e1, int t0, int t1, Emit&& emit) {
-  constexpr int V = 16 / sizeof(T);
-  for (; t0 < t1; t0 += kRows) {
-    if (t1 - t0 == 1) {
-      float acc[2][1];
-      if (p.x_vectors) dots<T, V, 1, 8>(p, e0, e1, t0, acc);
-      else dots<T, 1, 1, 16>(p, e0, e1, t0, acc);
-      emit(t0, e0, acc[0][0]);
-      if (e1 < p.E) emit(t0, e1, acc[1][0]);
-    } else {
-      float acc[2][kRows];
-      if (p.x_vectors) dots<T, V, kRows, 2>(p, e0, e1, t0, acc);
-      else dots<T, 1, kRows, 8>(p, e0, e1, t0, acc);
-#pragma unroll
-      for (int m = 0; m < kRows; ++m)
-        if (t0 + m < t1) {
-          emit(t0 + m, e0, acc[0][m]);
-          if (e1 < p.E) emit(t0 + m, e1, acc[1][m]);
-        }
-    }
-  }
-}
-
+// ... of the up to four tokens from t0 on, by a warp
 template <typename T>
 __device__ __forceinline__ void logits_by_warps(const LayerParams& p, int e, int t0) {
+  constexpr int V = 16 / sizeof(T);
   if (e >= p.E) return;
-  logits_of<T>(p, e, e + 1, t0, min(p.tokens, t0 + kRows), [&](int t, int expert, float v) {
-    if ((threadIdx.x & 31) == 0) p.logits[t * p.E + expert] = v;
-  });
+  auto put = [&](int t, const auto& acc, int m) {
+    if (threadIdx.x & 31) return;
+    p.logits[t * p.E + e] = acc[0][m];
+    if (e + 1 < p.E) p.logits[t * p.E + e + 1] = acc[1][m];
+  };
+  if (p.tokens - t0 == 1) {
+    float acc[2][1];
+    if (p.x_vectors) dots<T, V, 1, 8>(p, e, e + 1, t0, acc);
+    else dots<T, 1, 1, 16>(p, e, e + 1, t0, acc);
+    put(t0, acc, 0);
+  } else {
+    float acc[2][kRows];
+    if (p.x_vectors) dots<T, V, kRows, 2>(p, e, e + 1, t0, acc);
+    else dots<T, 1, kRows, 8>(p, e, e + 1, t0, acc);
+#pragma unroll
+    for (int m = 0; m < kRows; ++m)
+      if (t0 + m < p.tokens) put(t0 + m, acc, m);
+  }
 }
 // The logits in float32; 2.0 to 2.6 us, the latency of a router's row.
 template <typename T>
@@ -253,9 +245,6 @@ template <int V> struct Sums {
   __device__ __forceinline__ float get(int v) const {
     if constexpr (kPairs) return __uint_as_float(static_cast<uint32_t>(v & 1 ? raw[v / 2] >> 32 : raw[v / 2]));
     else return raw[v];
-  }
-  __device__ __forceinline__ void set(int v, float a, float b) {          // of v and v + 1
-    raw[v / 2] = pair(a, b);
   }
   static __device__ __forceinline__ unsigned long long pair(float a, float b) {
     unsigned long long r;
@@ -308,7 +297,7 @@ __device__ __forceinline__ void accumulate(Sums<V> (&acc)[M], const T* W, int w_
     if (c < end) load();
   }
 }
-// Weights on their way to shared memory, kDepth pieces of 64 bytes a thread, each thread's its own: what it asked for it reads, so that nobody waits for
+// Weights on their way to shared memory, DEPTH pieces of 64 bytes a thread, each thread's its own: what it asked for it reads, so that nobody waits for
 // others, and the next unit's weights come while this one's sums are joined.  (Into registers, with a wait for all that had been asked for before
 // more was, 43 MB came at 3.4 TB/s.)
 // SHIFT: rows that begin anywhere.  What comes are the 16-byte pieces of memory that a row's tile lies in, one more than it has, and a thread shifts its elements
