@@ -347,6 +347,56 @@ def test_weights_that_begin_anywhere(dtype, tokens, E, k, I, J, up_begin, down_b
         assert grown < up.numel() * t.itemsize
 
 
+@pytest.mark.parametrize("fp4_weights", [False, True])
+def test_padded_tokens_that_are_no_numbers(fp4_weights):
+    """Rows of a padded batch that hold anything: valid choices, each expert once, and not a bit of the other rows' results."""
+    tokens, E, k, I, J = 12, 9, 4, 136, 72
+    x, router = randn(tokens, I, seed=1, dtype=torch.bfloat16), randn(E, I, seed=2, dtype=torch.bfloat16)
+    if fp4_weights:
+        (u, us), (d, ds) = grid4(E, J, I, seed=3, low=120, high=124), grid4(E, I, J, seed=4)
+        run = lambda x: ops.routed_experts_few(x, router, u, d, k, up_scale=us, down_scale=ds)
+    else:
+        up, down = randn(E, I, J, seed=3, dtype=torch.bfloat16), randn(E, J, I, seed=4, dtype=torch.bfloat16)
+        run = lambda x: ops.routed_experts_few(x, router, up, down, k)
+    want = run(x)
+    y = x.clone()
+    y[1], y[4], y[5], y[11] = float("nan"), float("inf"), -float("inf"), 3e38
+    y[7, 3], y[8, 100] = float("nan"), -float("inf")
+    rest = torch.tensor([0, 2, 3, 6, 9, 10], device="cuda")
+    first = run(y)
+    for _ in range(3):
+        out, w, ids = run(y)
+        assert ((ids >= 0) & (ids < E)).all() and all(len(set(r)) == k for r in ids.tolist())
+        # (experts' tokens are read in fours: which ones share a read is no matter of their sums)
+        assert torch.equal(out[rest], want[0][rest]) and torch.equal(w[rest], want[1][rest]) and torch.equal(ids[rest], want[2][rest])
+        assert torch.equal(ids, first[2]) and torch.equal(out.isnan(), first[0].isnan()) and out[1].isnan().all()
+
+
+def test_weights_beyond_32_bits():
+    """Experts that lie more than 2^31 elements, and 2^32 bytes, behind the first one."""
+    E, I, J = 33, 8192, 8192
+    x = randn(3, I, seed=1, dtype=torch.bfloat16).abs()
+    router = torch.zeros(E, I, device="cuda", dtype=torch.bfloat16)
+    router[E - 1] = 1                                        # all tokens choose the last one
+    up, down = (torch.empty(E, a, b, device="cuda", dtype=torch.bfloat16) for a, b in ((I, J), (J, I)))
+    up[E - 1], down[E - 1] = randn(I, J, seed=2) * 2 / I ** 0.5, randn(J, I, seed=3) / J ** 0.5
+    out, w, ids = ops.routed_experts_few(x, router, up, down, 1)
+    assert (ids == E - 1).all()
+    want, off = layer64(x.double(), w.double(), torch.zeros_like(ids).long(), up[E - 1:].double(), down[E - 1:].double())
+    assert ((out.double() - want).abs() - off - want.abs() * 2.0 ** -8).max().item() <= 0
+    del up, down
+    E = 129                                                  # in 4 bits an expert's matrix is 2^25 bytes
+    router = torch.zeros(E, I, device="cuda", dtype=torch.bfloat16)
+    router[E - 1] = 1
+    up, down = (torch.empty(E, I, I // 2, device="cuda", dtype=torch.uint8) for _ in range(2))
+    us, ds = (torch.empty(E, I, I // 32, device="cuda", dtype=torch.uint8) for _ in range(2))
+    (up[E - 1], us[E - 1]), (down[E - 1], ds[E - 1]) = grid4(J, I, seed=3, low=120, high=124), grid4(I, J, seed=4)
+    out, w, ids = ops.routed_experts_few(x, router, up, down, 1, up_scale=us, down_scale=ds)
+    assert (ids == E - 1).all() and not out.isnan().any()
+    again = ops.routed_experts_few(x, router[E - 1:], up[E - 1:], down[E - 1:], 1, up_scale=us[E - 1:], down_scale=ds[E - 1:])[0]
+    assert torch.equal(out, again)
+
+
 def test_refusals():
     E, I, J = 4, 16, 8
     x, router, up, down = randn(3, I), randn(E, I), randn(E, I, J), randn(E, J, I)

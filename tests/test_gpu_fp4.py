@@ -237,6 +237,24 @@ def test_projection_of_experts_is_rounded_once(dtype, tokens, E, k, C, N):
     assert ((out.double() - want).abs() - off).max().item() <= 0
 
 
+@pytest.mark.parametrize("tokens", [1, 3, 300])
+def test_weights_beyond_32_bits(tokens):
+    """Experts whose weights lie more than 2^32 bytes behind the first one's; their last channels."""
+    E, N, C = 18, 16384, 32768
+    wq, ws = (torch.empty(E, N, n, device="cuda", dtype=torch.uint8) for n in (C // 2, C // 32))
+    last = 96
+    wq[E - 1], ws[E - 1] = 0, 127
+    wq[E - 1, -last:], ws[E - 1, -last:] = ops.quantize_rows_fp4(randn(last, C, seed=1))
+    q, s = ops.quantize_rows_fp4(randn(tokens, C, seed=2))
+    plan = ops.plan_experts(torch.full((tokens, 1), E - 1, dtype=torch.int32, device="cuda"), E)
+    x, w = fp4.rows(q, s), fp4.rows(wq[E - 1, -last:], ws[E - 1, -last:])
+    Y, size = x @ w.t(), x.abs() @ w.abs().t()
+    got = ops.expert_matmul_fp4(q, s, wq, ws, plan, out_dtype=torch.float32)
+    assert not got[:, :-last].any()
+    assert ((got[:, -last:].double() - Y).abs() - product_bound(size, Y, C, torch.float32)).max().item() <= 0
+    ops.check_status()
+
+
 # ---- far scales ---------------------------------------------------------------------------------------
 
 FAR = [(123, -20), (-20, 123), (124, -130), (-130, 124), (110, 8), (8, 110), (-100, 20), (20, -100), (100, -100), (-149, 110)]
