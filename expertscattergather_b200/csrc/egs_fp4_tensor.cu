@@ -16,9 +16,10 @@
 // one hands it over to the leader with a release at cluster scope, which the leader's wait acquires: releases by the storing warps themselves wait
 // for the scales that they have asked for behind a memory barrier (94 us for 74 at 8192 x 4096 -> 4096).  Scales word by word with cp.async: 106; 16 bytes of a row (two steps) at a time for 64: 80 for 70.
 //
-// 8192 x 4096 -> 4096: 63.5 us, 4.3 PFLOP/s (2.6 times the 16-bit rate; loads alone 47, all but the scales 61).  Bound by what the L2 gives all SMs, 9.6 TB/s of tiles and scales.
-// 65536 rows of 64 experts, 2048 -> 512: 59, of which 53 without the read-out; 512 -> 2048, two steps a tile: 86, without stores 70, without the read-out 55: 268 MB of
-// output (41) share the memory with the loads.  Rows of a block kept in shared memory for all column tiles: 72 for 55; a read-out of both halves at once: no gain.
+// 8192 x 4096 -> 4096: 66 us, 4.1 PFLOP/s (2.5 times the 16-bit rate; loads alone 47).  No unit is full (tensor pipe 55 %, L2 35 %): waits between the steps,
+// 16 pairs of 74 at work in the ninth round of tiles, 4256 columns for 4096.
+// 65536 rows of 64 experts, 2048 -> 512: 57, into float32 63, into 4 bits 55 and activated 68; 512 -> 2048, two steps a tile: 82, of which some 30 are the read-out, into float32 129: 268 and 537 MB of
+// output (41, 82) share the memory with the loads.  Rows of a block kept in shared memory for all column tiles: 72 for 55; a read-out of both halves at once: no gain.
 #include <cstddef>
 
 #include "egs_fp4.cuh"

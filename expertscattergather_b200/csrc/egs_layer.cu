@@ -768,8 +768,8 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ L
 // ---- weights in 4 bits -------------------------------------------------------------------------------------------------
 // Rows and weights become 16-bit floats, which hold them exactly, and go through the tensor cores (mma.sync: 16 columns, 16 contraction elements, up to eight
 // rows); a block's sums are exact, then times both scales into float32 sums.  (As integers through dp4a four columns and a block took 980
-// instructions a warp: 83 us a call, 8 tokens, 8 of 64 experts, 2048 x 512, 47 MB.  Now 35: 4.7 million warp instructions a product, a third of which ask for weights in pieces
-// of 32 bytes a row; with cold caches a product took 20 us, 16 without its arithmetic and 12 without its loads, and takes 17 now.)  The weights' bytes lie along the contraction (NC) or along the columns (CN).
+// instructions a warp: 83 us a call, 8 tokens, 8 of 64 experts, 2048 x 512, 47 MB.  Now 35 to 38: 4.3 (NC) to 5.1 million warp instructions a product, a third of which ask for
+// weights; with cold caches a product took 20 us, 16 without its arithmetic and 12 without its loads, and takes 14 (NC) to 17 now.)  The weights' bytes lie along the contraction (NC) or along the columns (CN).
 // A warp's stage: 4 blocks of the contraction x a tile of 32 columns, 2 KB of weights; kDepth4 stages are on their way, each warp's its own.  Lane (g, q) = (lane / 4,
 // lane % 4) multiplies columns 4 g .. 4 g + 3 and of each block the eight elements from 8 q on; their order is the same in both operands.
 constexpr int kTile4 = 32, kStage4 = 4, kDepth4 = 3, kThreads4 = 256, kWarps4 = kThreads4 / 32;
