@@ -88,10 +88,10 @@ __device__ __forceinline__ Block4 load_block(const uint8_t* row, int c, int C) {
 __device__ __forceinline__ float silu_exact(float x) { return x / __fadd_rn(1.f, expf(-x)); }
 // The same within 2^-20, relative, for every x: no branches, so that 32 of them go side by side (65536 rows, 2048 -> 512: 68 us, with silu_exact
 // 177, with the fast exponential, which is off by 2^-17 at -70, 60, without an activation 55).  exp(-|x|) is at most 1, so no sum is beyond 2.  In units of 2^-24 the exponential is off by 4, the two
-// products and the sum by 1 each, the reciprocal by 2; silu_exact by 6.  Below the logarithm of the largest float that one's exponential is infinite and its result 0.
+// products and the sum by 1 each, the reciprocal by 2; silu_exact by 6.  From -88.72284 on, the first float beyond the logarithm of the largest, that one's exponential is infinite and its result 0.
 __device__ __forceinline__ float silu_near(float x) {
   float t = expf(-fabsf(x)), r;
-  if (x < -88.72284f) t = 0.f;
+  if (x <= -88.72284f) t = 0.f;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
   return (x < 0.f ? x * t : x) * r;
 }

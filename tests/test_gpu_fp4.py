@@ -303,3 +303,27 @@ def test_activations_ahead_of_4_bits_are_the_exact_ones(path, tokens, E, k, C, N
     size, got = v.abs() / power, fp4.values(fp4.codes_of(y), ys, N) / power
     low_level, high_level = (level[torch.bucketize(size * f, edges)] for f in (1 - 2.0 ** -20, 1 + 2.0 ** -20))
     assert ((got.abs() >= low_level) & (got.abs() <= high_level) & ((got == 0) | (torch.sign(got) == torch.sign(v)))).all()
+
+
+def test_activations_where_the_exponential_ends():
+    """Sums on both sides of the first float whose exponential is infinite: 0 or a number as in the elementary form."""
+    N, edge = 256, int(88.72283935546875 * 2 ** 17)
+    sums = edge + torch.randint(-8, 9, (N,), generator=torch.Generator().manual_seed(1))
+    codes, C = torch.zeros(N, 192, dtype=torch.int32), 192
+    for n, total in enumerate(sums.tolist()):
+        for digit in range(6):                               # four bits of a sum to each block
+            left, at = total >> 4 * digit & 15, 32 * digit
+            for code in (7, 6, 5, 4, 2):                     # 6, 4, 3, 2, 1
+                while left >= fp4.LEVELS[code]:
+                    codes[n, at], left, at = code + 8, left - int(fp4.LEVELS[code]), at + 1
+    wq, ws = fp4.pack(codes)[None].cuda(), torch.zeros(1, N, 16, dtype=torch.uint8, device="cuda")
+    ws[..., :6] = torch.tensor([127 - 17 + 4 * digit for digit in range(6)], dtype=torch.uint8)
+    ws = ws[..., :6]
+    q, s = ops.quantize_rows_fp4(torch.ones(130, C, device="cuda"))
+    plan = ops.plan_experts(torch.zeros(130, 1, dtype=torch.int32, device="cuda"), 1)
+    for path in ("tensor", "generic"):
+        full = ops.expert_matmul_fp4(q, s, wq, ws, plan, out_dtype=torch.float32, path=path)
+        assert (full.double() * 2 ** 17 + sums.cuda()).abs().max() <= 2
+        elementary = full / (1 + torch.exp(-full))
+        got = fp4.rows(*ops.expert_matmul_fp4_rows(q, s, wq, ws, plan, activation="silu", path=path))
+        assert torch.equal(got == 0, elementary == 0) and (elementary == 0).any() and (elementary != 0).any()
